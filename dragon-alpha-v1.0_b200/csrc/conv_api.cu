@@ -76,6 +76,7 @@ enum Opt {
     OPT_HALO_PAD,       // channels that are no multiple of 32 on the halo kernels: 0 never, 1 by cost, 2 wherever possible
     OPT_F32_PLANES,     // fp32 products as three bf16 planes on the tensor cores: 0 never, 1 by cost, 2 always
     OPT_GATHER,         // 3xTF32 layers straight from their tensors as three bf16 planes: 0 never, 1 by cost, 2 wherever possible
+    OPT_FC_TILE,        // tiles of 16-bit FullConnect products: 0 by cost, 1 CTA pairs, 2 128 x 128, 3 128 x 64
     OPT_COUNT
 };
 struct OptDef { const char* name; int dflt; };
@@ -86,7 +87,7 @@ static const OptDef kOptDefs[OPT_COUNT] = {
     {"DW_STACKED", -1}, {"DW_DIAG", 1}, {"DW_CW", 0}, {"DW_R", 0}, {"DW_STATIC", 1}, {"CONV_PROF", 0}, {"SM_BUDGET", 0},
     {"SKINNY", 1}, {"HALO_DEEP", 1}, {"HALO_SPLITB", 0}, {"NVTX", 1}, {"DW_LANES", 0}, {"HALO_TAPSTACK", 1}, {"HALO_FLAT32", 1},
     {"DW_STRIDED", 1}, {"DW_TAPGROUPS", 1}, {"HALO_LATTICE", 1}, {"HALO_WINDOW", 1}, {"HALO_PAD", 1},
-    {"F32_PLANES", 1}, {"GATHER", 1},
+    {"F32_PLANES", 1}, {"GATHER", 1}, {"FC_TILE", 0},
 };
 static std::atomic<int> g_opt[OPT_COUNT];
 static std::once_flag g_opt_once;
@@ -121,7 +122,7 @@ static bool kernels_are_asked_for()
 {
     std::call_once(g_opt_once, init_opts);
     for (int i = 0; i < OPT_COUNT; ++i) {
-        if (i == OPT_CONV_PROF || i == OPT_SM_BUDGET || i == OPT_NVTX || i == OPT_DW_LANES || i == OPT_F32_PLANES || i == OPT_GATHER) continue;
+        if (i == OPT_CONV_PROF || i == OPT_SM_BUDGET || i == OPT_NVTX || i == OPT_DW_LANES || i == OPT_F32_PLANES || i == OPT_GATHER || i == OPT_FC_TILE) continue;
         if (g_opt[i].load(std::memory_order_relaxed) != kOptDefs[i].dflt) return true;
     }
     return false;
@@ -160,11 +161,8 @@ struct CallOptions {
 
 // One NVTX range per operator call (option NVTX, on by default): a timeline tool attached to the process shows
 // which contraction the kernels of a call belong to; without a tool a push / pop is a few nanoseconds.
-struct OpRange {
-    bool on;
-    explicit OpRange(const char* name) : on(opt(OPT_NVTX) != 0 && !t_dry) { if (on) nvtxRangePushA(name); }
-    ~OpRange() { if (on) nvtxRangePop(); }
-};
+OpRange::OpRange(const char* name) : on(opt(OPT_NVTX) != 0 && !t_dry) { if (on) nvtxRangePushA(name); }
+OpRange::~OpRange() { if (on) nvtxRangePop(); }
 
 // ---- per-device context ----------------------------------------------------------------------
 
@@ -298,6 +296,8 @@ int planes_launch_slice(int* ctas)
 // Option F32_PLANES; ALPHA_ALGO_SIMT asks for plain fp32 kernels.
 int option_f32_planes() { return cur_algo() == ALPHA_ALGO_SIMT ? 0 : opt(OPT_F32_PLANES); }
 
+int option_fc_tile() { return opt(OPT_FC_TILE); }
+
 // ---- scratch memory ----------------------------------------------------------------------------
 //
 // t_caller: scratch the caller of a native handed over for this one call (the CW / deltaW_buf
@@ -422,6 +422,34 @@ static void ws_rewind(DeviceCtx* c, cudaStream_t stream, const WsMark& m)
     std::lock_guard<std::mutex> lock(g_mu);
     auto it = c->workspace.find(stream);
     if (it != c->workspace.end()) it->second.used = m.block_used;
+}
+
+int call_begin(cudaStream_t stream)
+{
+    DeviceCtx* c;
+    const int rc = get_ctx(&c);
+    if (!rc) ws_begin(c, stream);
+    return rc;
+}
+int call_scratch(cudaStream_t stream, size_t bytes, void** out)
+{
+    DeviceCtx* c;
+    int rc = get_ctx(&c);
+    float* p = nullptr;
+    if (!rc) rc = get_workspace(c, stream, bytes, &p);
+    *out = p;
+    return rc;
+}
+bool dry_run() { return t_dry; }
+void dry_begin() { t_dry = true; t_dry_cur = t_dry_peak = 0; }
+size_t dry_end() { t_dry = false; return t_dry_peak; }
+int encode_tiled(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides_bytes, const cuuint32_t* box,
+                 CUtensorMapSwizzle swizzle)
+{
+    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = g_encodeTiled(m, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides_bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? ALPHA_OK : fail(ALPHA_E_CUDA, "cuTensorMapEncodeTiled failed (%d), rank %d box0 %u", (int)r, rank, box[0]);
 }
 
 static int check_launch(const char* what);

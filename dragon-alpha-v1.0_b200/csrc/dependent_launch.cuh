@@ -35,8 +35,9 @@ bool dependent_launches();
 // batch 512 4.39 -> 4.07 ms.  Only for kernels whose every thread does; an ordinary launch while the stream is being captured, where
 // the captured dependencies say it all, and under an SM budget (ten 56 x 56 x 64 layers on 100 SMs beside 100 small GEMMs of another
 // stream: the GEMMs end after 1.2 ms, after 2.1 ms with the successors resident on the other 48 SMs).
+// launch_after_clusters: the same with clusters of `cluster` CTAs (0: those of the kernel's own attribute, if any).
 template <class... Params, class... Args>
-inline void launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args)
+inline void launch_after_clusters(void (*kernel)(Params...), dim3 grid, dim3 block, unsigned cluster, size_t smem, cudaStream_t stream, Args&&... args)
 {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     bool plain = true;
@@ -47,13 +48,26 @@ inline void launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_
     } else {
         plain = cap != cudaStreamCaptureStatusNone;
     }
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2]{};
+    unsigned n = 0;
+    if (!plain) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster; attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = stream;
-    cfg.attrs = &attr; cfg.numAttrs = plain ? 0 : 1;
+    cfg.attrs = attr; cfg.numAttrs = n;
     cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);   // the caller looks at cudaGetLastError()
+}
+template <class... Params, class... Args>
+inline void launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args)
+{
+    launch_after_clusters(kernel, grid, block, 0, smem, stream, std::forward<Args>(args)...);
 }
 
 // The same for a kernel with more than 48 KB of dynamic shared memory.

@@ -1,0 +1,364 @@
+// FullConnect layers of a transformer: products with bias, activation and residual in their epilogue, the gated block, and their gradients.
+#include "../../include/alpha_conv_b200.h"
+#include "fc_delta.cuh"
+#include "fc_f32.cuh"
+#include "fc_mma.cuh"
+#include "fc_small.cuh"
+#include "host_common.h"
+
+#include <initializer_list>
+
+using namespace alpha;
+
+namespace {
+
+size_t type_bytes(int dtype) { return dtype == ALPHA_F32 ? 4 : 2; }
+
+struct Span { const void* ptr; size_t bytes; };
+bool overlap(const Span& a, const Span& b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.ptr), y = reinterpret_cast<uintptr_t>(b.ptr);
+    return a.ptr && b.ptr && x < y + b.bytes && y < x + a.bytes;
+}
+// What a call writes must overlap neither what it reads nor what else it writes.
+int check_spans(const char* what, std::initializer_list<Span> in, std::initializer_list<Span> out)
+{
+    for (const Span* o = out.begin(); o != out.end(); ++o) {
+        for (const Span& i : in)
+            if (overlap(*o, i)) return fail(ALPHA_E_ARG, "%s: an output overlaps an input", what);
+        for (const Span* q = out.begin(); q != o; ++q)
+            if (overlap(*o, *q)) return fail(ALPHA_E_ARG, "%s: two outputs overlap", what);
+    }
+    for (auto list : {in, out})
+        for (const Span& s : list)
+            if (reinterpret_cast<uintptr_t>(s.ptr) & 15) return fail(ALPHA_E_ARG, "%s: tensor pointers must be 16-byte aligned", what);
+    return ALPHA_OK;
+}
+
+int check_fc(const char* what, const AlphaFcShape* s, bool glu)
+{
+    if (!s) return fail(ALPHA_E_ARG, "%s: null shape", what);
+    if (s->rows <= 0 || s->IC <= 0 || s->OC <= 0) return fail(ALPHA_E_ARG, "%s: non-positive dimension (rows=%d IC=%d OC=%d)", what, s->rows, s->IC, s->OC);
+    if (s->dtype != ALPHA_F32 && s->dtype != ALPHA_BF16 && s->dtype != ALPHA_F16) return fail(ALPHA_E_ARG, "%s: unknown element type %d", what, s->dtype);
+    if (s->act < ALPHA_ACT_NONE || s->act > ALPHA_ACT_GELU_TANH) return fail(ALPHA_E_ARG, "%s: unknown activation %d", what, s->act);
+    if (s->act == ALPHA_ACT_LEAKY_RELU && !(s->k == s->k)) return fail(ALPHA_E_ARG, "%s: slope is NaN", what);
+    const int unit = s->dtype == ALPHA_F32 ? 4 : 8;
+    if (s->IC % unit || s->OC % unit)
+        return fail(ALPHA_E_ARG, "%s: IC=%d and OC=%d must be multiples of %d (rows of 16-byte words)", what, s->IC, s->OC, unit);
+    const long long wide = glu ? 2LL * s->OC : s->OC, most = 2147483647LL;
+    if (wide > most) return fail(ALPHA_E_ARG, "%s: more than 2^31-1 rows of W", what);
+    // the fp32 kernels address a tensor's elements with 32 bits
+    if (s->dtype == ALPHA_F32 && ((long long)s->rows * s->IC > most || wide * s->IC > most || s->rows * wide > most))
+        return fail(ALPHA_E_ARG, "%s: tensor has more than 2^31-1 elements", what);
+    return ALPHA_OK;
+}
+
+int launched(const char* what)
+{
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? ALPHA_OK : fail(ALPHA_E_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+}
+
+// ---- 16-bit products --------------------------------------------------------------------------------------------
+
+// Map of a row-major matrix of 16-bit elements, box of `in` columns x `rows` rows.
+int make_map(CUtensorMap* m, int dtype, const void* base, long long cols, long long rows, int in, int box_rows, CUtensorMapSwizzle swz)
+{
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, st[1] = {(cuuint64_t)cols * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)in, (cuuint32_t)box_rows};
+    return encode_tiled(m, dtype == ALPHA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, st, box, swz);
+}
+// Map of an output of `halves` blocks of `cols` columns a row, by which boxes of 32 x 32 elements are stored.
+int make_out_map(CUtensorMap* m, int dtype, const void* base, long long cols, int halves, long long rows)
+{
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)halves, (cuuint64_t)rows}, st[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * 2 * halves};
+    const cuuint32_t box[3] = {32, 1, 32};
+    return encode_tiled(m, dtype == ALPHA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, st, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+struct Product {
+    int dtype, rows, cols, K;        // outputs (glu: columns of a half), reduction
+    bool a_mn, b_mn, glu;
+    const void *A, *B, *bias, *residual;
+    void *Z, *Y;
+    int act; float k;
+};
+
+enum { kTilePair = 1, kTile128 = 2, kTile64 = 3 };
+
+template <class T, bool PAIR, int BN, bool GLU>
+void launch_mma(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& y, const CUtensorMap& z, const FcMma& p, int sms, cudaStream_t stream)
+{
+    using G = FcTile<PAIR, BN>;
+    constexpr int CTAS = PAIR ? 2 : 1;
+    const int total = p.m_tiles * p.n_tiles, most = sms / CTAS;
+    allow_smem<fc_mma_kernel<T, PAIR, BN, GLU>>();
+    launch_after_clusters(fc_mma_kernel<T, PAIR, BN, GLU>, dim3((total < most ? total : most) * CTAS), kFcThreads, PAIR ? 2 : 0, G::kSmem, stream, a, b, y, z, p);
+}
+
+// Tile of a product: that whose waves take least, a wave of 128 x 64 tiles counted as 0.36 and one of 128 x 128 as 0.58 of one of pairs'.
+int pick_tile(const Product& q, int sms)
+{
+    const int forced = option_fc_tile();
+    if (forced) return forced == kTilePair && sms < 2 ? kTile128 : forced;
+    const int cols = q.glu ? 2 * q.cols : q.cols;
+    auto waves = [&](int bm, int bn, int ctas) {
+        const long long tiles = (long long)((q.rows + bm - 1) / bm) * ((cols + bn - 1) / bn), most = sms / ctas;
+        return (double)((tiles + most - 1) / most);
+    };
+    const double pair = sms >= 2 ? waves(256, 256, 2) : 1e30, single = 0.58 * waves(128, 128, 1), narrow = 0.36 * waves(128, 64, 1);
+    return pair <= single && pair <= narrow ? kTilePair : single <= narrow ? kTile128 : kTile64;
+}
+
+int launch_product(const Product& q, cudaStream_t stream)
+{
+    int sms = 0, *status = nullptr;
+    int rc = device_sms(&sms);
+    if (!rc) rc = device_status_word(&status);
+    if (rc) return rc;
+    const int tile = pick_tile(q, sms), bm = tile == kTilePair ? 256 : 128, bn = tile == kTilePair ? 256 : tile == kTile128 ? 128 : 64;
+    const int out = q.glu ? bn / 2 : bn, br = tile == kTilePair ? 128 : bn;
+    FcMma p{};
+    p.rows = q.rows; p.cols = q.cols; p.K = q.K;
+    p.m_tiles = (q.rows + bm - 1) / bm; p.n_tiles = (q.cols + out - 1) / out; p.kb = (q.K + kFcBK - 1) / kFcBK;
+    if ((long long)p.m_tiles * p.n_tiles > 2147483647LL / kFcGroupM) return fail(ALPHA_E_ARG, "fullConnect: more tiles than a launch takes");
+    p.a_mn = q.a_mn; p.b_mn = q.b_mn;
+    p.a_rows = q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
+    p.b_up = q.cols;
+    p.idesc = q.dtype == ALPHA_BF16 ? make_idesc_bf16(bm, bn, q.a_mn, q.b_mn) : make_idesc_f16(bm, bn, q.a_mn, q.b_mn);
+    p.act = q.act; p.k = q.k; p.keep_z = q.Z != nullptr;
+    p.bias = q.bias; p.residual = q.residual; p.status = status;
+    CUtensorMap a, b, y, z;
+    const long long b_rows = q.glu ? 2LL * q.cols : q.cols;
+    rc = q.a_mn ? make_map(&a, q.dtype, q.A, q.rows, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) : make_map(&a, q.dtype, q.A, q.K, q.rows, 64, p.a_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = q.b_mn ? make_map(&b, q.dtype, q.B, q.cols, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
+                         : make_map(&b, q.dtype, q.B, q.K, b_rows, 64, q.glu && tile != kTilePair ? bn / 2 : br, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = make_out_map(&y, q.dtype, q.Y, q.cols, 1, q.rows);
+    if (!rc) rc = q.Z ? make_out_map(&z, q.dtype, q.Z, q.cols, q.glu ? 2 : 1, q.rows) : (z = y, ALPHA_OK);
+    if (rc) return rc;
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        if (q.glu) {
+            if (tile == kTilePair) launch_mma<T, true, 256, true>(a, b, y, z, p, sms, stream);
+            else if (tile == kTile128) launch_mma<T, false, 128, true>(a, b, y, z, p, sms, stream);
+            else launch_mma<T, false, 64, true>(a, b, y, z, p, sms, stream);
+        } else {
+            if (tile == kTilePair) launch_mma<T, true, 256, false>(a, b, y, z, p, sms, stream);
+            else if (tile == kTile128) launch_mma<T, false, 128, false>(a, b, y, z, p, sms, stream);
+            else launch_mma<T, false, 64, false>(a, b, y, z, p, sms, stream);
+        }
+    };
+    if (q.dtype == ALPHA_BF16) go(__nv_bfloat16{});
+    else go(__half{});
+    note_launch("fc");
+    note_plan("fc %s%dx%d", tile == kTilePair ? "pair " : "", bm, bn);
+    return launched("fc_mma_kernel");
+}
+
+// ---- fp32 products ----------------------------------------------------------------------------------------------
+
+template <int FORM>
+int launch_f32(const float* A, const float* B, int rows, int cols, int K, int lda, int ldb, const FcEpilogue& e, cudaStream_t stream)
+{
+    int sms = 0, slice = 0, *status = nullptr;
+    int rc = device_sms(&sms);
+    if (!rc) rc = planes_launch_slice(&slice);
+    if (!rc) rc = device_status_word(&status);
+    if (rc) return rc;
+    PlaneFc<FORM> p{};
+    p.A = A; p.B = B; p.rows = rows; p.cols = cols; p.K = K; p.lda = lda; p.ldb = ldb; p.e = e;
+    p.size = static_cast<size_t>(rows) * cols;
+    PlanePlan plan = plan_planes(rows, cols, K, 1, 16, static_cast<double>(p.size), 0, sms);
+    if (plan.ksplit > 1) {
+        void* ws = nullptr;
+        rc = call_scratch(stream, plan.ksplit * p.size * sizeof(float), &ws);
+        if (rc) return rc;
+        p.part = static_cast<float*>(ws);
+    }
+    p.ksplit = plan.ksplit;
+    if (dry_run()) return ALPHA_OK;
+    const dim3 grid((rows + kPlaneBM - 1) / kPlaneBM, (cols + plan.bn - 1) / plan.bn, plan.ksplit);
+    launch_planes(p, plan.bn, grid, slice, stream, status);
+    note_launch("fc");
+    note_plan("fc planes 128x%d ksplit=%d", plan.bn, plan.ksplit);
+    rc = launched("gemm_planes_kernel");
+    if (rc || plan.ksplit == 1) return rc;
+    const size_t n4 = p.size / 4, blocks = (n4 + 255) / 256;
+    launch_after(fc_parts_kernel<FORM == kFcGlu>, static_cast<unsigned>(blocks < sms * 8u ? blocks : sms * 8u), 256, 0, stream, reinterpret_cast<const float4*>(p.part), n4,
+                 plan.ksplit, cols / 4, e);
+    note_launch("fc");
+    return launched("fc_parts_kernel");
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------
+
+constexpr int kSmallRows = 4;
+
+template <class T, bool GLU>
+int launch_small(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, cudaStream_t stream)
+{
+    int sms = 0;
+    const int rc = device_sms(&sms);
+    if (rc) return rc;
+    FcSmall p{s->rows, s->IC, s->OC, 1, s->act, s->k, X, W, bias, residual, Z, Y};
+    const int units = GLU ? s->OC : (s->OC + 1) / 2, words = s->IC / Word16<T>::N;
+    // 16 warps an SM, each with 64 words of a row at least
+    while (p.ks < 8 && static_cast<long long>(units) * p.ks < 16LL * sms && words >= 128 * p.ks) p.ks *= 2;
+    const int teams = 8 / p.ks;
+    const unsigned blocks = (units + teams - 1) / teams;
+    if (s->rows == 1) launch_after(fc_small_kernel<T, 1, GLU>, blocks, 256, 0, stream, p);
+    else if (s->rows == 2) launch_after(fc_small_kernel<T, 2, GLU>, blocks, 256, 0, stream, p);
+    else launch_after(fc_small_kernel<T, 4, GLU>, blocks, 256, 0, stream, p);
+    note_launch("fc_small");
+    note_plan("fc small ks=%d", p.ks);
+    return launched("fc_small_kernel");
+}
+
+int forward(const char* what, const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, bool glu, cudaStream_t stream)
+{
+    int rc = call_begin(stream);
+    if (rc) return rc;
+    if (s->rows <= kSmallRows && !option_fc_tile()) {
+        if (dry_run()) return ALPHA_OK;
+        switch (s->dtype) {
+        case ALPHA_F32: return glu ? launch_small<float, true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<float, false>(s, X, W, bias, residual, Z, Y, stream);
+        case ALPHA_BF16:
+            return glu ? launch_small<__nv_bfloat16, true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<__nv_bfloat16, false>(s, X, W, bias, residual, Z, Y, stream);
+        default: return glu ? launch_small<__half, true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<__half, false>(s, X, W, bias, residual, Z, Y, stream);
+        }
+    }
+    if (s->dtype == ALPHA_F32) {
+        const FcEpilogue e{static_cast<const float*>(bias), static_cast<const float*>(residual), static_cast<float*>(Z), static_cast<float*>(Y), s->OC, s->act, s->k};
+        const float *x = static_cast<const float*>(X), *w = static_cast<const float*>(W);
+        return glu ? launch_f32<kFcGlu>(x, w, s->rows, 2 * s->OC, s->IC, s->IC, s->IC, e, stream) : launch_f32<kFcForward>(x, w, s->rows, s->OC, s->IC, s->IC, s->IC, e, stream);
+    }
+    if (dry_run()) return ALPHA_OK;
+    return launch_product(Product{s->dtype, s->rows, s->OC, s->IC, false, false, glu, X, W, bias, residual, Z, Y, s->act, s->k}, stream);
+}
+
+template <class T, bool GLU>
+int launch_delta(const AlphaFcShape* s, const void* dY, const void* Z, void* dZ, void* dB, cudaStream_t stream)
+{
+    int sms = 0;
+    int rc = device_sms(&sms);
+    if (rc) return rc;
+    const int wide = GLU ? 2 * s->OC : s->OC, words = s->OC / Word16<T>::N;
+    const unsigned gy = (words + 31) / 32;
+    // eight CTAs an SM, eight rows of a warp at least
+    long long gx = (sms * 8LL + gy - 1) / gy;
+    const long long by_rows = (s->rows + 63) / 64;
+    if (gx > by_rows) gx = by_rows;
+    FcDelta p{s->rows, s->OC, s->act, s->k, dY, Z, dZ, nullptr};
+    if (dB) {
+        void* ws = nullptr;
+        rc = call_scratch(stream, static_cast<size_t>(gx) * wide * sizeof(float), &ws);
+        if (rc) return rc;
+        p.part = static_cast<float*>(ws);
+    }
+    if (dry_run()) return ALPHA_OK;
+    launch_after(fc_delta_kernel<T, GLU>, dim3(gy, static_cast<unsigned>(gx)), 256, 0, stream, p);
+    note_launch("fc_delta");
+    rc = launched("fc_delta_kernel");
+    if (rc || !dB) return rc;
+    launch_after(fc_bias_kernel<T>, (wide + 31) / 32, 256, 0, stream, p.part, static_cast<int>(gx), wide, static_cast<T*>(dB));
+    note_launch("fc_delta");
+    return launched("fc_bias_kernel");
+}
+
+int delta(const char* what, const AlphaFcShape* s, const void* dY, const void* X, const void* W, const void* Z, void* dZ, void* dX, void* dW, void* dB, bool glu,
+          cudaStream_t stream)
+{
+    int rc = check_fc(what, s, glu);
+    if (rc) return rc;
+    const bool through = glu || s->act != ALPHA_ACT_NONE;           // dZ is not deltaY
+    if (!dY || (dX && !W) || (dW && !X)) return fail(ALPHA_E_ARG, "%s: null tensor pointer", what);
+    if (!dX && !dW && !dB) return fail(ALPHA_E_ARG, "%s: no gradient asked for", what);
+    if (through && (!Z || !dZ)) return fail(ALPHA_E_ARG, "%s: Z of the forward pass and memory for deltaZ are needed (deltaZ may be Z)", what);
+    const size_t b = type_bytes(s->dtype), wide = glu ? 2 * static_cast<size_t>(s->OC) : s->OC, rows = s->rows;
+    if (!through) { Z = nullptr; dZ = nullptr; }
+    const Span in_z{dZ == Z ? nullptr : Z, rows * wide * b};
+    rc = check_spans(what, {{dY, rows * s->OC * b}, {dW ? X : nullptr, rows * s->IC * b}, {dX ? W : nullptr, wide * s->IC * b}, in_z},
+                     {{dZ, rows * wide * b}, {dX, rows * s->IC * b}, {dW, wide * s->IC * b}, {dB, wide * b}});
+    if (!rc) rc = call_begin(stream);
+    if (rc) return rc;
+    if (through || dB) {
+        switch (s->dtype) {
+        case ALPHA_F32: rc = glu ? launch_delta<float, true>(s, dY, Z, dZ, dB, stream) : launch_delta<float, false>(s, dY, Z, dZ, dB, stream); break;
+        case ALPHA_BF16: rc = glu ? launch_delta<__nv_bfloat16, true>(s, dY, Z, dZ, dB, stream) : launch_delta<__nv_bfloat16, false>(s, dY, Z, dZ, dB, stream); break;
+        default: rc = glu ? launch_delta<__half, true>(s, dY, Z, dZ, dB, stream) : launch_delta<__half, false>(s, dY, Z, dZ, dB, stream);
+        }
+        if (rc) return rc;
+    }
+    const void* d = through ? dZ : dY;
+    const int w = static_cast<int>(wide);
+    if (s->dtype == ALPHA_F32) {
+        FcEpilogue e{nullptr, nullptr, nullptr, static_cast<float*>(dX), s->IC, ALPHA_ACT_NONE, 0.f};
+        const float* z = static_cast<const float*>(d);
+        if (dX) rc = launch_f32<kFcDeltaX>(z, static_cast<const float*>(W), s->rows, s->IC, w, w, s->IC, e, stream);
+        e.Y = static_cast<float*>(dW);
+        if (!rc && dW) rc = launch_f32<kFcDeltaW>(z, static_cast<const float*>(X), w, s->IC, s->rows, w, s->IC, e, stream);
+        return rc;
+    }
+    if (dry_run()) return ALPHA_OK;
+    if (dX) rc = launch_product(Product{s->dtype, s->rows, s->IC, w, false, true, false, d, W, nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f}, stream);
+    if (!rc && dW) rc = launch_product(Product{s->dtype, w, s->IC, s->rows, true, true, false, d, X, nullptr, nullptr, nullptr, dW, ALPHA_ACT_NONE, 0.f}, stream);
+    return rc;
+}
+
+}  // namespace
+
+extern "C" {
+
+int alpha_fullConnect(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, alpha_stream_t stream)
+{
+    OpRange range("alpha_fullConnect");
+    int rc = check_fc("fullConnect", s, false);
+    if (rc) return rc;
+    if (!X || !W || !Y) return fail(ALPHA_E_ARG, "fullConnect: null tensor pointer");
+    const size_t b = type_bytes(s->dtype), y = static_cast<size_t>(s->rows) * s->OC * b;
+    if (reinterpret_cast<uintptr_t>(residual) & 15) return fail(ALPHA_E_ARG, "fullConnect: tensor pointers must be 16-byte aligned");
+    rc = check_spans("fullConnect", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, static_cast<size_t>(s->OC) * s->IC * b}, {bias, s->OC * b}, {residual == Y ? nullptr : residual, y}},
+                     {{Y, y}, {Z, y}});
+    return rc ? rc : forward("fullConnect", s, X, W, bias, residual, Z, Y, false, static_cast<cudaStream_t>(stream));
+}
+
+int alpha_fullConnect_glu(const AlphaFcShape* s, const void* X, const void* W, const void* bias, void* Z, void* Y, alpha_stream_t stream)
+{
+    OpRange range("alpha_fullConnect_glu");
+    int rc = check_fc("fullConnect_glu", s, true);
+    if (rc) return rc;
+    if (!X || !W || !Y) return fail(ALPHA_E_ARG, "fullConnect_glu: null tensor pointer");
+    const size_t b = type_bytes(s->dtype), y = static_cast<size_t>(s->rows) * s->OC * b;
+    rc = check_spans("fullConnect_glu", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, 2 * static_cast<size_t>(s->OC) * s->IC * b}, {bias, 2 * s->OC * b}}, {{Y, y}, {Z, 2 * y}});
+    return rc ? rc : forward("fullConnect_glu", s, X, W, bias, nullptr, Z, Y, true, static_cast<cudaStream_t>(stream));
+}
+
+int alpha_fullConnect_delta(const AlphaFcShape* s, const void* deltaY, const void* X, const void* W, const void* Z, void* deltaZ, void* deltaX, void* deltaW, void* deltaB,
+                            alpha_stream_t stream)
+{
+    OpRange range("alpha_fullConnect_delta");
+    return delta("fullConnect_delta", s, deltaY, X, W, Z, deltaZ, deltaX, deltaW, deltaB, false, static_cast<cudaStream_t>(stream));
+}
+
+int alpha_fullConnect_glu_delta(const AlphaFcShape* s, const void* deltaY, const void* X, const void* W, const void* Z, void* deltaZ, void* deltaX, void* deltaW, void* deltaB,
+                                alpha_stream_t stream)
+{
+    OpRange range("alpha_fullConnect_glu_delta");
+    return delta("fullConnect_glu_delta", s, deltaY, X, W, Z, deltaZ, deltaX, deltaW, deltaB, true, static_cast<cudaStream_t>(stream));
+}
+
+int alpha_fullConnect_workspace_bytes(const AlphaFcShape* s, int glu, int op, size_t* bytes)
+{
+    if (!s || !bytes) return fail(ALPHA_E_ARG, "fullConnect_workspace_bytes: null argument");
+    if (op != ALPHA_OP_FORWARD && op != ALPHA_OP_DELTAX) return fail(ALPHA_E_ARG, "fullConnect_workspace_bytes: unknown op %d", op);
+    // the call itself with launches switched off: what it asks for is what it will ask for (tensors at placeholder addresses far apart)
+    auto at = [](int i) { return reinterpret_cast<void*>(static_cast<uintptr_t>(i + 1) << 44); };
+    dry_begin();
+    int rc;
+    if (op == ALPHA_OP_FORWARD) rc = glu ? alpha_fullConnect_glu(s, at(0), at(1), at(2), at(3), at(4), nullptr) : alpha_fullConnect(s, at(0), at(1), at(2), nullptr, at(3), at(4), nullptr);
+    else rc = (glu ? alpha_fullConnect_glu_delta : alpha_fullConnect_delta)(s, at(0), at(1), at(2), at(3), at(4), at(5), at(6), at(7), nullptr);
+    *bytes = dry_end();
+    return rc;
+}
+
+}  // extern "C"

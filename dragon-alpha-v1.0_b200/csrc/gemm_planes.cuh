@@ -637,13 +637,6 @@ __device__ __noinline__ void gemm_planes_look(const P& p, const typename P::Cta&
     if (again) gemm_planes_again<BN>(p, c, rows, outs, smem, tid);
 }
 
-// After a wait that ran out: time for what has been issued to end, before shared and tensor memory are given back.
-static __device__ __noinline__ void settle()
-{
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < 1000000ull) {}
-}
-
 template <int BN, class P, bool TMA_B>
 __global__ void __launch_bounds__(kPlaneThreads, 1) gemm_planes_kernel(const __grid_constant__ P p, const __grid_constant__ CUtensorMap tmB, const PlaneGrid grid, int* status)
 {

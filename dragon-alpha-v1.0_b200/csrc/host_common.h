@@ -29,5 +29,25 @@ int device_status_word(int** status);
 int planes_launch_slice(int* ctas);
 // Option F32_PLANES.
 int option_f32_planes();
+// Option FC_TILE.
+int option_fc_tile();
+
+// Scratch of one call, for the other translation units: call_begin starts a call on a stream (its block is carved from the start
+// again), call_scratch gives `bytes` of it.  Under dry_run() (between dry_begin and dry_end, which returns the bytes asked for)
+// nothing is allocated and callers launch nothing.
+int call_begin(cudaStream_t stream);
+int call_scratch(cudaStream_t stream, size_t bytes, void** out);
+bool dry_run();
+void dry_begin();
+size_t dry_end();
+// cuTensorMapEncodeTiled (after call_begin, which finds it).
+int encode_tiled(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides_bytes, const cuuint32_t* box,
+                 CUtensorMapSwizzle swizzle);
+// One NVTX range per operator call (option NVTX).
+struct OpRange {
+    bool on;
+    explicit OpRange(const char* name);
+    ~OpRange();
+};
 
 }  // namespace alpha

@@ -35,6 +35,13 @@ __device__ __forceinline__ bool elect_one()
     return pred != 0;
 }
 
+// After a wait that ran out: time for what has been issued to end, before shared and tensor memory are given back.
+static __device__ __noinline__ void settle()
+{
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {}
+}
+
 // Device status word: which role's bounded wait ran out first.
 enum KernelStatus : int {
     kStatusOk = 0,
@@ -252,6 +259,14 @@ __device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap
         "l"(reinterpret_cast<uint64_t>(m)), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* m, uint32_t cluster_bar, int c0, int c1)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(cluster_bar), "r"(c0), "r"(c1)
+        : "memory");
+}
 // Tensor memory of a CTA pair: one warp of each CTA (same warp index) issues these together.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols)
 {
@@ -371,6 +386,12 @@ __device__ __forceinline__ void tma_store_4d_a(const CUtensorMap* m, uint32_t sr
                  "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                  : "memory");
 }
+__device__ __forceinline__ void tma_store_3d_a(const CUtensorMap* m, uint32_t src, int c0, int c1, int c2)
+{
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(m)),
+                 "r"(src), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
 __device__ __forceinline__ void tma_store_commit()
 {
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -487,6 +508,7 @@ enum : uint32_t { kSwizzleNone = 0, kSwizzle128B_Base32B = 1, kSwizzle128B = 2, 
 //   MN-major tf32 (kSwizzle128B_Base32B): a block is 32 elements (128 B) wide, its swizzle atom
 //             4 K-rows deep (512 B); sbo = distance between 4-row K groups, lbo = distance between
 //             32-wide MN blocks.  One K=8 instruction spans two atoms.
+//   MN-major 16-bit (kSwizzle128B): a block is 64 elements (128 B) wide, its atom 8 K-rows deep (1024 B); lbo and sbo as below.
 //   MN-major 16-bit (kSwizzle64B): a block is 32 elements (64 B) wide, its atom 8 K-rows deep (512 B); sbo = distance between
 //             8-row K groups, lbo = distance between 32-wide MN blocks.  One K=16 instruction spans two atoms.
 __device__ __forceinline__ uint64_t make_smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo,
@@ -546,6 +568,40 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, bool a_mn_m
 {
     return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn_major ? 1u : 0u) << 15 | (b_mn_major ? 1u : 0u) << 16 |
            static_cast<uint32_t>(N >> 3) << 17 | static_cast<uint32_t>(M >> 4) << 24;
+}
+// The same with both operands fp16.
+__host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn_major, bool b_mn_major)
+{
+    return make_idesc_bf16(M, N, a_mn_major, b_mn_major) & ~(1u << 7 | 1u << 10);
+}
+// D[tmem] (+)= A * B for 16-bit operands, over one CTA or (PAIR) a CTA pair; one thread issues.
+template <bool PAIR>
+__device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate)
+{
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            ".reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %2};\n\t"
+            "mov.b64 db, {%3, %4};\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, {%7, %7, %7, %7, %7, %7, %7, %7}, p;\n\t"
+            "}\n" ::"r"(d_tmem),
+            "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            ".reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %2};\n\t"
+            "mov.b64 db, {%3, %4};\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
+            "}\n" ::"r"(d_tmem),
+            "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
 // Executed by a converged warp, issued by the lane whose `elected` is set; descriptors as (lo, hi) halves with offsets (16-byte units).
 template <uint32_t A_OFF, uint32_t B_OFF>

@@ -147,6 +147,10 @@ class CudaFloat32EngineBase:
     def _addr(a):
         return a.data_ptr() if isinstance(a, torch.Tensor) else int(a)
 
+    @classmethod
+    def _addr_or_none(cls, a):
+        return None if a is None else cls._addr(a)
+
     def conv3D(self, Y_address, OH, OW, X_address, IH, IW, W_address, FH, FW, N, IC, OC, sh, sw, ph, pw):
         """CudaFloat32EngineBase.conv3D (:1355-1474)."""
         a = self._addr
@@ -282,6 +286,28 @@ class CudaFloat32EngineBase:
         self._mm(self._lib.alpha_engine_batchMatMulT2, a(C_address), a(A_address), a(B_address), Batch, N, CM, BM, K,
                  _stream(self._stream))
 
+    # ---- FullConnect layers of a transformer (no counterpart in the reference, which runs matMul, linear_dual2D_row and the
+    # activation one after the other) ----
+    def fullConnect(self, Y_address, X_address, W_address, rows, IC, OC, dtype, act, k, Bias_address=None, Residual_address=None, Z_address=None):
+        """Y = act(X W^T + Bias) + Residual, Z = X W^T + Bias; addresses of X[rows, IC], W[OC, IC], and so on (alpha_fullConnect)."""
+        a = self._addr_or_none
+        _l.check(self._lib.alpha_fullConnect(C.byref(_l.AlphaFcShape(rows, IC, OC, dtype, act, k)), a(X_address), a(W_address), a(Bias_address), a(Residual_address),
+                                             a(Z_address), a(Y_address), _stream(self._stream)))
+
+    def fullConnect_glu(self, Y_address, X_address, W_address, rows, IC, OC, dtype, act, k, Bias_address=None, Z_address=None):
+        """Y = act(Z[:, :OC]) * Z[:, OC:], Z = X W^T + Bias with W[2 OC, IC] (alpha_fullConnect_glu)."""
+        a = self._addr_or_none
+        _l.check(self._lib.alpha_fullConnect_glu(C.byref(_l.AlphaFcShape(rows, IC, OC, dtype, act, k)), a(X_address), a(W_address), a(Bias_address), a(Z_address),
+                                                 a(Y_address), _stream(self._stream)))
+
+    def fullConnect_delta(self, deltaX_address, deltaW_address, deltaB_address, deltaY_address, X_address, W_address, Z_address, deltaZ_address, rows, IC, OC,
+                          dtype, act, k, glu=False):
+        """The gradients of fullConnect, or of fullConnect_glu (alpha_fullConnect_delta, alpha_fullConnect_glu_delta)."""
+        a = self._addr_or_none
+        fn = self._lib.alpha_fullConnect_glu_delta if glu else self._lib.alpha_fullConnect_delta
+        _l.check(fn(C.byref(_l.AlphaFcShape(rows, IC, OC, dtype, act, k)), a(deltaY_address), a(X_address), a(W_address), a(Z_address), a(deltaZ_address),
+                    a(deltaX_address), a(deltaW_address), a(deltaB_address), _stream(self._stream)))
+
     # ---- pooling, Java argument order (CudaFloat32EngineBase.java:2012-2215) ----
     def _pool(self, fn, N, IH, IW, IC, FH, FW, OH, OW, sh, sw, ph, pw, *ptrs_and_flags):
         s = _pool_shape(N, IH, IW, IC, FH, FW, OH, OW, sh, sw, ph, pw)
@@ -349,6 +375,26 @@ def _pad_both(t, n4, c4):
     with torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext():
         _l.check(_l.load().alpha_pad_rows(t.data_ptr(), rows, shape[-1], out.data_ptr(), rows // shape[0] * n4, c4, _stream()))
     return out
+
+
+_FC_TYPES = {torch.float32: _l.ALPHA_F32, torch.bfloat16: _l.ALPHA_BF16, torch.float16: _l.ALPHA_F16}
+
+
+def _fc_padded(t, n):
+    """t, dense, on a 16-byte boundary and with its last dimension zero-padded to n."""
+    if t.shape[-1] != n:
+        return _pad_both(t, t.shape[0], n)
+    t = t.contiguous()
+    if t.is_neg() or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format).resolve_neg()
+    return t
+
+
+def _fc_halves(t, oc, n):
+    """t, whose last dimension is two halves of oc, with each half zero-padded to n."""
+    if oc == n:
+        return _fc_padded(t, 2 * n)
+    return _fc_padded(t.reshape(-1, oc), n).reshape(t.shape[:-1] + (2 * n,))
 
 
 _pack_jobs = {n: struct.Struct("%dq" % (6 * n)).pack for n in (1, 2, 3)}
@@ -525,6 +571,166 @@ class Engine:
         C = _new(A, (n4, m4))
         self.base.matMulT2(C, Ap, Bp, n4, m4, k4)
         return C[:N, :M]
+
+    # ---- FullConnect layers of a transformer: the product with bias, activation and residual in its epilogue, the gated block, their
+    # gradients.  float32, bfloat16 or float16 tensors (all of one type); X may have any leading dimensions; IC and OC that are no
+    # multiples of 16 bytes are zero-padded as everywhere. ----
+    @staticmethod
+    def _fc_check(what, X, W, glu, act, **others):
+        if X.dtype not in _FC_TYPES:
+            raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, X.dtype))
+        if act not in _l.ACTS:
+            raise ValueError("%s: act must be one of %s, not %r" % (what, ", ".join(sorted(_l.ACTS)), act))
+        if X.dim() < 1 or W.dim() != 2 or W.shape[1] != X.shape[-1]:
+            raise ValueError("%s: X %s against W %s" % (what, tuple(X.shape), tuple(W.shape)))
+        if glu and W.shape[0] % 2:
+            raise ValueError("%s: W has %d rows, which are not gate rows and as many up rows" % (what, W.shape[0]))
+        IC, wide = X.shape[-1], W.shape[0]
+        OC = wide // 2 if glu else wide
+        if IC == 0 or OC == 0:
+            raise ValueError("%s: X %s against W %s" % (what, tuple(X.shape), tuple(W.shape)))
+        lead = tuple(X.shape[:-1])
+        shapes = {"Bias": (wide,), "Residual": lead + (OC,), "deltaY": lead + (OC,), "Z": lead + (wide,)}
+        for name, t in dict(others, W=W).items():
+            if t is None:
+                continue
+            if name != "W" and tuple(t.shape) != shapes[name]:
+                raise ValueError("%s: %s %s, expected %s" % (what, name, tuple(t.shape), shapes[name]))
+            if t.dtype != X.dtype or t.device != X.device:
+                raise ValueError("%s: %s is %s on %s, X %s on %s" % (what, name, t.dtype, t.device, X.dtype, X.device))
+        if not X.is_cuda:
+            raise ValueError("%s: tensors must be on a GPU" % what)
+        unit = 4 if X.dtype == torch.float32 else 8
+        return IC, OC, lead, -(-IC // unit) * unit, -(-OC // unit) * unit
+
+    def _fc_forward(self, what, X, W, Bias, act, k, Residual, save, glu):
+        IC, OC, lead, ic, oc = self._fc_check(what, X, W, glu, act, Bias=Bias, Residual=Residual)
+        halves = 2 if glu else 1
+        rows = X.numel() // IC
+        with self._on(X):
+            if rows == 0:
+                Y = X.new_empty(lead + (OC,))
+                return (Y, X.new_empty(lead + (halves * OC,))) if save else Y
+            Xp = _fc_padded(X.reshape(rows, IC), ic)
+            Wp = _fc_padded(W.reshape(halves, OC, IC) if oc != OC else W, ic)
+            if oc != OC:
+                padded = Wp.new_zeros((halves, oc, ic))
+                padded[:, :OC] = Wp.reshape(halves, OC, ic)
+                Wp = padded
+            Bp = None if Bias is None else _fc_halves(Bias, OC, oc) if glu else _fc_padded(Bias.reshape(1, OC), oc)
+            Rp = None if Residual is None else _fc_padded(Residual.reshape(rows, OC), oc)
+            Y, Z = X.new_empty((rows, oc)), X.new_empty((rows, halves * oc)) if save else None
+            if glu:
+                self.base.fullConnect_glu(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[X.dtype], _l.ACTS[act], float(k), Bp, Z)
+            else:
+                self.base.fullConnect(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[X.dtype], _l.ACTS[act], float(k), Bp, Rp, Z)
+        if oc != OC:
+            Y = Y[:, :OC]
+            if save:
+                Z = torch.cat((Z[:, :OC], Z[:, oc:oc + OC]), dim=1) if glu else Z[:, :OC]
+        Y = Y.reshape(lead + (OC,))
+        return (Y, Z.reshape(lead + (halves * OC,))) if save else Y
+
+    def _fc_delta(self, what, deltaY, X, W, Z, act, k, bias, glu):
+        IC, OC, lead, ic, oc = self._fc_check(what, X, W, glu, act, deltaY=deltaY, Z=Z)
+        through = glu or act != "none"
+        if through and Z is None:
+            raise ValueError("%s: Z of the forward pass is needed" % what)
+        halves = 2 if glu else 1
+        rows = X.numel() // IC
+        with self._on(X):
+            if rows == 0:
+                return torch.empty_like(X), torch.zeros_like(W), W.new_zeros((halves * OC,)) if bias else None
+            dYp, Xp = _fc_padded(deltaY.reshape(rows, OC), oc), _fc_padded(X.reshape(rows, IC), ic)
+            Wp = _fc_padded(W.reshape(halves, OC, IC) if oc != OC else W, ic)
+            if oc != OC:
+                padded = Wp.new_zeros((halves, oc, ic))
+                padded[:, :OC] = Wp.reshape(halves, OC, ic)
+                Wp = padded
+            Zp = dZ = None
+            if through:
+                Zp = _fc_halves(Z.reshape(rows, 2 * OC), OC, oc) if glu else _fc_padded(Z.reshape(rows, OC), oc)
+                dZ = torch.empty_like(Zp)
+            dX, dW = X.new_empty((rows, ic)), W.new_empty((halves, oc, ic))
+            dB = W.new_empty((halves, oc)) if bias else None
+            self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, oc, _FC_TYPES[X.dtype], _l.ACTS[act], float(k), glu)
+        dX = dX if ic == IC else dX[:, :IC]
+        if oc != OC or ic != IC:
+            dW = dW[:, :OC, :IC]
+        if bias:
+            dB = (dB if oc == OC else dB[:, :OC]).reshape(halves * OC)
+        return dX.reshape(lead + (IC,)), dW.reshape(halves * OC, IC), dB
+
+    def fullConnect(self, X, W, Bias=None, act="none", k=0.0, Residual=None, save=False):
+        """act(X W^T + Bias) + Residual in one pass; W [OC, IC], X [..., IC].  act: 'none', 'leakyRelu' (slope k; relu k = 0),
+        'sigmoid', 'silu', 'gelu' (of the normal distribution function) or 'gelu_tanh'.  save=True also returns
+        Z = X W^T + Bias, which fullConnect_delta reads."""
+        return self._fc_forward("fullConnect", X, W, Bias, act, k, Residual, save, False)
+
+    def fullConnect_delta(self, deltaY, X, W, Z=None, act="none", k=0.0, bias=False):
+        """(deltaX, deltaW, deltaB) of fullConnect from deltaY and its Z (not needed with act 'none'); deltaB is None without
+        bias=True.  The gradient of a residual is deltaY itself."""
+        return self._fc_delta("fullConnect_delta", deltaY, X, W, Z, act, k, bias, False)
+
+    def fullConnect_glu(self, X, W, Bias=None, act="silu", k=0.0, save=False):
+        """The gated block act(G) * U with [G | U] = Z = X W^T + Bias in one pass; W [2 OC, IC]: the gate rows, then the up rows.
+        save=True also returns Z, which fullConnect_glu_delta reads."""
+        return self._fc_forward("fullConnect_glu", X, W, Bias, act, k, None, save, True)
+
+    def fullConnect_glu_delta(self, deltaY, X, W, Z, act="silu", k=0.0, bias=False):
+        """(deltaX, deltaW, deltaB) of fullConnect_glu from deltaY and its Z; deltaB is None without bias=True."""
+        return self._fc_delta("fullConnect_glu_delta", deltaY, X, W, Z, act, k, bias, True)
+
+    # ---- all gradients of a step ----
+    def _on(self, t):
+        """t's device as the current one and, where the engine has a stream of its own, that as the current one: copies and memory of
+        the call then belong to the stream its kernels run on."""
+        s = self.base._stream
+        if s is not None:
+            if s.device != t.device:
+                raise ValueError("the engine's stream is on %s, the tensors on %s" % (s.device, t.device))
+            return torch.cuda.stream(s)
+        return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+    def _grads(self, what, grads, Out):
+        grads = list(grads)
+        Out = grads if Out is None else list(Out)
+        if len(Out) != len(grads):
+            raise ValueError("%s: %d gradients, %d outputs" % (what, len(grads), len(Out)))
+        table = (_l.AlphaGrad * max(len(grads), 1))()
+        for e, g, o in zip(table, grads, Out):
+            for t in (g, o):
+                if t.dtype not in _FC_TYPES:
+                    raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, t.dtype))
+                if not t.is_cuda or t.device != grads[0].device:
+                    raise ValueError("%s: tensors must be on one GPU" % what)
+                if not t.is_contiguous() or t.is_neg():
+                    raise ValueError("%s: tensors must be contiguous" % what)
+            if g.shape != o.shape:
+                raise ValueError("%s: gradient %s, output %s" % (what, tuple(g.shape), tuple(o.shape)))
+            e.grad, e.out, e.count, e.dtype, e.out_dtype = g.data_ptr(), o.data_ptr(), g.numel(), _FC_TYPES[g.dtype], _FC_TYPES[o.dtype]
+        return grads, table
+
+    def grad_norm(self, grads):
+        """The 2-norm of all elements of a list of gradients (float32, bfloat16, float16) as a 0-dimensional float32 tensor."""
+        grads, table = self._grads("grad_norm", grads, None)
+        if not grads:
+            return torch.zeros((), device="cuda")
+        with self._on(grads[0]):
+            norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+            _l.check(self.base._lib.alpha_grad_norm(len(grads), table, norm.data_ptr(), _stream(self.base._stream)))
+        return norm
+
+    def clip_grad_norm(self, grads, max_norm, Out=None):
+        """grad_norm, and every gradient scaled by min(1, max_norm / (norm + 1e-6)): in place, or into the tensors of Out, which may
+        be of another type.  Nothing waits for the norm on the host."""
+        grads, table = self._grads("clip_grad_norm", grads, Out)
+        if not grads:
+            return torch.zeros((), device="cuda")
+        with self._on(grads[0]):
+            norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+            _l.check(self.base._lib.alpha_clip_grad_norm(len(grads), table, float(max_norm), norm.data_ptr(), _stream(self.base._stream)))
+        return norm
 
     # Batched products with the engine's memory rule (only the last dimension of a tensor is padded to a multiple
     # of 4) and EngineCore's argument mapping (EngineCore.java:579-623): the row pitch and the logical row length

@@ -18,6 +18,18 @@ class AlphaPoolShape(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("N", "IH", "IW", "IC", "FH", "FW", "OH", "OW", "sh", "sw", "ph", "pw")]
 
 
+ALPHA_F32, ALPHA_BF16, ALPHA_F16 = 0, 1, 2
+ACTS = {"none": 0, "leakyRelu": 1, "sigmoid": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
+
+
+class AlphaFcShape(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("rows", "IC", "OC", "dtype", "act")] + [("k", C.c_float)]
+
+
+class AlphaGrad(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("count", C.c_int64), ("dtype", C.c_int), ("out_dtype", C.c_int)]
+
+
 class AlphaConvError(RuntimeError):
     """A call into the library returned a non-zero status; .code holds the ALPHA_E_* value."""
 
@@ -130,6 +142,15 @@ def load():
         getattr(lib, name).argtypes = [V, V, V, I, I, I, I, I, V]
     for name in ("batchMatMul", "batchMatMul_texture", "batchMatMulT1", "batchMatMulT2", "batchMatMulT2_texture"):
         getattr(lib, "alpha_Cuda_batchMatMul_" + name).argtypes = [SA, I, V, V, V, I, I, I, I, I]
+    # FullConnect layers of a transformer, and all gradients of a step
+    F, G = C.POINTER(AlphaFcShape), C.POINTER(AlphaGrad)
+    lib.alpha_fullConnect.argtypes = [F, V, V, V, V, V, V, V]
+    lib.alpha_fullConnect_glu.argtypes = [F, V, V, V, V, V, V]
+    lib.alpha_fullConnect_delta.argtypes = [F, V, V, V, V, V, V, V, V, V]
+    lib.alpha_fullConnect_glu_delta.argtypes = [F, V, V, V, V, V, V, V, V, V]
+    lib.alpha_fullConnect_workspace_bytes.argtypes = [F, I, I, C.POINTER(C.c_size_t)]
+    lib.alpha_grad_norm.argtypes = [I, G, V, V]
+    lib.alpha_clip_grad_norm.argtypes = [I, G, C.c_float, V, V]
     # pooling
     PS = C.POINTER(AlphaPoolShape)
     lib.alpha_pool2D_max.argtypes = [PS, V, V, V]
@@ -204,6 +225,13 @@ def workspace_bytes(shape, op):
     """Scratch bytes one call of `op` ('forward', 'deltaX', 'deltaW', 'bias_grad') on `shape` needs."""
     n = C.c_size_t(0)
     check(load().alpha_conv_workspace_bytes(C.byref(shape), OPS[op], C.byref(n)))
+    return n.value
+
+
+def fullConnect_workspace_bytes(shape, glu, op):
+    """Scratch bytes of a fullConnect (glu: fullConnect_glu) call: op 'forward', or 'deltaX' for that of all gradients."""
+    n = C.c_size_t(0)
+    check(load().alpha_fullConnect_workspace_bytes(C.byref(shape), int(bool(glu)), OPS[op], C.byref(n)))
     return n.value
 
 

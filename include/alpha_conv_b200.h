@@ -448,6 +448,67 @@ int alpha_engine_batchMatMulT1(float* C, const float* A, const float* B, int Bat
 int alpha_engine_batchMatMulT2(float* C, const float* A, const float* B, int Batch, int N, int CM, int BM, int K,
                                alpha_stream_t stream);
 
+/* ---- FullConnect layers of a transformer ----------------------------------------------------------------------
+ *
+ * The matrix product of a FullConnect layer with what surrounds it in the same pass, over fp32 or 16-bit tensors:
+ *   alpha_fullConnect        Z = X W^T + bias,  Y = act(Z) + residual          W[OC][IC], the layout of a 1x1 convolution's
+ *   alpha_fullConnect_glu    Z = X W^T + bias,  Y = act(Z[:, :OC]) * Z[:, OC:]  W[2 OC][IC]: OC gate rows, then OC up rows
+ * X[rows][IC], Y and residual [rows][OC], Z [rows][OC] (glu: [rows][2 OC]), bias[OC] (glu: [2 OC]); all of one type, dense,
+ * 16-byte aligned, IC and OC multiples of 4 (fp32) or 8 (16-bit).  bias, residual and Z may be NULL; Z keeps the sums for the
+ * backward pass.  residual may be Y itself; no other output may overlap an input (ALPHA_E_ARG).
+ * Sums, bias, activation and residual are fp32 and an output is rounded once; Y comes from the unrounded Z.  fp32 tensors are
+ * multiplied at fp32 accuracy whatever the math mode says (as three bf16 planes; up to four rows by FMAs), 16-bit ones by
+ * tcgen05.mma with fp32 accumulators.  fp32 tensors have fewer than 2^31 elements.
+ *
+ * The gradients, from deltaY and the Z that the forward call kept:
+ *   deltaZ = deltaY * act'(Z)          (glu: [deltaY * U * act'(G) | deltaY * act(G)], Z = [G | U])
+ *   deltaX = deltaZ W,  deltaW = deltaZ^T X,  deltaB = column sums of deltaZ;  the residual's gradient is deltaY itself
+ * deltaX, deltaW and deltaB may each be NULL (not computed).  deltaZ is memory of the caller's, the size of Z, and may be Z
+ * itself; it holds deltaZ rounded to the tensors' type afterwards.  ALPHA_ACT_NONE without gates needs neither Z nor deltaZ.
+ * At 0 the slope of a LeakyReLU is k.  Results do not depend on scheduling (fixed summation orders, no atomics). */
+#define ALPHA_F32 0
+#define ALPHA_BF16 1
+#define ALPHA_F16 2
+#define ALPHA_ACT_NONE 0
+#define ALPHA_ACT_LEAKY_RELU 1 /* z > 0 ? z : k z; ReLU with k = 0 */
+#define ALPHA_ACT_SIGMOID 2
+#define ALPHA_ACT_SILU 3       /* z sigmoid(z) */
+#define ALPHA_ACT_GELU 4       /* z times the normal distribution function */
+#define ALPHA_ACT_GELU_TANH 5  /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+typedef struct AlphaFcShape {
+    int rows, IC, OC;
+    int dtype;   /* ALPHA_F32, ALPHA_BF16 or ALPHA_F16: every tensor of the call */
+    int act;     /* ALPHA_ACT_* */
+    float k;     /* slope of ALPHA_ACT_LEAKY_RELU */
+} AlphaFcShape;
+int alpha_fullConnect(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y,
+                      alpha_stream_t stream);
+int alpha_fullConnect_delta(const AlphaFcShape* s, const void* deltaY, const void* X, const void* W, const void* Z, void* deltaZ,
+                            void* deltaX, void* deltaW, void* deltaB, alpha_stream_t stream);
+int alpha_fullConnect_glu(const AlphaFcShape* s, const void* X, const void* W, const void* bias, void* Z, void* Y, alpha_stream_t stream);
+int alpha_fullConnect_glu_delta(const AlphaFcShape* s, const void* deltaY, const void* X, const void* W, const void* Z, void* deltaZ,
+                                void* deltaX, void* deltaW, void* deltaB, alpha_stream_t stream);
+/* Scratch of a call, as alpha_conv_workspace_bytes: op ALPHA_OP_FORWARD, or ALPHA_OP_DELTAX for the call of all gradients. */
+int alpha_fullConnect_workspace_bytes(const AlphaFcShape* s, int glu, int op, size_t* bytes);
+
+/* ---- all gradients of a step -----------------------------------------------------------------------------------
+ *
+ * norm = sqrt(sum of the squares of all elements of n tensors), summed in fp64 in a fixed order (neither overflow nor underflow
+ * of a square; the same bits on every run), written to *norm as a float on the device; NaN or Inf elements give a NaN or Inf.
+ * alpha_clip_grad_norm also scales every element by c = min(1, max_norm / (norm + 1e-6)) (a NaN norm: by NaN), c as a float:
+ * out = c * grad, where out may be grad itself.  A tensor given in place (out == grad) is not touched where c = 1.
+ * The tensors may be of different types and any size from 0 on, aligned to their elements; out may have another type (a
+ * 16-bit gradient for a fp32 optimizer).  An output must not overlap any other tensor of the call (ALPHA_E_ARG).
+ * n = 0 is a norm of 0.  Scratch: 48 bytes for each SM (or of the SM budget) and 128 tensors. */
+typedef struct AlphaGrad {
+    const void* grad;
+    void* out;           /* alpha_clip_grad_norm only */
+    int64_t count;       /* elements */
+    int dtype, out_dtype; /* ALPHA_F32, ALPHA_BF16 or ALPHA_F16 */
+} AlphaGrad;
+int alpha_grad_norm(int n, const AlphaGrad* grads, float* norm, alpha_stream_t stream);
+int alpha_clip_grad_norm(int n, const AlphaGrad* grads, float max_norm, float* norm, alpha_stream_t stream);
+
 /* ---- 2D pooling (the operators between the convolutions of a network) ---------------------------------------
  * Replace the kernels behind src/cu32_src/Cuda_pool2D/Cuda_pool2D/pool2D.cuh and
  * src/cu32_src/Cuda_upool2D/Cuda_upool2D/upool2D.cuh.  NHWC fp32, any channel count (16-byte accesses when
