@@ -84,30 +84,69 @@ struct Product {
     int act; float k;
 };
 
-enum { kTilePair = 1, kTile128 = 2, kTile64 = 3 };
+// What a product of 16-bit operands runs on: CTA pairs of 256 x 256 outputs, or CTAs of 128 x bn, `split` of which share a tile.
+struct FcPlan { bool pair; int bn, split; };
 
-template <class T, bool PAIR, int BN, bool GLU>
-void launch_mma(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& y, const CUtensorMap& z, const FcMma& p, int sms, cudaStream_t stream)
+uint32_t tmem_columns(int bn, bool glu)
 {
-    using G = FcTile<PAIR, BN>;
-    constexpr int CTAS = PAIR ? 2 : 1;
-    const int total = p.m_tiles * p.n_tiles, most = sms / CTAS;
-    allow_smem<fc_mma_kernel<T, PAIR, BN, GLU>>();
-    launch_after_clusters(fc_mma_kernel<T, PAIR, BN, GLU>, dim3((total < most ? total : most) * CTAS), kFcThreads, PAIR ? 2 : 0, G::kSmem, stream, a, b, y, z, p);
+    // two accumulators from multiples of 32 columns on, read by chunks of 32 (glu: from their half on too)
+    auto up = [](int n) { return (n + 31) & ~31; };
+    const int last = glu && bn / 2 + up(bn / 2) > up(bn) ? bn / 2 + up(bn / 2) : up(bn);
+    uint32_t c = 32;
+    while (c < static_cast<uint32_t>(up(bn) + last)) c <<= 1;
+    return c;
 }
 
-// Tile of a product: that whose waves take least, a wave of 128 x 64 tiles counted as 0.36 and one of 128 x 128 as 0.58 of one of pairs'.
-int pick_tile(const Product& q, int sms)
+// The plan of least estimated time, after 250 measured ones (512 x 4096 x 4096 in us: 64 columns 26, 112 21, 128 21, pairs 27; 64 x 4096 x 1024: 64
+// columns 13, shared by two 11.6, 32 shared by four 9.7).  64 steps of a tile take 0.1375 us (four MMAs of up
+// to 128 columns, 64 clocks each whatever they hold, as A is read from shared memory; wider tiles have two stages and are slower), of a pair's 0.285;
+// all tiles' operands come through L2 at 18 TB/s, W and X from DRAM at 5.2; a launch 4 us until its first tile and after its last (pairs 5.7),
+// and a shared tile its exchange, eight CTAs also the wait for a place for them.
+FcPlan pick_plan(const Product& q, int sms)
 {
-    const int forced = option_fc_tile();
-    if (forced) return forced == kTilePair && sms < 2 ? kTile128 : forced;
-    const int cols = q.glu ? 2 * q.cols : q.cols;
-    auto waves = [&](int bm, int bn, int ctas) {
-        const long long tiles = (long long)((q.rows + bm - 1) / bm) * ((cols + bn - 1) / bn), most = sms / ctas;
-        return (double)((tiles + most - 1) / most);
+    const int forced = option_fc_tile() == 2 ? 0 : option_fc_tile();
+    const long long cols = q.glu ? 2LL * q.cols : q.cols, blocks = (q.K + kFcBK - 1) / kFcBK, stages = (blocks + 1) / 2;
+    FcPlan best{false, 64, 1};
+    double least = 1e300;
+    auto look = [&](bool pair, int bn, int split) {
+        const int out = q.glu ? bn / 2 : bn, bm = pair ? 256 : 128, ctas = pair ? 2 : 1;
+        const long long tiles = (long long)((q.rows + bm - 1) / bm) * ((q.cols + out - 1) / out), most = sms / (ctas * split);
+        if (most < 1 || (split > 1 && tiles > most)) return;
+        const long long waves = (tiles + most - 1) / most, each = (blocks + split - 1) / split;
+        const double step = pair ? 0.285 : 0.1375;
+        const double l2 = (double)tiles * blocks * (pair ? 512 : (q.a_mn || q.rows >= 128 ? 128 : q.rows) + bn) * 128 / 18e6;
+        const double mma = waves * each * step, dram = 2e-6 * ((double)q.rows + cols) * q.K / 5.2;
+        const double most_of = mma > l2 ? (mma > dram ? mma : dram) : (l2 > dram ? l2 : dram);
+        double time = 0.8 * most_of + 0.2 * (mma + l2 + dram);                // (the others are not quite hidden)
+        time += (pair ? 5.7 : 4.0 + 0.006 * bn) + (split == 1 ? 0.0 : split == 2 ? 2.5 : split == 4 ? 4.0 : 12.0);
+        if (time < least) { least = time; best = FcPlan{pair, bn, split}; }
     };
-    const double pair = sms >= 2 ? waves(256, 256, 2) : 1e30, single = 0.58 * waves(128, 128, 1), narrow = 0.36 * waves(128, 64, 1);
-    return pair <= single && pair <= narrow ? kTilePair : single <= narrow ? kTile128 : kTile64;
+    // (an operand that runs along its rows comes in boxes of 64 of them; no part of a shared tile is empty)
+    const int unit = q.b_mn ? 64 : 16;
+    auto parts = [&](int split) { return split == 1 || (split - 1) * ((stages + split - 1) / split) < stages; };
+    if (forced == 1 && sms >= 2) return FcPlan{true, 256, 1};
+    if (forced >= 1000) {
+        const int bn = forced % 1000 / unit * unit;
+        for (int split = forced / 1000; split > 1 && bn >= unit && bn <= 256; split /= 2)
+            if (split <= 8 && parts(split)) look(false, bn, split);
+        if (least == 1e300 && bn >= unit && bn <= 256) look(false, bn, 1);
+        return best;
+    }
+    look(true, 256, 1);
+    for (int bn = unit; bn <= 128; bn += unit)
+        for (int split = 1; split <= 8; split *= 2)
+            if (parts(split)) look(false, bn, split);
+    return best;
+}
+
+template <class T, bool PAIR, bool GLU>
+void launch_mma(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& y, const CUtensorMap& z, const FcMma& p, int sms, cudaStream_t stream)
+{
+    const int group = PAIR ? 2 : p.split, total = p.m_tiles * p.n_tiles, most = sms / group;
+    const unsigned grid = static_cast<unsigned>(p.split > 1 || total < most ? total : most) * group;
+    const uint32_t smem = p.stages * fc_blocks(PAIR) * fc_block_bytes(PAIR, p.a_rows, p.bn) + kFcStaging + 1024 + 512;
+    allow_smem<fc_mma_kernel<T, PAIR, GLU>>();
+    launch_after_clusters(fc_mma_kernel<T, PAIR, GLU>, dim3(grid), kFcThreads, group > 1 ? group : 0, smem, stream, a, b, y, z, p);
 }
 
 int launch_product(const Product& q, cudaStream_t stream)
@@ -116,42 +155,43 @@ int launch_product(const Product& q, cudaStream_t stream)
     int rc = device_sms(&sms);
     if (!rc) rc = device_status_word(&status);
     if (rc) return rc;
-    const int tile = pick_tile(q, sms), bm = tile == kTilePair ? 256 : 128, bn = tile == kTilePair ? 256 : tile == kTile128 ? 128 : 64;
-    const int out = q.glu ? bn / 2 : bn, br = tile == kTilePair ? 128 : bn;
+    const FcPlan plan = pick_plan(q, sms);
+    const int bm = plan.pair ? 256 : 128, bn = plan.bn, out = q.glu ? bn / 2 : bn, steps = kFcBK * fc_blocks(plan.pair);
     FcMma p{};
-    p.rows = q.rows; p.cols = q.cols; p.K = q.K;
-    p.m_tiles = (q.rows + bm - 1) / bm; p.n_tiles = (q.cols + out - 1) / out; p.kb = (q.K + kFcBK - 1) / kFcBK;
+    p.rows = q.rows; p.cols = q.cols;
+    p.m_tiles = (q.rows + bm - 1) / bm; p.n_tiles = (q.cols + out - 1) / out; p.kb = (q.K + steps - 1) / steps;
     if ((long long)p.m_tiles * p.n_tiles > 2147483647LL / kFcGroupM) return fail(ALPHA_E_ARG, "fullConnect: more tiles than a launch takes");
+    p.bn = bn; p.split = plan.split;
     p.a_mn = q.a_mn; p.b_mn = q.b_mn;
-    p.a_rows = q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
+    p.a_rows = plan.pair || q.a_mn || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
+    const uint32_t stage = fc_blocks(plan.pair) * fc_block_bytes(plan.pair, p.a_rows, bn);
+    p.stages = kFcRing / stage < kFcMaxStages ? kFcRing / stage : kFcMaxStages;
+    // shared tiles: the ring holds a part's sums afterwards
+    const uint32_t sums = (q.rows < 128 ? q.rows : 128) * (bn + 4) * 4;
+    while (p.split > 1 && p.stages * stage < sums && (p.stages + 1) * stage <= kFcRing) ++p.stages;
+    if (p.split > 1 && p.stages * stage < sums) return fail(ALPHA_E_ARG, "fullConnect: no plan");
     p.b_up = q.cols;
     p.idesc = q.dtype == ALPHA_BF16 ? make_idesc_bf16(bm, bn, q.a_mn, q.b_mn) : make_idesc_f16(bm, bn, q.a_mn, q.b_mn);
+    p.tmem = tmem_columns(bn, q.glu);
     p.act = q.act; p.k = q.k; p.keep_z = q.Z != nullptr;
-    p.bias = q.bias; p.residual = q.residual; p.status = status;
+    p.bias = q.bias; p.residual = q.residual; p.Y = q.Y; p.Z = q.Z; p.status = status;
     CUtensorMap a, b, y, z;
     const long long b_rows = q.glu ? 2LL * q.cols : q.cols;
     rc = q.a_mn ? make_map(&a, q.dtype, q.A, q.rows, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) : make_map(&a, q.dtype, q.A, q.K, q.rows, 64, p.a_rows, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = q.b_mn ? make_map(&b, q.dtype, q.B, q.cols, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
-                         : make_map(&b, q.dtype, q.B, q.K, b_rows, 64, q.glu && tile != kTilePair ? bn / 2 : br, CU_TENSOR_MAP_SWIZZLE_128B);
+                         : make_map(&b, q.dtype, q.B, q.K, b_rows, 64, plan.pair ? 128 : out, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = make_out_map(&y, q.dtype, q.Y, q.cols, 1, q.rows);
     if (!rc) rc = q.Z ? make_out_map(&z, q.dtype, q.Z, q.cols, q.glu ? 2 : 1, q.rows) : (z = y, ALPHA_OK);
     if (rc) return rc;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (q.glu) {
-            if (tile == kTilePair) launch_mma<T, true, 256, true>(a, b, y, z, p, sms, stream);
-            else if (tile == kTile128) launch_mma<T, false, 128, true>(a, b, y, z, p, sms, stream);
-            else launch_mma<T, false, 64, true>(a, b, y, z, p, sms, stream);
-        } else {
-            if (tile == kTilePair) launch_mma<T, true, 256, false>(a, b, y, z, p, sms, stream);
-            else if (tile == kTile128) launch_mma<T, false, 128, false>(a, b, y, z, p, sms, stream);
-            else launch_mma<T, false, 64, false>(a, b, y, z, p, sms, stream);
-        }
+        if (q.glu) plan.pair ? launch_mma<T, true, true>(a, b, y, z, p, sms, stream) : launch_mma<T, false, true>(a, b, y, z, p, sms, stream);
+        else plan.pair ? launch_mma<T, true, false>(a, b, y, z, p, sms, stream) : launch_mma<T, false, false>(a, b, y, z, p, sms, stream);
     };
     if (q.dtype == ALPHA_BF16) go(__nv_bfloat16{});
     else go(__half{});
     note_launch("fc");
-    note_plan("fc %s%dx%d", tile == kTilePair ? "pair " : "", bm, bn);
+    note_plan("fc %s%dx%d split=%d", plan.pair ? "pair " : "", bm, bn, plan.split);
     return launched("fc_mma_kernel");
 }
 
@@ -192,39 +232,64 @@ int launch_f32(const float* A, const float* B, int rows, int cols, int K, int ld
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
 
-constexpr int kSmallRows = 4;
+constexpr int kSmallRows = 4, kTokenRows = 16;   // fp32, 16-bit
 
-template <class T, bool GLU>
+template <bool GLU>
 int launch_small(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, cudaStream_t stream)
 {
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    FcSmall p{s->rows, s->IC, s->OC, 1, s->act, s->k, X, W, bias, residual, Z, Y};
-    const int units = GLU ? s->OC : (s->OC + 1) / 2, words = s->IC / Word16<T>::N;
+    FcSmall p{s->rows, s->IC, s->OC, 1, 1, s->act, s->k, X, W, bias, residual, Z, Y};
+    const int units = GLU ? s->OC : (s->OC + 1) / 2, words = s->IC / 4;
     // 16 warps an SM, each with 64 words of a row at least
     while (p.ks < 8 && static_cast<long long>(units) * p.ks < 16LL * sms && words >= 128 * p.ks) p.ks *= 2;
     const int teams = 8 / p.ks;
     const unsigned blocks = (units + teams - 1) / teams;
-    if (s->rows == 1) launch_after(fc_small_kernel<T, 1, GLU>, blocks, 256, 0, stream, p);
-    else if (s->rows == 2) launch_after(fc_small_kernel<T, 2, GLU>, blocks, 256, 0, stream, p);
-    else launch_after(fc_small_kernel<T, 4, GLU>, blocks, 256, 0, stream, p);
+    if (s->rows == 1) launch_after(fc_small_kernel<float, 1, GLU>, blocks, 256, 0, stream, p);
+    else if (s->rows == 2) launch_after(fc_small_kernel<float, 2, GLU>, blocks, 256, 0, stream, p);
+    else launch_after(fc_small_kernel<float, 4, GLU>, blocks, 256, 0, stream, p);
     note_launch("fc_small");
     note_plan("fc small ks=%d", p.ks);
     return launched("fc_small_kernel");
+}
+template <class T, bool GLU>
+int launch_token(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, cudaStream_t stream)
+{
+    int sms = 0;
+    const int rc = device_sms(&sms);
+    if (rc) return rc;
+    FcSmall p{s->rows, s->IC, s->OC, 1, 1, s->act, s->k, X, W, bias, residual, Z, Y};
+    // up to eight warps a row group, each with 4 blocks of 32 steps at least
+    while (p.ks < 8 && s->IC >= 256 * p.ks) p.ks *= 2;
+    const int teams = 8 / p.ks, groups = (s->OC + 15) / 16;
+    const long long blocks = (groups + teams - 1) / teams;
+    // row groups that leave SMs to fill are shared, as long as a warp keeps its 32-byte loads of eight rows in flight
+    const int pass = 64 * 8 * 4;
+    while (p.split < 8 && p.ks == 8 && blocks * p.split * 2 <= 4LL * sms && s->IC >= pass * p.split * 2) p.split *= 2;
+    if (blocks * p.split > 2147483647LL) p.split = 1;
+    const dim3 grid(static_cast<unsigned>(blocks * p.split));
+    const unsigned cluster = p.split > 1 ? p.split : 0;
+    if (s->rows <= 8) launch_after_clusters(fc_token_kernel<T, 1, GLU>, grid, 256, cluster, 0, stream, p);
+    else launch_after_clusters(fc_token_kernel<T, 2, GLU>, grid, 256, cluster, 0, stream, p);
+    note_launch("fc_small");
+    note_plan("fc token ks=%d split=%d", p.ks, p.split);
+    return launched("fc_token_kernel");
 }
 
 int forward(const char* what, const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, bool glu, cudaStream_t stream)
 {
     int rc = call_begin(stream);
     if (rc) return rc;
-    if (s->rows <= kSmallRows && !option_fc_tile()) {
+    // (of the gated block from nine rows on only where W is small: 2 x 11008 x 4096 on 16 rows 39 us, by tiles 37)
+    const bool token = s->rows <= 8 || (s->rows <= kTokenRows && (!glu || (long long)s->OC * s->IC <= 8 << 20));
+    if ((s->dtype == ALPHA_F32 ? s->rows <= kSmallRows : token) && !option_fc_tile()) {
         if (dry_run()) return ALPHA_OK;
         switch (s->dtype) {
-        case ALPHA_F32: return glu ? launch_small<float, true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<float, false>(s, X, W, bias, residual, Z, Y, stream);
+        case ALPHA_F32: return glu ? launch_small<true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<false>(s, X, W, bias, residual, Z, Y, stream);
         case ALPHA_BF16:
-            return glu ? launch_small<__nv_bfloat16, true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<__nv_bfloat16, false>(s, X, W, bias, residual, Z, Y, stream);
-        default: return glu ? launch_small<__half, true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<__half, false>(s, X, W, bias, residual, Z, Y, stream);
+            return glu ? launch_token<__nv_bfloat16, true>(s, X, W, bias, residual, Z, Y, stream) : launch_token<__nv_bfloat16, false>(s, X, W, bias, residual, Z, Y, stream);
+        default: return glu ? launch_token<__half, true>(s, X, W, bias, residual, Z, Y, stream) : launch_token<__half, false>(s, X, W, bias, residual, Z, Y, stream);
         }
     }
     if (s->dtype == ALPHA_F32) {

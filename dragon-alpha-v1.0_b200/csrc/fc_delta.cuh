@@ -39,40 +39,56 @@ __global__ void __launch_bounds__(256) fc_delta_kernel(const __grid_constant__ F
     if (word < words) {
         with_act(p.act, [&](auto a) {
             constexpr int ACT = decltype(a)::value;
-#pragma unroll 2
-            for (long long r = blockIdx.y * 8 + warp; r < p.rows; r += gridDim.y * 8) {
-                const size_t at = static_cast<size_t>(r) * words + word, zt = GLU ? at + static_cast<size_t>(r) * words : at;
-                float d[N];
-                V::load(__ldg(dY + at), d);
-                if constexpr (GLU) {
-                    float g[N], u[N];
-                    V::load(Z[zt], g);
-                    V::load(Z[zt + words], u);
+            // kRows rows in flight: their loads leave before the first is used
+            constexpr int kRows = GLU ? 2 : 4;
+            const long long stride = gridDim.y * 8;
+            for (long long r0 = blockIdx.y * 8 + warp; r0 < p.rows; r0 += kRows * stride) {
+                uint4 wd[kRows], wg[kRows], wu[kRows];
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        float value, slope;
-                        act_both<ACT, V::kFast>(g[i], p.k, value, slope);
-                        g[i] = d[i] * u[i] * slope;
-                        u[i] = d[i] * value;
-                        acc[0][i] += g[i];
-                        acc[1][i] += u[i];
-                    }
-                    dZ[zt] = V::store(g);
-                    dZ[zt + words] = V::store(u);
-                } else {
-                    if constexpr (ACT != ALPHA_ACT_NONE) {
-                        float z[N];
-                        V::load(Z[zt], z);
+                for (int q = 0; q < kRows; ++q) {
+                    const long long r = r0 + q * stride < p.rows ? r0 + q * stride : r0;
+                    const size_t at = static_cast<size_t>(r) * words + word, zt = GLU ? at + static_cast<size_t>(r) * words : at;
+                    wd[q] = __ldg(dY + at);
+                    if constexpr (GLU || ACT != ALPHA_ACT_NONE) wg[q] = Z[zt];
+                    if constexpr (GLU) wu[q] = Z[zt + words];
+                }
+#pragma unroll
+                for (int q = 0; q < kRows; ++q) {
+                    const long long r = r0 + q * stride;
+                    if (r >= p.rows) break;
+                    const size_t at = static_cast<size_t>(r) * words + word, zt = GLU ? at + static_cast<size_t>(r) * words : at;
+                    float d[N];
+                    V::load(wd[q], d);
+                    if constexpr (GLU) {
+                        float g[N], u[N];
+                        V::load(wg[q], g);
+                        V::load(wu[q], u);
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
                             float value, slope;
-                            act_both<ACT, V::kFast>(z[i], p.k, value, slope);
-                            d[i] *= slope;
+                            act_both<ACT, V::kFast>(g[i], p.k, value, slope);
+                            g[i] = d[i] * u[i] * slope;
+                            u[i] = d[i] * value;
+                            acc[0][i] += g[i];
+                            acc[1][i] += u[i];
                         }
-                        dZ[zt] = V::store(d);
-                    }
+                        dZ[zt] = V::store(g);
+                        dZ[zt + words] = V::store(u);
+                    } else {
+                        if constexpr (ACT != ALPHA_ACT_NONE) {
+                            float z[N];
+                            V::load(wg[q], z);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) acc[0][i] += d[i];
+                            for (int i = 0; i < N; ++i) {
+                                float value, slope;
+                                act_both<ACT, V::kFast>(z[i], p.k, value, slope);
+                                d[i] *= slope;
+                            }
+                            dZ[zt] = V::store(d);
+                        }
+#pragma unroll
+                        for (int i = 0; i < N; ++i) acc[0][i] += d[i];
+                    }
                 }
             }
         });

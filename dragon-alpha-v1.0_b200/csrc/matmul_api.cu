@@ -69,6 +69,39 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ P
     }
 }
 
+// The same for up to eight tensors of 2- or 4-byte elements; a thread per 16-byte destination word.
+struct PadWordsJob {
+    const void* src;
+    uint4* dst;
+    unsigned rows, cols, first;   // first: word of the launch that is this job's first
+    FastDiv by_words;
+};
+struct PadWordsJobs { PadWordsJob job[8]; int n; };
+template <class E>
+__global__ void __launch_bounds__(256) pad_words_kernel(const __grid_constant__ PadWordsJobs p, unsigned all)
+{
+    constexpr unsigned N = 16 / sizeof(E);
+    grid_dependency_wait();
+    grid_dependency_trigger();
+    for (unsigned w = blockIdx.x * blockDim.x + threadIdx.x; w < all; w += gridDim.x * blockDim.x) {
+        int q = 0;
+        while (q + 1 < p.n && w >= p.job[q + 1].first) ++q;
+        const PadWordsJob& j = p.job[q];
+        unsigned r, x;
+        j.by_words.divmod(w - j.first, r, x);
+        const unsigned c = x * N;
+        union { E e[N]; uint4 v; } word;
+        word.v = make_uint4(0, 0, 0, 0);
+        if (r < j.rows && c < j.cols) {
+            const E* s = static_cast<const E*>(j.src) + static_cast<size_t>(r) * j.cols + c;
+#pragma unroll
+            for (unsigned i = 0; i < N; ++i)
+                if (c + i < j.cols) word.e[i] = __ldg(s + i);
+        }
+        j.dst[w - j.first] = word.v;
+    }
+}
+
 // `rows` matrix rows as the pixels of a 1x1 convolution: images of 1 x 4 pixels when the row count
 // allows it (the engine pads every dimension to a multiple of 4), single pixels otherwise.  The
 // kernels flatten 1x1 problems over all pixels anyway; the image shape only matters to their fallbacks.
@@ -293,6 +326,50 @@ int alpha_pad_rows_many(int n, const long long* jobs, alpha_stream_t stream)
         }
     }
     if (!rc && held) rc = launch_pad_rows(p, all, sms, static_cast<cudaStream_t>(stream));
+    return rc;
+}
+
+int alpha_pad_rows_typed(int n, const long long* jobs, int dtype, alpha_stream_t stream)
+{
+    if (n <= 0 || !jobs) return fail(ALPHA_E_ARG, "pad_rows: no jobs");
+    if (dtype != ALPHA_F32 && dtype != ALPHA_BF16 && dtype != ALPHA_F16) return fail(ALPHA_E_ARG, "pad_rows: unknown element type %d", dtype);
+    const long long size = dtype == ALPHA_F32 ? 4 : 2, per = 16 / size;
+    for (int i = 0; i < n; ++i) {
+        const long long *q = jobs + 6 * i, rows = q[1], cols = q[2], rows4 = q[4], cols4 = q[5];
+        if (!q[0] || !q[3]) return fail(ALPHA_E_ARG, "pad_rows: null pointer");
+        if (rows <= 0 || cols <= 0 || rows4 < rows || cols4 < cols || cols4 % per != 0 || cols4 > 2147483640LL)
+            return fail(ALPHA_E_ARG, "pad_rows: bad shape (%lld x %lld into %lld x %lld)", rows, cols, rows4, cols4);
+        if ((q[3] & 15) || (q[0] & (size - 1))) return fail(ALPHA_E_ARG, "pad_rows: the destination must be 16-byte aligned, the source to its elements");
+    }
+    int sms = 0;
+    int rc = device_sms(&sms);
+    PadWordsJobs p{};
+    long long all = 0;
+    auto launch = [&] {
+        const long long want = (all + 255) / 256;
+        const unsigned blocks = static_cast<unsigned>(want < sms * 16LL ? want : sms * 16LL);
+        if (size == 4) launch_after(pad_words_kernel<unsigned>, blocks, 256, 0, static_cast<cudaStream_t>(stream), p, static_cast<unsigned>(all));
+        else launch_after(pad_words_kernel<unsigned short>, blocks, 256, 0, static_cast<cudaStream_t>(stream), p, static_cast<unsigned>(all));
+        note_launch("pad_rows");
+        p.n = 0;
+        all = 0;
+        const cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? ALPHA_OK : fail(ALPHA_E_CUDA, "pad_words_kernel launch failed: %s", cudaGetErrorString(e));
+    };
+    for (int i = 0; i < n && !rc; ++i) {
+        const long long *q = jobs + 6 * i, rows = q[1], cols = q[2], rows4 = q[4], words = q[5] / per, most = kPadMost / words;
+        const char* src = reinterpret_cast<const char*>(static_cast<uintptr_t>(q[0]));
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uintptr_t>(q[3]));
+        for (long long r0 = 0; r0 < rows4 && !rc; r0 += most) {
+            const long long m = rows4 - r0 < most ? rows4 - r0 : most, have = rows - r0 < 0 ? 0 : (rows - r0 < m ? rows - r0 : m);
+            if (p.n == 8 || all + m * words > kPadMost) rc = launch();
+            if (rc) break;
+            p.job[p.n++] = PadWordsJob{src + r0 * cols * size, dst + r0 * words, static_cast<unsigned>(have), static_cast<unsigned>(cols), static_cast<unsigned>(all),
+                                       fast_div(static_cast<int>(words))};
+            all += m * words;
+        }
+    }
+    if (!rc && p.n) rc = launch();
     return rc;
 }
 

@@ -182,6 +182,19 @@ __device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// A float in any CTA's shared memory, by its cluster address.
+__device__ __forceinline__ float ld_shared_cluster(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void cluster_sync_all()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -207,6 +220,16 @@ __device__ __forceinline__ bool mbar_try_wait_cluster_a(uint32_t bar, uint32_t p
         : "memory");
     return ok != 0;
 }
+// Whether a phase has completed, without waiting for it (try_wait may suspend the thread for microseconds).
+template <bool CLUSTER> __device__ __forceinline__ bool mbar_test_a(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    if constexpr (CLUSTER)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 static __device__ __noinline__ bool mbar_wait_cluster_a(uint32_t bar, uint32_t parity)
 {
     if (mbar_try_wait_cluster_a(bar, parity)) return true;
@@ -223,6 +246,11 @@ static __device__ __noinline__ bool mbar_wait_cluster_a(uint32_t bar, uint32_t p
 __device__ __forceinline__ void mma_commit_pair(uint32_t cluster_bar)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_bar) : "memory");
+}
+// The same on both CTAs' barriers at once; `bar` is the address in either.
+__device__ __forceinline__ void mma_commit_both(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 // D[tmem] (+)= A * B over a CTA pair (M = 256: 128 rows per CTA; each CTA holds N / 2 rows of B).
 __device__ __forceinline__ void mma_tf32_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
@@ -574,33 +602,37 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn_ma
 {
     return make_idesc_bf16(M, N, a_mn_major, b_mn_major) & ~(1u << 7 | 1u << 10);
 }
-// D[tmem] (+)= A * B for 16-bit operands, over one CTA or (PAIR) a CTA pair; one thread issues.
+// D[tmem] (+)= A * B for 16-bit operands, over one CTA or (PAIR) a CTA pair.  Executed by a converged warp, issued by the lane whose `elected`
+// is set: operands that are the same in all lanes stay in uniform registers (issued by one lane of a divergent warp, an instruction took 140 clocks
+// whatever its shape).
 template <bool PAIR>
-__device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate)
+__device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate, uint32_t elected)
 {
     if constexpr (PAIR)
         asm volatile(
             "{\n\t"
-            ".reg .pred p;\n\t"
+            ".reg .pred p, q;\n\t"
             ".reg .b64 da, db;\n\t"
             "mov.b64 da, {%1, %2};\n\t"
             "mov.b64 db, {%3, %4};\n\t"
             "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, {%7, %7, %7, %7, %7, %7, %7, %7}, p;\n\t"
+            "setp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t"
             "}\n" ::"r"(d_tmem),
-            "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
+            "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(elected)
             : "memory");
     else
         asm volatile(
             "{\n\t"
-            ".reg .pred p;\n\t"
+            ".reg .pred p, q;\n\t"
             ".reg .b64 da, db;\n\t"
             "mov.b64 da, {%1, %2};\n\t"
             "mov.b64 db, {%3, %4};\n\t"
             "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
+            "setp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
             "}\n" ::"r"(d_tmem),
-            "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+            "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(elected)
             : "memory");
 }
 // Executed by a converged warp, issued by the lane whose `elected` is set; descriptors as (lo, hi) halves with offsets (16-byte units).

@@ -291,13 +291,13 @@ class CudaFloat32EngineBase:
     def fullConnect(self, Y_address, X_address, W_address, rows, IC, OC, dtype, act, k, Bias_address=None, Residual_address=None, Z_address=None):
         """Y = act(X W^T + Bias) + Residual, Z = X W^T + Bias; addresses of X[rows, IC], W[OC, IC], and so on (alpha_fullConnect)."""
         a = self._addr_or_none
-        _l.check(self._lib.alpha_fullConnect(C.byref(_l.AlphaFcShape(rows, IC, OC, dtype, act, k)), a(X_address), a(W_address), a(Bias_address), a(Residual_address),
+        _l.check(self._lib.alpha_fullConnect(C.byref(_cached_fc_shape(rows, IC, OC, dtype, act, float(k))), a(X_address), a(W_address), a(Bias_address), a(Residual_address),
                                              a(Z_address), a(Y_address), _stream(self._stream)))
 
     def fullConnect_glu(self, Y_address, X_address, W_address, rows, IC, OC, dtype, act, k, Bias_address=None, Z_address=None):
         """Y = act(Z[:, :OC]) * Z[:, OC:], Z = X W^T + Bias with W[2 OC, IC] (alpha_fullConnect_glu)."""
         a = self._addr_or_none
-        _l.check(self._lib.alpha_fullConnect_glu(C.byref(_l.AlphaFcShape(rows, IC, OC, dtype, act, k)), a(X_address), a(W_address), a(Bias_address), a(Z_address),
+        _l.check(self._lib.alpha_fullConnect_glu(C.byref(_cached_fc_shape(rows, IC, OC, dtype, act, float(k))), a(X_address), a(W_address), a(Bias_address), a(Z_address),
                                                  a(Y_address), _stream(self._stream)))
 
     def fullConnect_delta(self, deltaX_address, deltaW_address, deltaB_address, deltaY_address, X_address, W_address, Z_address, deltaZ_address, rows, IC, OC,
@@ -305,7 +305,7 @@ class CudaFloat32EngineBase:
         """The gradients of fullConnect, or of fullConnect_glu (alpha_fullConnect_delta, alpha_fullConnect_glu_delta)."""
         a = self._addr_or_none
         fn = self._lib.alpha_fullConnect_glu_delta if glu else self._lib.alpha_fullConnect_delta
-        _l.check(fn(C.byref(_l.AlphaFcShape(rows, IC, OC, dtype, act, k)), a(deltaY_address), a(X_address), a(W_address), a(Z_address), a(deltaZ_address),
+        _l.check(fn(C.byref(_cached_fc_shape(rows, IC, OC, dtype, act, float(k))), a(deltaY_address), a(X_address), a(W_address), a(Z_address), a(deltaZ_address),
                     a(deltaX_address), a(deltaW_address), a(deltaB_address), _stream(self._stream)))
 
     # ---- pooling, Java argument order (CudaFloat32EngineBase.java:2012-2215) ----
@@ -378,23 +378,80 @@ def _pad_both(t, n4, c4):
 
 
 _FC_TYPES = {torch.float32: _l.ALPHA_F32, torch.bfloat16: _l.ALPHA_BF16, torch.float16: _l.ALPHA_F16}
+_cached_fc_shape = functools.lru_cache(maxsize=512)(_l.AlphaFcShape)
 
 
-def _fc_padded(t, n):
-    """t, dense, on a 16-byte boundary and with its last dimension zero-padded to n."""
-    if t.shape[-1] != n:
-        return _pad_both(t, t.shape[0], n)
-    t = t.contiguous()
-    if t.is_neg() or t.data_ptr() % 16:
-        return t.clone(memory_format=torch.contiguous_format).resolve_neg()
-    return t
+def _fc_pack(dtype, *jobs):
+    """The operands of one call, (t, groups, rows, cols, rows4, cols4) each: t holds `groups` matrices of rows x cols, wanted dense, on a 16-byte
+    boundary and zero-padded to rows4 x cols4.  Those that need padding are written by one launch into one block of memory.  Returns tensors (None for
+    None), or addresses inside the block, and the block (to be held until the call has been enqueued)."""
+    out, plan, size = [], [], 0
+    for job in jobs:
+        t = job[0]
+        if t is None:
+            out.append(None)
+            continue
+        if not t.is_contiguous():
+            t = t.contiguous()
+        if t.is_neg():                      # (a lazily negated view: its memory is not its value)
+            t = t.resolve_neg()
+        _, groups, rows, cols, rows4, cols4 = job
+        if cols != cols4 or rows != rows4:
+            plan.append((len(out), t, groups, rows, cols, rows4, cols4, size))
+            size += (groups * rows4 * cols4 + 127) // 128 * 128     # (each starts on 256 bytes, like a tensor of its own)
+        elif t.data_ptr() % 16:
+            t = t.clone()
+        out.append(t)
+    if not plan:
+        return out, None
+    block = plan[0][1].new_empty(size)
+    base, each, values = block.data_ptr(), block.element_size(), []
+    for i, t, groups, rows, cols, rows4, cols4, at in plan:
+        out[i], src = base + at * each, t.data_ptr()
+        for g in range(groups):
+            values += (src + g * rows * cols * each, rows, cols, out[i] + g * rows4 * cols4 * each, rows4, cols4)
+    _l.check(_l.load().alpha_pad_rows_typed(len(values) // 6, struct.pack("%dq" % len(values), *values), _FC_TYPES[dtype], _stream()))
+    return out, (block, [job[1] for job in plan])
 
 
-def _fc_halves(t, oc, n):
-    """t, whose last dimension is two halves of oc, with each half zero-padded to n."""
-    if oc == n:
-        return _fc_padded(t, 2 * n)
-    return _fc_padded(t.reshape(-1, oc), n).reshape(t.shape[:-1] + (2 * n,))
+@functools.lru_cache(maxsize=512)
+def _fc_plan(what, glu, xs, ws, dtype):
+    """Sizes of a FullConnect call on X of shape xs and W of shape ws: IC, OC, padded IC and OC, rows, halves of W, shapes of Y and Z."""
+    if dtype not in _FC_TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, dtype))
+    if len(xs) < 1 or len(ws) != 2 or ws[1] != xs[-1]:
+        raise ValueError("%s: X %s against W %s" % (what, tuple(xs), tuple(ws)))
+    if glu and ws[0] % 2:
+        raise ValueError("%s: W has %d rows, which are not gate rows and as many up rows" % (what, ws[0]))
+    IC, halves = xs[-1], 2 if glu else 1
+    OC, lead = ws[0] // halves, tuple(xs[:-1])
+    if IC == 0 or OC == 0:
+        raise ValueError("%s: X %s against W %s" % (what, tuple(xs), tuple(ws)))
+    rows, unit = 1, 4 if dtype == torch.float32 else 8
+    for n in lead:
+        rows *= n
+    return IC, OC, -(-IC // unit) * unit, -(-OC // unit) * unit, rows, halves, lead + (OC,), lead + (halves * OC,)
+
+
+def _fc_check(what, X, W, others):
+    """The tensors of a call are of X's type and on its GPU, and of the shapes expected: (name, tensor or None, shape) each."""
+    dtype, device = X.dtype, X.get_device()
+    if device < 0:
+        raise ValueError("%s: tensors must be on a GPU" % what)
+    for name, t, shape in (("W", W, None),) + others:
+        if t is None:
+            continue
+        if shape is not None and t.shape != shape:
+            raise ValueError("%s: %s %s, expected %s" % (what, name, tuple(t.shape), shape))
+        if t.dtype != dtype or t.get_device() != device:
+            raise ValueError("%s: %s is %s on %s, X %s on %s" % (what, name, t.dtype, t.device, dtype, X.device))
+
+
+def _fc_act(what, act):
+    code = _l.ACTS.get(act)
+    if code is None:
+        raise ValueError("%s: act must be one of %s, not %r" % (what, ", ".join(sorted(_l.ACTS)), act))
+    return code
 
 
 _pack_jobs = {n: struct.Struct("%dq" % (6 * n)).pack for n in (1, 2, 3)}
@@ -575,91 +632,52 @@ class Engine:
     # ---- FullConnect layers of a transformer: the product with bias, activation and residual in its epilogue, the gated block, their
     # gradients.  float32, bfloat16 or float16 tensors (all of one type); X may have any leading dimensions; IC and OC that are no
     # multiples of 16 bytes are zero-padded as everywhere. ----
-    @staticmethod
-    def _fc_check(what, X, W, glu, act, **others):
-        if X.dtype not in _FC_TYPES:
-            raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, X.dtype))
-        if act not in _l.ACTS:
-            raise ValueError("%s: act must be one of %s, not %r" % (what, ", ".join(sorted(_l.ACTS)), act))
-        if X.dim() < 1 or W.dim() != 2 or W.shape[1] != X.shape[-1]:
-            raise ValueError("%s: X %s against W %s" % (what, tuple(X.shape), tuple(W.shape)))
-        if glu and W.shape[0] % 2:
-            raise ValueError("%s: W has %d rows, which are not gate rows and as many up rows" % (what, W.shape[0]))
-        IC, wide = X.shape[-1], W.shape[0]
-        OC = wide // 2 if glu else wide
-        if IC == 0 or OC == 0:
-            raise ValueError("%s: X %s against W %s" % (what, tuple(X.shape), tuple(W.shape)))
-        lead = tuple(X.shape[:-1])
-        shapes = {"Bias": (wide,), "Residual": lead + (OC,), "deltaY": lead + (OC,), "Z": lead + (wide,)}
-        for name, t in dict(others, W=W).items():
-            if t is None:
-                continue
-            if name != "W" and tuple(t.shape) != shapes[name]:
-                raise ValueError("%s: %s %s, expected %s" % (what, name, tuple(t.shape), shapes[name]))
-            if t.dtype != X.dtype or t.device != X.device:
-                raise ValueError("%s: %s is %s on %s, X %s on %s" % (what, name, t.dtype, t.device, X.dtype, X.device))
-        if not X.is_cuda:
-            raise ValueError("%s: tensors must be on a GPU" % what)
-        unit = 4 if X.dtype == torch.float32 else 8
-        return IC, OC, lead, -(-IC // unit) * unit, -(-OC // unit) * unit
-
     def _fc_forward(self, what, X, W, Bias, act, k, Residual, save, glu):
-        IC, OC, lead, ic, oc = self._fc_check(what, X, W, glu, act, Bias=Bias, Residual=Residual)
-        halves = 2 if glu else 1
-        rows = X.numel() // IC
+        dtype = X.dtype
+        IC, OC, ic, oc, rows, halves, ys, zs = _fc_plan(what, glu, X.shape, W.shape, dtype)
+        code = _fc_act(what, act)
+        _fc_check(what, X, W, (("Bias", Bias, (halves * OC,)), ("Residual", Residual, ys)))
         with self._on(X):
             if rows == 0:
-                Y = X.new_empty(lead + (OC,))
-                return (Y, X.new_empty(lead + (halves * OC,))) if save else Y
-            Xp = _fc_padded(X.reshape(rows, IC), ic)
-            Wp = _fc_padded(W.reshape(halves, OC, IC) if oc != OC else W, ic)
-            if oc != OC:
-                padded = Wp.new_zeros((halves, oc, ic))
-                padded[:, :OC] = Wp.reshape(halves, OC, ic)
-                Wp = padded
-            Bp = None if Bias is None else _fc_halves(Bias, OC, oc) if glu else _fc_padded(Bias.reshape(1, OC), oc)
-            Rp = None if Residual is None else _fc_padded(Residual.reshape(rows, OC), oc)
-            Y, Z = X.new_empty((rows, oc)), X.new_empty((rows, halves * oc)) if save else None
+                return (X.new_empty(ys), X.new_empty(zs)) if save else X.new_empty(ys)
+            (Xp, Wp, Bp, Rp), _held = _fc_pack(dtype, (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic), (Bias, 1, halves, OC, halves, oc),
+                                               (Residual, 1, rows, OC, rows, oc))
+            even = oc == OC
+            Y = X.new_empty(ys if even else (rows, oc))
+            Z = X.new_empty(zs if even else (rows, halves * oc)) if save else None
             if glu:
-                self.base.fullConnect_glu(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[X.dtype], _l.ACTS[act], float(k), Bp, Z)
+                self.base.fullConnect_glu(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Z)
             else:
-                self.base.fullConnect(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[X.dtype], _l.ACTS[act], float(k), Bp, Rp, Z)
-        if oc != OC:
-            Y = Y[:, :OC]
-            if save:
-                Z = torch.cat((Z[:, :OC], Z[:, oc:oc + OC]), dim=1) if glu else Z[:, :OC]
-        Y = Y.reshape(lead + (OC,))
-        return (Y, Z.reshape(lead + (halves * OC,))) if save else Y
+                self.base.fullConnect(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Rp, Z)
+            if not even:
+                Y = Y[:, :OC].reshape(ys)
+                if save:
+                    Z = Z.reshape(rows, halves, oc)[:, :, :OC].reshape(zs)
+        return (Y, Z) if save else Y
 
     def _fc_delta(self, what, deltaY, X, W, Z, act, k, bias, glu):
-        IC, OC, lead, ic, oc = self._fc_check(what, X, W, glu, act, deltaY=deltaY, Z=Z)
+        dtype = X.dtype
+        IC, OC, ic, oc, rows, halves, ys, zs = _fc_plan(what, glu, X.shape, W.shape, dtype)
+        code = _fc_act(what, act)
+        _fc_check(what, X, W, (("deltaY", deltaY, ys), ("Z", Z, zs)))
         through = glu or act != "none"
         if through and Z is None:
             raise ValueError("%s: Z of the forward pass is needed" % what)
-        halves = 2 if glu else 1
-        rows = X.numel() // IC
         with self._on(X):
             if rows == 0:
-                return torch.empty_like(X), torch.zeros_like(W), W.new_zeros((halves * OC,)) if bias else None
-            dYp, Xp = _fc_padded(deltaY.reshape(rows, OC), oc), _fc_padded(X.reshape(rows, IC), ic)
-            Wp = _fc_padded(W.reshape(halves, OC, IC) if oc != OC else W, ic)
-            if oc != OC:
-                padded = Wp.new_zeros((halves, oc, ic))
-                padded[:, :OC] = Wp.reshape(halves, OC, ic)
-                Wp = padded
-            Zp = dZ = None
-            if through:
-                Zp = _fc_halves(Z.reshape(rows, 2 * OC), OC, oc) if glu else _fc_padded(Z.reshape(rows, OC), oc)
-                dZ = torch.empty_like(Zp)
+                return X.new_empty(X.shape), W.new_zeros(W.shape), W.new_zeros((halves * OC,)) if bias else None
+            (dYp, Xp, Wp, Zp), _held = _fc_pack(dtype, (deltaY, 1, rows, OC, rows, oc), (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic),
+                                                (Z if through else None, 1, rows * halves, OC, rows * halves, oc))
+            dZ = X.new_empty((rows, halves * oc)) if through else None
             dX, dW = X.new_empty((rows, ic)), W.new_empty((halves, oc, ic))
             dB = W.new_empty((halves, oc)) if bias else None
-            self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, oc, _FC_TYPES[X.dtype], _l.ACTS[act], float(k), glu)
-        dX = dX if ic == IC else dX[:, :IC]
-        if oc != OC or ic != IC:
-            dW = dW[:, :OC, :IC]
-        if bias:
-            dB = (dB if oc == OC else dB[:, :OC]).reshape(halves * OC)
-        return dX.reshape(lead + (IC,)), dW.reshape(halves * OC, IC), dB
+            self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, oc, _FC_TYPES[dtype], code, k, glu)
+            if ic != IC:
+                dX = dX[:, :IC]
+            if ic != IC or oc != OC:
+                dW = dW[:, :OC, :IC]
+                dB = dB[:, :OC] if bias else None
+            return dX.reshape(X.shape), dW.reshape(W.shape), dB.reshape(halves * OC) if bias else None
 
     def fullConnect(self, X, W, Bias=None, act="none", k=0.0, Residual=None, save=False):
         """act(X W^T + Bias) + Residual in one pass; W [OC, IC], X [..., IC].  act: 'none', 'leakyRelu' (slope k; relu k = 0),
@@ -692,30 +710,38 @@ class Engine:
             return torch.cuda.stream(s)
         return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
 
-    def _grads(self, what, grads, Out):
-        grads = list(grads)
-        Out = grads if Out is None else list(Out)
-        if len(Out) != len(grads):
-            raise ValueError("%s: %d gradients, %d outputs" % (what, len(grads), len(Out)))
-        table = (_l.AlphaGrad * max(len(grads), 1))()
-        for e, g, o in zip(table, grads, Out):
-            for t in (g, o):
-                if t.dtype not in _FC_TYPES:
-                    raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, t.dtype))
-                if not t.is_cuda or t.device != grads[0].device:
+    @staticmethod
+    def _grads(what, grads, Out):
+        """The tensors as the table the library reads (AlphaGrad: two addresses, a count, two types)."""
+        device, values = grads[0].get_device(), []
+        for g, o in zip(grads, Out):
+            code = _FC_TYPES.get(g.dtype)
+            if g.get_device() != device or device < 0:
+                raise ValueError("%s: tensors must be on one GPU" % what)
+            if not g.is_contiguous() or g.is_neg():
+                raise ValueError("%s: tensors must be contiguous" % what)
+            if o is g:
+                at = g.data_ptr()
+                to, out_code = at, code
+            else:
+                at, to, out_code = g.data_ptr(), o.data_ptr(), _FC_TYPES.get(o.dtype)
+                if o.get_device() != device:
                     raise ValueError("%s: tensors must be on one GPU" % what)
-                if not t.is_contiguous() or t.is_neg():
+                if not o.is_contiguous() or o.is_neg():
                     raise ValueError("%s: tensors must be contiguous" % what)
-            if g.shape != o.shape:
-                raise ValueError("%s: gradient %s, output %s" % (what, tuple(g.shape), tuple(o.shape)))
-            e.grad, e.out, e.count, e.dtype, e.out_dtype = g.data_ptr(), o.data_ptr(), g.numel(), _FC_TYPES[g.dtype], _FC_TYPES[o.dtype]
-        return grads, table
+                if g.shape != o.shape:
+                    raise ValueError("%s: gradient %s, output %s" % (what, tuple(g.shape), tuple(o.shape)))
+            if code is None or out_code is None:
+                raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, g.dtype if code is None else o.dtype))
+            values += (at, to, g.numel(), code | out_code << 32)
+        return struct.pack("<%dq" % len(values), *values)
 
     def grad_norm(self, grads):
         """The 2-norm of all elements of a list of gradients (float32, bfloat16, float16) as a 0-dimensional float32 tensor."""
-        grads, table = self._grads("grad_norm", grads, None)
+        grads = list(grads)
         if not grads:
             return torch.zeros((), device="cuda")
+        table = self._grads("grad_norm", grads, grads)
         with self._on(grads[0]):
             norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
             _l.check(self.base._lib.alpha_grad_norm(len(grads), table, norm.data_ptr(), _stream(self.base._stream)))
@@ -724,9 +750,13 @@ class Engine:
     def clip_grad_norm(self, grads, max_norm, Out=None):
         """grad_norm, and every gradient scaled by min(1, max_norm / (norm + 1e-6)): in place, or into the tensors of Out, which may
         be of another type.  Nothing waits for the norm on the host."""
-        grads, table = self._grads("clip_grad_norm", grads, Out)
+        grads = list(grads)
+        Out = grads if Out is None else list(Out)
+        if len(Out) != len(grads):
+            raise ValueError("clip_grad_norm: %d gradients, %d outputs" % (len(grads), len(Out)))
         if not grads:
             return torch.zeros((), device="cuda")
+        table = self._grads("clip_grad_norm", grads, Out)
         with self._on(grads[0]):
             norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
             _l.check(self.base._lib.alpha_clip_grad_norm(len(grads), table, float(max_norm), norm.data_ptr(), _stream(self.base._stream)))

@@ -60,6 +60,7 @@ def load():
     lib.alpha_conv3d_deltaW.argtypes = [P, V, V, V, V]
     lib.alpha_pad_rows.argtypes = [V, C.c_longlong, I, V, C.c_longlong, I, V]
     lib.alpha_pad_rows_many.argtypes = [I, C.c_char_p, V]
+    lib.alpha_pad_rows_typed.argtypes = [I, C.c_char_p, I, V]
     lib.alpha_conv_bias_grad.argtypes = [V, C.c_longlong, I, V, V]
     lib.alpha_conv3d_deltaW_bias.argtypes = [P, V, V, V, V, V]
     lib.alpha_conv3d_forward_ex.argtypes = [P, V, V, V, V, I, I, V]
@@ -143,7 +144,7 @@ def load():
     for name in ("batchMatMul", "batchMatMul_texture", "batchMatMulT1", "batchMatMulT2", "batchMatMulT2_texture"):
         getattr(lib, "alpha_Cuda_batchMatMul_" + name).argtypes = [SA, I, V, V, V, I, I, I, I, I]
     # FullConnect layers of a transformer, and all gradients of a step
-    F, G = C.POINTER(AlphaFcShape), C.POINTER(AlphaGrad)
+    F, G = C.POINTER(AlphaFcShape), C.c_void_p      # (a table of AlphaGrad, or its bytes)
     lib.alpha_fullConnect.argtypes = [F, V, V, V, V, V, V, V]
     lib.alpha_fullConnect_glu.argtypes = [F, V, V, V, V, V, V]
     lib.alpha_fullConnect_delta.argtypes = [F, V, V, V, V, V, V, V, V, V]
