@@ -7,7 +7,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libalpha_conv_b200.so")
 SOURCES = ["conv_api.cu", "native_api.cu", "matmul_api.cu", "pool_api.cu", "fc_api.cu", "grad_norm.cu", "jni_shim.cpp"]
 HEADERS = ["conv_kernels.cuh", "conv_halo.cuh", "conv_halo_pair.cuh", "conv_dw_halo.cuh", "winograd.cuh", "conv_tapstack.cuh", "sm100_ptx.cuh", "fast_div.cuh", "gemm_f32.cuh", "gemm_planes.cuh", "dependent_launch.cuh",
-           "once_per_device.h", "host_common.h", "fc_act.cuh", "fc_mma.cuh", "fc_small.cuh", "fc_delta.cuh", "fc_f32.cuh"]
+           "once_per_device.h", "host_common.h", "fc_act.cuh", "fc_mma.cuh", "fc_small.cuh", "fc_delta.cuh", "fc_f32.cuh", "fc_pair_f32.cuh"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-shared", "-Xcompiler", "-fPIC"]
 

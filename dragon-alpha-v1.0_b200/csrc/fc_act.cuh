@@ -13,23 +13,23 @@ struct Sigmoid { float pos, neg; };
 template <bool FAST> __device__ __forceinline__ Sigmoid sigmoid_both(float z)
 {
     const float e = FAST ? __expf(-fabsf(z)) : expf(-fabsf(z));
-    const float big = FAST ? __fdividef(1.f, 1.f + e) : 1.f / (1.f + e), small = e * big;
+    const float big = __fdividef(1.f, 1.f + e), small = e * big;
     return z >= 0.f ? Sigmoid{big, small} : Sigmoid{small, big};
 }
 
-// Value and slope of activation ACT at z.  FAST: exponentials and quotients to 2 or 3 units of 2^-23, for results that are rounded to 16
-// bits; else correctly rounded quotients and expf.  z = -Inf gives NaN where the definition is -Inf * 0 (silu, gelu).
+// Value and slope of activation ACT at z.  Quotients err by 2 units of 2^-23, exponentials by as much, or (FAST, for results that are rounded to
+// 16 bits) by 2 + |argument| units.  z = -Inf gives NaN where the definition is -Inf * 0 (silu, gelu).
 template <int ACT, bool FAST> __device__ __forceinline__ float act_value(float z, float k)
 {
     if constexpr (ACT == ALPHA_ACT_NONE) return z;
     else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) return z > 0.f ? z : k * z;
     else if constexpr (ACT == ALPHA_ACT_SIGMOID) return FAST ? __fdividef(1.f, 1.f + __expf(-z)) : sigmoid_both<FAST>(z).pos;
-    else if constexpr (ACT == ALPHA_ACT_SILU) return FAST ? __fdividef(z, 1.f + __expf(-z)) : z / (1.f + expf(-z));
+    else if constexpr (ACT == ALPHA_ACT_SILU) return __fdividef(z, 1.f + (FAST ? __expf(-z) : expf(-z)));
     else if constexpr (ACT == ALPHA_ACT_GELU) return 0.5f * z * erfcf(-0.70710678f * z);
     else {
         // z (1 + tanh(u)) / 2 = z sigmoid(2 u)
         const float u2 = 1.59576912f * (z + 0.044715f * z * z * z);
-        return FAST ? __fdividef(z, 1.f + __expf(-u2)) : z / (1.f + expf(-u2));
+        return __fdividef(z, 1.f + (FAST ? __expf(-u2) : expf(-u2)));
     }
 }
 template <int ACT, bool FAST> __device__ __forceinline__ void act_both(float z, float k, float& value, float& slope)

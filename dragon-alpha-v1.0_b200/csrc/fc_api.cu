@@ -3,6 +3,7 @@
 #include "fc_delta.cuh"
 #include "fc_f32.cuh"
 #include "fc_mma.cuh"
+#include "fc_pair_f32.cuh"
 #include "fc_small.cuh"
 #include "host_common.h"
 
@@ -197,37 +198,231 @@ int launch_product(const Product& q, cudaStream_t stream)
 
 // ---- fp32 products ----------------------------------------------------------------------------------------------
 
-template <int FORM>
-int launch_f32(const float* A, const float* B, int rows, int cols, int K, int lda, int ldb, const FcEpilogue& e, cudaStream_t stream)
+template <bool GLU>
+int launch_parts(const float* part, size_t size, int parts, int rows, const FcEpilogue& e, int sms, cudaStream_t stream)
 {
-    int sms = 0, slice = 0, *status = nullptr;
-    int rc = device_sms(&sms);
-    if (!rc) rc = planes_launch_slice(&slice);
-    if (!rc) rc = device_status_word(&status);
+    const int per_row = e.cols / (GLU ? 2 : 4);
+    const size_t words = static_cast<size_t>(rows) * per_row, blocks = (words + 255) / 256;
+    launch_after(fc_parts_kernel<GLU>, static_cast<unsigned>(blocks < sms * 8u ? blocks : sms * 8u), 256, 0, stream, part, size, parts, fast_div(per_row), words, e);
+    note_launch("fc");
+    return launched("fc_parts_kernel");
+}
+
+// A product of fp32 matrices: rows x cols outputs (glu: cols of both halves), K steps; `form` says which operand runs along the reduction.
+struct ProductF32 { const float *A, *B; int rows, cols, K, lda, ldb; FcEpilogue e; };
+
+// Planes of a matrix in scratch: [plane][row][pitch], pitch in bf16 elements.
+struct Planes { void* ptr = nullptr; const float* src = nullptr; int rows = 0, cols = 0, pitch = 0; };
+Planes planes_of(const float* src, int rows, int cols) { return Planes{nullptr, src, rows, cols, (cols + 7) / 8 * 8}; }
+size_t plane_bytes(const Planes& p) { return (6 * static_cast<size_t>(p.rows) * p.pitch + 255) & ~static_cast<size_t>(255); }
+int launch_split(const Planes* const* list, int n, int sms, cudaStream_t stream)
+{
+    SplitJobs j{};
+    for (int i = 0; i < n; ++i) {
+        const Planes& p = *list[i];
+        j.job[j.n++] = SplitJob{p.src, static_cast<uint2*>(p.ptr), static_cast<unsigned>(p.rows), static_cast<unsigned>(p.cols / 4), j.total, fast_div(p.pitch / 4)};
+        j.total += static_cast<unsigned>(p.rows) * static_cast<unsigned>(p.pitch / 4);
+    }
+    const unsigned blocks = (j.total + 255) / 256, most = static_cast<unsigned>(sms) * 16;
+    launch_after(fc_split_kernel, blocks < most ? blocks : most, 256, 0, stream, j);
+    note_launch("fc");
+    return launched("fc_split_kernel");
+}
+
+// Parts of the reduction on CTA pairs and the time of that product (us): a window of 64 steps of a tile 2.26, an item 2, a launch 5; the parts
+// written and read.  (Estimated / measured, with the split: 2048 x 2048 x 2048 92 / 88, 4096 x 1024 x 4096 170 / 174, 512 x 4096 x 1000 44 / 40.)
+struct PairPlan { int parts; double time; };
+PairPlan pick_pair(int rows, int out_cols, bool glu, int K, int sms)
+{
+    const int pairs = sms / 2, out = glu ? 128 : 256, windows = (K + 63) / 64;
+    PairPlan best{1, 1e300};
+    if (pairs < 1) return best;
+    const double tiles = static_cast<double>((rows + 255) / 256) * ((out_cols + out - 1) / out), size = static_cast<double>(rows) * out_cols * (glu ? 2 : 1);
+    for (int parts = 1; parts <= 32 && parts <= windows; ++parts) {
+        const int each = (windows + parts - 1) / parts;
+        if ((parts - 1) * each >= windows) continue;                      // (no part is empty)
+        const double waves = static_cast<double>(static_cast<long long>((tiles * parts + pairs - 1) / pairs));
+        const double time = 5.0 + waves * (each * 2.26 + 2.0) + (parts > 1 ? 3.0 + size * 4e-6 * (2 * parts + 1) / 6.0 : 0.0);
+        if (time < best.time) best = PairPlan{parts, time};
+    }
+    return best;
+}
+double split_time(size_t elements) { return 2.0 + elements * 10e-6 / 8.0; }
+
+template <int FORM>
+int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, int parts, void* part, int sms, int* status, cudaStream_t stream)
+{
+    constexpr bool GLU = FORM == kFcGlu, A_MN = FORM == kFcDeltaW, B_MN = FORM == kFcDeltaX || FORM == kFcDeltaW;
+    const int cols = GLU ? q.cols / 2 : q.cols, out = GLU ? 128 : 256, halves = GLU ? 2 : 1;
+    PairF32 p{};
+    p.rows = q.rows; p.cols = cols; p.K = q.K;
+    p.m_tiles = (q.rows + 255) / 256; p.n_tiles = (cols + out - 1) / out; p.windows = (q.K + 63) / 64; p.parts = parts;
+    p.a_mn = A_MN; p.b_mn = B_MN; p.b_up = cols;
+    p.idesc = make_idesc_bf16(256, 256, A_MN, B_MN);
+    p.A = q.A; p.B = q.B;
+    p.a_row = A_MN ? 1 : q.lda; p.a_k = A_MN ? q.lda : 1;
+    p.b_col = B_MN ? 1 : q.ldb; p.b_k = B_MN ? q.ldb : 1;
+    p.bias = q.e.bias; p.residual = q.e.residual; p.act = q.e.act; p.k = q.e.k; p.keep_z = parts == 1 && q.e.Z;
+    p.status = status;
+    const size_t size = static_cast<size_t>(q.rows) * q.cols;
+    void* ws = parts > 1 ? part : q.e.Y;
+    auto map = [](CUtensorMap* m, const Planes& s, bool mn) {
+        const cuuint64_t dims[3] = {(cuuint64_t)s.pitch, (cuuint64_t)s.rows, 3}, st[2] = {(cuuint64_t)s.pitch * 2, (cuuint64_t)s.pitch * 2 * s.rows};
+        const cuuint32_t box[3] = {64, mn ? 64u : 128u, 1};
+        return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, s.ptr, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    auto out_map = [&](CUtensorMap* m, const void* base, int h, int copies) {
+        const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)h, (cuuint64_t)q.rows, (cuuint64_t)copies};
+        const cuuint64_t st[3] = {(cuuint64_t)cols * 4, (cuuint64_t)cols * 4 * h, (cuuint64_t)cols * 4 * h * q.rows};
+        const cuuint32_t box[4] = {32, 1, 32, 1};
+        return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    CUtensorMap a, b, y, z;
+    int rc = map(&a, A, A_MN);
+    if (!rc) rc = map(&b, B, B_MN);
+    if (!rc) rc = out_map(&y, ws, parts > 1 ? halves : 1, parts);
+    if (!rc) rc = p.keep_z ? out_map(&z, q.e.Z, halves, 1) : (z = y, ALPHA_OK);
+    if (rc) return rc;
+    const long long items = static_cast<long long>(p.m_tiles) * p.n_tiles * parts;
+    const unsigned pairs = static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
+    allow_smem<fc_pair_f32_kernel<GLU>>();
+    launch_after_clusters(fc_pair_f32_kernel<GLU>, dim3(2 * pairs), kPairF32Threads, 2, kPairF32Smem, stream, a, b, y, z, p);
+    note_launch("fc");
+    note_plan("fc planes pair 256x256 parts=%d", parts);
+    rc = launched("fc_pair_f32_kernel");
+    return rc || parts == 1 ? rc : launch_parts<GLU>(static_cast<const float*>(ws), size, parts, q.rows, q.e, sms, stream);
+}
+
+// The same from the fp32 tensors as they lie; without `may_split` in no scratch.
+template <int FORM>
+int launch_gathered(const ProductF32& q, const PlanePlan& plan, int sms, int* status, cudaStream_t stream)
+{
+    int slice = 0;
+    int rc = planes_launch_slice(&slice);
     if (rc) return rc;
     PlaneFc<FORM> p{};
-    p.A = A; p.B = B; p.rows = rows; p.cols = cols; p.K = K; p.lda = lda; p.ldb = ldb; p.e = e;
-    p.size = static_cast<size_t>(rows) * cols;
-    PlanePlan plan = plan_planes(rows, cols, K, 1, 16, static_cast<double>(p.size), 0, sms);
-    if (plan.ksplit > 1) {
+    p.A = q.A; p.B = q.B; p.rows = q.rows; p.cols = q.cols; p.K = q.K; p.lda = q.lda; p.ldb = q.ldb; p.e = q.e;
+    p.size = static_cast<size_t>(q.rows) * q.cols;
+    p.ksplit = plan.ksplit;
+    if (p.ksplit > 1) {
         void* ws = nullptr;
-        rc = call_scratch(stream, plan.ksplit * p.size * sizeof(float), &ws);
+        rc = call_scratch(stream, p.ksplit * p.size * sizeof(float), &ws);
         if (rc) return rc;
         p.part = static_cast<float*>(ws);
     }
-    p.ksplit = plan.ksplit;
     if (dry_run()) return ALPHA_OK;
-    const dim3 grid((rows + kPlaneBM - 1) / kPlaneBM, (cols + plan.bn - 1) / plan.bn, plan.ksplit);
+    const dim3 grid((q.rows + kPlaneBM - 1) / kPlaneBM, (q.cols + plan.bn - 1) / plan.bn, p.ksplit);
     launch_planes(p, plan.bn, grid, slice, stream, status);
     note_launch("fc");
-    note_plan("fc planes 128x%d ksplit=%d", plan.bn, plan.ksplit);
+    note_plan("fc planes 128x%d ksplit=%d", plan.bn, p.ksplit);
     rc = launched("gemm_planes_kernel");
-    if (rc || plan.ksplit == 1) return rc;
-    const size_t n4 = p.size / 4, blocks = (n4 + 255) / 256;
-    launch_after(fc_parts_kernel<FORM == kFcGlu>, static_cast<unsigned>(blocks < sms * 8u ? blocks : sms * 8u), 256, 0, stream, reinterpret_cast<const float4*>(p.part), n4,
-                 plan.ksplit, cols / 4, e);
-    note_launch("fc");
-    return launched("fc_parts_kernel");
+    return rc || p.ksplit == 1 ? rc : launch_parts<FORM == kFcGlu>(p.part, p.size, p.ksplit, q.rows, q.e, sms, stream);
+}
+
+template <int FORM> PlanePlan pick_gathered(const ProductF32& q, int sms, int most = 16)
+{
+    return plan_planes(q.rows, q.cols, q.K, 1, most, static_cast<double>(q.rows) * q.cols, 0, sms);
+}
+// In any case: without parts where their scratch is refused.
+template <int FORM> int run_gathered(const ProductF32& q, int sms, int* status, cudaStream_t stream)
+{
+    const int rc = launch_gathered<FORM>(q, pick_gathered<FORM>(q, sms), sms, status, stream);
+    return rc == ALPHA_E_NOSCRATCH || rc == ALPHA_E_CAPTURE ? launch_gathered<FORM>(q, pick_gathered<FORM>(q, sms, 1), sms, status, stream) : rc;
+}
+
+// One or two products by pairs over operands that are split together; 1 where their scratch is refused (nothing has been launched then).
+struct PairWork {
+    Planes p[3];
+    int n = 0;
+    size_t parts = 0;          // bytes of the larger of the products' parts
+    int sms = 0, *status = nullptr;
+    void* part = nullptr;
+    int add(const float* src, int rows, int cols) { p[n] = planes_of(src, rows, cols); return n++; }
+    void want(const ProductF32& q, int k) { const size_t bytes = k > 1 ? k * static_cast<size_t>(q.rows) * q.cols * sizeof(float) : 0; if (bytes > parts) parts = bytes; }
+    size_t elements() const { size_t e = 0; for (int i = 0; i < n; ++i) e += static_cast<size_t>(p[i].rows) * p[i].pitch; return e; }
+    bool fits() const { return elements() < 4ull << 31; }           // 32-bit indices of words of four
+    int split(cudaStream_t stream)
+    {
+        size_t bytes = parts;
+        for (int i = 0; i < n; ++i) bytes += plane_bytes(p[i]);
+        void* ws = nullptr;
+        const int rc = call_scratch(stream, bytes, &ws);
+        if (rc) return rc == ALPHA_E_NOSCRATCH || rc == ALPHA_E_CAPTURE ? 1 : rc;
+        if (dry_run()) return ALPHA_OK;
+        char* at = static_cast<char*>(ws);
+        for (int i = 0; i < n; ++i) { p[i].ptr = at; at += plane_bytes(p[i]); }
+        part = at;
+        const Planes* list[3] = {&p[0], &p[1], &p[2]};
+        return launch_split(list, n, sms, stream);
+    }
+};
+
+// Option FC_TILE: 1 pairs, 2 never, else where their estimated time is less.
+bool pairs_pay(double pair, double other)
+{
+    const int forced = option_fc_tile();
+    return forced == 1 || (forced != 2 && pair < other);
+}
+
+template <int FORM>
+int forward_f32(const ProductF32& q, cudaStream_t stream)
+{
+    PairWork w;
+    int rc = device_sms(&w.sms);
+    if (!rc) rc = device_status_word(&w.status);
+    if (rc) return rc;
+    const PairPlan pair = pick_pair(q.rows, FORM == kFcGlu ? q.cols / 2 : q.cols, FORM == kFcGlu, q.K, w.sms);
+    const int a = w.add(q.A, q.rows, q.K), b = w.add(q.B, q.cols, q.K);
+    w.want(q, pair.parts);
+    if (w.sms >= 2 && w.fits() && pairs_pay(pair.time + split_time(w.elements()), pick_gathered<FORM>(q, w.sms).time)) {
+        rc = w.split(stream);
+        if (rc == 0) return dry_run() ? ALPHA_OK : launch_pair<FORM>(q, w.p[a], w.p[b], pair.parts, w.part, w.sms, w.status, stream);
+        if (rc < 0) return rc;
+    }
+    return run_gathered<FORM>(q, w.sms, w.status, stream);
+}
+
+// deltaX = dZ W and deltaW = dZ^T X (either may be missing).
+int delta_f32(const float* dZ, const float* X, const float* W, float* dX, float* dW, int rows, int wide, int IC, cudaStream_t stream)
+{
+    const FcEpilogue plain{nullptr, nullptr, nullptr, nullptr, IC, ALPHA_ACT_NONE, 0.f};
+    ProductF32 x{dZ, W, rows, IC, wide, wide, IC, plain}, w{dZ, X, wide, IC, rows, wide, IC, plain};
+    x.e.Y = dX; w.e.Y = dW;
+    int sms = 0, *status = nullptr;
+    int rc = device_sms(&sms);
+    if (!rc) rc = device_status_word(&status);
+    if (rc) return rc;
+    // which of them by pairs: both share the planes of dZ
+    const PairPlan px = pick_pair(rows, IC, false, wide, sms), pw = pick_pair(wide, IC, false, rows, sms);
+    const double gx = pick_gathered<kFcDeltaX>(x, sms).time, gw = pick_gathered<kFcDeltaW>(w, sms).time;
+    PairWork best;
+    bool best_x = false, best_w = false;
+    double least = 1e300;
+    for (int form = 0; form < 4; ++form) {
+        const bool bx = form & 1, bw = form & 2;
+        if ((bx && !dX) || (bw && !dW) || (form && sms < 2)) continue;
+        if (option_fc_tile() == 1 && sms >= 2 && (bx != (dX != nullptr) || bw != (dW != nullptr))) continue;
+        if (option_fc_tile() == 2 && form) continue;
+        PairWork v;
+        v.sms = sms; v.status = status;
+        if (form) v.add(dZ, rows, wide);
+        if (bx) { v.add(W, wide, IC); v.want(x, px.parts); }
+        if (bw) { v.add(X, rows, IC); v.want(w, pw.parts); }
+        if (!v.fits()) continue;
+        const double time = (dX ? (bx ? px.time : gx) : 0.0) + (dW ? (bw ? pw.time : gw) : 0.0) + (form ? split_time(v.elements()) : 0.0);
+        if (time < least) { least = time; best = v; best_x = bx; best_w = bw; }
+    }
+    if (best.n) {
+        rc = best.split(stream);
+        if (rc < 0) return rc;
+        if (rc == 1) best_x = best_w = false;
+    }
+    rc = ALPHA_OK;
+    if (best_x && !dry_run()) rc = launch_pair<kFcDeltaX>(x, best.p[0], best.p[1], px.parts, best.part, sms, status, stream);
+    if (!rc && best_w && !dry_run()) rc = launch_pair<kFcDeltaW>(w, best.p[0], best.p[best_x ? 2 : 1], pw.parts, best.part, sms, status, stream);
+    if (!rc && dX && !best_x) rc = run_gathered<kFcDeltaX>(x, sms, status, stream);
+    if (!rc && dW && !best_w) rc = run_gathered<kFcDeltaW>(w, sms, status, stream);
+    return rc;
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
@@ -295,7 +490,8 @@ int forward(const char* what, const AlphaFcShape* s, const void* X, const void* 
     if (s->dtype == ALPHA_F32) {
         const FcEpilogue e{static_cast<const float*>(bias), static_cast<const float*>(residual), static_cast<float*>(Z), static_cast<float*>(Y), s->OC, s->act, s->k};
         const float *x = static_cast<const float*>(X), *w = static_cast<const float*>(W);
-        return glu ? launch_f32<kFcGlu>(x, w, s->rows, 2 * s->OC, s->IC, s->IC, s->IC, e, stream) : launch_f32<kFcForward>(x, w, s->rows, s->OC, s->IC, s->IC, s->IC, e, stream);
+        return glu ? forward_f32<kFcGlu>(ProductF32{x, w, s->rows, 2 * s->OC, s->IC, s->IC, s->IC, e}, stream)
+                   : forward_f32<kFcForward>(ProductF32{x, w, s->rows, s->OC, s->IC, s->IC, s->IC, e}, stream);
     }
     if (dry_run()) return ALPHA_OK;
     return launch_product(Product{s->dtype, s->rows, s->OC, s->IC, false, false, glu, X, W, bias, residual, Z, Y, s->act, s->k}, stream);
@@ -357,12 +553,8 @@ int delta(const char* what, const AlphaFcShape* s, const void* dY, const void* X
     const void* d = through ? dZ : dY;
     const int w = static_cast<int>(wide);
     if (s->dtype == ALPHA_F32) {
-        FcEpilogue e{nullptr, nullptr, nullptr, static_cast<float*>(dX), s->IC, ALPHA_ACT_NONE, 0.f};
-        const float* z = static_cast<const float*>(d);
-        if (dX) rc = launch_f32<kFcDeltaX>(z, static_cast<const float*>(W), s->rows, s->IC, w, w, s->IC, e, stream);
-        e.Y = static_cast<float*>(dW);
-        if (!rc && dW) rc = launch_f32<kFcDeltaW>(z, static_cast<const float*>(X), w, s->IC, s->rows, w, s->IC, e, stream);
-        return rc;
+        return delta_f32(static_cast<const float*>(d), static_cast<const float*>(X), static_cast<const float*>(W), static_cast<float*>(dX), static_cast<float*>(dW), s->rows, w,
+                         s->IC, stream);
     }
     if (dry_run()) return ALPHA_OK;
     if (dX) rc = launch_product(Product{s->dtype, s->rows, s->IC, w, false, true, false, d, W, nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f}, stream);

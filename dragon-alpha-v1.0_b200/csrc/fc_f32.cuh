@@ -6,7 +6,7 @@
 namespace alpha {
 
 // What becomes of the sums of a layer: four consecutive columns of a row, glu (gate, up, gate, up) of two units.  Rows are given by
-// their place in Y, from which Z and R follow (the same pitch; glu: Z twice).
+// their place in Y, from which Z and R follow (the same pitch; glu: Z twice).  Parts of sums lie [part][row][column], glu [part][row][gates, ups].
 struct FcEpilogue {
     const float *bias, *residual;
     float *Z, *Y;
@@ -94,25 +94,41 @@ struct PlaneFc {
     {
         const int j = c.n0 + col;
         if (!row || j >= cols) return;
-        if (ksplit > 1 || FORM == kFcDeltaX || FORM == kFcDeltaW) *reinterpret_cast<float4*>(row + j) = o;
+        if (ksplit > 1 && FORM == kFcGlu) {
+            *reinterpret_cast<float2*>(row + (j >> 1)) = make_float2(o.x, o.z);
+            *reinterpret_cast<float2*>(row + e.cols + (j >> 1)) = make_float2(o.y, o.w);
+        } else if (ksplit > 1 || FORM == kFcDeltaX || FORM == kFcDeltaW) *reinterpret_cast<float4*>(row + j) = o;
         else fc_finish<FORM == kFcGlu>(e, row, j, o);
     }
 };
 
-// The parts of a product added in order, then finished.
+// The parts of a product added in order, then finished: four outputs a thread, glu two.
 template <bool GLU>
-__global__ void __launch_bounds__(256) fc_parts_kernel(const float4* __restrict__ part, size_t n4, int parts, int cols4, const __grid_constant__ FcEpilogue e)
+__global__ void __launch_bounds__(256) fc_parts_kernel(const float* __restrict__ part, size_t size, int parts, FastDiv by_words, size_t words, const __grid_constant__ FcEpilogue e)
 {
     grid_dependency_wait();
     grid_dependency_trigger();
-    for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n4; i += static_cast<size_t>(gridDim.x) * 256) {
-        float4 s = __ldg(part + i);
-        for (int q = 1; q < parts; ++q) {
-            const float4 v = __ldg(part + q * n4 + i);
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < words; i += static_cast<size_t>(gridDim.x) * 256) {
+        unsigned row, q;
+        by_words.divmod(static_cast<unsigned>(i), row, q);
+        float* out = e.Y + static_cast<size_t>(row) * e.cols;
+        if constexpr (GLU) {
+            const float* at = part + 2 * static_cast<size_t>(row) * e.cols + 2 * q;
+            float2 g = make_float2(0.f, 0.f), u = g;
+            for (int s = 0; s < parts; ++s, at += size) {
+                const float2 a = __ldg(reinterpret_cast<const float2*>(at)), b = __ldg(reinterpret_cast<const float2*>(at + e.cols));
+                g.x += a.x; g.y += a.y; u.x += b.x; u.y += b.y;
+            }
+            fc_finish<true>(e, out, 4 * q, make_float4(g.x, u.x, g.y, u.y));
+        } else {
+            const float* at = part + static_cast<size_t>(row) * e.cols + 4 * q;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int r = 0; r < parts; ++r, at += size) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(at));
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            fc_finish<false>(e, out, 4 * q, s);
         }
-        const size_t row = i / cols4;
-        fc_finish<GLU>(e, e.Y + row * e.cols, static_cast<int>(i - row * cols4) * 4, s);
     }
 }
 

@@ -108,7 +108,7 @@ def test_forward_activations(eng, lib, dtype, act, glu, rows):
 
 # CTA pairs, the plan by cost, tiles of some widths, tiles shared by 2, 4 and 8 CTAs
 @pytest.mark.parametrize("tile", (1, 2, 1016, 1064, 1112, 1256, 2080, 4048, 8256))
-@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("glu", (False, True), ids=("fc", "glu"))
 @pytest.mark.parametrize("shape", [(1, 64, 8), (77, 200, 136), (700, 520, 1304), (2500, 128, 1544)], ids=lambda s: "x".join(map(str, s)))
 def test_forward_tiles(eng, lib, dtype, glu, tile, shape):
@@ -171,7 +171,7 @@ def test_delta_activations(eng, lib, dtype, act, glu):
 
 # CTA pairs, the plan by cost, tiles of some widths, tiles shared by 2, 4 and 8 CTAs
 @pytest.mark.parametrize("tile", (1, 2, 1016, 1064, 1112, 1256, 2080, 4048, 8256))
-@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(3, 8, 16), (700, 520, 1304), (1500, 1544, 200)], ids=lambda s: "x".join(map(str, s)))
 def test_delta_tiles(eng, lib, dtype, tile, shape):
     old = lib.set_option("FC_TILE", tile)
