@@ -17,6 +17,22 @@ template <bool FAST> __device__ __forceinline__ Sigmoid sigmoid_both(float z)
     return z >= 0.f ? Sigmoid{big, small} : Sigmoid{small, big};
 }
 
+// The normal distribution function at z and exp(-z^2 / 2), to 9e-6 of its value for |z| < 9: with x = |z| / sqrt(2), erfc(x) = exp(-x^2) erfcx(x), and
+// erfcx(x) as a polynomial in t = 1 / (1 + 0.44 x), fitted by weighted least squares for 0 <= x <= 12 (relative error 5.2e-6).  Enough for results
+// of 11 bits; erfcf with an exponential beside it took twice the time of the whole gradient pass (117 us instead of 60, 4096 x 11008).
+struct NormalCdf { float cdf, exp; };
+__device__ __forceinline__ NormalCdf normal_cdf_16(float z)
+{
+    const float t = __fdividef(1.f, fmaf(0.44f * 0.70710678f, fabsf(z), 1.f)), e = __expf(-0.5f * z * z);
+    float p = fmaf(t, -0.14610653f, 0.35065508f);
+    p = fmaf(t, p, 0.0407281f);
+    p = fmaf(t, p, 0.26358804f);
+    p = fmaf(t, p, 0.24256907f);
+    p = fmaf(t, p, 0.24856107f);
+    const float tail = 0.5f * t * p * e;
+    return NormalCdf{z >= 0.f ? 1.f - tail : tail, e};
+}
+
 // Value and slope of activation ACT at z.  Quotients err by 2 units of 2^-23, exponentials by as much, or (FAST, for results that are rounded to
 // 16 bits) by 2 + |argument| units.  z = -Inf gives NaN where the definition is -Inf * 0 (silu, gelu).
 template <int ACT, bool FAST> __device__ __forceinline__ float act_value(float z, float k)
@@ -25,7 +41,7 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_value(float z
     else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) return z > 0.f ? z : k * z;
     else if constexpr (ACT == ALPHA_ACT_SIGMOID) return FAST ? __fdividef(1.f, 1.f + __expf(-z)) : sigmoid_both<FAST>(z).pos;
     else if constexpr (ACT == ALPHA_ACT_SILU) return __fdividef(z, 1.f + (FAST ? __expf(-z) : expf(-z)));
-    else if constexpr (ACT == ALPHA_ACT_GELU) return 0.5f * z * erfcf(-0.70710678f * z);
+    else if constexpr (ACT == ALPHA_ACT_GELU) return FAST ? z * normal_cdf_16(z).cdf : 0.5f * z * erfcf(-0.70710678f * z);
     else {
         // z (1 + tanh(u)) / 2 = z sigmoid(2 u)
         const float u2 = 1.59576912f * (z + 0.044715f * z * z * z);
@@ -43,8 +59,8 @@ template <int ACT, bool FAST> __device__ __forceinline__ void act_both(float z, 
         const Sigmoid s = sigmoid_both<FAST>(z);
         value = z * s.pos; slope = s.pos * (1.f + z * s.neg);
     } else if constexpr (ACT == ALPHA_ACT_GELU) {
-        const float cdf = 0.5f * erfcf(-0.70710678f * z), zz = -0.5f * z * z;
-        value = z * cdf; slope = cdf + z * 0.39894228f * (FAST ? __expf(zz) : expf(zz));
+        const NormalCdf n = FAST ? normal_cdf_16(z) : NormalCdf{0.5f * erfcf(-0.70710678f * z), expf(-0.5f * z * z)};
+        value = z * n.cdf; slope = n.cdf + z * 0.39894228f * n.exp;
     } else {
         const Sigmoid s = sigmoid_both<FAST>(1.59576912f * (z + 0.044715f * z * z * z));
         // (from |z| = 16 on the slope is 0 or 1, and the square of a larger z may overflow)

@@ -505,8 +505,9 @@ int launch_delta(const AlphaFcShape* s, const void* dY, const void* Z, void* dZ,
     if (rc) return rc;
     const int wide = GLU ? 2 * s->OC : s->OC, words = s->OC / Word16<T>::N;
     const unsigned gy = (words + 31) / 32;
-    // eight CTAs an SM, eight rows of a warp at least
-    long long gx = (sms * 8LL + gy - 1) / gy;
+    // one wave of CTAs, eight rows of a warp at least
+    long long gx = sms * (long long)kDeltaCtas / gy;
+    if (gx < 1) gx = 1;
     const long long by_rows = (s->rows + 63) / 64;
     if (gx > by_rows) gx = by_rows;
     FcDelta p{s->rows, s->OC, s->act, s->k, dY, Z, dZ, nullptr};

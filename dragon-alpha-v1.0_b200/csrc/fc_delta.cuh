@@ -21,8 +21,9 @@ struct FcDelta {
     float* part;                    // [gridDim.y][cols, glu: 2 cols] or nullptr
 };
 
+constexpr int kDeltaCtas = 3;           // of an SM
 template <class T, bool GLU>
-__global__ void __launch_bounds__(256) fc_delta_kernel(const __grid_constant__ FcDelta p)
+__global__ void __launch_bounds__(256, kDeltaCtas) fc_delta_kernel(const __grid_constant__ FcDelta p)
 {
     using V = Word16<T>;
     constexpr int N = V::N, HALVES = GLU ? 2 : 1;
@@ -43,7 +44,7 @@ __global__ void __launch_bounds__(256) fc_delta_kernel(const __grid_constant__ F
             constexpr int kRows = GLU ? 2 : 4;
             const long long stride = gridDim.y * 8;
             for (long long r0 = blockIdx.y * 8 + warp; r0 < p.rows; r0 += kRows * stride) {
-                uint4 wd[kRows], wg[kRows], wu[kRows];
+                uint4 wd[kRows], wg[kRows], wu[GLU ? kRows : 1];
 #pragma unroll
                 for (int q = 0; q < kRows; ++q) {
                     const long long r = r0 + q * stride < p.rows ? r0 + q * stride : r0;

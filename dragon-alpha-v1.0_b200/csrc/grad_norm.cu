@@ -63,6 +63,14 @@ template <class F> __device__ __forceinline__ void with_type(int type, F&& f)
     else f(__half{});
 }
 
+// (a gradient may be its own output: not by the read-only path)
+__device__ __forceinline__ uint4 load_once(const uint4* p)
+{
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 template <int N> __device__ __forceinline__ double word_squares(const float (&f)[N])
 {
     float s = f[0] * f[0];
@@ -88,17 +96,25 @@ __device__ __forceinline__ double cta_sum(double s, double* shared)
     return s;
 }
 
-// Elements of a chunk as words: word(i) for whole words, single(v) for the elements of words at the ends (v counts from the boundary).
+// Elements of a chunk: word(w, number) for whole words, single(v) for the elements of words at the ends of the tensor (v counts from the boundary).
+// A chunk of whole words is loaded at once, so that all loads of a thread are in flight together.
 template <int N, class Word, class Single>
-__device__ __forceinline__ void walk_chunk(const GradTensor& t, long long begin, Word&& word, Single&& single)
+__device__ __forceinline__ void walk_chunk(const GradTensor& t, const uint4* base, long long begin, Word&& word, Single&& single)
 {
     const long long end = t.lead + t.count;                          // in elements from the boundary
-    const long long stop = begin + kGradChunk < end ? begin + kGradChunk : end;
     constexpr int kWords = kGradChunk / N / kGradThreads;
-#pragma unroll 4
-    for (int i = 0; i < kWords; ++i) {
-        const long long v = begin + static_cast<long long>(i * kGradThreads + static_cast<int>(threadIdx.x)) * N;
-        if (v >= t.lead && v + N <= stop) word(v / N);
+    if (begin >= t.lead && begin + kGradChunk <= end) {
+        const long long first = begin / N + threadIdx.x;
+        uint4 w[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = load_once(base + first + i * kGradThreads);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) word(w[i], first + i * kGradThreads);
+        return;
+    }
+    const long long stop = begin + kGradChunk < end ? begin + kGradChunk : end;
+    for (long long v = begin + static_cast<long long>(threadIdx.x) * N; v < stop; v += static_cast<long long>(kGradThreads) * N) {
+        if (v >= t.lead && v + N <= stop) word(load_once(base + v / N), v / N);
         else
             for (long long e = v < t.lead ? t.lead : v; e < v + N && e < stop; ++e) single(e);
     }
@@ -117,10 +133,10 @@ __global__ void __launch_bounds__(kGradThreads) grad_squares_kernel(const __grid
             using T = decltype(type);
             constexpr int N = Word16<T>::N;
             const T* base = static_cast<const T*>(t.grad) - t.lead;
-            walk_chunk<N>(t, begin,
-                [&](long long w) {
+            walk_chunk<N>(t, reinterpret_cast<const uint4*>(base), begin,
+                [&](const uint4& v, long long) {
                     float f[N];
-                    Word16<T>::load(__ldg(reinterpret_cast<const uint4*>(base) + w), f);
+                    Word16<T>::load(v, f);
                     sum += word_squares(f);
                 },
                 [&](long long e) { const double x = element(base + e); sum = fma(x, x, sum); });
@@ -169,10 +185,10 @@ __global__ void __launch_bounds__(kGradThreads) grad_scale_kernel(const __grid_c
             with_type(t.out_type, [&](auto out_type) {
                 using O = decltype(out_type);
                 O* out = static_cast<O*>(t.out) - t.lead;
-                walk_chunk<N>(t, begin,
-                    [&](long long w) {
+                walk_chunk<N>(t, reinterpret_cast<const uint4*>(base), begin,
+                    [&](const uint4& v, long long w) {
                         float f[N];
-                        Word16<T>::load(reinterpret_cast<const uint4*>(base)[w], f);
+                        Word16<T>::load(v, f);
 #pragma unroll
                         for (int i = 0; i < N; ++i) f[i] = f[i] * c * tail;
                         if constexpr (sizeof(O) <= sizeof(T) && N < Word16<O>::N) {      // half a word of a narrower type
