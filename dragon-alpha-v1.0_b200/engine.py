@@ -147,9 +147,9 @@ class CudaFloat32EngineBase:
     def _addr(a):
         return a.data_ptr() if isinstance(a, torch.Tensor) else int(a)
 
-    @classmethod
-    def _addr_or_none(cls, a):
-        return None if a is None else cls._addr(a)
+    @staticmethod
+    def _addr_or_none(a):
+        return a if a is None or type(a) is int else a.data_ptr() if isinstance(a, torch.Tensor) else int(a)
 
     def conv3D(self, Y_address, OH, OW, X_address, IH, IW, W_address, FH, FW, N, IC, OC, sh, sw, ph, pw):
         """CudaFloat32EngineBase.conv3D (:1355-1474)."""
@@ -383,35 +383,40 @@ _cached_fc_shape = functools.lru_cache(maxsize=512)(_l.AlphaFcShape)
 
 def _fc_pack(dtype, *jobs):
     """The operands of one call, (t, groups, rows, cols, rows4, cols4) each: t holds `groups` matrices of rows x cols, wanted dense, on a 16-byte
-    boundary and zero-padded to rows4 x cols4.  Those that need padding are written by one launch into one block of memory.  Returns tensors (None for
-    None), or addresses inside the block, and the block (to be held until the call has been enqueued)."""
-    out, plan, size = [], [], 0
-    for job in jobs:
-        t = job[0]
+    boundary and zero-padded to rows4 x cols4.  Those that need padding are written by one launch into one block of memory.  Returns addresses (None for
+    None) and what has to be held until the call has been enqueued."""
+    out, held, plan, size = [], [], [], 0
+    for t, groups, rows, cols, rows4, cols4 in jobs:
         if t is None:
             out.append(None)
             continue
         if not t.is_contiguous():
             t = t.contiguous()
+            held.append(t)
         if t.is_neg():                      # (a lazily negated view: its memory is not its value)
             t = t.resolve_neg()
-        _, groups, rows, cols, rows4, cols4 = job
+            held.append(t)
+        at = t.data_ptr()
         if cols != cols4 or rows != rows4:
-            plan.append((len(out), t, groups, rows, cols, rows4, cols4, size))
+            plan.append((len(out), at, groups, rows, cols, rows4, cols4, size, t))
             size += (groups * rows4 * cols4 + 127) // 128 * 128     # (each starts on 256 bytes, like a tensor of its own)
-        elif t.data_ptr() % 16:
+        elif at & 15:
             t = t.clone()
-        out.append(t)
-    if not plan:
-        return out, None
-    block = plan[0][1].new_empty(size)
-    base, each, values = block.data_ptr(), block.element_size(), []
-    for i, t, groups, rows, cols, rows4, cols4, at in plan:
-        out[i], src = base + at * each, t.data_ptr()
-        for g in range(groups):
-            values += (src + g * rows * cols * each, rows, cols, out[i] + g * rows4 * cols4 * each, rows4, cols4)
-    _l.check(_l.load().alpha_pad_rows_typed(len(values) // 6, struct.pack("%dq" % len(values), *values), _FC_TYPES[dtype], _stream()))
-    return out, (block, [job[1] for job in plan])
+            held.append(t)
+            at = t.data_ptr()
+        out.append(at)
+    if plan:
+        block = torch.empty(size, dtype=dtype, device=plan[0][8].device)
+        base, each, values = block.data_ptr(), block.element_size(), []
+        for i, src, groups, rows, cols, rows4, cols4, at, _ in plan:
+            out[i] = to = base + at * each
+            for _ in range(groups):
+                values += (src, rows, cols, to, rows4, cols4)
+                src += rows * cols * each
+                to += rows4 * cols4 * each
+        _l.check(_l.load().alpha_pad_rows_typed(len(values) // 6, struct.pack("%dq" % len(values), *values), _FC_TYPES[dtype], _stream()))
+        held.append(block)
+    return out, held
 
 
 @functools.lru_cache(maxsize=512)
@@ -650,7 +655,9 @@ class Engine:
             else:
                 self.base.fullConnect(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Rp, Z)
             if not even:
-                Y = Y[:, :OC].reshape(ys)
+                Y = Y.narrow(1, 0, OC)
+                if len(ys) != 2:
+                    Y = Y.reshape(ys)
                 if save:
                     Z = Z.reshape(rows, halves, oc)[:, :, :OC].reshape(zs)
         return (Y, Z) if save else Y
@@ -673,11 +680,11 @@ class Engine:
             dB = W.new_empty((halves, oc)) if bias else None
             self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, oc, _FC_TYPES[dtype], code, k, glu)
             if ic != IC:
-                dX = dX[:, :IC]
+                dX = dX.narrow(1, 0, IC)
             if ic != IC or oc != OC:
                 dW = dW[:, :OC, :IC]
                 dB = dB[:, :OC] if bias else None
-            return dX.reshape(X.shape), dW.reshape(W.shape), dB.reshape(halves * OC) if bias else None
+            return dX if X.dim() == 2 else dX.reshape(X.shape), dW.reshape(W.shape), dB.reshape(halves * OC) if bias else None
 
     def fullConnect(self, X, W, Bias=None, act="none", k=0.0, Residual=None, save=False):
         """act(X W^T + Bias) + Residual in one pass; W [OC, IC], X [..., IC].  act: 'none', 'leakyRelu' (slope k; relu k = 0),
@@ -713,28 +720,29 @@ class Engine:
     @staticmethod
     def _grads(what, grads, Out):
         """The tensors as the table the library reads (AlphaGrad: two addresses, a count, two types)."""
-        device, values = grads[0].get_device(), []
+        device, values, types = grads[0].get_device(), [], _FC_TYPES
         for g, o in zip(grads, Out):
-            code = _FC_TYPES.get(g.dtype)
-            if g.get_device() != device or device < 0:
-                raise ValueError("%s: tensors must be on one GPU" % what)
-            if not g.is_contiguous() or g.is_neg():
-                raise ValueError("%s: tensors must be contiguous" % what)
-            if o is g:
-                at = g.data_ptr()
-                to, out_code = at, code
-            else:
-                at, to, out_code = g.data_ptr(), o.data_ptr(), _FC_TYPES.get(o.dtype)
-                if o.get_device() != device:
-                    raise ValueError("%s: tensors must be on one GPU" % what)
-                if not o.is_contiguous() or o.is_neg():
-                    raise ValueError("%s: tensors must be contiguous" % what)
-                if g.shape != o.shape:
-                    raise ValueError("%s: gradient %s, output %s" % (what, tuple(g.shape), tuple(o.shape)))
-            if code is None or out_code is None:
-                raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, g.dtype if code is None else o.dtype))
+            code = out_code = types.get(g.dtype)
+            at = to = g.data_ptr()
+            good = g.get_device() == device and g.is_contiguous() and not g.is_neg()
+            if o is not g:
+                to, out_code = o.data_ptr(), types.get(o.dtype)
+                good = good and o.get_device() == device and o.is_contiguous() and not o.is_neg() and o.shape == g.shape
+            if not good or device < 0 or code is None or out_code is None:
+                Engine._refuse_grads(what, device, g, o)
             values += (at, to, g.numel(), code | out_code << 32)
         return struct.pack("<%dq" % len(values), *values)
+
+    @staticmethod
+    def _refuse_grads(what, device, g, o):
+        if device < 0 or g.get_device() != device or o.get_device() != device:
+            raise ValueError("%s: tensors must be on one GPU" % what)
+        for t in (g, o):
+            if t.dtype not in _FC_TYPES:
+                raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, t.dtype))
+            if not t.is_contiguous() or t.is_neg():
+                raise ValueError("%s: tensors must be contiguous" % what)
+        raise ValueError("%s: gradient %s, output %s" % (what, tuple(g.shape), tuple(o.shape)))
 
     def grad_norm(self, grads):
         """The 2-norm of all elements of a list of gradients (float32, bfloat16, float16) as a 0-dimensional float32 tensor."""

@@ -91,3 +91,40 @@ def test_clip_arguments(lib):
         refused(lib, clip(lib, ok, norm=bad, scale=False), "norm must be")
     refused(lib, lib.load().alpha_grad_norm(2, None, 20 << 32, None), "no tensors")
     refused(lib, lib.load().alpha_grad_norm(-1, None, 20 << 32, None), "no tensors")
+
+
+# ---- Engine: shapes, types and devices, before anything is launched (tensors of the meta and the CPU device) ----
+
+@pytest.fixture(scope="module")
+def eng(pkg):
+    return pkg.submodule("engine").Engine()
+
+
+def _t(*shape, dtype=None):
+    torch = pytest.importorskip("torch")
+    return torch.zeros(shape, dtype=dtype or torch.float32)
+
+
+@pytest.mark.parametrize("glu", (False, True))
+def test_engine_forward(eng, glu):
+    torch = pytest.importorskip("torch")
+    fn = eng.fullConnect_glu if glu else eng.fullConnect
+    for args, kw, word in [
+        ((_t(4, 8), _t(6, 9)), {}, "against W"), ((_t(4, 8), _t(6, 8, 1)), {}, "against W"), ((_t(4, 0), _t(6, 0)), {}, "against W"), ((_t(4, 8), _t(0, 8)), {}, "against W"),
+        ((_t(4, 8, dtype=torch.float64), _t(6, 8, dtype=torch.float64)), {}, "float32, bfloat16 or float16"), ((_t(4, 8), _t(6, 8)), dict(act="relu"), "act must be one of"),
+        ((_t(4, 8), _t(6, 8)), {}, "on a GPU"),
+    ]:
+        with pytest.raises(ValueError, match=word):
+            fn(*args, **kw)
+    if glu:
+        with pytest.raises(ValueError, match="gate rows and as many up rows"):
+            fn(_t(4, 8), _t(7, 8))
+
+
+def test_engine_grads(eng):
+    with pytest.raises(ValueError, match="1 gradients, 2 outputs"):
+        eng.clip_grad_norm([_t(4)], 1.0, Out=[_t(4), _t(4)])
+    with pytest.raises(ValueError, match="on one GPU"):
+        eng.clip_grad_norm([_t(4)], 1.0)
+    with pytest.raises(ValueError, match="on one GPU"):
+        eng.grad_norm([_t(4)])

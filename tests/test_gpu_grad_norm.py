@@ -109,3 +109,56 @@ def test_same_bits(eng):
     first = eng.grad_norm(grads)
     for _ in range(20):
         assert torch.equal(eng.grad_norm(grads), first)
+
+
+def test_capture_and_replay(eng, pkg):
+    lib = pkg.submodule("lib")
+    grads = [torch.randn(n, device="cuda") for n in (5000, 123)]
+    out = [torch.empty_like(g) for g in grads]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        with pytest.raises(lib.AlphaConvError) as e:
+            eng.clip_grad_norm(grads, 1.0, Out=out)          # (no scratch yet)
+        assert e.value.code == -6
+    with torch.cuda.stream(s):
+        eng.clip_grad_norm(grads, 1.0, Out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        norm = eng.clip_grad_norm(grads, 1.0, Out=out)
+    for a in grads:
+        a.mul_(3.0)
+    torch.cuda.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    ref = norm64(grads)
+    check_norm(norm, ref)
+    for o, a in zip(out, grads):
+        check_scaled(o, a, ref, 1.0)
+
+
+def test_nothing_to_do(eng):
+    assert float(eng.grad_norm([])) == 0 and float(eng.clip_grad_norm([], 1.0)) == 0
+    empty = torch.empty(0, device="cuda")
+    assert float(eng.grad_norm([empty])) == 0 and float(eng.clip_grad_norm([empty, empty], 1.0)) == 0
+    zeros = torch.zeros(100000, device="cuda")
+    assert float(eng.clip_grad_norm([zeros], 1.0)) == 0 and not zeros.any()
+    ones = torch.ones(10, device="cuda")
+    eng.clip_grad_norm([ones], 0.0)
+    assert not ones.any()
+    ones = torch.ones(10, device="cuda")
+    eng.clip_grad_norm([ones], float("inf"))
+    assert (ones == 1).all()
+
+
+def test_more_than_2_31_elements(eng):
+    big = torch.full((2 ** 31 + 12345,), 2.0 ** -10, device="cuda", dtype=torch.bfloat16)
+    big[-1] = 3.0
+    ref = math.sqrt((big.numel() - 1) * 2.0 ** -20 + 9.0)
+    check_norm(eng.clip_grad_norm([big], ref / 2), ref)
+    half = 2.0 ** -11 * (ref / (ref + 1e-6))
+    for at in (0, 2 ** 31 - 1, 2 ** 31, big.numel() - 2):
+        assert abs(float(big[at]) - half) <= 2.0 ** -8 * half
+    assert abs(float(big[-1]) - 1.5) <= 2.0 ** -7
