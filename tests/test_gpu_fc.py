@@ -431,6 +431,7 @@ def test_capture_and_replay(eng, lib, dtype, rows):
     assert all(torch.equal(a, b) for a, b in zip(out, want))
     del g
     # a stream that has no scratch yet: partial column sums need some, the rest runs without
+    lib.release_workspace()
     s = torch.cuda.Stream()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g, stream=s):

@@ -117,6 +117,7 @@ def test_capture_and_replay(eng, pkg):
     out = [torch.empty_like(g) for g in grads]
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
+    lib.release_workspace()                                  # (streams come from a pool: this one may have served another test)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g, stream=s):
         with pytest.raises(lib.AlphaConvError) as e:
