@@ -69,14 +69,6 @@ int make_map(CUtensorMap* m, int dtype, const void* base, long long cols, long l
     const cuuint32_t box[2] = {(cuuint32_t)in, (cuuint32_t)box_rows};
     return encode_tiled(m, dtype == ALPHA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, st, box, swz);
 }
-// Map of an output of `halves` blocks of `cols` columns a row, by which boxes of 32 x 32 elements are stored.
-int make_out_map(CUtensorMap* m, int dtype, const void* base, long long cols, int halves, long long rows)
-{
-    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)halves, (cuuint64_t)rows}, st[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * 2 * halves};
-    const cuuint32_t box[3] = {32, 1, 32};
-    return encode_tiled(m, dtype == ALPHA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, st, box, CU_TENSOR_MAP_SWIZZLE_64B);
-}
-
 struct Product {
     int dtype, rows, cols, K;        // outputs (glu: columns of a half), reduction
     bool a_mn, b_mn, glu;
@@ -141,13 +133,13 @@ FcPlan pick_plan(const Product& q, int sms)
 }
 
 template <class T, bool PAIR, bool GLU>
-void launch_mma(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& y, const CUtensorMap& z, const FcMma& p, int sms, cudaStream_t stream)
+void launch_mma(const CUtensorMap& a, const CUtensorMap& b, const FcMma& p, int sms, cudaStream_t stream)
 {
     const int group = PAIR ? 2 : p.split, total = p.m_tiles * p.n_tiles, most = sms / group;
     const unsigned grid = static_cast<unsigned>(p.split > 1 || total < most ? total : most) * group;
     const uint32_t smem = p.stages * fc_blocks(PAIR) * fc_block_bytes(PAIR, p.a_rows, p.bn) + kFcStaging + 1024 + 512;
     allow_smem<fc_mma_kernel<T, PAIR, GLU>>();
-    launch_after_clusters(fc_mma_kernel<T, PAIR, GLU>, dim3(grid), kFcThreads, group > 1 ? group : 0, smem, stream, a, b, y, z, p);
+    launch_after_clusters(fc_mma_kernel<T, PAIR, GLU>, dim3(grid), kFcThreads, group > 1 ? group : 0, smem, stream, a, b, p);
 }
 
 int launch_product(const Product& q, cudaStream_t stream)
@@ -176,18 +168,16 @@ int launch_product(const Product& q, cudaStream_t stream)
     p.tmem = tmem_columns(bn, q.glu);
     p.act = q.act; p.k = q.k; p.keep_z = q.Z != nullptr;
     p.bias = q.bias; p.residual = q.residual; p.Y = q.Y; p.Z = q.Z; p.status = status;
-    CUtensorMap a, b, y, z;
+    CUtensorMap a, b;
     const long long b_rows = q.glu ? 2LL * q.cols : q.cols;
     rc = q.a_mn ? make_map(&a, q.dtype, q.A, q.rows, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) : make_map(&a, q.dtype, q.A, q.K, q.rows, 64, p.a_rows, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = q.b_mn ? make_map(&b, q.dtype, q.B, q.cols, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
                          : make_map(&b, q.dtype, q.B, q.K, b_rows, 64, plan.pair ? 128 : out, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = make_out_map(&y, q.dtype, q.Y, q.cols, 1, q.rows);
-    if (!rc) rc = q.Z ? make_out_map(&z, q.dtype, q.Z, q.cols, q.glu ? 2 : 1, q.rows) : (z = y, ALPHA_OK);
     if (rc) return rc;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (q.glu) plan.pair ? launch_mma<T, true, true>(a, b, y, z, p, sms, stream) : launch_mma<T, false, true>(a, b, y, z, p, sms, stream);
-        else plan.pair ? launch_mma<T, true, false>(a, b, y, z, p, sms, stream) : launch_mma<T, false, false>(a, b, y, z, p, sms, stream);
+        if (q.glu) plan.pair ? launch_mma<T, true, true>(a, b, p, sms, stream) : launch_mma<T, false, true>(a, b, p, sms, stream);
+        else plan.pair ? launch_mma<T, true, false>(a, b, p, sms, stream) : launch_mma<T, false, false>(a, b, p, sms, stream);
     };
     if (q.dtype == ALPHA_BF16) go(__nv_bfloat16{});
     else go(__half{});

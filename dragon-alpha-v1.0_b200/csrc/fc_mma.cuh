@@ -25,7 +25,7 @@
 namespace alpha {
 
 constexpr int kFcThreads = 320, kFcBK = 64, kFcGroupM = 8, kFcMaxStages = 16;
-constexpr uint32_t kFcRing = 196608, kFcStaging = 8 * 4096;              // staging: two boxes of 32 x 32 elements for each epilogue warp
+constexpr uint32_t kFcRing = 196608, kFcStaging = 8 * 4096;              // staging: two buffers of 32 x 32 elements for each epilogue warp
 constexpr uint32_t kFcSmemMost = kFcRing + kFcStaging + 1024 + 512;
 
 struct FcMma {
@@ -46,8 +46,7 @@ __host__ __device__ constexpr uint32_t fc_block_bytes(bool pair, int a_rows, int
 
 template <class T, bool PAIR, bool GLU>
 __global__ void __launch_bounds__(kFcThreads, 1)
-    fc_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
-                  const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ FcMma p)
+    fc_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ FcMma p)
 {
     constexpr int CTAS = PAIR ? 2 : 1, KB = fc_blocks(PAIR);
     const int BN = PAIR ? 256 : p.bn, OUT = GLU ? BN / 2 : BN, S = PAIR ? 6 : p.stages, split = PAIR ? 1 : p.split;
@@ -65,8 +64,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         for (int i = 0; i < S; ++i) { mbar_init(&bars[i], 1); mbar_init(&bars[kFcMaxStages + i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&bars[2 * kFcMaxStages + i], 1); mbar_init(&bars[2 * kFcMaxStages + 2 + i], 8 * CTAS); }
         fence_barrier_init();
-        prefetch_tmap(&tmA); prefetch_tmap(&tmB); prefetch_tmap(&tmY);
-        if (p.keep_z) prefetch_tmap(&tmZ);
+        prefetch_tmap(&tmA); prefetch_tmap(&tmB);
     }
     if (warp == 1) {
         if constexpr (PAIR) { tmem_alloc_pair(tmem_holder, 512); tmem_relinquish_pair(); }
@@ -94,66 +92,90 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     const uint32_t stage_a = smem_a + S * kStage + (warp - 2) * 4096;
     uint32_t sbuf = 0;
     bool ok = true;
-    // A lane's 32 columns leave through shared memory as a box of 32 rows x 64 bytes; of a last chunk of fewer columns, which a box would
-    // pass, in words of eight.
-    auto put = [&](const float (&f)[32], T* tensor, size_t pitch, int row, int col0, int width, auto&& store) {
-        if (PAIR || width >= 32) {
-            if (lane == 0) tma_store_wait_read<1>();
-            __syncwarp();
-            const uint32_t buf = stage_a + sbuf * 2048;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint4 w = Word16<T>::store(f + 8 * q);
-                st_shared_v4(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)));
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) { store(buf); tma_store_commit(); }
-            sbuf ^= 1u;
-        } else if (row < p.rows) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (8 * q < width && col0 + 8 * q < p.cols) *reinterpret_cast<uint4*>(tensor + static_cast<size_t>(row) * pitch + col0 + 8 * q) = Word16<T>::store(f + 8 * q);
-        }
+    // A warp's 32 rows x 32 columns change hands in shared memory between lanes that hold a row (the accumulator's layout) and lanes that hold 16 bytes of
+    // row 8 j + lane / 4, eight rows of 64 bytes to an instruction, as global memory is read and written.  Two buffers in turn, so that one barrier of the
+    // warp serves each.  (By TMA stores, with their fence and the wait for the buffer, 7966 x 64 x 8136 with silu
+    // and R took 182 us, with what follows 87.)
+    const uint32_t row_at = stage_a + lane * 64, word_at = stage_a + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+    auto row_word = [&](int q) { return row_at + sbuf * 2048 + ((q ^ ((lane >> 1) & 3)) << 4); };
+    // word j of a lane lies 8 rows further: the swizzle is that of its row
+    auto lane_word = [&](int j) { return word_at + sbuf * 2048 + j * 512; };
+    auto inside = [&](int row0, int col0, int width, int j) {
+        const int c = 8 * (lane & 3);
+        return row0 + 8 * j + (lane >> 2) < p.rows && c < width && col0 + c < p.cols;
     };
-    // f += 32 columns of a vector or a row (its width a multiple of 8; R may be Y itself, so not by the read-only path)
-    auto add = [&](float (&f)[32], const T* from, int col0) {
+    auto put = [&](const float (&f)[32], T* tensor, size_t pitch, int row0, int col0, int width) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint4 w = Word16<T>::store(f + 8 * q);
+            st_shared_v4(row_word(q), make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)));
+        }
+        __syncwarp();
+        T* to = tensor + static_cast<size_t>(row0 + (lane >> 2)) * pitch + col0 + 8 * (lane & 3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j, to += 8 * pitch) {
+            const float4 w = ld_shared_v4(lane_word(j));
+            if (inside(row0, col0, width, j)) *reinterpret_cast<float4*>(to) = w;
+        }
+        sbuf ^= 1u;
+    };
+    // The words of R that put() will write over, or zeros (R may be Y itself: not by the read-only path).
+    auto fetch = [&](uint4 (&r)[4], int row0, int col0, int width) {
+        const T* from = static_cast<const T*>(p.residual) + static_cast<size_t>(row0 + (lane >> 2)) * p.cols + col0 + 8 * (lane & 3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j, from += 8 * p.cols) r[j] = inside(row0, col0, width, j) ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+    };
+    auto add_fetched = [&](float (&f)[32], const uint4 (&r)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            st_shared_v4(lane_word(j), make_float4(__uint_as_float(r[j].x), __uint_as_float(r[j].y), __uint_as_float(r[j].z), __uint_as_float(r[j].w)));
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 w = ld_shared_v4(row_word(q));
+            float b[8];
+            Word16<T>::load(make_uint4(__float_as_uint(w.x), __float_as_uint(w.y), __float_as_uint(w.z), __float_as_uint(w.w)), b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[8 * q + i] += b[i];
+        }
+        sbuf ^= 1u;
+    };
+    // f += 32 columns of the bias (its length a multiple of 8)
+    auto add_bias = [&](float (&f)[32], const T* from, int col0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             if (col0 + 8 * q < p.cols) {
                 float b[8];
-                Word16<T>::load(*reinterpret_cast<const uint4*>(from + col0 + 8 * q), b);
+                Word16<T>::load(__ldg(reinterpret_cast<const uint4*>(from + col0 + 8 * q)), b);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[8 * q + i] += b[i];
             }
     };
-    // The epilogue of 32 rows x (up to) 32 columns: the sums of a lane's row in z (glu: and u).
-    auto finish = [&](float (&z)[32], float (&u)[32], int row0, int col0, int width) {
+    // The epilogue of 32 rows x (up to) 32 columns: the sums of a lane's row in z (glu: and u), the words of R in r.
+    auto finish = [&](float (&z)[32], float (&u)[32], const uint4 (&r)[4], int row0, int col0, int width) {
         const T* bias = static_cast<const T*>(p.bias);
-        const T* residual = static_cast<const T*>(p.residual);
         T *Y = static_cast<T*>(p.Y), *Z = static_cast<T*>(p.Z);
-        const int row = row0 + lane;
         if constexpr (GLU) {
-            if (bias) { add(z, bias, col0); add(u, bias + p.cols, col0); }
+            if (bias) { add_bias(z, bias, col0); add_bias(u, bias + p.cols, col0); }
             if (p.keep_z) {
                 const size_t pitch = 2 * static_cast<size_t>(p.cols);
-                put(z, Z, pitch, row, col0, width, [&](uint32_t buf) { tma_store_3d_a(&tmZ, buf, col0, 0, row0); });
-                put(u, Z + p.cols, pitch, row, col0, width, [&](uint32_t buf) { tma_store_3d_a(&tmZ, buf, col0, 1, row0); });
+                put(z, Z, pitch, row0, col0, width);
+                put(u, Z + p.cols, pitch, row0, col0, width);
             }
             with_act(p.act, [&](auto a) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, true>(z[i], p.k) * u[i];
             });
         } else {
-            if (bias) add(z, bias, col0);
-            if (p.keep_z) put(z, Z, p.cols, row, col0, width, [&](uint32_t buf) { tma_store_3d_a(&tmZ, buf, col0, 0, row0); });
+            if (bias) add_bias(z, bias, col0);
+            if (p.keep_z) put(z, Z, p.cols, row0, col0, width);
             with_act(p.act, [&](auto a) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, true>(z[i], p.k);
             });
-            if (residual && row < p.rows) add(z, residual + static_cast<size_t>(row) * p.cols, col0);
+            if (p.residual) add_fetched(z, r);
         }
-        put(z, Y, p.cols, row, col0, width, [&](uint32_t buf) { tma_store_3d_a(&tmY, buf, col0, 0, row0); });
+        put(z, Y, p.cols, row0, col0, width);
     };
 
     // Both issuing warps walk their loops as a whole, so that counters, coordinates and descriptors are uniform values; one lane issues.
@@ -258,11 +280,33 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         for (int t = first; t < total; t += step) {
             int m0, n0;
             tile_at(t, m0, n0);
+            const int row0 = m0 + quad * 32;
+            // R: the next tile's to L2, and the first chunk of this one before the sums are there (8192 x 64 x 8192 with R 90 us without the former)
+            uint4 r[4] = {};
+            const bool fetching = !GLU && p.residual && row0 < p.rows && (PAIR || split == 1);
+            if (!GLU && p.residual && (PAIR || split == 1)) {
+                int m1, n1;
+                tile_at(t + step < total ? t + step : t, m1, n1);
+                const int row = m1 + quad * 32 + lane;
+                for (int c = half * 32; c < OUT; c += 64)
+                    if (row < p.rows && n1 + c < p.cols) prefetch_l2(static_cast<const T*>(p.residual) + static_cast<size_t>(row) * p.cols + n1 + c);
+            }
+            if (fetching) fetch(r, row0, n0 + half * 32, OUT - half * 32);
             ok = mbar_wait_a(afull_a + 8 * ap.idx, ap.phase);
             if (!ok) { report(p.status, kStatusEpilogueTimeout); settle(); break; }
             tc_fence_after_sync();
             const uint32_t d = lanes + ap.idx * acc_pitch;
-            const int row0 = m0 + quad * 32;
+            // The accumulator is given back when its last columns are in registers, before they are stored; the arrival orders no memory (a release
+            // across the pair waited for the tile's stores: 7592 x 24 x 2 x 3968 45 us instead of 35).
+            auto give_back = [&] {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_cluster_relaxed(aempty_L + 8 * ap.idx);
+                    else mbar_arrive_relaxed_a(aempty_L + 8 * ap.idx);
+                }
+            };
+            bool held = true;
             if (row0 < p.rows) {
                 if (!PAIR && split > 1) {
                     // the ring is idle: [row][column] with four floats more, so that the words of eight rows lie in different banks
@@ -283,16 +327,13 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                         float z[32], u[32];
                         load32(d + c, z);
                         if constexpr (GLU) load32(d + OUT + c, u);
-                        finish(z, u, row0, n0 + c, OUT - c);
+                        if (c + 64 >= OUT || n0 + c + 64 >= p.cols) { give_back(); held = false; }
+                        finish(z, u, r, row0, n0 + c, OUT - c);
+                        if (fetching && c + 64 < OUT) fetch(r, row0, n0 + c + 64, OUT - c - 64);
                     }
                 }
             }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (PAIR) mbar_arrive_cluster(aempty_L + 8 * ap.idx);
-                else mbar_arrive_a(aempty_L + 8 * ap.idx);
-            }
+            if (held) give_back();
             ap.advance(2);
         }
     }
@@ -325,11 +366,12 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                             }
                         }
                     }
-                finish(z, u, row0, n0 + c, OUT - c);
+                uint4 r[4] = {};
+                if (!GLU && p.residual) fetch(r, row0, n0 + c, OUT - c);
+                finish(z, u, r, row0, n0 + c, OUT - c);
             }
         }
     }
-    if (warp >= 2 && lane == 0) tma_store_wait_all();
     tc_fence_before_sync();
     __syncthreads();
     if (PAIR || split > 1) cluster_sync_all();   // no CTA leaves while another may still reach its shared memory

@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         auto release = [&](uint32_t bar) {
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(bar);
+            if (lane == 0) mbar_arrive_cluster_relaxed(bar);
         };
         // 32 columns of a lane's row leave as a box of 32 rows x 128 bytes
         auto put = [&](const float (&f)[32], auto&& store) {

@@ -421,7 +421,8 @@ def _fc_pack(dtype, *jobs):
 
 @functools.lru_cache(maxsize=512)
 def _fc_plan(what, glu, xs, ws, dtype):
-    """Sizes of a FullConnect call on X of shape xs and W of shape ws: IC, OC, padded IC and OC, rows, halves of W, shapes of Y and Z."""
+    """Sizes of a FullConnect call on X of shape xs and W of shape ws: IC, OC, padded IC and OC, rows, halves of W, shapes of Y, Z and a
+    bias."""
     if dtype not in _FC_TYPES:
         raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, dtype))
     if len(xs) < 1 or len(ws) != 2 or ws[1] != xs[-1]:
@@ -435,21 +436,24 @@ def _fc_plan(what, glu, xs, ws, dtype):
     rows, unit = 1, 4 if dtype == torch.float32 else 8
     for n in lead:
         rows *= n
-    return IC, OC, -(-IC // unit) * unit, -(-OC // unit) * unit, rows, halves, lead + (OC,), lead + (halves * OC,)
+    return IC, OC, -(-IC // unit) * unit, -(-OC // unit) * unit, rows, halves, lead + (OC,), lead + (halves * OC,), (halves * OC,)
 
 
 def _fc_check(what, X, W, others):
-    """The tensors of a call are of X's type and on its GPU, and of the shapes expected: (name, tensor or None, shape) each."""
+    """The tensors of a call are of X's type and on its GPU, and of the shapes expected: (name, tensor or None, shape) each.  Returns the GPU."""
     dtype, device = X.dtype, X.get_device()
     if device < 0:
         raise ValueError("%s: tensors must be on a GPU" % what)
-    for name, t, shape in (("W", W, None),) + others:
+    if W.dtype != dtype or W.get_device() != device:
+        others += (("W", W, W.shape),)
+    for name, t, shape in others:
         if t is None:
             continue
-        if shape is not None and t.shape != shape:
+        if t.shape != shape:
             raise ValueError("%s: %s %s, expected %s" % (what, name, tuple(t.shape), shape))
         if t.dtype != dtype or t.get_device() != device:
             raise ValueError("%s: %s is %s on %s, X %s on %s" % (what, name, t.dtype, t.device, dtype, X.device))
+    return device
 
 
 def _fc_act(what, act):
@@ -638,53 +642,64 @@ class Engine:
     # gradients.  float32, bfloat16 or float16 tensors (all of one type); X may have any leading dimensions; IC and OC that are no
     # multiples of 16 bytes are zero-padded as everywhere. ----
     def _fc_forward(self, what, X, W, Bias, act, k, Residual, save, glu):
-        dtype = X.dtype
-        IC, OC, ic, oc, rows, halves, ys, zs = _fc_plan(what, glu, X.shape, W.shape, dtype)
+        plan = _fc_plan(what, glu, X.shape, W.shape, X.dtype)
         code = _fc_act(what, act)
-        _fc_check(what, X, W, (("Bias", Bias, (halves * OC,)), ("Residual", Residual, ys)))
+        device = _fc_check(what, X, W, (("Bias", Bias, plan[8]), ("Residual", Residual, plan[6])) if Bias is not None or Residual is not None else ())
+        if self.base._stream is None and device == torch._C._cuda_getDevice():
+            return self._fc_run(X, W, Bias, code, k, Residual, save, glu, plan)
         with self._on(X):
-            if rows == 0:
-                return (X.new_empty(ys), X.new_empty(zs)) if save else X.new_empty(ys)
-            (Xp, Wp, Bp, Rp), _held = _fc_pack(dtype, (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic), (Bias, 1, halves, OC, halves, oc),
-                                               (Residual, 1, rows, OC, rows, oc))
-            even = oc == OC
-            Y = X.new_empty(ys if even else (rows, oc))
-            Z = X.new_empty(zs if even else (rows, halves * oc)) if save else None
-            if glu:
-                self.base.fullConnect_glu(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Z)
-            else:
-                self.base.fullConnect(Y, Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Rp, Z)
-            if not even:
-                Y = Y.narrow(1, 0, OC)
-                if len(ys) != 2:
-                    Y = Y.reshape(ys)
-                if save:
-                    Z = Z.reshape(rows, halves, oc)[:, :, :OC].reshape(zs)
+            return self._fc_run(X, W, Bias, code, k, Residual, save, glu, plan)
+
+    def _fc_run(self, X, W, Bias, code, k, Residual, save, glu, plan):
+        IC, OC, ic, oc, rows, halves, ys, zs, _ = plan
+        dtype = X.dtype
+        if rows == 0:
+            return (X.new_empty(ys), X.new_empty(zs)) if save else X.new_empty(ys)
+        (Xp, Wp, Bp, Rp), _held = _fc_pack(dtype, (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic), (Bias, 1, halves, OC, halves, oc), (Residual, 1, rows, OC, rows, oc))
+        even = oc == OC
+        Y = X.new_empty(ys if even else (rows, oc))
+        Z = X.new_empty(zs if even else (rows, halves * oc)) if save else None
+        if glu:
+            self.base.fullConnect_glu(Y.data_ptr(), Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Z)
+        else:
+            self.base.fullConnect(Y.data_ptr(), Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Rp, Z)
+        if not even:
+            Y = Y.narrow(1, 0, OC)
+            if len(ys) != 2:
+                Y = Y.reshape(ys)
+            if save:
+                Z = Z.reshape(rows, halves, oc)[:, :, :OC].reshape(zs)
         return (Y, Z) if save else Y
 
     def _fc_delta(self, what, deltaY, X, W, Z, act, k, bias, glu):
-        dtype = X.dtype
-        IC, OC, ic, oc, rows, halves, ys, zs = _fc_plan(what, glu, X.shape, W.shape, dtype)
+        plan = _fc_plan(what, glu, X.shape, W.shape, X.dtype)
         code = _fc_act(what, act)
-        _fc_check(what, X, W, (("deltaY", deltaY, ys), ("Z", Z, zs)))
-        through = glu or act != "none"
-        if through and Z is None:
+        device = _fc_check(what, X, W, (("deltaY", deltaY, plan[6]), ("Z", Z, plan[7])))
+        if Z is None and (glu or act != "none"):
             raise ValueError("%s: Z of the forward pass is needed" % what)
+        if self.base._stream is None and device == torch._C._cuda_getDevice():
+            return self._fc_run_delta(deltaY, X, W, Z, code, k, bias, glu, plan)
         with self._on(X):
-            if rows == 0:
-                return X.new_empty(X.shape), W.new_zeros(W.shape), W.new_zeros((halves * OC,)) if bias else None
-            (dYp, Xp, Wp, Zp), _held = _fc_pack(dtype, (deltaY, 1, rows, OC, rows, oc), (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic),
-                                                (Z if through else None, 1, rows * halves, OC, rows * halves, oc))
-            dZ = X.new_empty((rows, halves * oc)) if through else None
-            dX, dW = X.new_empty((rows, ic)), W.new_empty((halves, oc, ic))
-            dB = W.new_empty((halves, oc)) if bias else None
-            self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, oc, _FC_TYPES[dtype], code, k, glu)
-            if ic != IC:
-                dX = dX.narrow(1, 0, IC)
-            if ic != IC or oc != OC:
-                dW = dW[:, :OC, :IC]
-                dB = dB[:, :OC] if bias else None
-            return dX if X.dim() == 2 else dX.reshape(X.shape), dW.reshape(W.shape), dB.reshape(halves * OC) if bias else None
+            return self._fc_run_delta(deltaY, X, W, Z, code, k, bias, glu, plan)
+
+    def _fc_run_delta(self, deltaY, X, W, Z, code, k, bias, glu, plan):
+        IC, OC, ic, oc, rows, halves, _, _, _ = plan
+        dtype = X.dtype
+        if rows == 0:
+            return X.new_empty(X.shape), W.new_zeros(W.shape), W.new_zeros((halves * OC,)) if bias else None
+        through = glu or code != 0
+        (dYp, Xp, Wp, Zp), _held = _fc_pack(dtype, (deltaY, 1, rows, OC, rows, oc), (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic),
+                                            (Z if through else None, 1, rows * halves, OC, rows * halves, oc))
+        dZ = X.new_empty((rows, halves * oc)) if through else None
+        dX, dW = X.new_empty((rows, ic)), W.new_empty((halves, oc, ic))
+        dB = W.new_empty((halves, oc)) if bias else None
+        self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, oc, _FC_TYPES[dtype], code, k, glu)
+        if ic != IC:
+            dX = dX.narrow(1, 0, IC)
+        if ic != IC or oc != OC:
+            dW = dW[:, :OC, :IC]
+            dB = dB[:, :OC] if bias else None
+        return dX if X.dim() == 2 else dX.reshape(X.shape), dW.reshape(W.shape), dB.reshape(halves * OC) if bias else None
 
     def fullConnect(self, X, W, Bias=None, act="none", k=0.0, Residual=None, save=False):
         """act(X W^T + Bias) + Residual in one pass; W [OC, IC], X [..., IC].  act: 'none', 'leakyRelu' (slope k; relu k = 0),
