@@ -14,6 +14,8 @@ using namespace alpha;
 namespace {
 
 size_t type_bytes(int dtype) { return dtype == ALPHA_F32 ? 4 : 2; }
+// Columns from one row (half) to the next of tensors that are OC wide.
+int fc_pitch(int OC) { return (OC + 7) / 8 * 8; }
 
 struct Span { const void* ptr; size_t bytes; };
 bool overlap(const Span& a, const Span& b)
@@ -44,9 +46,8 @@ int check_fc(const char* what, const AlphaFcShape* s, bool glu)
     if (s->act < ALPHA_ACT_NONE || s->act > ALPHA_ACT_GELU_TANH) return fail(ALPHA_E_ARG, "%s: unknown activation %d", what, s->act);
     if (s->act == ALPHA_ACT_LEAKY_RELU && !(s->k == s->k)) return fail(ALPHA_E_ARG, "%s: slope is NaN", what);
     const int unit = s->dtype == ALPHA_F32 ? 4 : 8;
-    if (s->IC % unit || s->OC % unit)
-        return fail(ALPHA_E_ARG, "%s: IC=%d and OC=%d must be multiples of %d (rows of 16-byte words)", what, s->IC, s->OC, unit);
-    const long long wide = glu ? 2LL * s->OC : s->OC, most = 2147483647LL;
+    if (s->IC % unit) return fail(ALPHA_E_ARG, "%s: IC=%d must be a multiple of %d (rows of 16-byte words)", what, s->IC, unit);
+    const long long wide = (glu ? 2LL : 1LL) * (((long long)s->OC + 7) / 8 * 8), most = 2147483647LL;
     if (wide > most) return fail(ALPHA_E_ARG, "%s: more than 2^31-1 rows of W", what);
     // the fp32 kernels address a tensor's elements with 32 bits
     if (s->dtype == ALPHA_F32 && ((long long)s->rows * s->IC > most || wide * s->IC > most || s->rows * wide > most))
@@ -62,17 +63,23 @@ int launched(const char* what)
 
 // ---- 16-bit products --------------------------------------------------------------------------------------------
 
-// Map of a row-major matrix of 16-bit elements, box of `in` columns x `rows` rows.
-int make_map(CUtensorMap* m, int dtype, const void* base, long long cols, long long rows, int in, int box_rows, CUtensorMapSwizzle swz)
+// An operand as three dimensions, innermost first, with the strides of the outer two (elements).
+struct Operand { const void* ptr; bool mn; long long d0, d1, d2, s1, s2; };
+
+int make_map(CUtensorMap* m, int dtype, const Operand& o, int b0, int b1, int b2)
 {
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, st[1] = {(cuuint64_t)cols * 2};
-    const cuuint32_t box[2] = {(cuuint32_t)in, (cuuint32_t)box_rows};
-    return encode_tiled(m, dtype == ALPHA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, st, box, swz);
+    const cuuint64_t dims[3] = {(cuuint64_t)o.d0, (cuuint64_t)o.d1, (cuuint64_t)o.d2}, st[2] = {(cuuint64_t)o.s1 * 2, (cuuint64_t)o.s2 * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)b0, (cuuint32_t)b1, (cuuint32_t)b2};
+    return encode_tiled(m, dtype == ALPHA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, o.ptr, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
+
+// rows x cols outputs (glu: cols of a half; rows of each of m_halves halves) over k_halves halves of K steps.
+// A: (step, half, row), or (row, half, step) where it runs along its rows (mn); B: (step, column, half) or (column, step, half).
 struct Product {
-    int dtype, rows, cols, K;        // outputs (glu: columns of a half), reduction
-    bool a_mn, b_mn, glu;
-    const void *A, *B, *bias, *residual;
+    int dtype, rows, cols, pitch, K, m_halves, k_halves;
+    bool glu;
+    Operand A, B;
+    const void *bias, *residual;
     void *Z, *Y;
     int act; float k;
 };
@@ -98,24 +105,24 @@ uint32_t tmem_columns(int bn, bool glu)
 FcPlan pick_plan(const Product& q, int sms)
 {
     const int forced = option_fc_tile() == 2 ? 0 : option_fc_tile();
-    const long long cols = q.glu ? 2LL * q.cols : q.cols, blocks = (q.K + kFcBK - 1) / kFcBK, stages = (blocks + 1) / 2;
+    const long long cols = q.glu ? 2LL * q.cols : q.cols, blocks = (long long)q.k_halves * ((q.K + kFcBK - 1) / kFcBK), stages = (blocks + 1) / 2;
     FcPlan best{false, 64, 1};
     double least = 1e300;
     auto look = [&](bool pair, int bn, int split) {
         const int out = q.glu ? bn / 2 : bn, bm = pair ? 256 : 128, ctas = pair ? 2 : 1;
-        const long long tiles = (long long)((q.rows + bm - 1) / bm) * ((q.cols + out - 1) / out), most = sms / (ctas * split);
+        const long long tiles = (long long)q.m_halves * ((q.rows + bm - 1) / bm) * ((q.cols + out - 1) / out), most = sms / (ctas * split);
         if (most < 1 || (split > 1 && tiles > most)) return;
         const long long waves = (tiles + most - 1) / most, each = (blocks + split - 1) / split;
         const double step = pair ? 0.285 : 0.1375;
-        const double l2 = (double)tiles * blocks * (pair ? 512 : (q.a_mn || q.rows >= 128 ? 128 : q.rows) + bn) * 128 / 18e6;
-        const double mma = waves * each * step, dram = 2e-6 * ((double)q.rows + cols) * q.K / 5.2;
+        const double l2 = (double)tiles * blocks * (pair ? 512 : (q.A.mn || q.rows >= 128 ? 128 : q.rows) + bn) * 128 / 18e6;
+        const double mma = waves * each * step, dram = 2e-6 * ((double)q.rows * q.m_halves + cols) * q.K * q.k_halves / 5.2;
         const double most_of = mma > l2 ? (mma > dram ? mma : dram) : (l2 > dram ? l2 : dram);
         double time = 0.8 * most_of + 0.2 * (mma + l2 + dram);                // (the others are not quite hidden)
         time += (pair ? 5.7 : 4.0 + 0.006 * bn) + (split == 1 ? 0.0 : split == 2 ? 2.5 : split == 4 ? 4.0 : 12.0);
         if (time < least) { least = time; best = FcPlan{pair, bn, split}; }
     };
     // (an operand that runs along its rows comes in boxes of 64 of them; no part of a shared tile is empty)
-    const int unit = q.b_mn ? 64 : 16;
+    const int unit = q.B.mn ? 64 : 16;
     auto parts = [&](int split) { return split == 1 || (split - 1) * ((stages + split - 1) / split) < stages; };
     if (forced == 1 && sms >= 2) return FcPlan{true, 256, 1};
     if (forced >= 1000) {
@@ -151,28 +158,29 @@ int launch_product(const Product& q, cudaStream_t stream)
     const FcPlan plan = pick_plan(q, sms);
     const int bm = plan.pair ? 256 : 128, bn = plan.bn, out = q.glu ? bn / 2 : bn, steps = kFcBK * fc_blocks(plan.pair);
     FcMma p{};
-    p.rows = q.rows; p.cols = q.cols;
-    p.m_tiles = (q.rows + bm - 1) / bm; p.n_tiles = (q.cols + out - 1) / out; p.kb = (q.K + steps - 1) / steps;
-    if ((long long)p.m_tiles * p.n_tiles > 2147483647LL / kFcGroupM) return fail(ALPHA_E_ARG, "fullConnect: more tiles than a launch takes");
+    p.rows = q.rows; p.cols = q.pitch;
+    const int k_blocks = (q.K + kFcBK - 1) / kFcBK;
+    p.m_half = (q.rows + bm - 1) / bm; p.n_tiles = (q.cols + out - 1) / out;
+    p.k_half = q.k_halves > 1 ? k_blocks : 1 << 29;
+    p.kb = static_cast<int>(((long long)k_blocks * q.k_halves * kFcBK + steps - 1) / steps);
+    if ((long long)p.m_half * q.m_halves * p.n_tiles > 2147483647LL / kFcGroupM) return fail(ALPHA_E_ARG, "fullConnect: more tiles than a launch takes");
+    p.m_tiles = p.m_half * q.m_halves;
     p.bn = bn; p.split = plan.split;
-    p.a_mn = q.a_mn; p.b_mn = q.b_mn;
-    p.a_rows = plan.pair || q.a_mn || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
+    p.a_mn = q.A.mn; p.b_mn = q.B.mn;
+    p.a_rows = plan.pair || q.A.mn || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
     const uint32_t stage = fc_blocks(plan.pair) * fc_block_bytes(plan.pair, p.a_rows, bn);
     p.stages = kFcRing / stage < kFcMaxStages ? kFcRing / stage : kFcMaxStages;
     // shared tiles: the ring holds a part's sums afterwards
     const uint32_t sums = (q.rows < 128 ? q.rows : 128) * (bn + 4) * 4;
     while (p.split > 1 && p.stages * stage < sums && (p.stages + 1) * stage <= kFcRing) ++p.stages;
     if (p.split > 1 && p.stages * stage < sums) return fail(ALPHA_E_ARG, "fullConnect: no plan");
-    p.b_up = q.cols;
-    p.idesc = q.dtype == ALPHA_BF16 ? make_idesc_bf16(bm, bn, q.a_mn, q.b_mn) : make_idesc_f16(bm, bn, q.a_mn, q.b_mn);
+    p.idesc = q.dtype == ALPHA_BF16 ? make_idesc_bf16(bm, bn, q.A.mn, q.B.mn) : make_idesc_f16(bm, bn, q.A.mn, q.B.mn);
     p.tmem = tmem_columns(bn, q.glu);
     p.act = q.act; p.k = q.k; p.keep_z = q.Z != nullptr;
     p.bias = q.bias; p.residual = q.residual; p.Y = q.Y; p.Z = q.Z; p.status = status;
     CUtensorMap a, b;
-    const long long b_rows = q.glu ? 2LL * q.cols : q.cols;
-    rc = q.a_mn ? make_map(&a, q.dtype, q.A, q.rows, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) : make_map(&a, q.dtype, q.A, q.K, q.rows, 64, p.a_rows, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = q.b_mn ? make_map(&b, q.dtype, q.B, q.cols, q.K, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
-                         : make_map(&b, q.dtype, q.B, q.K, b_rows, 64, plan.pair ? 128 : out, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = q.A.mn ? make_map(&a, q.dtype, q.A, 64, 1, 64) : make_map(&a, q.dtype, q.A, 64, 1, p.a_rows);
+    if (!rc) rc = q.B.mn ? make_map(&b, q.dtype, q.B, 64, 64, 1) : make_map(&b, q.dtype, q.B, 64, plan.pair ? 128 : out, 1);
     if (rc) return rc;
     auto go = [&](auto t) {
         using T = decltype(t);
@@ -198,8 +206,8 @@ int launch_parts(const float* part, size_t size, int parts, int rows, const FcEp
     return launched("fc_parts_kernel");
 }
 
-// A product of fp32 matrices: rows x cols outputs (glu: cols of both halves), K steps; `form` says which operand runs along the reduction.
-struct ProductF32 { const float *A, *B; int rows, cols, K, lda, ldb; FcEpilogue e; };
+// A product of fp32 matrices as PlaneFc forms it: rows x cols sums over K steps (padding of both halves of Z among rows, columns or steps).
+struct ProductF32 { const float *A, *B; int rows, cols, K, OC, pitch, halves, lda, ldb; FcEpilogue e; };
 
 // Planes of a matrix in scratch: [plane][row][pitch], pitch in bf16 elements.
 struct Planes { void* ptr = nullptr; const float* src = nullptr; int rows = 0, cols = 0, pitch = 0; };
@@ -222,12 +230,12 @@ int launch_split(const Planes* const* list, int n, int sms, cudaStream_t stream)
 // Parts of the reduction on CTA pairs and the time of that product (us): a window of 64 steps of a tile 2.26, an item 2, a launch 5; the parts
 // written and read.  (Estimated / measured, with the split: 2048 x 2048 x 2048 92 / 88, 4096 x 1024 x 4096 170 / 174, 512 x 4096 x 1000 44 / 40.)
 struct PairPlan { int parts; double time; };
-PairPlan pick_pair(int rows, int out_cols, bool glu, int K, int sms)
+PairPlan pick_pair(int rows, int m_halves, int out_cols, bool glu, int K, int k_halves, int sms)
 {
-    const int pairs = sms / 2, out = glu ? 128 : 256, windows = (K + 63) / 64;
+    const int pairs = sms / 2, out = glu ? 128 : 256, windows = k_halves * ((K + 63) / 64);
     PairPlan best{1, 1e300};
     if (pairs < 1) return best;
-    const double tiles = static_cast<double>((rows + 255) / 256) * ((out_cols + out - 1) / out), size = static_cast<double>(rows) * out_cols * (glu ? 2 : 1);
+    const double tiles = static_cast<double>(m_halves) * ((rows + 255) / 256) * ((out_cols + out - 1) / out), size = static_cast<double>(rows) * m_halves * out_cols * (glu ? 2 : 1);
     for (int parts = 1; parts <= 32 && parts <= windows; ++parts) {
         const int each = (windows + parts - 1) / parts;
         if ((parts - 1) * each >= windows) continue;                      // (no part is empty)
@@ -243,35 +251,52 @@ template <int FORM>
 int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, int parts, void* part, int sms, int* status, cudaStream_t stream)
 {
     constexpr bool GLU = FORM == kFcGlu, A_MN = FORM == kFcDeltaW, B_MN = FORM == kFcDeltaX || FORM == kFcDeltaW;
-    const int cols = GLU ? q.cols / 2 : q.cols, out = GLU ? 128 : 256, halves = GLU ? 2 : 1;
+    const bool forward = FORM == kFcForward || FORM == kFcGlu;
+    const int out = GLU ? 128 : 256, m_halves = A_MN ? q.halves : 1, k_halves = FORM == kFcDeltaX ? q.halves : 1;
+    const int cols = forward ? q.OC : q.cols, steps = FORM == kFcDeltaX ? q.OC : q.K;
     PairF32 p{};
-    p.rows = q.rows; p.cols = cols; p.K = q.K;
-    p.m_tiles = (q.rows + 255) / 256; p.n_tiles = (cols + out - 1) / out; p.windows = (q.K + 63) / 64; p.parts = parts;
-    p.a_mn = A_MN; p.b_mn = B_MN; p.b_up = cols;
+    p.rows = A_MN ? q.OC : q.rows; p.cols = cols; p.pitch = q.e.cols; p.K = steps;
+    p.m_half = (p.rows + 255) / 256; p.m_tiles = p.m_half * m_halves; p.n_tiles = (cols + out - 1) / out;
+    const int windows = (steps + 63) / 64;
+    p.w_half = k_halves > 1 ? windows : 1 << 29; p.windows = windows * k_halves; p.parts = parts;
+    p.a_mn = A_MN; p.b_mn = B_MN;
     p.idesc = make_idesc_bf16(256, 256, A_MN, B_MN);
     p.A = q.A; p.B = q.B;
-    p.a_row = A_MN ? 1 : q.lda; p.a_k = A_MN ? q.lda : 1;
-    p.b_col = B_MN ? 1 : q.ldb; p.b_k = B_MN ? q.ldb : 1;
+    p.a_row = A_MN ? 1 : q.lda; p.a_k = A_MN ? q.lda : 1; p.a_half = q.pitch;
+    p.b_col = B_MN ? 1 : q.ldb; p.b_k = B_MN ? q.ldb : 1; p.b_half = static_cast<long long>(q.OC) * q.ldb;
     p.bias = q.e.bias; p.residual = q.e.residual; p.act = q.e.act; p.k = q.e.k; p.keep_z = parts == 1 && q.e.Z;
     p.status = status;
-    const size_t size = static_cast<size_t>(q.rows) * q.cols;
+    // sums and results: (column, half of the columns or rows, row, part)
+    const int out_pitch = forward ? q.pitch : q.cols;
+    const size_t size = static_cast<size_t>(p.rows) * m_halves * out_pitch * (GLU ? 2 : 1);
     void* ws = parts > 1 ? part : q.e.Y;
-    auto map = [](CUtensorMap* m, const Planes& s, bool mn) {
-        const cuuint64_t dims[3] = {(cuuint64_t)s.pitch, (cuuint64_t)s.rows, 3}, st[2] = {(cuuint64_t)s.pitch * 2, (cuuint64_t)s.pitch * 2 * s.rows};
-        const cuuint32_t box[3] = {64, mn ? 64u : 128u, 1};
-        return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, s.ptr, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    // operands: (step, half, row, plane) or (row, half, step, plane) for A; (step, column, half, plane) or (column, step, half, plane) for B
+    auto map = [](CUtensorMap* m, const Planes& s, long long d0, long long d1, long long d2, long long s1, long long s2, int b1, int b2) {
+        const cuuint64_t dims[4] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2, 3}, st[3] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2, (cuuint64_t)s.pitch * 2 * s.rows};
+        const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1};
+        return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, s.ptr, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    auto out_map = [&](CUtensorMap* m, const void* base, int h, int copies) {
-        const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)h, (cuuint64_t)q.rows, (cuuint64_t)copies};
-        const cuuint64_t st[3] = {(cuuint64_t)cols * 4, (cuuint64_t)cols * 4 * h, (cuuint64_t)cols * 4 * h * q.rows};
+    auto out_map = [&](CUtensorMap* m, const void* base, int h, bool by_rows, int copies) {
+        const long long row = by_rows ? out_pitch : static_cast<long long>(out_pitch) * h, half = by_rows ? static_cast<long long>(out_pitch) * p.rows : out_pitch;
+        const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)h, (cuuint64_t)p.rows, (cuuint64_t)copies}, st[3] = {(cuuint64_t)half * 4, (cuuint64_t)row * 4, (cuuint64_t)out_pitch * 4 * h * p.rows};
         const cuuint32_t box[4] = {32, 1, 32, 1};
         return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
     CUtensorMap a, b, y, z;
-    int rc = map(&a, A, A_MN);
-    if (!rc) rc = map(&b, B, B_MN);
-    if (!rc) rc = out_map(&y, ws, parts > 1 ? halves : 1, parts);
-    if (!rc) rc = p.keep_z ? out_map(&z, q.e.Z, halves, 1) : (z = y, ALPHA_OK);
+    const long long OC = q.OC, pa = A.pitch, pb = B.pitch;
+    int rc;
+    if constexpr (FORM == kFcDeltaX) {
+        rc = map(&a, A, OC, q.halves, q.rows, q.pitch, pa, 1, 128);
+        if (!rc) rc = map(&b, B, q.cols, OC, q.halves, pb, OC * pb, 64, 1);
+    } else if constexpr (FORM == kFcDeltaW) {
+        rc = map(&a, A, OC, q.halves, q.K, q.pitch, pa, 1, 64);
+        if (!rc) rc = map(&b, B, q.cols, q.K, 1, pb, q.K * pb, 64, 1);
+    } else {
+        rc = map(&a, A, q.K, 1, q.rows, pa, pa, 1, 128);
+        if (!rc) rc = map(&b, B, q.K, OC, q.halves, pb, OC * pb, 128, 1);
+    }
+    if (!rc) rc = A_MN ? out_map(&y, ws, q.halves, true, parts) : out_map(&y, ws, GLU && parts > 1 ? 2 : 1, false, parts);
+    if (!rc) rc = p.keep_z ? out_map(&z, q.e.Z, GLU ? 2 : 1, false, 1) : (z = y, ALPHA_OK);
     if (rc) return rc;
     const long long items = static_cast<long long>(p.m_tiles) * p.n_tiles * parts;
     const unsigned pairs = static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
@@ -280,7 +305,7 @@ int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, int parts
     note_launch("fc");
     note_plan("fc planes pair 256x256 parts=%d", parts);
     rc = launched("fc_pair_f32_kernel");
-    return rc || parts == 1 ? rc : launch_parts<GLU>(static_cast<const float*>(ws), size, parts, q.rows, q.e, sms, stream);
+    return rc || parts == 1 ? rc : launch_parts<GLU>(static_cast<const float*>(ws), size, parts, p.rows * m_halves, q.e, sms, stream);
 }
 
 // The same from the fp32 tensors as they lie; without `may_split` in no scratch.
@@ -291,8 +316,9 @@ int launch_gathered(const ProductF32& q, const PlanePlan& plan, int sms, int* st
     int rc = planes_launch_slice(&slice);
     if (rc) return rc;
     PlaneFc<FORM> p{};
-    p.A = q.A; p.B = q.B; p.rows = q.rows; p.cols = q.cols; p.K = q.K; p.lda = q.lda; p.ldb = q.ldb; p.e = q.e;
-    p.size = static_cast<size_t>(q.rows) * q.cols;
+    p.A = q.A; p.B = q.B; p.rows = q.rows; p.cols = q.cols; p.K = q.K; p.OC = q.OC; p.pitch = q.pitch; p.lda = q.lda; p.ldb = q.ldb; p.e = q.e;
+    const int out_rows = FORM == kFcDeltaW ? q.halves * q.OC : q.rows;
+    p.size = static_cast<size_t>(out_rows) * q.cols;
     p.ksplit = plan.ksplit;
     if (p.ksplit > 1) {
         void* ws = nullptr;
@@ -306,7 +332,7 @@ int launch_gathered(const ProductF32& q, const PlanePlan& plan, int sms, int* st
     note_launch("fc");
     note_plan("fc planes 128x%d ksplit=%d", plan.bn, p.ksplit);
     rc = launched("gemm_planes_kernel");
-    return rc || p.ksplit == 1 ? rc : launch_parts<FORM == kFcGlu>(p.part, p.size, p.ksplit, q.rows, q.e, sms, stream);
+    return rc || p.ksplit == 1 ? rc : launch_parts<FORM == kFcGlu>(p.part, p.size, p.ksplit, out_rows, q.e, sms, stream);
 }
 
 template <int FORM> PlanePlan pick_gathered(const ProductF32& q, int sms, int most = 16)
@@ -328,7 +354,7 @@ struct PairWork {
     int sms = 0, *status = nullptr;
     void* part = nullptr;
     int add(const float* src, int rows, int cols) { p[n] = planes_of(src, rows, cols); return n++; }
-    void want(const ProductF32& q, int k) { const size_t bytes = k > 1 ? k * static_cast<size_t>(q.rows) * q.cols * sizeof(float) : 0; if (bytes > parts) parts = bytes; }
+    void want(const ProductF32& q, int k) { const size_t bytes = k > 1 ? k * static_cast<size_t>(q.rows) * q.cols * sizeof(float) : 0; if (bytes > parts) parts = bytes; }   // (padding too)
     size_t elements() const { size_t e = 0; for (int i = 0; i < n; ++i) e += static_cast<size_t>(p[i].rows) * p[i].pitch; return e; }
     bool fits() const { return elements() < 4ull << 31; }           // 32-bit indices of words of four
     int split(cudaStream_t stream)
@@ -361,8 +387,8 @@ int forward_f32(const ProductF32& q, cudaStream_t stream)
     int rc = device_sms(&w.sms);
     if (!rc) rc = device_status_word(&w.status);
     if (rc) return rc;
-    const PairPlan pair = pick_pair(q.rows, FORM == kFcGlu ? q.cols / 2 : q.cols, FORM == kFcGlu, q.K, w.sms);
-    const int a = w.add(q.A, q.rows, q.K), b = w.add(q.B, q.cols, q.K);
+    const PairPlan pair = pick_pair(q.rows, 1, q.OC, FORM == kFcGlu, q.K, 1, w.sms);
+    const int a = w.add(q.A, q.rows, q.K), b = w.add(q.B, q.halves * q.OC, q.K);
     w.want(q, pair.parts);
     if (w.sms >= 2 && w.fits() && pairs_pay(pair.time + split_time(w.elements()), pick_gathered<FORM>(q, w.sms).time)) {
         rc = w.split(stream);
@@ -373,17 +399,18 @@ int forward_f32(const ProductF32& q, cudaStream_t stream)
 }
 
 // deltaX = dZ W and deltaW = dZ^T X (either may be missing).
-int delta_f32(const float* dZ, const float* X, const float* W, float* dX, float* dW, int rows, int wide, int IC, cudaStream_t stream)
+int delta_f32(const float* dZ, const float* X, const float* W, float* dX, float* dW, int rows, int OC, int halves, int IC, cudaStream_t stream)
 {
     const FcEpilogue plain{nullptr, nullptr, nullptr, nullptr, IC, ALPHA_ACT_NONE, 0.f};
-    ProductF32 x{dZ, W, rows, IC, wide, wide, IC, plain}, w{dZ, X, wide, IC, rows, wide, IC, plain};
+    const int pitch = fc_pitch(OC), wide = halves * pitch;
+    ProductF32 x{dZ, W, rows, IC, wide, OC, pitch, halves, wide, IC, plain}, w{dZ, X, wide, IC, rows, OC, pitch, halves, wide, IC, plain};
     x.e.Y = dX; w.e.Y = dW;
     int sms = 0, *status = nullptr;
     int rc = device_sms(&sms);
     if (!rc) rc = device_status_word(&status);
     if (rc) return rc;
     // which of them by pairs: both share the planes of dZ
-    const PairPlan px = pick_pair(rows, IC, false, wide, sms), pw = pick_pair(wide, IC, false, rows, sms);
+    const PairPlan px = pick_pair(rows, 1, IC, false, OC, halves, sms), pw = pick_pair(OC, halves, IC, false, rows, 1, sms);
     const double gx = pick_gathered<kFcDeltaX>(x, sms).time, gw = pick_gathered<kFcDeltaW>(w, sms).time;
     PairWork best;
     bool best_x = false, best_w = false;
@@ -396,7 +423,7 @@ int delta_f32(const float* dZ, const float* X, const float* W, float* dX, float*
         PairWork v;
         v.sms = sms; v.status = status;
         if (form) v.add(dZ, rows, wide);
-        if (bx) { v.add(W, wide, IC); v.want(x, px.parts); }
+        if (bx) { v.add(W, halves * OC, IC); v.want(x, px.parts); }
         if (bw) { v.add(X, rows, IC); v.want(w, pw.parts); }
         if (!v.fits()) continue;
         const double time = (dX ? (bx ? px.time : gx) : 0.0) + (dW ? (bw ? pw.time : gw) : 0.0) + (form ? split_time(v.elements()) : 0.0);
@@ -425,7 +452,7 @@ int launch_small(const AlphaFcShape* s, const void* X, const void* W, const void
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    FcSmall p{s->rows, s->IC, s->OC, 1, 1, s->act, s->k, X, W, bias, residual, Z, Y};
+    FcSmall p{s->rows, s->IC, s->OC, fc_pitch(s->OC), 1, 1, s->act, s->k, X, W, bias, residual, Z, Y};
     const int units = GLU ? s->OC : (s->OC + 1) / 2, words = s->IC / 4;
     // 16 warps an SM, each with 64 words of a row at least
     while (p.ks < 8 && static_cast<long long>(units) * p.ks < 16LL * sms && words >= 128 * p.ks) p.ks *= 2;
@@ -444,7 +471,7 @@ int launch_token(const AlphaFcShape* s, const void* X, const void* W, const void
     int sms = 0;
     const int rc = device_sms(&sms);
     if (rc) return rc;
-    FcSmall p{s->rows, s->IC, s->OC, 1, 1, s->act, s->k, X, W, bias, residual, Z, Y};
+    FcSmall p{s->rows, s->IC, s->OC, fc_pitch(s->OC), 1, 1, s->act, s->k, X, W, bias, residual, Z, Y};
     // up to eight warps a row group, each with 4 blocks of 32 steps at least
     while (p.ks < 8 && s->IC >= 256 * p.ks) p.ks *= 2;
     const int teams = 8 / p.ks, groups = (s->OC + 15) / 16;
@@ -478,13 +505,16 @@ int forward(const char* what, const AlphaFcShape* s, const void* X, const void* 
         }
     }
     if (s->dtype == ALPHA_F32) {
-        const FcEpilogue e{static_cast<const float*>(bias), static_cast<const float*>(residual), static_cast<float*>(Z), static_cast<float*>(Y), s->OC, s->act, s->k};
+        const int pitch = fc_pitch(s->OC);
+        const FcEpilogue e{static_cast<const float*>(bias), static_cast<const float*>(residual), static_cast<float*>(Z), static_cast<float*>(Y), pitch, s->act, s->k};
         const float *x = static_cast<const float*>(X), *w = static_cast<const float*>(W);
-        return glu ? forward_f32<kFcGlu>(ProductF32{x, w, s->rows, 2 * s->OC, s->IC, s->IC, s->IC, e}, stream)
-                   : forward_f32<kFcForward>(ProductF32{x, w, s->rows, s->OC, s->IC, s->IC, s->IC, e}, stream);
+        return glu ? forward_f32<kFcGlu>(ProductF32{x, w, s->rows, 2 * pitch, s->IC, s->OC, pitch, 2, s->IC, s->IC, e}, stream)
+                   : forward_f32<kFcForward>(ProductF32{x, w, s->rows, pitch, s->IC, s->OC, pitch, 1, s->IC, s->IC, e}, stream);
     }
     if (dry_run()) return ALPHA_OK;
-    return launch_product(Product{s->dtype, s->rows, s->OC, s->IC, false, false, glu, X, W, bias, residual, Z, Y, s->act, s->k}, stream);
+    const long long IC = s->IC, OC = s->OC;
+    return launch_product(Product{s->dtype, s->rows, s->OC, fc_pitch(s->OC), s->IC, 1, 1, glu, Operand{X, false, IC, 1, s->rows, IC, IC}, Operand{W, false, IC, OC, glu ? 2 : 1, IC, OC * IC},
+                                  bias, residual, Z, Y, s->act, s->k}, stream);
 }
 
 template <class T, bool GLU>
@@ -493,14 +523,14 @@ int launch_delta(const AlphaFcShape* s, const void* dY, const void* Z, void* dZ,
     int sms = 0;
     int rc = device_sms(&sms);
     if (rc) return rc;
-    const int wide = GLU ? 2 * s->OC : s->OC, words = s->OC / Word16<T>::N;
+    const int pitch = fc_pitch(s->OC), wide = GLU ? 2 * pitch : pitch, words = pitch / Word16<T>::N;
     const unsigned gy = (words + 31) / 32;
     // one wave of CTAs, eight rows of a warp at least
     long long gx = sms * (long long)kDeltaCtas / gy;
     if (gx < 1) gx = 1;
     const long long by_rows = (s->rows + 63) / 64;
     if (gx > by_rows) gx = by_rows;
-    FcDelta p{s->rows, s->OC, s->act, s->k, dY, Z, dZ, nullptr};
+    FcDelta p{s->rows, pitch, s->OC, s->act, s->k, dY, Z, dZ, nullptr};
     if (dB) {
         void* ws = nullptr;
         rc = call_scratch(stream, static_cast<size_t>(gx) * wide * sizeof(float), &ws);
@@ -526,11 +556,11 @@ int delta(const char* what, const AlphaFcShape* s, const void* dY, const void* X
     if (!dY || (dX && !W) || (dW && !X)) return fail(ALPHA_E_ARG, "%s: null tensor pointer", what);
     if (!dX && !dW && !dB) return fail(ALPHA_E_ARG, "%s: no gradient asked for", what);
     if (through && (!Z || !dZ)) return fail(ALPHA_E_ARG, "%s: Z of the forward pass and memory for deltaZ are needed (deltaZ may be Z)", what);
-    const size_t b = type_bytes(s->dtype), wide = glu ? 2 * static_cast<size_t>(s->OC) : s->OC, rows = s->rows;
+    const size_t b = type_bytes(s->dtype), pitch = fc_pitch(s->OC), wide = (glu ? 2 : 1) * pitch, units = (glu ? 2 : 1) * static_cast<size_t>(s->OC), rows = s->rows;
     if (!through) { Z = nullptr; dZ = nullptr; }
     const Span in_z{dZ == Z ? nullptr : Z, rows * wide * b};
-    rc = check_spans(what, {{dY, rows * s->OC * b}, {dW ? X : nullptr, rows * s->IC * b}, {dX ? W : nullptr, wide * s->IC * b}, in_z},
-                     {{dZ, rows * wide * b}, {dX, rows * s->IC * b}, {dW, wide * s->IC * b}, {dB, wide * b}});
+    rc = check_spans(what, {{dY, rows * pitch * b}, {dW ? X : nullptr, rows * s->IC * b}, {dX ? W : nullptr, units * s->IC * b}, in_z},
+                     {{dZ, rows * wide * b}, {dX, rows * s->IC * b}, {dW, units * s->IC * b}, {dB, wide * b}});
     if (!rc) rc = call_begin(stream);
     if (rc) return rc;
     if (through || dB) {
@@ -542,14 +572,16 @@ int delta(const char* what, const AlphaFcShape* s, const void* dY, const void* X
         if (rc) return rc;
     }
     const void* d = through ? dZ : dY;
-    const int w = static_cast<int>(wide);
-    if (s->dtype == ALPHA_F32) {
-        return delta_f32(static_cast<const float*>(d), static_cast<const float*>(X), static_cast<const float*>(W), static_cast<float*>(dX), static_cast<float*>(dW), s->rows, w,
-                         s->IC, stream);
-    }
+    if (s->dtype == ALPHA_F32)
+        return delta_f32(static_cast<const float*>(d), static_cast<const float*>(X), static_cast<const float*>(W), static_cast<float*>(dX), static_cast<float*>(dW), s->rows, s->OC,
+                         glu ? 2 : 1, s->IC, stream);
     if (dry_run()) return ALPHA_OK;
-    if (dX) rc = launch_product(Product{s->dtype, s->rows, s->IC, w, false, true, false, d, W, nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f}, stream);
-    if (!rc && dW) rc = launch_product(Product{s->dtype, w, s->IC, s->rows, true, true, false, d, X, nullptr, nullptr, nullptr, dW, ALPHA_ACT_NONE, 0.f}, stream);
+    const long long IC = s->IC, OC = s->OC, p = pitch, n = s->rows;
+    const int halves = glu ? 2 : 1;
+    if (dX) rc = launch_product(Product{s->dtype, s->rows, s->IC, s->IC, s->OC, 1, halves, false, Operand{d, false, OC, halves, n, p, halves * p}, Operand{W, true, IC, OC, halves, IC, OC * IC},
+                                        nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f}, stream);
+    if (!rc && dW) rc = launch_product(Product{s->dtype, s->OC, s->IC, s->IC, s->rows, halves, 1, false, Operand{d, true, OC, halves, n, p, halves * p}, Operand{X, true, IC, n, 1, IC, n * IC},
+                                               nullptr, nullptr, nullptr, dW, ALPHA_ACT_NONE, 0.f}, stream);
     return rc;
 }
 
@@ -563,9 +595,9 @@ int alpha_fullConnect(const AlphaFcShape* s, const void* X, const void* W, const
     int rc = check_fc("fullConnect", s, false);
     if (rc) return rc;
     if (!X || !W || !Y) return fail(ALPHA_E_ARG, "fullConnect: null tensor pointer");
-    const size_t b = type_bytes(s->dtype), y = static_cast<size_t>(s->rows) * s->OC * b;
+    const size_t b = type_bytes(s->dtype), pitch = fc_pitch(s->OC), y = s->rows * pitch * b;
     if (reinterpret_cast<uintptr_t>(residual) & 15) return fail(ALPHA_E_ARG, "fullConnect: tensor pointers must be 16-byte aligned");
-    rc = check_spans("fullConnect", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, static_cast<size_t>(s->OC) * s->IC * b}, {bias, s->OC * b}, {residual == Y ? nullptr : residual, y}},
+    rc = check_spans("fullConnect", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, static_cast<size_t>(s->OC) * s->IC * b}, {bias, pitch * b}, {residual == Y ? nullptr : residual, y}},
                      {{Y, y}, {Z, y}});
     return rc ? rc : forward("fullConnect", s, X, W, bias, residual, Z, Y, false, static_cast<cudaStream_t>(stream));
 }
@@ -576,8 +608,8 @@ int alpha_fullConnect_glu(const AlphaFcShape* s, const void* X, const void* W, c
     int rc = check_fc("fullConnect_glu", s, true);
     if (rc) return rc;
     if (!X || !W || !Y) return fail(ALPHA_E_ARG, "fullConnect_glu: null tensor pointer");
-    const size_t b = type_bytes(s->dtype), y = static_cast<size_t>(s->rows) * s->OC * b;
-    rc = check_spans("fullConnect_glu", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, 2 * static_cast<size_t>(s->OC) * s->IC * b}, {bias, 2 * s->OC * b}}, {{Y, y}, {Z, 2 * y}});
+    const size_t b = type_bytes(s->dtype), pitch = fc_pitch(s->OC), y = s->rows * pitch * b;
+    rc = check_spans("fullConnect_glu", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, 2 * static_cast<size_t>(s->OC) * s->IC * b}, {bias, 2 * pitch * b}}, {{Y, y}, {Z, 2 * y}});
     return rc ? rc : forward("fullConnect_glu", s, X, W, bias, nullptr, Z, Y, true, static_cast<cudaStream_t>(stream));
 }
 

@@ -14,7 +14,7 @@ namespace alpha {
 
 struct FcDelta {
     long long rows;
-    int cols;                       // OC
+    int cols, OC;                   // columns of a half with their padding, and without: deltaZ's padding is zeros
     int act; float k;
     const void *dY, *Z;
     void* dZ;                       // nullptr: column sums only (no activation)
@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(256, kDeltaCtas) fc_delta_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, words = p.cols / N, word = blockIdx.x * 32 + lane;
     const uint4 *dY = static_cast<const uint4*>(p.dY), *Z = static_cast<const uint4*>(p.Z);
     uint4* dZ = static_cast<uint4*>(p.dZ);
+    const int whole = p.OC - word * N;                                   // columns of the lane's word that are not padding
     float acc[HALVES][N];
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -70,6 +71,7 @@ __global__ void __launch_bounds__(256, kDeltaCtas) fc_delta_kernel(const __grid_
                             act_both<ACT, V::kFast>(g[i], p.k, value, slope);
                             g[i] = d[i] * u[i] * slope;
                             u[i] = d[i] * value;
+                            if (i >= whole) g[i] = u[i] = 0.f;
                             acc[0][i] += g[i];
                             acc[1][i] += u[i];
                         }
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(256, kDeltaCtas) fc_delta_kernel(const __grid_
                             for (int i = 0; i < N; ++i) {
                                 float value, slope;
                                 act_both<ACT, V::kFast>(z[i], p.k, value, slope);
-                                d[i] *= slope;
+                                d[i] = i >= whole ? 0.f : d[i] * slope;
                             }
                             dZ[zt] = V::store(d);
                         }

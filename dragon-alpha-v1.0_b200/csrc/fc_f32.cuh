@@ -10,7 +10,7 @@ namespace alpha {
 struct FcEpilogue {
     const float *bias, *residual;
     float *Z, *Y;
-    int cols, act; float k;         // cols: of Y
+    int cols, act; float k;         // cols: pitch of Y, and of either half of Z and the bias
 };
 template <bool GLU> __device__ __noinline__ void fc_finish(const FcEpilogue& e, float* row, int col, float4 o)
 {
@@ -52,17 +52,19 @@ template <bool GLU> __device__ __noinline__ void fc_finish(const FcEpilogue& e, 
 
 enum FcForm : int { kFcForward, kFcGlu, kFcDeltaX, kFcDeltaW };
 
-// Rows x columns outputs over K steps in `ksplit` parts (bz), each into its own copy of the sums, or finished at once.  All dimensions
-// but the rows of a K-major A and the steps of deltaW are multiples of 4.
+// Rows x columns outputs over K steps in `ksplit` parts (bz), each into its own copy of the sums, or finished at once.  Tensors that are OC wide
+// have a pitch of `pitch` columns (a half), W and deltaW do not: the padding among rows, columns and steps has no words of W and no outputs.
 template <int FORM>
 struct PlaneFc {
     static constexpr bool kAk = FORM != kFcDeltaW, kBk = FORM == kFcForward || FORM == kFcGlu, kTail = false, kCopyB = false;
     const float *A, *B;
-    int rows, cols, K, lda, ldb, ksplit;
+    int rows, cols, K, OC, pitch, lda, ldb, ksplit;
     float* part; size_t size;       // ksplit > 1
     FcEpilogue e;
     struct Cta { int m0, n0, s0, s1, K; float* out; };
 
+    // Place of a column of Z among the rows of W, -1: padding.
+    __device__ int unit_of(int c) const { const int up = c >= pitch ? 1 : 0, j = c - up * pitch; return j < OC ? j + up * OC : -1; }
     __device__ bool cta(Cta& c, int BM, int BN, int bx, int by, int sp) const
     {
         c.m0 = bx * BM; c.n0 = by * BN;
@@ -79,16 +81,25 @@ struct PlaneFc {
     __device__ PlaneAt a_row(const Cta& c, int m) const { return PlaneAt{static_cast<uint32_t>(kAk ? (c.m0 + m) * lda : c.m0 + m), c.m0 + m < rows ? 1u : 0u}; }
     __device__ PlaneAt b_row(const Cta& c, int col) const
     {
-        const int j = c.n0 + col, at = FORM == kFcGlu ? (j >> 1) + (j & 1) * e.cols : j;      // glu: gate and up rows in turn
-        return PlaneAt{static_cast<uint32_t>(kBk ? at * ldb : at), j < cols ? 1u : 0u};
+        const int j = c.n0 + col;
+        if (!kBk) return PlaneAt{static_cast<uint32_t>(j), j < cols ? 1u : 0u};
+        const int unit = FORM == kFcGlu ? j >> 1 : j;                                           // glu: gate and up rows in turn
+        return PlaneAt{static_cast<uint32_t>((FORM == kFcGlu ? unit + (j & 1) * OC : unit) * ldb), unit < OC ? 1u : 0u};
     }
     __device__ PlaneAt a_step(const Cta&, int k) const { return PlaneAt{static_cast<uint32_t>(k * (kAk ? 1 : lda)), k < K ? 1u : kNoStep}; }
-    __device__ PlaneAt b_step(const Cta&, int k) const { return PlaneAt{static_cast<uint32_t>(k * (kBk ? 1 : ldb)), k < K ? 1u : kNoStep}; }
+    __device__ PlaneAt b_step(const Cta&, int k) const
+    {
+        if (FORM != kFcDeltaX) return PlaneAt{static_cast<uint32_t>(k * (kBk ? 1 : ldb)), k < K ? 1u : kNoStep};
+        const int unit = k < K ? unit_of(k) : -1;
+        return unit >= 0 ? PlaneAt{static_cast<uint32_t>(unit * ldb), 1u} : PlaneAt{0u, kNoStep};
+    }
     __device__ static bool use_a(const PlaneAt& row, const PlaneAt& step) { return plane_meets(row, step); }
     __device__ static bool use_b(const PlaneAt& row, const PlaneAt& step) { return plane_meets(row, step); }
     __device__ float* row_out(const Cta& c, int m) const
     {
-        return c.m0 + m < rows ? c.out + static_cast<size_t>(c.m0 + m) * (ksplit > 1 ? cols : e.cols) : nullptr;
+        if (c.m0 + m >= rows) return nullptr;
+        const int row = FORM == kFcDeltaW ? unit_of(c.m0 + m) : c.m0 + m;
+        return row >= 0 ? c.out + static_cast<size_t>(row) * (ksplit > 1 ? cols : e.cols) : nullptr;
     }
     __device__ void store(const Cta& c, float* row, int col, const float4& o) const
     {

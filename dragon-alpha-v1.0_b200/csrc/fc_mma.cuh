@@ -5,7 +5,8 @@
 //   glu:          B holds gate rows and up rows; g and u the two sums of a unit, Y = act(g) u, Z = [g | u]
 // Forward A = X, B = W; deltaX A = dZ, B = W read along its rows (MN-major); deltaW A = dZ, B = X, both MN-major.  Either operand's memory
 // may run along k (a box of 64 steps x rows, 128-byte rows) or along its rows (boxes of 64 rows x 64 steps): the MMA's descriptors take both,
-// so nothing is transposed.  What a box reads past a matrix is zeros and past a half of W belongs to columns that are not stored.
+// so nothing is transposed.  Gate and up rows of W, and the halves of Z, are one more dimension of the maps, (step, half, row) or (step, row, half), so
+// that what a box reads past a matrix or past a half of it is zeros: no size but IC has to be a multiple of anything.
 //
 // PAIR: two CTAs of a cluster form 256 x 256 outputs (tcgen05 cta_group::2): each holds its 128 rows of A and half of the rows of B, so that
 // shared memory is read and filled with half of B.  Persistent: a pair walks over tiles, in groups of kFcGroupM row tiles so that the tiles in
@@ -29,11 +30,11 @@ constexpr uint32_t kFcRing = 196608, kFcStaging = 8 * 4096;              // stag
 constexpr uint32_t kFcSmemMost = kFcRing + kFcStaging + 1024 + 512;
 
 struct FcMma {
-    int rows, cols;               // outputs (glu: columns of a half)
+    int rows, cols;               // outputs: rows of a half, pitch (glu: of a half of Z too)
     int m_tiles, n_tiles, kb;     // tiles, stages of the reduction
+    int m_half, k_half;           // tiles of rows, blocks of 64 steps of the first half (deltaW, deltaX with gates)
     int bn, stages, split;        // columns of a CTA's accumulator (glu: of both halves), stages of its ring, CTAs that share a tile
     int a_mn, b_mn, a_rows;       // operands that run along their rows; rows of a box of A that runs along k
-    int b_up;                     // glu: first row of the up half of B
     uint32_t idesc, tmem;         // tmem: columns of tensor memory
     int act, keep_z; float k;
     const void *bias, *residual;
@@ -81,10 +82,12 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     // (shared tiles: the launch has a cluster for each)
     const int total = p.m_tiles * p.n_tiles, step = gridDim.x / (CTAS * split), first = blockIdx.x / (CTAS * split);
     const int k_each = (p.kb + split - 1) / split, k_begin = PAIR ? 0 : static_cast<int>(rank) * k_each, k_end = k_begin + k_each < p.kb ? k_begin + k_each : p.kb;
+    int hm = 0;                                   // half of the output's rows
     auto tile_at = [&](int t, int& m0, int& n0) {
         const int per = kFcGroupM * p.n_tiles, g = t / per, r = t - g * per, left = p.m_tiles - g * kFcGroupM, rows = left < kFcGroupM ? left : kFcGroupM;
-        const int n = r / rows;
-        m0 = (g * kFcGroupM + r - n * rows) * (128 * CTAS) + (PAIR ? static_cast<int>(rank) * 128 : 0);
+        const int n = r / rows, m = g * kFcGroupM + r - n * rows;
+        hm = m >= p.m_half ? 1 : 0;
+        m0 = (m - hm * p.m_half) * (128 * CTAS) + (PAIR ? static_cast<int>(rank) * 128 : 0);
         n0 = n * OUT;
     };
     const uint32_t smem_a = smem_u32(smem);
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     // The epilogue of 32 rows x (up to) 32 columns: the sums of a lane's row in z (glu: and u), the words of R in r.
     auto finish = [&](float (&z)[32], float (&u)[32], const uint4 (&r)[4], int row0, int col0, int width) {
         const T* bias = static_cast<const T*>(p.bias);
-        T *Y = static_cast<T*>(p.Y), *Z = static_cast<T*>(p.Z);
+        T *Y = static_cast<T*>(p.Y) + (hm ? static_cast<size_t>(p.rows) * p.cols : 0), *Z = static_cast<T*>(p.Z);
         if constexpr (GLU) {
             if (bias) { add_bias(z, bias, col0); add_bias(u, bias + p.cols, col0); }
             if (p.keep_z) {
@@ -184,9 +187,9 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         const uint32_t full_L = PAIR ? __shfl_sync(0xffffffffu, mapa_u32(full_a, 0), 0) : full_0, elected = elect_one();
         const uint32_t tx = CTAS * kStage;
         const int my = PAIR ? __shfl_sync(0xffffffffu, static_cast<int>(rank), 0) : 0;
-        auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1) {
-            if constexpr (PAIR) tma_load_2d_pair(dst, m, bar, c0, c1);
-            else tma_load_2d_a(dst, m, bar, c0, c1);
+        auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+            if constexpr (PAIR) tma_load_3d_pair(dst, m, bar, c0, c1, c2);
+            else tma_load_3d_a(dst, m, bar, c0, c1, c2);
         };
         RingPos rp;
         for (int t = first; t < total && ok; t += step) {
@@ -201,23 +204,24 @@ __global__ void __launch_bounds__(kFcThreads, 1)
 #pragma unroll
                     for (int q = 0; q < KB; ++q) {
                         const uint32_t a = base + rp.idx * kStage + q * kBlock, b = a + kA;
-                        const int k0 = (kb * KB + q) * kFcBK;
+                        // (the block after the last of an odd number lies past both halves)
+                        const int block = kb * KB + q, hk = block >= p.k_half ? (block - p.k_half >= p.k_half ? 2 : 1) : 0, k0 = (block - hk * p.k_half) * kFcBK;
                         if (p.a_mn) {
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) load(a + j * 8192, &tmA, bar, m0 + 64 * j, k0);
+                            for (int j = 0; j < 2; ++j) load(a + j * 8192, &tmA, bar, m0 + 64 * j, hm, k0);
                         } else {
-                            load(a, &tmA, bar, k0, m0);
+                            load(a, &tmA, bar, k0, hk, m0);
                         }
                         if constexpr (GLU) {
                             // columns [gate | up] of the accumulator
-                            if constexpr (PAIR) load(b, &tmB, bar, k0, n0 + (my ? p.b_up : 0));
-                            else { load(b, &tmB, bar, k0, n0); load(b + kB / 2, &tmB, bar, k0, n0 + p.b_up); }
+                            if constexpr (PAIR) load(b, &tmB, bar, k0, n0, my);
+                            else { load(b, &tmB, bar, k0, n0, 0); load(b + kB / 2, &tmB, bar, k0, n0, 1); }
                         } else {
                             const int b0 = n0 + my * 128;
                             if (p.b_mn) {
-                                for (int j = 0; j < static_cast<int>(kB >> 13); ++j) load(b + j * 8192, &tmB, bar, b0 + 64 * j, k0);
+                                for (int j = 0; j < static_cast<int>(kB >> 13); ++j) load(b + j * 8192, &tmB, bar, b0 + 64 * j, k0, hk);
                             } else {
-                                load(b, &tmB, bar, k0, b0);
+                                load(b, &tmB, bar, k0, b0, 0);
                             }
                         }
                     }
@@ -286,7 +290,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
             const bool fetching = !GLU && p.residual && row0 < p.rows && (PAIR || split == 1);
             if (!GLU && p.residual && (PAIR || split == 1)) {
                 int m1, n1;
-                tile_at(t + step < total ? t + step : t, m1, n1);
+                tile_at(t + step < total ? t + step : t, m1, n1);       // (one half: R goes with a forward product)
                 const int row = m1 + quad * 32 + lane;
                 for (int c = half * 32; c < OUT; c += 64)
                     if (row < p.rows && n1 + c < p.cols) prefetch_l2(static_cast<const T*>(p.residual) + static_cast<size_t>(row) * p.cols + n1 + c);

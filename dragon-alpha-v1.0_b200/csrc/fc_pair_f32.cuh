@@ -48,34 +48,40 @@ __global__ void __launch_bounds__(256) fc_split_kernel(const __grid_constant__ S
 }
 
 struct PairF32 {
-    int rows, cols;                // outputs (glu: columns of a half)
+    int rows, cols, pitch, K;      // outputs (glu: columns of a half; rows of a half), pitch of Y, R and halves of Z and the bias; steps (of a half)
     int m_tiles, n_tiles, windows, parts;   // windows: of 64 steps
-    int a_mn, b_mn, b_up, K;
+    int m_half, w_half;            // tiles of rows, windows of the first half (deltaW, deltaX with gates)
+    int a_mn, b_mn;
     uint32_t idesc;
-    const float *A, *B;            // the fp32 operands: element (row, k) at A[row * a_row + k * a_k], (column, k) at B[column * b_col + k * b_k]
-    long long a_row, a_k, b_col, b_k;
+    // the fp32 operands: element (row, k) of half h at A[h * a_half + row * a_row + k * a_k], (column, k) at B[h * b_half + column * b_col + k * b_k]
+    const float *A, *B;
+    long long a_row, a_k, a_half, b_col, b_k, b_half;
     const float *bias, *residual;
     int act, keep_z; float k;
     int* status;
 };
 
-// 32 columns of a row (unit columns from col0 on, of B's rows from `up` on) as sums of FMAs in ascending k.  Columns past the last are formed as the last.
-static __device__ __noinline__ void form_row_f32(const PairF32& p, int row, int col0, int up, int k0, int k1, float* z)
+// 32 columns of a row from col0 on, of halves ha and hb of the operands' rows, over windows [w0, w1), as sums of FMAs in ascending k.  Columns past
+// the last are formed as the last.
+static __device__ __noinline__ void form_row_f32(const PairF32& p, int row, int col0, int ha, int hb, int w0, int w1, float* z)
 {
     float acc[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-    const float *a = p.A + row * p.a_row, *b = p.B + static_cast<long long>(up) * p.b_col;
-    for (int k = k0; k < k1; ++k) {
-        const float av = __ldg(a + k * p.a_k);
+    for (int w = w0; w < w1; ++w) {
+        const int hk = w >= p.w_half ? 1 : 0, k0 = (w - hk * p.w_half) * 64, k1 = k0 + 64 < p.K ? k0 + 64 : p.K;
+        const float *a = p.A + (ha + hk) * p.a_half + row * p.a_row, *b = p.B + (hb + hk) * p.b_half;
+        for (int k = k0; k < k1; ++k) {
+            const float av = __ldg(a + k * p.a_k);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] = fmaf(av, __ldg(b + (col0 + i < p.cols ? col0 + i : p.cols - 1) * p.b_col + k * p.b_k), acc[i]);
+            for (int i = 0; i < 32; ++i) acc[i] = fmaf(av, __ldg(b + (col0 + i < p.cols ? col0 + i : p.cols - 1) * p.b_col + k * p.b_k), acc[i]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 32; ++i) z[i] = acc[i];
 }
 
-// tmY: the result, or where parts > 1 the sums [part][row][halves][column]
+// tmY: the result, or where parts > 1 the sums, as (column, half, row, part)
 template <bool GLU>
 __global__ void __launch_bounds__(kPairF32Threads, 1)
     fc_pair_f32_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
@@ -112,14 +118,15 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
     const uint32_t tmem_base = *tmem_holder, smem_a = smem_u32(smem);
 
     const int tiles = p.m_tiles * p.n_tiles, total = tiles * p.parts, step = gridDim.x / 2, first = blockIdx.x / 2;
-    struct Item { int m0, n0, w0, w1, part; };
+    struct Item { int m0, n0, w0, w1, part, hm; };
     auto item_at = [&](int t) {
         Item i;
         i.part = t / tiles;
         t -= i.part * tiles;
         constexpr int GROUP = 4;                      // row tiles that are walked together: what is in flight shares rows in L2
-        const int per = GROUP * p.n_tiles, g = t / per, r = t - g * per, left = p.m_tiles - g * GROUP, rows = left < GROUP ? left : GROUP, n = r / rows;
-        i.m0 = (g * GROUP + r - n * rows) * 256 + static_cast<int>(rank) * 128;
+        const int per = GROUP * p.n_tiles, g = t / per, r = t - g * per, left = p.m_tiles - g * GROUP, rows = left < GROUP ? left : GROUP, n = r / rows, m = g * GROUP + r - n * rows;
+        i.hm = m >= p.m_half ? 1 : 0;
+        i.m0 = (m - i.hm * p.m_half) * 256 + static_cast<int>(rank) * 128;
         i.n0 = n * OUT;
         const int each = (p.windows + p.parts - 1) / p.parts;
         i.w0 = i.part * each < p.windows ? i.part * each : p.windows;
@@ -135,25 +142,25 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         RingPos rp;
         for (int t = first; t < total && ok; t += step) {
             const Item it = item_at(t);
-            const int b0 = GLU ? it.n0 + (my ? p.b_up : 0) : it.n0 + my * 128;
+            const int b0 = GLU ? it.n0 : it.n0 + my * 128;
             for (int s = 3 * it.w0; s < 3 * it.w1; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait_a(empty_0 + 8 * rp.idx, rp.phase ^ 1));
                 if (!ok) { report(p.status, kStatusProducerTimeout); settle(); break; }
                 if (elected) {
                     if (my == 0) mbar_arrive_expect_tx_a(full_0 + 8 * rp.idx, 2 * kPairF32Slot);
                     const uint32_t bar = full_L + 8 * rp.idx, a = base + rp.idx * kPairF32Slot, b = a + kPairF32Operand;
-                    const int k0 = s / 3 * 64, plane = s % 3;
+                    const int w = s / 3, plane = s % 3, hk = w >= p.w_half ? 1 : 0, k0 = (w - hk * p.w_half) * 64;
                     if (p.a_mn) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) tma_load_3d_pair(a + j * 8192, &tmA, bar, it.m0 + 64 * j, k0, plane);
+                        for (int j = 0; j < 2; ++j) tma_load_4d_pair(a + j * 8192, &tmA, bar, it.m0 + 64 * j, it.hm, k0, plane);
                     } else {
-                        tma_load_3d_pair(a, &tmA, bar, k0, it.m0, plane);
+                        tma_load_4d_pair(a, &tmA, bar, k0, hk, it.m0, plane);
                     }
                     if (p.b_mn) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) tma_load_3d_pair(b + j * 8192, &tmB, bar, b0 + 64 * j, k0, plane);
+                        for (int j = 0; j < 2; ++j) tma_load_4d_pair(b + j * 8192, &tmB, bar, b0 + 64 * j, k0, hk, plane);
                     } else {
-                        tma_load_3d_pair(b, &tmB, bar, k0, b0, plane);
+                        tma_load_4d_pair(b, &tmB, bar, k0, b0, GLU ? my : 0, plane);
                     }
                 }
                 __syncwarp();
@@ -277,7 +284,6 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
                 least = min(least, min(u - 1, v - 1));          // (zero as the largest)
             }
             const bool again = __any_sync(0xffffffffu, most >= 0xff000000u || least < 2u * 0x08800000u);
-            const int k0 = it.w0 * 64, k1 = it.w1 * 64 < p.K ? it.w1 * 64 : p.K;
             const int row = row0 + lane;
             // The sums go back to the side columns, which are free now, and come chunk by chunk through one copy of the code below: unrolled over the
             // registers that hold them it took 25 us to fetch (of 111, 2048 x 2048 x 2048), and indexed they would live in local memory.
@@ -294,10 +300,10 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             }
             tmem_st_wait();
             // 32 sums from column c on, or, where some of the warp's do not stand, formed once more (rows past the last as the last)
-            auto take = [&](int c, int col0, int up, float (&f)[32]) {
+            auto take = [&](int c, int col0, int hb, float (&f)[32]) {
                 if (again) {
                     float formed[32];
-                    form_row_f32(p, row < p.rows ? row : p.rows - 1, col0, up, k0, k1, formed);
+                    form_row_f32(p, row < p.rows ? row : p.rows - 1, col0, it.hm, hb, it.w0, it.w1, formed);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) f[i] = formed[i];
                     return;
@@ -311,7 +317,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             auto add = [&](float (&f)[32], const float* from, int col0) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    if (col0 + 4 * q < p.cols) {
+                    if (col0 + 4 * q < p.pitch) {
                         const float4 v = *reinterpret_cast<const float4*>(from + col0 + 4 * q);
                         f[4 * q] += v.x; f[4 * q + 1] += v.y; f[4 * q + 2] += v.z; f[4 * q + 3] += v.w;
                     }
@@ -323,13 +329,13 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
                     if (col0 >= p.cols) break;
                     float z[32], u[32];
                     take(col_a + c, col0, 0, z);
-                    take(col_b + c, col0, p.b_up, u);
+                    take(col_b + c, col0, 1, u);
                     if (p.parts > 1) {
                         put(z, [&] { tma_store_4d_a(&tmY, buf, col0, 0, row0, it.part); });
                         put(u, [&] { tma_store_4d_a(&tmY, buf, col0, 1, row0, it.part); });
                         continue;
                     }
-                    if (p.bias) { add(z, p.bias, col0); add(u, p.bias + p.cols, col0); }
+                    if (p.bias) { add(z, p.bias, col0); add(u, p.bias + p.pitch, col0); }
                     if (p.keep_z) {
                         put(z, [&] { tma_store_4d_a(&tmZ, buf, col0, 0, row0, 0); });
                         put(u, [&] { tma_store_4d_a(&tmZ, buf, col0, 1, row0, 0); });
@@ -354,9 +360,9 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
 #pragma unroll
                             for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, false>(z[i], p.k);
                         });
-                        if (p.residual && row < p.rows) add(z, p.residual + static_cast<size_t>(row) * p.cols, col0);
+                        if (p.residual && row < p.rows) add(z, p.residual + static_cast<size_t>(row) * p.pitch, col0);
                     }
-                    put(z, [&] { tma_store_4d_a(&tmY, buf, col0, 0, row0, it.part); });
+                    put(z, [&] { tma_store_4d_a(&tmY, buf, col0, it.hm, row0, it.part); });
                 }
             }
             release(side_free_L);

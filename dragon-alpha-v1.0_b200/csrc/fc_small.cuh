@@ -11,7 +11,7 @@
 namespace alpha {
 
 struct FcSmall {
-    int rows, IC, OC, ks;          // ks: warps of a CTA that share two rows of W, or a row group (1, 2, 4, 8)
+    int rows, IC, OC, pitch, ks;   // pitch: of Y and R, and of either half of Z and the bias; ks: warps of a CTA that share two rows of W, or a row group (1, 2, 4, 8)
     int split;                     // CTAs of a cluster that share a row group (16-bit)
     int act; float k;
     const void *X, *W, *bias, *residual;
@@ -122,12 +122,12 @@ __global__ void __launch_bounds__(256) fc_small_kernel(const __grid_constant__ F
     }
     const T* bias = static_cast<const T*>(p.bias);
     T *Z = static_cast<T*>(p.Z), *Y = static_cast<T*>(p.Y);
-    const size_t at = static_cast<size_t>(r) * p.OC + col;
+    const size_t at = static_cast<size_t>(r) * p.pitch + col;
     if (bias) z += to_float(bias[col]);
-    if (GLU && bias) up += to_float(bias[p.OC + col]);
+    if (GLU && bias) up += to_float(bias[p.pitch + col]);
     if (Z) {
-        Z[GLU ? at + static_cast<size_t>(r) * p.OC : at] = from_float<T>(z);
-        if (GLU) Z[at + static_cast<size_t>(r + 1) * p.OC] = from_float<T>(up);
+        Z[GLU ? at + static_cast<size_t>(r) * p.pitch : at] = from_float<T>(z);
+        if (GLU) Z[at + static_cast<size_t>(r + 1) * p.pitch] = from_float<T>(up);
     }
     with_act(p.act, [&](auto a) { z = act_value<decltype(a)::value, Word16<T>::kFast>(z, p.k); });
     if (GLU) z *= up;
@@ -271,12 +271,12 @@ __global__ void __launch_bounds__(256) fc_token_kernel(const __grid_constant__ F
         const int o = e & 15, r = (e >> 4) % COLS, team = e / (16 * COLS), col = (block * teams + team) * 16 + o;
         if (r >= p.rows || col >= p.OC) continue;
         float z = sum(team, 0, o, r), up = GLU ? sum(team, MT - 1, o, r) : 0.f;
-        const size_t at = static_cast<size_t>(r) * p.OC + col;
+        const size_t at = static_cast<size_t>(r) * p.pitch + col;
         if (bias) z += to_float(bias[col]);
-        if (GLU && bias) up += to_float(bias[p.OC + col]);
+        if (GLU && bias) up += to_float(bias[p.pitch + col]);
         if (Z) {
-            Z[GLU ? at + static_cast<size_t>(r) * p.OC : at] = from_float<T>(z);
-            if (GLU) Z[at + static_cast<size_t>(r + 1) * p.OC] = from_float<T>(up);
+            Z[GLU ? at + static_cast<size_t>(r) * p.pitch : at] = from_float<T>(z);
+            if (GLU) Z[at + static_cast<size_t>(r + 1) * p.pitch] = from_float<T>(up);
         }
         with_act(p.act, [&](auto a) { z = act_value<decltype(a)::value, true>(z, p.k); });
         if (GLU) z *= up;

@@ -436,7 +436,7 @@ def _fc_plan(what, glu, xs, ws, dtype):
     rows, unit = 1, 4 if dtype == torch.float32 else 8
     for n in lead:
         rows *= n
-    return IC, OC, -(-IC // unit) * unit, -(-OC // unit) * unit, rows, halves, lead + (OC,), lead + (halves * OC,), (halves * OC,)
+    return IC, OC, -(-IC // unit) * unit, -(-OC // 8) * 8, rows, halves, lead + (OC,), lead + (halves * OC,), (halves * OC,)
 
 
 def _fc_check(what, X, W, others):
@@ -639,8 +639,8 @@ class Engine:
         return C[:N, :M]
 
     # ---- FullConnect layers of a transformer: the product with bias, activation and residual in its epilogue, the gated block, their
-    # gradients.  float32, bfloat16 or float16 tensors (all of one type); X may have any leading dimensions; IC and OC that are no
-    # multiples of 16 bytes are zero-padded as everywhere. ----
+    # gradients.  float32, bfloat16 or float16 tensors (all of one type); X may have any leading dimensions; IC that is no multiple of 16 bytes
+    # is zero-padded as everywhere, and so are tensors of OC columns that is no multiple of 8 (not W). ----
     def _fc_forward(self, what, X, W, Bias, act, k, Residual, save, glu):
         plan = _fc_plan(what, glu, X.shape, W.shape, X.dtype)
         code = _fc_act(what, act)
@@ -655,14 +655,14 @@ class Engine:
         dtype = X.dtype
         if rows == 0:
             return (X.new_empty(ys), X.new_empty(zs)) if save else X.new_empty(ys)
-        (Xp, Wp, Bp, Rp), _held = _fc_pack(dtype, (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic), (Bias, 1, halves, OC, halves, oc), (Residual, 1, rows, OC, rows, oc))
+        (Xp, Wp, Bp, Rp), _held = _fc_pack(dtype, (X, 1, rows, IC, rows, ic), (W, 1, halves * OC, IC, halves * OC, ic), (Bias, 1, halves, OC, halves, oc), (Residual, 1, rows, OC, rows, oc))
         even = oc == OC
         Y = X.new_empty(ys if even else (rows, oc))
         Z = X.new_empty(zs if even else (rows, halves * oc)) if save else None
         if glu:
-            self.base.fullConnect_glu(Y.data_ptr(), Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Z)
+            self.base.fullConnect_glu(Y.data_ptr(), Xp, Wp, rows, ic, OC, _FC_TYPES[dtype], code, k, Bp, Z)
         else:
-            self.base.fullConnect(Y.data_ptr(), Xp, Wp, rows, ic, oc, _FC_TYPES[dtype], code, k, Bp, Rp, Z)
+            self.base.fullConnect(Y.data_ptr(), Xp, Wp, rows, ic, OC, _FC_TYPES[dtype], code, k, Bp, Rp, Z)
         if not even:
             Y = Y.narrow(1, 0, OC)
             if len(ys) != 2:
@@ -688,18 +688,17 @@ class Engine:
         if rows == 0:
             return X.new_empty(X.shape), W.new_zeros(W.shape), W.new_zeros((halves * OC,)) if bias else None
         through = glu or code != 0
-        (dYp, Xp, Wp, Zp), _held = _fc_pack(dtype, (deltaY, 1, rows, OC, rows, oc), (X, 1, rows, IC, rows, ic), (W, halves, OC, IC, oc, ic),
+        (dYp, Xp, Wp, Zp), _held = _fc_pack(dtype, (deltaY, 1, rows, OC, rows, oc), (X, 1, rows, IC, rows, ic), (W, 1, halves * OC, IC, halves * OC, ic),
                                             (Z if through else None, 1, rows * halves, OC, rows * halves, oc))
         dZ = X.new_empty((rows, halves * oc)) if through else None
-        dX, dW = X.new_empty((rows, ic)), W.new_empty((halves, oc, ic))
+        dX, dW = X.new_empty((rows, ic)), W.new_empty((halves * OC, ic))
         dB = W.new_empty((halves, oc)) if bias else None
-        self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, oc, _FC_TYPES[dtype], code, k, glu)
+        self.base.fullConnect_delta(dX, dW, dB, dYp, Xp, Wp, Zp, dZ, rows, ic, OC, _FC_TYPES[dtype], code, k, glu)
         if ic != IC:
-            dX = dX.narrow(1, 0, IC)
-        if ic != IC or oc != OC:
-            dW = dW[:, :OC, :IC]
-            dB = dB[:, :OC] if bias else None
-        return dX if X.dim() == 2 else dX.reshape(X.shape), dW.reshape(W.shape), dB.reshape(halves * OC) if bias else None
+            dX, dW = dX.narrow(1, 0, IC), dW.narrow(1, 0, IC)
+        if bias:
+            dB = (dB if oc == OC else dB.narrow(1, 0, OC)).reshape(halves * OC)
+        return dX if X.dim() == 2 else dX.reshape(X.shape), dW, dB
 
     def fullConnect(self, X, W, Bias=None, act="none", k=0.0, Residual=None, save=False):
         """act(X W^T + Bias) + Residual in one pass; W [OC, IC], X [..., IC].  act: 'none', 'leakyRelu' (slope k; relu k = 0),

@@ -455,9 +455,11 @@ int alpha_engine_batchMatMulT2(float* C, const float* A, const float* B, int Bat
  * The matrix product of a FullConnect layer with what surrounds it in the same pass, over fp32 or 16-bit tensors:
  *   alpha_fullConnect        Z = X W^T + bias,  Y = act(Z) + residual          W[OC][IC], the layout of a 1x1 convolution's
  *   alpha_fullConnect_glu    Z = X W^T + bias,  Y = act(Z[:, :OC]) * Z[:, OC:]  W[2 OC][IC]: OC gate rows, then OC up rows
- * X[rows][IC], Y and residual [rows][OC], Z [rows][OC] (glu: [rows][2 OC]), bias[OC] (glu: [2 OC]); all of one type, dense,
- * 16-byte aligned, IC and OC multiples of 4 (fp32) or 8 (16-bit).  bias, residual and Z may be NULL; Z keeps the sums for the
- * backward pass.  residual may be Y itself; no other output may overlap an input (ALPHA_E_ARG).
+ * All tensors are of one type, dense and 16-byte aligned; IC is a multiple of 4 (fp32) or 8 (16-bit), OC any number.  X[rows][IC].
+ * Tensors that are OC wide have P = OC rounded up to a multiple of 8 columns: Y and residual [rows][P], Z [rows][P] (glu:
+ * [rows][2][P], gates and ups), bias[P] (glu: [2][P]); what their columns from OC on hold is not used, and not kept.
+ * bias, residual and Z may be NULL; Z keeps the sums for the backward pass.  residual may be Y itself; no other output may
+ * overlap an input (ALPHA_E_ARG).
  * Sums, bias, activation and residual are fp32 and an output is rounded once; Y comes from the unrounded Z.  fp32 tensors are
  * multiplied at fp32 accuracy whatever the math mode says (as three bf16 planes; up to four rows by FMAs), 16-bit ones by
  * tcgen05.mma with fp32 accumulators.  fp32 tensors have fewer than 2^31 elements.
@@ -465,6 +467,7 @@ int alpha_engine_batchMatMulT2(float* C, const float* A, const float* B, int Bat
  * The gradients, from deltaY and the Z that the forward call kept:
  *   deltaZ = deltaY * act'(Z)          (glu: [deltaY * U * act'(G) | deltaY * act(G)], Z = [G | U])
  *   deltaX = deltaZ W,  deltaW = deltaZ^T X,  deltaB = column sums of deltaZ;  the residual's gradient is deltaY itself
+ * with deltaX, deltaW like X, W and deltaY, deltaB like Y, bias.
  * deltaX, deltaW and deltaB may each be NULL (not computed).  deltaZ is memory of the caller's, the size of Z, and may be Z
  * itself; it holds deltaZ rounded to the tensors' type afterwards.  ALPHA_ACT_NONE without gates needs neither Z nor deltaZ.
  * At 0 the slope of a LeakyReLU is k.  Results do not depend on scheduling (fixed summation orders, no atomics). */

@@ -26,7 +26,7 @@ def call(lib, rows=16, IC=64, OC=32, dtype=BF16, act=0, k=0.0, x=X, w=W, b=None,
 @pytest.mark.parametrize("glu", (False, True))
 @pytest.mark.parametrize("kw,word", [
     (dict(rows=0), "non-positive"), (dict(rows=-1), "non-positive"), (dict(IC=0), "non-positive"), (dict(OC=0), "non-positive"),
-    (dict(IC=60), "multiples of 8"), (dict(OC=36), "multiples of 8"), (dict(IC=62, dtype=0), "multiples of 4"),
+    (dict(IC=60), "multiple of 8"), (dict(IC=62, dtype=0), "multiple of 4"),
     (dict(dtype=3), "element type"), (dict(dtype=-1), "element type"), (dict(act=6), "activation"), (dict(act=-1), "activation"),
     (dict(act=1, k=float("nan")), "slope"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"),
     (dict(x=X + 8), "aligned"), (dict(w=W + 2), "aligned"), (dict(y=Y + 4), "aligned"), (dict(b=B + 8), "aligned"), (dict(z=Z + 8), "aligned"),
@@ -51,7 +51,7 @@ def delta(lib, rows=16, IC=64, OC=32, dtype=BF16, act=3, dy=Y, x=X, w=W, z=Z, dz
 
 @pytest.mark.parametrize("glu", (False, True))
 @pytest.mark.parametrize("kw,word", [
-    (dict(rows=0), "non-positive"), (dict(dtype=7), "element type"), (dict(act=9), "activation"), (dict(OC=33), "multiples"),
+    (dict(rows=0), "non-positive"), (dict(dtype=7), "element type"), (dict(act=9), "activation"), (dict(IC=33), "multiple"),
     (dict(dy=None), "null"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(z=None), "Z of the forward pass"), (dict(dz=None), "Z of the forward pass"),
     (dict(dx=None, dw=None, db=None), "no gradient"), (dict(dz=Y), "overlaps"), (dict(dz=Z + 16), "overlaps"), (dict(dx=X), "overlaps"), (dict(dw=W), "overlaps"),
     (dict(dx=Z), "overlap"), (dict(db=9 << 32), "overlap"), (dict(dx=(8 << 32) + 8), "aligned"), (dict(db=(10 << 32) + 2), "aligned"),

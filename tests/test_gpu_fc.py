@@ -589,3 +589,44 @@ def test_feed_forward_step(eng, dtype, tol, tokens):
     assert abs(float(norm) - float(n)) <= tol * float(n)
     for m, g in zip(master, grads[1:]):
         assert rel(m, g * min(1.0, 0.5 / (float(n) + 1e-6))) <= 2 * tol
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("glu", (False, True), ids=("fc", "glu"))
+@pytest.mark.parametrize("tile", (0, 1, 2, 2064))
+def test_what_padding_columns_hold_does_not_matter(eng, lib, dtype, glu, tile):
+    """OC = 44 in tensors of 48 columns, the last four of every input NaN."""
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    t = TYPES[dtype]
+    code = {"f32": 0, "bf16": 1, "f16": 2}[dtype]
+    IC, OC, P, H = 136, 44, 48, 2 if glu else 1
+    old = lib.set_option("FC_TILE", tile)
+    try:
+        for rows in (1, 9, 70, 300):
+            X, W, B = rand(gen, rows, IC, dtype=t), rand(gen, H * OC, IC, scale=0.1, dtype=t), rand(gen, H * OC, dtype=t)
+            R, dY = rand(gen, rows, OC, dtype=t), rand(gen, rows, OC, dtype=t)
+
+            def wide(a, n):                      # (..., n * OC) as (..., n, P) with NaN behind
+                out = torch.full(a.shape[:-1] + (n, P), float("nan"), dtype=t, device="cuda")
+                out[..., :OC] = a.reshape(a.shape[:-1] + (n, OC))
+                return out
+            for act in ("silu",) if glu else ("silu", "none"):
+                if glu:
+                    want, wz = eng.fullConnect_glu(X, W, B, act=act, save=True)
+                else:
+                    want, wz = eng.fullConnect(X, W, B, act=act, Residual=R, save=True)
+                Y, Z = torch.empty(rows, P, dtype=t, device="cuda"), torch.empty(rows, H, P, dtype=t, device="cuda")
+                if glu:
+                    eng.base.fullConnect_glu(Y, X, W, rows, IC, OC, code, lib.ACTS[act], 0.0, wide(B, 2), Z)
+                else:
+                    eng.base.fullConnect(Y, X, W, rows, IC, OC, code, lib.ACTS[act], 0.0, wide(B, 1), wide(R, 1), Z)
+                assert torch.equal(Y[:, :OC], want) and torch.equal(Z[..., :OC].reshape(rows, H * OC), wz)
+                grads = (eng.fullConnect_glu_delta if glu else eng.fullConnect_delta)(dY, X, W, wz, act=act, bias=True)
+                dX, dW, dB = torch.empty_like(X), torch.empty_like(W), torch.empty(H, P, dtype=t, device="cuda")
+                eng.base.fullConnect_delta(dX, dW, dB, wide(dY, 1), X, W, wide(wz, H), torch.empty_like(Z), rows, IC, OC, code, lib.ACTS[act], 0.0, glu)
+                for got, ref in ((dX, grads[0]), (dW, grads[1]), (dB[:, :OC].reshape(-1), grads[2])):
+                    # (fp32: where the padding makes a sum NaN it is formed once more by FMAs)
+                    assert torch.equal(got, ref) if dtype != "f32" else (got - ref).abs().max() <= 1e-5 * ref.abs().max()
+    finally:
+        lib.set_option("FC_TILE", old)
+    assert lib.device_status() == 0
