@@ -7,6 +7,7 @@
 #include "fc_small.cuh"
 #include "host_common.h"
 
+#include <algorithm>
 #include <initializer_list>
 
 using namespace alpha;
@@ -97,78 +98,97 @@ uint32_t tmem_columns(int bn, bool glu)
     return c;
 }
 
-// The plan of least estimated time, after 250 measured ones (512 x 4096 x 4096 in us: 64 columns 26, 112 21, 128 21, pairs 27; 64 x 4096 x 1024: 64
-// columns 13, shared by two 11.6, 32 shared by four 9.7).  64 steps of a tile take 0.1375 us (four MMAs of up
-// to 128 columns, 64 clocks each whatever they hold, as A is read from shared memory; wider tiles have two stages and are slower), of a pair's 0.285;
-// all tiles' operands come through L2 at 18 TB/s, W and X from DRAM at 5.2; a launch 4 us until its first tile and after its last (pairs 5.7),
-// and a shared tile its exchange, eight CTAs also the wait for a place for them.
-FcPlan pick_plan(const Product& q, int sms)
+// The plan of least estimated time, after some 500 measured ones (512 x 4096 x 4096 in us: 64 columns 26, 112 21, 128 21, pairs 27; 64 x 4096 x 1024: 64
+// columns 13, shared by two 11.6, 32 shared by four 9.7; 6656 x 73 x 7296: pairs 30, 128 columns 35, 64 45).  64 steps of a tile take 0.1375 us (four
+// MMAs of up to 128 columns, 64 clocks each whatever they hold, as A is read from shared memory), or what the ring's stages leave of a copy's 1.15 us;
+// a pair's 0.285; a tile's outputs 0.5 us and 0.008 a column, a pair's 2.1; all tiles' operands come through L2 at 18 TB/s, tensors from and
+// to DRAM at 5.2; a launch 4 us until its first tile and after its last (pairs 5.7), and a shared tile its exchange, eight CTAs also the wait for a
+// place for them.
+double plan_time(const Product& q, bool pair, int bn, int split, int sms, double* fixed, bool* fits)
 {
-    const int forced = option_fc_tile() == 2 ? 0 : option_fc_tile();
-    const long long cols = q.glu ? 2LL * q.cols : q.cols, blocks = (long long)q.k_halves * ((q.K + kFcBK - 1) / kFcBK), stages = (blocks + 1) / 2;
+    const long long cols = q.glu ? 2LL * q.cols : q.cols, blocks = (long long)q.k_halves * ((q.K + kFcBK - 1) / kFcBK);
+    const int out = q.glu ? bn / 2 : bn, bm = pair ? 256 : 128, ctas = pair ? 2 : 1;
+    const long long tiles = (long long)q.m_halves * ((q.rows + bm - 1) / bm) * ((q.cols + out - 1) / out), most = sms / (ctas * split);
+    *fits = most >= 1 && (split == 1 || tiles <= most);
+    if (!*fits) return 0.0;
+    const long long waves = (tiles + most - 1) / most, each = (blocks + split - 1) / split;
+    const int a_rows = q.A.mn || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
+    const int ring = static_cast<int>(kFcRing / (fc_blocks(false) * fc_block_bytes(false, a_rows, bn)));
+    const double step = pair ? 0.285 : std::max(0.1375, 0.575 / (std::min(ring, (int)kFcMaxStages) - 1));
+    const double tile = std::max(each * step, pair ? 2.1 : 0.5 + 0.008 * bn);
+    const double l2 = (double)tiles * blocks * (pair ? 512 : a_rows + bn) * 128 / 18e6;
+    const double mma = waves * tile, n = (double)q.rows * q.m_halves;
+    const double dram = 2e-6 * ((n + cols) * q.K * q.k_halves + n * (q.cols + (q.Z ? cols : 0) + (q.residual ? q.cols : 0))) / 5.2;
+    const double most_of = mma > l2 ? (mma > dram ? mma : dram) : (l2 > dram ? l2 : dram);
+    *fixed = (pair ? 5.7 : 4.0 + 0.006 * bn) + (split == 1 ? 0.0 : split == 2 ? 2.5 : split == 4 ? 4.0 : 12.0);
+    return 0.8 * most_of + 0.2 * (mma + l2 + dram);                // (the others are not quite hidden)
+}
+// Two products by one launch: their tiles fill the same waves.
+double two_time(const Product& x, const Product& w, const FcPlan& plan, int sms)
+{
+    double time = 0.0, fixed = 0.0;
+    const int most = sms / (plan.pair ? 2 : 1), bm = plan.pair ? 256 : 128;
+    double busy = 0.0;
+    for (const Product* q : {&x, &w}) {
+        bool fits;
+        const double t = plan_time(*q, plan.pair, plan.bn, 1, sms, &fixed, &fits);
+        const long long tiles = (long long)q->m_halves * ((q->rows + bm - 1) / bm) * ((q->cols + plan.bn - 1) / plan.bn), whole = (tiles + most - 1) / most;
+        time += t * tiles / (whole * most);                                      // (what it would be without idle places)
+        busy = std::max(busy, t / whole);
+    }
+    return fixed + std::max(busy, time + 0.5 * busy);
+}
+
+FcPlan pick_plan(const Product& q, int sms, double* time_of = nullptr)
+{
+    const int forced = option_fc_tile() == 2 || option_fc_tile() == 3 ? 0 : option_fc_tile();
+    const long long stages = ((long long)q.k_halves * ((q.K + kFcBK - 1) / kFcBK) + 1) / 2;
     FcPlan best{false, 64, 1};
     double least = 1e300;
     auto look = [&](bool pair, int bn, int split) {
-        const int out = q.glu ? bn / 2 : bn, bm = pair ? 256 : 128, ctas = pair ? 2 : 1;
-        const long long tiles = (long long)q.m_halves * ((q.rows + bm - 1) / bm) * ((q.cols + out - 1) / out), most = sms / (ctas * split);
-        if (most < 1 || (split > 1 && tiles > most)) return;
-        const long long waves = (tiles + most - 1) / most, each = (blocks + split - 1) / split;
-        const double step = pair ? 0.285 : 0.1375;
-        const double l2 = (double)tiles * blocks * (pair ? 512 : (q.A.mn || q.rows >= 128 ? 128 : q.rows) + bn) * 128 / 18e6;
-        const double mma = waves * each * step, dram = 2e-6 * ((double)q.rows * q.m_halves + cols) * q.K * q.k_halves / 5.2;
-        const double most_of = mma > l2 ? (mma > dram ? mma : dram) : (l2 > dram ? l2 : dram);
-        double time = 0.8 * most_of + 0.2 * (mma + l2 + dram);                // (the others are not quite hidden)
-        time += (pair ? 5.7 : 4.0 + 0.006 * bn) + (split == 1 ? 0.0 : split == 2 ? 2.5 : split == 4 ? 4.0 : 12.0);
+        bool fits;
+        double fixed = 0.0, time = plan_time(q, pair, bn, split, sms, &fixed, &fits);
+        if (!fits) return;
+        time += fixed;
         if (time < least) { least = time; best = FcPlan{pair, bn, split}; }
     };
     // (an operand that runs along its rows comes in boxes of 64 of them; no part of a shared tile is empty)
     const int unit = q.B.mn ? 64 : 16;
     auto parts = [&](int split) { return split == 1 || (split - 1) * ((stages + split - 1) / split) < stages; };
-    if (forced == 1 && sms >= 2) return FcPlan{true, 256, 1};
-    if (forced >= 1000) {
+    if (forced == 1 && sms >= 2) { look(true, 256, 1); best = FcPlan{true, 256, 1}; }
+    else if (forced >= 1000) {
         const int bn = forced % 1000 / unit * unit;
         for (int split = forced / 1000; split > 1 && bn >= unit && bn <= 256; split /= 2)
             if (split <= 8 && parts(split)) look(false, bn, split);
         if (least == 1e300 && bn >= unit && bn <= 256) look(false, bn, 1);
-        return best;
+    } else {
+        look(true, 256, 1);
+        for (int bn = unit; bn <= 128; bn += unit)
+            for (int split = 1; split <= 8; split *= 2)
+                if (parts(split)) look(false, bn, split);
     }
-    look(true, 256, 1);
-    for (int bn = unit; bn <= 128; bn += unit)
-        for (int split = 1; split <= 8; split *= 2)
-            if (parts(split)) look(false, bn, split);
+    if (time_of) *time_of = least;
     return best;
 }
 
-template <class T, bool PAIR, bool GLU>
-void launch_mma(const CUtensorMap& a, const CUtensorMap& b, const FcMma& p, int sms, cudaStream_t stream)
-{
-    const int group = PAIR ? 2 : p.split, total = p.m_tiles * p.n_tiles, most = sms / group;
-    const unsigned grid = static_cast<unsigned>(p.split > 1 || total < most ? total : most) * group;
-    const uint32_t smem = p.stages * fc_blocks(PAIR) * fc_block_bytes(PAIR, p.a_rows, p.bn) + kFcStaging + 1024 + 512;
-    allow_smem<fc_mma_kernel<T, PAIR, GLU>>();
-    launch_after_clusters(fc_mma_kernel<T, PAIR, GLU>, dim3(grid), kFcThreads, group > 1 ? group : 0, smem, stream, a, b, p);
-}
+// A product as the kernel takes it.
+struct Prepared { FcMma p; CUtensorMap a, b; };
 
-int launch_product(const Product& q, cudaStream_t stream)
+int prepare(const Product& q, const FcPlan& plan, int a_rows, int* status, Prepared* out)
 {
-    int sms = 0, *status = nullptr;
-    int rc = device_sms(&sms);
-    if (!rc) rc = device_status_word(&status);
-    if (rc) return rc;
-    const FcPlan plan = pick_plan(q, sms);
-    const int bm = plan.pair ? 256 : 128, bn = plan.bn, out = q.glu ? bn / 2 : bn, steps = kFcBK * fc_blocks(plan.pair);
-    FcMma p{};
+    const int bm = plan.pair ? 256 : 128, bn = plan.bn, cols_of = q.glu ? bn / 2 : bn, steps = kFcBK * fc_blocks(plan.pair);
+    FcMma& p = out->p;
+    p = FcMma{};
     p.rows = q.rows; p.cols = q.pitch;
     const int k_blocks = (q.K + kFcBK - 1) / kFcBK;
-    p.m_half = (q.rows + bm - 1) / bm; p.n_tiles = (q.cols + out - 1) / out;
+    p.m_half = (q.rows + bm - 1) / bm; p.n_tiles = (q.cols + cols_of - 1) / cols_of;
     p.k_half = q.k_halves > 1 ? k_blocks : 1 << 29;
     p.kb = static_cast<int>(((long long)k_blocks * q.k_halves * kFcBK + steps - 1) / steps);
-    if ((long long)p.m_half * q.m_halves * p.n_tiles > 2147483647LL / kFcGroupM) return fail(ALPHA_E_ARG, "fullConnect: more tiles than a launch takes");
+    if ((long long)p.m_half * q.m_halves * p.n_tiles > 2147483647LL / (2 * kFcGroupM)) return fail(ALPHA_E_ARG, "fullConnect: more tiles than a launch takes");
     p.m_tiles = p.m_half * q.m_halves;
     p.bn = bn; p.split = plan.split;
-    p.a_mn = q.A.mn; p.b_mn = q.B.mn;
-    p.a_rows = plan.pair || q.A.mn || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
-    const uint32_t stage = fc_blocks(plan.pair) * fc_block_bytes(plan.pair, p.a_rows, bn);
+    p.a_mn = q.A.mn; p.b_mn = q.B.mn; p.a_rows = a_rows;
+    const uint32_t stage = fc_blocks(plan.pair) * fc_block_bytes(plan.pair, a_rows, bn);
     p.stages = kFcRing / stage < kFcMaxStages ? kFcRing / stage : kFcMaxStages;
     // shared tiles: the ring holds a part's sums afterwards
     const uint32_t sums = (q.rows < 128 ? q.rows : 128) * (bn + 4) * 4;
@@ -178,20 +198,74 @@ int launch_product(const Product& q, cudaStream_t stream)
     p.tmem = tmem_columns(bn, q.glu);
     p.act = q.act; p.k = q.k; p.keep_z = q.Z != nullptr;
     p.bias = q.bias; p.residual = q.residual; p.Y = q.Y; p.Z = q.Z; p.status = status;
-    CUtensorMap a, b;
-    rc = q.A.mn ? make_map(&a, q.dtype, q.A, 64, 1, 64) : make_map(&a, q.dtype, q.A, 64, 1, p.a_rows);
-    if (!rc) rc = q.B.mn ? make_map(&b, q.dtype, q.B, 64, 64, 1) : make_map(&b, q.dtype, q.B, 64, plan.pair ? 128 : out, 1);
+    const int rc = q.A.mn ? make_map(&out->a, q.dtype, q.A, 64, 1, 64) : make_map(&out->a, q.dtype, q.A, 64, 1, a_rows);
     if (rc) return rc;
+    return q.B.mn ? make_map(&out->b, q.dtype, q.B, 64, 64, 1) : make_map(&out->b, q.dtype, q.B, 64, plan.pair ? 128 : cols_of, 1);
+}
+
+template <class T, bool PAIR, bool GLU, bool TWO>
+void launch_mma(const Prepared& x, const Prepared& y, int sms, cudaStream_t stream)
+{
+    const FcMma& p = x.p;
+    const int group = PAIR ? 2 : p.split, total = p.m_tiles * p.n_tiles + (TWO ? y.p.m_tiles * y.p.n_tiles : 0), most = sms / group;
+    const unsigned grid = static_cast<unsigned>(p.split > 1 || total < most ? total : most) * group;
+    const uint32_t smem = p.stages * fc_blocks(PAIR) * fc_block_bytes(PAIR, p.a_rows, p.bn) + kFcStaging + 1024 + 512;
+    allow_smem<fc_mma_kernel<T, PAIR, GLU, TWO>>();
+    launch_after_clusters(fc_mma_kernel<T, PAIR, GLU, TWO>, dim3(grid), kFcThreads, group > 1 ? group : 0, smem, stream, x.a, x.b, x.p, y.a, y.b, y.p);
+}
+
+// One product, or (other != nullptr) two of one type without gates by one launch.
+int launch_planned(const Product& q, const Product* other, const FcPlan& plan, int sms, int* status, cudaStream_t stream)
+{
+    Prepared x, y;
+    const int a_rows = plan.pair || q.A.mn || other || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
+    int rc = prepare(q, plan, a_rows, status, &x);
+    if (!rc && other) rc = prepare(*other, plan, a_rows, status, &y);
+    if (rc) return rc;
+    const Prepared& z = other ? y : x;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (q.glu) plan.pair ? launch_mma<T, true, true>(a, b, p, sms, stream) : launch_mma<T, false, true>(a, b, p, sms, stream);
-        else plan.pair ? launch_mma<T, true, false>(a, b, p, sms, stream) : launch_mma<T, false, false>(a, b, p, sms, stream);
+        if (other) plan.pair ? launch_mma<T, true, false, true>(x, z, sms, stream) : launch_mma<T, false, false, true>(x, z, sms, stream);
+        else if (q.glu) plan.pair ? launch_mma<T, true, true, false>(x, z, sms, stream) : launch_mma<T, false, true, false>(x, z, sms, stream);
+        else plan.pair ? launch_mma<T, true, false, false>(x, z, sms, stream) : launch_mma<T, false, false, false>(x, z, sms, stream);
     };
     if (q.dtype == ALPHA_BF16) go(__nv_bfloat16{});
     else go(__half{});
     note_launch("fc");
-    note_plan("fc %s%dx%d split=%d", plan.pair ? "pair " : "", bm, bn, plan.split);
+    note_plan("fc %s%s%dx%d split=%d", other ? "two " : "", plan.pair ? "pair " : "", plan.pair ? 256 : 128, plan.bn, plan.split);
     return launched("fc_mma_kernel");
+}
+
+int launch_product(const Product& q, cudaStream_t stream)
+{
+    int sms = 0, *status = nullptr;
+    int rc = device_sms(&sms);
+    if (!rc) rc = device_status_word(&status);
+    return rc ? rc : launch_planned(q, nullptr, pick_plan(q, sms), sms, status, stream);
+}
+
+// deltaX and deltaW: by a launch each, or together where the waves of both take less than those of either and a second launch's fill and drain.
+int launch_products(const Product& x, const Product& w, cudaStream_t stream)
+{
+    int sms = 0, *status = nullptr;
+    int rc = device_sms(&sms);
+    if (!rc) rc = device_status_word(&status);
+    if (rc) return rc;
+    FcPlan plan{false, 0, 1}, best{false, 0, 1};
+    double apart = 0.0, least = 1e300;
+    const FcPlan px = pick_plan(x, sms, &apart), pw = pick_plan(w, sms, &least);
+    apart += least;
+    least = 1e300;
+    const int forced = option_fc_tile();
+    for (int form = 0; form < 3 && x.rows >= 128; ++form) {
+        plan = form == 0 ? FcPlan{true, 256, 1} : FcPlan{false, form == 1 ? 128 : 64, 1};
+        if ((plan.pair && sms < 2) || (forced == 1 && !plan.pair) || forced == 3 || forced >= 1000) continue;
+        const double time = two_time(x, w, plan, sms);
+        if (time < least) { least = time; best = plan; }
+    }
+    if (best.bn && least < 0.97 * apart) return launch_planned(x, &w, best, sms, status, stream);
+    rc = launch_planned(x, nullptr, px, sms, status, stream);
+    return rc ? rc : launch_planned(w, nullptr, pw, sms, status, stream);
 }
 
 // ---- fp32 products ----------------------------------------------------------------------------------------------
@@ -495,7 +569,7 @@ int forward(const char* what, const AlphaFcShape* s, const void* X, const void* 
     if (rc) return rc;
     // (of the gated block from nine rows on only where W is small: 2 x 11008 x 4096 on 16 rows 39 us, by tiles 37)
     const bool token = s->rows <= 8 || (s->rows <= kTokenRows && (!glu || (long long)s->OC * s->IC <= 8 << 20));
-    if ((s->dtype == ALPHA_F32 ? s->rows <= kSmallRows : token) && !option_fc_tile()) {
+    if ((s->dtype == ALPHA_F32 ? s->rows <= kSmallRows : token) && (!option_fc_tile() || option_fc_tile() == 3)) {
         if (dry_run()) return ALPHA_OK;
         switch (s->dtype) {
         case ALPHA_F32: return glu ? launch_small<true>(s, X, W, bias, residual, Z, Y, stream) : launch_small<false>(s, X, W, bias, residual, Z, Y, stream);
@@ -578,10 +652,13 @@ int delta(const char* what, const AlphaFcShape* s, const void* dY, const void* X
     if (dry_run()) return ALPHA_OK;
     const long long IC = s->IC, OC = s->OC, p = pitch, n = s->rows;
     const int halves = glu ? 2 : 1;
-    if (dX) rc = launch_product(Product{s->dtype, s->rows, s->IC, s->IC, s->OC, 1, halves, false, Operand{d, false, OC, halves, n, p, halves * p}, Operand{W, true, IC, OC, halves, IC, OC * IC},
-                                        nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f}, stream);
-    if (!rc && dW) rc = launch_product(Product{s->dtype, s->OC, s->IC, s->IC, s->rows, halves, 1, false, Operand{d, true, OC, halves, n, p, halves * p}, Operand{X, true, IC, n, 1, IC, n * IC},
-                                               nullptr, nullptr, nullptr, dW, ALPHA_ACT_NONE, 0.f}, stream);
+    const Product x{s->dtype, s->rows, s->IC, s->IC, s->OC, 1, halves, false, Operand{d, false, OC, halves, n, p, halves * p}, Operand{W, true, IC, OC, halves, IC, OC * IC},
+                    nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f};
+    const Product w{s->dtype, s->OC, s->IC, s->IC, s->rows, halves, 1, false, Operand{d, true, OC, halves, n, p, halves * p}, Operand{X, true, IC, n, 1, IC, n * IC},
+                    nullptr, nullptr, nullptr, dW, ALPHA_ACT_NONE, 0.f};
+    if (dX && dW) return launch_products(x, w, stream);
+    if (dX) rc = launch_product(x, stream);
+    if (dW) rc = launch_product(w, stream);
     return rc;
 }
 

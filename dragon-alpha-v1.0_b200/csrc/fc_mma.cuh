@@ -45,9 +45,11 @@ struct FcMma {
 __host__ __device__ constexpr int fc_blocks(bool pair) { return pair ? 1 : 2; }
 __host__ __device__ constexpr uint32_t fc_block_bytes(bool pair, int a_rows, int bn) { return static_cast<uint32_t>(a_rows + (pair ? bn / 2 : bn)) * 128; }
 
-template <class T, bool PAIR, bool GLU>
+// TWO: the tiles of a second product of the same geometry follow those of the first (deltaX and deltaW, neither of which may fill the SMs).
+template <class T, bool PAIR, bool GLU, bool TWO>
 __global__ void __launch_bounds__(kFcThreads, 1)
-    fc_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ FcMma p)
+    fc_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ FcMma p, const __grid_constant__ CUtensorMap tmA2,
+                  const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ FcMma p2)
 {
     constexpr int CTAS = PAIR ? 2 : 1, KB = fc_blocks(PAIR);
     const int BN = PAIR ? 256 : p.bn, OUT = GLU ? BN / 2 : BN, S = PAIR ? 6 : p.stages, split = PAIR ? 1 : p.split;
@@ -66,6 +68,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         for (int i = 0; i < 2; ++i) { mbar_init(&bars[2 * kFcMaxStages + i], 1); mbar_init(&bars[2 * kFcMaxStages + 2 + i], 8 * CTAS); }
         fence_barrier_init();
         prefetch_tmap(&tmA); prefetch_tmap(&tmB);
+        if (TWO) { prefetch_tmap(&tmA2); prefetch_tmap(&tmB2); }
     }
     if (warp == 1) {
         if constexpr (PAIR) { tmem_alloc_pair(tmem_holder, 512); tmem_relinquish_pair(); }
@@ -80,15 +83,22 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     const uint32_t tmem_base = *tmem_holder;
 
     // (shared tiles: the launch has a cluster for each)
-    const int total = p.m_tiles * p.n_tiles, step = gridDim.x / (CTAS * split), first = blockIdx.x / (CTAS * split);
-    const int k_each = (p.kb + split - 1) / split, k_begin = PAIR ? 0 : static_cast<int>(rank) * k_each, k_end = k_begin + k_each < p.kb ? k_begin + k_each : p.kb;
-    int hm = 0;                                   // half of the output's rows
+    const int tiles = p.m_tiles * p.n_tiles, total = tiles + (TWO ? p2.m_tiles * p2.n_tiles : 0), step = gridDim.x / (CTAS * split), first = blockIdx.x / (CTAS * split);
+    const FcMma* cur = &p;                        // the product of the tile at hand
+    int hm = 0;                                   // the half of its rows
     auto tile_at = [&](int t, int& m0, int& n0) {
-        const int per = kFcGroupM * p.n_tiles, g = t / per, r = t - g * per, left = p.m_tiles - g * kFcGroupM, rows = left < kFcGroupM ? left : kFcGroupM;
+        if (TWO) cur = t < tiles ? &p : &p2;
+        if (TWO && t >= tiles) t -= tiles;
+        const int per = kFcGroupM * cur->n_tiles, g = t / per, r = t - g * per, left = cur->m_tiles - g * kFcGroupM, rows = left < kFcGroupM ? left : kFcGroupM;
         const int n = r / rows, m = g * kFcGroupM + r - n * rows;
-        hm = m >= p.m_half ? 1 : 0;
-        m0 = (m - hm * p.m_half) * (128 * CTAS) + (PAIR ? static_cast<int>(rank) * 128 : 0);
+        hm = m >= cur->m_half ? 1 : 0;
+        m0 = (m - hm * cur->m_half) * (128 * CTAS) + (PAIR ? static_cast<int>(rank) * 128 : 0);
         n0 = n * OUT;
+    };
+    auto steps_of = [&](int& begin, int& end) {
+        const int each = (cur->kb + split - 1) / split;
+        begin = PAIR ? 0 : static_cast<int>(rank) * each;
+        end = begin + each < cur->kb ? begin + each : cur->kb;
     };
     const uint32_t smem_a = smem_u32(smem);
     const int quad = warp & 3, half = (warp - 2) >> 2;
@@ -105,7 +115,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     auto lane_word = [&](int j) { return word_at + sbuf * 2048 + j * 512; };
     auto inside = [&](int row0, int col0, int width, int j) {
         const int c = 8 * (lane & 3);
-        return row0 + 8 * j + (lane >> 2) < p.rows && c < width && col0 + c < p.cols;
+        return row0 + 8 * j + (lane >> 2) < cur->rows && c < width && col0 + c < cur->cols;
     };
     auto put = [&](const float (&f)[32], T* tensor, size_t pitch, int row0, int col0, int width) {
 #pragma unroll
@@ -124,9 +134,9 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     };
     // The words of R that put() will write over, or zeros (R may be Y itself: not by the read-only path).
     auto fetch = [&](uint4 (&r)[4], int row0, int col0, int width) {
-        const T* from = static_cast<const T*>(p.residual) + static_cast<size_t>(row0 + (lane >> 2)) * p.cols + col0 + 8 * (lane & 3);
+        const T* from = static_cast<const T*>(cur->residual) + static_cast<size_t>(row0 + (lane >> 2)) * cur->cols + col0 + 8 * (lane & 3);
 #pragma unroll
-        for (int j = 0; j < 4; ++j, from += 8 * p.cols) r[j] = inside(row0, col0, width, j) ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 4; ++j, from += 8 * cur->cols) r[j] = inside(row0, col0, width, j) ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
     };
     auto add_fetched = [&](float (&f)[32], const uint4 (&r)[4]) {
 #pragma unroll
@@ -147,7 +157,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     auto add_bias = [&](float (&f)[32], const T* from, int col0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            if (col0 + 8 * q < p.cols) {
+            if (col0 + 8 * q < cur->cols) {
                 float b[8];
                 Word16<T>::load(__ldg(reinterpret_cast<const uint4*>(from + col0 + 8 * q)), b);
 #pragma unroll
@@ -156,29 +166,29 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     };
     // The epilogue of 32 rows x (up to) 32 columns: the sums of a lane's row in z (glu: and u), the words of R in r.
     auto finish = [&](float (&z)[32], float (&u)[32], const uint4 (&r)[4], int row0, int col0, int width) {
-        const T* bias = static_cast<const T*>(p.bias);
-        T *Y = static_cast<T*>(p.Y) + (hm ? static_cast<size_t>(p.rows) * p.cols : 0), *Z = static_cast<T*>(p.Z);
+        const T* bias = static_cast<const T*>(cur->bias);
+        T *Y = static_cast<T*>(cur->Y) + (hm ? static_cast<size_t>(cur->rows) * cur->cols : 0), *Z = static_cast<T*>(cur->Z);
         if constexpr (GLU) {
-            if (bias) { add_bias(z, bias, col0); add_bias(u, bias + p.cols, col0); }
-            if (p.keep_z) {
-                const size_t pitch = 2 * static_cast<size_t>(p.cols);
+            if (bias) { add_bias(z, bias, col0); add_bias(u, bias + cur->cols, col0); }
+            if (cur->keep_z) {
+                const size_t pitch = 2 * static_cast<size_t>(cur->cols);
                 put(z, Z, pitch, row0, col0, width);
-                put(u, Z + p.cols, pitch, row0, col0, width);
+                put(u, Z + cur->cols, pitch, row0, col0, width);
             }
-            with_act(p.act, [&](auto a) {
+            with_act(cur->act, [&](auto a) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, true>(z[i], p.k) * u[i];
+                for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, true>(z[i], cur->k) * u[i];
             });
         } else {
             if (bias) add_bias(z, bias, col0);
-            if (p.keep_z) put(z, Z, p.cols, row0, col0, width);
-            with_act(p.act, [&](auto a) {
+            if (cur->keep_z) put(z, Z, cur->cols, row0, col0, width);
+            with_act(cur->act, [&](auto a) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, true>(z[i], p.k);
+                for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, true>(z[i], cur->k);
             });
-            if (p.residual) add_fetched(z, r);
+            if (cur->residual) add_fetched(z, r);
         }
-        put(z, Y, p.cols, row0, col0, width);
+        put(z, Y, cur->cols, row0, col0, width);
     };
 
     // Both issuing warps walk their loops as a whole, so that counters, coordinates and descriptors are uniform values; one lane issues.
@@ -195,6 +205,10 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         for (int t = first; t < total && ok; t += step) {
             int m0, n0;
             tile_at(t, m0, n0);
+            int k_begin, k_end;
+            steps_of(k_begin, k_end);
+            const CUtensorMap *mA = TWO && t >= tiles ? &tmA2 : &tmA, *mB = TWO && t >= tiles ? &tmB2 : &tmB;
+            const int a_mn = cur->a_mn, b_mn = cur->b_mn, k_half = cur->k_half;
             for (int kb = k_begin; kb < k_end; ++kb) {
                 ok = __all_sync(0xffffffffu, mbar_wait_a(empty_0 + 8 * rp.idx, rp.phase ^ 1));
                 if (!ok) { report(p.status, kStatusProducerTimeout); settle(); break; }
@@ -205,23 +219,23 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                     for (int q = 0; q < KB; ++q) {
                         const uint32_t a = base + rp.idx * kStage + q * kBlock, b = a + kA;
                         // (the block after the last of an odd number lies past both halves)
-                        const int block = kb * KB + q, hk = block >= p.k_half ? (block - p.k_half >= p.k_half ? 2 : 1) : 0, k0 = (block - hk * p.k_half) * kFcBK;
-                        if (p.a_mn) {
+                        const int block = kb * KB + q, hk = block >= k_half ? (block - k_half >= k_half ? 2 : 1) : 0, k0 = (block - hk * k_half) * kFcBK;
+                        if (a_mn) {
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) load(a + j * 8192, &tmA, bar, m0 + 64 * j, hm, k0);
+                            for (int j = 0; j < 2; ++j) load(a + j * 8192, mA, bar, m0 + 64 * j, hm, k0);
                         } else {
-                            load(a, &tmA, bar, k0, hk, m0);
+                            load(a, mA, bar, k0, hk, m0);
                         }
                         if constexpr (GLU) {
                             // columns [gate | up] of the accumulator
-                            if constexpr (PAIR) load(b, &tmB, bar, k0, n0, my);
-                            else { load(b, &tmB, bar, k0, n0, 0); load(b + kB / 2, &tmB, bar, k0, n0, 1); }
+                            if constexpr (PAIR) load(b, mB, bar, k0, n0, my);
+                            else { load(b, mB, bar, k0, n0, 0); load(b + kB / 2, mB, bar, k0, n0, 1); }
                         } else {
                             const int b0 = n0 + my * 128;
-                            if (p.b_mn) {
-                                for (int j = 0; j < static_cast<int>(kB >> 13); ++j) load(b + j * 8192, &tmB, bar, b0 + 64 * j, k0, hk);
+                            if (b_mn) {
+                                for (int j = 0; j < static_cast<int>(kB >> 13); ++j) load(b + j * 8192, mB, bar, b0 + 64 * j, k0, hk);
                             } else {
-                                load(b, &tmB, bar, k0, b0, 0);
+                                load(b, mB, bar, k0, b0, 0);
                             }
                         }
                     }
@@ -234,8 +248,6 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         if (!PAIR || rank == 0) {
             constexpr uint32_t dhi = (1024u >> 4) | (1u << 14) | (static_cast<uint32_t>(kSwizzle128B) << 29);
             const uint32_t base = __shfl_sync(0xffffffffu, smem_a, 0), tmem = __shfl_sync(0xffffffffu, tmem_base, 0), elected = elect_one();
-            const uint32_t a_k = p.a_mn ? 128u : 2u, b_k = p.b_mn ? 128u : 2u;               // 16 steps further, in 16-byte units
-            const uint32_t a_lo0 = smem_desc_lo(base, p.a_mn ? 8192u : 16u), b_lo0 = smem_desc_lo(base + kA, p.b_mn ? 8192u : 16u);
             const uint32_t full_0 = __shfl_sync(0xffffffffu, full_a, 0), empty_0 = full_0 + 8 * kFcMaxStages, afull_0 = empty_0 + 8 * kFcMaxStages, aempty_0 = afull_0 + 16;
             auto commit = [&](uint32_t bar) {
                 if constexpr (PAIR) mma_commit_both(bar);
@@ -250,6 +262,11 @@ __global__ void __launch_bounds__(kFcThreads, 1)
             RingPos rp, ap;
             bool next = false;                            // the stage at rp is known to be full
             for (int t = first; t < total && ok; t += step) {
+                if (TWO) cur = t < tiles ? &p : &p2;
+                int k_begin, k_end;
+                steps_of(k_begin, k_end);
+                const uint32_t a_k = cur->a_mn ? 128u : 2u, b_k = cur->b_mn ? 128u : 2u, idesc = cur->idesc;      // 16 steps further, in 16-byte units
+                const uint32_t a_lo0 = smem_desc_lo(base, cur->a_mn ? 8192u : 16u), b_lo0 = smem_desc_lo(base + kA, cur->b_mn ? 8192u : 16u);
                 if (!wait(aempty_0 + 8 * ap.idx, ap.phase ^ 1)) break;
                 tc_fence_after_sync();
                 const uint32_t d = tmem + ap.idx * acc_pitch;
@@ -261,7 +278,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                     for (uint32_t q = 0; q < KB; ++q)
 #pragma unroll
                         for (uint32_t kk = 0; kk < 4; ++kk)
-                            mma_16bit<PAIR>(d, a + q * (kBlock >> 4) + kk * a_k, dhi, b + q * (kBlock >> 4) + kk * b_k, dhi, p.idesc, kb > k_begin || q || kk ? 1u : 0u, elected);
+                            mma_16bit<PAIR>(d, a + q * (kBlock >> 4) + kk * a_k, dhi, b + q * (kBlock >> 4) + kk * b_k, dhi, idesc, kb > k_begin || q || kk ? 1u : 0u, elected);
                     if (elected) commit(done);
                     if (++rp.idx == S) { rp.idx = 0; rp.phase ^= 1u; }
                     next = mbar_test_a<PAIR>(full_0 + 8 * rp.idx, rp.phase);     // (beside the MMAs just issued)
@@ -287,13 +304,13 @@ __global__ void __launch_bounds__(kFcThreads, 1)
             const int row0 = m0 + quad * 32;
             // R: the next tile's to L2, and the first chunk of this one before the sums are there (8192 x 64 x 8192 with R 90 us without the former)
             uint4 r[4] = {};
-            const bool fetching = !GLU && p.residual && row0 < p.rows && (PAIR || split == 1);
-            if (!GLU && p.residual && (PAIR || split == 1)) {
+            const bool fetching = !GLU && cur->residual && row0 < cur->rows && (PAIR || split == 1);
+            if (!GLU && cur->residual && (PAIR || split == 1)) {
                 int m1, n1;
                 tile_at(t + step < total ? t + step : t, m1, n1);       // (one half: R goes with a forward product)
                 const int row = m1 + quad * 32 + lane;
                 for (int c = half * 32; c < OUT; c += 64)
-                    if (row < p.rows && n1 + c < p.cols) prefetch_l2(static_cast<const T*>(p.residual) + static_cast<size_t>(row) * p.cols + n1 + c);
+                    if (row < cur->rows && n1 + c < cur->cols) prefetch_l2(static_cast<const T*>(cur->residual) + static_cast<size_t>(row) * cur->cols + n1 + c);
             }
             if (fetching) fetch(r, row0, n0 + half * 32, OUT - half * 32);
             ok = mbar_wait_a(afull_a + 8 * ap.idx, ap.phase);
@@ -311,7 +328,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                 }
             };
             bool held = true;
-            if (row0 < p.rows) {
+            if (row0 < cur->rows) {
                 if (!PAIR && split > 1) {
                     // the ring is idle: [row][column] with four floats more, so that the words of eight rows lie in different banks
                     const uint32_t to = smem_a + static_cast<uint32_t>(quad * 32 + lane) * (BN + 4) * 4;
@@ -319,7 +336,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                     for (int c = half * 32; c < BN; c += 64) {
                         float z[32];
                         load32(d + c, z);
-                        if (row0 + lane < p.rows)
+                        if (row0 + lane < cur->rows)
 #pragma unroll
                             for (int q = 0; q < 8; ++q)
                                 if (c + 4 * q < BN) st_shared_v4(to + (c + 4 * q) * 4, make_float4(z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]));
@@ -327,11 +344,11 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                 } else {
 #pragma unroll 1
                     for (int c = half * 32; c < OUT; c += 64) {
-                        if (n0 + c >= p.cols) break;
+                        if (n0 + c >= cur->cols) break;
                         float z[32], u[32];
                         load32(d + c, z);
                         if constexpr (GLU) load32(d + OUT + c, u);
-                        if (c + 64 >= OUT || n0 + c + 64 >= p.cols) { give_back(); held = false; }
+                        if (c + 64 >= OUT || n0 + c + 64 >= cur->cols) { give_back(); held = false; }
                         finish(z, u, r, row0, n0 + c, OUT - c);
                         if (fetching && c + 64 < OUT) fetch(r, row0, n0 + c + 64, OUT - c - 64);
                     }
@@ -348,15 +365,15 @@ __global__ void __launch_bounds__(kFcThreads, 1)
             int m0, n0;
             tile_at(first, m0, n0);
             // shares of 32 rows x 32 columns, CTAs and warps in turn
-            const int quads = (p.rows - m0 + 31) / 32 < 4 ? (p.rows - m0 + 31) / 32 : 4, chunks = (OUT + 31) / 32;
+            const int quads = (cur->rows - m0 + 31) / 32 < 4 ? (cur->rows - m0 + 31) / 32 : 4, chunks = (OUT + 31) / 32;
             for (int i = static_cast<int>(rank) * 8 + warp - 2; i < quads * chunks; i += split * 8) {
                 const int q4 = i / chunks, c = (i - q4 * chunks) * 32, row0 = m0 + q4 * 32;
-                if (n0 + c >= p.cols) continue;
+                if (n0 + c >= cur->cols) continue;
                 const uint32_t from = smem_a + static_cast<uint32_t>(q4 * 32 + lane) * (BN + 4) * 4;
                 float z[32], u[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) z[j] = u[j] = 0.f;
-                if (row0 + lane < p.rows)
+                if (row0 + lane < cur->rows)
                     for (int r = 0; r < split; ++r) {
                         const uint32_t peer = mapa_u32(from, r);
 #pragma unroll
@@ -371,7 +388,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                         }
                     }
                 uint4 r[4] = {};
-                if (!GLU && p.residual) fetch(r, row0, n0 + c, OUT - c);
+                if (!GLU && cur->residual) fetch(r, row0, n0 + c, OUT - c);
                 finish(z, u, r, row0, n0 + c, OUT - c);
             }
         }

@@ -106,8 +106,8 @@ def test_forward_activations(eng, lib, dtype, act, glu, rows):
     forward_case(eng, lib, dtype, rows, 256, 136, act, glu, bias=True, residual=not glu, save=True)
 
 
-# CTA pairs, the plan by cost, tiles of some widths, tiles shared by 2, 4 and 8 CTAs
-@pytest.mark.parametrize("tile", (1, 2, 1016, 1064, 1112, 1256, 2080, 4048, 8256))
+# CTA pairs, the plan by cost with deltaX and deltaW together or apart, tiles of some widths, tiles shared by 2, 4 and 8 CTAs
+@pytest.mark.parametrize("tile", (1, 2, 3, 1016, 1064, 1112, 1256, 2080, 4048, 8256))
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("glu", (False, True), ids=("fc", "glu"))
 @pytest.mark.parametrize("shape", [(1, 64, 8), (77, 200, 136), (700, 520, 1304), (2500, 128, 1544)], ids=lambda s: "x".join(map(str, s)))
@@ -169,8 +169,8 @@ def test_delta_activations(eng, lib, dtype, act, glu):
     delta_case(eng, lib, dtype, 150, 136, 200, act, glu, bias=act != "silu")
 
 
-# CTA pairs, the plan by cost, tiles of some widths, tiles shared by 2, 4 and 8 CTAs
-@pytest.mark.parametrize("tile", (1, 2, 1016, 1064, 1112, 1256, 2080, 4048, 8256))
+# CTA pairs, the plan by cost with deltaX and deltaW together or apart, tiles of some widths, tiles shared by 2, 4 and 8 CTAs
+@pytest.mark.parametrize("tile", (1, 2, 3, 1016, 1064, 1112, 1256, 2080, 4048, 8256))
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(3, 8, 16), (700, 520, 1304), (1500, 1544, 200)], ids=lambda s: "x".join(map(str, s)))
 def test_delta_tiles(eng, lib, dtype, tile, shape):
@@ -630,3 +630,27 @@ def test_what_padding_columns_hold_does_not_matter(eng, lib, dtype, glu, tile):
     finally:
         lib.set_option("FC_TILE", old)
     assert lib.device_status() == 0
+
+
+@pytest.mark.parametrize("rows,IC,OC", [(608, 536, 745), (1005, 560, 1488), (658, 144, 723), (1044, 664, 358), (128, 72, 40), (4169, 936, 1422)])
+@pytest.mark.parametrize("glu", (False, True), ids=("fc", "glu"))
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+def test_both_gradients_by_one_launch(eng, lib, dtype, glu, rows, IC, OC):
+    """deltaX and deltaW in one launch have the bits of a launch each of the same tiles, and the same sums in any case."""
+    delta_case(eng, lib, dtype, rows, IC, OC, "silu", glu, True)
+    gen = torch.Generator(device="cuda").manual_seed(18)
+    t = TYPES[dtype]
+    H = 2 if glu else 1
+    X, W, dY, Z = rand(gen, rows, IC, dtype=t), rand(gen, H * OC, IC, scale=0.1, dtype=t), rand(gen, rows, OC, dtype=t), rand(gen, rows, H * OC, dtype=t)
+    fn = eng.fullConnect_glu_delta if glu else eng.fullConnect_delta
+    both = fn(dY, X, W, Z, act="silu")
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(both[:2], fn(dY, X, W, Z, act="silu")[:2]))
+    old = lib.set_option("FC_TILE", 3)
+    try:
+        apart = fn(dY, X, W, Z, act="silu")
+    finally:
+        lib.set_option("FC_TILE", old)
+    for a, b in zip(both[:2], apart[:2]):
+        # (a reduction split in another way differs in the last place)
+        assert ((a.double() - b.double()).abs() <= torch.finfo(t).eps * b.double().abs() + 2e-3 * torch.finfo(t).eps / 2.0 ** -7 * b.double().abs().max()).all()
