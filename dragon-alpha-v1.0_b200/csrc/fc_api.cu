@@ -39,10 +39,13 @@ int check_spans(const char* what, std::initializer_list<Span> in, std::initializ
     return ALPHA_OK;
 }
 
+constexpr int kMostDim = 2147483647 - 1023;
 int check_fc(const char* what, const AlphaFcShape* s, bool glu)
 {
     if (!s) return fail(ALPHA_E_ARG, "%s: null shape", what);
     if (s->rows <= 0 || s->IC <= 0 || s->OC <= 0) return fail(ALPHA_E_ARG, "%s: non-positive dimension (rows=%d IC=%d OC=%d)", what, s->rows, s->IC, s->OC);
+    // (a tile's last row or column, past the tensor's, is an int too)
+    if (s->rows > kMostDim || s->IC > kMostDim || s->OC > kMostDim) return fail(ALPHA_E_ARG, "%s: dimension of more than %d (rows=%d IC=%d OC=%d)", what, kMostDim, s->rows, s->IC, s->OC);
     if (s->dtype != ALPHA_F32 && s->dtype != ALPHA_BF16 && s->dtype != ALPHA_F16) return fail(ALPHA_E_ARG, "%s: unknown element type %d", what, s->dtype);
     if (s->act < ALPHA_ACT_NONE || s->act > ALPHA_ACT_GELU_TANH) return fail(ALPHA_E_ARG, "%s: unknown activation %d", what, s->act);
     if (s->act == ALPHA_ACT_LEAKY_RELU && !(s->k == s->k)) return fail(ALPHA_E_ARG, "%s: slope is NaN", what);

@@ -161,7 +161,7 @@ template <> __device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], u
 template <class T, int NT, bool GLU>
 __global__ void __launch_bounds__(256) fc_token_kernel(const __grid_constant__ FcSmall p)
 {
-        constexpr int MT = GLU ? 2 : 1, UNROLL = (GLU ? 2 : 4) / NT, COLS = 8 * NT;
+    constexpr int MT = GLU ? 2 : 1, UNROLL = (GLU ? 2 : 4) / NT, COLS = 8 * NT;
     __shared__ float part[8][MT][16][COLS + 1];
     const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0, block = blockIdx.x / p.split;
     grid_dependency_wait();

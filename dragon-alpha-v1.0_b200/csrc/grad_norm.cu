@@ -14,6 +14,7 @@
 #include "host_common.h"
 
 #include <algorithm>
+#include <exception>
 #include <vector>
 
 namespace alpha {
@@ -222,7 +223,11 @@ int check_grads(const char* what, int n, const AlphaGrad* grads, const float* no
     if (!norm || (reinterpret_cast<uintptr_t>(norm) & 3)) return fail(ALPHA_E_ARG, "%s: norm must be a device pointer to a float", what);
     struct Range { uintptr_t from, to; bool write; };
     std::vector<Range> ranges;
-    ranges.reserve(2 * static_cast<size_t>(n) + 1);
+    try {
+        ranges.reserve(2 * static_cast<size_t>(n) + 1);
+    } catch (const std::exception&) {
+        return fail(ALPHA_E_NOSCRATCH, "%s: no host memory to check %d tensors", what, n);
+    }
     auto add = [&](const void* p, size_t bytes, bool write) { ranges.push_back(Range{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, write}); };
     add(norm, sizeof(float), true);
     for (int i = 0; i < n; ++i) {

@@ -436,6 +436,8 @@ def _fc_plan(what, glu, xs, ws, dtype):
     rows, unit = 1, 4 if dtype == torch.float32 else 8
     for n in lead:
         rows *= n
+    if max(rows, IC, OC) > 2 ** 31 - 1024:       # (an int of the library's)
+        raise ValueError("%s: X %s against W %s is too large" % (what, tuple(xs), tuple(ws)))
     return IC, OC, -(-IC // unit) * unit, -(-OC // 8) * 8, rows, halves, lead + (OC,), lead + (halves * OC,), (halves * OC,)
 
 

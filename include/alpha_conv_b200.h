@@ -462,7 +462,7 @@ int alpha_engine_batchMatMulT2(float* C, const float* A, const float* B, int Bat
  * overlap an input (ALPHA_E_ARG).
  * Sums, bias, activation and residual are fp32 and an output is rounded once; Y comes from the unrounded Z.  fp32 tensors are
  * multiplied at fp32 accuracy whatever the math mode says (as three bf16 planes; up to four rows by FMAs), 16-bit ones by
- * tcgen05.mma with fp32 accumulators.  fp32 tensors have fewer than 2^31 elements.
+ * tcgen05.mma with fp32 accumulators.  fp32 tensors have fewer than 2^31 elements; rows, IC and OC are at most 2^31 - 1024.
  *
  * The gradients, from deltaY and the Z that the forward call kept:
  *   deltaZ = deltaY * act'(Z)          (glu: [deltaY * U * act'(G) | deltaY * act(G)], Z = [G | U])

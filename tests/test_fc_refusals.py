@@ -1,5 +1,6 @@
 """What fullConnect, its gradients and clip_grad_norm refuse, at the C ABI: every check comes before the device is looked at."""
 import ctypes as C
+import struct
 
 import pytest
 
@@ -31,6 +32,7 @@ def call(lib, rows=16, IC=64, OC=32, dtype=BF16, act=0, k=0.0, x=X, w=W, b=None,
     (dict(act=1, k=float("nan")), "slope"), (dict(x=None), "null"), (dict(w=None), "null"), (dict(y=None), "null"),
     (dict(x=X + 8), "aligned"), (dict(w=W + 2), "aligned"), (dict(y=Y + 4), "aligned"), (dict(b=B + 8), "aligned"), (dict(z=Z + 8), "aligned"),
     (dict(y=X), "overlaps"), (dict(y=X + 16 * 64 * 2 - 16), "overlaps"), (dict(z=W), "overlaps"), (dict(z=Y), "overlap"), (dict(b=Y), "overlaps"),
+    (dict(rows=2 ** 31 - 1023), "dimension"), (dict(IC=2 ** 31 - 8), "dimension"), (dict(OC=2 ** 31 - 1), "dimension"),
     (dict(rows=1 << 20, IC=4096, dtype=0), "2^31-1"), (dict(rows=1 << 20, OC=4096, dtype=0), "2^31-1"),
 ])
 def test_forward(lib, glu, kw, word):
@@ -128,3 +130,24 @@ def test_engine_grads(eng):
         eng.clip_grad_norm([_t(4)], 1.0)
     with pytest.raises(ValueError, match="on one GPU"):
         eng.grad_norm([_t(4)])
+
+
+@pytest.mark.parametrize("glu", (False, True))
+def test_engine_sizes_past_an_int(eng, glu):
+    torch = pytest.importorskip("torch")
+    t = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device="meta")
+    for x, w in ((t(2 ** 31, 8), t(16, 8)), (t(2 ** 16, 2 ** 15, 8), t(16, 8)), (t(2, 2 ** 31), t(16, 2 ** 31)), (t(2, 8), t(2 ** 32, 8))):
+        with pytest.raises(ValueError, match="too large"):
+            (eng.fullConnect_glu if glu else eng.fullConnect)(x, w)
+
+
+@pytest.mark.parametrize("job,dtype,word", [
+    ((X, 3, 5, Y, 3, 8), 3, "element type"), ((X, 3, 5, Y, 3, 8), -1, "element type"), ((0, 3, 5, Y, 3, 8), 1, "null"), ((X, 3, 5, 0, 3, 8), 1, "null"),
+    ((X, 0, 5, Y, 3, 8), 1, "bad shape"), ((X, 3, 0, Y, 3, 8), 1, "bad shape"), ((X, 3, 5, Y, 2, 8), 1, "bad shape"), ((X, 3, 9, Y, 3, 8), 1, "bad shape"),
+    ((X, 3, 5, Y, 3, 12), 1, "bad shape"), ((X, 3, 5, Y, 3, 6), 0, "bad shape"), ((X, 3, 5, Y, 3, 1 << 31), 1, "bad shape"),
+    ((X + 1, 3, 5, Y, 3, 8), 1, "aligned"), ((X + 2, 3, 5, Y, 3, 8), 0, "aligned"), ((X, 3, 5, Y + 8, 3, 8), 1, "aligned"),
+])
+def test_pad_rows_typed(lib, job, dtype, word):
+    refused(lib, lib.load().alpha_pad_rows_typed(1, struct.pack("6q", *job), dtype, None), word)
+    refused(lib, lib.load().alpha_pad_rows_typed(2, struct.pack("12q", X, 1, 8, Z, 1, 8, *job), dtype, None), word)
+    refused(lib, lib.load().alpha_pad_rows_typed(0, b"", 1, None), "no jobs")
