@@ -304,32 +304,37 @@ int launch_split(const Planes* const* list, int n, int sms, cudaStream_t stream)
     return launched("fc_split_kernel");
 }
 
-// Parts of the reduction on CTA pairs and the time of that product (us): a window of 64 steps of a tile 2.26, an item 2, a launch 5; the parts
-// written and read.  (Estimated / measured, with the split: 2048 x 2048 x 2048 92 / 88, 4096 x 1024 x 4096 170 / 174, 512 x 4096 x 1000 44 / 40.)
-struct PairPlan { int parts; double time; };
+// Columns of a pair's tile, parts of the reduction, and the time of that product (us): a window of 64 steps of a tile 2.26 (1.34 with 128 columns, whose tiles
+// fill the waves more evenly), a tile 2 (1.8), a launch 5; the parts written and read.  Measured / estimated, with the split of the operands, over 150 products
+// of 2 to 60 GFLOP: 0.97 with a deviation of 10 % (0.95, 7 %); what is chosen takes 1.003 of the best.
+struct PairPlan { int bn, parts; double time; };
 PairPlan pick_pair(int rows, int m_halves, int out_cols, bool glu, int K, int k_halves, int sms)
 {
-    const int pairs = sms / 2, out = glu ? 128 : 256, windows = k_halves * ((K + 63) / 64);
-    PairPlan best{1, 1e300};
+    const int pairs = sms / 2, windows = k_halves * ((K + 63) / 64);
+    PairPlan best{256, 1, 1e300};
     if (pairs < 1) return best;
-    const double tiles = static_cast<double>(m_halves) * ((rows + 255) / 256) * ((out_cols + out - 1) / out), size = static_cast<double>(rows) * m_halves * out_cols * (glu ? 2 : 1);
-    for (int parts = 1; parts <= 32 && parts <= windows; ++parts) {
-        const int each = (windows + parts - 1) / parts;
-        if ((parts - 1) * each >= windows) continue;                      // (no part is empty)
-        const double waves = static_cast<double>(static_cast<long long>((tiles * parts + pairs - 1) / pairs));
-        const double time = 5.0 + waves * (each * 2.26 + 2.0) + (parts > 1 ? 3.0 + size * 4e-6 * (2 * parts + 1) / 6.0 : 0.0);
-        if (time < best.time) best = PairPlan{parts, time};
+    for (int bn = 256; bn >= 128; bn /= 2) {
+        if (option_fc_tile() == (bn == 256 ? 11 : 1)) continue;
+        const int out = glu ? bn / 2 : bn;
+        const double tiles = static_cast<double>(m_halves) * ((rows + 255) / 256) * ((out_cols + out - 1) / out), size = static_cast<double>(rows) * m_halves * out_cols * (glu ? 2 : 1);
+        for (int parts = 1; parts <= 32 && parts <= windows; ++parts) {
+            const int each = (windows + parts - 1) / parts;
+            if ((parts - 1) * each >= windows) continue;                      // (no part is empty)
+            const double waves = static_cast<double>(static_cast<long long>((tiles * parts + pairs - 1) / pairs));
+            const double time = 5.0 + waves * (bn == 256 ? each * 2.26 + 2.0 : each * 1.34 + 1.8) + (parts > 1 ? 3.0 + size * 4e-6 * (2 * parts + 1) / 6.0 : 0.0);
+            if (time < best.time) best = PairPlan{bn, parts, time};
+        }
     }
     return best;
 }
 double split_time(size_t elements) { return 2.0 + elements * 10e-6 / 8.0; }
 
 template <int FORM>
-int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, int parts, void* part, int sms, int* status, cudaStream_t stream)
+int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, int sms, int* status, cudaStream_t stream)
 {
     constexpr bool GLU = FORM == kFcGlu, A_MN = FORM == kFcDeltaW, B_MN = FORM == kFcDeltaX || FORM == kFcDeltaW;
     const bool forward = FORM == kFcForward || FORM == kFcGlu;
-    const int out = GLU ? 128 : 256, m_halves = A_MN ? q.halves : 1, k_halves = FORM == kFcDeltaX ? q.halves : 1;
+    const int bn = plan.bn, parts = plan.parts, out = GLU ? bn / 2 : bn, m_halves = A_MN ? q.halves : 1, k_halves = FORM == kFcDeltaX ? q.halves : 1;
     const int cols = forward ? q.OC : q.cols, steps = FORM == kFcDeltaX ? q.OC : q.K;
     PairF32 p{};
     p.rows = A_MN ? q.OC : q.rows; p.cols = cols; p.pitch = q.e.cols; p.K = steps;
@@ -337,7 +342,7 @@ int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, int parts
     const int windows = (steps + 63) / 64;
     p.w_half = k_halves > 1 ? windows : 1 << 29; p.windows = windows * k_halves; p.parts = parts;
     p.a_mn = A_MN; p.b_mn = B_MN;
-    p.idesc = make_idesc_bf16(256, 256, A_MN, B_MN);
+    p.idesc = make_idesc_bf16(256, bn, A_MN, B_MN);
     p.A = q.A; p.B = q.B;
     p.a_row = A_MN ? 1 : q.lda; p.a_k = A_MN ? q.lda : 1; p.a_half = q.pitch;
     p.b_col = B_MN ? 1 : q.ldb; p.b_k = B_MN ? q.ldb : 1; p.b_half = static_cast<long long>(q.OC) * q.ldb;
@@ -370,17 +375,22 @@ int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, int parts
         if (!rc) rc = map(&b, B, q.cols, q.K, 1, pb, q.K * pb, 64, 1);
     } else {
         rc = map(&a, A, q.K, 1, q.rows, pa, pa, 1, 128);
-        if (!rc) rc = map(&b, B, q.K, OC, q.halves, pb, OC * pb, 128, 1);
+        if (!rc) rc = map(&b, B, q.K, OC, q.halves, pb, OC * pb, bn / 2, 1);
     }
     if (!rc) rc = A_MN ? out_map(&y, ws, q.halves, true, parts) : out_map(&y, ws, GLU && parts > 1 ? 2 : 1, false, parts);
     if (!rc) rc = p.keep_z ? out_map(&z, q.e.Z, GLU ? 2 : 1, false, 1) : (z = y, ALPHA_OK);
     if (rc) return rc;
     const long long items = static_cast<long long>(p.m_tiles) * p.n_tiles * parts;
     const unsigned pairs = static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
-    allow_smem<fc_pair_f32_kernel<GLU>>();
-    launch_after_clusters(fc_pair_f32_kernel<GLU>, dim3(2 * pairs), kPairF32Threads, 2, kPairF32Smem, stream, a, b, y, z, p);
+    auto go = [&](auto width) {
+        constexpr int BN = decltype(width)::value;
+        allow_smem<fc_pair_f32_kernel<GLU, BN>>();
+        launch_after_clusters(fc_pair_f32_kernel<GLU, BN>, dim3(2 * pairs), kPairF32Threads, 2, pair_f32_smem(BN), stream, a, b, y, z, p);
+    };
+    if (bn == 256) go(std::integral_constant<int, 256>{});
+    else go(std::integral_constant<int, 128>{});
     note_launch("fc");
-    note_plan("fc planes pair 256x256 parts=%d", parts);
+    note_plan("fc planes pair 256x%d parts=%d", bn, parts);
     rc = launched("fc_pair_f32_kernel");
     return rc || parts == 1 ? rc : launch_parts<GLU>(static_cast<const float*>(ws), size, parts, p.rows * m_halves, q.e, sms, stream);
 }
@@ -414,7 +424,9 @@ int launch_gathered(const ProductF32& q, const PlanePlan& plan, int sms, int* st
 
 template <int FORM> PlanePlan pick_gathered(const ProductF32& q, int sms, int most = 16)
 {
-    return plan_planes(q.rows, q.cols, q.K, 1, most, static_cast<double>(q.rows) * q.cols, 0, sms);
+    PlanePlan plan = plan_planes(q.rows, q.cols, q.K, 1, most, static_cast<double>(q.rows) * q.cols, 0, sms);
+    plan.time *= 1.2;         // (measured / estimated of 150 products 1.26 in the mean, 10 % about it: both operands are split as they are staged, and come from DRAM)
+    return plan;
 }
 // In any case: without parts where their scratch is refused.
 template <int FORM> int run_gathered(const ProductF32& q, int sms, int* status, cudaStream_t stream)
@@ -450,11 +462,11 @@ struct PairWork {
     }
 };
 
-// Option FC_TILE: 1 pairs, 2 never, else where their estimated time is less.
+// Option FC_TILE: 1 or 11 pairs, 2 never, else where their estimated time is less.
 bool pairs_pay(double pair, double other)
 {
     const int forced = option_fc_tile();
-    return forced == 1 || (forced != 2 && pair < other);
+    return forced == 1 || forced == 11 || (forced != 2 && pair < other);
 }
 
 template <int FORM>
@@ -469,7 +481,7 @@ int forward_f32(const ProductF32& q, cudaStream_t stream)
     w.want(q, pair.parts);
     if (w.sms >= 2 && w.fits() && pairs_pay(pair.time + split_time(w.elements()), pick_gathered<FORM>(q, w.sms).time)) {
         rc = w.split(stream);
-        if (rc == 0) return dry_run() ? ALPHA_OK : launch_pair<FORM>(q, w.p[a], w.p[b], pair.parts, w.part, w.sms, w.status, stream);
+        if (rc == 0) return dry_run() ? ALPHA_OK : launch_pair<FORM>(q, w.p[a], w.p[b], pair, w.part, w.sms, w.status, stream);
         if (rc < 0) return rc;
     }
     return run_gathered<FORM>(q, w.sms, w.status, stream);
@@ -495,7 +507,7 @@ int delta_f32(const float* dZ, const float* X, const float* W, float* dX, float*
     for (int form = 0; form < 4; ++form) {
         const bool bx = form & 1, bw = form & 2;
         if ((bx && !dX) || (bw && !dW) || (form && sms < 2)) continue;
-        if (option_fc_tile() == 1 && sms >= 2 && (bx != (dX != nullptr) || bw != (dW != nullptr))) continue;
+        if ((option_fc_tile() == 1 || option_fc_tile() == 11) && sms >= 2 && (bx != (dX != nullptr) || bw != (dW != nullptr))) continue;
         if (option_fc_tile() == 2 && form) continue;
         PairWork v;
         v.sms = sms; v.status = status;
@@ -512,8 +524,8 @@ int delta_f32(const float* dZ, const float* X, const float* W, float* dX, float*
         if (rc == 1) best_x = best_w = false;
     }
     rc = ALPHA_OK;
-    if (best_x && !dry_run()) rc = launch_pair<kFcDeltaX>(x, best.p[0], best.p[1], px.parts, best.part, sms, status, stream);
-    if (!rc && best_w && !dry_run()) rc = launch_pair<kFcDeltaW>(w, best.p[0], best.p[best_x ? 2 : 1], pw.parts, best.part, sms, status, stream);
+    if (best_x && !dry_run()) rc = launch_pair<kFcDeltaX>(x, best.p[0], best.p[1], px, best.part, sms, status, stream);
+    if (!rc && best_w && !dry_run()) rc = launch_pair<kFcDeltaW>(w, best.p[0], best.p[best_x ? 2 : 1], pw, best.part, sms, status, stream);
     if (!rc && dX && !best_x) rc = run_gathered<kFcDeltaX>(x, sms, status, stream);
     if (!rc && dW && !best_w) rc = run_gathered<kFcDeltaW>(w, sms, status, stream);
     return rc;

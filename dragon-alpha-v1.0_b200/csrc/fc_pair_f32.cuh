@@ -10,6 +10,8 @@
 // power limit).  us here / gathering: 8192 x 4096 x 4096 1110 / 2020 (247 TFLOP/s), 2048 x 2048 x 2048 88 / 136; from few tiles on the other is faster.
 // Operands: [plane][row][pitch]; a slot of the ring holds one plane of both for 64 steps, boxes of 64 steps x 128 rows, or of 64 rows x 64
 // steps where memory runs along the rows (128-byte rows either way: the copies take two clocks a row, and with boxes of 32 steps bound the kernel).
+// BN: 256 columns, or 128, whose tiles cost 0.6 of one and fill the waves of a launch more evenly (us, 256 / 128: gated 1000 x 1024 x 2 x 2752, 88 or 172 tiles
+// on 74 pairs, 82 / 76; 4381 x 1004 x 2 x 182 37.5 / 34; 2048 x 2048 x 2048 85 / 97).
 // The MMAs of a window go with the slots: hh; hm, mh, mm; hl, lh.  A work item is a tile and a part of the reduction; parts are added by another launch.
 // Words that are not the sum of their planes arrive as NaN.  A warp that finds a sum that is not finite, or below 2^-110 and not zero, forms its
 // 32 rows x 128 columns once more by FMAs from the fp32 tensors, in ascending k.
@@ -20,7 +22,9 @@
 namespace alpha {
 
 constexpr int kPairF32Threads = 320, kPairF32Slots = 6;
-constexpr uint32_t kPairF32Operand = 128 * 128, kPairF32Slot = 2 * kPairF32Operand, kPairF32Smem = kPairF32Slots * kPairF32Slot + 8 * 4096 + 1024 + 256;
+constexpr uint32_t kPairF32Operand = 128 * 128;                                    // 128 rows of A of a CTA, 64 steps of a plane
+__host__ __device__ constexpr uint32_t pair_f32_slot(int bn) { return kPairF32Operand + bn / 2 * 128; }
+__host__ __device__ constexpr uint32_t pair_f32_smem(int bn) { return kPairF32Slots * pair_f32_slot(bn) + 8 * 4096 + 1024 + 256; }
 
 // Up to three fp32 matrices as planes, dst[plane][row][pitch]; columns past cols are zeros.
 struct SplitJob { const float* src; uint2* dst; unsigned rows, cols4, first; FastDiv by_pitch4; };
@@ -82,12 +86,13 @@ static __device__ __noinline__ void form_row_f32(const PairF32& p, int row, int 
 }
 
 // tmY: the result, or where parts > 1 the sums, as (column, half, row, part)
-template <bool GLU>
+template <bool GLU, int BN>
 __global__ void __launch_bounds__(kPairF32Threads, 1)
     fc_pair_f32_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
                        const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ PairF32 p)
 {
-    constexpr int S = kPairF32Slots, OUT = GLU ? 128 : 256;
+    constexpr int S = kPairF32Slots, OUT = GLU ? BN / 2 : BN, HALF = BN / 2, QUARTER = BN / 4;
+    constexpr uint32_t kPairF32Slot = pair_f32_slot(BN);
     constexpr uint32_t kHh = 0, kSide = 256;          // columns of tensor memory
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         RingPos rp;
         for (int t = first; t < total && ok; t += step) {
             const Item it = item_at(t);
-            const int b0 = GLU ? it.n0 : it.n0 + my * 128;
+            const int b0 = GLU ? it.n0 : it.n0 + my * HALF;
             for (int s = 3 * it.w0; s < 3 * it.w1; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait_a(empty_0 + 8 * rp.idx, rp.phase ^ 1));
                 if (!ok) { report(p.status, kStatusProducerTimeout); settle(); break; }
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
                     }
                     if (p.b_mn) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) tma_load_4d_pair(b + j * 8192, &tmB, bar, b0 + 64 * j, k0, hk, plane);
+                        for (int j = 0; j < BN / 128; ++j) tma_load_4d_pair(b + j * 8192, &tmB, bar, b0 + 64 * j, k0, hk, plane);
                     } else {
                         tma_load_4d_pair(b, &tmB, bar, k0, b0, GLU ? my : 0, plane);
                     }
@@ -223,16 +228,16 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         __syncwarp();
     } else {
         const int quad = warp & 3, half = (warp - 2) >> 2;
-        // 64 sums from either column on (glu: gates, and the units' other halves)
-        const int col_a = (GLU ? 64 : 128) * half, col_b = GLU ? 128 + col_a : col_a + 64;
+        // QUARTER sums from either column on (glu: gates, and the units' other halves)
+        const int col_a = (GLU ? QUARTER : HALF) * half, col_b = GLU ? HALF + col_a : col_a + QUARTER;
         const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quad * 32) << 16), hh_free_L = mapa_u32(hh_free_a, 0), side_free_L = mapa_u32(side_free_a, 0);
         const uint32_t buf = smem_a + S * kPairF32Slot + (warp - 2) * 4096;
-        unsigned long long acc[64];
+        unsigned long long acc[QUARTER];
         auto add_columns = [&](uint32_t from) {
 #pragma unroll
-            for (int x = 0; x < 128; x += 16) {
+            for (int x = 0; x < HALF; x += 16) {
                 uint32_t v[16];
-                tmem_ld_32x16(lanes + from + (x < 64 ? col_a + x : col_b + x - 64), v);
+                tmem_ld_32x16(lanes + from + (x < QUARTER ? col_a + x : col_b + x - QUARTER), v);
                 tmem_ld_wait();
 #pragma unroll
                 for (int q = 0; q < 16; q += 2) acc[(x + q) / 2] = add2(acc[(x + q) / 2], pack2(__uint_as_float(v[q]), __uint_as_float(v[q + 1])));
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         for (int t = first; t < total && ok; t += step, ++item) {
             const Item it = item_at(t);
 #pragma unroll
-            for (int x = 0; x < 64; ++x) acc[x] = 0ull;
+            for (int x = 0; x < QUARTER; ++x) acc[x] = 0ull;
             for (int w = it.w0; w < it.w1; ++w, ++window) {
                 if (!wait(hh_full_a, window & 1)) break;
                 tc_fence_after_sync();
@@ -276,7 +281,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             if (row0 >= p.rows) { release(side_free_L); continue; }
             uint32_t most = 0, least = 0xffffffffu;
 #pragma unroll
-            for (int x = 0; x < 64; ++x) {
+            for (int x = 0; x < QUARTER; ++x) {
                 float a, b;
                 unpack2(acc[x], a, b);
                 const uint32_t u = __float_as_uint(a) << 1, v = __float_as_uint(b) << 1;
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             // The sums go back to the side columns, which are free now, and come chunk by chunk through one copy of the code below: unrolled over the
             // registers that hold them it took 25 us to fetch (of 111, 2048 x 2048 x 2048), and indexed they would live in local memory.
 #pragma unroll
-            for (int x = 0; x < 128; x += 16) {
+            for (int x = 0; x < HALF; x += 16) {
                 uint32_t v[16];
 #pragma unroll
                 for (int q = 0; q < 16; q += 2) {
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
                     unpack2(acc[(x + q) / 2], a, b);
                     v[q] = __float_as_uint(a); v[q + 1] = __float_as_uint(b);
                 }
-                tmem_st_32x16(lanes + kSide + (x < 64 ? col_a + x : col_b + x - 64), v);
+                tmem_st_32x16(lanes + kSide + (x < QUARTER ? col_a + x : col_b + x - QUARTER), v);
             }
             tmem_st_wait();
             // 32 sums from column c on, or, where some of the warp's do not stand, formed once more (rows past the last as the last)
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             };
             if constexpr (GLU) {
 #pragma unroll 1
-                for (int c = 0; c < 64; c += 32) {
+                for (int c = 0; c < QUARTER; c += 32) {
                     const int col0 = it.n0 + col_a + c;
                     if (col0 >= p.cols) break;
                     float z[32], u[32];
@@ -348,7 +353,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
                 }
             } else {
 #pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
+                for (int c = 0; c < HALF; c += 32) {
                     const int col0 = it.n0 + col_a + c;
                     if (col0 >= p.cols) break;
                     float z[32];

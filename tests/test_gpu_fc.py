@@ -654,3 +654,24 @@ def test_both_gradients_by_one_launch(eng, lib, dtype, glu, rows, IC, OC):
     for a, b in zip(both[:2], apart[:2]):
         # (a reduction split in another way differs in the last place)
         assert ((a.double() - b.double()).abs() <= torch.finfo(t).eps * b.double().abs() + 2e-3 * torch.finfo(t).eps / 2.0 ** -7 * b.double().abs().max()).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 64, 8), (77, 200, 136), (257, 132, 129), (700, 520, 1304), (2500, 128, 1544), (1500, 1544, 200)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("glu", (False, True), ids=("fc", "glu"))
+def test_f32_pairs_of_128_columns(eng, lib, glu, shape):
+    """The pair kernel's narrow tiles, parts of a reduction included: forward and gradients, finite or not."""
+    rows, IC, OC = shape
+    old = lib.set_option("FC_TILE", 11)
+    try:
+        forward_case(eng, lib, "f32", rows, IC, OC, "gelu", glu, bias=True, residual=not glu, save=True)
+        assert "256x128" in lib.last_plan(), lib.last_plan()
+        delta_case(eng, lib, "f32", rows, IC, OC, "silu", glu, True)
+        assert "256x128" in lib.last_plan(), lib.last_plan()
+    finally:
+        lib.set_option("FC_TILE", old)
+    test_f32_not_finite(eng, lib, 70, 11, "pairs of 128 columns", glu)
+
+
+@pytest.mark.parametrize("x_scale,w_scale", [(1e-25, 1e-10), (1e-37, 1e11), (1e25, 1e10), (1e-38, 1.0)])
+def test_f32_range_of_128_columns(eng, lib, x_scale, w_scale):
+    test_f32_range(eng, lib, 70, 11, "pairs of 128 columns", x_scale, w_scale)
