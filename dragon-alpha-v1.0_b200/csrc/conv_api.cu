@@ -76,7 +76,7 @@ enum Opt {
     OPT_HALO_PAD,       // channels that are no multiple of 32 on the halo kernels: 0 never, 1 by cost, 2 wherever possible
     OPT_F32_PLANES,     // fp32 products as three bf16 planes on the tensor cores: 0 never, 1 by cost, 2 always
     OPT_GATHER,         // 3xTF32 layers straight from their tensors as three bf16 planes: 0 never, 1 by cost, 2 wherever possible
-    OPT_FC_TILE,        // FullConnect products: 0 by cost, 1 CTA pairs (fp32: 11 their tiles of 128 columns), 2 by cost without the kernels of few rows (fp32: without pairs), 16-bit: 3 by cost, a launch for every product, 1000 split + columns
+    OPT_FC_TILE,        // FullConnect products: 0 by cost, 1 CTA pairs, 11 pairs with tiles of 128 columns, 2 by cost without the kernels of few rows (fp32: without pairs), 16-bit: 3 by cost, a launch for every product, 1000 split + columns
     OPT_COUNT
 };
 struct OptDef { const char* name; int dflt; };

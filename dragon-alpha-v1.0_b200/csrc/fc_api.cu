@@ -101,30 +101,33 @@ uint32_t tmem_columns(int bn, bool glu)
     return c;
 }
 
-// The plan of least estimated time, after some 500 measured ones (512 x 4096 x 4096 in us: 64 columns 26, 112 21, 128 21, pairs 27; 64 x 4096 x 1024: 64
-// columns 13, shared by two 11.6, 32 shared by four 9.7; 6656 x 73 x 7296: pairs 30, 128 columns 35, 64 45).  64 steps of a tile take 0.1375 us (four
-// MMAs of up to 128 columns, 64 clocks each whatever they hold, as A is read from shared memory), or what the ring's stages leave of a copy's 1.15 us;
-// a pair's 0.285; a tile's outputs 0.5 us and 0.008 a column, a pair's 2.1; all tiles' operands come through L2 at 18 TB/s, tensors from and
-// to DRAM at 5.2; a launch 4 us until its first tile and after its last (pairs 5.7), and a shared tile its exchange, eight CTAs also the wait for a
-// place for them.
+// The plan of least estimated time (512 x 4096 x 4096 in us: 64 columns 27.6, 128 22, pairs of 256 columns 27, of 128 19.7; 64 x 4096 x 1024: 64
+// columns 13, shared by two 11.6, 32 shared by four 9.7; 2048 x 2048 x 2048: pairs of 256 columns 17.8, of 128 18.7, 128 20).  64 steps of a tile
+// take 0.139 us (four MMAs of up to 128 columns, 64 clocks each whatever they hold, as A is read from shared memory), or what the ring's stages leave of a
+// copy's latency, or their bytes at the 112 KB/us that one SM takes in: 128 x 128 is bound by these, a pair of 256 x 128 brings three quarters of
+// them, one of 256 x 256 (0.32 us) half of them an output.  All tiles' operands come through L2 at 15 TB/s, tensors from and to DRAM at 5.9; a launch 4.4 us
+// until its first tile and after its last (pairs 5.8), and a shared tile its exchange, eight CTAs also the wait for a place for them.  Fitted to 1750 measured
+// plans of 220 products: 13 % about the measured time, and what is chosen takes 1.009 of the best.
 double plan_time(const Product& q, bool pair, int bn, int split, int sms, double* fixed, bool* fits)
 {
     const long long cols = q.glu ? 2LL * q.cols : q.cols, blocks = (long long)q.k_halves * ((q.K + kFcBK - 1) / kFcBK);
     const int out = q.glu ? bn / 2 : bn, bm = pair ? 256 : 128, ctas = pair ? 2 : 1;
     const long long tiles = (long long)q.m_halves * ((q.rows + bm - 1) / bm) * ((q.cols + out - 1) / out), most = sms / (ctas * split);
-    *fits = most >= 1 && (split == 1 || tiles <= most);
+    // (clusters of four or more do not fill every group of SMs: 32 of 37, and a second wave costs as much as the first)
+    *fits = most >= 1 && (split == 1 || tiles <= (split < 4 ? most : most * 87 / 100));
     if (!*fits) return 0.0;
     const long long waves = (tiles + most - 1) / most, each = (blocks + split - 1) / split;
-    const int a_rows = q.A.mn || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
-    const int ring = static_cast<int>(kFcRing / (fc_blocks(false) * fc_block_bytes(false, a_rows, bn)));
-    const double step = pair ? 0.285 : std::max(0.1375, 0.575 / (std::min(ring, (int)kFcMaxStages) - 1));
-    const double tile = std::max(each * step, pair ? 2.1 : 0.5 + 0.008 * bn);
-    const double l2 = (double)tiles * blocks * (pair ? 512 : a_rows + bn) * 128 / 18e6;
+    const int a_rows = pair || q.A.mn || q.rows >= 128 ? 128 : (q.rows + 7) / 8 * 8;
+    const uint32_t block = fc_block_bytes(pair, a_rows, bn);
+    const int ring = static_cast<int>(kFcRing / (fc_blocks(pair, bn) * block));
+    const double in = block / 112e3, step = pair ? (bn == 256 ? 0.32 : in) : std::max(std::max(0.139, in), 0.49 / (std::min(ring, (int)kFcMaxStages) - 1));
+    const double tile = std::max(each * step, (pair ? 0.28 : 0.68) + 0.0053 * bn);
+    const double l2 = (double)tiles * blocks * block * ctas / 15e6;
     const double mma = waves * tile, n = (double)q.rows * q.m_halves;
-    const double dram = 2e-6 * ((n + cols) * q.K * q.k_halves + n * (q.cols + (q.Z ? cols : 0) + (q.residual ? q.cols : 0))) / 5.2;
-    const double most_of = mma > l2 ? (mma > dram ? mma : dram) : (l2 > dram ? l2 : dram);
-    *fixed = (pair ? 5.7 : 4.0 + 0.006 * bn) + (split == 1 ? 0.0 : split == 2 ? 2.5 : split == 4 ? 4.0 : 12.0);
-    return 0.8 * most_of + 0.2 * (mma + l2 + dram);                // (the others are not quite hidden)
+    const double dram = 2e-6 * ((n + cols) * q.K * q.k_halves + n * (q.cols + (q.Z ? cols : 0) + (q.residual ? q.cols : 0))) / 5.9;
+    const double most_of = std::max(mma, std::max(l2, dram));
+    *fixed = (pair ? 5.8 : 4.4 + 0.0078 * bn) + (split == 1 ? 0.0 : split == 2 ? 3.0 : split == 4 ? 5.3 : 12.0);
+    return 0.86 * most_of + 0.14 * (mma + l2 + dram);                // (the others are not quite hidden)
 }
 // Two products by one launch: their tiles fill the same waves.
 double two_time(const Product& x, const Product& w, const FcPlan& plan, int sms)
@@ -158,7 +161,7 @@ FcPlan pick_plan(const Product& q, int sms, double* time_of = nullptr)
     // (an operand that runs along its rows comes in boxes of 64 of them; no part of a shared tile is empty)
     const int unit = q.B.mn ? 64 : 16;
     auto parts = [&](int split) { return split == 1 || (split - 1) * ((stages + split - 1) / split) < stages; };
-    if (forced == 1 && sms >= 2) { look(true, 256, 1); best = FcPlan{true, 256, 1}; }
+    if ((forced == 1 || forced == 11) && sms >= 2) { look(true, forced == 1 ? 256 : 128, 1); best = FcPlan{true, forced == 1 ? 256 : 128, 1}; }
     else if (forced >= 1000) {
         const int bn = forced % 1000 / unit * unit;
         for (int split = forced / 1000; split > 1 && bn >= unit && bn <= 256; split /= 2)
@@ -166,6 +169,7 @@ FcPlan pick_plan(const Product& q, int sms, double* time_of = nullptr)
         if (least == 1e300 && bn >= unit && bn <= 256) look(false, bn, 1);
     } else {
         look(true, 256, 1);
+        look(true, 128, 1);
         for (int bn = unit; bn <= 128; bn += unit)
             for (int split = 1; split <= 8; split *= 2)
                 if (parts(split)) look(false, bn, split);
@@ -179,7 +183,7 @@ struct Prepared { FcMma p; CUtensorMap a, b; };
 
 int prepare(const Product& q, const FcPlan& plan, int a_rows, int* status, Prepared* out)
 {
-    const int bm = plan.pair ? 256 : 128, bn = plan.bn, cols_of = q.glu ? bn / 2 : bn, steps = kFcBK * fc_blocks(plan.pair);
+    const int bm = plan.pair ? 256 : 128, bn = plan.bn, cols_of = q.glu ? bn / 2 : bn, steps = kFcBK * fc_blocks(plan.pair, bn);
     FcMma& p = out->p;
     p = FcMma{};
     p.rows = q.rows; p.cols = q.pitch;
@@ -191,7 +195,7 @@ int prepare(const Product& q, const FcPlan& plan, int a_rows, int* status, Prepa
     p.m_tiles = p.m_half * q.m_halves;
     p.bn = bn; p.split = plan.split;
     p.a_mn = q.A.mn; p.b_mn = q.B.mn; p.a_rows = a_rows;
-    const uint32_t stage = fc_blocks(plan.pair) * fc_block_bytes(plan.pair, a_rows, bn);
+    const uint32_t stage = fc_blocks(plan.pair, bn) * fc_block_bytes(plan.pair, a_rows, bn);
     p.stages = kFcRing / stage < kFcMaxStages ? kFcRing / stage : kFcMaxStages;
     // shared tiles: the ring holds a part's sums afterwards
     const uint32_t sums = (q.rows < 128 ? q.rows : 128) * (bn + 4) * 4;
@@ -203,16 +207,16 @@ int prepare(const Product& q, const FcPlan& plan, int a_rows, int* status, Prepa
     p.bias = q.bias; p.residual = q.residual; p.Y = q.Y; p.Z = q.Z; p.status = status;
     const int rc = q.A.mn ? make_map(&out->a, q.dtype, q.A, 64, 1, 64) : make_map(&out->a, q.dtype, q.A, 64, 1, a_rows);
     if (rc) return rc;
-    return q.B.mn ? make_map(&out->b, q.dtype, q.B, 64, 64, 1) : make_map(&out->b, q.dtype, q.B, 64, plan.pair ? 128 : cols_of, 1);
+    return q.B.mn ? make_map(&out->b, q.dtype, q.B, 64, 64, 1) : make_map(&out->b, q.dtype, q.B, 64, plan.pair ? bn / 2 : cols_of, 1);
 }
 
-template <class T, bool PAIR, bool GLU, bool TWO>
+template <class T, int PAIR, bool GLU, bool TWO>
 void launch_mma(const Prepared& x, const Prepared& y, int sms, cudaStream_t stream)
 {
     const FcMma& p = x.p;
     const int group = PAIR ? 2 : p.split, total = p.m_tiles * p.n_tiles + (TWO ? y.p.m_tiles * y.p.n_tiles : 0), most = sms / group;
     const unsigned grid = static_cast<unsigned>(p.split > 1 || total < most ? total : most) * group;
-    const uint32_t smem = p.stages * fc_blocks(PAIR) * fc_block_bytes(PAIR, p.a_rows, p.bn) + kFcStaging + 1024 + 512;
+    const uint32_t smem = p.stages * fc_blocks(PAIR != 0, p.bn) * fc_block_bytes(PAIR != 0, p.a_rows, p.bn) + kFcStaging + 1024 + 512;
     allow_smem<fc_mma_kernel<T, PAIR, GLU, TWO>>();
     launch_after_clusters(fc_mma_kernel<T, PAIR, GLU, TWO>, dim3(grid), kFcThreads, group > 1 ? group : 0, smem, stream, x.a, x.b, x.p, y.a, y.b, y.p);
 }
@@ -228,9 +232,15 @@ int launch_planned(const Product& q, const Product* other, const FcPlan& plan, i
     const Prepared& z = other ? y : x;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (other) plan.pair ? launch_mma<T, true, false, true>(x, z, sms, stream) : launch_mma<T, false, false, true>(x, z, sms, stream);
-        else if (q.glu) plan.pair ? launch_mma<T, true, true, false>(x, z, sms, stream) : launch_mma<T, false, true, false>(x, z, sms, stream);
-        else plan.pair ? launch_mma<T, true, false, false>(x, z, sms, stream) : launch_mma<T, false, false, false>(x, z, sms, stream);
+        auto by = [&](auto pair) {
+            constexpr int PAIR = decltype(pair)::value;
+            if (other) launch_mma<T, PAIR, false, true>(x, z, sms, stream);
+            else if (q.glu) launch_mma<T, PAIR, true, false>(x, z, sms, stream);
+            else launch_mma<T, PAIR, false, false>(x, z, sms, stream);
+        };
+        if (!plan.pair) by(std::integral_constant<int, 0>{});
+        else if (plan.bn == 256) by(std::integral_constant<int, 256>{});
+        else by(std::integral_constant<int, 128>{});
     };
     if (q.dtype == ALPHA_BF16) go(__nv_bfloat16{});
     else go(__half{});
@@ -260,9 +270,9 @@ int launch_products(const Product& x, const Product& w, cudaStream_t stream)
     apart += least;
     least = 1e300;
     const int forced = option_fc_tile();
-    for (int form = 0; form < 3 && x.rows >= 128; ++form) {
-        plan = form == 0 ? FcPlan{true, 256, 1} : FcPlan{false, form == 1 ? 128 : 64, 1};
-        if ((plan.pair && sms < 2) || (forced == 1 && !plan.pair) || forced == 3 || forced >= 1000) continue;
+    for (int form = 0; form < 4 && x.rows >= 128; ++form) {
+        plan = form < 2 ? FcPlan{true, form ? 128 : 256, 1} : FcPlan{false, form == 2 ? 128 : 64, 1};
+        if ((plan.pair && sms < 2) || (forced == 1 && form != 0) || (forced == 11 && form != 1) || forced == 3 || forced >= 1000) continue;
         const double time = two_time(x, w, plan, sms);
         if (time < least) { least = time; best = plan; }
     }

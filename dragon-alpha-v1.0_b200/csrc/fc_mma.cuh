@@ -13,6 +13,9 @@
 // flight share rows of A and B in L2; accumulators alternate between two halves of tensor memory, so that the epilogue of a tile runs
 // beside the MMAs of the next.  8192 x 22016 x 4096: 963 to 1060 us, 1.53 to 1.39 PFLOP/s (the card's power limit; cuBLAS's own rate there is 1.39).
 //
+// With 256 x 128 outputs, in stages of two blocks of 64 steps, tiles that would fill no wave of the wide ones: an SM takes in 112 KB a us, of which a pair of
+// 128 columns needs three quarters of what two CTAs of 128 x 128 do (512 x 4096 x 4096 us: 19.7, CTAs 22, pairs of 256 columns 27).
+//
 // Otherwise a CTA forms 128 x bn outputs, bn a multiple of 16 that the host picks so that the tiles fill the SMs evenly, in stages of two
 // blocks of 64 steps (a stage costs its issuing warp some 400 clocks whatever it holds: 64 columns, 16384 steps 55 -> 35 us).  Of few rows only
 // those are staged, which leaves the ring to B: it streams 160 KB of W ahead.  Where tiles are fewer than SMs a cluster of `split` CTAs
@@ -42,18 +45,18 @@ struct FcMma {
     int* status;
 };
 // Blocks of 64 steps of a stage, and its bytes.
-__host__ __device__ constexpr int fc_blocks(bool pair) { return pair ? 1 : 2; }
+__host__ __device__ constexpr int fc_blocks(bool pair, int bn) { return pair && bn == 256 ? 1 : 2; }
 __host__ __device__ constexpr uint32_t fc_block_bytes(bool pair, int a_rows, int bn) { return static_cast<uint32_t>(a_rows + (pair ? bn / 2 : bn)) * 128; }
 
-// TWO: the tiles of a second product of the same geometry follow those of the first (deltaX and deltaW, neither of which may fill the SMs).
-template <class T, bool PAIR, bool GLU, bool TWO>
+// PAIR: columns of a pair's tiles, 256 or 128, or 0.  TWO: the tiles of a second product of the same geometry follow those of the first (deltaX and deltaW, neither of which may fill the SMs).
+template <class T, int PAIR, bool GLU, bool TWO>
 __global__ void __launch_bounds__(kFcThreads, 1)
     fc_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ FcMma p, const __grid_constant__ CUtensorMap tmA2,
                   const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ FcMma p2)
 {
-    constexpr int CTAS = PAIR ? 2 : 1, KB = fc_blocks(PAIR);
-    const int BN = PAIR ? 256 : p.bn, OUT = GLU ? BN / 2 : BN, S = PAIR ? 6 : p.stages, split = PAIR ? 1 : p.split;
-    const uint32_t kA = PAIR ? 16384u : static_cast<uint32_t>(p.a_rows) * 128, kB = PAIR ? 16384u : static_cast<uint32_t>(BN) * 128, kBlock = kA + kB, kStage = KB * kBlock;
+    constexpr int CTAS = PAIR ? 2 : 1, KB = fc_blocks(PAIR != 0, PAIR);
+    const int BN = PAIR ? PAIR : p.bn, OUT = GLU ? BN / 2 : BN, S = PAIR ? static_cast<int>(kFcRing / (KB * fc_block_bytes(true, 128, PAIR))) : p.stages, split = PAIR ? 1 : p.split;
+    const uint32_t kA = PAIR ? 16384u : static_cast<uint32_t>(p.a_rows) * 128, kB = PAIR ? PAIR * 64u : static_cast<uint32_t>(BN) * 128, kBlock = kA + kB, kStage = KB * kBlock;
     const int acc_pitch = (BN + 31) & ~31;        // columns from one accumulator to the other
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                             if constexpr (PAIR) load(b, mB, bar, k0, n0, my);
                             else { load(b, mB, bar, k0, n0, 0); load(b + kB / 2, mB, bar, k0, n0, 1); }
                         } else {
-                            const int b0 = n0 + my * 128;
+                            const int b0 = n0 + my * (BN / 2);
                             if (b_mn) {
                                 for (int j = 0; j < static_cast<int>(kB >> 13); ++j) load(b + j * 8192, mB, bar, b0 + 64 * j, k0, hk);
                             } else {
@@ -278,10 +281,10 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                     for (uint32_t q = 0; q < KB; ++q)
 #pragma unroll
                         for (uint32_t kk = 0; kk < 4; ++kk)
-                            mma_16bit<PAIR>(d, a + q * (kBlock >> 4) + kk * a_k, dhi, b + q * (kBlock >> 4) + kk * b_k, dhi, idesc, kb > k_begin || q || kk ? 1u : 0u, elected);
+                            mma_16bit<PAIR != 0>(d, a + q * (kBlock >> 4) + kk * a_k, dhi, b + q * (kBlock >> 4) + kk * b_k, dhi, idesc, kb > k_begin || q || kk ? 1u : 0u, elected);
                     if (elected) commit(done);
                     if (++rp.idx == S) { rp.idx = 0; rp.phase ^= 1u; }
-                    next = mbar_test_a<PAIR>(full_0 + 8 * rp.idx, rp.phase);     // (beside the MMAs just issued)
+                    next = mbar_test_a<PAIR != 0>(full_0 + 8 * rp.idx, rp.phase);     // (beside the MMAs just issued)
                 }
                 if (ok && elected) commit(afull_0 + 8 * ap.idx);
                 ap.advance(2);

@@ -675,3 +675,18 @@ def test_f32_pairs_of_128_columns(eng, lib, glu, shape):
 @pytest.mark.parametrize("x_scale,w_scale", [(1e-25, 1e-10), (1e-37, 1e11), (1e25, 1e10), (1e-38, 1.0)])
 def test_f32_range_of_128_columns(eng, lib, x_scale, w_scale):
     test_f32_range(eng, lib, 70, 11, "pairs of 128 columns", x_scale, w_scale)
+
+
+@pytest.mark.parametrize("shape", [(1, 64, 8), (77, 200, 136), (257, 136, 129), (700, 520, 1304), (2500, 128, 1544), (1500, 1544, 200)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("glu", (False, True), ids=("fc", "glu"))
+def test_16bit_pairs_of_128_columns(eng, lib, dtype, glu, shape):
+    rows, IC, OC = shape
+    old = lib.set_option("FC_TILE", 11)
+    try:
+        forward_case(eng, lib, dtype, rows, IC, OC, "silu", glu, bias=True, residual=not glu, save=True)
+        assert "pair 256x128" in lib.last_plan(), lib.last_plan()
+        delta_case(eng, lib, dtype, rows, IC, OC, "gelu", glu, True)
+        assert "pair 256x128" in lib.last_plan(), lib.last_plan()
+    finally:
+        lib.set_option("FC_TILE", old)
