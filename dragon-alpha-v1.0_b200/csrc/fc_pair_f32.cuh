@@ -268,6 +268,9 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             const Item it = item_at(t);
 #pragma unroll
             for (int x = 0; x < QUARTER; ++x) acc[x] = 0ull;
+            // R to L2, while the windows run
+            if (!GLU && p.residual && p.parts == 1 && it.m0 + quad * 32 + lane < p.rows)
+                for (int c = it.n0 + col_a; c < it.n0 + col_a + HALF && c < p.cols; c += 32) prefetch_l2(p.residual + static_cast<size_t>(it.m0 + quad * 32 + lane) * p.pitch + c);
             for (int w = it.w0; w < it.w1; ++w, ++window) {
                 if (!wait(hh_full_a, window & 1)) break;
                 tc_fence_after_sync();
@@ -319,13 +322,17 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
 #pragma unroll
                 for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
             };
+            // (all loads before the first addition; with R in L2 by then 7664 x 420 x 7248 with R and Z took 512 us, now 477)
             auto add = [&](float (&f)[32], const float* from, int col0) {
+                float4 v[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4* at = reinterpret_cast<const float4*>(from + (col0 + 4 * q < p.pitch ? col0 + 4 * q : 0));
+                    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w) : "l"(at) : "memory");
+                }
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    if (col0 + 4 * q < p.pitch) {
-                        const float4 v = *reinterpret_cast<const float4*>(from + col0 + 4 * q);
-                        f[4 * q] += v.x; f[4 * q + 1] += v.y; f[4 * q + 2] += v.z; f[4 * q + 3] += v.w;
-                    }
+                    if (col0 + 4 * q < p.pitch) { f[4 * q] += v[q].x; f[4 * q + 1] += v[q].y; f[4 * q + 2] += v[q].z; f[4 * q + 3] += v[q].w; }
             };
             if constexpr (GLU) {
 #pragma unroll 1
