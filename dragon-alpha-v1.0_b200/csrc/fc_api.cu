@@ -557,9 +557,9 @@ int launch_small(const AlphaFcShape* s, const void* X, const void* W, const void
     while (p.ks < 8 && static_cast<long long>(units) * p.ks < 16LL * sms && words >= 128 * p.ks) p.ks *= 2;
     const int teams = 8 / p.ks;
     const unsigned blocks = (units + teams - 1) / teams;
-    if (s->rows == 1) launch_after(fc_small_kernel<float, 1, GLU>, blocks, 256, 0, stream, p);
-    else if (s->rows == 2) launch_after(fc_small_kernel<float, 2, GLU>, blocks, 256, 0, stream, p);
-    else launch_after(fc_small_kernel<float, 4, GLU>, blocks, 256, 0, stream, p);
+    if (s->rows == 1) launch_after(fc_small_kernel<1, GLU>, blocks, 256, 0, stream, p);
+    else if (s->rows == 2) launch_after(fc_small_kernel<2, GLU>, blocks, 256, 0, stream, p);
+    else launch_after(fc_small_kernel<4, GLU>, blocks, 256, 0, stream, p);
     note_launch("fc_small");
     note_plan("fc small ks=%d", p.ks);
     return launched("fc_small_kernel");

@@ -45,7 +45,8 @@ __global__ void __launch_bounds__(256, kDeltaCtas) fc_delta_kernel(const __grid_
             constexpr int kRows = GLU ? 2 : 4;
             const long long stride = gridDim.y * 8;
             for (long long r0 = blockIdx.y * 8 + warp; r0 < p.rows; r0 += kRows * stride) {
-                uint4 wd[kRows], wg[kRows], wu[GLU ? kRows : 1];
+                uint4 wd[kRows], wg[kRows];
+                [[maybe_unused]] uint4 wu[GLU ? kRows : 1];
 #pragma unroll
                 for (int q = 0; q < kRows; ++q) {
                     const long long r = r0 + q * stride < p.rows ? r0 + q * stride : r0;

@@ -30,7 +30,6 @@ namespace alpha {
 
 constexpr int kFcThreads = 320, kFcBK = 64, kFcGroupM = 8, kFcMaxStages = 16;
 constexpr uint32_t kFcRing = 196608, kFcStaging = 8 * 4096;              // staging: two buffers of 32 x 32 elements for each epilogue warp
-constexpr uint32_t kFcSmemMost = kFcRing + kFcStaging + 1024 + 512;
 
 struct FcMma {
     int rows, cols;               // outputs: rows of a half, pitch (glu: of a half of Z too)

@@ -1,4 +1,4 @@
-// A FullConnect layer over few rows (tokens of a serving program): Y = act(X W^T + b) + R, or the gated block.
+// A FullConnect layer over few rows (tokens of a serving program): Y = act(X W^T + b) + R, or the gated block; first fp32, 16-bit tensors below.
 //
 // Bound: one read of W.  A warp owns two rows of W (glu: the gate and the up row of a unit), or a KS-th of their words, and
 // streams them past L1 in 16-byte words, UNROLL of each row in flight per lane; X (R rows) is read again by every warp and stays in L1.
@@ -18,14 +18,6 @@ struct FcSmall {
     void *Z, *Y;
 };
 
-// Two floats of a word of 16 (or 32) bits elements, as an f32x2 operand.
-template <class T> __device__ __forceinline__ void word_pairs(const uint4& w, unsigned long long (&v)[Word16<T>::N / 2])
-{
-    float f[Word16<T>::N];
-    Word16<T>::load(w, f);
-#pragma unroll
-    for (int i = 0; i < Word16<T>::N / 2; ++i) v[i] = pack2(f[2 * i], f[2 * i + 1]);
-}
 __device__ __forceinline__ uint4 load_streamed(const uint4* p)
 {
     uint4 v;
@@ -39,18 +31,16 @@ __device__ __forceinline__ void load_streamed_32(const uint4* p, uint4 (&v)[2])
                  : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w) : "l"(p));
 }
 template <class T> __device__ __forceinline__ float to_float(T x);
-template <> __device__ __forceinline__ float to_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 template <class T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
-template <class T, int R, bool GLU>
+template <int R, bool GLU>
 __global__ void __launch_bounds__(256) fc_small_kernel(const __grid_constant__ FcSmall p)
 {
-    constexpr int N = Word16<T>::N, UNROLL = R == 1 ? 4 : 2;
+    constexpr int N = 4, UNROLL = R == 1 ? 4 : 2;
     __shared__ float part[8][2 * R];
     grid_dependency_wait();
     grid_dependency_trigger();
@@ -71,16 +61,15 @@ __global__ void __launch_bounds__(256) fc_small_kernel(const __grid_constant__ F
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[0][r] = acc[1][r] = 0ull;
         auto madd = [&](const uint4& a, const uint4& b, int at) {
-            unsigned long long v0[N / 2], v1[N / 2];
-            word_pairs<T>(a, v0);
-            word_pairs<T>(b, v1);
+            auto two = [](uint32_t lo, uint32_t hi) { return pack2(__uint_as_float(lo), __uint_as_float(hi)); };
+            const unsigned long long a0 = two(a.x, a.y), a1 = two(a.z, a.w), b0 = two(b.x, b.y), b1 = two(b.z, b.w);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 if (R > 1 && r >= p.rows) break;
-                unsigned long long xv[N / 2];
-                word_pairs<T>(__ldg(x + static_cast<size_t>(r) * words + at), xv);
-#pragma unroll
-                for (int i = 0; i < N / 2; ++i) { ffma2(acc[0][r], v0[i], xv[i]); ffma2(acc[1][r], v1[i], xv[i]); }
+                const uint4 v = __ldg(x + static_cast<size_t>(r) * words + at);
+                const unsigned long long x0 = two(v.x, v.y), x1 = two(v.z, v.w);
+                ffma2(acc[0][r], a0, x0); ffma2(acc[1][r], b0, x0);
+                ffma2(acc[0][r], a1, x1); ffma2(acc[1][r], b1, x1);
             }
         };
         int at = begin + lane;
@@ -120,19 +109,19 @@ __global__ void __launch_bounds__(256) fc_small_kernel(const __grid_constant__ F
         z += part[team * p.ks + s][q];
         if (GLU) up += part[team * p.ks + s][R + r];
     }
-    const T* bias = static_cast<const T*>(p.bias);
-    T *Z = static_cast<T*>(p.Z), *Y = static_cast<T*>(p.Y);
+    const float* bias = static_cast<const float*>(p.bias);
+    float *Z = static_cast<float*>(p.Z), *Y = static_cast<float*>(p.Y);
     const size_t at = static_cast<size_t>(r) * p.pitch + col;
-    if (bias) z += to_float(bias[col]);
-    if (GLU && bias) up += to_float(bias[p.pitch + col]);
+    if (bias) z += bias[col];
+    if (GLU && bias) up += bias[p.pitch + col];
     if (Z) {
-        Z[GLU ? at + static_cast<size_t>(r) * p.pitch : at] = from_float<T>(z);
-        if (GLU) Z[at + static_cast<size_t>(r + 1) * p.pitch] = from_float<T>(up);
+        Z[GLU ? at + static_cast<size_t>(r) * p.pitch : at] = z;
+        if (GLU) Z[at + static_cast<size_t>(r + 1) * p.pitch] = up;
     }
-    with_act(p.act, [&](auto a) { z = act_value<decltype(a)::value, Word16<T>::kFast>(z, p.k); });
+    with_act(p.act, [&](auto a) { z = act_value<decltype(a)::value, false>(z, p.k); });
     if (GLU) z *= up;
-    else if (p.residual) z += to_float(static_cast<const T*>(p.residual)[at]);
-    Y[at] = from_float<T>(z);
+    else if (p.residual) z += static_cast<const float*>(p.residual)[at];
+    Y[at] = z;
 }
 
 // ---- 16-bit tensors ----------------------------------------------------------------------------------------------
