@@ -624,10 +624,10 @@ int launch_delta(const AlphaFcShape* s, const void* dY, const void* Z, void* dZ,
     if (rc) return rc;
     const int pitch = fc_pitch(s->OC), wide = GLU ? 2 * pitch : pitch, words = pitch / Word16<T>::N;
     const unsigned gy = (words + 31) / 32;
-    // one wave of CTAs, eight rows of a warp at least
-    long long gx = sms * (long long)kDeltaCtas / gy;
+    // one wave of CTAs, four rows of a warp at least
+    long long gx = sms * static_cast<long long>(delta_ctas<GLU>()) / gy;
     if (gx < 1) gx = 1;
-    const long long by_rows = (s->rows + 63) / 64;
+    const long long by_rows = (s->rows + 31) / 32;
     if (gx > by_rows) gx = by_rows;
     FcDelta p{s->rows, pitch, s->OC, s->act, s->k, dY, Z, dZ, nullptr};
     if (dB) {

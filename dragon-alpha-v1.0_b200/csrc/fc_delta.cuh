@@ -21,9 +21,12 @@ struct FcDelta {
     float* part;                    // [gridDim.y][cols, glu: 2 cols] or nullptr
 };
 
-constexpr int kDeltaCtas = 3;           // of an SM
+// CTAs of an SM, each warp with one row in flight: rows ahead in registers, or the loop unrolled, cost more than they hid, as the grid then no longer
+// sweeps one band of rows.  us with deltaB, before with two or four rows ahead on three CTAs / now: 8192 x 11008 glu silu 182 / 151, 4096 x 16384 silu 109 / 84
+// and leakyRelu 87 / 66 (5.1 and 6.1 TB/s: an exponential and a quotient an element), fp32 4096 x 16384 165 / 125.
+template <bool GLU> __host__ __device__ constexpr int delta_ctas() { return GLU ? 3 : 6; }
 template <class T, bool GLU>
-__global__ void __launch_bounds__(256, kDeltaCtas) fc_delta_kernel(const __grid_constant__ FcDelta p)
+__global__ void __launch_bounds__(256, delta_ctas<GLU>()) fc_delta_kernel(const __grid_constant__ FcDelta p)
 {
     using V = Word16<T>;
     constexpr int N = V::N, HALVES = GLU ? 2 : 1;
@@ -41,58 +44,45 @@ __global__ void __launch_bounds__(256, kDeltaCtas) fc_delta_kernel(const __grid_
     if (word < words) {
         with_act(p.act, [&](auto a) {
             constexpr int ACT = decltype(a)::value;
-            // kRows rows in flight: their loads leave before the first is used
-            constexpr int kRows = GLU ? 2 : 4;
-            const long long stride = gridDim.y * 8;
-            for (long long r0 = blockIdx.y * 8 + warp; r0 < p.rows; r0 += kRows * stride) {
-                uint4 wd[kRows], wg[kRows];
-                [[maybe_unused]] uint4 wu[GLU ? kRows : 1];
+#pragma unroll 1
+            for (long long r = blockIdx.y * 8 + warp; r < p.rows; r += gridDim.y * 8) {
+                const size_t at = static_cast<size_t>(r) * words + word, zt = GLU ? at + static_cast<size_t>(r) * words : at;
+                const uint4 wd = __ldg(dY + at);
+                uint4 wz[HALVES];
+                if constexpr (GLU || ACT != ALPHA_ACT_NONE) wz[0] = Z[zt];
+                if constexpr (GLU) wz[HALVES - 1] = Z[zt + words];
+                float d[N];
+                V::load(wd, d);
+                if constexpr (GLU) {
+                    float g[N], u[N];
+                    V::load(wz[0], g);
+                    V::load(wz[HALVES - 1], u);
 #pragma unroll
-                for (int q = 0; q < kRows; ++q) {
-                    const long long r = r0 + q * stride < p.rows ? r0 + q * stride : r0;
-                    const size_t at = static_cast<size_t>(r) * words + word, zt = GLU ? at + static_cast<size_t>(r) * words : at;
-                    wd[q] = __ldg(dY + at);
-                    if constexpr (GLU || ACT != ALPHA_ACT_NONE) wg[q] = Z[zt];
-                    if constexpr (GLU) wu[q] = Z[zt + words];
-                }
-#pragma unroll
-                for (int q = 0; q < kRows; ++q) {
-                    const long long r = r0 + q * stride;
-                    if (r >= p.rows) break;
-                    const size_t at = static_cast<size_t>(r) * words + word, zt = GLU ? at + static_cast<size_t>(r) * words : at;
-                    float d[N];
-                    V::load(wd[q], d);
-                    if constexpr (GLU) {
-                        float g[N], u[N];
-                        V::load(wg[q], g);
-                        V::load(wu[q], u);
+                    for (int i = 0; i < N; ++i) {
+                        float value, slope;
+                        act_both<ACT, V::kFast>(g[i], p.k, value, slope);
+                        g[i] = d[i] * u[i] * slope;
+                        u[i] = d[i] * value;
+                        if (i >= whole) g[i] = u[i] = 0.f;
+                        acc[0][i] += g[i];
+                        acc[1][i] += u[i];
+                    }
+                    dZ[zt] = V::store(g);
+                    dZ[zt + words] = V::store(u);
+                } else {
+                    if constexpr (ACT != ALPHA_ACT_NONE) {
+                        float z[N];
+                        V::load(wz[0], z);
 #pragma unroll
                         for (int i = 0; i < N; ++i) {
                             float value, slope;
-                            act_both<ACT, V::kFast>(g[i], p.k, value, slope);
-                            g[i] = d[i] * u[i] * slope;
-                            u[i] = d[i] * value;
-                            if (i >= whole) g[i] = u[i] = 0.f;
-                            acc[0][i] += g[i];
-                            acc[1][i] += u[i];
+                            act_both<ACT, V::kFast>(z[i], p.k, value, slope);
+                            d[i] = i >= whole ? 0.f : d[i] * slope;
                         }
-                        dZ[zt] = V::store(g);
-                        dZ[zt + words] = V::store(u);
-                    } else {
-                        if constexpr (ACT != ALPHA_ACT_NONE) {
-                            float z[N];
-                            V::load(wg[q], z);
-#pragma unroll
-                            for (int i = 0; i < N; ++i) {
-                                float value, slope;
-                                act_both<ACT, V::kFast>(z[i], p.k, value, slope);
-                                d[i] = i >= whole ? 0.f : d[i] * slope;
-                            }
-                            dZ[zt] = V::store(d);
-                        }
-#pragma unroll
-                        for (int i = 0; i < N; ++i) acc[0][i] += d[i];
+                        dZ[zt] = V::store(d);
                     }
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[0][i] += d[i];
                 }
             }
         });
