@@ -109,7 +109,8 @@ int alpha_conv_debug_counters(unsigned long long* out, int n);
  *     stream is being captured into a CUDA graph a call that would have to grow the block fails with
  *     ALPHA_E_CAPTURE instead: run the step once eagerly, or alpha_conv_reserve_workspace, before
  *     capturing.  A block that a capture saw stays allocated until alpha_conv_release_workspace,
- *     because replays of that graph keep addressing it.  Layers that an older kernel runs with less scratch or
+ *     because replays of that graph keep addressing it: replays of graphs captured on one stream, and
+ *     eager calls on it, have to follow one another, as calls on a stream do.  Layers that an older kernel runs with less scratch or
  *     none (odd channel counts, strided layers) take that kernel instead, in a capture as in a small block: the same
  *     contraction to rounding, not the same bits.
  *   - A host that owns all device memory hands in its own block with alpha_conv_set_workspace
