@@ -151,7 +151,7 @@ def load():
     lib.alpha_fullConnect_glu_delta.argtypes = [F, V, V, V, V, V, V, V, V, V]
     lib.alpha_fullConnect_workspace_bytes.argtypes = [F, I, I, C.POINTER(C.c_size_t)]
     lib.alpha_grad_norm.argtypes = [I, G, V, V]
-    lib.alpha_clip_grad_norm.argtypes = [I, G, C.c_float, V, V]
+    lib.alpha_clip_grad_norm.argtypes = [I, G, C.c_double, V, V]
     # pooling
     PS = C.POINTER(AlphaPoolShape)
     lib.alpha_pool2D_max.argtypes = [PS, V, V, V]

@@ -501,8 +501,8 @@ int alpha_fullConnect_workspace_bytes(const AlphaFcShape* s, int glu, int op, si
  *
  * norm = sqrt(sum of the squares of all elements of n tensors), summed in fp64 in a fixed order (neither overflow nor underflow
  * of a square; the same bits on every run), written to *norm as a float on the device; NaN or Inf elements give a NaN or Inf.
- * alpha_clip_grad_norm also scales every element by c = min(1, max_norm / (norm + 1e-6)) (a NaN norm: by NaN), c as a float:
- * out = c * grad, where out may be grad itself.  A tensor given in place (out == grad) is not touched where c = 1.
+ * alpha_clip_grad_norm also scales every element by c = min(1, max_norm / (norm + 1e-6)) (a NaN norm: by NaN):
+ * out = c * grad, rounded to fp32 and from there to out's type; out may be grad itself.  A tensor given in place (out == grad) is not touched where c = 1.
  * The tensors may be of different types and any size from 0 on, aligned to their elements; out may have another type (a
  * 16-bit gradient for a fp32 optimizer).  An output must not overlap any other tensor of the call (ALPHA_E_ARG).
  * n = 0 is a norm of 0.  Scratch: 48 bytes for each SM (or of the SM budget) and 128 tensors. */
@@ -513,7 +513,7 @@ typedef struct AlphaGrad {
     int dtype, out_dtype; /* ALPHA_F32, ALPHA_BF16 or ALPHA_F16 */
 } AlphaGrad;
 int alpha_grad_norm(int n, const AlphaGrad* grads, float* norm, alpha_stream_t stream);
-int alpha_clip_grad_norm(int n, const AlphaGrad* grads, float max_norm, float* norm, alpha_stream_t stream);
+int alpha_clip_grad_norm(int n, const AlphaGrad* grads, double max_norm, float* norm, alpha_stream_t stream);
 
 /* ---- 2D pooling (the operators between the convolutions of a network) ---------------------------------------
  * Replace the kernels behind src/cu32_src/Cuda_pool2D/Cuda_pool2D/pool2D.cuh and

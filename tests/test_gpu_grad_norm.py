@@ -163,3 +163,18 @@ def test_more_than_2_31_elements(eng):
     for at in (0, 2 ** 31 - 1, 2 ** 31, big.numel() - 2):
         assert abs(float(big[at]) - half) <= 2.0 ** -8 * half
     assert abs(float(big[-1]) - 1.5) <= 2.0 ** -7
+
+
+@pytest.mark.parametrize("max_norm", (1.0, 0.37, 1e-3, 1e-25, 123.456))
+@pytest.mark.parametrize("n", (3, 10001))
+def test_a_product_is_rounded_once(eng, n, max_norm):
+    """Gradients whose squares sum without rounding: the factor is that of fp64, and an fp32 output errs by its own rounding only (2^-24, and 2^-47 of the
+    factor's two floats; of the smallest by the denormals' spacing)."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    g = torch.randint(-200, 201, (n,), device="cuda", generator=gen).float() / 64
+    for t in (torch.float32, torch.bfloat16):
+        grad, out = g.to(t), torch.empty_like(g)
+        c = min(1.0, max_norm / (math.sqrt(float((grad.double() ** 2).sum())) + 1e-6))
+        eng.clip_grad_norm([grad], max_norm, Out=[out])
+        want = grad.double() * c
+        assert ((out.double() - want).abs() <= 2.0 ** -24 * (1 + 2.0 ** -20) * want.abs() + 2.0 ** -149).all()
