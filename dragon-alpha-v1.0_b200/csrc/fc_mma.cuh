@@ -11,7 +11,7 @@
 // PAIR: two CTAs of a cluster form 256 x 256 outputs (tcgen05 cta_group::2): each holds its 128 rows of A and half of the rows of B, so that
 // shared memory is read and filled with half of B.  Persistent: a pair walks over tiles, in groups of kFcGroupM row tiles so that the tiles in
 // flight share rows of A and B in L2; accumulators alternate between two halves of tensor memory, so that the epilogue of a tile runs
-// beside the MMAs of the next.  8192 x 22016 x 4096: 963 to 1060 us, 1.53 to 1.39 PFLOP/s (the card's power limit; cuBLAS's own rate there is 1.39).
+// beside the MMAs of the next.  8192 x 22016 x 4096, Z kept: 935 us in short runs, 1090 in long ones, 1.58 and 1.36 PFLOP/s (the power limit: cuBLAS falls from 1.68 to 1.39).
 //
 // With 256 x 128 outputs, in stages of two blocks of 64 steps, tiles that would fill no wave of the wide ones: an SM takes in 112 KB a us, of which a pair of
 // 128 columns needs three quarters of what two CTAs of 128 x 128 do (512 x 4096 x 4096 us: 19.7, CTAs 22, pairs of 256 columns 27).

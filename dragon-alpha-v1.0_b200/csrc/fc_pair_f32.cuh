@@ -7,7 +7,7 @@
 // six cta_group::2 MMAs of 128 clocks for 16 steps, each CTA's tensor memory holding hh in 256 columns and the rest in the other 256.
 // hh needs no second buffer: its four MMAs of a window of 64 steps come first, and while the twenty others run (2560 clocks) the epilogue
 // warps fetch it.  Bound: the MMAs, a sixth of the bf16 rate (280 TFLOP/s of fp32 products at the measured 1.68 PFLOP/s, 232 under the
-// power limit).  us here / gathering: 8192 x 4096 x 4096 1110 / 2020 (247 TFLOP/s), 2048 x 2048 x 2048 88 / 136; from few tiles on the other is faster.
+// power limit).  us here / gathering: 8192 x 4096 x 4096 1110 / 2020 (247 TFLOP/s), 2048 x 2048 x 2048 85 / 135; of few tiles the other is faster.
 // Operands: [plane][row][pitch]; a slot of the ring holds one plane of both for 64 steps, boxes of 64 steps x 128 rows, or of 64 rows x 64
 // steps where memory runs along the rows (128-byte rows either way: the copies take two clocks a row, and with boxes of 32 steps bound the kernel).
 // BN: 256 columns, or 128, whose tiles cost 0.6 of one and fill the waves of a launch more evenly (us, 256 / 128: gated 1000 x 1024 x 2 x 2752, 88 or 172 tiles
