@@ -47,6 +47,9 @@ struct FcMma {
 __host__ __device__ constexpr int fc_blocks(bool pair, int bn) { return pair && bn == 256 ? 1 : 2; }
 __host__ __device__ constexpr uint32_t fc_block_bytes(bool pair, int a_rows, int bn) { return static_cast<uint32_t>(a_rows + (pair ? bn / 2 : bn)) * 128; }
 
+// Elements from a row of a tensor to the one `rows` further (a pitch alone may be 2^31 - 1024).
+__host__ __device__ constexpr size_t fc_rows_on(int rows, size_t pitch) { return rows * pitch; }
+
 // PAIR: columns of a pair's tiles, 256 or 128, or 0.  TWO: the tiles of a second product of the same geometry follow those of the first (deltaX and deltaW, neither of which may fill the SMs).
 template <class T, int PAIR, bool GLU, bool TWO>
 __global__ void __launch_bounds__(kFcThreads, 1)
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         __syncwarp();
         T* to = tensor + static_cast<size_t>(row0 + (lane >> 2)) * pitch + col0 + 8 * (lane & 3);
 #pragma unroll
-        for (int j = 0; j < 4; ++j, to += 8 * pitch) {
+        for (int j = 0; j < 4; ++j, to += fc_rows_on(8, pitch)) {
             const float4 w = ld_shared_v4(lane_word(j));
             if (inside(row0, col0, width, j)) *reinterpret_cast<float4*>(to) = w;
         }
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     auto fetch = [&](uint4 (&r)[4], int row0, int col0, int width) {
         const T* from = static_cast<const T*>(cur->residual) + static_cast<size_t>(row0 + (lane >> 2)) * cur->cols + col0 + 8 * (lane & 3);
 #pragma unroll
-        for (int j = 0; j < 4; ++j, from += 8 * cur->cols) r[j] = inside(row0, col0, width, j) ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 4; ++j, from += fc_rows_on(8, cur->cols)) r[j] = inside(row0, col0, width, j) ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
     };
     auto add_fetched = [&](float (&f)[32], const uint4 (&r)[4]) {
 #pragma unroll
