@@ -774,7 +774,7 @@ static bool pad_beats_patch(int K, int taps, int ncols, int mode3x, double idle,
 static int patch_ksplit(const AlphaConvShape* s, int mode3x, int sms);
 // A route that needs scratch may not take away what a route without any could do: under stream capture, in a caller-owned
 // workspace or on a full card the call then goes on to the older route, with the scratch it had at its start (ws_rewind).
-static inline bool scratch_refused(int rc)
+bool scratch_refused(int rc)
 {
     const bool no_memory = t_no_memory;
     t_no_memory = false;

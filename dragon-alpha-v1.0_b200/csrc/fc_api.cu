@@ -442,7 +442,7 @@ template <int FORM> PlanePlan pick_gathered(const ProductF32& q, int sms, int mo
 template <int FORM> int run_gathered(const ProductF32& q, int sms, int* status, cudaStream_t stream)
 {
     const int rc = launch_gathered<FORM>(q, pick_gathered<FORM>(q, sms), sms, status, stream);
-    return rc == ALPHA_E_NOSCRATCH || rc == ALPHA_E_CAPTURE ? launch_gathered<FORM>(q, pick_gathered<FORM>(q, sms, 1), sms, status, stream) : rc;
+    return rc && scratch_refused(rc) ? launch_gathered<FORM>(q, pick_gathered<FORM>(q, sms, 1), sms, status, stream) : rc;
 }
 
 // One or two products by pairs over operands that are split together; 1 where their scratch is refused (nothing has been launched then).
@@ -462,7 +462,7 @@ struct PairWork {
         for (int i = 0; i < n; ++i) bytes += plane_bytes(p[i]);
         void* ws = nullptr;
         const int rc = call_scratch(stream, bytes, &ws);
-        if (rc) return rc == ALPHA_E_NOSCRATCH || rc == ALPHA_E_CAPTURE ? 1 : rc;
+        if (rc) return scratch_refused(rc) ? 1 : rc;
         if (dry_run()) return ALPHA_OK;
         char* at = static_cast<char*>(ws);
         for (int i = 0; i < n; ++i) { p[i].ptr = at; at += plane_bytes(p[i]); }

@@ -37,6 +37,8 @@ int option_fc_tile();
 // nothing is allocated and callers launch nothing.
 int call_begin(cudaStream_t stream);
 int call_scratch(cudaStream_t stream, size_t bytes, void** out);
+// Whether `rc` is a refusal of scratch (a capture, a block given by the caller, a full card) that a route with less, or none, may answer.
+bool scratch_refused(int rc);
 bool dry_run();
 void dry_begin();
 size_t dry_end();

@@ -34,3 +34,47 @@ def test_residual_of_2_28_columns(eng, lib):
     for r in range(rows):
         assert (Y[r].float() == want[r]).all(), r
     assert lib.device_status() == 0
+
+
+def test_f32_runs_without_scratch_where_the_card_is_full(eng, lib):
+    """Operands split once need 157 MB of scratch; where cudaMalloc refuses it the products are gathered, as they are in a capture."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    rows, IC, OC = 8192, 2048, 2048
+    X, dY = torch.randn(rows, IC, device="cuda", generator=gen), torch.randn(rows, OC, device="cuda", generator=gen)
+    W = torch.randn(OC, IC, device="cuda", generator=gen) * IC ** -0.5
+    Y, Z, dZ, dX, dW, dB = (torch.empty_like(t) for t in (dY, dY, dY, X, W, W[0]))
+    plans = []
+
+    def step():
+        eng.base.fullConnect(Y, X, W, rows, IC, OC, 0, lib.ACTS["silu"], 0.0, None, None, Z)
+        plans.append(lib.last_plan())
+        eng.base.fullConnect_delta(dX, dW, dB, dY, X, W, Z, dZ, rows, IC, OC, 0, lib.ACTS["silu"], 0.0)
+        plans.append(lib.last_plan())
+
+    step()                                          # (kernels take memory when they are first used: both routes once)
+    old = lib.set_option("FC_TILE", 2)
+    try:
+        step()
+    finally:
+        lib.set_option("FC_TILE", old)
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (Y, Z, dX, dW, dB)]
+    for t in (Y, Z, dX, dW, dB):
+        t.fill_(float("nan"))
+    lib.release_workspace()
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    hog = torch.empty(free - (100 << 20), dtype=torch.uint8, device="cuda")
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            step()
+        torch.cuda.synchronize()
+    finally:
+        del hog
+        torch.cuda.empty_cache()
+    assert "pair" in plans[0] and "pair" in plans[1], plans
+    assert "planes 128x" in plans[4] and "planes 128x" in plans[5], plans
+    # sums of K terms with deviation sqrt(K): either way within a few 2^-23 of that
+    for got, ref in zip((Y, Z, dX, dW, dB), want):
+        assert float((got - ref).norm() / ref.norm()) <= 2.0 ** -20
+    assert lib.device_status() == 0
