@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -10,6 +11,21 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (run with -m gpu on the GPU box)")
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_runtest_call(item):
+    """No garbage collection inside a stream capture: a CUDA graph that an earlier test left in a reference cycle (an exception's traceback holds its
+    frame) would be destroyed there, which invalidates the capture."""
+    if "capture" not in item.name:
+        yield
+        return
+    gc.collect()
+    gc.disable()
+    try:
+        yield
+    finally:
+        gc.enable()
 
 
 @pytest.fixture(scope="session")
