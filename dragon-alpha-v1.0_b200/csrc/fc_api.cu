@@ -300,16 +300,19 @@ struct ProductF32 { const float *A, *B; int rows, cols, K, OC, pitch, halves, ld
 struct Planes { void* ptr = nullptr; const float* src = nullptr; int rows = 0, cols = 0, pitch = 0; };
 Planes planes_of(const float* src, int rows, int cols) { return Planes{nullptr, src, rows, cols, (cols + 7) / 8 * 8}; }
 size_t plane_bytes(const Planes& p) { return (6 * static_cast<size_t>(p.rows) * p.pitch + 255) & ~static_cast<size_t>(255); }
-int launch_split(const Planes* const* list, int n, int sms, cudaStream_t stream)
+unsigned most_split_ctas(int sms) { return static_cast<unsigned>(sms) * 16; }
+int launch_split(const Planes* const* list, int n, uint32_t* seen, int* ctas, int sms, cudaStream_t stream)
 {
     SplitJobs j{};
+    j.seen = seen;
     for (int i = 0; i < n; ++i) {
         const Planes& p = *list[i];
         j.job[j.n++] = SplitJob{p.src, static_cast<uint2*>(p.ptr), static_cast<unsigned>(p.rows), static_cast<unsigned>(p.cols / 4), j.total, fast_div(p.pitch / 4)};
         j.total += static_cast<unsigned>(p.rows) * static_cast<unsigned>(p.pitch / 4);
     }
-    const unsigned blocks = (j.total + 255) / 256, most = static_cast<unsigned>(sms) * 16;
-    launch_after(fc_split_kernel, blocks < most ? blocks : most, 256, 0, stream, j);
+    const unsigned blocks = (j.total + 255) / 256, most = most_split_ctas(sms);
+    *ctas = static_cast<int>(blocks < most ? blocks : most);
+    launch_after(fc_split_kernel, *ctas, 256, 0, stream, j);
     note_launch("fc");
     return launched("fc_split_kernel");
 }
@@ -330,6 +333,9 @@ PairPlan pick_pair(int rows, int m_halves, int out_cols, bool glu, int K, int k_
         for (int parts = 1; parts <= 32 && parts <= windows; ++parts) {
             const int each = (windows + parts - 1) / parts;
             if ((parts - 1) * each >= windows) continue;                      // (no part is empty)
+            // (sums formed once more take 0.1 us a step and 32 columns, 0.8 s of 32768 windows: a pair's next item waits 2 s at most.  All SMs need no such
+            // tensor as fits for a second item of that length, a few of them may)
+            if (each > 32768 && tiles * parts > pairs) continue;
             const double waves = static_cast<double>(static_cast<long long>((tiles * parts + pairs - 1) / pairs));
             const double time = 5.0 + waves * (bn == 256 ? each * 2.26 + 2.0 : each * 1.34 + 1.8) + (parts > 1 ? 3.0 + size * 4e-6 * (2 * parts + 1) / 6.0 : 0.0);
             if (time < best.time) best = PairPlan{bn, parts, time};
@@ -340,7 +346,7 @@ PairPlan pick_pair(int rows, int m_halves, int out_cols, bool glu, int K, int k_
 double split_time(size_t elements) { return 2.0 + elements * 10e-6 / 8.0; }
 
 template <int FORM>
-int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, int sms, int* status, cudaStream_t stream)
+int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, const uint32_t* seen, int seen_n, int sms, int* status, cudaStream_t stream)
 {
     constexpr bool GLU = FORM == kFcGlu, A_MN = FORM == kFcDeltaW, B_MN = FORM == kFcDeltaX || FORM == kFcDeltaW;
     const bool forward = FORM == kFcForward || FORM == kFcGlu;
@@ -357,7 +363,7 @@ int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const Pai
     p.a_row = A_MN ? 1 : q.lda; p.a_k = A_MN ? q.lda : 1; p.a_half = q.pitch;
     p.b_col = B_MN ? 1 : q.ldb; p.b_k = B_MN ? q.ldb : 1; p.b_half = static_cast<long long>(q.OC) * q.ldb;
     p.bias = q.e.bias; p.residual = q.e.residual; p.act = q.e.act; p.k = q.e.k; p.keep_z = parts == 1 && q.e.Z;
-    p.status = status;
+    p.status = status; p.seen = seen; p.seen_n = seen_n;
     // sums and results: (column, half of the columns or rows, row, part)
     const int out_pitch = forward ? q.pitch : q.cols;
     const size_t size = static_cast<size_t>(p.rows) * m_halves * out_pitch * (GLU ? 2 : 1);
@@ -452,23 +458,27 @@ struct PairWork {
     size_t parts = 0;          // bytes of the larger of the products' parts
     int sms = 0, *status = nullptr;
     void* part = nullptr;
+    uint32_t* seen = nullptr; int seen_n = 0;
     int add(const float* src, int rows, int cols) { p[n] = planes_of(src, rows, cols); return n++; }
     void want(const ProductF32& q, int k) { const size_t bytes = k > 1 ? k * static_cast<size_t>(q.rows) * q.cols * sizeof(float) : 0; if (bytes > parts) parts = bytes; }   // (padding too)
     size_t elements() const { size_t e = 0; for (int i = 0; i < n; ++i) e += static_cast<size_t>(p[i].rows) * p[i].pitch; return e; }
     bool fits() const { return elements() < 4ull << 31; }           // 32-bit indices of words of four
     int split(cudaStream_t stream)
     {
-        size_t bytes = parts;
+        const size_t seen_bytes = (most_split_ctas(sms) * sizeof(uint32_t) + 255) & ~static_cast<size_t>(255);
+        size_t bytes = parts + seen_bytes;
         for (int i = 0; i < n; ++i) bytes += plane_bytes(p[i]);
         void* ws = nullptr;
         const int rc = call_scratch(stream, bytes, &ws);
         if (rc) return scratch_refused(rc) ? 1 : rc;
         if (dry_run()) return ALPHA_OK;
         char* at = static_cast<char*>(ws);
+        seen = reinterpret_cast<uint32_t*>(at);
+        at += seen_bytes;
         for (int i = 0; i < n; ++i) { p[i].ptr = at; at += plane_bytes(p[i]); }
         part = at;
         const Planes* list[3] = {&p[0], &p[1], &p[2]};
-        return launch_split(list, n, sms, stream);
+        return launch_split(list, n, seen, &seen_n, sms, stream);
     }
 };
 
@@ -491,7 +501,7 @@ int forward_f32(const ProductF32& q, cudaStream_t stream)
     w.want(q, pair.parts);
     if (w.sms >= 2 && w.fits() && pairs_pay(pair.time + split_time(w.elements()), pick_gathered<FORM>(q, w.sms).time)) {
         rc = w.split(stream);
-        if (rc == 0) return dry_run() ? ALPHA_OK : launch_pair<FORM>(q, w.p[a], w.p[b], pair, w.part, w.sms, w.status, stream);
+        if (rc == 0) return dry_run() ? ALPHA_OK : launch_pair<FORM>(q, w.p[a], w.p[b], pair, w.part, w.seen, w.seen_n, w.sms, w.status, stream);
         if (rc < 0) return rc;
     }
     return run_gathered<FORM>(q, w.sms, w.status, stream);
@@ -534,8 +544,8 @@ int delta_f32(const float* dZ, const float* X, const float* W, float* dX, float*
         if (rc == 1) best_x = best_w = false;
     }
     rc = ALPHA_OK;
-    if (best_x && !dry_run()) rc = launch_pair<kFcDeltaX>(x, best.p[0], best.p[1], px, best.part, sms, status, stream);
-    if (!rc && best_w && !dry_run()) rc = launch_pair<kFcDeltaW>(w, best.p[0], best.p[best_x ? 2 : 1], pw, best.part, sms, status, stream);
+    if (best_x && !dry_run()) rc = launch_pair<kFcDeltaX>(x, best.p[0], best.p[1], px, best.part, best.seen, best.seen_n, sms, status, stream);
+    if (!rc && best_w && !dry_run()) rc = launch_pair<kFcDeltaW>(w, best.p[0], best.p[best_x ? 2 : 1], pw, best.part, best.seen, best.seen_n, sms, status, stream);
     if (!rc && dX && !best_x) rc = run_gathered<kFcDeltaX>(x, sms, status, stream);
     if (!rc && dW && !best_w) rc = run_gathered<kFcDeltaW>(w, sms, status, stream);
     return rc;

@@ -78,3 +78,148 @@ def test_f32_runs_without_scratch_where_the_card_is_full(eng, lib):
     for got, ref in zip((Y, Z, dX, dW, dB), want):
         assert float((got - ref).norm() / ref.norm()) <= 2.0 ** -20
     assert lib.device_status() == 0
+
+
+# ---- fp32 products: operands of every magnitude, without a cost for the ordinary ones beside them ----
+
+PAIRS = pytest.mark.parametrize("tile", (1, 11, 2), ids=("pairs", "pairs of 128 columns", "gathered"))
+
+
+@pytest.fixture
+def tiled(lib):
+    held = []
+
+    def set_tile(tile):
+        held.append(lib.set_option("FC_TILE", tile))
+    yield set_tile
+    for old in reversed(held):
+        lib.set_option("FC_TILE", old)
+    assert lib.device_status() == 0, lib.last_error()
+
+
+def near(got, a, b):
+    """got = a b: (K / 16 + 8) 2^-22 of the sum of magnitudes (hh accumulators truncate, at most 2^-23 of a product is dropped), an output's rounding, and the last place of a
+    denormal, 2^-149, in each product and sum."""
+    K = a.shape[1]
+    ref, S = a.double() @ b.double(), a.double().abs() @ b.double().abs()
+    bad = ~((got.double() - ref).abs() <= (K / 16 + 8) * 2.0 ** -22 * S + 2.0 ** -24 * ref.abs() + K * 2.0 ** -148)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+def powers(n):
+    """2^0 ... 2^-148, n of them."""
+    return torch.exp2(-torch.linspace(0, 148, n, dtype=torch.float64, device="cuda"))
+
+
+def of_magnitudes(gen, what, m, n):
+    t = torch.randn(m, n, device="cuda", generator=gen, dtype=torch.float64)
+    if what == "rows":
+        t *= powers(m)[:, None]
+    elif what == "columns":
+        t *= powers(n)
+    elif what == "elements":
+        t *= torch.exp2(-torch.randint(0, 149, (m, n), device="cuda", generator=gen).double())
+    return t.float()
+
+
+@PAIRS
+@pytest.mark.parametrize("first,second", [("rows", ""), ("columns", ""), ("elements", ""), ("", "rows"), ("", "columns"), ("", "elements"), ("rows", "rows"), ("elements", "elements")])
+def test_f32_of_every_magnitude(eng, tiled, tile, first, second):
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    tiled(tile)
+    rows, IC, OC = 301, 204, 149
+    X, W, V, dY = of_magnitudes(gen, first, rows, IC), of_magnitudes(gen, second, OC, IC), of_magnitudes(gen, second, 2 * OC, IC), of_magnitudes(gen, first, rows, OC)
+    near(eng.fullConnect(X, W), X, W.T)
+    near(eng.fullConnect_glu(X, V, act="none", save=True)[1], X, V.T)
+    dX, dW, _ = eng.fullConnect_delta(dY, X, W)
+    near(dX, dY, W)
+    near(dW, dY.T, X)
+    # (gates and ups of deltaZ: act 'none' and U = G = 1 make both of them deltaY)
+    one = torch.ones(rows, 2 * OC, device="cuda")
+    dX, dV, _ = eng.fullConnect_glu_delta(dY, X, V, one, act="none")
+    both = torch.cat([dY, dY], 1)
+    near(dX, both, V)
+    near(dV, both.T, X)
+
+
+@PAIRS
+@pytest.mark.parametrize("everywhere", (True, False))
+def test_f32_rows_and_columns_of_zeros_beside_tiny_elements(eng, tiled, tile, everywhere):
+    """`everywhere`: a column of X and of W holds denormals, in the rows that are zero otherwise too."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    tiled(tile)
+    rows, IC, OC = 520, 300, 260
+    X, W, dY = of_magnitudes(gen, "", rows, IC), of_magnitudes(gen, "", OC, IC), of_magnitudes(gen, "", rows, OC)
+    X[::3], W[::5], dY[:, ::7] = 0, 0, 0
+    X[1, 5] = W[2, 9] = dY[4, 8] = 1e-36
+    if everywhere:
+        X[:, 11] = W[:, 12] = 3e-40
+    Y = eng.fullConnect(X, W)
+    near(Y, X, W.T)
+    zero = (X.double().abs() @ W.double().abs().T) == 0
+    assert bool(zero[::3].all()) != everywhere and not Y[zero].any()
+    dX, dW, _ = eng.fullConnect_delta(dY, X, W)
+    near(dX, dY, W)
+    near(dW, dY.T, X)
+    assert not dW[::7].any()
+
+
+@PAIRS
+def test_f32_infinite_beside_tiny_elements(eng, tiled, tile):
+    """What an Inf meets is Inf or NaN as in 64 bits, its neighbours in a word keep their values."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    tiled(tile)
+    rows, IC, OC = 300, 200, 136
+    X, W = of_magnitudes(gen, "", rows, IC), of_magnitudes(gen, "", OC, IC)
+    X[7, 20], X[7, 21], X[8, 21], X[9, 22], X[40, 23] = float("inf"), 1e-36, 1e-37, 3.4e38, float("nan")
+    W[:, 20:24] *= 2.0 ** -20
+    Y = eng.fullConnect(X, W)
+    ref = X.double() @ W.double().T
+    assert torch.equal(torch.isnan(Y), torch.isnan(ref)) and torch.equal(torch.isinf(Y), torch.isinf(ref))
+    fine = torch.ones(rows, dtype=torch.bool, device="cuda")
+    fine[7] = fine[40] = False
+    near(Y[fine], X[fine], W.T)
+
+
+def test_f32_softmax_tails_cost_little(eng, lib):
+    """deltaY of a classifier whose softmax has tails of 1e-30 to 1e-45: the sums it goes into are ordinary, and are not formed once more.  They
+    took 53 times as long as without."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    rows, IC, OC = 512, 4096, 1000
+    X, W = torch.randn(rows, IC, device="cuda", generator=gen), torch.randn(OC, IC, device="cuda", generator=gen) * IC ** -0.5
+    logits = torch.randn(rows, OC, device="cuda", generator=gen)
+    times = []
+    for sharp in (1, 40):
+        dY = torch.softmax(logits * sharp, 1)
+        assert bool(((dY > 0) & (dY < 1e-33)).any()) == (sharp > 1)
+        best = 1e9
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            dX, dW, _ = eng.fullConnect_delta(dY, X, W)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        assert "pair" in lib.last_plan()
+        times.append(best)
+        near(dX, dY, W)
+        near(dW, dY.T, X)
+    assert times[1] <= 5 * times[0], times
+
+
+def test_f32_long_reductions_on_few_sms(eng, lib):
+    """Two tiles in turn on one pair, 2.2 million steps each: should the sums of the first have to be formed once more, the second could wait too long.  They are cut, or gathered."""
+    rows, IC, OC = 257, 2200000, 128
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    X, W = torch.randn(rows, IC, device="cuda", generator=gen), torch.randn(OC, IC, device="cuda", generator=gen)
+    old = lib.set_option("SM_BUDGET", 2)
+    try:
+        Y = eng.fullConnect(X, W)
+        plan = lib.last_plan()
+        assert "planes 128x" in plan or int(plan.split("parts=")[1]) > 1, plan
+    finally:
+        lib.set_option("SM_BUDGET", old)
+    some = torch.tensor([0, 100, 255, 256], device="cuda")
+    near(Y[some], X[some], W.T)
+    eng.fullConnect(X, W)
+    assert lib.device_status() == 0
