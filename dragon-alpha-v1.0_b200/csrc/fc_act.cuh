@@ -33,12 +33,20 @@ __device__ __forceinline__ NormalCdf normal_cdf_16(float z)
     return NormalCdf{z >= 0.f ? 1.f - tail : tail, e};
 }
 
+// k z of a LeakyReLU.  With k = 0 it is a ReLU, whose value at -Inf is 0 and not the NaN of 0 * -Inf; a NaN stays one.
+__device__ __forceinline__ float leaky(float z, float k)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(z), "f"(k == 0.f ? -0x1.fffffep127f : -__int_as_float(0x7f800000)));
+    return k * y;
+}
+
 // Value and slope of activation ACT at z.  Quotients err by 2 units of 2^-23, exponentials by as much, or (FAST, for results that are rounded to
-// 16 bits) by 2 + |argument| units.  z = -Inf gives NaN where the definition is -Inf * 0 (silu, gelu).
+// 16 bits) by 2 + |argument| units.  z = -Inf gives NaN where the definition is -Inf * 0 (silu, gelu, gelu_tanh).
 template <int ACT, bool FAST> __device__ __forceinline__ float act_value(float z, float k)
 {
     if constexpr (ACT == ALPHA_ACT_NONE) return z;
-    else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) return z > 0.f ? z : k * z;
+    else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) return z > 0.f ? z : leaky(z, k);
     else if constexpr (ACT == ALPHA_ACT_SIGMOID) return FAST ? __fdividef(1.f, 1.f + __expf(-z)) : sigmoid_both<FAST>(z).pos;
     else if constexpr (ACT == ALPHA_ACT_SILU) return __fdividef(z, 1.f + (FAST ? __expf(-z) : expf(-z)));
     else if constexpr (ACT == ALPHA_ACT_GELU) return FAST ? z * normal_cdf_16(z).cdf : 0.5f * z * erfcf(-0.70710678f * z);
@@ -51,7 +59,7 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_value(float z
 template <int ACT, bool FAST> __device__ __forceinline__ void act_both(float z, float k, float& value, float& slope)
 {
     if constexpr (ACT == ALPHA_ACT_NONE) { value = z; slope = 1.f; }
-    else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) { slope = z > 0.f ? 1.f : k; value = slope * z; }
+    else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) { slope = z > 0.f ? 1.f : k; value = z > 0.f ? z : leaky(z, k); }
     else if constexpr (ACT == ALPHA_ACT_SIGMOID) {
         const Sigmoid s = sigmoid_both<FAST>(z);
         value = s.pos; slope = s.pos * s.neg;

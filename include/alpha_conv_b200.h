@@ -471,7 +471,7 @@ int alpha_engine_batchMatMulT2(float* C, const float* A, const float* B, int Bat
  * with deltaX, deltaW like X, W and deltaY, deltaB like Y, bias.
  * deltaX, deltaW and deltaB may each be NULL (not computed).  deltaZ is memory of the caller's, the size of Z, and may be Z
  * itself; it holds deltaZ rounded to the tensors' type afterwards.  ALPHA_ACT_NONE without gates needs neither Z nor deltaZ.
- * At 0 the slope of a LeakyReLU is k.  Results do not depend on scheduling (fixed summation orders, no atomics). */
+ * At 0 the slope of a LeakyReLU is k.  At -Inf a ReLU (k = 0) gives 0; silu, gelu and gelu_tanh, whose formulas are -Inf * 0 there, NaN.  Results do not depend on scheduling (fixed summation orders, no atomics). */
 #define ALPHA_F32 0
 #define ALPHA_BF16 1
 #define ALPHA_F16 2

@@ -223,3 +223,48 @@ def test_f32_long_reductions_on_few_sms(eng, lib):
     near(Y[some], X[some], W.T)
     eng.fullConnect(X, W)
     assert lib.device_status() == 0
+
+
+# ---- activations at the ends of their range ----
+
+ROUTES = [("f32", 2, 0), ("f32", 70, 2), ("f32", 70, 1), ("bf16", 2, 0), ("bf16", 70, 0), ("f16", 2, 0), ("f16", 70, 1)]
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def through_act(eng, tiled, dtype, rows, tile, act, k, values):
+    """act of `values` (at most 8), the same by the gated block (U = 1), and both gradients of deltaY = 1; rows x 8 each, the values as columns.  W takes
+    them through unchanged: X is 1 in its first column and 0 behind, W has them as its first column."""
+    t = TYPES[dtype]
+    tiled(tile)
+    z = torch.tensor(values, device="cuda").to(t)
+    X = torch.zeros(rows, 8, device="cuda", dtype=t)
+    X[:, 0] = 1
+    bias = torch.zeros(8, device="cuda", dtype=t)
+    bias[:len(values)] = z                          # (by the bias: an Inf in W would meet zeros)
+    W = torch.zeros(8, 8, device="cuda", dtype=t)
+    y = eng.fullConnect(X, W, bias, act=act, k=k)
+    g = eng.fullConnect_glu(X, torch.zeros(16, 8, device="cuda", dtype=t), torch.cat([bias, torch.ones_like(bias)]), act=act, k=k)
+    Z = bias.expand(rows, 8).contiguous()
+    one = torch.ones(rows, 8, device="cuda", dtype=t)
+    # deltaB sums a column's rows: of one row it is deltaZ itself
+    slope = eng.fullConnect_delta(one[:1], X[:1], W, Z[:1], act=act, k=k, bias=True)[2]
+    both = eng.fullConnect_glu_delta(one[:1], X[:1], torch.zeros(16, 8, device="cuda", dtype=t), torch.cat([Z, one], 1)[:1], act=act, k=k, bias=True)[2]
+    assert torch.equal(torch.nan_to_num(both[:8], 99.0), torch.nan_to_num(slope, 99.0))
+    n = len(values)
+    assert all(torch.equal(torch.nan_to_num(r, 99.0), torch.nan_to_num(a[0], 99.0)) for a in (y, g) for r in a)
+    return z.double(), y[0, :n].double(), g[0, :n].double(), both[8:8 + n].double(), slope[:n].double()
+
+
+@pytest.mark.parametrize("dtype,rows,tile", ROUTES)
+@pytest.mark.parametrize("k", (0.0, 0.2, 1.0, -0.5))
+def test_relu_of_infinities(eng, tiled, dtype, rows, tile, k):
+    """A LeakyReLU of slope 0 is a ReLU: 0 at -Inf.  Any other slope times -Inf is infinite; NaN stays."""
+    inf, nan = float("inf"), float("nan")
+    z, *values, slope = through_act(eng, tiled, dtype, rows, tile, "leakyRelu", k, [-inf, inf, nan, -2.0, 3.0, 0.0])
+    want = torch.tensor([-inf * k if k else 0.0, inf, nan, -2.0 * k, 3.0, 0.0], device="cuda", dtype=torch.float64)
+    for y in values:
+        assert torch.equal(torch.isnan(y), torch.isnan(want))
+        fine = ~torch.isnan(want)
+        assert torch.equal(torch.isinf(y), torch.isinf(want)) and torch.equal(y[torch.isinf(want)], want[torch.isinf(want)])
+        assert ((y - want)[fine & torch.isfinite(want)].abs() <= torch.finfo(TYPES[dtype]).eps * want[fine & torch.isfinite(want)].abs()).all()
+    assert torch.equal(slope.to(TYPES[dtype]), torch.tensor([k, 1.0, k, k, 1.0, k], device="cuda").to(TYPES[dtype]).double().to(TYPES[dtype]))
