@@ -8,7 +8,8 @@
 
 namespace alpha {
 
-// Sigmoid of z, and of -z, from one exponential of a value that cannot overflow: neither loses the digits that 1 - s would.
+// Sigmoid of z, and of -z, from one exponential of a value that cannot overflow: neither loses the digits that 1 - s would, nor is there a quotient by more than
+// 2^126, for which __fdividef gives 0 (silu(-88) is -5e-37, no denormal).
 struct Sigmoid { float pos, neg; };
 template <bool FAST> __device__ __forceinline__ Sigmoid sigmoid_both(float z)
 {
@@ -47,13 +48,12 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_value(float z
 {
     if constexpr (ACT == ALPHA_ACT_NONE) return z;
     else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) return z > 0.f ? z : leaky(z, k);
-    else if constexpr (ACT == ALPHA_ACT_SIGMOID) return FAST ? __fdividef(1.f, 1.f + __expf(-z)) : sigmoid_both<FAST>(z).pos;
-    else if constexpr (ACT == ALPHA_ACT_SILU) return __fdividef(z, 1.f + (FAST ? __expf(-z) : expf(-z)));
+    else if constexpr (ACT == ALPHA_ACT_SIGMOID) return sigmoid_both<FAST>(z).pos;
+    else if constexpr (ACT == ALPHA_ACT_SILU) return z * sigmoid_both<FAST>(z).pos;
     else if constexpr (ACT == ALPHA_ACT_GELU) return FAST ? z * normal_cdf_16(z).cdf : 0.5f * z * erfcf(-0.70710678f * z);
     else {
         // z (1 + tanh(u)) / 2 = z sigmoid(2 u)
-        const float u2 = 1.59576912f * (z + 0.044715f * z * z * z);
-        return __fdividef(z, 1.f + (FAST ? __expf(-u2) : expf(-u2)));
+        return z * sigmoid_both<FAST>(1.59576912f * (z + 0.044715f * z * z * z)).pos;
     }
 }
 template <int ACT, bool FAST> __device__ __forceinline__ void act_both(float z, float k, float& value, float& slope)

@@ -268,3 +268,24 @@ def test_relu_of_infinities(eng, tiled, dtype, rows, tile, k):
         assert torch.equal(torch.isinf(y), torch.isinf(want)) and torch.equal(y[torch.isinf(want)], want[torch.isinf(want)])
         assert ((y - want)[fine & torch.isfinite(want)].abs() <= torch.finfo(TYPES[dtype]).eps * want[fine & torch.isfinite(want)].abs()).all()
     assert torch.equal(slope.to(TYPES[dtype]), torch.tensor([k, 1.0, k, k, 1.0, k], device="cuda").to(TYPES[dtype]).double().to(TYPES[dtype]))
+
+
+@pytest.mark.parametrize("dtype,rows,tile", [r for r in ROUTES if r[0] != "f16"])
+@pytest.mark.parametrize("act", ("silu", "gelu_tanh", "sigmoid"))
+def test_small_values_of_large_arguments(eng, tiled, dtype, rows, tile, act):
+    """Values far below zero, down to where fp32 has no normal numbers, in the forward pass and in the gradient of the ups alike.
+
+    Errors: the exponential's 2 units of 2^-23 (of the type's fast one 2 + 1.16 |argument|), the argument's rounding as often as the argument is large - of
+    gelu_tanh seven roundings of it -, three more roundings, and the output's; of denormals their spacing, times |z| where it is multiplied by it."""
+    t = TYPES[dtype]
+    half = torch.finfo(t).eps / 2
+    values = {"gelu_tanh": [-9.0, -10.0, -10.1, -10.2, -10.25, -10.3], "silu": [-80.0, -87.0, -87.5, -88.0, -90.0, -92.0], "sigmoid": [-80.0, -86.0, -87.0, -87.3, -88.0, -100.0]}[act]
+    z, y, g, up, _ = through_act(eng, tiled, dtype, rows, tile, act, 0.0, values)
+    u = z if act != "gelu_tanh" else 1.5957691216057308 * (z + 0.044715 * z ** 3)
+    s = torch.exp(u) / (1 + torch.exp(u))
+    want = (s if act == "sigmoid" else z * s)[:len(values)]
+    z, u = z[:len(values)], u[:len(values)]
+    rel = 2.0 ** -23 * ((2 if dtype == "f32" else 2 + 1.16 * u.abs()) + 3) + (7 * 2.0 ** -24 * u.abs() if act == "gelu_tanh" else 0)
+    tiny = (1 if act == "sigmoid" else z.abs()) * 2.0 ** -148 + (2.0 ** -134 if dtype == "bf16" else 2.0 ** -149)
+    for got in (y, g, up):
+        assert ((got - want).abs() <= (rel + half) * want.abs() * 1.01 + tiny).all(), (got, want)
