@@ -467,6 +467,69 @@ def _fc_act(what, act):
     return code
 
 
+def _same_memory(g, o):
+    return g is o or (g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.shape == o.shape and g.stride() == o.stride() and g.is_neg() == o.is_neg())
+
+
+def _memory_of(t):
+    """Where a tensor lies: its first byte, the byte after its last, and, if its elements are rows of `wide` bytes `pitch` apart, these (else 0, 0; a dense tensor
+    is one row).  None where elements may share memory."""
+    dims = sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1)
+    size, wide, pitch, reach = t.element_size(), 1, 0, 1         # in elements; reach: from the first to after the last
+    for st, n in dims:
+        if st < reach:
+            return None
+        if not pitch and st == wide:
+            wide *= n
+        elif not pitch:
+            pitch, rows = st, n
+        elif st == pitch * rows:
+            rows *= n
+        else:
+            pitch = -1
+        reach += (n - 1) * st
+    at = t.data_ptr()
+    if pitch < 0:
+        return at, at + reach * size, 0, 0
+    return at, at + reach * size, wide * size, pitch * size
+
+
+def _apart(a, b):
+    """Whether two tensors (_memory_of) share no byte, as far as can be told: disjoint, or columns of rows of one pitch."""
+    if a[0] > b[0]:
+        a, b = b, a
+    if a[1] <= b[0]:
+        return True
+    if not a[2] or not b[2] or (a[3] and b[3] and a[3] != b[3]):
+        return False
+    pitch, d = a[3] or b[3], b[0] - a[0]
+    if not pitch or (not a[3] and a[2] > pitch) or (not b[3] and b[2] > pitch):
+        return False
+    d %= pitch
+    return d >= a[2] and d + b[2] <= pitch
+
+
+def _refuse_overlaps(what, grads, Out):
+    """Raises where an output overlaps itself, another output or a gradient that is not its own (as the library does for dense tensors)."""
+    places = []                          # (place, written)
+    for g, o in zip(grads, Out):
+        if o.numel() == 0:
+            continue
+        place = _memory_of(o)
+        if place is None:
+            raise ValueError("%s: elements of an output share memory" % what)
+        places.append((place, True))
+        if not _same_memory(g, o):
+            places.append((_memory_of(g) or (g.data_ptr(), g.data_ptr() + g.element_size() * (1 + sum((n - 1) * st for n, st in zip(g.shape, g.stride()))), 0, 0), False))
+    places.sort()
+    for i, (a, write) in enumerate(places):
+        for b, other in itertools.islice(places, i + 1, None):
+            if b[0] >= a[1]:
+                break
+            if (write or other) and not _apart(a, b):
+                raise ValueError("%s: an output overlaps another tensor" % what)
+
+
 _pack_jobs = {n: struct.Struct("%dq" % (6 * n)).pack for n in (1, 2, 3)}
 
 
@@ -736,18 +799,16 @@ class Engine:
         return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
 
     @staticmethod
-    def _grads(what, grads, Out):
-        """The tensors as the table the library reads (AlphaGrad: two addresses, a count, two types)."""
+    def _check_grads(what, grads, Out):
+        """Raises for tensors the library would not read, else returns (all of them, their type codes, whether all are dense)."""
         # (a pass over all tensors for each question: half the time of a loop that asks them one by one)
         T, device, both = torch.Tensor, grads[0].get_device(), grads if Out is grads else grads + Out
-        n, at = len(grads), list(map(T.data_ptr, both))
         codes = list(map(_FC_TYPES.get, map(_dtype_of, both)))
-        if (device < 0 or set(map(T.get_device, both)) != {device} or not all(map(T.is_contiguous, both)) or any(map(T.is_neg, both)) or None in codes
+        if (device < 0 or set(map(T.get_device, both)) != {device} or None in codes
                 or (both is not grads and list(map(_shape_of, grads)) != list(map(_shape_of, Out)))):
             for g, o in zip(grads, Out):
                 Engine._refuse_grads(what, device, g, o)
-        types = [g | o << 32 for g, o in zip(codes, codes[-n:])]
-        return struct.pack("<%dq" % (4 * n), *itertools.chain.from_iterable(zip(at, at[-n:], map(T.numel, grads), types)))
+        return both, codes, all(map(T.is_contiguous, both)) and not any(map(T.is_neg, both))
 
     @staticmethod
     def _refuse_grads(what, device, g, o):
@@ -757,35 +818,73 @@ class Engine:
         for t in (g, o):
             if t.dtype not in _FC_TYPES:
                 raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, t.dtype))
-            if not t.is_contiguous() or t.is_neg():
-                raise ValueError("%s: tensors must be contiguous" % what)
         if g.shape != o.shape:
             raise ValueError("%s: gradient %s, output %s" % (what, tuple(g.shape), tuple(o.shape)))
+
+    @staticmethod
+    def _grad_table(n, both, codes):
+        """The tensors as the table the library reads (AlphaGrad: two addresses, a count, two types)."""
+        at = list(map(torch.Tensor.data_ptr, both))
+        types = [g | o << 32 for g, o in zip(codes, codes[-n:])]
+        return struct.pack("<%dq" % (4 * n), *itertools.chain.from_iterable(zip(at, at[-n:], map(torch.Tensor.numel, both), types)))
+
+    @staticmethod
+    def _dense_grads(what, grads, Out):
+        """Dense copies of the tensors that are not (an output that is one gets its own), and the pairs (output, copy) to be copied back.  Such are the views that
+        fullConnect_delta returns where IC is no multiple of 16 bytes."""
+        _refuse_overlaps(what, grads, Out)
+        dense, to, back = [], [], []
+        for g, o in zip(grads, Out):
+            same = _same_memory(g, o)
+            d = g.resolve_neg().contiguous()
+            if o.is_contiguous() and not o.is_neg():
+                t = o
+            elif same:
+                t = d                                   # (a copy of its own: g is not dense)
+            else:
+                t = torch.empty(o.shape, dtype=o.dtype, device=o.device)
+            if t is not o:
+                back.append((o, t))
+            dense.append(t if same else d)
+            to.append(t)
+        return dense, to, back
 
     def grad_norm(self, grads):
         """The 2-norm of all elements of a list of gradients (float32, bfloat16, float16) as a 0-dimensional float32 tensor."""
         grads = list(grads)
         if not grads:
             return torch.zeros((), device="cuda")
-        table = self._grads("grad_norm", grads, grads)
+        both, codes, dense = self._check_grads("grad_norm", grads, grads)
         with self._on(grads[0]):
+            if not dense:
+                with torch.no_grad():
+                    both = [g.resolve_neg().contiguous() for g in grads]
             norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-            _l.check(self.base._lib.alpha_grad_norm(len(grads), table, norm.data_ptr(), _stream(self.base._stream)))
+            _l.check(self.base._lib.alpha_grad_norm(len(grads), self._grad_table(len(grads), both, codes), norm.data_ptr(), _stream(self.base._stream)))
         return norm
 
     def clip_grad_norm(self, grads, max_norm, Out=None):
         """grad_norm, and every gradient scaled by min(1, max_norm / (norm + 1e-6)): in place, or into the tensors of Out, which may
-        be of another type.  Nothing waits for the norm on the host."""
+        be of another type.  Nothing waits for the norm on the host.  Tensors that are not dense go through copies; an output must not overlap itself or
+        another tensor of the call."""
         grads = list(grads)
         Out = grads if Out is None else list(Out)
         if len(Out) != len(grads):
             raise ValueError("clip_grad_norm: %d gradients, %d outputs" % (len(grads), len(Out)))
         if not grads:
             return torch.zeros((), device="cuda")
-        table = self._grads("clip_grad_norm", grads, Out)
+        both, codes, dense = self._check_grads("clip_grad_norm", grads, Out)
+        max_norm, back = float(max_norm), ()
         with self._on(grads[0]):
+            if not dense:
+                with torch.no_grad():
+                    src, to, back = self._dense_grads("clip_grad_norm", grads, Out)
+                both, codes = src + to, codes if len(codes) > len(grads) else codes + codes
             norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-            _l.check(self.base._lib.alpha_clip_grad_norm(len(grads), table, float(max_norm), norm.data_ptr(), _stream(self.base._stream)))
+            _l.check(self.base._lib.alpha_clip_grad_norm(len(grads), self._grad_table(len(grads), both, codes), max_norm, norm.data_ptr(), _stream(self.base._stream)))
+            with torch.no_grad():
+                for o, t in back:
+                    o.copy_(t)
         return norm
 
     # Batched products with the engine's memory rule (only the last dimension of a tensor is padded to a multiple
