@@ -29,9 +29,10 @@ def _stream(stream=None):
 
 
 # Shapes as the C structures the library reads (it never writes them): a program calls a few layers over and over.  The caches see
-# plain ints only: 3.0 would find the entry of 3, and a tensor the entry it made before its value changed.
+# plain ints only (and the slope as a float): 3.0 would find the entry of 3, and a tensor the entry it made before its value changed.
 _cached_conv_shape = functools.lru_cache(maxsize=512)(_l.AlphaConvShape)
 _cached_pool_shape = functools.lru_cache(maxsize=512)(_l.AlphaPoolShape)
+_cached_fc_shape = functools.lru_cache(maxsize=512)(_l.AlphaFcShape)
 
 
 def _conv_shape(*dims):
@@ -40,6 +41,10 @@ def _conv_shape(*dims):
 
 def _pool_shape(*dims):
     return _cached_pool_shape(*map(operator.index, dims))
+
+
+def _fc_shape(rows, IC, OC, dtype, act, k):
+    return _cached_fc_shape(*map(operator.index, (rows, IC, OC, dtype, act)), float(k))
 
 
 def _new(like, shape, dtype=torch.float32):
@@ -292,13 +297,13 @@ class CudaFloat32EngineBase:
     def fullConnect(self, Y_address, X_address, W_address, rows, IC, OC, dtype, act, k, Bias_address=None, Residual_address=None, Z_address=None):
         """Y = act(X W^T + Bias) + Residual, Z = X W^T + Bias; addresses of X[rows, IC], W[OC, IC], and so on (alpha_fullConnect)."""
         a = self._addr_or_none
-        _l.check(self._lib.alpha_fullConnect(C.byref(_cached_fc_shape(rows, IC, OC, dtype, act, float(k))), a(X_address), a(W_address), a(Bias_address), a(Residual_address),
+        _l.check(self._lib.alpha_fullConnect(C.byref(_fc_shape(rows, IC, OC, dtype, act, k)), a(X_address), a(W_address), a(Bias_address), a(Residual_address),
                                              a(Z_address), a(Y_address), _stream(self._stream)))
 
     def fullConnect_glu(self, Y_address, X_address, W_address, rows, IC, OC, dtype, act, k, Bias_address=None, Z_address=None):
         """Y = act(Z[:, :OC]) * Z[:, OC:], Z = X W^T + Bias with W[2 OC, IC] (alpha_fullConnect_glu)."""
         a = self._addr_or_none
-        _l.check(self._lib.alpha_fullConnect_glu(C.byref(_cached_fc_shape(rows, IC, OC, dtype, act, float(k))), a(X_address), a(W_address), a(Bias_address), a(Z_address),
+        _l.check(self._lib.alpha_fullConnect_glu(C.byref(_fc_shape(rows, IC, OC, dtype, act, k)), a(X_address), a(W_address), a(Bias_address), a(Z_address),
                                                  a(Y_address), _stream(self._stream)))
 
     def fullConnect_delta(self, deltaX_address, deltaW_address, deltaB_address, deltaY_address, X_address, W_address, Z_address, deltaZ_address, rows, IC, OC,
@@ -306,7 +311,7 @@ class CudaFloat32EngineBase:
         """The gradients of fullConnect, or of fullConnect_glu (alpha_fullConnect_delta, alpha_fullConnect_glu_delta)."""
         a = self._addr_or_none
         fn = self._lib.alpha_fullConnect_glu_delta if glu else self._lib.alpha_fullConnect_delta
-        _l.check(fn(C.byref(_cached_fc_shape(rows, IC, OC, dtype, act, float(k))), a(deltaY_address), a(X_address), a(W_address), a(Z_address), a(deltaZ_address),
+        _l.check(fn(C.byref(_fc_shape(rows, IC, OC, dtype, act, k)), a(deltaY_address), a(X_address), a(W_address), a(Z_address), a(deltaZ_address),
                     a(deltaX_address), a(deltaW_address), a(deltaB_address), _stream(self._stream)))
 
     # ---- pooling, Java argument order (CudaFloat32EngineBase.java:2012-2215) ----
@@ -380,7 +385,6 @@ def _pad_both(t, n4, c4):
 
 _dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
 _FC_TYPES = {torch.float32: _l.ALPHA_F32, torch.bfloat16: _l.ALPHA_BF16, torch.float16: _l.ALPHA_F16}
-_cached_fc_shape = functools.lru_cache(maxsize=512)(_l.AlphaFcShape)
 
 
 def _fc_pack(dtype, *jobs):
