@@ -164,7 +164,8 @@ FcPlan pick_plan(const Product& q, int sms, double* time_of = nullptr)
     if ((forced == 1 || forced == 11) && sms >= 2) { look(true, forced == 1 ? 256 : 128, 1); best = FcPlan{true, forced == 1 ? 256 : 128, 1}; }
     else if (forced >= 1000) {
         const int bn = forced % 1000 / unit * unit;
-        for (int split = forced / 1000; split > 1 && bn >= unit && bn <= 256; split /= 2)
+        // (half as many CTAs, and so on, where a part would be empty or the clusters do not run at once)
+        for (int split = forced / 1000; split > 1 && bn >= unit && bn <= 256 && least == 1e300; split /= 2)
             if (split <= 8 && parts(split)) look(false, bn, split);
         if (least == 1e300 && bn >= unit && bn <= 256) look(false, bn, 1);
     } else {
