@@ -599,12 +599,14 @@ int launch_token(const AlphaFcShape* s, const void* X, const void* W, const void
     return launched("fc_token_kernel");
 }
 
-int forward(const char* what, const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, bool glu, cudaStream_t stream)
+int forward(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* residual, void* Z, void* Y, bool glu, cudaStream_t stream)
 {
     int rc = call_begin(stream);
     if (rc) return rc;
-    // (of the gated block from nine rows on only where W is small: 2 x 11008 x 4096 on 16 rows 39 us, by tiles 37)
-    const bool token = s->rows <= 8 || (s->rows <= kTokenRows && (!glu || (long long)s->OC * s->IC <= 8 << 20));
+    // Of the gated block from nine rows on only where W is small.  us of bf16, 9 to 16 rows, W from DRAM, this kernel / tiles: 2 x 1024 x 1024 5.4-5.9 / 6.6-7.0, 2 x 2752 x
+    // 1024 6.7 / 7.3, 2 x 2048 x 2048 9.6 / 9.5, 2 x 4096 x 2048 11.5 / 10.8, 2 x 5504 x 4096 31 / 20, 2 x 11008 x 4096 49 / 35; without gates 1024 x 1024 3.5 / 6.9, 4096 x
+    // 4096 10.9 / 12.9, 5504 x 4096 12 / 15.8, 11008 x 4096 23.0 / 21.4, 8192 x 8192 27 / 28.
+    const bool token = s->rows <= 8 || (s->rows <= kTokenRows && (!glu || (long long)s->OC * s->IC <= 4 << 20));
     if ((s->dtype == ALPHA_F32 ? s->rows <= kSmallRows : token) && (!option_fc_tile() || option_fc_tile() == 3)) {
         if (dry_run()) return ALPHA_OK;
         switch (s->dtype) {
@@ -712,7 +714,7 @@ int alpha_fullConnect(const AlphaFcShape* s, const void* X, const void* W, const
     if (reinterpret_cast<uintptr_t>(residual) & 15) return fail(ALPHA_E_ARG, "fullConnect: tensor pointers must be 16-byte aligned");
     rc = check_spans("fullConnect", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, static_cast<size_t>(s->OC) * s->IC * b}, {bias, pitch * b}, {residual == Y ? nullptr : residual, y}},
                      {{Y, y}, {Z, y}});
-    return rc ? rc : forward("fullConnect", s, X, W, bias, residual, Z, Y, false, static_cast<cudaStream_t>(stream));
+    return rc ? rc : forward(s, X, W, bias, residual, Z, Y, false, static_cast<cudaStream_t>(stream));
 }
 
 int alpha_fullConnect_glu(const AlphaFcShape* s, const void* X, const void* W, const void* bias, void* Z, void* Y, alpha_stream_t stream)
@@ -723,7 +725,7 @@ int alpha_fullConnect_glu(const AlphaFcShape* s, const void* X, const void* W, c
     if (!X || !W || !Y) return fail(ALPHA_E_ARG, "fullConnect_glu: null tensor pointer");
     const size_t b = type_bytes(s->dtype), pitch = fc_pitch(s->OC), y = s->rows * pitch * b;
     rc = check_spans("fullConnect_glu", {{X, static_cast<size_t>(s->rows) * s->IC * b}, {W, 2 * static_cast<size_t>(s->OC) * s->IC * b}, {bias, 2 * pitch * b}}, {{Y, y}, {Z, 2 * y}});
-    return rc ? rc : forward("fullConnect_glu", s, X, W, bias, nullptr, Z, Y, true, static_cast<cudaStream_t>(stream));
+    return rc ? rc : forward(s, X, W, bias, nullptr, Z, Y, true, static_cast<cudaStream_t>(stream));
 }
 
 int alpha_fullConnect_delta(const AlphaFcShape* s, const void* deltaY, const void* X, const void* W, const void* Z, void* deltaZ, void* deltaX, void* deltaW, void* deltaB,
