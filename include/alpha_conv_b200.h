@@ -462,16 +462,20 @@ int alpha_engine_batchMatMulT2(float* C, const float* A, const float* B, int Bat
  * bias, residual and Z may be NULL; Z keeps the sums for the backward pass.  residual may be Y itself; no other output may
  * overlap an input (ALPHA_E_ARG).
  * Sums, bias, activation and residual are fp32 and an output is rounded once; Y comes from the unrounded Z.  fp32 tensors are
- * multiplied at fp32 accuracy whatever the math mode says (as three bf16 planes; up to four rows by FMAs), 16-bit ones by
- * tcgen05.mma with fp32 accumulators.  fp32 tensors have fewer than 2^31 elements; rows, IC and OC are at most 2^31 - 1024.
+ * multiplied at fp32 accuracy whatever the math mode, the algorithm and option F32_PLANES say (as three bf16 planes on the tensor
+ * cores; up to four rows by FMAs), 16-bit ones by the tensor cores with fp32 accumulators (tcgen05.mma; up to 16 rows mma.sync).
+ * fp32 tensors have fewer than 2^31 elements; rows, IC and OC are at most 2^31 - 1024.
  *
  * The gradients, from deltaY and the Z that the forward call kept:
  *   deltaZ = deltaY * act'(Z)          (glu: [deltaY * U * act'(G) | deltaY * act(G)], Z = [G | U])
  *   deltaX = deltaZ W,  deltaW = deltaZ^T X,  deltaB = column sums of deltaZ;  the residual's gradient is deltaY itself
  * with deltaX, deltaW like X, W and deltaY, deltaB like Y, bias.
  * deltaX, deltaW and deltaB may each be NULL (not computed).  deltaZ is memory of the caller's, the size of Z, and may be Z
- * itself; it holds deltaZ rounded to the tensors' type afterwards.  ALPHA_ACT_NONE without gates needs neither Z nor deltaZ.
- * At 0 the slope of a LeakyReLU is k.  At -Inf a ReLU (k = 0) gives 0; silu, gelu and gelu_tanh, whose formulas are -Inf * 0 there, NaN.  Results do not depend on scheduling (fixed summation orders, no atomics). */
+ * itself; it holds deltaZ rounded to the tensors' type afterwards, and the products read it so: in fp16 an element of deltaZ from
+ * 65520 on is Inf and one up to 2^-25 is 0, whatever W and X would have made of it (deltaB sums what it was before).
+ * ALPHA_ACT_NONE without gates needs neither Z nor deltaZ.
+ * At 0 the slope of a LeakyReLU is k.  At -Inf a ReLU (k = 0) gives 0; silu, gelu and gelu_tanh, whose formulas are -Inf * 0 there,
+ * NaN.  Results do not depend on scheduling (fixed summation orders, no atomics). */
 #define ALPHA_F32 0
 #define ALPHA_BF16 1
 #define ALPHA_F16 2
@@ -499,10 +503,12 @@ int alpha_fullConnect_workspace_bytes(const AlphaFcShape* s, int glu, int op, si
 
 /* ---- all gradients of a step -----------------------------------------------------------------------------------
  *
- * norm = sqrt(sum of the squares of all elements of n tensors), summed in fp64 in a fixed order (neither overflow nor underflow
- * of a square; the same bits on every run), written to *norm as a float on the device; NaN or Inf elements give a NaN or Inf.
+ * norm = sqrt(sum of the squares of all elements of n tensors), written to *norm as a float on the device; NaN or Inf elements
+ * give a NaN or Inf.  The squares of 16 bytes (four or eight elements) are added in fp32, where they may leave its range in fp64,
+ * and everything else in fp64, in a fixed order: neither overflow nor underflow of a square, the same bits on every run.
  * alpha_clip_grad_norm also scales every element by c = min(1, max_norm / (norm + 1e-6)) (a NaN norm: by NaN):
- * out = c * grad, rounded to fp32 and from there to out's type; out may be grad itself.  A tensor given in place (out == grad) is not touched where c = 1.
+ * out = c * grad, rounded to fp32 and from there to out's type (16-bit outputs: with c rounded to fp32 too); out may be grad
+ * itself.  A tensor given in place (out == grad) is not touched where c = 1.
  * The tensors may be of different types and any size from 0 on, aligned to their elements; out may have another type (a
  * 16-bit gradient for a fp32 optimizer).  An output must not overlap any other tensor of the call (ALPHA_E_ARG).
  * n = 0 is a norm of 0.  Scratch: 48 bytes for each SM (or of the SM budget) and 128 tensors. */

@@ -289,3 +289,25 @@ def test_small_values_of_large_arguments(eng, tiled, dtype, rows, tile, act):
     tiny = (1 if act == "sigmoid" else z.abs()) * 2.0 ** -148 + (2.0 ** -134 if dtype == "bf16" else 2.0 ** -149)
     for got in (y, g, up):
         assert ((got - want).abs() <= (rel + half) * want.abs() * 1.01 + tiny).all(), (got, want)
+
+
+# ---- what the rounding of deltaZ means in fp16 ----
+
+@pytest.mark.parametrize("rows", (3, 200))
+@pytest.mark.parametrize("tile", (0, 1))
+def test_f16_deltaZ_has_the_range_of_f16(eng, tiled, rows, tile):
+    """deltaY U of 90000 and of 1e-8 in fp16: Inf and 0 in the gradients of X and W; the bias gradient sums what they were before they were rounded."""
+    tiled(tile)
+    IC, OC, t = 64, 40, torch.float16
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    X, W = torch.rand(rows, IC, device="cuda", generator=gen).add(1).to(t), torch.rand(2 * OC, IC, device="cuda", generator=gen).add(1).to(t)
+    Z, dY = torch.ones(rows, 2 * OC, device="cuda", dtype=t), torch.ones(rows, OC, device="cuda", dtype=t)
+    Z[1, OC + 3], dY[1, 3] = 300, 300                      # U and deltaY: deltaG is 90000
+    Z[:, OC + 5], dY[:, 5] = 1e-4, 1e-4                    # deltaG is 1e-8 in every row, deltaU 1e-4
+    dX, dW, dB = eng.fullConnect_glu_delta(dY, X, W, Z, act="none", bias=True)
+    assert torch.isinf(dX[1]).all() and torch.isfinite(dX[0]).all() and torch.isfinite(dX[2:]).all()
+    assert torch.isinf(dW[3]).all() and torch.isfinite(dW[4:]).all() and not dW[5].any()
+    assert torch.isinf(dB[3])
+    small = rows * float(Z[0, OC + 5]) * float(dY[0, 5])
+    # (a sum of `rows` terms, rounded to fp16, whose denormals are 2^-24 apart)
+    assert abs(float(dB[5]) - small) <= 2.0 ** -25 + rows * 2.0 ** -24 * small
