@@ -886,9 +886,10 @@ class Engine:
                 both, codes = src + to, codes if len(codes) > len(grads) else codes + codes
             norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
             _l.check(self.base._lib.alpha_clip_grad_norm(len(grads), self._grad_table(len(grads), both, codes), max_norm, norm.data_ptr(), _stream(self.base._stream)))
-            with torch.no_grad():
-                for o, t in back:
-                    o.copy_(t)
+            if back:
+                with torch.no_grad():
+                    for o, t in back:
+                        o.copy_(t)
         return norm
 
     # Batched products with the engine's memory rule (only the last dimension of a tensor is padded to a multiple
