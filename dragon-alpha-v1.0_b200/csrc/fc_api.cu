@@ -259,6 +259,8 @@ int launch_product(const Product& q, cudaStream_t stream)
 }
 
 // deltaX and deltaW: by a launch each, or together where the waves of both take less than those of either and a second launch's fill and drain.
+// (Chosen for 120 drawn bf16 shapes: 1.30 times as fast as apart in the geometric mean, 395 x 344 x 480 6.3 us instead of 11.9; slower for 15 of them, 5330 x 400 x 600 36 instead of 30.
+// Estimates within 3 % of one another are no reason for it.)
 int launch_products(const Product& x, const Product& w, cudaStream_t stream)
 {
     int sms = 0, *status = nullptr;

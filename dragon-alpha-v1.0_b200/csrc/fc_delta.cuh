@@ -24,6 +24,7 @@ struct FcDelta {
 // CTAs of an SM, each warp with one row in flight: rows ahead in registers, or the loop unrolled, cost more than they hid, as the grid then no longer
 // sweeps one band of rows.  us with deltaB, before with two or four rows ahead on three CTAs / now: 8192 x 11008 glu silu 182 / 151, 4096 x 16384 silu 109 / 84
 // and leakyRelu 87 / 66 (5.1 and 6.1 TB/s: an exponential and a quotient an element), fp32 4096 x 16384 165 / 125.
+// Layers of few columns leave lanes idle, and take what 128 columns take: 65536 rows fp32 silu with deltaB, 10 columns 17, 128 20 (101 MB), 512 66.
 template <bool GLU> __host__ __device__ constexpr int delta_ctas() { return GLU ? 3 : 6; }
 template <class T, bool GLU>
 __global__ void __launch_bounds__(256, delta_ctas<GLU>()) fc_delta_kernel(const __grid_constant__ FcDelta p)
