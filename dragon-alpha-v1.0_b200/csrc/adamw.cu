@@ -1,0 +1,455 @@
+// One AdamW step over many tensors.
+//
+//   g' = c g,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// One pass over every array, one launch for every 128 tensors: bound by HBM.  A CTA takes every gridDim.x-th chunk of 4096 elements of the launch; a thread has 4
+// elements of each of four rows of 1024, so that all its loads are in flight together and every load of a warp is consecutive.
+//
+// Moments of 8 bits: an e4m3 code for each element and a power of two for each block of 32, the smallest with which none is above 448, so that scaling is exact
+// in both directions.  A code is rounded up or down at random, with the probability that keeps its mean: v moves by one part in 1 / (1 - b2) a step, codes lie 6 to
+// 12 % apart, and one rounded to nearest would never fall again.  The random bits are a hash of seed, step, tensor and element: 16 for either
+// moment, nothing is kept, and the same call gives the same bits.  The update itself uses the moments before they are rounded.  A v that is not 0 gets a code that is not 0
+// (2^-9 of the scale at least): m / sqrt(0) is what would blow up a step.
+//
+// Moments are formed by separate fp32 products and sums, m = fl(fl(b1 m) + fl((1 - b1) g')): their codes do not depend on how a compiler fuses them.  Quotient
+// and root of the update are good to 2 units of 2^-23 of the update.
+#include "../../include/alpha_conv_b200.h"
+#include "dependent_launch.cuh"
+#include "fc_act.cuh"
+#include "host_common.h"
+
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <exception>
+#include <vector>
+
+namespace alpha {
+namespace {
+
+constexpr int kAdamTensors = 128, kAdamThreads = 256, kAdamRows = 4;
+constexpr int kAdamRow = 4 * kAdamThreads, kAdamChunk = kAdamRow * kAdamRows, kAdamBlock = 32;
+constexpr uint32_t kAdamSeed = 0x243F6A88u;
+enum : unsigned char { kNoType = 255 };
+
+struct AdamTensor {
+    void* p;
+    const void* g;
+    void *m, *v;
+    uint8_t *m_scale, *v_scale;          // 8 bits
+    void* out;
+    long long count;
+    double weight_decay;
+    uint32_t number;                     // of the tensor in the call
+    unsigned char type, grad_type, out_type, words;   // words: every array starts on a 16-byte boundary
+};
+struct AdamTable {
+    AdamTensor t[kAdamTensors];
+    unsigned first[kAdamTensors + 1];    // first chunk of each tensor; the last: chunks in all
+    int n;
+};
+struct AdamStep {
+    double lr, beta1, beta2, max_norm;
+    float b1, b1c, b2, b2c, eps;         // beta and 1 - beta
+    float size, root;                    // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), where lr and t are the host's
+    uint32_t step, seed;                 // (the low 32 bits of the step)
+    const float *lr_at, *norm;
+    const long long* step_at;
+};
+
+__host__ __device__ __forceinline__ uint32_t mix32(uint32_t x)
+{
+    x = (x ^ (x >> 16)) * 0x9E3779B9u;   // the golden ratio's and e's binary digits
+    x = (x ^ (x >> 15)) * 0xB7E15163u;
+    return x ^ (x >> 16);
+}
+
+// Four elements at a time, as floats.
+struct Four { float f[4]; };
+template <class T> struct FourOf;
+template <> struct FourOf<float> {
+    using Raw = float4;
+    static __device__ Four get(const Raw& r) { return Four{{r.x, r.y, r.z, r.w}}; }
+    static __device__ Raw put(const Four& v) { return make_float4(v.f[0], v.f[1], v.f[2], v.f[3]); }
+};
+template <class T> struct FourOf16 {
+    using Raw = uint2;
+    static __device__ Four get(const Raw& r)
+    {
+        Four v;
+        unpack16<T>(r.x, v.f[0], v.f[1]);
+        unpack16<T>(r.y, v.f[2], v.f[3]);
+        return v;
+    }
+    static __device__ Raw put(const Four& v) { return make_uint2(pack16<T>(v.f[0], v.f[1]), pack16<T>(v.f[2], v.f[3])); }
+};
+template <> struct FourOf<__nv_bfloat16> : FourOf16<__nv_bfloat16> {};
+template <> struct FourOf<__half> : FourOf16<__half> {};
+
+__device__ __forceinline__ float2 e4m3_pair(uint32_t codes)
+{
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ Four e4m3_get(uint32_t codes)
+{
+    const float2 a = e4m3_pair(codes & 0xffffu), b = e4m3_pair(codes >> 16);
+    return Four{{a.x, a.y, b.x, b.y}};
+}
+__device__ __forceinline__ uint32_t e4m3_put(const Four& v)
+{
+    return __nv_cvt_float2_to_fp8x2(make_float2(v.f[0], v.f[1]), __NV_SATFINITE, __NV_E4M3)
+         | static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v.f[2], v.f[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
+}
+// The value of an exponent byte (0: 2^-127, 255: NaN), and the byte of a block whose largest magnitude is `most`.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte == 0 ? 0x400000u : byte == 255 ? 0x7fc00000u : byte << 23); }
+__device__ __forceinline__ uint32_t scale_for(float most)
+{
+    const uint32_t bits = __float_as_uint(most);
+    const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);       // 448 = 1.75 * 2^8
+    return static_cast<uint32_t>(e < 1 ? 1 : e > 254 ? 254 : e);
+}
+// y, at most 448, to one of the codes beside it; `random` of 16 bits.  Below 2^-6 codes are 2^-9 apart, as they are from there to 2^-5.
+template <bool FLOOR> __device__ __forceinline__ float round_e4m3(float y, uint32_t random)
+{
+    float a = fabsf(y);
+    const float shift = a < 0x1p-6f ? 0x1p-6f : 0.f;
+    a = __uint_as_float((__float_as_uint(__fadd_rn(a, shift)) + (random << 4)) & ~0xfffffu) - shift;
+    if (FLOOR && y > 0.f) a = fmaxf(a, 0x1p-9f);
+    return copysignf(a, y);
+}
+
+// What a launch's elements have in common.
+struct AdamUse { float b1, b1c, b2, b2c, eps, size, root, c; };
+
+struct AdamNew { float p, m, v; };
+__device__ __forceinline__ AdamNew adam_element(const AdamUse& u, float keep, float p, float g, float m, float v)
+{
+    g = __fmul_rn(g, u.c);
+    m = __fadd_rn(__fmul_rn(m, u.b1), __fmul_rn(g, u.b1c));
+    v = __fadd_rn(__fmul_rn(v, u.b2), __fmul_rn(__fmul_rn(g, g), u.b2c));
+    const float by = fmaf(sqrtf(v), u.root, u.eps);
+    return AdamNew{fmaf(p, keep, -__fdividef(m, by) * u.size), m, v};
+}
+
+template <class F> __device__ __forceinline__ void with_type(int type, F&& f)
+{
+    if (type == ALPHA_F32) f(float{});
+    else if (type == ALPHA_BF16) f(__nv_bfloat16{});
+    else f(__half{});
+}
+__device__ __forceinline__ float get_one(const void* p, long long i, int type)
+{
+    return type == ALPHA_F32 ? static_cast<const float*>(p)[i] : type == ALPHA_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void put_one(void* p, long long i, int type, float x)
+{
+    if (type == ALPHA_F32) static_cast<float*>(p)[i] = x;
+    else if (type == ALPHA_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+    else static_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
+// The rows of an array that a thread has of a chunk.
+template <class Raw> __device__ __forceinline__ void get_rows(Raw (&r)[kAdamRows], const void* p, long long first)
+{
+    const Raw* at = reinterpret_cast<const Raw*>(p) + first / 4;
+#pragma unroll
+    for (int i = 0; i < kAdamRows; ++i) r[i] = __ldcs(at + i * kAdamThreads);
+}
+template <class T> __device__ __forceinline__ void get_typed(Four (&f)[kAdamRows], const void* p, long long first)
+{
+    typename FourOf<T>::Raw r[kAdamRows];
+    get_rows(r, p, first);
+#pragma unroll
+    for (int i = 0; i < kAdamRows; ++i) f[i] = FourOf<T>::get(r[i]);
+}
+__device__ __forceinline__ void put_rows(void* p, long long first, int type, const Four (&f)[kAdamRows])
+{
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        typename FourOf<T>::Raw* at = reinterpret_cast<typename FourOf<T>::Raw*>(p) + first / 4;
+#pragma unroll
+        for (int i = 0; i < kAdamRows; ++i) __stcs(at + i * kAdamThreads, FourOf<T>::put(f[i]));
+    });
+}
+
+// (a warp's 32 lanes, or the eight that hold a block)
+template <int LANES> __device__ __forceinline__ float most_of(float x)
+{
+#pragma unroll
+    for (int d = LANES / 2; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+}
+
+template <bool EIGHT>
+__device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamUse& u, float keep, uint32_t key, long long begin)
+{
+    const long long first = begin + 4 * threadIdx.x;
+    Four p[kAdamRows], g[kAdamRows], m[kAdamRows], v[kAdamRows];
+    if constexpr (EIGHT) {
+        uint32_t mc[kAdamRows], vc[kAdamRows];
+        uint8_t ms[kAdamRows], vs[kAdamRows];
+        get_rows(mc, t.m, first);
+        get_rows(vc, t.v, first);
+#pragma unroll
+        for (int i = 0; i < kAdamRows; ++i) {
+            ms[i] = t.m_scale[(first + i * kAdamRow) / kAdamBlock];
+            vs[i] = t.v_scale[(first + i * kAdamRow) / kAdamBlock];
+        }
+        with_type(t.type, [&](auto x) { get_typed<decltype(x)>(p, t.p, first); });
+        with_type(t.grad_type, [&](auto x) { get_typed<decltype(x)>(g, t.g, first); });
+#pragma unroll
+        for (int i = 0; i < kAdamRows; ++i) {
+            m[i] = e4m3_get(mc[i]);
+            v[i] = e4m3_get(vc[i]);
+            const float a = scale_of(ms[i]), b = scale_of(vs[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { m[i].f[j] *= a; v[i].f[j] *= b; }
+        }
+    } else {
+        get_typed<float>(m, t.m, first);
+        get_typed<float>(v, t.v, first);
+        with_type(t.type, [&](auto x) { get_typed<decltype(x)>(p, t.p, first); });
+        with_type(t.grad_type, [&](auto x) { get_typed<decltype(x)>(g, t.g, first); });
+    }
+#pragma unroll
+    for (int i = 0; i < kAdamRows; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const AdamNew e = adam_element(u, keep, p[i].f[j], g[i].f[j], m[i].f[j], v[i].f[j]);
+            p[i].f[j] = e.p; m[i].f[j] = e.m; v[i].f[j] = e.v;
+        }
+    put_rows(t.p, first, t.type, p);
+    if (t.out_type != kNoType) put_rows(t.out, first, t.out_type, p);
+    if constexpr (!EIGHT) {
+        put_rows(t.m, first, ALPHA_F32, m);
+        put_rows(t.v, first, ALPHA_F32, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kAdamRows; ++i) {
+        const long long at = first + i * kAdamRow;
+        float mm = 0.f, vm = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { mm = fmaxf(mm, fabsf(m[i].f[j])); vm = fmaxf(vm, v[i].f[j]); }
+        const uint32_t a = scale_for(most_of<8>(mm)), b = scale_for(most_of<8>(vm));
+        const float ai = __uint_as_float((254u - a) << 23), bi = __uint_as_float((254u - b) << 23);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t random = mix32((static_cast<uint32_t>(at) + j) ^ key);
+            m[i].f[j] = round_e4m3<false>(m[i].f[j] * ai, random & 0xffffu);
+            v[i].f[j] = round_e4m3<true>(v[i].f[j] * bi, random >> 16);
+        }
+        __stcs(reinterpret_cast<uint32_t*>(t.m) + at / 4, e4m3_put(m[i]));
+        __stcs(reinterpret_cast<uint32_t*>(t.v) + at / 4, e4m3_put(v[i]));
+        if ((threadIdx.x & 7) == 0) {
+            t.m_scale[at / kAdamBlock] = static_cast<uint8_t>(a);
+            t.v_scale[at / kAdamBlock] = static_cast<uint8_t>(b);
+        }
+    }
+}
+
+// Element by element, a block of 32 to a warp: the end of a tensor, and arrays that do not start on 16-byte boundaries.
+template <bool EIGHT>
+__device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u, float keep, uint32_t key, long long begin)
+{
+    const long long end = begin + kAdamChunk < t.count ? begin + kAdamChunk : t.count;
+    for (long long at = begin + (threadIdx.x & ~31u); at < end; at += kAdamThreads) {
+        const long long e = at + (threadIdx.x & 31);
+        const bool in = e < end;
+        AdamNew x{0.f, 0.f, 0.f};
+        if (in) {
+            float m, v;
+            if constexpr (EIGHT) {
+                m = e4m3_pair(static_cast<const uint8_t*>(t.m)[e]).x * scale_of(t.m_scale[e / kAdamBlock]);
+                v = e4m3_pair(static_cast<const uint8_t*>(t.v)[e]).x * scale_of(t.v_scale[e / kAdamBlock]);
+            } else {
+                m = static_cast<const float*>(t.m)[e];
+                v = static_cast<const float*>(t.v)[e];
+            }
+            x = adam_element(u, keep, get_one(t.p, e, t.type), get_one(t.g, e, t.grad_type), m, v);
+            put_one(t.p, e, t.type, x.p);
+            if (t.out_type != kNoType) put_one(t.out, e, t.out_type, x.p);
+        }
+        if constexpr (!EIGHT) {
+            if (in) {
+                static_cast<float*>(t.m)[e] = x.m;
+                static_cast<float*>(t.v)[e] = x.v;
+            }
+            continue;
+        }
+        const uint32_t a = scale_for(most_of<32>(fabsf(x.m))), b = scale_for(most_of<32>(x.v));     // (and a barrier of the warp: the old scales have been read)
+        const uint32_t random = mix32(static_cast<uint32_t>(e) ^ key);
+        const float m = round_e4m3<false>(x.m * __uint_as_float((254u - a) << 23), random & 0xffffu), v = round_e4m3<true>(x.v * __uint_as_float((254u - b) << 23), random >> 16);
+        if (in) {
+            const uint32_t codes = e4m3_put(Four{{m, v, 0.f, 0.f}});
+            static_cast<uint8_t*>(t.m)[e] = static_cast<uint8_t>(codes);
+            static_cast<uint8_t*>(t.v)[e] = static_cast<uint8_t>(codes >> 8);
+            if ((threadIdx.x & 31) == 0) {
+                t.m_scale[e / kAdamBlock] = static_cast<uint8_t>(a);
+                t.v_scale[e / kAdamBlock] = static_cast<uint8_t>(b);
+            }
+        }
+    }
+}
+
+template <bool EIGHT>
+__global__ void __launch_bounds__(kAdamThreads, EIGHT ? 4 : 3) adamw_kernel(const __grid_constant__ AdamTable table, const __grid_constant__ AdamStep s)
+{
+    __shared__ float shared[2];
+    grid_dependency_wait();
+    grid_dependency_trigger();
+    AdamUse u{s.b1, s.b1c, s.b2, s.b2c, s.eps, s.size, s.root, 1.f};
+    if (s.norm) {
+        const float norm = *s.norm;
+        if (!(norm < __int_as_float(0x7f800000))) return;            // NaN or Inf: the step is left out
+        const double ratio = s.max_norm / (static_cast<double>(norm) + 1e-6);
+        if (ratio < 1.0) u.c = static_cast<float>(ratio);
+    }
+    const double lr = s.lr_at ? static_cast<double>(*s.lr_at) : s.lr;
+    const long long step = s.step_at ? *s.step_at : static_cast<long long>(s.step);
+    if (s.lr_at || s.step_at) {
+        if (threadIdx.x == 0) {
+            shared[0] = static_cast<float>(lr / (1.0 - pow(s.beta1, static_cast<double>(step))));
+            shared[1] = static_cast<float>(1.0 / sqrt(1.0 - pow(s.beta2, static_cast<double>(step))));
+        }
+        __syncthreads();
+        u.size = shared[0];
+        u.root = shared[1];
+    }
+    const uint32_t call_key = EIGHT ? mix32(kAdamSeed ^ mix32(s.seed) ^ static_cast<uint32_t>(step)) : 0u;
+    for (unsigned chunk = blockIdx.x; chunk < table.first[table.n]; chunk += gridDim.x) {
+        int lo = 0, hi = table.n;                // first[lo] <= chunk < first[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (table.first[mid] <= chunk) lo = mid;
+            else hi = mid;
+        }
+        const AdamTensor& t = table.t[lo];
+        const long long begin = static_cast<long long>(chunk - table.first[lo]) * kAdamChunk;
+        const float keep = static_cast<float>(1.0 - lr * t.weight_decay);
+        uint32_t key = EIGHT ? mix32(call_key ^ t.number) : 0u;
+        if (EIGHT && begin >> 32) key = mix32(key ^ static_cast<uint32_t>(begin >> 32));
+        if (t.words && begin + kAdamChunk <= t.count) whole_chunk<EIGHT>(t, u, keep, key, begin);
+        else ragged_chunk<EIGHT>(t, u, keep, key, begin);
+    }
+}
+
+int launched(const char* what)
+{
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? ALPHA_OK : fail(ALPHA_E_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+}
+int type_size(int dtype) { return dtype == ALPHA_F32 ? 4 : 2; }
+
+int check_adamw(int n, const AlphaAdamW* list, const AlphaAdamWStep* s)
+{
+    if (!s || n < 0 || (n && !list)) return fail(ALPHA_E_ARG, "adamW: null argument");
+    if (!(s->beta1 >= 0.0 && s->beta1 < 1.0 && s->beta2 >= 0.0 && s->beta2 < 1.0)) return fail(ALPHA_E_ARG, "adamW: beta1=%g beta2=%g must be in [0, 1)", s->beta1, s->beta2);
+    if (!(s->eps >= 0.0) || !(s->eps <= 3e38)) return fail(ALPHA_E_ARG, "adamW: eps=%g must be finite and not negative", s->eps);
+    if (!s->step_device && s->step < 1) return fail(ALPHA_E_ARG, "adamW: step %lld, the first is 1", static_cast<long long>(s->step));
+    if (!s->lr_device && !(s->lr >= 0.0 && s->lr <= 3e38)) return fail(ALPHA_E_ARG, "adamW: lr=%g must be finite and not negative", s->lr);
+    if (s->norm && !(s->max_norm >= 0.0)) return fail(ALPHA_E_ARG, "adamW: max_norm must not be negative or NaN");
+    if ((reinterpret_cast<uintptr_t>(s->norm) & 3) || (reinterpret_cast<uintptr_t>(s->lr_device) & 3) || (reinterpret_cast<uintptr_t>(s->step_device) & 7))
+        return fail(ALPHA_E_ARG, "adamW: norm, lr and step on the device must be aligned to their types");
+    struct Range { uintptr_t from, to; bool write; };
+    std::vector<Range> ranges;
+    try {
+        ranges.reserve(7 * static_cast<size_t>(n) + 3);
+    } catch (const std::exception&) {
+        return fail(ALPHA_E_NOSCRATCH, "adamW: no host memory to check %d tensors", n);
+    }
+    auto add = [&](const void* p, size_t bytes, bool write) { if (p) ranges.push_back(Range{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, write}); };
+    add(s->norm, 4, false);
+    add(s->lr_device, 4, false);
+    add(s->step_device, 8, false);
+    auto known = [](int t) { return t == ALPHA_F32 || t == ALPHA_BF16 || t == ALPHA_F16; };
+    for (int i = 0; i < n; ++i) {
+        const AlphaAdamW& a = list[i];
+        if (!known(a.dtype) || !known(a.grad_dtype) || (a.out && !known(a.out_dtype))) return fail(ALPHA_E_ARG, "adamW: unknown element type of tensor %d", i);
+        if (a.moment_bits != list[0].moment_bits || (a.moment_bits != 32 && a.moment_bits != 8)) return fail(ALPHA_E_ARG, "adamW: moments of all tensors have 32 bits, or all 8 (tensor %d: %d)", i, a.moment_bits);
+        if (a.count < 0 || a.count >= 1LL << 42) return fail(ALPHA_E_ARG, "adamW: tensor %d has %lld elements", i, static_cast<long long>(a.count));
+        if (!(a.weight_decay >= 0.0 && a.weight_decay <= 3e38)) return fail(ALPHA_E_ARG, "adamW: weight decay of tensor %d must be finite and not negative", i);
+        if (a.count == 0) continue;
+        const bool eight = a.moment_bits == 8;
+        if (!a.param || !a.grad || !a.m || !a.v || (eight && (!a.m_scale || !a.v_scale))) return fail(ALPHA_E_ARG, "adamW: null pointer of tensor %d", i);
+        const size_t ps = type_size(a.dtype), gs = type_size(a.grad_dtype), os = type_size(a.out_dtype), ms = eight ? 1 : 4, scales = (a.count + kAdamBlock - 1) / kAdamBlock;
+        auto off = [](const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
+        if (off(a.param, ps) || off(a.grad, gs) || off(a.m, ms) || off(a.v, ms) || (a.out && off(a.out, os))) return fail(ALPHA_E_ARG, "adamW: tensor %d is not aligned to its elements", i);
+        add(a.param, a.count * ps, true);
+        add(a.grad, a.count * gs, false);
+        add(a.m, a.count * ms, true);
+        add(a.v, a.count * ms, true);
+        if (eight) { add(a.m_scale, scales, true); add(a.v_scale, scales, true); }
+        add(a.out, a.count * os, true);
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    uintptr_t read = 0, written = 0;          // ends of the ranges so far
+    for (const Range& r : ranges) {
+        if (r.from < written || (r.write && r.from < read)) return fail(ALPHA_E_ARG, "adamW: what a step writes overlaps another tensor");
+        (r.write ? written : read) = std::max(r.write ? written : read, r.to);
+    }
+    return ALPHA_OK;
+}
+
+int run_adamw(int n, const AlphaAdamW* list, const AlphaAdamWStep* s, cudaStream_t stream)
+{
+    int rc = check_adamw(n, list, s);
+    if (!rc) rc = call_begin(stream);
+    int sms = 0;
+    if (!rc) rc = device_sms(&sms);
+    if (rc || dry_run()) return rc;
+    AdamStep a{};
+    a.lr = s->lr; a.beta1 = s->beta1; a.beta2 = s->beta2; a.max_norm = s->max_norm;
+    a.b1 = static_cast<float>(s->beta1); a.b1c = static_cast<float>(1.0 - s->beta1);
+    a.b2 = static_cast<float>(s->beta2); a.b2c = static_cast<float>(1.0 - s->beta2);
+    a.eps = static_cast<float>(s->eps);
+    a.size = static_cast<float>(s->lr / (1.0 - pow(s->beta1, static_cast<double>(s->step))));
+    a.root = static_cast<float>(1.0 / sqrt(1.0 - pow(s->beta2, static_cast<double>(s->step))));
+    a.step = static_cast<uint32_t>(s->step); a.seed = s->seed;
+    a.lr_at = s->lr_device; a.norm = s->norm; a.step_at = reinterpret_cast<const long long*>(s->step_device);
+    AdamTable t;
+    t.n = 0;
+    long long chunks = 0;
+    const bool eight = n && list[0].moment_bits == 8;
+    const long long most = sms * (eight ? 4LL : 3LL);
+    for (int i = 0; i <= n; ++i) {
+        long long more = 0;
+        if (i < n) {
+            if (list[i].count == 0) continue;
+            more = (list[i].count + kAdamChunk - 1) / kAdamChunk;
+        }
+        if (t.n && (i == n || t.n == kAdamTensors || chunks + more > 2147483647LL)) {
+            t.first[t.n] = static_cast<unsigned>(chunks);
+            const unsigned grid = static_cast<unsigned>(chunks < most ? chunks : most);
+            if (eight) launch_after(adamw_kernel<true>, grid, kAdamThreads, 0, stream, t, a);
+            else launch_after(adamw_kernel<false>, grid, kAdamThreads, 0, stream, t, a);
+            note_launch("adamw");
+            rc = launched("adamw_kernel");
+            if (rc) return rc;
+            t.n = 0;
+            chunks = 0;
+        }
+        if (i == n) break;
+        const AlphaAdamW& l = list[i];
+        AdamTensor& d = t.t[t.n];
+        d = AdamTensor{l.param, l.grad, l.m, l.v, static_cast<uint8_t*>(l.m_scale), static_cast<uint8_t*>(l.v_scale), l.out, l.count, l.weight_decay, static_cast<uint32_t>(i),
+                       static_cast<unsigned char>(l.dtype), static_cast<unsigned char>(l.grad_dtype), static_cast<unsigned char>(l.out ? l.out_dtype : kNoType), 0};
+        uintptr_t low = 0;
+        for (const void* p : {static_cast<const void*>(l.param), l.grad, static_cast<const void*>(l.m), static_cast<const void*>(l.v), static_cast<const void*>(l.out)}) low |= reinterpret_cast<uintptr_t>(p);
+        d.words = low % 16 == 0;
+        t.first[t.n++] = static_cast<unsigned>(chunks);
+        chunks += more;
+    }
+    return ALPHA_OK;
+}
+
+}  // namespace
+}  // namespace alpha
+
+extern "C" int alpha_adamW(int n, const AlphaAdamW* tensors, const AlphaAdamWStep* step, alpha_stream_t stream)
+{
+    alpha::OpRange range("alpha_adamW");
+    return alpha::run_adamw(n, tensors, step, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,193 @@
+// Group normalisation with an activation, and its gradients: which kernels a call runs on.
+#include "group_norm.cuh"
+#include "host_checks.h"
+
+#include <algorithm>
+#include <numeric>
+
+using namespace alpha;
+
+namespace {
+
+int check_norm(const char* what, const AlphaNormShape* s)
+{
+    if (!s) return fail(ALPHA_E_ARG, "%s: null shape", what);
+    if (s->N <= 0 || s->positions <= 0 || s->C <= 0 || s->groups <= 0) return fail(ALPHA_E_ARG, "%s: non-positive dimension (N=%d positions=%d C=%d groups=%d)", what, s->N, s->positions, s->C, s->groups);
+    if (s->C % s->groups) return fail(ALPHA_E_ARG, "%s: %d channels are not %d groups of one size", what, s->C, s->groups);
+    // (what a thread or a CTA comes to past a tensor's end is an int too)
+    const int most = 2147483647 - (1 << 20);
+    if (s->positions > most || s->C > most || static_cast<long long>(s->N) * s->C > most) return fail(ALPHA_E_ARG, "%s: more than %d positions or channels of all samples", what, most);
+    if (!known_type(s->dtype)) return fail(ALPHA_E_ARG, "%s: unknown element type %d", what, s->dtype);
+    if (s->affine_dtype != s->dtype && s->affine_dtype != ALPHA_F32) return fail(ALPHA_E_ARG, "%s: gamma and beta are of the tensors' type or fp32, not type %d", what, s->affine_dtype);
+    if (s->act < ALPHA_ACT_NONE || s->act > ALPHA_ACT_GELU_TANH) return fail(ALPHA_E_ARG, "%s: unknown activation %d", what, s->act);
+    if (s->act == ALPHA_ACT_LEAKY_RELU && !(s->k == s->k)) return fail(ALPHA_E_ARG, "%s: slope is NaN", what);
+    if (!(s->eps >= 0.f && s->eps <= 3e38f)) return fail(ALPHA_E_ARG, "%s: eps=%g must be finite and not negative", what, s->eps);
+    return ALPHA_OK;
+}
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+Norm norm_of(const AlphaNormShape* s)
+{
+    Norm p{};
+    p.N = s->N; p.R = s->positions; p.C = s->C; p.G = s->groups; p.D = s->C / s->groups;
+    p.affine_f32 = s->affine_dtype == ALPHA_F32;
+    p.eps = s->eps; p.act = s->act; p.k = s->k;
+    return p;
+}
+
+// The slab and the cluster of least estimated time; false: no slab fits.
+bool plan_resident(Norm& p, int V, bool back, int sms, size_t* smem)
+{
+    const long long unit = static_cast<long long>(p.D) * V / std::gcd(p.D, V);
+    if (unit / V > kNormThreads || p.C % V) return false;
+    const int unit_words = static_cast<int>(unit / V), units = static_cast<int>(p.C / unit);
+    double least = 1e300;
+    for (int each = 1; each <= kNormThreads / unit_words && each <= units; ++each) {
+        if (units % each) continue;
+        const int words = unit_words * each, slabs = units / each;
+        for (int cl = 1; cl <= 8; cl *= 2) {
+            const int part = (p.R + cl - 1) / cl;
+            const long long ctas = static_cast<long long>(p.N) * slabs * cl;
+            if (static_cast<long long>(cl - 1) * part >= p.R || part > (1 << 20) || ctas > 2147483647LL) continue;
+            const size_t bytes = norm_smem(back, V, part, words, words * V / p.D);
+            if (bytes > 224 * 1024) continue;
+            const double at_once = std::min(2.0, static_cast<double>(static_cast<int>(227 * 1024 / (bytes + 1024)))), waves = std::max(1.0, ctas / (sms * at_once));
+            // us: what a CTA waits for besides its bytes, and its share of the bytes an SM takes in and gives out
+            const double narrow = words >= 4 ? 1.0 : words == 2 ? 1.15 : words == 1 ? 1.6 : 1.1;
+            const double time = waves * (3.0 + 0.4 * cl + at_once * part * words * 16.0 * (back ? 3 : 2) / 45e3 * narrow);
+            if (time < least) {
+                least = time;
+                p.words = words; p.slabs = slabs; p.cluster = cl; p.part = part; p.rows = kNormThreads / p.words;
+                *smem = bytes;
+            }
+        }
+    }
+    return least < 1e300;
+}
+// Column blocks of up to 64 words, and runs of positions that fill the SMs.
+void plan_streamed(Norm& p, int V, int sms)
+{
+    const int words = p.C / V;
+    p.blocks = (words + 63) / 64;
+    p.words = (words + p.blocks - 1) / p.blocks;
+    p.blocks = (words + p.words - 1) / p.words;
+    p.rows = kNormThreads / p.words;
+    const long long others = static_cast<long long>(p.N) * p.blocks, least = 8LL * p.rows;        // positions of a run
+    long long runs = std::max(1LL, 16LL * sms / others);
+    runs = std::min(runs, std::max(1LL, p.R / least));
+    p.part = static_cast<int>((p.R + runs - 1) / runs);
+    p.runs = (p.R + p.part - 1) / p.part;
+}
+
+template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgamma, void* dbeta, cudaStream_t stream)
+{
+    constexpr int V = Word16<T>::N;
+    int sms = 0;
+    int rc = call_begin(stream);
+    if (!rc) rc = device_sms(&sms);
+    if (rc) return rc;
+    const bool words = p.C % V == 0 && aligned(p.X, 16) && aligned(p.out, 16) && aligned(p.dY, 16);
+    size_t smem = 0;
+    const bool resident = words && plan_resident(p, V, BACK, sms, &smem);
+    if (!resident) plan_streamed(p, words ? V : 1, sms);
+    void* ws = nullptr;
+    auto scratch = [&](size_t bytes) { return rc = rc ? rc : call_scratch(stream, bytes, &ws); };
+    if (BACK && !scratch(static_cast<size_t>(p.N) * p.C * sizeof(float2))) p.sums = static_cast<float2*>(ws);
+    if (!resident && !scratch(static_cast<size_t>(p.N) * p.G * sizeof(float2))) p.group = static_cast<float2*>(ws);
+    if (!resident && !scratch(static_cast<size_t>(p.N) * p.runs * p.C * sizeof(float2))) p.partial = static_cast<float2*>(ws);
+    if (rc || dry_run()) return rc;
+    if (resident) {
+        allow_smem<norm_resident_kernel<T, BACK>>();
+        launch_after_clusters(norm_resident_kernel<T, BACK>, dim3(static_cast<unsigned>(p.N) * p.slabs * p.cluster), kNormThreads, p.cluster > 1 ? p.cluster : 0, smem, stream, p);
+        note_launch("norm");
+        note_plan("norm resident words=%d cluster=%d part=%d", p.words, p.cluster, p.part);
+        rc = launched("norm_resident_kernel");
+    } else {
+        const long long ctas = static_cast<long long>(p.N) * p.runs * p.blocks;
+        if (ctas > 2147483647LL) return fail(ALPHA_E_ARG, "%s: more CTAs than a launch takes", what);
+        const unsigned grid = static_cast<unsigned>(ctas);
+        if (words) launch_after(norm_sums_kernel<T, V, BACK>, grid, kNormThreads, 0, stream, p);
+        else launch_after(norm_sums_kernel<T, 1, BACK>, grid, kNormThreads, 0, stream, p);
+        note_launch("norm");
+        rc = launched("norm_sums_kernel");
+        if (rc) return rc;
+        launch_after(norm_join_kernel<T, BACK>, static_cast<unsigned>(p.N * p.G), kNormThreads, 0, stream, p);
+        note_launch("norm");
+        rc = launched("norm_join_kernel");
+        if (rc) return rc;
+        if (words) launch_after(norm_apply_kernel<T, V, BACK>, grid, kNormThreads, 0, stream, p);
+        else launch_after(norm_apply_kernel<T, 1, BACK>, grid, kNormThreads, 0, stream, p);
+        note_launch("norm");
+        note_plan("norm streamed words=%d runs=%d part=%d", p.words, p.runs, p.part);
+        rc = launched("norm_apply_kernel");
+    }
+    if (rc || !dgamma) return rc;
+    launch_after(norm_affine_kernel<T>, (p.C + 31) / 32, 256, 0, stream, p.sums, p.N, p.C, dgamma, dbeta, p.affine_f32);
+    note_launch("norm");
+    return launched("norm_affine_kernel");
+}
+
+}  // namespace
+
+extern "C" {
+
+int alpha_groupNorm(const AlphaNormShape* s, const void* X, const void* gamma, const void* beta, float* mean, float* rstd, void* Y, alpha_stream_t stream)
+{
+    OpRange range("alpha_groupNorm");
+    int rc = check_norm("groupNorm", s);
+    if (rc) return rc;
+    if (!X || !Y || !gamma != !beta || !mean != !rstd) return fail(ALPHA_E_ARG, "groupNorm: null tensor pointer");
+    const size_t b = type_bytes(s->dtype), a = type_bytes(s->affine_dtype), n = static_cast<size_t>(s->N) * s->positions * s->C * b, g = static_cast<size_t>(s->N) * s->groups * 4;
+    if (!aligned(X, b) || !aligned(Y, b) || !aligned(gamma, a) || !aligned(beta, a) || !aligned(mean, 4) || !aligned(rstd, 4)) return fail(ALPHA_E_ARG, "groupNorm: tensors must be aligned to their elements");
+    rc = check_overlaps("groupNorm", {{X, n}, {gamma, s->C * a}, {beta, s->C * a}}, {{Y, n}, {mean, g}, {rstd, g}});
+    if (rc) return rc;
+    Norm p = norm_of(s);
+    p.X = X; p.out = Y; p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (s->dtype == ALPHA_F32) return run_norm<float, false>(p, "groupNorm", nullptr, nullptr, st);
+    if (s->dtype == ALPHA_BF16) return run_norm<__nv_bfloat16, false>(p, "groupNorm", nullptr, nullptr, st);
+    return run_norm<__half, false>(p, "groupNorm", nullptr, nullptr, st);
+}
+
+int alpha_groupNorm_delta(const AlphaNormShape* s, const void* deltaY, const void* X, const float* mean, const float* rstd, const void* gamma, const void* beta, void* deltaX,
+                          void* deltaGamma, void* deltaBeta, alpha_stream_t stream)
+{
+    OpRange range("alpha_groupNorm_delta");
+    int rc = check_norm("groupNorm_delta", s);
+    if (rc) return rc;
+    if (!deltaY || !X || !mean || !rstd || !deltaX || !gamma != !beta || !deltaGamma != !deltaBeta) return fail(ALPHA_E_ARG, "groupNorm_delta: null tensor pointer");
+    const size_t b = type_bytes(s->dtype), a = type_bytes(s->affine_dtype), n = static_cast<size_t>(s->N) * s->positions * s->C * b, g = static_cast<size_t>(s->N) * s->groups * 4, c = s->C * a;
+    if (!aligned(X, b) || !aligned(deltaY, b) || !aligned(deltaX, b) || !aligned(gamma, a) || !aligned(beta, a) || !aligned(deltaGamma, a) || !aligned(deltaBeta, a) || !aligned(mean, 4) || !aligned(rstd, 4))
+        return fail(ALPHA_E_ARG, "groupNorm_delta: tensors must be aligned to their elements");
+    rc = check_overlaps("groupNorm_delta", {{deltaY, n}, {X, n}, {mean, g}, {rstd, g}, {gamma, c}, {beta, c}}, {{deltaX, n}, {deltaGamma, c}, {deltaBeta, c}});
+    if (rc) return rc;
+    Norm p = norm_of(s);
+    p.X = X; p.dY = deltaY; p.out = deltaX; p.gamma = gamma; p.beta = beta; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (s->dtype == ALPHA_F32) return run_norm<float, true>(p, "groupNorm_delta", deltaGamma, deltaBeta, st);
+    if (s->dtype == ALPHA_BF16) return run_norm<__nv_bfloat16, true>(p, "groupNorm_delta", deltaGamma, deltaBeta, st);
+    return run_norm<__half, true>(p, "groupNorm_delta", deltaGamma, deltaBeta, st);
+}
+
+int alpha_groupNorm_workspace_bytes(const AlphaNormShape* s, int op, size_t* bytes)
+{
+    if (!s || !bytes) return fail(ALPHA_E_ARG, "groupNorm_workspace_bytes: null argument");
+    if (op != ALPHA_OP_FORWARD && op != ALPHA_OP_DELTAX) return fail(ALPHA_E_ARG, "groupNorm_workspace_bytes: unknown op %d", op);
+    // the call itself with launches switched off (tensors at placeholder addresses far apart); those of elements that start on no 16-byte boundary need the most
+    auto at = [&](int i) { return reinterpret_cast<void*>((static_cast<uintptr_t>(i + 1) << 44) + 4); };
+    auto f = [&](int i) { return static_cast<float*>(at(i)); };
+    auto words = [&](int i) { return reinterpret_cast<void*>(static_cast<uintptr_t>(i + 1) << 44); };
+    size_t most = 0;
+    int rc = ALPHA_OK;
+    for (int form = 0; form < 2 && !rc; ++form) {
+        dry_begin();
+        auto t = [&](int i) { return form ? words(i) : at(i); };
+        rc = op == ALPHA_OP_FORWARD ? alpha_groupNorm(s, t(0), at(1), at(2), f(3), f(4), t(5), nullptr)
+                                    : alpha_groupNorm_delta(s, t(0), t(1), f(2), f(3), at(4), at(5), t(6), at(7), at(8), nullptr);
+        most = std::max(most, dry_end());
+    }
+    *bytes = most;
+    return rc;
+}
+
+}  // extern "C"

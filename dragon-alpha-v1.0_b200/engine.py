@@ -43,6 +43,13 @@ def _pool_shape(*dims):
     return _cached_pool_shape(*map(operator.index, dims))
 
 
+_cached_norm_shape = functools.lru_cache(maxsize=512)(_l.AlphaNormShape)
+
+
+def _norm_shape(N, positions, C, groups, dtype, affine_dtype, act, k, eps):
+    return _cached_norm_shape(*map(operator.index, (N, positions, C, groups, dtype, affine_dtype, act)), float(k), float(eps))
+
+
 def _fc_shape(rows, IC, OC, dtype, act, k):
     return _cached_fc_shape(*map(operator.index, (rows, IC, OC, dtype, act)), float(k))
 
@@ -314,6 +321,18 @@ class CudaFloat32EngineBase:
         _l.check(fn(C.byref(_fc_shape(rows, IC, OC, dtype, act, k)), a(deltaY_address), a(X_address), a(W_address), a(Z_address), a(deltaZ_address),
                     a(deltaX_address), a(deltaW_address), a(deltaB_address), _stream(self._stream)))
 
+    # ---- group normalisation (shape: AlphaNormShape) ----
+    def groupNorm(self, shape, X_address, gamma_address, beta_address, mean_address, rstd_address, Y_address):
+        b, a = self._addr_or_none, self._addr
+        _l.check(self._lib.alpha_groupNorm(C.byref(shape), a(X_address), b(gamma_address), b(beta_address), b(mean_address), b(rstd_address), a(Y_address), _stream(self._stream)))
+        return self
+
+    def groupNorm_delta(self, shape, deltaY_address, X_address, mean_address, rstd_address, gamma_address, beta_address, deltaX_address, deltaGamma_address, deltaBeta_address):
+        b, a = self._addr_or_none, self._addr
+        _l.check(self._lib.alpha_groupNorm_delta(C.byref(shape), a(deltaY_address), a(X_address), a(mean_address), a(rstd_address), b(gamma_address), b(beta_address),
+                                                 a(deltaX_address), b(deltaGamma_address), b(deltaBeta_address), _stream(self._stream)))
+        return self
+
     # ---- pooling, Java argument order (CudaFloat32EngineBase.java:2012-2215) ----
     def _pool(self, fn, N, IH, IW, IC, FH, FW, OH, OW, sh, sw, ph, pw, *ptrs_and_flags):
         s = _pool_shape(N, IH, IW, IC, FH, FW, OH, OW, sh, sw, ph, pw)
@@ -383,6 +402,7 @@ def _pad_both(t, n4, c4):
     return out
 
 
+_ADAMW_ROW = struct.Struct("@7Pqd4i")      # AlphaAdamW
 _dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
 _FC_TYPES = {torch.float32: _l.ALPHA_F32, torch.bfloat16: _l.ALPHA_BF16, torch.float16: _l.ALPHA_F16}
 
@@ -532,6 +552,38 @@ def _refuse_overlaps(what, grads, Out):
                 break
             if (write or other) and not _apart(a, b):
                 raise ValueError("%s: an output overlaps another tensor" % what)
+
+
+def _dense(t):
+    """t as dense memory that holds its values."""
+    return t.resolve_neg().contiguous()
+
+
+class AdamWState:
+    """The moments of Engine.adamW, a list of each: float32 tensors of the parameters' shapes, or (8 bits) float8_e4m3fn codes of these shapes with
+    float8_e8m0fnu scales, one for every 32 elements in the order they lie in.  Engine.adamW_state makes one; a program that keeps its moments elsewhere (views of a flat
+    buffer, a checkpoint) passes its own dense tensors."""
+
+    def __init__(self, m, v, m_scale=None, v_scale=None):
+        self.m, self.v = list(m), list(v)
+        if (m_scale is None) != (v_scale is None):
+            raise ValueError("AdamWState: scales of both moments, or of neither")
+        self.m_scale, self.v_scale = (None, None) if m_scale is None else (list(m_scale), list(v_scale))
+        self.bits = 32 if m_scale is None else 8
+        lists = [self.m, self.v] + ([self.m_scale, self.v_scale] if self.bits == 8 else [])
+        if len(set(map(len, lists))) != 1:
+            raise ValueError("AdamWState: lists of different lengths")
+        code = torch.float32 if self.bits == 32 else torch.float8_e4m3fn
+        for i, (a, b) in enumerate(zip(self.m, self.v)):
+            if a.dtype != code or b.dtype != code or a.shape != b.shape:
+                raise ValueError("AdamWState: moments of tensor %d are %s %s and %s %s, expected %s of one shape" % (i, a.dtype, tuple(a.shape), b.dtype, tuple(b.shape), code))
+        if self.bits == 8:
+            for i, (a, s, t) in enumerate(zip(self.m, self.m_scale, self.v_scale)):
+                if any(x.dtype != torch.float8_e8m0fnu or x.numel() != -(-a.numel() // 32) for x in (s, t)):
+                    raise ValueError("AdamWState: scales of tensor %d must be %d float8_e8m0fnu values" % (i, -(-a.numel() // 32)))
+        for t in itertools.chain.from_iterable(lists):
+            if not t.is_contiguous() or t.is_neg():
+                raise ValueError("AdamWState: moments must be dense")
 
 
 _pack_jobs = {n: struct.Struct("%dq" % (6 * n)).pack for n in (1, 2, 3)}
@@ -891,6 +943,160 @@ class Engine:
                     for o, t in back:
                         o.copy_(t)
         return norm
+
+    # ---- the optimizer's step after them ----
+    @staticmethod
+    def adamW_state(params, bits=32):
+        """Moments of 0 for the tensors of `params`, of 32 or 8 bits."""
+        params = list(params)
+        if bits == 32:
+            return AdamWState(*([torch.zeros(p.shape, dtype=torch.float32, device=p.device) for p in params] for _ in range(2)))
+        if bits != 8:
+            raise ValueError("adamW_state: moments of 32 or 8 bits, not %r" % (bits,))
+        codes, scales = ([[torch.zeros(shape(p), dtype=torch.uint8, device=p.device).view(t) for p in params] for _ in range(2)] for shape, t in (
+            (lambda p: p.shape, torch.float8_e4m3fn), (lambda p: (-(-p.numel() // 32),), torch.float8_e8m0fnu)))
+        return AdamWState(*codes, *scales)
+
+    @staticmethod
+    def _device_value(what, name, x, dtype, device):
+        """(value, None) of a number, (0, address) of a tensor of one element on the GPU."""
+        if not isinstance(x, torch.Tensor):
+            return x, None
+        if x.dtype != dtype or x.numel() != 1 or x.get_device() != device or x.is_neg():
+            raise ValueError("%s: %s on the GPU must be one %s value beside the tensors" % (what, name, dtype))
+        return 0, x.data_ptr()
+
+    def adamW(self, params, grads, state, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, max_norm=None, norm=None, Out=None, seed=0):
+        """One AdamW step in place over lists of parameters and gradients (float32, bfloat16, float16; those without a gradient, None, are left out)
+        and their moments (AdamWState):  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+            p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps).
+        step (from 1 on) and lr may be tensors of one int64 and float32 value on the GPU, for a step that a graph replays; weight_decay one number or one for each tensor.
+        max_norm: gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way, and not written; norm is that of grad_norm unless given (one float32 value on the
+        GPU), and a step whose norm is NaN or Inf changes nothing.  Out: tensors of the parameters' shapes (None: none) that take the new values in their own type, the 16-bit
+        copies of float32 weights.  seed (32 bits): of the rounding of 8-bit moments.  Returns the norm, or None without max_norm."""
+        params, grads = list(params), list(grads)
+        n = len(params)
+        outs = [None] * n if Out is None else list(Out)
+        decay = [float(weight_decay)] * n if not isinstance(weight_decay, (list, tuple)) else [float(d) for d in weight_decay]
+        if len(grads) != n or len(outs) != n or len(decay) != n or len(state.m) != n:
+            raise ValueError("adamW: %d parameters, %d gradients, moments of %d, %d outputs, %d weight decays" % (n, len(grads), len(state.m), len(outs), len(decay)))
+        if norm is not None and max_norm is None:
+            raise ValueError("adamW: a norm without max_norm")
+        if not 0 <= operator.index(seed) < 2 ** 32:
+            raise ValueError("adamW: seed must have 32 bits")
+        used = [i for i in range(n) if grads[i] is not None]
+        if not used:
+            return None if max_norm is None else norm if norm is not None else self.grad_norm([])
+        device = params[used[0]].get_device()
+        if device < 0:
+            raise ValueError("adamW: tensors must be on a GPU")
+        eight = state.bits == 8
+        rows = []
+        for i in used:
+            p, g, o = params[i], grads[i], outs[i]
+            for name, t in (("parameter", p), ("gradient", g), ("output", o)):
+                if t is None:
+                    continue
+                if t.dtype not in _FC_TYPES:
+                    raise ValueError("adamW: %s %d must be float32, bfloat16 or float16, not %s" % (name, i, t.dtype))
+                if t.shape != p.shape or t.get_device() != device:
+                    raise ValueError("adamW: %s %d is %s on %s, parameter %s on %s" % (name, i, tuple(t.shape), t.device, tuple(p.shape), p.device))
+                if t is not g and (not t.is_contiguous() or t.is_neg()):
+                    raise ValueError("adamW: %s %d must be dense" % (name, i))
+            moments = (state.m[i], state.v[i]) + ((state.m_scale[i], state.v_scale[i]) if eight else ())
+            if state.m[i].numel() != p.numel() or any(t.get_device() != device for t in moments):
+                raise ValueError("adamW: moments %d are %s on %s, parameter %s on %s" % (i, tuple(state.m[i].shape), state.m[i].device, tuple(p.shape), p.device))
+            rows.append((i, p, g, o, moments))
+        lr, lr_at = self._device_value("adamW", "lr", lr, torch.float32, device)
+        step, step_at = self._device_value("adamW", "step", step, torch.int64, device)
+        with self._on(params[used[0]]), torch.no_grad():
+            held = [_dense(g) for _, _, g, _, _ in rows]
+            if max_norm is not None and norm is None:
+                norm = self.grad_norm(held)
+            norm_at = None
+            if max_norm is not None:
+                _, norm_at = self._device_value("adamW", "norm", norm, torch.float32, device)
+                if norm_at is None:
+                    raise ValueError("adamW: norm must be a tensor on the GPU")
+            # (pad: the table keeps the number of each tensor among all, which the random bits of its moments go by)
+            table = bytearray()
+            at = 0
+            for (i, p, g, o, moments), d in zip(rows, held):
+                while at < i:
+                    table += _ADAMW_ROW.pack(0, 0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0, 0, state.bits)
+                    at += 1
+                table += _ADAMW_ROW.pack(p.data_ptr(), d.data_ptr(), *(t.data_ptr() for t in moments), *(() if eight else (0, 0)), 0 if o is None else o.data_ptr(), p.numel(),
+                                         decay[i], _FC_TYPES[p.dtype], _FC_TYPES[g.dtype], 0 if o is None else _FC_TYPES[o.dtype], state.bits)
+                at += 1
+            how = _l.AlphaAdamWStep(float(lr), float(beta1), float(beta2), float(eps), 0.0 if max_norm is None else float(max_norm), operator.index(step), norm_at, lr_at, step_at,
+                                    operator.index(seed))
+            _l.check(self.base._lib.alpha_adamW(at, bytes(table), C.byref(how), _stream(self.base._stream)))
+        return norm
+
+    # ---- group normalisation ----
+    def groupNorm(self, X, groups, gamma=None, beta=None, eps=1e-5, act="none", k=0.0, save=False):
+        """act((X - mean) / sqrt(variance + eps) * gamma + beta) of channels-last tensors X [N, ..., C] (float32, bfloat16, float16), mean and variance over the
+        positions and the channels of each of `groups` groups of neighbours.  gamma, beta [C]: of X's type or float32, both or neither.  act as in fullConnect.  save=True
+        also returns mean and rstd [N, groups] (float32), which groupNorm_delta reads."""
+        shape, gamma, beta = self._norm_call("groupNorm", X, groups, gamma, beta, eps, act, k, ())
+        if shape is None:
+            return (X.new_empty(X.shape), _new(X, (0, groups)), _new(X, (0, groups))) if save else X.new_empty(X.shape)
+        with self._on(X), torch.no_grad():
+            X = _dense(X)
+            Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+            mean, rstd = (_new(X, (X.shape[0], groups)), _new(X, (X.shape[0], groups))) if save else (None, None)
+            self.base.groupNorm(shape, X, gamma, beta, mean, rstd, Y)
+        return (Y, mean, rstd) if save else Y
+
+    def groupNorm_delta(self, deltaY, X, mean, rstd, gamma=None, beta=None, act="none", k=0.0):
+        """(deltaX, deltaGamma, deltaBeta) of groupNorm from deltaY, its X and the mean and rstd it saved; the latter two None without gamma and beta."""
+        if mean.dim() != 2:
+            raise ValueError("groupNorm_delta: mean %s, expected [N, groups]" % (tuple(mean.shape),))
+        groups = mean.shape[1]
+        kept = (X.shape[0] if X.dim() else 0, groups)
+        shape, gamma, beta = self._norm_call("groupNorm_delta", X, groups, gamma, beta, 0.0, act, k,
+                                                   (("deltaY", deltaY, tuple(X.shape), X.dtype), ("mean", mean, kept, torch.float32), ("rstd", rstd, kept, torch.float32)))
+        if shape is None:
+            return X.new_empty(X.shape), *(None if gamma is None else torch.zeros_like(gamma) for _ in range(2))
+        with self._on(X), torch.no_grad():
+            deltaY, X, mean, rstd = _dense(deltaY), _dense(X), _dense(mean), _dense(rstd)
+            dX = torch.empty(X.shape, dtype=X.dtype, device=X.device)
+            dG, dB = (torch.empty_like(gamma), torch.empty_like(gamma)) if gamma is not None else (None, None)
+            self.base.groupNorm_delta(shape, deltaY, X, mean, rstd, gamma, beta, dX, dG, dB)
+        return dX, dG, dB
+
+    def _norm_call(self, what, X, groups, gamma, beta, eps, act, k, others):
+        """The checked call: its shape (None where X holds nothing), gamma and beta as dense memory."""
+        code, groups = _fc_act(what, act), operator.index(groups)
+        if X.dtype not in _FC_TYPES:
+            raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, X.dtype))
+        if X.dim() < 2 or groups < 1 or X.shape[-1] < 1 or X.shape[-1] % groups:
+            raise ValueError("%s: X %s in %d groups of channels" % (what, tuple(X.shape), groups))
+        if (gamma is None) != (beta is None):
+            raise ValueError("%s: gamma and beta, or neither" % what)
+        channels, affine = X.shape[-1], X.dtype
+        if gamma is not None:
+            affine = gamma.dtype if gamma.dtype == torch.float32 else X.dtype
+            others += (("gamma", gamma, (channels,), affine), ("beta", beta, (channels,), affine))
+        if X.get_device() < 0:
+            raise ValueError("%s: tensors must be on a GPU" % what)
+        for name, t, shape, dtype in others:
+            if tuple(t.shape) != shape:
+                raise ValueError("%s: %s %s, expected %s" % (what, name, tuple(t.shape), shape))
+            if t.dtype != dtype or t.get_device() != X.get_device():
+                raise ValueError("%s: %s is %s on %s, X %s on %s" % (what, name, t.dtype, t.device, X.dtype, X.device))
+        positions = 1
+        for n in X.shape[1:-1]:
+            positions *= n
+        if positions == 0:
+            raise ValueError("%s: X %s has no positions to take a mean of" % (what, tuple(X.shape)))
+        if X.shape[0] == 0:
+            return None, gamma, beta
+        if max(X.shape[0] * channels, positions) >= 2 ** 31:
+            raise ValueError("%s: X %s is too large" % (what, tuple(X.shape)))
+        with self._on(X), torch.no_grad():
+            gamma, beta = (None if t is None else _dense(t) for t in (gamma, beta))
+        return _norm_shape(X.shape[0], positions, channels, groups, _FC_TYPES[X.dtype], _FC_TYPES[affine], code, k, eps), gamma, beta
 
     # Batched products with the engine's memory rule (only the last dimension of a tensor is padded to a multiple
     # of 4) and EngineCore's argument mapping (EngineCore.java:579-623): the row pitch and the logical row length

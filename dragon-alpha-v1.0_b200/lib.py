@@ -30,6 +30,20 @@ class AlphaGrad(C.Structure):
     _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("count", C.c_int64), ("dtype", C.c_int), ("out_dtype", C.c_int)]
 
 
+class AlphaNormShape(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("N", "positions", "C", "groups", "dtype", "affine_dtype", "act")] + [("k", C.c_float), ("eps", C.c_float)]
+
+
+class AlphaAdamW(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "m", "v", "m_scale", "v_scale", "out")] + [("count", C.c_int64), ("weight_decay", C.c_double)] + [
+        (n, C.c_int) for n in ("dtype", "grad_dtype", "out_dtype", "moment_bits")]
+
+
+class AlphaAdamWStep(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "max_norm")] + [("step", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("norm", "lr_device", "step_device")] + [("seed", C.c_uint32)]
+
+
 class AlphaConvError(RuntimeError):
     """A call into the library returned a non-zero status; .code holds the ALPHA_E_* value."""
 
@@ -152,6 +166,11 @@ def load():
     lib.alpha_fullConnect_workspace_bytes.argtypes = [F, I, I, C.POINTER(C.c_size_t)]
     lib.alpha_grad_norm.argtypes = [I, G, V, V]
     lib.alpha_clip_grad_norm.argtypes = [I, G, C.c_double, V, V]
+    NS = C.POINTER(AlphaNormShape)
+    lib.alpha_groupNorm.argtypes = [NS, V, V, V, V, V, V, V]
+    lib.alpha_groupNorm_delta.argtypes = [NS, V, V, V, V, V, V, V, V, V, V]
+    lib.alpha_groupNorm_workspace_bytes.argtypes = [NS, I, C.POINTER(C.c_size_t)]
+    lib.alpha_adamW.argtypes = [I, G, C.POINTER(AlphaAdamWStep), V]      # (a table of AlphaAdamW, or its bytes)
     # pooling
     PS = C.POINTER(AlphaPoolShape)
     lib.alpha_pool2D_max.argtypes = [PS, V, V, V]
@@ -233,6 +252,13 @@ def fullConnect_workspace_bytes(shape, glu, op):
     """Scratch bytes of a fullConnect (glu: fullConnect_glu) call: op 'forward', or 'deltaX' for that of all gradients."""
     n = C.c_size_t(0)
     check(load().alpha_fullConnect_workspace_bytes(C.byref(shape), int(bool(glu)), OPS[op], C.byref(n)))
+    return n.value
+
+
+def groupNorm_workspace_bytes(shape, op):
+    """Scratch bytes of a groupNorm call ('forward') or of its gradients' ('deltaX')."""
+    n = C.c_size_t(0)
+    check(load().alpha_groupNorm_workspace_bytes(C.byref(shape), OPS[op], C.byref(n)))
     return n.value
 
 

@@ -501,6 +501,32 @@ int alpha_fullConnect_glu_delta(const AlphaFcShape* s, const void* deltaY, const
 /* Scratch of a call, as alpha_conv_workspace_bytes: op ALPHA_OP_FORWARD, or ALPHA_OP_DELTAX for the call of all gradients. */
 int alpha_fullConnect_workspace_bytes(const AlphaFcShape* s, int glu, int op, size_t* bytes);
 
+/* ---- group normalisation -----------------------------------------------------------------------------------------
+ *
+ * Channels-last tensors X[N][positions][C] of fp32, bf16 or fp16, C channels in `groups` groups of D = C / groups neighbours:
+ *   mean, rstd = 1 / sqrt(variance + eps) over the positions and the D channels of (sample, group)
+ *   Y = act((X - mean) rstd gamma + beta)
+ * gamma, beta [C]: of the tensors' type or fp32 (affine_dtype), or both NULL (1 and 0).  mean, rstd [N][groups] of fp32, for the backward
+ * pass; both may be NULL.  The gradients, from deltaY and what the forward call read and left:
+ *   dz = deltaY act'(z), z formed again;  deltaGamma = sum dz xh, deltaBeta = sum dz over samples and positions, xh = (X - mean) rstd
+ *   deltaX = rstd (dz gamma - mean of dz gamma - xh (mean of dz gamma xh))
+ * deltaGamma and deltaBeta, of affine_dtype, may both be NULL.  Tensors are dense and aligned to their elements (those that start on 16-byte
+ * boundaries, with rows of whole 16-byte words, take the faster kernels); no output may overlap an input (ALPHA_E_ARG).
+ * Everything is formed in fp32 and rounded once; sums do not depend on scheduling.  Scratch (alpha_groupNorm_workspace_bytes): partial sums of groups that do not
+ * fit into shared memory, and the channels' sums of a backward call. */
+typedef struct AlphaNormShape {
+    int N, positions, C, groups;
+    int dtype, affine_dtype; /* ALPHA_F32, ALPHA_BF16 or ALPHA_F16 */
+    int act;                 /* ALPHA_ACT_* */
+    float k;                 /* slope of ALPHA_ACT_LEAKY_RELU */
+    float eps;
+} AlphaNormShape;
+int alpha_groupNorm(const AlphaNormShape* s, const void* X, const void* gamma, const void* beta, float* mean, float* rstd, void* Y, alpha_stream_t stream);
+int alpha_groupNorm_delta(const AlphaNormShape* s, const void* deltaY, const void* X, const float* mean, const float* rstd, const void* gamma, const void* beta,
+                          void* deltaX, void* deltaGamma, void* deltaBeta, alpha_stream_t stream);
+/* op ALPHA_OP_FORWARD or ALPHA_OP_DELTAX; enough for any alignment of the tensors. */
+int alpha_groupNorm_workspace_bytes(const AlphaNormShape* s, int op, size_t* bytes);
+
 /* ---- all gradients of a step -----------------------------------------------------------------------------------
  *
  * norm = sqrt(sum of the squares of all elements of n tensors), written to *norm as a float on the device; NaN or Inf elements
@@ -520,6 +546,39 @@ typedef struct AlphaGrad {
 } AlphaGrad;
 int alpha_grad_norm(int n, const AlphaGrad* grads, float* norm, alpha_stream_t stream);
 int alpha_clip_grad_norm(int n, const AlphaGrad* grads, double max_norm, float* norm, alpha_stream_t stream);
+
+/* ---- an optimizer step ------------------------------------------------------------------------------------------
+ *
+ * AdamW over n tensors:  g' = c g,  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps),  all in fp32, p rounded once to its type.
+ * c = 1, or with `norm` (a float on the device, as alpha_grad_norm leaves it) min(1, max_norm / (norm + 1e-6)) rounded to fp32; a norm that is NaN
+ * or Inf leaves the step out: nothing is changed.  `out` (may be NULL): the new p in another type, a 16-bit copy of fp32 weights.
+ * Moments of 32 bits are floats.  Moments of 8 bits are e4m3 codes, m_scale and v_scale exponent bytes (2^(byte - 127); 0: 2^-127, 255: NaN) for every
+ * 32 elements, (count + 31) / 32 of them; what a step writes is rounded up or down at random so that its mean is kept, with 16 bits of a hash of seed, step, the tensor's
+ * number in the call and the element's (the same call gives the same bits), and a v that is not 0 gets a code that is not 0.  Codes and scales of 0 are moments of 0.
+ * lr_device and step_device (may be NULL) replace lr and step by values on the device, for steps that a graph replays.
+ * Tensors may be of different types and any size from 0 on, aligned to their elements; the moments of all have the same number of bits.  What is
+ * written must not overlap any other tensor of the call (ALPHA_E_ARG).  No scratch. */
+typedef struct AlphaAdamW {
+    void* param;
+    const void* grad;
+    void *m, *v;                 /* floats, or codes of 8 bits */
+    void *m_scale, *v_scale;     /* 8 bits only */
+    void* out;
+    int64_t count;               /* elements */
+    double weight_decay;
+    int dtype, grad_dtype, out_dtype; /* ALPHA_F32, ALPHA_BF16 or ALPHA_F16 */
+    int moment_bits;             /* 32 or 8 */
+} AlphaAdamW;
+typedef struct AlphaAdamWStep {
+    double lr, beta1, beta2, eps, max_norm;
+    int64_t step;                /* 1 for the first */
+    const float* norm;
+    const float* lr_device;
+    const int64_t* step_device;
+    uint32_t seed;
+} AlphaAdamWStep;
+int alpha_adamW(int n, const AlphaAdamW* tensors, const AlphaAdamWStep* step, alpha_stream_t stream);
 
 /* ---- 2D pooling (the operators between the convolutions of a network) ---------------------------------------
  * Replace the kernels behind src/cu32_src/Cuda_pool2D/Cuda_pool2D/pool2D.cuh and
