@@ -440,6 +440,18 @@ int call_scratch(cudaStream_t stream, size_t bytes, void** out)
     *out = p;
     return rc;
 }
+ScratchMark call_mark(cudaStream_t stream)
+{
+    DeviceCtx* c;
+    if (get_ctx(&c)) return ScratchMark{0, 0, 0};
+    const WsMark m = ws_mark(c, stream);
+    return ScratchMark{m.block_used, m.caller_used, m.dry_cur};
+}
+void call_rewind(cudaStream_t stream, const ScratchMark& m)
+{
+    DeviceCtx* c;
+    if (!get_ctx(&c)) ws_rewind(c, stream, WsMark{m.block, m.caller, m.dry});
+}
 bool dry_run() { return t_dry; }
 void dry_begin() { t_dry = true; t_dry_cur = t_dry_peak = 0; }
 size_t dry_end() { t_dry = false; return t_dry_peak; }

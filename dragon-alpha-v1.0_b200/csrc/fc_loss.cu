@@ -1,0 +1,281 @@
+// Softmax cross entropy on top of a FullConnect layer whose logits are not kept, and its gradients.
+//
+//   z = X W^T + bias,  lse = log sum exp z,  loss = lse - z[label]
+//   dz = dL (exp(z - lse) - [label]),  deltaX = dz W,  deltaW = dz^T X,  deltaB = column sums of dz
+//
+// 16-bit tensors.  Forward: one product whose epilogue reduces each tile's row to its largest logit and the sum of exponentials about it (8 bytes for 128 or fewer logits), and a
+// pass that joins them.  Gradients, piece by piece of the classes: logits formed once more, their gradients rounded to the tensors' type into scratch as the epilogue
+// of that product, and the two products that read them; deltaX is summed in fp32 over the pieces.  dz is rounded once, as deltaZ of a FullConnect layer is; in fp16 it is held times a
+// power of two (the largest |dL| at 2^14 or above), as a probability of 1e-5 over 1e4 rows would not be a normal number, and the outputs are scaled back in fp32.
+// Bound by the tensor cores: 2 (forward) and 6 (gradients) rows x classes x IC operations; for few rows by reading W.
+//
+// fp32 tensors: products at fp32 accuracy as those of the layer, logits of a piece in scratch.
+#include "fc_loss.cuh"
+#include "fc_product.cuh"
+
+using namespace alpha;
+
+namespace alpha {
+// fp32 products of a call that has begun (fc_api.cu).
+int fc_logits_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Y, cudaStream_t stream);
+int fc_gradients_f32(const AlphaFcShape* s, const float* dZ, const float* X, const float* W, float* dX, float* dW, cudaStream_t stream);
+}
+
+namespace {
+
+constexpr size_t kPieceBytes = 256u << 20;       // of logits or their gradients in scratch
+
+struct Loss {
+    const AlphaFcShape* s;
+    const void *X, *W, *bias, *label;
+    int label_bytes;
+    cudaStream_t stream;
+};
+
+const char* at_class(const void* p, size_t first, size_t row_bytes) { return static_cast<const char*>(p) + first * row_bytes; }
+
+int join(const Loss& c, const float2* part, int slots, int row0, int rows, const float* at_label, float* loss, float* lse)
+{
+    int across = 1;
+    while (across < 32 && across < rows) across *= 2;
+    const char* label = at_class(c.label, row0, c.label_bytes);
+    launch_after(loss_join_kernel, (rows + across - 1) / across, kJoinThreads, 0, c.stream, part, slots, rows, across, label, c.label_bytes, c.s->OC, at_label, loss ? loss + row0 : nullptr,
+                 lse ? lse + row0 : nullptr);
+    note_launch("fc_loss");
+    return launched("loss_join_kernel");
+}
+
+int forward_16(const Loss& c, float* loss, float* lse)
+{
+    const long long IC = c.s->IC, OC = c.s->OC;
+    int sms = 0, *status = nullptr;
+    int rc = device_sms(&sms);
+    if (!rc) rc = device_status_word(&status);
+    if (rc) return rc;
+    // runs of rows whose parts take about the size of a piece (a slot for 128 classes, where there are many rows)
+    long long run = static_cast<long long>(kPieceBytes / 8) / ((OC + 127) / 128);
+    run = std::min<long long>(std::max(4096LL, run / 256 * 256), c.s->rows);
+    const ScratchMark mark = call_mark(c.stream);
+    for (long long row0 = 0; row0 < c.s->rows; row0 += run) {
+        call_rewind(c.stream, mark);
+        const int rows = static_cast<int>(std::min<long long>(run, c.s->rows - row0));
+        Product q{c.s->dtype, rows, c.s->OC, fc_pitch(c.s->OC), c.s->IC, 1, 1, false, Operand{at_class(c.X, row0, IC * 2), false, IC, 1, rows, IC, IC}, Operand{c.W, false, IC, OC, 1, IC, OC * IC}, c.bias, nullptr, nullptr, nullptr,
+                  ALPHA_ACT_NONE, 0.f, FcLoss{}};
+        float2 dummy;
+        q.loss.part = &dummy;                         // (the plan: nothing is written but parts)
+        const FcPlan plan = pick_plan(q, sms, nullptr, 1);
+        const long long slots = 2 * ((OC + plan.bn - 1) / plan.bn);
+        void *part = nullptr, *at_label = nullptr;
+        rc = call_scratch(c.stream, static_cast<size_t>(slots) * rows * sizeof(float2), &part);
+        if (!rc) rc = call_scratch(c.stream, rows * sizeof(float), &at_label);
+        if (rc) return rc;
+        if (dry_run()) continue;
+        q.loss.label = at_class(c.label, row0, c.label_bytes); q.loss.label_bytes = c.label_bytes; q.loss.classes = c.s->OC;
+        q.loss.part = static_cast<float2*>(part); q.loss.at_label = static_cast<float*>(at_label);
+        rc = launch_planned<kFcStats>(q, nullptr, plan, sms, status, c.stream);
+        if (!rc) rc = join(c, q.loss.part, static_cast<int>(slots), static_cast<int>(row0), rows, q.loss.at_label, loss, lse);
+        if (rc) return rc;
+    }
+    return ALPHA_OK;
+}
+
+// deltaB of a piece from its dz.
+template <class T> int column_sums(const T* dz, int rows, int pitch, const float* scale, T* dB, int sms, cudaStream_t stream)
+{
+    const int blocks = (pitch + 32 * Word16<T>::N - 1) / (32 * Word16<T>::N), most = std::max(1, 8 * sms / blocks), parts = std::min((rows + 31) / 32, most);
+    void* part = nullptr;
+    int rc = call_scratch(stream, static_cast<size_t>(parts) * pitch * sizeof(float), &part);
+    if (rc || dry_run()) return rc;
+    launch_after(loss_columns_kernel<T>, dim3(blocks, parts), 256, 0, stream, dz, rows, pitch, static_cast<float*>(part));
+    note_launch("fc_loss");
+    rc = launched("loss_columns_kernel");
+    if (rc) return rc;
+    launch_after(loss_bias_kernel<T>, (pitch + 255) / 256, 256, 0, stream, static_cast<const float*>(part), parts, pitch, scale, dB);
+    note_launch("fc_loss");
+    return launched("loss_bias_kernel");
+}
+
+// Classes of a piece: all, or as many as fit, in even pieces of multiples of `unit`.
+long long piece_classes(long long rows, long long classes, size_t size, long long unit)
+{
+    const long long fit = std::max<long long>(unit, static_cast<long long>(kPieceBytes / size) / rows / unit * unit), pieces = (classes + fit - 1) / fit;
+    return std::min(classes, ((classes + pieces - 1) / pieces + unit - 1) / unit * unit);
+}
+
+template <class T> int delta_16(const Loss& c, const float* dL, int dL_step, const float* lse, void* dX, void* dW, void* dB)
+{
+    const long long rows = c.s->rows, IC = c.s->IC, OC = c.s->OC, piece = piece_classes(rows, OC, 2, 256), pieces = (OC + piece - 1) / piece;
+    int sms = 0;
+    int rc = device_sms(&sms);
+    void *dz = nullptr, *sums = nullptr, *scale = nullptr;
+    if (!rc) rc = call_scratch(c.stream, static_cast<size_t>(rows) * fc_pitch(static_cast<int>(piece)) * 2, &dz);
+    if (!rc && dX && pieces > 1) rc = call_scratch(c.stream, static_cast<size_t>(rows) * IC * 4, &sums);
+    if (!rc && c.s->dtype == ALPHA_F16) rc = call_scratch(c.stream, 2 * sizeof(float), &scale);
+    if (rc) return rc;
+    if (scale && !dry_run()) {
+        launch_after(loss_scale_kernel, 1, 1024, 0, c.stream, dL, dL_step ? c.s->rows : 1, static_cast<float*>(scale));
+        note_launch("fc_loss");
+        rc = launched("loss_scale_kernel");
+        if (rc) return rc;
+    }
+    const ScratchMark mark = call_mark(c.stream);
+    for (long long first = 0; first < OC; first += piece) {
+        call_rewind(c.stream, mark);
+        const long long cols = std::min(piece, OC - first), pitch = fc_pitch(static_cast<int>(cols));
+        const int dtype = c.s->dtype;
+        const T* W = static_cast<const T*>(c.W) + first * IC;
+        FcLoss l{};
+        l.label = c.label; l.label_bytes = c.label_bytes; l.base = static_cast<int>(first); l.classes = c.s->OC;
+        l.lse = lse; l.grad = dL; l.grad_step = dL_step; l.scale = static_cast<const float*>(scale);
+        if (!dry_run()) {
+            const Product z{dtype, c.s->rows, static_cast<int>(cols), static_cast<int>(pitch), c.s->IC, 1, 1, false, Operand{c.X, false, IC, 1, rows, IC, IC}, Operand{W, false, IC, cols, 1, IC, cols * IC},
+                            c.bias ? static_cast<const T*>(c.bias) + first : nullptr, nullptr, nullptr, dz, ALPHA_ACT_NONE, 0.f, l};
+            rc = launch_product<kFcSoftmaxDelta>(z, c.stream);
+            if (rc) return rc;
+            FcLoss of_x{}, of_w{};
+            of_x.scale = of_w.scale = l.scale;
+            of_x.sums = static_cast<float*>(sums); of_x.first = first == 0; of_x.last = first + cols == OC;
+            const Product x{dtype, c.s->rows, c.s->IC, c.s->IC, static_cast<int>(cols), 1, 1, false, Operand{dz, false, cols, 1, rows, pitch, pitch}, Operand{W, true, IC, cols, 1, IC, cols * IC},
+                            nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f, of_x};
+            const Product w{dtype, static_cast<int>(cols), c.s->IC, c.s->IC, c.s->rows, 1, 1, false, Operand{dz, true, cols, 1, rows, pitch, pitch}, Operand{c.X, true, IC, rows, 1, IC, rows * IC},
+                            nullptr, nullptr, nullptr, dW ? static_cast<T*>(dW) + first * IC : nullptr, ALPHA_ACT_NONE, 0.f, of_w};
+            if (dX && dW) rc = launch_products<kFcSum>(x, w, c.stream);
+            else if (dX) rc = launch_product<kFcSum>(x, c.stream);
+            else if (dW) rc = launch_product<kFcSum>(w, c.stream);
+            if (rc) return rc;
+        }
+        if (dB) rc = column_sums(static_cast<const T*>(dz), c.s->rows, static_cast<int>(pitch), l.scale, static_cast<T*>(dB) + first, sms, c.stream);
+        if (rc) return rc;
+    }
+    return ALPHA_OK;
+}
+
+int forward_f32(const Loss& c, float* loss, float* lse)
+{
+    const long long rows = c.s->rows, IC = c.s->IC, OC = c.s->OC, piece = piece_classes(rows, OC, 4, 8), pieces = (OC + piece - 1) / piece;
+    void *z = nullptr, *part = nullptr, *at_label = nullptr;
+    int rc = call_scratch(c.stream, static_cast<size_t>(rows) * fc_pitch(static_cast<int>(piece)) * 4, &z);
+    if (!rc) rc = call_scratch(c.stream, static_cast<size_t>(pieces) * rows * sizeof(float2), &part);
+    if (!rc) rc = call_scratch(c.stream, rows * sizeof(float), &at_label);
+    const ScratchMark mark = call_mark(c.stream);
+    for (long long first = 0; first < OC && !rc; first += piece) {
+        call_rewind(c.stream, mark);
+        AlphaFcShape s = *c.s;
+        s.OC = static_cast<int>(std::min(piece, OC - first));
+        rc = fc_logits_f32(&s, static_cast<const float*>(c.X), static_cast<const float*>(c.W) + first * IC, c.bias ? static_cast<const float*>(c.bias) + first : nullptr, static_cast<float*>(z), c.stream);
+        if (rc || dry_run()) continue;
+        launch_after(loss_rows_kernel, static_cast<unsigned>(rows), kRowThreads, 0, c.stream, static_cast<const float*>(z), fc_pitch(s.OC), s.OC, static_cast<int>(first), c.s->OC, c.s->rows, c.label,
+                     c.label_bytes, static_cast<float2*>(part) + first / piece * rows, static_cast<float*>(at_label));
+        note_launch("fc_loss");
+        rc = launched("loss_rows_kernel");
+    }
+    if (rc || dry_run()) return rc;
+    return join(c, static_cast<const float2*>(part), static_cast<int>(pieces), 0, c.s->rows, static_cast<const float*>(at_label), loss, lse);
+}
+
+int delta_f32(const Loss& c, const float* dL, int dL_step, const float* lse, float* dX, float* dW, float* dB)
+{
+    const long long rows = c.s->rows, IC = c.s->IC, OC = c.s->OC, piece = piece_classes(rows, OC, 4, 8), pieces = (OC + piece - 1) / piece;
+    int sms = 0;
+    int rc = device_sms(&sms);
+    void *dz = nullptr, *more = nullptr;
+    if (!rc) rc = call_scratch(c.stream, static_cast<size_t>(rows) * fc_pitch(static_cast<int>(piece)) * 4, &dz);
+    if (!rc && dX && pieces > 1) rc = call_scratch(c.stream, static_cast<size_t>(rows) * IC * 4, &more);
+    const ScratchMark mark = call_mark(c.stream);
+    for (long long first = 0; first < OC && !rc; first += piece) {
+        call_rewind(c.stream, mark);
+        AlphaFcShape s = *c.s;
+        s.OC = static_cast<int>(std::min(piece, OC - first));
+        const float *X = static_cast<const float*>(c.X), *W = static_cast<const float*>(c.W) + first * IC;
+        float* z = static_cast<float*>(dz);
+        rc = fc_logits_f32(&s, X, W, c.bias ? static_cast<const float*>(c.bias) + first : nullptr, z, c.stream);
+        if (!rc && !dry_run()) {
+            launch_after(loss_delta_kernel, static_cast<unsigned>(rows), kRowThreads, 0, c.stream, z, fc_pitch(s.OC), s.OC, static_cast<int>(first), c.s->OC, c.label, c.label_bytes, lse, dL, dL_step);
+            note_launch("fc_loss");
+            rc = launched("loss_delta_kernel");
+        }
+        if (rc) return rc;
+        float* x = dX && first ? static_cast<float*>(more) : dX;
+        call_rewind(c.stream, mark);                 // (what the logits' product was given)
+        if (dX || dW) rc = fc_gradients_f32(&s, z, X, W, x, dW ? dW + first * IC : nullptr, c.stream);
+        if (!rc && dX && first && !dry_run()) {
+            const size_t words = static_cast<size_t>(rows) * IC / 4;
+            launch_after(loss_add_kernel, static_cast<unsigned>(std::min<size_t>((words + 255) / 256, 8u * sms)), 256, 0, c.stream, reinterpret_cast<float4*>(dX), reinterpret_cast<const float4*>(x), words);
+            note_launch("fc_loss");
+            rc = launched("loss_add_kernel");
+        }
+        if (!rc && dB) rc = column_sums(z, c.s->rows, fc_pitch(s.OC), nullptr, dB + first, sms, c.stream);
+    }
+    return rc;
+}
+
+int check_loss(const char* what, const AlphaFcShape* s, const void* label, int label_bytes)
+{
+    const int rc = check_fc(what, s, false);
+    if (rc) return rc;
+    if (s->act != ALPHA_ACT_NONE) return fail(ALPHA_E_ARG, "%s: logits have no activation", what);
+    if (!label || (label_bytes != 4 && label_bytes != 8) || reinterpret_cast<uintptr_t>(label) % label_bytes) return fail(ALPHA_E_ARG, "%s: labels are integers of 4 or 8 bytes", what);
+    return ALPHA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int alpha_fullConnect_softmax_crossEntropy(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* label, int label_bytes, float* loss, float* lse,
+                                           alpha_stream_t stream)
+{
+    OpRange range("alpha_fullConnect_softmax_crossEntropy");
+    const char* what = "fullConnect_softmax_crossEntropy";
+    int rc = check_loss(what, s, label, label_bytes);
+    if (rc) return rc;
+    if (!X || !W || (!loss && !lse)) return fail(ALPHA_E_ARG, "%s: null tensor pointer", what);
+    if ((reinterpret_cast<uintptr_t>(loss) | reinterpret_cast<uintptr_t>(lse)) & 3) return fail(ALPHA_E_ARG, "%s: loss and lse are floats", what);
+    const size_t b = type_bytes(s->dtype), rows = s->rows;
+    const Span x{X, rows * s->IC * b}, w{W, static_cast<size_t>(s->OC) * s->IC * b}, v{bias, fc_pitch(s->OC) * b};
+    rc = check_spans(what, {x, w, v}, {});
+    if (!rc) rc = check_overlaps(what, {x, w, v, {label, rows * label_bytes}}, {{loss, rows * 4}, {lse, rows * 4}});
+    if (!rc) rc = call_begin(static_cast<cudaStream_t>(stream));
+    if (rc) return rc;
+    const Loss c{s, X, W, bias, label, label_bytes, static_cast<cudaStream_t>(stream)};
+    return s->dtype == ALPHA_F32 ? forward_f32(c, loss, lse) : forward_16(c, loss, lse);
+}
+
+int alpha_fullConnect_softmax_crossEntropy_delta(const AlphaFcShape* s, const float* deltaL, int deltaL_step, const void* X, const void* W, const void* bias, const void* label,
+                                                 int label_bytes, const float* lse, void* deltaX, void* deltaW, void* deltaB, alpha_stream_t stream)
+{
+    OpRange range("alpha_fullConnect_softmax_crossEntropy_delta");
+    const char* what = "fullConnect_softmax_crossEntropy_delta";
+    int rc = check_loss(what, s, label, label_bytes);
+    if (rc) return rc;
+    if (!deltaL || !X || !W || !lse) return fail(ALPHA_E_ARG, "%s: null tensor pointer", what);
+    if (!deltaX && !deltaW && !deltaB) return fail(ALPHA_E_ARG, "%s: no gradient asked for", what);
+    if (deltaL_step != 0 && deltaL_step != 1) return fail(ALPHA_E_ARG, "%s: deltaL is one value (step 0) or one for each row (step 1)", what);
+    if ((reinterpret_cast<uintptr_t>(deltaL) | reinterpret_cast<uintptr_t>(lse)) & 3) return fail(ALPHA_E_ARG, "%s: deltaL and lse are floats", what);
+    const size_t b = type_bytes(s->dtype), rows = s->rows, pitch = fc_pitch(s->OC);
+    const Span x{X, rows * s->IC * b}, w{W, static_cast<size_t>(s->OC) * s->IC * b}, v{bias, pitch * b}, dx{deltaX, x.bytes}, dw{deltaW, w.bytes}, db{deltaB, v.bytes};
+    rc = check_spans(what, {x, w, v}, {dx, dw, db});
+    if (!rc) rc = check_overlaps(what, {{label, rows * label_bytes}, {lse, rows * 4}, {deltaL, deltaL_step ? rows * 4 : 4}}, {dx, dw, db});
+    if (!rc) rc = call_begin(static_cast<cudaStream_t>(stream));
+    if (rc) return rc;
+    const Loss c{s, X, W, bias, label, label_bytes, static_cast<cudaStream_t>(stream)};
+    if (s->dtype == ALPHA_F32) return delta_f32(c, deltaL, deltaL_step, lse, static_cast<float*>(deltaX), static_cast<float*>(deltaW), static_cast<float*>(deltaB));
+    if (s->dtype == ALPHA_BF16) return delta_16<__nv_bfloat16>(c, deltaL, deltaL_step, lse, deltaX, deltaW, deltaB);
+    return delta_16<__half>(c, deltaL, deltaL_step, lse, deltaX, deltaW, deltaB);
+}
+
+int alpha_fullConnect_softmax_crossEntropy_workspace_bytes(const AlphaFcShape* s, int op, size_t* bytes)
+{
+    if (!s || !bytes) return fail(ALPHA_E_ARG, "fullConnect_softmax_crossEntropy_workspace_bytes: null argument");
+    if (op != ALPHA_OP_FORWARD && op != ALPHA_OP_DELTAX) return fail(ALPHA_E_ARG, "fullConnect_softmax_crossEntropy_workspace_bytes: unknown op %d", op);
+    // the call itself with launches switched off (tensors at placeholder addresses far apart)
+    auto at = [](int i) { return reinterpret_cast<void*>(static_cast<uintptr_t>(i + 1) << 44); };
+    auto f = [&](int i) { return static_cast<float*>(at(i)); };
+    dry_begin();
+    const int rc = op == ALPHA_OP_FORWARD ? alpha_fullConnect_softmax_crossEntropy(s, at(0), at(1), at(2), at(3), 8, f(4), f(5), nullptr)
+                                          : alpha_fullConnect_softmax_crossEntropy_delta(s, f(0), 1, at(1), at(2), at(3), at(4), 8, f(5), at(6), at(7), at(8), nullptr);
+    *bytes = dry_end();
+    return rc;
+}
+
+}  // extern "C"

@@ -31,6 +31,20 @@ namespace alpha {
 constexpr int kFcThreads = 320, kFcBK = 64, kFcGroupM = 8, kFcMaxStages = 16;
 constexpr uint32_t kFcRing = 196608, kFcStaging = 8 * 4096;              // staging: two buffers of 32 x 32 elements for each epilogue warp
 
+// What becomes of the sums: a layer's outputs; the largest logit of each row and the sum of exponentials about it; the gradient of a softmax's cross
+// entropy with respect to its logits; sums that several products add up in fp32.
+enum FcEpilogueKind : int { kFcLayer, kFcStats, kFcSoftmaxDelta, kFcSum };
+// What the latter three read and write.  A row whose label is not one of the `classes` classes does not count: its gradient is 0.
+struct FcLoss {
+    const void* label; int label_bytes;      // of each row, of 4 or 8 bytes
+    int base, classes;                       // the product's first column among the classes, and how many there are
+    float2* part;                            // [2 n_tiles][rows] (largest, sum), of either half of the epilogue's warps
+    float* at_label;                         // [rows] logits of the labels
+    const float *lse, *grad; int grad_step;  // [rows] logarithms of the sums; gradients of the rows' losses, or (step 0) of all
+    const float* scale;                      // power of two that keeps fp16 gradients of logits normal, and its inverse (or NULL)
+    float* sums;                             // [rows][pitch] of kFcSum, or NULL: one product
+    int first, last;                         // product of those that add up
+};
 struct FcMma {
     int rows, cols;               // outputs: rows of a half, pitch (glu: of a half of Z too)
     int m_tiles, n_tiles, kb;     // tiles, stages of the reduction
@@ -42,16 +56,24 @@ struct FcMma {
     const void *bias, *residual;
     void *Y, *Z;
     int* status;
+    FcLoss loss;
 };
 // Blocks of 64 steps of a stage, and its bytes.
 __host__ __device__ constexpr int fc_blocks(bool pair, int bn) { return pair && bn == 256 ? 1 : 2; }
 __host__ __device__ constexpr uint32_t fc_block_bytes(bool pair, int a_rows, int bn) { return static_cast<uint32_t>(a_rows + (pair ? bn / 2 : bn)) * 128; }
 
+__device__ __forceinline__ float exp2f_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Elements from a row of a tensor to the one `rows` further (a pitch alone may be 2^31 - 1024).
 __host__ __device__ constexpr size_t fc_rows_on(int rows, size_t pitch) { return rows * pitch; }
 
 // PAIR: columns of a pair's tiles, 256 or 128, or 0.  TWO: the tiles of a second product of the same geometry follow those of the first (deltaX and deltaW, neither of which may fill the SMs).
-template <class T, int PAIR, bool GLU, bool TWO>
+template <class T, int PAIR, bool GLU, bool TWO, int EPI>
 __global__ void __launch_bounds__(kFcThreads, 1)
     fc_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ FcMma p, const __grid_constant__ CUtensorMap tmA2,
                   const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ FcMma p2)
@@ -173,7 +195,24 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     auto finish = [&](float (&z)[32], float (&u)[32], const uint4 (&r)[4], int row0, int col0, int width) {
         const T* bias = static_cast<const T*>(cur->bias);
         T *Y = static_cast<T*>(cur->Y) + (hm ? static_cast<size_t>(cur->rows) * cur->cols : 0), *Z = static_cast<T*>(cur->Z);
-        if constexpr (GLU) {
+        if constexpr (EPI == kFcSum) {
+            // (a lane has 128 bytes of its row of the fp32 sums)
+            const FcLoss& l = cur->loss;
+            if (l.sums && row0 + lane < cur->rows) {
+                float* at = l.sums + static_cast<size_t>(row0 + lane) * cur->cols + col0;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    if (4 * q >= width || col0 + 4 * q >= cur->cols) continue;
+                    float4* word = reinterpret_cast<float4*>(at + 4 * q);
+                    if (!l.first) { const float4 v = *word; z[4 * q] += v.x; z[4 * q + 1] += v.y; z[4 * q + 2] += v.z; z[4 * q + 3] += v.w; }
+                    if (!l.last) *word = make_float4(z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]);
+                }
+            }
+            if (l.sums && !l.last) return;
+            const float by = l.scale ? __ldg(l.scale + 1) : 1.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] *= by;
+        } else if constexpr (GLU) {
             if (bias) { add_bias(z, bias, col0); add_bias(u, bias + cur->cols, col0); }
             if (cur->keep_z) {
                 const size_t pitch = 2 * static_cast<size_t>(cur->cols);
@@ -194,6 +233,63 @@ __global__ void __launch_bounds__(kFcThreads, 1)
             if (cur->residual) add_fetched(z, r);
         }
         put(z, Y, cur->cols, row0, col0, width);
+    };
+
+    // The epilogues over classes: a lane has 32 neighbouring logits of a row.
+    float most = 0.f, mass = 0.f, lse = 0.f, grad = 0.f;      // the largest and the sum so far; the row's logarithm and gradient
+    long long label = -1;                                      // its class, counted from the product's first column; else negative
+    auto begin_row = [&](int row) {
+        const FcLoss& l = cur->loss;
+        most = -__int_as_float(0x7f800000);
+        mass = lse = grad = 0.f;
+        label = -1;
+        if (row >= cur->rows) return;
+        label = l.label_bytes == 8 ? __ldg(static_cast<const long long*>(l.label) + row) : __ldg(static_cast<const int*>(l.label) + row);
+        const bool counts = label >= 0 && label < l.classes;
+        if constexpr (EPI == kFcSoftmaxDelta) {
+            lse = __ldg(l.lse + row);
+            if (counts) grad = __ldg(l.grad + static_cast<size_t>(row) * l.grad_step) * (l.scale ? __ldg(l.scale) : 1.f);
+        }
+        label = counts ? label - l.base : -1LL << 40;
+    };
+    constexpr float kLog2e = 1.44269504f;
+    auto stats = [&](float (&z)[32], int row, int col0, int width) {
+        const FcLoss& l = cur->loss;
+        if (cur->bias) add_bias(z, static_cast<const T*>(cur->bias), col0);
+        if (l.base + col0 + width > l.classes) width = l.classes - l.base - col0;
+        if (width < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i >= width) z[i] = -__int_as_float(0x7f800000);
+        }
+        const long long at = label - col0;
+        if (at >= 0 && at < 32 && at < width) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (at == i) l.at_label[row] = z[i];
+        }
+        float m = z[0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) m = fmaxf(m, z[i]);
+        m = fmaxf(m, most);
+        // (a row of -Inf so far: exponentials about 0 are 0, and a NaN among them stays one)
+        const float about = m > -__int_as_float(0x7f800000) ? m : 0.f;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += exp2f_approx((z[i] - about) * kLog2e);
+        mass = fmaf(mass, exp2f_approx((most - about) * kLog2e), s);
+        most = m;
+    };
+    auto softmax_delta = [&](float (&z)[32], int col0) {
+        const FcLoss& l = cur->loss;
+        if (cur->bias) add_bias(z, static_cast<const T*>(cur->bias), col0);
+        const long long at = label - col0;
+        const bool counts = label > -1LL << 40;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float p = exp2f_approx((z[i] - lse) * kLog2e);
+            z[i] = counts && l.base + col0 + i < l.classes ? grad * (at == i ? p - 1.f : p) : 0.f;
+        }
     };
 
     // Both issuing warps walk their loops as a whole, so that counters, coordinates and descriptors are uniform values; one lane issues.
@@ -333,6 +429,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                 }
             };
             bool held = true;
+            if constexpr (EPI == kFcStats || EPI == kFcSoftmaxDelta) begin_row(row0 + lane);
             if (row0 < cur->rows) {
                 if (!PAIR && split > 1) {
                     // the ring is idle: [row][column] with four floats more, so that the words of eight rows lie in different banks
@@ -354,12 +451,17 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                         load32(d + c, z);
                         if constexpr (GLU) load32(d + OUT + c, u);
                         if (c + 64 >= OUT || n0 + c + 64 >= cur->cols) { give_back(); held = false; }
-                        finish(z, u, r, row0, n0 + c, OUT - c);
+                        if constexpr (EPI == kFcStats) stats(z, row0 + lane, n0 + c, OUT - c);
+                        else if constexpr (EPI == kFcSoftmaxDelta) { softmax_delta(z, n0 + c); put(z, static_cast<T*>(cur->Y), cur->cols, row0, n0 + c, OUT - c); }
+                        else finish(z, u, r, row0, n0 + c, OUT - c);
                         if (fetching && c + 64 < OUT) fetch(r, row0, n0 + c + 64, OUT - c - 64);
                     }
                 }
             }
             if (held) give_back();
+            if constexpr (EPI == kFcStats) {
+                if (row0 + lane < cur->rows) cur->loss.part[(static_cast<size_t>(n0 / OUT) * 2 + half) * cur->rows + row0 + lane] = make_float2(most, mass);
+            }
             ap.advance(2);
         }
     }

@@ -37,6 +37,10 @@ int option_fc_tile();
 // nothing is allocated and callers launch nothing.
 int call_begin(cudaStream_t stream);
 int call_scratch(cudaStream_t stream, size_t bytes, void** out);
+// What a call asks for between a mark and its rewind may be used again after it (by kernels that run later on the same stream).
+struct ScratchMark { size_t block, caller, dry; };
+ScratchMark call_mark(cudaStream_t stream);
+void call_rewind(cudaStream_t stream, const ScratchMark& m);
 // Whether `rc` is a refusal of scratch (a capture, a block given by the caller, a full card) that a route with less, or none, may answer.
 bool scratch_refused(int rc);
 bool dry_run();

@@ -321,6 +321,20 @@ class CudaFloat32EngineBase:
         _l.check(fn(C.byref(_fc_shape(rows, IC, OC, dtype, act, k)), a(deltaY_address), a(X_address), a(W_address), a(Z_address), a(deltaZ_address),
                     a(deltaX_address), a(deltaW_address), a(deltaB_address), _stream(self._stream)))
 
+    def fullConnect_softmax_crossEntropy(self, loss_address, lse_address, X_address, W_address, Bias_address, label_address, label_bytes, rows, IC, OC, dtype):
+        """loss = lse - z[label], lse = log sum exp z, z = X W^T + Bias (alpha_fullConnect_softmax_crossEntropy)."""
+        a = self._addr_or_none
+        _l.check(self._lib.alpha_fullConnect_softmax_crossEntropy(C.byref(_fc_shape(rows, IC, OC, dtype, 0, 0.0)), a(X_address), a(W_address), a(Bias_address), a(label_address),
+                                                                  label_bytes, a(loss_address), a(lse_address), _stream(self._stream)))
+
+    def fullConnect_softmax_crossEntropy_delta(self, deltaX_address, deltaW_address, deltaB_address, deltaL_address, deltaL_step, X_address, W_address, Bias_address, label_address,
+                                               label_bytes, lse_address, rows, IC, OC, dtype):
+        """The gradients of fullConnect_softmax_crossEntropy (alpha_fullConnect_softmax_crossEntropy_delta)."""
+        a = self._addr_or_none
+        _l.check(self._lib.alpha_fullConnect_softmax_crossEntropy_delta(C.byref(_fc_shape(rows, IC, OC, dtype, 0, 0.0)), a(deltaL_address), deltaL_step, a(X_address), a(W_address),
+                                                                        a(Bias_address), a(label_address), label_bytes, a(lse_address), a(deltaX_address), a(deltaW_address),
+                                                                        a(deltaB_address), _stream(self._stream)))
+
     # ---- group normalisation (shape: AlphaNormShape) ----
     def groupNorm(self, shape, X_address, gamma_address, beta_address, mean_address, rstd_address, Y_address):
         b, a = self._addr_or_none, self._addr
@@ -842,6 +856,59 @@ class Engine:
     def fullConnect_glu_delta(self, deltaY, X, W, Z, act="silu", k=0.0, bias=False):
         """(deltaX, deltaW, deltaB) of fullConnect_glu from deltaY and its Z; deltaB is None without bias=True."""
         return self._fc_delta("fullConnect_glu_delta", deltaY, X, W, Z, act, k, bias, True)
+
+    # ---- the loss on top of such a layer ----
+    def _loss_call(self, what, X, W, label, Bias, others):
+        """The checked call's plan, and label as dense memory."""
+        plan = _fc_plan(what, False, X.shape, W.shape, X.dtype)
+        device = _fc_check(what, X, W, (("Bias", Bias, plan[8]),) if Bias is not None else ())
+        lead = X.shape[:-1]
+        if label.dtype not in (torch.int64, torch.int32):
+            raise ValueError("%s: label must be int64 or int32, not %s" % (what, label.dtype))
+        for name, t in (("label", label),) + others:
+            if t.shape != lead or t.get_device() != device:
+                raise ValueError("%s: %s %s on %s, expected %s on %s" % (what, name, tuple(t.shape), t.device, tuple(lead), X.device))
+            if name != "label" and t.dtype != torch.float32:
+                raise ValueError("%s: %s must be float32, not %s" % (what, name, t.dtype))
+        return plan
+
+    def fullConnect_softmax_crossEntropy(self, X, W, label, Bias=None, save=False):
+        """The softmax cross entropy of every row of X [..., IC] over the classes of a FullConnect layer, logsumexp(z) - z[label] with z = X W^T + Bias, as float32 [...].
+        The logits are not kept.  W [OC, IC]; label [...] int64 or int32; a row whose label is not in [0, OC) does not count: its loss is 0.  save=True also returns
+        the logsumexp of every row, which fullConnect_softmax_crossEntropy_delta reads."""
+        IC, OC, ic, oc, rows, *_ = self._loss_call("fullConnect_softmax_crossEntropy", X, W, label, Bias, ())
+        with self._on(X), torch.no_grad():
+            loss = _new(X, X.shape[:-1])
+            lse = _new(X, X.shape[:-1]) if save else None
+            if rows:
+                (Xp, Wp, Bp), _held = _fc_pack(X.dtype, (X, 1, rows, IC, rows, ic), (W, 1, OC, IC, OC, ic), (Bias, 1, 1, OC, 1, oc))
+                label = label.contiguous()
+                self.base.fullConnect_softmax_crossEntropy(loss, lse, Xp, Wp, Bp, label, label.element_size(), rows, ic, OC, _FC_TYPES[X.dtype])
+        return (loss, lse) if save else loss
+
+    def fullConnect_softmax_crossEntropy_delta(self, deltaL, X, W, label, lse, Bias=None):
+        """(deltaX, deltaW, deltaB) of fullConnect_softmax_crossEntropy from the gradients of the rows' losses and the lse it saved; deltaB is None without Bias.  deltaL: float32 of
+        the losses' shape, or one number for all (a float, or a tensor of one float32 value)."""
+        what = "fullConnect_softmax_crossEntropy_delta"
+        step = 0
+        if isinstance(deltaL, torch.Tensor) and (deltaL.dim() or X.dim() == 1):
+            step = 1
+        IC, OC, ic, oc, rows, *_ = self._loss_call(what, X, W, label, Bias, (("lse", lse),) + ((("deltaL", deltaL),) if step else ()))
+        if not step and isinstance(deltaL, torch.Tensor) and (deltaL.dtype != torch.float32 or deltaL.get_device() != X.get_device()):
+            raise ValueError("%s: deltaL must be float32 on %s, not %s on %s" % (what, X.device, deltaL.dtype, deltaL.device))
+        with self._on(X), torch.no_grad():
+            if rows == 0:
+                return X.new_empty(X.shape), W.new_zeros(W.shape), None if Bias is None else W.new_zeros((OC,))
+            if not isinstance(deltaL, torch.Tensor):
+                deltaL = torch.full((), float(deltaL), dtype=torch.float32, device=X.device)
+            (Xp, Wp, Bp), _held = _fc_pack(X.dtype, (X, 1, rows, IC, rows, ic), (W, 1, OC, IC, OC, ic), (Bias, 1, 1, OC, 1, oc))
+            label, lse, deltaL = label.contiguous(), _dense(lse), _dense(deltaL)
+            dX, dW = X.new_empty((rows, ic)), W.new_empty((OC, ic))
+            dB = None if Bias is None else W.new_empty((oc,))
+            self.base.fullConnect_softmax_crossEntropy_delta(dX, dW, dB, deltaL, step, Xp, Wp, Bp, label, label.element_size(), lse, rows, ic, OC, _FC_TYPES[X.dtype])
+        if ic != IC:
+            dX, dW = dX.narrow(1, 0, IC), dW.narrow(1, 0, IC)
+        return dX if X.dim() == 2 else dX.reshape(X.shape), dW, None if dB is None else dB if oc == OC else dB.narrow(0, 0, OC)
 
     # ---- all gradients of a step ----
     def _on(self, t):

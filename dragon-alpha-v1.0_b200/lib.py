@@ -166,6 +166,10 @@ def load():
     lib.alpha_fullConnect_workspace_bytes.argtypes = [F, I, I, C.POINTER(C.c_size_t)]
     lib.alpha_grad_norm.argtypes = [I, G, V, V]
     lib.alpha_clip_grad_norm.argtypes = [I, G, C.c_double, V, V]
+    name = "alpha_fullConnect_softmax_crossEntropy"
+    getattr(lib, name).argtypes = [F, V, V, V, V, I, V, V, V]
+    getattr(lib, name + "_delta").argtypes = [F, V, I, V, V, V, V, I, V, V, V, V, V]
+    getattr(lib, name + "_workspace_bytes").argtypes = [F, I, C.POINTER(C.c_size_t)]
     NS = C.POINTER(AlphaNormShape)
     lib.alpha_groupNorm.argtypes = [NS, V, V, V, V, V, V, V]
     lib.alpha_groupNorm_delta.argtypes = [NS, V, V, V, V, V, V, V, V, V, V]
@@ -252,6 +256,13 @@ def fullConnect_workspace_bytes(shape, glu, op):
     """Scratch bytes of a fullConnect (glu: fullConnect_glu) call: op 'forward', or 'deltaX' for that of all gradients."""
     n = C.c_size_t(0)
     check(load().alpha_fullConnect_workspace_bytes(C.byref(shape), int(bool(glu)), OPS[op], C.byref(n)))
+    return n.value
+
+
+def fullConnect_softmax_crossEntropy_workspace_bytes(shape, op):
+    """Scratch bytes of a fullConnect_softmax_crossEntropy call ('forward') or of its gradients' ('deltaX')."""
+    n = C.c_size_t(0)
+    check(load().alpha_fullConnect_softmax_crossEntropy_workspace_bytes(C.byref(shape), OPS[op], C.byref(n)))
     return n.value
 
 

@@ -501,6 +501,26 @@ int alpha_fullConnect_glu_delta(const AlphaFcShape* s, const void* deltaY, const
 /* Scratch of a call, as alpha_conv_workspace_bytes: op ALPHA_OP_FORWARD, or ALPHA_OP_DELTAX for the call of all gradients. */
 int alpha_fullConnect_workspace_bytes(const AlphaFcShape* s, int glu, int op, size_t* bytes);
 
+/* ---- softmax cross entropy on top of a FullConnect layer ----------------------------------------------------------
+ *
+ * The loss of rows over OC classes (a vocabulary) whose logits are not kept:
+ *   z = X W^T + bias,  lse = log sum over classes of exp z,  loss = lse - z[label]
+ * X[rows][IC], W[OC][IC], bias[P] (P = OC rounded up to a multiple of 8; may be NULL) as in alpha_fullConnect (s->act ALPHA_ACT_NONE); label: an integer of
+ * 4 or 8 bytes (label_bytes) for each row.  A row whose label is not in [0, OC) does not count: its loss is 0, and so are its gradients.  loss and lse, floats for
+ * each row; either may be NULL.  A class whose logit is -Inf (a bias of -Inf) has the probability 0.
+ * The gradients, from deltaL (one float for each row with deltaL_step 1, one for all with 0) and the lse of the forward call, logits formed again:
+ *   dz = deltaL (exp(z - lse) - [label]),  deltaX = dz W,  deltaW = dz^T X,  deltaB = column sums of dz      (deltaX, deltaW, deltaB: each may be NULL)
+ * Sums, exponentials and logarithms are fp32; dz is rounded to the tensors' type once (fp16: times a power of two that brings the largest |deltaL| to 2^14 or
+ * above), as the deltaZ of alpha_fullConnect_delta is, and outputs once.  fp32 tensors have fp32 accuracy, and fewer than 2^31 elements (rows x OC among them).
+ * No output may overlap anything else.  Results do not depend on scheduling.  Scratch (the function below): parts of the rows' sums, logits or their
+ * gradients for a piece of the classes (up to 256 MB), fp32 sums of deltaX where there are several. */
+int alpha_fullConnect_softmax_crossEntropy(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* label, int label_bytes, float* loss, float* lse,
+                                           alpha_stream_t stream);
+int alpha_fullConnect_softmax_crossEntropy_delta(const AlphaFcShape* s, const float* deltaL, int deltaL_step, const void* X, const void* W, const void* bias, const void* label,
+                                                 int label_bytes, const float* lse, void* deltaX, void* deltaW, void* deltaB, alpha_stream_t stream);
+/* op ALPHA_OP_FORWARD or ALPHA_OP_DELTAX (all gradients) */
+int alpha_fullConnect_softmax_crossEntropy_workspace_bytes(const AlphaFcShape* s, int op, size_t* bytes);
+
 /* ---- group normalisation -----------------------------------------------------------------------------------------
  *
  * Channels-last tensors X[N][positions][C] of fp32, bf16 or fp16, C channels in `groups` groups of D = C / groups neighbours:
