@@ -18,6 +18,7 @@
 #include "dependent_launch.cuh"
 #include "fc_act.cuh"
 #include "host_common.h"
+#include "pairs.cuh"
 
 #include <cuda_fp8.h>
 
@@ -65,24 +66,24 @@ __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x)
     return x ^ (x >> 16);
 }
 
-// Four elements at a time, as floats.
-struct Four { float f[4]; };
+// Four elements at a time, as two pairs of floats.
+struct Four { float2 f[2]; };
 template <class T> struct FourOf;
 template <> struct FourOf<float> {
     using Raw = float4;
-    static __device__ Four get(const Raw& r) { return Four{{r.x, r.y, r.z, r.w}}; }
-    static __device__ Raw put(const Four& v) { return make_float4(v.f[0], v.f[1], v.f[2], v.f[3]); }
+    static __device__ Four get(const Raw& r) { return Four{{make_float2(r.x, r.y), make_float2(r.z, r.w)}}; }
+    static __device__ Raw put(const Four& v) { return make_float4(v.f[0].x, v.f[0].y, v.f[1].x, v.f[1].y); }
 };
 template <class T> struct FourOf16 {
     using Raw = uint2;
     static __device__ Four get(const Raw& r)
     {
         Four v;
-        unpack16<T>(r.x, v.f[0], v.f[1]);
-        unpack16<T>(r.y, v.f[2], v.f[3]);
+        unpack16<T>(r.x, v.f[0].x, v.f[0].y);
+        unpack16<T>(r.y, v.f[1].x, v.f[1].y);
         return v;
     }
-    static __device__ Raw put(const Four& v) { return make_uint2(pack16<T>(v.f[0], v.f[1]), pack16<T>(v.f[2], v.f[3])); }
+    static __device__ Raw put(const Four& v) { return make_uint2(pack16<T>(v.f[0].x, v.f[0].y), pack16<T>(v.f[1].x, v.f[1].y)); }
 };
 template <> struct FourOf<__nv_bfloat16> : FourOf16<__nv_bfloat16> {};
 template <> struct FourOf<__half> : FourOf16<__half> {};
@@ -92,45 +93,42 @@ __device__ __forceinline__ float2 e4m3_pair(uint32_t codes)
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-__device__ __forceinline__ Four e4m3_get(uint32_t codes)
-{
-    const float2 a = e4m3_pair(codes & 0xffffu), b = e4m3_pair(codes >> 16);
-    return Four{{a.x, a.y, b.x, b.y}};
-}
+__device__ __forceinline__ Four e4m3_get(uint32_t codes) { return Four{{e4m3_pair(codes & 0xffffu), e4m3_pair(codes >> 16)}}; }
 __device__ __forceinline__ uint32_t e4m3_put(const Four& v)
 {
-    return __nv_cvt_float2_to_fp8x2(make_float2(v.f[0], v.f[1]), __NV_SATFINITE, __NV_E4M3)
-         | static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(v.f[2], v.f[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
+    return __nv_cvt_float2_to_fp8x2(v.f[0], __NV_SATFINITE, __NV_E4M3) | static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(v.f[1], __NV_SATFINITE, __NV_E4M3)) << 16;
 }
 // The value of an exponent byte (0: 2^-127, 255: NaN), and the byte of a block whose largest magnitude is `most`.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte == 0 ? 0x400000u : byte == 255 ? 0x7fc00000u : byte << 23); }
 __device__ __forceinline__ uint32_t scale_for(float most)
 {
-    const uint32_t bits = __float_as_uint(most);
-    const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);       // 448 = 1.75 * 2^8
-    return static_cast<uint32_t>(e < 1 ? 1 : e > 254 ? 254 : e);
+    // the exponent of most / 448, up where its mantissa is above 1.75 (448 = 1.75 * 2^8): adding 2^21 - 1 to the bits carries into it then
+    const int e = static_cast<int>((__float_as_uint(most) + 0x1fffffu) >> 23) - 8;
+    return static_cast<uint32_t>(e < 1 ? 1 : e);
 }
-// y, at most 448, to one of the codes beside it; `random` of 16 bits.  Below 2^-6 codes are 2^-9 apart, as they are from there to 2^-5.
+// y, at most 448, to one of the codes beside it; `random` of 16 bits, times 16.  Codes are 2^-9 apart below 2^-6, as they are from there to 2^-5: such a y is moved there
+// first.  (The sign is the top bit, which no carry reaches.)  FLOOR: of a y that is not negative, and if it is not 0 nor is its code.
 template <bool FLOOR> __device__ __forceinline__ float round_e4m3(float y, uint32_t random)
 {
-    float a = fabsf(y);
-    const float shift = a < 0x1p-6f ? 0x1p-6f : 0.f;
-    a = __uint_as_float((__float_as_uint(__fadd_rn(a, shift)) + (random << 4)) & ~0xfffffu) - shift;
-    if (FLOOR && y > 0.f) a = fmaxf(a, 0x1p-9f);
-    return copysignf(a, y);
+    const float shift = fabsf(y) < 0x1p-6f ? (FLOOR ? 0x1p-6f : copysignf(0x1p-6f, y)) : 0.f;
+    const float a = __uint_as_float((__float_as_uint(__fadd_rn(y, shift)) + random) & ~0xfffffu) - shift;
+    if (!FLOOR) return a;
+    return y > 0.f ? fmaxf(a, 0x1p-9f) : a;
 }
 
 // What a launch's elements have in common.
 struct AdamUse { float b1, b1c, b2, b2c, eps, size, root, c; };
 
-struct AdamNew { float p, m, v; };
-__device__ __forceinline__ AdamNew adam_element(const AdamUse& u, float keep, float p, float g, float m, float v)
+__device__ __forceinline__ float sqrt_approx(float x) { float y; asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// Two elements: p, m and v are replaced.
+__device__ __forceinline__ void adam_pair(const AdamUse& u, float keep, float2& p, float2 g, float2& m, float2& v)
 {
-    g = __fmul_rn(g, u.c);
-    m = __fadd_rn(__fmul_rn(m, u.b1), __fmul_rn(g, u.b1c));
-    v = __fadd_rn(__fmul_rn(v, u.b2), __fmul_rn(__fmul_rn(g, g), u.b2c));
-    const float by = fmaf(sqrtf(v), u.root, u.eps);
-    return AdamNew{fmaf(p, keep, -__fdividef(m, by) * u.size), m, v};
+    g = mul2(g, twice(u.c));
+    m = add2(mul2(m, twice(u.b1)), mul2(g, twice(u.b1c)));
+    v = add2(mul2(v, twice(u.b2)), mul2(mul2(g, g), twice(u.b2c)));
+    const float2 by = fma2(make_float2(sqrt_approx(v.x), sqrt_approx(v.y)), twice(u.root), twice(u.eps));
+    p = fma2(mul2(m, make_float2(rcp_approx(by.x), rcp_approx(by.y))), twice(-u.size), mul2(p, twice(keep)));
 }
 
 template <class F> __device__ __forceinline__ void with_type(int type, F&& f)
@@ -205,7 +203,7 @@ __device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamUse& 
             v[i] = e4m3_get(vc[i]);
             const float a = scale_of(ms[i]), b = scale_of(vs[i]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { m[i].f[j] *= a; v[i].f[j] *= b; }
+            for (int j = 0; j < 2; ++j) { m[i].f[j] = mul2(m[i].f[j], twice(a)); v[i].f[j] = mul2(v[i].f[j], twice(b)); }
         }
     } else {
         get_typed<float>(m, t.m, first);
@@ -216,10 +214,7 @@ __device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamUse& 
 #pragma unroll
     for (int i = 0; i < kAdamRows; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const AdamNew e = adam_element(u, keep, p[i].f[j], g[i].f[j], m[i].f[j], v[i].f[j]);
-            p[i].f[j] = e.p; m[i].f[j] = e.m; v[i].f[j] = e.v;
-        }
+        for (int j = 0; j < 2; ++j) adam_pair(u, keep, p[i].f[j], g[i].f[j], m[i].f[j], v[i].f[j]);
     put_rows(t.p, first, t.type, p);
     if (t.out_type != kNoType) put_rows(t.out, first, t.out_type, p);
     if constexpr (!EIGHT) {
@@ -227,25 +222,27 @@ __device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamUse& 
         put_rows(t.v, first, ALPHA_F32, v);
         return;
     }
+    uint32_t* mc = reinterpret_cast<uint32_t*>(t.m) + first / 4;
+    uint32_t* vc = reinterpret_cast<uint32_t*>(t.v) + first / 4;
+    uint8_t *ms = t.m_scale + first / kAdamBlock, *vs = t.v_scale + first / kAdamBlock;
 #pragma unroll
     for (int i = 0; i < kAdamRows; ++i) {
-        const long long at = first + i * kAdamRow;
-        float mm = 0.f, vm = 0.f;
+        const float mm = fmaxf(fmaxf(fabsf(m[i].f[0].x), fabsf(m[i].f[0].y)), fmaxf(fabsf(m[i].f[1].x), fabsf(m[i].f[1].y)));
+        const float vm = fmaxf(fmaxf(v[i].f[0].x, v[i].f[0].y), fmaxf(v[i].f[1].x, v[i].f[1].y));
+        const uint32_t a = scale_for(most_of<8>(mm)), b = scale_for(most_of<8>(vm)), at = static_cast<uint32_t>(first) + i * kAdamRow;
+        const float2 ai = twice(__uint_as_float((254u - a) << 23)), bi = twice(__uint_as_float((254u - b) << 23));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { mm = fmaxf(mm, fabsf(m[i].f[j])); vm = fmaxf(vm, v[i].f[j]); }
-        const uint32_t a = scale_for(most_of<8>(mm)), b = scale_for(most_of<8>(vm));
-        const float ai = __uint_as_float((254u - a) << 23), bi = __uint_as_float((254u - b) << 23);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t random = mix32((static_cast<uint32_t>(at) + j) ^ key);
-            m[i].f[j] = round_e4m3<false>(m[i].f[j] * ai, random & 0xffffu);
-            v[i].f[j] = round_e4m3<true>(v[i].f[j] * bi, random >> 16);
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t r0 = mix32((at + 2 * j) ^ key), r1 = mix32((at + 2 * j + 1) ^ key);
+            const float2 x = mul2(m[i].f[j], ai), y = mul2(v[i].f[j], bi);
+            m[i].f[j] = make_float2(round_e4m3<false>(x.x, (r0 << 4) & 0xffff0u), round_e4m3<false>(x.y, (r1 << 4) & 0xffff0u));
+            v[i].f[j] = make_float2(round_e4m3<true>(y.x, (r0 >> 12) & 0xffff0u), round_e4m3<true>(y.y, (r1 >> 12) & 0xffff0u));
         }
-        __stcs(reinterpret_cast<uint32_t*>(t.m) + at / 4, e4m3_put(m[i]));
-        __stcs(reinterpret_cast<uint32_t*>(t.v) + at / 4, e4m3_put(v[i]));
+        __stcs(mc + i * kAdamThreads, e4m3_put(m[i]));
+        __stcs(vc + i * kAdamThreads, e4m3_put(v[i]));
         if ((threadIdx.x & 7) == 0) {
-            t.m_scale[at / kAdamBlock] = static_cast<uint8_t>(a);
-            t.v_scale[at / kAdamBlock] = static_cast<uint8_t>(b);
+            ms[i * (kAdamRow / kAdamBlock)] = static_cast<uint8_t>(a);
+            vs[i * (kAdamRow / kAdamBlock)] = static_cast<uint8_t>(b);
         }
     }
 }
@@ -258,32 +255,33 @@ __device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u,
     for (long long at = begin + (threadIdx.x & ~31u); at < end; at += kAdamThreads) {
         const long long e = at + (threadIdx.x & 31);
         const bool in = e < end;
-        AdamNew x{0.f, 0.f, 0.f};
+        float2 p{0.f, 0.f}, m = p, v = p;                    // (the second of each pair is 0 and goes nowhere)
         if (in) {
-            float m, v;
             if constexpr (EIGHT) {
-                m = e4m3_pair(static_cast<const uint8_t*>(t.m)[e]).x * scale_of(t.m_scale[e / kAdamBlock]);
-                v = e4m3_pair(static_cast<const uint8_t*>(t.v)[e]).x * scale_of(t.v_scale[e / kAdamBlock]);
+                m.x = e4m3_pair(static_cast<const uint8_t*>(t.m)[e]).x * scale_of(t.m_scale[e / kAdamBlock]);
+                v.x = e4m3_pair(static_cast<const uint8_t*>(t.v)[e]).x * scale_of(t.v_scale[e / kAdamBlock]);
             } else {
-                m = static_cast<const float*>(t.m)[e];
-                v = static_cast<const float*>(t.v)[e];
+                m.x = static_cast<const float*>(t.m)[e];
+                v.x = static_cast<const float*>(t.v)[e];
             }
-            x = adam_element(u, keep, get_one(t.p, e, t.type), get_one(t.g, e, t.grad_type), m, v);
-            put_one(t.p, e, t.type, x.p);
-            if (t.out_type != kNoType) put_one(t.out, e, t.out_type, x.p);
+            p.x = get_one(t.p, e, t.type);
+            adam_pair(u, keep, p, make_float2(get_one(t.g, e, t.grad_type), 0.f), m, v);
+            put_one(t.p, e, t.type, p.x);
+            if (t.out_type != kNoType) put_one(t.out, e, t.out_type, p.x);
         }
         if constexpr (!EIGHT) {
             if (in) {
-                static_cast<float*>(t.m)[e] = x.m;
-                static_cast<float*>(t.v)[e] = x.v;
+                static_cast<float*>(t.m)[e] = m.x;
+                static_cast<float*>(t.v)[e] = v.x;
             }
             continue;
         }
-        const uint32_t a = scale_for(most_of<32>(fabsf(x.m))), b = scale_for(most_of<32>(x.v));     // (and a barrier of the warp: the old scales have been read)
+        const uint32_t a = scale_for(most_of<32>(fabsf(m.x))), b = scale_for(most_of<32>(v.x));     // (and a barrier of the warp: the old scales have been read)
         const uint32_t random = mix32(static_cast<uint32_t>(e) ^ key);
-        const float m = round_e4m3<false>(x.m * __uint_as_float((254u - a) << 23), random & 0xffffu), v = round_e4m3<true>(x.v * __uint_as_float((254u - b) << 23), random >> 16);
+        m.x = round_e4m3<false>(m.x * __uint_as_float((254u - a) << 23), (random << 4) & 0xffff0u);
+        v.x = round_e4m3<true>(v.x * __uint_as_float((254u - b) << 23), (random >> 12) & 0xffff0u);
         if (in) {
-            const uint32_t codes = e4m3_put(Four{{m, v, 0.f, 0.f}});
+            const uint32_t codes = e4m3_put(Four{{make_float2(m.x, v.x), make_float2(0.f, 0.f)}});
             static_cast<uint8_t*>(t.m)[e] = static_cast<uint8_t>(codes);
             static_cast<uint8_t*>(t.v)[e] = static_cast<uint8_t>(codes >> 8);
             if ((threadIdx.x & 31) == 0) {
@@ -295,7 +293,7 @@ __device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u,
 }
 
 template <bool EIGHT>
-__global__ void __launch_bounds__(kAdamThreads, EIGHT ? 4 : 3) adamw_kernel(const __grid_constant__ AdamTable table, const __grid_constant__ AdamStep s)
+__global__ void __launch_bounds__(kAdamThreads, 3) adamw_kernel(const __grid_constant__ AdamTable table, const __grid_constant__ AdamStep s)
 {
     __shared__ float shared[2];
     grid_dependency_wait();
@@ -413,7 +411,7 @@ int run_adamw(int n, const AlphaAdamW* list, const AlphaAdamWStep* s, cudaStream
     t.n = 0;
     long long chunks = 0;
     const bool eight = n && list[0].moment_bits == 8;
-    const long long most = sms * (eight ? 4LL : 3LL);
+    const long long most = sms * 3LL;
     for (int i = 0; i <= n; ++i) {
         long long more = 0;
         if (i < n) {

@@ -35,13 +35,21 @@ Norm norm_of(const AlphaNormShape* s)
     return p;
 }
 
-// The slab and the cluster of least estimated time; false: no slab fits.
-bool plan_resident(Norm& p, int V, bool back, int sms, size_t* smem)
+// us of a wave of CTAs with `elements` each, `at_once` of them on an SM: what an SM takes in and gives out (45 KB a us), its instructions beside that
+// where there are several CTAs, after it where there is one; and what a CTA waits for whatever it holds.
+double norm_time(bool back, int size, double elements, int at_once, double narrow, int cl)
 {
-    const long long unit = static_cast<long long>(p.D) * V / std::gcd(p.D, V);
-    if (unit / V > kNormThreads || p.C % V) return false;
-    const int unit_words = static_cast<int>(unit / V), units = static_cast<int>(p.C / unit);
-    double least = 1e300;
+    const double memory = at_once * elements * size * (back ? 3 : 2) / 45e3 * narrow, math = at_once * elements * (back ? 18.0 : 12.0) / 32 / 4000.0;
+    const double hidden = at_once == 1 ? 0.0 : at_once == 2 ? 0.6 : 0.8;
+    return 2.5 + 0.3 * cl + std::max(memory, math) + (1.0 - hidden) * std::min(memory, math);
+}
+// The slab and the cluster of least estimated time (us); false: no slab fits.
+bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* least)
+{
+    const long long unit = static_cast<long long>(p.D) * 4 / std::gcd(p.D, 4);
+    *least = 1e300;
+    if (unit / 4 > kNormThreads || p.C % 4) return false;
+    const int unit_words = static_cast<int>(unit / 4), units = static_cast<int>(p.C / unit);
     for (int each = 1; each <= kNormThreads / unit_words && each <= units; ++each) {
         if (units % each) continue;
         const int words = unit_words * each, slabs = units / each;
@@ -49,20 +57,20 @@ bool plan_resident(Norm& p, int V, bool back, int sms, size_t* smem)
             const int part = (p.R + cl - 1) / cl;
             const long long ctas = static_cast<long long>(p.N) * slabs * cl;
             if (static_cast<long long>(cl - 1) * part >= p.R || part > (1 << 20) || ctas > 2147483647LL) continue;
-            const size_t bytes = norm_smem(back, V, part, words, words * V / p.D);
+            const size_t bytes = norm_smem(back, size, part, words, words * 4 / p.D) + 16;
             if (bytes > 224 * 1024) continue;
-            const double at_once = std::min(2.0, static_cast<double>(static_cast<int>(227 * 1024 / (bytes + 1024)))), waves = std::max(1.0, ctas / (sms * at_once));
-            // us: what a CTA waits for besides its bytes, and its share of the bytes an SM takes in and gives out
-            const double narrow = words >= 4 ? 1.0 : words == 2 ? 1.15 : words == 1 ? 1.6 : 1.1;
-            const double time = waves * (3.0 + 0.4 * cl + at_once * part * words * 16.0 * (back ? 3 : 2) / 45e3 * narrow);
-            if (time < least) {
-                least = time;
-                p.words = words; p.slabs = slabs; p.cluster = cl; p.part = part; p.rows = kNormThreads / p.words;
+            const int fit = static_cast<int>(227 * 1024 / (bytes + 1024)), at_once = fit < 4 ? fit : 4;
+            const double elements = static_cast<double>(part) * words * 4, waves = std::max(1.0, static_cast<double>(ctas) / (sms * at_once));
+            const double row = words * 4.0 * size, narrow = row >= 64 ? 1.0 : row >= 32 ? 1.15 : 2.0;
+            const double time = norm_time(back, size, elements, at_once, narrow, cl) * waves;
+            if (time < *least) {
+                *least = time;
+                p.words = words; p.slabs = slabs; p.cluster = cl; p.part = part; p.rows = kNormThreads / words;
                 *smem = bytes;
             }
         }
     }
-    return least < 1e300;
+    return *least < 1e300;
 }
 // Column blocks of up to 64 words, and runs of positions that fill the SMs.
 void plan_streamed(Norm& p, int V, int sms)
@@ -73,7 +81,7 @@ void plan_streamed(Norm& p, int V, int sms)
     p.blocks = (words + p.words - 1) / p.words;
     p.rows = kNormThreads / p.words;
     const long long others = static_cast<long long>(p.N) * p.blocks, least = 8LL * p.rows;        // positions of a run
-    long long runs = std::max(1LL, 16LL * sms / others);
+    long long runs = std::max(1LL, 8LL * sms / others);
     runs = std::min(runs, std::max(1LL, p.R / least));
     p.part = static_cast<int>((p.R + runs - 1) / runs);
     p.runs = (p.R + p.part - 1) / p.part;
@@ -81,15 +89,19 @@ void plan_streamed(Norm& p, int V, int sms)
 
 template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgamma, void* dbeta, cudaStream_t stream)
 {
-    constexpr int V = Word16<T>::N;
     int sms = 0;
     int rc = call_begin(stream);
     if (!rc) rc = device_sms(&sms);
     if (rc) return rc;
-    const bool words = p.C % V == 0 && aligned(p.X, 16) && aligned(p.out, 16) && aligned(p.dY, 16);
+    const size_t word = 4 * sizeof(T);
+    const bool words = p.C % 4 == 0 && aligned(p.X, word) && aligned(p.out, word) && aligned(p.dY, word);
+    // streamed: both passes over the tensors, the second through L2 as far as that holds them, and two more launches
+    const double bytes = static_cast<double>(p.N) * p.R * p.C * sizeof(T) * (BACK ? 2 : 1), rate = 45e3 * sms;
+    const double streamed = 8.0 + bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate;
     size_t smem = 0;
-    const bool resident = words && plan_resident(p, V, BACK, sms, &smem);
-    if (!resident) plan_streamed(p, words ? V : 1, sms);
+    double least = 0.0;
+    const bool resident = words && plan_resident(p, sizeof(T), BACK, sms, &smem, &least) && least < streamed;
+    if (!resident) plan_streamed(p, words ? 4 : 1, sms);
     void* ws = nullptr;
     auto scratch = [&](size_t bytes) { return rc = rc ? rc : call_scratch(stream, bytes, &ws); };
     if (BACK && !scratch(static_cast<size_t>(p.N) * p.C * sizeof(float2))) p.sums = static_cast<float2*>(ws);
@@ -106,16 +118,16 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
         const long long ctas = static_cast<long long>(p.N) * p.runs * p.blocks;
         if (ctas > 2147483647LL) return fail(ALPHA_E_ARG, "%s: more CTAs than a launch takes", what);
         const unsigned grid = static_cast<unsigned>(ctas);
-        if (words) launch_after(norm_sums_kernel<T, V, BACK>, grid, kNormThreads, 0, stream, p);
+        if (words) launch_after(norm_sums_kernel<T, 4, BACK>, grid, kNormThreads, 0, stream, p);
         else launch_after(norm_sums_kernel<T, 1, BACK>, grid, kNormThreads, 0, stream, p);
         note_launch("norm");
         rc = launched("norm_sums_kernel");
         if (rc) return rc;
-        launch_after(norm_join_kernel<T, BACK>, static_cast<unsigned>(p.N * p.G), kNormThreads, 0, stream, p);
+        launch_after(norm_join_kernel<T, BACK>, static_cast<unsigned>(p.N * p.G), kJoinNormThreads, 0, stream, p);
         note_launch("norm");
         rc = launched("norm_join_kernel");
         if (rc) return rc;
-        if (words) launch_after(norm_apply_kernel<T, V, BACK>, grid, kNormThreads, 0, stream, p);
+        if (words) launch_after(norm_apply_kernel<T, 4, BACK>, grid, kNormThreads, 0, stream, p);
         else launch_after(norm_apply_kernel<T, 1, BACK>, grid, kNormThreads, 0, stream, p);
         note_launch("norm");
         note_plan("norm streamed words=%d runs=%d part=%d", p.words, p.runs, p.part);
