@@ -125,8 +125,10 @@ __device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.
 __device__ __forceinline__ void adam_pair(const AdamUse& u, float keep, float2& p, float2 g, float2& m, float2& v)
 {
     g = mul2(g, twice(u.c));
-    m = add2(mul2(m, twice(u.b1)), mul2(g, twice(u.b1c)));
-    v = add2(mul2(v, twice(u.b2)), mul2(mul2(g, g), twice(u.b2c)));
+    // (sums one by one: the assembler fuses a packed product with a packed sum, whatever their rounding)
+    const float2 m0 = mul2(m, twice(u.b1)), m1 = mul2(g, twice(u.b1c)), v0 = mul2(v, twice(u.b2)), v1 = mul2(mul2(g, g), twice(u.b2c));
+    m = make_float2(__fadd_rn(m0.x, m1.x), __fadd_rn(m0.y, m1.y));
+    v = make_float2(__fadd_rn(v0.x, v1.x), __fadd_rn(v0.y, v1.y));
     const float2 by = fma2(make_float2(sqrt_approx(v.x), sqrt_approx(v.y)), twice(u.root), twice(u.eps));
     p = fma2(mul2(m, make_float2(rcp_approx(by.x), rcp_approx(by.y))), twice(-u.size), mul2(p, twice(keep)));
 }

@@ -3,10 +3,17 @@
 #include "host_checks.h"
 
 #include <algorithm>
+#include <cmath>
 #include <numeric>
 
 using namespace alpha;
 
+#ifdef NORM_DEV
+#include <cstdlib>
+#define NORM_FORCE(w, c) (!getenv("NW") || (w == atoi(getenv("NW")) && c == atoi(getenv("NC"))))
+#else
+#define NORM_FORCE(w, c) true
+#endif
 namespace {
 
 int check_norm(const char* what, const AlphaNormShape* s)
@@ -35,15 +42,15 @@ Norm norm_of(const AlphaNormShape* s)
     return p;
 }
 
-// us of a wave of CTAs with `elements` each, `at_once` of them on an SM: what an SM takes in and gives out (45 KB a us), its instructions beside that
-// where there are several CTAs, after it where there is one; and what a CTA waits for whatever it holds.
-double norm_time(bool back, int size, double elements, int at_once, double narrow, int cl)
+// Instructions an element takes: in the passes over shared memory, and in the streamed ones.
+double norm_instructions(const Norm& p, bool back, bool streamed)
 {
-    const double memory = at_once * elements * size * (back ? 3 : 2) / 45e3 * narrow, math = at_once * elements * (back ? 18.0 : 12.0) / 32 / 4000.0;
-    const double hidden = at_once == 1 ? 0.0 : at_once == 2 ? 0.6 : 0.8;
-    return 2.5 + 0.3 * cl + std::max(memory, math) + (1.0 - hidden) * std::min(memory, math);
+    const bool plain = p.act == ALPHA_ACT_NONE || p.act == ALPHA_ACT_LEAKY_RELU;
+    return streamed ? (back ? (plain ? 26.0 : 42.0) : (plain ? 17.0 : 23.0)) : (back ? (plain ? 14.0 : 22.0) : (plain ? 9.0 : 15.0));
 }
-// The slab and the cluster of least estimated time (us); false: no slab fits.
+// The slab and the cluster of least estimated time (us); false: no slab fits.  A CTA takes of its SM what its bytes take at 45 KB a us or its instructions at 4000 a us (of a
+// warp), whichever is more - both, and its loads' latency, where it is alone there - and its sums and barriers, 0.9 us (backward 2) and 0.1 for each CTA of the cluster.
+// Measured / estimated over 35 plans of five tensors: 0.98 with a deviation of 12 %.
 bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* least)
 {
     const long long unit = static_cast<long long>(p.D) * 4 / std::gcd(p.D, 4);
@@ -57,13 +64,19 @@ bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* 
             const int part = (p.R + cl - 1) / cl;
             const long long ctas = static_cast<long long>(p.N) * slabs * cl;
             if (static_cast<long long>(cl - 1) * part >= p.R || part > (1 << 20) || ctas > 2147483647LL) continue;
-            const size_t bytes = norm_smem(back, size, part, words, words * 4 / p.D) + 16;
+            const size_t bytes = norm_smem(back, size, part, words, words * 4 / p.D, cl);
             if (bytes > 224 * 1024) continue;
-            const int fit = static_cast<int>(227 * 1024 / (bytes + 1024)), at_once = fit < 4 ? fit : 4;
-            const double elements = static_cast<double>(part) * words * 4, waves = std::max(1.0, static_cast<double>(ctas) / (sms * at_once));
-            const double row = words * 4.0 * size, narrow = row >= 64 ? 1.0 : row >= 32 ? 1.15 : 2.0;
-            const double time = norm_time(back, size, elements, at_once, narrow, cl) * waves;
-            if (time < *least) {
+            const int fit = static_cast<int>(227 * 1024 / (bytes + 1024)), most = 1024 / kNormThreads, at_once = fit < most ? fit : most;
+            const double elements = static_cast<double>(part) * words * 4, places = sms * at_once * (cl < 4 ? 1.0 : 0.9);
+            const double row = words * 4.0 * size, narrow = row >= 64 ? 1.0 : row >= 32 ? 1.1 : 2.0;
+            const double memory = elements * size * (back ? 3 : 2) / 45e3 * narrow, math = elements * norm_instructions(p, back, false) / 32 / 4000.0;
+            const double alone = at_once == 1 ? 1.0 : at_once == 2 ? 0.4 : 0.0;
+            const double each_cta = std::max(memory, math) + alone * (std::min(memory, math) + 1.5) + (back ? 2.0 : 0.9) + 0.1 * cl;
+            // (what is there at once runs at once, in whole waves as long as these are few)
+            const double waves = ctas / places, rounds = waves <= 1.0 ? 1.0 : waves < 4.0 ? std::ceil(waves) * 0.5 + waves * 0.5 : waves;
+            const double on_sm = waves <= 1.0 ? std::max(1.0, std::ceil(static_cast<double>(ctas) / sms)) : at_once;
+            const double time = 4.0 + rounds * on_sm * each_cta;
+            if (NORM_FORCE(words, cl) && time < *least) {
                 *least = time;
                 p.words = words; p.slabs = slabs; p.cluster = cl; p.part = part; p.rows = kNormThreads / words;
                 *smem = bytes;
@@ -72,16 +85,19 @@ bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* 
     }
     return *least < 1e300;
 }
-// Column blocks of up to 64 words, and runs of positions that fill the SMs.
+// Column blocks of up to 64 words, of whole groups where one fits, and runs of positions that fill the SMs once.
 void plan_streamed(Norm& p, int V, int sms)
 {
     const int words = p.C / V;
+    const long long unit = p.D / std::gcd(p.D, V);                   // words of the fewest whole groups
+    p.whole = unit <= 64;
     p.blocks = (words + 63) / 64;
     p.words = (words + p.blocks - 1) / p.blocks;
+    if (p.whole) p.words = static_cast<int>(p.words < unit ? unit : p.words / unit * unit);
     p.blocks = (words + p.words - 1) / p.words;
     p.rows = kNormThreads / p.words;
     const long long others = static_cast<long long>(p.N) * p.blocks, least = 8LL * p.rows;        // positions of a run
-    long long runs = std::max(1LL, 8LL * sms / others);
+    long long runs = std::max(1LL, 4LL * sms / others);
     runs = std::min(runs, std::max(1LL, p.R / least));
     p.part = static_cast<int>((p.R + runs - 1) / runs);
     p.runs = (p.R + p.part - 1) / p.part;
@@ -97,14 +113,22 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
     const bool words = p.C % 4 == 0 && aligned(p.X, word) && aligned(p.out, word) && aligned(p.dY, word);
     // streamed: both passes over the tensors, the second through L2 as far as that holds them, and two more launches
     const double bytes = static_cast<double>(p.N) * p.R * p.C * sizeof(T) * (BACK ? 2 : 1), rate = 45e3 * sms;
-    const double streamed = 8.0 + bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate;
+    const double math = static_cast<double>(p.N) * p.R * p.C * norm_instructions(p, BACK, true) / 32 / (3800.0 * sms);
+    const double streamed = (NORM_FORCE(-1, -1) ? 14.0 : 1e9) + std::max(math, bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate);
     size_t smem = 0;
     double least = 0.0;
     const bool resident = words && plan_resident(p, sizeof(T), BACK, sms, &smem, &least) && least < streamed;
-    if (!resident) plan_streamed(p, words ? 4 : 1, sms);
+    if (!resident) { plan_streamed(p, words ? 4 : 1, sms); p.cluster = 1; }
+    p.by_words = fast_div(p.words); p.by_D = fast_div(p.D);
+    if (resident) {
+        p.groups = p.words * 4 / p.D;
+        p.slots = p.D % 4 == 0 ? 1 : p.D == 2 ? 2 : 4;
+        p.span = p.D * p.slots / 4 > 0 ? p.D * p.slots / 4 : 1;
+        p.by_slabs = fast_div(p.slabs); p.by_cluster = fast_div(p.cluster); p.by_span = fast_div(p.span);
+    }
     void* ws = nullptr;
     auto scratch = [&](size_t bytes) { return rc = rc ? rc : call_scratch(stream, bytes, &ws); };
-    if (BACK && !scratch(static_cast<size_t>(p.N) * p.C * sizeof(float2))) p.sums = static_cast<float2*>(ws);
+    if (BACK && !scratch(static_cast<size_t>(p.N) * p.cluster * p.C * sizeof(float2))) p.sums = static_cast<float2*>(ws);
     if (!resident && !scratch(static_cast<size_t>(p.N) * p.G * sizeof(float2))) p.group = static_cast<float2*>(ws);
     if (!resident && !scratch(static_cast<size_t>(p.N) * p.runs * p.C * sizeof(float2))) p.partial = static_cast<float2*>(ws);
     if (rc || dry_run()) return rc;
@@ -118,8 +142,13 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
         const long long ctas = static_cast<long long>(p.N) * p.runs * p.blocks;
         if (ctas > 2147483647LL) return fail(ALPHA_E_ARG, "%s: more CTAs than a launch takes", what);
         const unsigned grid = static_cast<unsigned>(ctas);
-        if (words) launch_after(norm_sums_kernel<T, 4, BACK>, grid, kNormThreads, 0, stream, p);
-        else launch_after(norm_sums_kernel<T, 1, BACK>, grid, kNormThreads, 0, stream, p);
+        auto by = [&](auto width) {
+            constexpr int V = decltype(width)::value;
+            constexpr size_t ring = NormRows<T, V, BACK>::kBytes, sums = 2 * V * kNormThreads * sizeof(float);
+            launch_after(norm_sums_kernel<T, V, BACK>, grid, kNormThreads, ring > sums ? ring : sums, stream, p);
+        };
+        if (words) by(std::integral_constant<int, 4>{});
+        else by(std::integral_constant<int, 1>{});
         note_launch("norm");
         rc = launched("norm_sums_kernel");
         if (rc) return rc;
@@ -127,14 +156,14 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
         note_launch("norm");
         rc = launched("norm_join_kernel");
         if (rc) return rc;
-        if (words) launch_after(norm_apply_kernel<T, 4, BACK>, grid, kNormThreads, 0, stream, p);
+        if (words) launch_after(norm_apply_kernel<T, 4, BACK>, grid, kNormThreads, NormRows<T, 4, BACK>::kBytes, stream, p);
         else launch_after(norm_apply_kernel<T, 1, BACK>, grid, kNormThreads, 0, stream, p);
         note_launch("norm");
         note_plan("norm streamed words=%d runs=%d part=%d", p.words, p.runs, p.part);
         rc = launched("norm_apply_kernel");
     }
     if (rc || !dgamma) return rc;
-    launch_after(norm_affine_kernel<T>, (p.C + 31) / 32, 256, 0, stream, p.sums, p.N, p.C, dgamma, dbeta, p.affine_f32);
+    launch_after(norm_affine_kernel<T>, (p.C + 31) / 32, 256, 0, stream, p.sums, p.N * p.cluster, p.C, dgamma, dbeta, p.affine_f32);
     note_launch("norm");
     return launched("norm_affine_kernel");
 }

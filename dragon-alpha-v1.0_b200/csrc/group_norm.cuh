@@ -19,13 +19,19 @@
 // difference of large sums.  Sums are fp32, joined in a fixed order.
 #pragma once
 #include "dependent_launch.cuh"
+#include "fast_div.cuh"
 #include "fc_act.cuh"
 #include "pairs.cuh"
 #include "sm100_ptx.cuh"
 
+#include <type_traits>
+
 namespace alpha {
 
-constexpr int kNormThreads = 256;
+#ifndef NORM_T
+#define NORM_T 256
+#endif
+constexpr int kNormThreads = NORM_T;
 
 struct Norm {
     const void *X, *dY;
@@ -33,15 +39,19 @@ struct Norm {
     const void *gamma, *beta;       // (or NULL: 1 and 0)
     int affine_f32;                 // gamma and beta are floats
     float *mean, *rstd;             // [N][G]: written by a forward call (may be NULL), read by a backward one
-    float2* sums;                   // [N][C] sums of dz and dz xh
+    float2* sums;                   // [N][cluster][C] sums of dz and dz xh
     int N, R, C, G, D;
     float eps, k;
     int act;
     // resident: words of a slab, slabs of a row, CTAs that share a slab, positions of each, rows of threads
     int words, slabs, cluster, part, rows;
+    int groups;                     // of a slab
+    int slots, span;                // sums of a word that belong to different groups (1, 2 or 4), and how many of a row a group has
+    FastDiv by_words, by_slabs, by_cluster, by_D, by_span;
     // streamed: column blocks of `words` words, runs of `part` positions
     int blocks, runs;
-    float2* partial;                // [N][runs][C] mean and sum of squared differences, or sums of dz and dz xh
+    int whole;                      // forward: a column block holds whole groups, whose partial sums are kept and not those of channels
+    float2* partial;                // [N][runs][C, or G] mean and sum of squared differences, or sums of dz and dz xh
     float2* group;                  // [N][G] mean and rstd, or s1 and s2
 };
 
@@ -109,9 +119,21 @@ template <class T, int V> __device__ __forceinline__ void load_affine(const Norm
 {
 #pragma unroll
     for (int j = 0; j < (V + 1) / 2; ++j) {
-        gamma[j] = make_float2(affine_at<T>(p.gamma, c + 2 * j, p.affine_f32, 1.f), V > 1 ? affine_at<T>(p.gamma, c + 2 * j + 1, p.affine_f32, 1.f) : 0.f);
-        beta[j] = make_float2(affine_at<T>(p.beta, c + 2 * j, p.affine_f32, 0.f), V > 1 ? affine_at<T>(p.beta, c + 2 * j + 1, p.affine_f32, 0.f) : 0.f);
+        gamma[j] = twice(1.f);
+        beta[j] = twice(0.f);
     }
+    if (!p.gamma) return;
+    auto load = [&](auto type) {
+        using A = decltype(type);
+        const A *g = static_cast<const A*>(p.gamma) + c, *b = static_cast<const A*>(p.beta) + c;
+#pragma unroll
+        for (int j = 0; j < (V + 1) / 2; ++j) {
+            gamma[j] = make_float2(static_cast<float>(g[2 * j]), V > 1 ? static_cast<float>(g[2 * j + (V > 1)]) : 0.f);
+            beta[j] = make_float2(static_cast<float>(b[2 * j]), V > 1 ? static_cast<float>(b[2 * j + (V > 1)]) : 0.f);
+        }
+    };
+    if (sizeof(T) == 4 || p.affine_f32) load(float{});
+    else load(T{});
 }
 
 template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const void* from)
@@ -119,7 +141,12 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, con
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// (all groups but the last N)
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ float warp_sum(float x)
 {
 #pragma unroll
@@ -134,68 +161,86 @@ __device__ __forceinline__ void put_sums(float* red, const float2 (&s)[2])
     red[2 * kNormThreads + threadIdx.x] = s[1].x;
     red[3 * kNormThreads + threadIdx.x] = s[1].y;
 }
-// Channels' sums: over the rows of threads, into red[c % 4][c / 4].  `share` threads, neighbouring lanes, add a channel's (a power of two that divides 32).
+// The same for sums of groups only: those of a group are added first, where a word lies in one or in two.
+__device__ __forceinline__ void put_group_sums(float* red, const Norm& p, const float2 (&s)[2])
+{
+    if (p.slots == 4) return put_sums(red, s);
+    const float a = s[0].x + s[0].y, b = s[1].x + s[1].y;
+    red[threadIdx.x] = p.slots == 1 ? a + b : a;
+    if (p.slots == 2) red[kNormThreads + threadIdx.x] = b;
+}
+// Groups' sums over `rows` rows of `span` slots, a warp to a group: f(group, sum) in its first lane.
+template <class F> __device__ __forceinline__ void group_sums(const float* red, const Norm& p, int slots, int span, const FastDiv& by_span, int rows, int groups, F&& f)
+{
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, shift = slots == 4 ? 2 : slots - 1, count = rows * span;
+    for (int g = warp; g < groups; g += kNormThreads / 32) {
+        float s = 0.f;
+        for (int i = lane; i < count; i += 32) {
+            unsigned row, k;
+            by_span.divmod(static_cast<unsigned>(i), row, k);
+            k += g * span;
+            s += red[(k & (slots - 1)) * kNormThreads + row * p.words + (k >> shift)];
+        }
+        s = warp_sum(s);
+        if (lane == 0) f(g, s);
+    }
+}
+// Channels' sums: over the rows of threads, into the first: red[c % 4][c / 4].  `share` threads, neighbouring lanes, add a channel's (a power of two that divides 32).
 __device__ __forceinline__ void channel_sums(float* red, const Norm& p, int arrays)
 {
-    const int wide = 4 * p.words, total = arrays * wide;
-    int share = 1;
-    while (share < 32 && total * share * 2 <= kNormThreads) share *= 2;
-    __syncthreads();
-    const int lane = threadIdx.x % share;
-    for (int c0 = 0; c0 < total; c0 += kNormThreads / share) {
-        const int c = c0 + static_cast<int>(threadIdx.x) / share, array = c / wide, ch = c - array * wide;
+    const int total = arrays * 4 * p.words;
+    int shift = 0;
+    while (shift < 5 && total << (shift + 1) <= kNormThreads) ++shift;
+    const int share = 1 << shift, lane = threadIdx.x & (share - 1);
+    for (int c0 = 0; c0 < total; c0 += kNormThreads >> shift) {
+        const int c = c0 + static_cast<int>(threadIdx.x >> shift);
+        unsigned array = 0, word = 0;                             // arrays of a word's channels
+        p.by_words.divmod(static_cast<unsigned>(c), array, word);
         float s = 0.f;
-        const float* at = red + (array * 4 + ch % 4) * kNormThreads + ch / 4;
+        float* at = red + array * kNormThreads + word;
         if (c < total)
             for (int r = lane; r < p.rows; r += share) s += at[r * p.words];
         for (int d = share / 2; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         __syncwarp();
-        if (c < total && lane == 0) red[(array * 4 + ch % 4) * kNormThreads + ch / 4] = s;
-    }
-    __syncthreads();
-}
-// Groups' sums of channels' sums, a warp to a group: f(group, sum) in every lane.
-template <class F> __device__ __forceinline__ void group_sums(const float* red, const Norm& p, int groups, F&& f)
-{
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int g = warp; g < groups; g += kNormThreads / 32) {
-        float s = 0.f;
-        for (int i = lane; i < p.D; i += 32) {
-            const int c = g * p.D + i;
-            s += red[(c % 4) * kNormThreads + c / 4];
-        }
-        f(g, warp_sum(s));
+        if (c < total && lane == 0) at[0] = s;
     }
 }
 
-// Shared memory of a resident CTA: its words of X, backward 16 bytes for each of deltaY and dz, four (eight) sums of each thread, and the groups'.
-__host__ __device__ inline size_t norm_smem(bool back, int size, int part, int words, int groups)
+__device__ __forceinline__ void st_cluster_f2(uint32_t at, float x, float y) { asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory"); }
+
+// Shared memory of a resident CTA: its words of X, backward 16 bytes for each of deltaY and dz; four (eight) sums of each thread, the groups' sums of every CTA of the cluster, their total.
+__host__ __device__ inline size_t norm_smem(bool back, int size, int part, int words, int groups, int cluster)
 {
-    return static_cast<size_t>(part) * words * (4 * size + (back ? 16 : 0)) + kNormThreads * 16 * (back ? 2 : 1) + static_cast<size_t>(groups) * 16;
+    const size_t tensors = (static_cast<size_t>(part) * words * (4 * size + (back ? 16 : 0)) + 15) & ~static_cast<size_t>(15);
+    return tensors + kNormThreads * 16 * (back ? 2 : 1) + static_cast<size_t>(groups) * 8 * (cluster + 1);
 }
 
 template <class T, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __grid_constant__ Norm p)
+__global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_resident_kernel(const __grid_constant__ Norm p)
 {
     using W = NormWord<T, 4>;
     using Raw = typename W::Raw;
     extern __shared__ __align__(128) uint8_t smem[];
-    const int cl = p.cluster, rank = cl > 1 ? static_cast<int>(cluster_ctarank()) : 0, item = blockIdx.x / cl, n = item / p.slabs, slab = item - n * p.slabs;
+    const int cl = p.cluster, rank = cl > 1 ? static_cast<int>(cluster_ctarank()) : 0, groups = p.groups;
+    unsigned item, n, slab, ty_, tx_, unused;
+    p.by_cluster.divmod(blockIdx.x, item, unused);
+    p.by_slabs.divmod(item, n, slab);
+    p.by_words.divmod(threadIdx.x, ty_, tx_);
     const int r0 = rank * p.part, mine = min(p.part, p.R - r0);             // (positive: no part is empty)
-    const int ty = threadIdx.x / p.words, tx = threadIdx.x - ty * p.words, c0 = slab * p.words * 4, groups = p.words * 4 / p.D, g0 = c0 / p.D, c = c0 + tx * 4;
+    const int ty = ty_, tx = tx_, c = slab * p.words * 4 + tx * 4;
     const bool busy = ty < p.rows;
     const int first = busy ? ty * p.words + tx : 0, step = p.rows * p.words, last = busy ? mine * p.words : 0;      // its words: first, first + step, ... < last
     float4* ds = reinterpret_cast<float4*>(smem);                                                                    // deltaY, then dz
     Raw* xs = reinterpret_cast<Raw*>(smem + (BACK ? static_cast<size_t>(p.part) * p.words * 16 : 0));
     float* red = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(xs) + ((static_cast<size_t>(p.part) * p.words * sizeof(Raw) + 15) & ~static_cast<size_t>(15)));
-    float2* own = reinterpret_cast<float2*>(red + 4 * kNormThreads * (BACK ? 2 : 1));      // this CTA's sums of each group
-    float2* all = own + groups;                                                            // the cluster's
-    const size_t from = (static_cast<size_t>(n) * p.R + r0 + ty) * p.C + c, jump = static_cast<size_t>(p.rows) * p.C;
+    float2* parts = reinterpret_cast<float2*>(red + 4 * kNormThreads * (BACK ? 2 : 1));    // [rank][group], written by every CTA of the cluster
+    float2* all = parts + cl * groups;
+    const size_t from = (static_cast<size_t>(n) * p.R + r0 + ty) * p.C + c, jump = static_cast<size_t>(p.rows) * p.C, at_group = static_cast<size_t>(n) * p.G + slab * groups;
     grid_dependency_wait();
     grid_dependency_trigger();
     {
         const T *x = static_cast<const T*>(p.X) + from, *y = BACK ? static_cast<const T*>(p.dY) + from : nullptr;
-        const uint32_t to = smem_u32(xs), to_y = smem_u32(ds);
+        const uint32_t to_y = smem_u32(ds), to = smem_u32(xs);
 #pragma unroll 4
         for (int i = first; i < last; i += step) {
             copy_async<sizeof(Raw)>(to + i * sizeof(Raw), x);
@@ -203,15 +248,33 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
             if (BACK) { copy_async<sizeof(Raw)>(to_y + i * 16, y); y += jump; }
         }
     }
-    float2 gamma[2], beta[2], mean[2], s[2], q[2];
-    load_affine<T, 4>(p, c, gamma, beta);
-    const int gi[4] = {c / p.D - g0, (c + 1) / p.D - g0, (c + 2) / p.D - g0, (c + 3) / p.D - g0};         // groups of its channels
+    int gi[4];                                                                             // groups of its channels, within the slab
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        unsigned g;
+        p.by_D.divmod(static_cast<unsigned>(tx * 4 + j), g, unused);
+        gi[j] = static_cast<int>(g);
+    }
     const float count = static_cast<float>(p.R) * static_cast<float>(p.D);
+    float2 gamma[2], beta[2], mean[2], s[2], q[2];            // (means negated)
+    load_affine<T, 4>(p, c, gamma, beta);
     T* out = static_cast<T*>(p.out) + from;
 #pragma unroll
     for (int j = 0; j < 2; ++j) s[j] = q[j] = make_float2(0.f, 0.f);
+    // a group's two sums to every CTA of the cluster; then all have them
+    auto share = [&](int g, float x, float y) {
+        if (cl == 1) { parts[g] = make_float2(x, y); return; }
+        const uint32_t at = smem_u32(parts + rank * groups + g);
+        for (int r = 0; r < cl; ++r) st_cluster_f2(mapa_u32(at, r), x, y);
+    };
+    auto shared_by_all = [&] {
+        if (cl > 1) cluster_sync_all();
+        else __syncthreads();
+    };
+    // (a cluster's CTAs have all begun before one writes to another)
+    if (cl > 1) cluster_arrive();
+    copies_done();
     if constexpr (!BACK) {
-        copies_done();
         const float own_count = static_cast<float>(mine) * static_cast<float>(p.D);
 #pragma unroll 4
         for (int i = first; i < last; i += step) {
@@ -220,50 +283,48 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
             s[0] = add2(s[0], f[0]);
             s[1] = add2(s[1], f[1]);
         }
-        put_sums(red, s);
-        channel_sums(red, p, 1);
-        group_sums(red, p, groups, [&](int g, float sum) { if ((threadIdx.x & 31) == 0) own[g].x = sum / own_count; });
+        put_group_sums(red, p, s);
         __syncthreads();
-        mean[0] = make_float2(own[gi[0]].x, own[gi[1]].x);
-        mean[1] = make_float2(own[gi[2]].x, own[gi[3]].x);
+        group_sums(red, p, p.slots, p.span, p.by_span, p.rows, groups, [&](int g, float sum) { all[g].x = sum / own_count; });
+        __syncthreads();
+        mean[0] = neg2(make_float2(all[gi[0]].x, all[gi[1]].x));
+        mean[1] = neg2(make_float2(all[gi[2]].x, all[gi[3]].x));
 #pragma unroll 4
         for (int i = first; i < last; i += step) {
             float2 f[2];
             W::load(xs[i], f);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) { f[j] = add2(f[j], neg2(mean[j])); q[j] = fma2(f[j], f[j], q[j]); }
+            for (int j = 0; j < 2; ++j) { f[j] = add2(f[j], mean[j]); q[j] = fma2(f[j], f[j], q[j]); }
         }
-        put_sums(red, q);
-        channel_sums(red, p, 1);
-        group_sums(red, p, groups, [&](int g, float sum) { if ((threadIdx.x & 31) == 0) own[g].y = sum; });
-        if (cl > 1) cluster_sync_all();
-        else __syncthreads();
+        put_group_sums(red, p, q);
+        if (cl > 1) cluster_wait();
+        __syncthreads();
+        group_sums(red, p, p.slots, p.span, p.by_span, p.rows, groups, [&](int g, float sum) { share(g, all[g].x, sum); });
+        shared_by_all();
         // mean and rstd of a group from its parts
         for (int g = threadIdx.x; g < groups; g += kNormThreads) {
-            float m = own[g].x, squares = own[g].y;
+            float m = parts[g].x, squares = parts[g].y;
             if (cl > 1) {
-                const uint32_t at = smem_u32(own + g);
                 float sum = 0.f;
-                for (int r = 0; r < cl; ++r) sum = fmaf(ld_shared_cluster(mapa_u32(at, r)), static_cast<float>(min(p.part, p.R - r * p.part)), sum);
+                for (int r = 0; r < cl; ++r) sum = fmaf(parts[r * groups + g].x, static_cast<float>(min(p.part, p.R - r * p.part)), sum);
                 m = sum / static_cast<float>(p.R);
                 squares = 0.f;
                 for (int r = 0; r < cl; ++r) {
-                    const uint32_t peer = mapa_u32(at, r);
-                    const float d = ld_shared_cluster(peer) - m;
-                    squares += ld_shared_cluster(peer + 4) + d * d * (static_cast<float>(min(p.part, p.R - r * p.part)) * static_cast<float>(p.D));
+                    const float2 e = parts[r * groups + g];
+                    const float d = e.x - m;
+                    squares += e.y + d * d * (static_cast<float>(min(p.part, p.R - r * p.part)) * static_cast<float>(p.D));
                 }
             }
             const float r = 1.f / sqrtf(squares / count + p.eps);
             all[g] = make_float2(m, r);
             if (rank == 0 && p.mean) {
-                p.mean[static_cast<size_t>(n) * p.G + g0 + g] = m;
-                p.rstd[static_cast<size_t>(n) * p.G + g0 + g] = r;
+                p.mean[at_group + g] = m;
+                p.rstd[at_group + g] = r;
             }
         }
-        if (cl > 1) cluster_sync_all();          // (and no CTA leaves while another may still read its sums)
-        else __syncthreads();
-        mean[0] = make_float2(all[gi[0]].x, all[gi[1]].x);
-        mean[1] = make_float2(all[gi[2]].x, all[gi[3]].x);
+        __syncthreads();
+        mean[0] = neg2(make_float2(all[gi[0]].x, all[gi[1]].x));
+        mean[1] = neg2(make_float2(all[gi[2]].x, all[gi[3]].x));
         gamma[0] = mul2(gamma[0], make_float2(all[gi[0]].y, all[gi[1]].y));
         gamma[1] = mul2(gamma[1], make_float2(all[gi[2]].y, all[gi[3]].y));
         with_act(p.act, [&](auto a) {
@@ -274,7 +335,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
                 W::load(xs[i], f);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    f[j] = fma2(add2(f[j], neg2(mean[j])), gamma[j], beta[j]);
+                    f[j] = fma2(add2(f[j], mean[j]), gamma[j], beta[j]);
                     f[j] = make_float2(norm_value<ACT, kNormFast<T>>(f[j].x, p.k), norm_value<ACT, kNormFast<T>>(f[j].y, p.k));
                 }
                 *reinterpret_cast<Raw*>(out) = W::store(f);
@@ -283,15 +344,13 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
         });
     } else {
         // s: sums of dz, q: of dz (x - mean)
-        const size_t at_group = static_cast<size_t>(n) * p.G + g0;
         float2 rstd[2], scale[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            mean[j] = make_float2(p.mean[at_group + gi[2 * j]], p.mean[at_group + gi[2 * j + 1]]);
+            mean[j] = neg2(make_float2(p.mean[at_group + gi[2 * j]], p.mean[at_group + gi[2 * j + 1]]));
             rstd[j] = make_float2(p.rstd[at_group + gi[2 * j]], p.rstd[at_group + gi[2 * j + 1]]);
             scale[j] = mul2(rstd[j], gamma[j]);
         }
-        copies_done();
         with_act(p.act, [&](auto a) {
             constexpr int ACT = decltype(a)::value;
 #pragma unroll 2
@@ -301,7 +360,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
                 W::load(*reinterpret_cast<const Raw*>(ds + i), y);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    x[j] = add2(x[j], neg2(mean[j]));
+                    x[j] = add2(x[j], mean[j]);
                     const float2 z = fma2(x[j], scale[j], beta[j]);
                     y[j] = mul2(y[j], make_float2(norm_slope<ACT, kNormFast<T>>(z.x, p.k), norm_slope<ACT, kNormFast<T>>(z.y, p.k)));
                     s[j] = add2(s[j], y[j]);
@@ -314,48 +373,46 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
         for (int j = 0; j < 2; ++j) q[j] = mul2(q[j], rstd[j]);
         put_sums(red, s);
         put_sums(red + 4 * kNormThreads, q);
+        __syncthreads();
         channel_sums(red, p, 2);
-        // over the cluster: every CTA adds all parts in the same order
-        float keep[8];
-        if (cl > 1) cluster_sync_all();
+        __syncthreads();
         if (threadIdx.x < p.words) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                keep[j] = 0.f;
-                if (cl == 1) { keep[j] = red[j * kNormThreads + threadIdx.x]; continue; }
-                const uint32_t at = smem_u32(red + j * kNormThreads + threadIdx.x);
-                for (int r = 0; r < cl; ++r) keep[j] += ld_shared_cluster(mapa_u32(at, r));
-            }
-        }
-        if (cl > 1) cluster_sync_all();          // (all parts have been read)
-        if (threadIdx.x < p.words) {
+            // the CTA's sums of its channels, for deltaGamma and deltaBeta; weighted by gamma for those of the groups
             const float by[4] = {gamma[0].x, gamma[0].y, gamma[1].x, gamma[1].y};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (rank == 0) p.sums[static_cast<size_t>(n) * p.C + c + j] = make_float2(keep[j], keep[4 + j]);
-                red[j * kNormThreads + threadIdx.x] = keep[j] * by[j];
-                red[(4 + j) * kNormThreads + threadIdx.x] = keep[4 + j] * by[j];
+                float *x = red + j * kNormThreads + threadIdx.x, *y = x + 4 * kNormThreads;
+                p.sums[(static_cast<size_t>(n) * cl + rank) * p.C + c + j] = make_float2(*x, *y);
+                *x *= by[j];
+                *y *= by[j];
             }
         }
+        if (cl > 1) cluster_wait();
         __syncthreads();
-        group_sums(red, p, groups, [&](int g, float sum) { if ((threadIdx.x & 31) == 0) all[g].x = sum / count; });
-        group_sums(red + 4 * kNormThreads, p, groups, [&](int g, float sum) { if ((threadIdx.x & 31) == 0) all[g].y = sum / count; });
+        group_sums(red, p, 4, p.D, p.by_D, 1, groups, [&](int g, float sum) { all[g].x = sum; });
+        group_sums(red + 4 * kNormThreads, p, 4, p.D, p.by_D, 1, groups, [&](int g, float sum) { share(g, all[g].x, sum); });
+        shared_by_all();
+        for (int g = threadIdx.x; g < groups; g += kNormThreads) {
+            float2 sum = parts[g];
+            for (int r = 1; r < cl; ++r) { sum.x += parts[r * groups + g].x; sum.y += parts[r * groups + g].y; }
+            all[g] = make_float2(sum.x / count, sum.y / count);
+        }
         __syncthreads();
         // deltaX = scale dz + more (x - mean) + base
         float2 more[2], base[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float2 a = all[gi[2 * j]], b = all[gi[2 * j + 1]];
-            base[j] = neg2(mul2(rstd[j], make_float2(a.x, b.x)));
-            more[j] = neg2(mul2(mul2(rstd[j], rstd[j]), make_float2(a.y, b.y)));
+            const float2 d = all[gi[2 * j]], e = all[gi[2 * j + 1]];
+            base[j] = neg2(mul2(rstd[j], make_float2(d.x, e.x)));
+            more[j] = neg2(mul2(mul2(rstd[j], rstd[j]), make_float2(d.y, e.y)));
         }
 #pragma unroll 4
         for (int i = first; i < last; i += step) {
             float2 x[2];
             W::load(xs[i], x);
             const float4 d = ds[i];
-            x[0] = fma2(make_float2(d.x, d.y), scale[0], fma2(add2(x[0], neg2(mean[0])), more[0], base[0]));
-            x[1] = fma2(make_float2(d.z, d.w), scale[1], fma2(add2(x[1], neg2(mean[1])), more[1], base[1]));
+            x[0] = fma2(make_float2(d.x, d.y), scale[0], fma2(add2(x[0], mean[0]), more[0], base[0]));
+            x[1] = fma2(make_float2(d.z, d.w), scale[1], fma2(add2(x[1], mean[1]), more[1], base[1]));
             *reinterpret_cast<Raw*>(out) = W::store(x);
             out += jump;
         }
@@ -363,6 +420,58 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
 }
 
 // ---- streamed ---------------------------------------------------------------------------------------------------
+
+// A thread's words of one or two tensors, row after row, U of them at a time.  Words of four elements come by asynchronous copies two batches ahead, through shared
+// memory where each thread has places of its own (48 KB a CTA, four of them on an SM: a load into registers for each batch left HBM idle in between, 512 x 512 x 256 bf16
+// 89 us instead of 72); single elements are loaded as they are used.
+template <class T, int V, bool TWO> struct NormRows {
+    using Raw = typename NormWord<T, V>::Raw;
+    static constexpr int S = 3, U = (sizeof(T) == 2 ? 8 : 4) / (TWO ? 2 : 1);
+    static constexpr size_t kBytes = V == 1 ? 0 : static_cast<size_t>(kNormThreads) * sizeof(Raw) * U * S * (TWO ? 2 : 1);
+    const T *x, *y;
+    size_t step;                     // elements from a row to the thread's next
+    int total;                       // its rows
+    Raw* ring;
+    __device__ Raw* at(int batch, int i, int second) const { return ring + ((batch % S * U + i) * (TWO ? 2 : 1) + second) * kNormThreads + threadIdx.x; }
+    __device__ void issue(int batch) const
+    {
+        if constexpr (V != 1) {
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int k = batch * U + i;
+                if (k >= total) break;
+                copy_async<sizeof(Raw)>(smem_u32(at(batch, i, 0)), x + k * step);
+                if (TWO) copy_async<sizeof(Raw)>(smem_u32(at(batch, i, 1)), y + k * step);
+            }
+            copies_commit();
+        }
+    }
+    // f(first row, rows, words of x, words of y) for each batch; rows < U: the last
+    template <class F> __device__ void each(F&& f) const
+    {
+        if constexpr (V != 1)
+            for (int b = 0; b < S - 1; ++b) issue(b);
+        const int batches = (total + U - 1) / U;
+        for (int b = 0; b < batches; ++b) {
+            Raw rx[U], ry[U];
+            const int have = min(U, total - b * U);
+            if constexpr (V != 1) {
+                issue(b + S - 1);
+                copies_wait<S - 1>();
+#pragma unroll
+                for (int i = 0; i < U; ++i) { rx[i] = *at(b, i, 0); if (TWO) ry[i] = *at(b, i, 1); }
+            } else {
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const size_t o = (static_cast<size_t>(b) * U + (i < have ? i : 0)) * step;
+                    rx[i] = x[o];
+                    if (TWO) ry[i] = y[o];
+                }
+            }
+            f(b * U, have, rx, ry);
+        }
+    }
+};
 
 // Where a CTA of the streamed passes is: a block of columns, a run of positions, a sample.
 struct NormAt { int n, run, count, ty, word; bool busy; size_t from; };
@@ -381,126 +490,156 @@ template <int V> __device__ __forceinline__ NormAt norm_at(const Norm& p, unsign
 }
 // Mean and squared differences of a run, or its sums of dz and dz xh, for every channel.
 template <class T, int V, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, 4) norm_sums_kernel(const __grid_constant__ Norm p)
+__global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_sums_kernel(const __grid_constant__ Norm p)
 {
     using W = NormWord<T, V>;
-    using Raw = typename W::Raw;
-    constexpr int U = BACK ? 4 : 8, P = (V + 1) / 2;
-    __shared__ float red[2 * V * kNormThreads];
+    using Rows = NormRows<T, V, BACK>;
+    using Raw = typename Rows::Raw;
+    constexpr int U = Rows::U, P = (V + 1) / 2;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* red = reinterpret_cast<float*>(smem);              // 2 V sums of each thread, over the ring when that has been read
     grid_dependency_wait();
     grid_dependency_trigger();
     const NormAt a = norm_at<V>(p, blockIdx.x);
     float2 s[P], q[P];
 #pragma unroll
     for (int j = 0; j < P; ++j) s[j] = q[j] = make_float2(0.f, 0.f);
-    if (a.busy) {
-        const T *x = static_cast<const T*>(p.X) + a.from, *y = BACK ? static_cast<const T*>(p.dY) + a.from : nullptr;
-        const size_t step = static_cast<size_t>(p.rows) * p.C;
+    if (a.busy && a.ty < a.count) {
+        const size_t begin = a.from + static_cast<size_t>(a.ty) * p.C;
+        const Rows rows{static_cast<const T*>(p.X) + begin, BACK ? static_cast<const T*>(p.dY) + begin : nullptr, static_cast<size_t>(p.rows) * p.C, (a.count - a.ty + p.rows - 1) / p.rows,
+                        reinterpret_cast<Raw*>(smem)};
         if constexpr (!BACK) {
             float seen = 0.f;                     // s: mean of what has been seen, q: its squared differences
-            for (int r = a.ty; r < a.count; r += U * p.rows) {
-                Raw raw[U];
-                int have = (a.count - r + p.rows - 1) / p.rows;
-                if (have > U) have = U;
-                const T* at = x + static_cast<size_t>(r) * p.C;
-#pragma unroll
-                for (int i = 0; i < U; ++i) raw[i] = *reinterpret_cast<const Raw*>(at + (i < have ? i : 0) * step);
-                const float each = static_cast<float>(have), total = seen + each, weight = each / total, inverse = 1.f / each;
+            rows.each([&](int, int have, const Raw (&raw)[U], const Raw (&)[U]) {
+                const float each = static_cast<float>(have), total = seen + each, weight = __fdividef(each, total), inverse = have == U ? 1.f / U : __fdividef(1.f, each);
                 float2 m[P], d2[P];
 #pragma unroll
                 for (int j = 0; j < P; ++j) m[j] = d2[j] = make_float2(0.f, 0.f);
+                auto pass = [&](auto whole) {
 #pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    float2 f[P];
-                    W::load(raw[i], f);
+                    for (int i = 0; i < U; ++i) {
+                        if (!decltype(whole)::value && i >= have) break;
+                        float2 f[P];
+                        W::load(raw[i], f);
 #pragma unroll
-                    for (int j = 0; j < P; ++j) m[j] = i < have ? add2(m[j], f[j]) : m[j];
-                }
-#pragma unroll
-                for (int j = 0; j < P; ++j) m[j] = mul2(m[j], make_float2(inverse, inverse));
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    float2 f[P];
-                    W::load(raw[i], f);
-#pragma unroll
-                    for (int j = 0; j < P; ++j) {
-                        const float2 d = add2(f[j], neg2(m[j]));
-                        d2[j] = i < have ? fma2(d, d, d2[j]) : d2[j];
+                        for (int j = 0; j < P; ++j) m[j] = add2(m[j], f[j]);
                     }
-                }
+#pragma unroll
+                    for (int j = 0; j < P; ++j) m[j] = mul2(m[j], twice(-inverse));      // (the negated mean)
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        if (!decltype(whole)::value && i >= have) break;
+                        float2 f[P];
+                        W::load(raw[i], f);
+#pragma unroll
+                        for (int j = 0; j < P; ++j) {
+                            const float2 d = add2(f[j], m[j]);
+                            d2[j] = fma2(d, d, d2[j]);
+                        }
+                    }
+                };
+                if (have == U) pass(std::true_type{});
+                else pass(std::false_type{});
                 const float cross = seen * weight;
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
-                    const float2 d = add2(m[j], neg2(s[j]));
-                    s[j] = fma2(d, make_float2(weight, weight), s[j]);
-                    q[j] = add2(q[j], fma2(mul2(d, d), make_float2(cross, cross), d2[j]));
+                    const float2 d = neg2(add2(m[j], s[j]));
+                    s[j] = fma2(d, twice(weight), s[j]);
+                    q[j] = add2(q[j], fma2(mul2(d, d), twice(cross), d2[j]));
                 }
                 seen = total;
-            }
+            });
         } else {
             float2 mean[P], rstd[P], gamma[P], beta[P];
             load_affine<T, V>(p, a.word * V, gamma, beta);
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 const size_t g = static_cast<size_t>(a.n) * p.G + (a.word * V + 2 * j) / p.D, h = static_cast<size_t>(a.n) * p.G + (a.word * V + 2 * j + (V > 1)) / p.D;
-                mean[j] = make_float2(p.mean[g], p.mean[h]);
+                mean[j] = neg2(make_float2(p.mean[g], p.mean[h]));
                 rstd[j] = make_float2(p.rstd[g], p.rstd[h]);
                 gamma[j] = mul2(gamma[j], rstd[j]);
             }
             with_act(p.act, [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
-                for (int r = a.ty; r < a.count; r += U * p.rows) {
-                    Raw rx[U], ry[U];
-                    const size_t at = static_cast<size_t>(r) * p.C;
+                rows.each([&](int, int have, const Raw (&rx)[U], const Raw (&ry)[U]) {
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
-                        const size_t o = at + (r + i * p.rows < a.count ? i : 0) * step;
-                        rx[i] = *reinterpret_cast<const Raw*>(x + o);
-                        ry[i] = *reinterpret_cast<const Raw*>(y + o);
-                    }
-#pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        if (r + i * p.rows >= a.count) break;
+                        if (i >= have) break;
                         float2 fx[P], fy[P];
                         W::load(rx[i], fx);
                         W::load(ry[i], fy);
 #pragma unroll
                         for (int j = 0; j < P; ++j) {
-                            fx[j] = add2(fx[j], neg2(mean[j]));
+                            fx[j] = add2(fx[j], mean[j]);
                             const float2 z = fma2(fx[j], gamma[j], beta[j]);
                             fy[j] = mul2(fy[j], make_float2(norm_slope<ACT, kNormFast<T>>(z.x, p.k), V > 1 ? norm_slope<ACT, kNormFast<T>>(z.y, p.k) : 0.f));
                             s[j] = add2(s[j], fy[j]);
                             q[j] = fma2(fy[j], fx[j], q[j]);
                         }
                     }
-                }
+                });
             });
 #pragma unroll
             for (int j = 0; j < P; ++j) q[j] = mul2(q[j], rstd[j]);
         }
     }
+    copies_done();
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         red[j * kNormThreads + threadIdx.x] = j % 2 ? s[j / 2].y : s[j / 2].x;
         red[(V + j) * kNormThreads + threadIdx.x] = j % 2 ? q[j / 2].y : q[j / 2].x;
     }
     __syncthreads();
-    float2* to = p.partial + (static_cast<size_t>(a.n) * p.runs + a.run) * p.C;
+    const int per = !BACK && p.whole ? p.G : p.C;
+    float2* to = p.partial + (static_cast<size_t>(a.n) * p.runs + a.run) * per;
     const int first = (a.word - (static_cast<int>(threadIdx.x) - a.ty * p.words)) * V, wide = min(p.words * V, p.C - first);
     const int rows = min(p.rows, a.count);
-    for (int c = threadIdx.x; c < wide; c += kNormThreads) {
-        const float *ms = red + (c % V) * kNormThreads + c / V, *qs = ms + V * kNormThreads;
+    // `share` threads, neighbouring lanes, add a channel's
+    int shift = 0;
+    while (shift < 5 && wide << (shift + 1) <= kNormThreads) ++shift;
+    const int share = 1 << shift, lane = threadIdx.x & (share - 1);
+    auto shared_sum = [&](float x) {
+        for (int d = share / 2; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        return x;
+    };
+    for (int c0 = 0; c0 < wide; c0 += kNormThreads >> shift) {
+        const int c = c0 + static_cast<int>(threadIdx.x >> shift);
+        float *ms = red + (c % V) * kNormThreads + c / V, *qs = ms + V * kNormThreads;
+        const int mine = c < wide ? rows : 0;
         float sum = 0.f, squares = 0.f;
         if constexpr (BACK) {
-            for (int r = 0; r < rows; ++r) { sum += ms[r * p.words]; squares += qs[r * p.words]; }
+            for (int r = lane; r < mine; r += share) { sum += ms[r * p.words]; squares += qs[r * p.words]; }
+            sum = shared_sum(sum);
+            squares = shared_sum(squares);
         } else {
             const int each = a.count / p.rows, left = a.count - each * p.rows;
             auto had = [&](int r) { return static_cast<float>(each + (r < left ? 1 : 0)); };
-            for (int r = 0; r < rows; ++r) sum = fmaf(ms[r * p.words], had(r), sum);
-            sum /= static_cast<float>(a.count);
-            for (int r = 0; r < rows; ++r) { const float d = ms[r * p.words] - sum; squares += fmaf(d * d, had(r), qs[r * p.words]); }
+            for (int r = lane; r < mine; r += share) sum = fmaf(ms[r * p.words], had(r), sum);
+            sum = shared_sum(sum) / static_cast<float>(a.count);
+            for (int r = lane; r < mine; r += share) { const float d = ms[r * p.words] - sum; squares += fmaf(d * d, had(r), qs[r * p.words]); }
+            squares = shared_sum(squares);
         }
-        to[first + c] = make_float2(sum, squares);
+        __syncwarp();
+        if (c < wide && lane == 0) {
+            if (!BACK && p.whole) { ms[0] = sum; qs[0] = squares; }
+            else to[first + c] = make_float2(sum, squares);
+        }
+    }
+    if (BACK || !p.whole) return;
+    __syncthreads();
+    // groups from their channels, a thread to a group (D is 64 * V at most)
+    const float count = static_cast<float>(a.count);
+    for (int g = threadIdx.x; g < wide / p.D; g += kNormThreads) {
+        float sum = 0.f, squares = 0.f;
+        for (int d = 0; d < p.D; ++d) { const int c = g * p.D + d; sum += red[(c % V) * kNormThreads + c / V]; }
+        sum /= static_cast<float>(p.D);
+        for (int d = 0; d < p.D; ++d) {
+            const int c = g * p.D + d;
+            const float e = red[(c % V) * kNormThreads + c / V] - sum;
+            squares += fmaf(e * e, count, red[(V + c % V) * kNormThreads + c / V]);
+        }
+        to[first / p.D + g] = make_float2(sum, squares);
     }
 }
 
@@ -524,23 +663,24 @@ __global__ void __launch_bounds__(kJoinNormThreads) norm_join_kernel(const __gri
     grid_dependency_wait();
     grid_dependency_trigger();
     const int n = blockIdx.x / p.G, g = blockIdx.x - n * p.G;
-    const float2* from = p.partial + static_cast<size_t>(n) * p.runs * p.C + g * p.D;
     const float count = static_cast<float>(p.R) * static_cast<float>(p.D);
     if constexpr (!BACK) {
-        const int entries = p.runs * p.D;
+        const int D = p.whole ? 1 : p.D, per = p.whole ? p.G : p.C, entries = p.runs * D;
+        const float channels = static_cast<float>(p.whole ? p.D : 1);
+        const float2* from = p.partial + static_cast<size_t>(n) * p.runs * per + g * D;
         float sum = 0.f, squares = 0.f;
 #pragma unroll 4
         for (int i = threadIdx.x; i < entries; i += kJoinNormThreads) {
-            const int run = i / p.D;
-            sum = fmaf(from[static_cast<size_t>(run) * p.C + i - run * p.D].x, static_cast<float>(min(p.part, p.R - run * p.part)), sum);
+            const int run = i / D;
+            sum = fmaf(from[static_cast<size_t>(run) * per + i - run * D].x, static_cast<float>(min(p.part, p.R - run * p.part)), sum);
         }
-        const float mean = block_sum(sum, shared) / count;
+        const float mean = block_sum(sum, shared) * channels / count;
 #pragma unroll 4
         for (int i = threadIdx.x; i < entries; i += kJoinNormThreads) {
-            const int run = i / p.D;
-            const float2 e = from[static_cast<size_t>(run) * p.C + i - run * p.D];
+            const int run = i / D;
+            const float2 e = from[static_cast<size_t>(run) * per + i - run * D];
             const float d = e.x - mean;
-            squares += fmaf(d * d, static_cast<float>(min(p.part, p.R - run * p.part)), e.y);
+            squares += fmaf(d * d, static_cast<float>(min(p.part, p.R - run * p.part)) * channels, e.y);
         }
         const float rstd = 1.f / sqrtf(block_sum(squares, shared) / count + p.eps);
         if (threadIdx.x == 0) {
@@ -548,6 +688,7 @@ __global__ void __launch_bounds__(kJoinNormThreads) norm_join_kernel(const __gri
             if (p.mean) { p.mean[blockIdx.x] = mean; p.rstd[blockIdx.x] = rstd; }
         }
     } else {
+        const float2* from = p.partial + static_cast<size_t>(n) * p.runs * p.C + g * p.D;
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         float s1 = 0.f, s2 = 0.f;
         for (int d = warp; d < p.D; d += kJoinNormThreads / 32) {
@@ -559,7 +700,7 @@ __global__ void __launch_bounds__(kJoinNormThreads) norm_join_kernel(const __gri
             if (lane == 0) {
                 const int c = g * p.D + d;
                 const float gamma = affine_at<T>(p.gamma, c, p.affine_f32, 1.f);
-                p.sums[static_cast<size_t>(n) * p.C + c] = make_float2(a, b);
+                p.sums[static_cast<size_t>(n) * p.C + c] = make_float2(a, b);     // (streamed: a row for each sample)
                 s1 = fmaf(a, gamma, s1);
                 s2 = fmaf(b, gamma, s2);
             }
@@ -571,15 +712,17 @@ __global__ void __launch_bounds__(kJoinNormThreads) norm_join_kernel(const __gri
 }
 // The outputs, from the end of the tensors.
 template <class T, int V, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(const __grid_constant__ Norm p)
+__global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_apply_kernel(const __grid_constant__ Norm p)
 {
     using W = NormWord<T, V>;
-    using Raw = typename W::Raw;
-    constexpr int U = 4, P = (V + 1) / 2;
+    using Rows = NormRows<T, V, BACK>;
+    using Raw = typename Rows::Raw;
+    constexpr int U = Rows::U, P = (V + 1) / 2;
+    extern __shared__ __align__(128) uint8_t smem[];
     grid_dependency_wait();
     grid_dependency_trigger();
     const NormAt a = norm_at<V>(p, gridDim.x - 1 - blockIdx.x);
-    if (!a.busy) return;
+    if (!a.busy || a.ty >= a.count) return;
     float2 mean[P], gamma[P], beta[P], more[P], base[P];
     load_affine<T, V>(p, a.word * V, gamma, beta);
 #pragma unroll
@@ -588,38 +731,30 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(const __gri
         const float2 t = p.group[g], u = p.group[h];
         if constexpr (BACK) {
             const float2 rstd = make_float2(p.rstd[g], p.rstd[h]);
-            mean[j] = make_float2(p.mean[g], p.mean[h]);
+            mean[j] = neg2(make_float2(p.mean[g], p.mean[h]));
             gamma[j] = mul2(gamma[j], rstd);
             base[j] = neg2(mul2(rstd, make_float2(t.x, u.x)));
             more[j] = neg2(mul2(mul2(rstd, rstd), make_float2(t.y, u.y)));
         } else {
-            mean[j] = make_float2(t.x, u.x);
+            mean[j] = neg2(make_float2(t.x, u.x));
             gamma[j] = mul2(gamma[j], make_float2(t.y, u.y));
         }
     }
-    const T *x = static_cast<const T*>(p.X) + a.from, *y = BACK ? static_cast<const T*>(p.dY) + a.from : nullptr;
-    T* out = static_cast<T*>(p.out) + a.from;
-    const size_t step = static_cast<size_t>(p.rows) * p.C;
+    const size_t begin = a.from + static_cast<size_t>(a.ty) * p.C, step = static_cast<size_t>(p.rows) * p.C;
+    const Rows rows{static_cast<const T*>(p.X) + begin, BACK ? static_cast<const T*>(p.dY) + begin : nullptr, step, (a.count - a.ty + p.rows - 1) / p.rows, reinterpret_cast<Raw*>(smem)};
+    T* out = static_cast<T*>(p.out) + begin;
     with_act(p.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
-        for (int r = a.ty; r < a.count; r += U * p.rows) {
-            Raw rx[U], ry[U];
-            const size_t at = static_cast<size_t>(r) * p.C;
+        rows.each([&](int, int have, const Raw (&rx)[U], const Raw (&ry)[U]) {
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                const size_t o = at + (r + i * p.rows < a.count ? i : 0) * step;
-                rx[i] = *reinterpret_cast<const Raw*>(x + o);
-                if (BACK) ry[i] = *reinterpret_cast<const Raw*>(y + o);
-            }
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (r + i * p.rows >= a.count) break;
+                if (i >= have) break;
                 float2 f[P], fy[P];
                 W::load(rx[i], f);
                 if (BACK) W::load(ry[i], fy);
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
-                    f[j] = add2(f[j], neg2(mean[j]));
+                    f[j] = add2(f[j], mean[j]);
                     const float2 z = fma2(f[j], gamma[j], beta[j]);
                     if constexpr (BACK) {
                         fy[j] = mul2(fy[j], make_float2(norm_slope<ACT, kNormFast<T>>(z.x, p.k), V > 1 ? norm_slope<ACT, kNormFast<T>>(z.y, p.k) : 0.f));
@@ -628,9 +763,10 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(const __gri
                         f[j] = make_float2(norm_value<ACT, kNormFast<T>>(z.x, p.k), V > 1 ? norm_value<ACT, kNormFast<T>>(z.y, p.k) : 0.f);
                     }
                 }
-                *reinterpret_cast<Raw*>(out + at + i * step) = W::store(f);
+                *reinterpret_cast<Raw*>(out) = W::store(f);
+                out += step;
             }
-        }
+        });
     });
 }
 
