@@ -5,8 +5,9 @@
 //
 // 16-bit tensors.  Forward: one product whose epilogue reduces each tile's row to its largest logit and the sum of exponentials about it (8 bytes for 128 or fewer logits), and a
 // pass that joins them.  Gradients, piece by piece of the classes: logits formed once more, their gradients rounded to the tensors' type into scratch as the epilogue
-// of that product, and the two products that read them; deltaX is summed in fp32 over the pieces.  dz is rounded once, as deltaZ of a FullConnect layer is; in fp16 it is held times a
-// power of two (the largest |dL| at 2^14 or above), as a probability of 1e-5 over 1e4 rows would not be a normal number, and the outputs are scaled back in fp32.
+// of that product, and the two products that read them; deltaX is summed in fp32 over the pieces.  dz is rounded once, as deltaZ of a FullConnect layer is; a dL that all rows share
+// is left to the outputs.  In fp16 dz is held times a power of two (the largest |dL| at 2^14 or above), as a probability of 1e-5 over 1e4 rows would not be a normal
+// number, and the outputs are scaled back in fp32.
 // Bound by the tensor cores: 2 (forward) and 6 (gradients) rows x classes x IC operations; for few rows by reading W.
 //
 // fp32 tensors: products at fp32 accuracy as those of the layer, logits of a piece in scratch.
@@ -63,7 +64,8 @@ int forward_16(const Loss& c, float* loss, float* lse)
                   ALPHA_ACT_NONE, 0.f, FcLoss{}};
         float2 dummy;
         q.loss.part = &dummy;                         // (the plan: nothing is written but parts)
-        const FcPlan plan = pick_plan(q, sms, nullptr, 1);
+        FcPlan plan = pick_plan(q, sms, nullptr, 1);
+        if (!plan.pair) plan.bn = std::min(plan.bn, 128);       // (wider ones can be asked for by option FC_TILE)
         const long long slots = 2 * ((OC + plan.bn - 1) / plan.bn);
         void *part = nullptr, *at_label = nullptr;
         rc = call_scratch(c.stream, static_cast<size_t>(slots) * rows * sizeof(float2), &part);
@@ -80,7 +82,7 @@ int forward_16(const Loss& c, float* loss, float* lse)
 }
 
 // deltaB of a piece from its dz.
-template <class T> int column_sums(const T* dz, int rows, int pitch, const float* scale, T* dB, int sms, cudaStream_t stream)
+template <class T> int column_sums(const T* dz, int rows, int pitch, const float* by, float factor, T* dB, int sms, cudaStream_t stream)
 {
     const int blocks = (pitch + 32 * Word16<T>::N - 1) / (32 * Word16<T>::N), most = std::max(1, 8 * sms / blocks), parts = std::min((rows + 31) / 32, most);
     void* part = nullptr;
@@ -90,7 +92,7 @@ template <class T> int column_sums(const T* dz, int rows, int pitch, const float
     note_launch("fc_loss");
     rc = launched("loss_columns_kernel");
     if (rc) return rc;
-    launch_after(loss_bias_kernel<T>, (pitch + 255) / 256, 256, 0, stream, static_cast<const float*>(part), parts, pitch, scale, dB);
+    launch_after(loss_bias_kernel<T>, (pitch + 255) / 256, 256, 0, stream, static_cast<const float*>(part), parts, pitch, by, factor, dB);
     note_launch("fc_loss");
     return launched("loss_bias_kernel");
 }
@@ -110,14 +112,18 @@ template <class T> int delta_16(const Loss& c, const float* dL, int dL_step, con
     void *dz = nullptr, *sums = nullptr, *scale = nullptr;
     if (!rc) rc = call_scratch(c.stream, static_cast<size_t>(rows) * fc_pitch(static_cast<int>(piece)) * 2, &dz);
     if (!rc && dX && pieces > 1) rc = call_scratch(c.stream, static_cast<size_t>(rows) * IC * 4, &sums);
-    if (!rc && c.s->dtype == ALPHA_F16) rc = call_scratch(c.stream, 2 * sizeof(float), &scale);
+    const bool f16 = c.s->dtype == ALPHA_F16;
+    if (!rc && f16 && dL_step) rc = call_scratch(c.stream, 2 * sizeof(float), &scale);
     if (rc) return rc;
     if (scale && !dry_run()) {
-        launch_after(loss_scale_kernel, 1, 1024, 0, c.stream, dL, dL_step ? c.s->rows : 1, static_cast<float*>(scale));
+        launch_after(loss_scale_kernel, 1, 1024, 0, c.stream, dL, c.s->rows, static_cast<float*>(scale));
         note_launch("fc_loss");
         rc = launched("loss_scale_kernel");
         if (rc) return rc;
     }
+    // One gradient for all rows stays out of dz, which then is p - [label] (most are 1 or near: they would all be rounded alike) and, in fp16, 2^14 times that.
+    const float held = f16 && !dL_step ? 0x1p14f : 1.f;
+    const float *out_by = dL_step ? (scale ? static_cast<const float*>(scale) + 1 : nullptr) : dL, out_factor = 1.f / held;
     const ScratchMark mark = call_mark(c.stream);
     for (long long first = 0; first < OC; first += piece) {
         call_rewind(c.stream, mark);
@@ -126,14 +132,14 @@ template <class T> int delta_16(const Loss& c, const float* dL, int dL_step, con
         const T* W = static_cast<const T*>(c.W) + first * IC;
         FcLoss l{};
         l.label = c.label; l.label_bytes = c.label_bytes; l.base = static_cast<int>(first); l.classes = c.s->OC;
-        l.lse = lse; l.grad = dL; l.grad_step = dL_step; l.scale = static_cast<const float*>(scale);
+        l.lse = lse; l.grad = dL_step ? dL : nullptr; l.scale = static_cast<const float*>(scale); l.held = held;
         if (!dry_run()) {
             const Product z{dtype, c.s->rows, static_cast<int>(cols), static_cast<int>(pitch), c.s->IC, 1, 1, false, Operand{c.X, false, IC, 1, rows, IC, IC}, Operand{W, false, IC, cols, 1, IC, cols * IC},
                             c.bias ? static_cast<const T*>(c.bias) + first : nullptr, nullptr, nullptr, dz, ALPHA_ACT_NONE, 0.f, l};
             rc = launch_product<kFcSoftmaxDelta>(z, c.stream);
             if (rc) return rc;
             FcLoss of_x{}, of_w{};
-            of_x.scale = of_w.scale = l.scale;
+            of_x.out_by = of_w.out_by = out_by; of_x.out_factor = of_w.out_factor = out_factor;
             of_x.sums = static_cast<float*>(sums); of_x.first = first == 0; of_x.last = first + cols == OC;
             const Product x{dtype, c.s->rows, c.s->IC, c.s->IC, static_cast<int>(cols), 1, 1, false, Operand{dz, false, cols, 1, rows, pitch, pitch}, Operand{W, true, IC, cols, 1, IC, cols * IC},
                             nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f, of_x};
@@ -144,7 +150,7 @@ template <class T> int delta_16(const Loss& c, const float* dL, int dL_step, con
             else if (dW) rc = launch_product<kFcSum>(w, c.stream);
             if (rc) return rc;
         }
-        if (dB) rc = column_sums(static_cast<const T*>(dz), c.s->rows, static_cast<int>(pitch), l.scale, static_cast<T*>(dB) + first, sms, c.stream);
+        if (dB) rc = column_sums(static_cast<const T*>(dz), c.s->rows, static_cast<int>(pitch), out_by, out_factor, static_cast<T*>(dB) + first, sms, c.stream);
         if (rc) return rc;
     }
     return ALPHA_OK;
@@ -204,7 +210,7 @@ int delta_f32(const Loss& c, const float* dL, int dL_step, const float* lse, flo
             note_launch("fc_loss");
             rc = launched("loss_add_kernel");
         }
-        if (!rc && dB) rc = column_sums(z, c.s->rows, fc_pitch(s.OC), nullptr, dB + first, sms, c.stream);
+        if (!rc && dB) rc = column_sums(z, c.s->rows, fc_pitch(s.OC), nullptr, 1.f, dB + first, sms, c.stream);
     }
     return rc;
 }

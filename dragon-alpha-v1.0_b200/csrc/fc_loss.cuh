@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) loss_columns_kernel(const T* __restrict__
     }
 }
 template <class T>
-__global__ void __launch_bounds__(256) loss_bias_kernel(const float* __restrict__ part, int parts, int pitch, const float* scale, T* out)
+__global__ void __launch_bounds__(256) loss_bias_kernel(const float* __restrict__ part, int parts, int pitch, const float* by, float factor, T* out)
 {
     grid_dependency_wait();
     grid_dependency_trigger();
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256) loss_bias_kernel(const float* __restrict_
     if (c >= pitch) return;
     float s = 0.f;
     for (int i = 0; i < parts; ++i) s += part[static_cast<size_t>(i) * pitch + c];
-    out[c] = static_cast<T>(scale ? s * scale[1] : s);
+    out[c] = static_cast<T>(s * ((by ? *by : 1.f) * factor));
 }
 
 // ---- fp32: logits of a piece of the classes lie in memory ---------------------------------------------------------

@@ -21,6 +21,9 @@
 // those are staged, which leaves the ring to B: it streams 160 KB of W ahead.  Where tiles are fewer than SMs a cluster of `split` CTAs
 // shares a tile's reduction; each leaves its sums in its shared memory, and the cluster's CTAs finish a share of the columns each, adding
 // the parts through distributed shared memory in order.
+//
+// kFcStats: the tensor cores truncate as they add, toward 0, and a loss of fp32 shows it (4096 steps: 2 to 3e-6 of it).  They add 1024 steps; the epilogue's warps add those sums in
+// registers, rounded to nearest (5e-7 to 9e-7), beside the MMAs of the next 1024.
 // Warps: 0 TMA producer, 1 MMA issuer, 2-9 epilogue (two per quarter of the lanes, chunks of 32 columns in turn).
 #pragma once
 #include "fc_act.cuh"
@@ -29,6 +32,7 @@
 namespace alpha {
 
 constexpr int kFcThreads = 320, kFcBK = 64, kFcGroupM = 8, kFcMaxStages = 16;
+constexpr int kFcSegment = 1024;             // steps that kFcStats adds up on the tensor cores
 constexpr uint32_t kFcRing = 196608, kFcStaging = 8 * 4096;              // staging: two buffers of 32 x 32 elements for each epilogue warp
 
 // What becomes of the sums: a layer's outputs; the largest logit of each row and the sum of exponentials about it; the gradient of a softmax's cross
@@ -40,8 +44,9 @@ struct FcLoss {
     int base, classes;                       // the product's first column among the classes, and how many there are
     float2* part;                            // [2 n_tiles][rows] (largest, sum), of either half of the epilogue's warps
     float* at_label;                         // [rows] logits of the labels
-    const float *lse, *grad; int grad_step;  // [rows] logarithms of the sums; gradients of the rows' losses, or (step 0) of all
-    const float* scale;                      // power of two that keeps fp16 gradients of logits normal, and its inverse (or NULL)
+    const float *lse, *grad;                 // [rows] logarithms of the sums; gradients of the rows' losses (NULL: the outputs are multiplied by one for all)
+    const float *scale; float held;          // gradients of logits are held times *scale (NULL: 1) and `held`, powers of two that keep those of fp16 normal
+    const float* out_by; float out_factor;   // kFcSum: what outputs are multiplied by (NULL: 1), and once more
     float* sums;                             // [rows][pitch] of kFcSum, or NULL: one product
     int first, last;                         // product of those that add up
 };
@@ -82,6 +87,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     const int BN = PAIR ? PAIR : p.bn, OUT = GLU ? BN / 2 : BN, S = PAIR ? static_cast<int>(kFcRing / (KB * fc_block_bytes(true, 128, PAIR))) : p.stages, split = PAIR ? 1 : p.split;
     const uint32_t kA = PAIR ? 16384u : static_cast<uint32_t>(p.a_rows) * 128, kB = PAIR ? PAIR * 64u : static_cast<uint32_t>(BN) * 128, kBlock = kA + kB, kStage = KB * kBlock;
     const int acc_pitch = (BN + 31) & ~31;        // columns from one accumulator to the other
+    constexpr int kSegment = kFcSegment / (kFcBK * KB), kChunks = PAIR == 256 ? 4 : 2;      // kFcStats: stages that are added at a time; chunks of columns of a warp
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * kStage + kFcStaging);
@@ -209,7 +215,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                 }
             }
             if (l.sums && !l.last) return;
-            const float by = l.scale ? __ldg(l.scale + 1) : 1.f;
+            const float by = (l.out_by ? __ldg(l.out_by) : 1.f) * l.out_factor;
 #pragma unroll
             for (int i = 0; i < 32; ++i) z[i] *= by;
         } else if constexpr (GLU) {
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         const bool counts = label >= 0 && label < l.classes;
         if constexpr (EPI == kFcSoftmaxDelta) {
             lse = __ldg(l.lse + row);
-            if (counts) grad = __ldg(l.grad + static_cast<size_t>(row) * l.grad_step) * (l.scale ? __ldg(l.scale) : 1.f);
+            if (counts) grad = (l.grad ? __ldg(l.grad + row) : 1.f) * (l.scale ? __ldg(l.scale) : 1.f) * l.held;
         }
         label = counts ? label - l.base : -1LL << 40;
     };
@@ -368,10 +374,18 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                 steps_of(k_begin, k_end);
                 const uint32_t a_k = cur->a_mn ? 128u : 2u, b_k = cur->b_mn ? 128u : 2u, idesc = cur->idesc;      // 16 steps further, in 16-byte units
                 const uint32_t a_lo0 = smem_desc_lo(base, cur->a_mn ? 8192u : 16u), b_lo0 = smem_desc_lo(base + kA, cur->b_mn ? 8192u : 16u);
-                if (!wait(aempty_0 + 8 * ap.idx, ap.phase ^ 1)) break;
-                tc_fence_after_sync();
-                const uint32_t d = tmem + ap.idx * acc_pitch;
+                uint32_t d = 0;
                 for (int kb = k_begin; kb < k_end; ++kb) {
+                    const bool start = kb == k_begin || (EPI == kFcStats && (kb - k_begin) % kSegment == 0);
+                    if (start) {
+                        if (EPI == kFcStats && kb > k_begin) {
+                            if (elected) commit(afull_0 + 8 * ap.idx);
+                            ap.advance(2);
+                        }
+                        if (!wait(aempty_0 + 8 * ap.idx, ap.phase ^ 1)) { ok = false; break; }
+                        tc_fence_after_sync();
+                        d = tmem + ap.idx * acc_pitch;
+                    }
                     if (!__all_sync(0xffffffffu, next) && !wait(full_0 + 8 * rp.idx, rp.phase)) { ok = false; break; }
                     tc_fence_after_sync();
                     const uint32_t a = a_lo0 + rp.idx * (kStage >> 4), b = b_lo0 + rp.idx * (kStage >> 4), done = empty_0 + 8 * rp.idx;
@@ -379,7 +393,7 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                     for (uint32_t q = 0; q < KB; ++q)
 #pragma unroll
                         for (uint32_t kk = 0; kk < 4; ++kk)
-                            mma_16bit<PAIR != 0>(d, a + q * (kBlock >> 4) + kk * a_k, dhi, b + q * (kBlock >> 4) + kk * b_k, dhi, idesc, kb > k_begin || q || kk ? 1u : 0u, elected);
+                            mma_16bit<PAIR != 0>(d, a + q * (kBlock >> 4) + kk * a_k, dhi, b + q * (kBlock >> 4) + kk * b_k, dhi, idesc, !start || q || kk ? 1u : 0u, elected);
                     if (elected) commit(done);
                     if (++rp.idx == S) { rp.idx = 0; rp.phase ^= 1u; }
                     next = mbar_test_a<PAIR != 0>(full_0 + 8 * rp.idx, rp.phase);     // (beside the MMAs just issued)
@@ -414,6 +428,46 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                     if (row < cur->rows && n1 + c < cur->cols) prefetch_l2(static_cast<const T*>(cur->residual) + static_cast<size_t>(row) * cur->cols + n1 + c);
             }
             if (fetching) fetch(r, row0, n0 + half * 32, OUT - half * 32);
+            if constexpr (EPI == kFcStats) {
+                if (cur->kb > kSegment) {
+                    float sums[kChunks][32];
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sums[c][i] = 0.f;
+                    for (int kb = 0; kb < cur->kb; kb += kSegment) {
+                        ok = mbar_wait_a(afull_a + 8 * ap.idx, ap.phase);
+                        if (!ok) { report(p.status, kStatusEpilogueTimeout); settle(); break; }
+                        tc_fence_after_sync();
+#pragma unroll
+                        for (int c = 0; c < kChunks; ++c) {
+                            const int col = half * 32 + 64 * c;
+                            if (row0 >= cur->rows || col >= OUT || n0 + col >= cur->cols) continue;
+                            uint32_t v[32];
+                            tmem_ld_32x32(lanes + ap.idx * acc_pitch + col, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sums[c][i] += __uint_as_float(v[i]);
+                        }
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (PAIR) mbar_arrive_cluster_relaxed(aempty_L + 8 * ap.idx);
+                            else mbar_arrive_relaxed_a(aempty_L + 8 * ap.idx);
+                        }
+                        ap.advance(2);
+                    }
+                    if (!ok) break;
+                    begin_row(row0 + lane);
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) {
+                        const int col = half * 32 + 64 * c;
+                        if (row0 < cur->rows && col < OUT && n0 + col < cur->cols) stats(sums[c], row0 + lane, n0 + col, OUT - col);
+                    }
+                    if (row0 + lane < cur->rows) cur->loss.part[(static_cast<size_t>(n0 / OUT) * 2 + half) * cur->rows + row0 + lane] = make_float2(most, mass);
+                    continue;
+                }
+            }
             ok = mbar_wait_a(afull_a + 8 * ap.idx, ap.phase);
             if (!ok) { report(p.status, kStatusEpilogueTimeout); settle(); break; }
             tc_fence_after_sync();
