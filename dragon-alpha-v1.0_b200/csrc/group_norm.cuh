@@ -79,33 +79,42 @@ template <class T> struct NormWord<T, 1> {
 };
 template <class T> constexpr bool kNormFast = sizeof(T) == 2;
 
-// Activations of 16-bit tensors by a sigmoid without the care that quotients and exponentials of denormal results take (good to 2^-21 of its value; below 1e-38 it is 0).
-__device__ __forceinline__ Sigmoid sigmoid_lean(float z)
+// Activations of 16-bit tensors by s = 1 / (1 + exp(-u)), good to 2^-21 of its value down to u = -87 and 0 below that (1e-38); two values at a time.
+__device__ __forceinline__ float2 exp_of(float2 u)                // exp(-u)
 {
-    float e, big;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.44269504f * fabsf(z)));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(big) : "f"(1.f + e));
-    const float small = e * big;
-    return z >= 0.f ? Sigmoid{big, small} : Sigmoid{small, big};
+    u = mul2(u, twice(-1.44269504f));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(u.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(u.y));
+    return u;
 }
-template <int ACT, bool FAST> __device__ __forceinline__ float norm_value(float z, float k)
+__device__ __forceinline__ float2 inverse_of(float2 x)
 {
-    if constexpr (FAST && ACT == ALPHA_ACT_SILU) return z * sigmoid_lean(z).pos;
-    else if constexpr (FAST && ACT == ALPHA_ACT_GELU_TANH) return z * sigmoid_lean(1.59576912f * (z + 0.044715f * z * z * z)).pos;
-    else if constexpr (FAST && ACT == ALPHA_ACT_SIGMOID) return sigmoid_lean(z).pos;
-    else return act_value<ACT, FAST>(z, k);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x.y));
+    return x;
 }
-template <int ACT, bool FAST> __device__ __forceinline__ float norm_slope(float z, float k)
+template <int ACT, bool FAST> __device__ __forceinline__ float2 norm_value(float2 z, float k)
 {
-    if constexpr (FAST && ACT == ALPHA_ACT_SILU) {
-        const Sigmoid s = sigmoid_lean(z);
-        return s.pos * fmaf(z, s.neg, 1.f);
-    } else if constexpr (FAST && ACT == ALPHA_ACT_SIGMOID) {
-        const Sigmoid s = sigmoid_lean(z);
-        return s.pos * s.neg;
+    if constexpr (ACT == ALPHA_ACT_NONE) return z;
+    else if constexpr (FAST && (ACT == ALPHA_ACT_SILU || ACT == ALPHA_ACT_SIGMOID || ACT == ALPHA_ACT_GELU_TANH)) {
+        // (gelu_tanh: z sigmoid(2 sqrt(2 / pi) (z + 0.044715 z^3)))
+        const float2 u = ACT == ALPHA_ACT_GELU_TANH ? mul2(z, fma2(mul2(z, z), twice(1.59576912f * 0.044715f), twice(1.59576912f))) : z, s = inverse_of(add2(twice(1.f), exp_of(u)));
+        return ACT == ALPHA_ACT_SIGMOID ? s : mul2(z, s);
+    } else return make_float2(act_value<ACT, FAST>(z.x, k), act_value<ACT, FAST>(z.y, k));
+}
+template <int ACT, bool FAST> __device__ __forceinline__ float2 norm_slope(float2 z, float k)
+{
+    if constexpr (ACT == ALPHA_ACT_NONE) return twice(1.f);
+    else if constexpr (ACT == ALPHA_ACT_LEAKY_RELU) return make_float2(z.x > 0.f ? 1.f : k, z.y > 0.f ? 1.f : k);
+    else if constexpr (FAST && (ACT == ALPHA_ACT_SILU || ACT == ALPHA_ACT_SIGMOID)) {
+        z = make_float2(fmaxf(z.x, -87.f), fmaxf(z.y, -87.f));      // (no exponential of Inf; a NaN's gradient is that of deltaY)
+        const float2 e = exp_of(z), s = inverse_of(add2(twice(1.f), e)), rest = mul2(e, s);
+        return mul2(s, ACT == ALPHA_ACT_SILU ? fma2(z, rest, twice(1.f)) : rest);
     } else {
-        float value, slope;
-        act_both<ACT, FAST>(z, k, value, slope);
+        float value;
+        float2 slope;
+        act_both<ACT, FAST>(z.x, k, value, slope.x);
+        act_both<ACT, FAST>(z.y, k, value, slope.y);
         return slope;
     }
 }
@@ -336,7 +345,7 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_reside
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     f[j] = fma2(add2(f[j], mean[j]), gamma[j], beta[j]);
-                    f[j] = make_float2(norm_value<ACT, kNormFast<T>>(f[j].x, p.k), norm_value<ACT, kNormFast<T>>(f[j].y, p.k));
+                    f[j] = norm_value<ACT, kNormFast<T>>(f[j], p.k);
                 }
                 *reinterpret_cast<Raw*>(out) = W::store(f);
                 out += jump;
@@ -362,7 +371,7 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_reside
                 for (int j = 0; j < 2; ++j) {
                     x[j] = add2(x[j], mean[j]);
                     const float2 z = fma2(x[j], scale[j], beta[j]);
-                    y[j] = mul2(y[j], make_float2(norm_slope<ACT, kNormFast<T>>(z.x, p.k), norm_slope<ACT, kNormFast<T>>(z.y, p.k)));
+                    if (ACT != ALPHA_ACT_NONE) y[j] = mul2(y[j], norm_slope<ACT, kNormFast<T>>(z, p.k));
                     s[j] = add2(s[j], y[j]);
                     q[j] = fma2(y[j], x[j], q[j]);
                 }
@@ -436,12 +445,19 @@ template <class T, int V, bool TWO> struct NormRows {
     __device__ void issue(int batch) const
     {
         if constexpr (V != 1) {
+            const int have = min(U, total - batch * U);
+            const uint32_t to = smem_u32(at(batch, 0, 0));
+            const T *fx = x + batch * U * step, *fy = y + batch * U * step;
+            auto copy = [&](int i) {
+                copy_async<sizeof(Raw)>(to + i * (TWO ? 2 : 1) * kNormThreads * sizeof(Raw), fx);
+                fx += step;
+                if (TWO) { copy_async<sizeof(Raw)>(to + (2 * i + 1) * kNormThreads * sizeof(Raw), fy); fy += step; }
+            };
+            if (have == U) {
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int k = batch * U + i;
-                if (k >= total) break;
-                copy_async<sizeof(Raw)>(smem_u32(at(batch, i, 0)), x + k * step);
-                if (TWO) copy_async<sizeof(Raw)>(smem_u32(at(batch, i, 1)), y + k * step);
+                for (int i = 0; i < U; ++i) copy(i);
+            } else {
+                for (int i = 0; i < have; ++i) copy(i);
             }
             copies_commit();
         }
@@ -572,7 +588,7 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_sums_k
                         for (int j = 0; j < P; ++j) {
                             fx[j] = add2(fx[j], mean[j]);
                             const float2 z = fma2(fx[j], gamma[j], beta[j]);
-                            fy[j] = mul2(fy[j], make_float2(norm_slope<ACT, kNormFast<T>>(z.x, p.k), V > 1 ? norm_slope<ACT, kNormFast<T>>(z.y, p.k) : 0.f));
+                            if (ACT != ALPHA_ACT_NONE) fy[j] = mul2(fy[j], norm_slope<ACT, kNormFast<T>>(z, p.k));
                             s[j] = add2(s[j], fy[j]);
                             q[j] = fma2(fy[j], fx[j], q[j]);
                         }
@@ -757,10 +773,10 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_apply_
                     f[j] = add2(f[j], mean[j]);
                     const float2 z = fma2(f[j], gamma[j], beta[j]);
                     if constexpr (BACK) {
-                        fy[j] = mul2(fy[j], make_float2(norm_slope<ACT, kNormFast<T>>(z.x, p.k), V > 1 ? norm_slope<ACT, kNormFast<T>>(z.y, p.k) : 0.f));
+                        if (ACT != ALPHA_ACT_NONE) fy[j] = mul2(fy[j], norm_slope<ACT, kNormFast<T>>(z, p.k));
                         f[j] = fma2(fy[j], gamma[j], fma2(f[j], more[j], base[j]));
                     } else {
-                        f[j] = make_float2(norm_value<ACT, kNormFast<T>>(z.x, p.k), V > 1 ? norm_value<ACT, kNormFast<T>>(z.y, p.k) : 0.f);
+                        f[j] = norm_value<ACT, kNormFast<T>>(z, p.k);
                     }
                 }
                 *reinterpret_cast<Raw*>(out) = W::store(f);

@@ -43,13 +43,6 @@ def _pool_shape(*dims):
     return _cached_pool_shape(*map(operator.index, dims))
 
 
-_cached_norm_shape = functools.lru_cache(maxsize=512)(_l.AlphaNormShape)
-
-
-def _norm_shape(N, positions, C, groups, dtype, affine_dtype, act, k, eps):
-    return _cached_norm_shape(*map(operator.index, (N, positions, C, groups, dtype, affine_dtype, act)), float(k), float(eps))
-
-
 def _fc_shape(rows, IC, OC, dtype, act, k):
     return _cached_fc_shape(*map(operator.index, (rows, IC, OC, dtype, act)), float(k))
 
@@ -416,7 +409,14 @@ def _pad_both(t, n4, c4):
     return out
 
 
-_ADAMW_ROW = struct.Struct("@7Pqd4i")      # AlphaAdamW
+
+
+@functools.lru_cache(maxsize=64)
+def _adamw_rows(n):
+    """n AlphaAdamW rows."""
+    return struct.Struct("@" + "7Pqd4i" * n)
+
+
 _dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
 _FC_TYPES = {torch.float32: _l.ALPHA_F32, torch.bfloat16: _l.ALPHA_BF16, torch.float16: _l.ALPHA_F16}
 
@@ -571,6 +571,32 @@ def _refuse_overlaps(what, grads, Out):
 def _dense(t):
     """t as dense memory that holds its values."""
     return t.resolve_neg().contiguous()
+
+
+def _dense_now(t):
+    """The same without a call where there is nothing to do (None: None)."""
+    return t if t is None or (t.is_contiguous() and not t.is_neg()) else _dense(t.detach())
+
+
+@functools.lru_cache(maxsize=512)
+def _norm_plan(what, shape, groups, dtype, affine, act, k, eps):
+    """The library's shape of a group normalisation and that of its means, or None where X holds no samples."""
+    if dtype not in _FC_TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, dtype))
+    if len(shape) < 2 or groups < 1 or shape[-1] < 1 or shape[-1] % groups:
+        raise ValueError("%s: X %s in %d groups of channels" % (what, tuple(shape), groups))
+    if affine not in (None, dtype, torch.float32):
+        raise ValueError("%s: gamma and beta are %s, X %s" % (what, affine, dtype))
+    positions = 1
+    for n in shape[1:-1]:
+        positions *= n
+    if positions == 0:
+        raise ValueError("%s: X %s has no positions to take a mean of" % (what, tuple(shape)))
+    if shape[0] == 0:
+        return None
+    if max(shape[0] * shape[-1], positions) >= 2 ** 31:
+        raise ValueError("%s: X %s is too large" % (what, tuple(shape)))
+    return _l.AlphaNormShape(shape[0], positions, shape[-1], groups, _FC_TYPES[dtype], _FC_TYPES[affine or dtype], act, k, eps), (shape[0], groups)
 
 
 class AdamWState:
@@ -1041,129 +1067,143 @@ class Engine:
         max_norm: gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way, and not written; norm is that of grad_norm unless given (one float32 value on the
         GPU), and a step whose norm is NaN or Inf changes nothing.  Out: tensors of the parameters' shapes (None: none) that take the new values in their own type, the 16-bit
         copies of float32 weights.  seed (32 bits): of the rounding of 8-bit moments.  Returns the norm, or None without max_norm."""
-        params, grads = list(params), list(grads)
+        what, params, grads = "adamW", list(params), list(grads)
         n = len(params)
-        outs = [None] * n if Out is None else list(Out)
-        decay = [float(weight_decay)] * n if not isinstance(weight_decay, (list, tuple)) else [float(d) for d in weight_decay]
-        if len(grads) != n or len(outs) != n or len(decay) != n or len(state.m) != n:
-            raise ValueError("adamW: %d parameters, %d gradients, moments of %d, %d outputs, %d weight decays" % (n, len(grads), len(state.m), len(outs), len(decay)))
+        outs = None if Out is None else list(Out)
+        decay = [float(weight_decay)] * n if not isinstance(weight_decay, (list, tuple)) else list(map(float, weight_decay))
+        if len(grads) != n or len(decay) != n or len(state.m) != n or (outs is not None and len(outs) != n):
+            raise ValueError("adamW: %d parameters, %d gradients, moments of %d, %s outputs, %d weight decays" % (n, len(grads), len(state.m), n if outs is None else len(outs), len(decay)))
         if norm is not None and max_norm is None:
             raise ValueError("adamW: a norm without max_norm")
-        if not 0 <= operator.index(seed) < 2 ** 32:
+        seed = operator.index(seed)
+        if not 0 <= seed < 2 ** 32:
             raise ValueError("adamW: seed must have 32 bits")
-        used = [i for i in range(n) if grads[i] is not None]
+        used = grads if all(g is not None for g in grads) else [g for g in grads if g is not None]
         if not used:
             return None if max_norm is None else norm if norm is not None else self.grad_norm([])
-        device = params[used[0]].get_device()
-        if device < 0:
-            raise ValueError("adamW: tensors must be on a GPU")
         eight = state.bits == 8
-        rows = []
-        for i in used:
-            p, g, o = params[i], grads[i], outs[i]
-            for name, t in (("parameter", p), ("gradient", g), ("output", o)):
-                if t is None:
-                    continue
-                if t.dtype not in _FC_TYPES:
-                    raise ValueError("adamW: %s %d must be float32, bfloat16 or float16, not %s" % (name, i, t.dtype))
-                if t.shape != p.shape or t.get_device() != device:
-                    raise ValueError("adamW: %s %d is %s on %s, parameter %s on %s" % (name, i, tuple(t.shape), t.device, tuple(p.shape), p.device))
-                if t is not g and (not t.is_contiguous() or t.is_neg()):
-                    raise ValueError("adamW: %s %d must be dense" % (name, i))
-            moments = (state.m[i], state.v[i]) + ((state.m_scale[i], state.v_scale[i]) if eight else ())
-            if state.m[i].numel() != p.numel() or any(t.get_device() != device for t in moments):
-                raise ValueError("adamW: moments %d are %s on %s, parameter %s on %s" % (i, tuple(state.m[i].shape), state.m[i].device, tuple(p.shape), p.device))
-            rows.append((i, p, g, o, moments))
-        lr, lr_at = self._device_value("adamW", "lr", lr, torch.float32, device)
-        step, step_at = self._device_value("adamW", "step", step, torch.int64, device)
-        with self._on(params[used[0]]), torch.no_grad():
-            held = [_dense(g) for _, _, g, _, _ in rows]
-            if max_norm is not None and norm is None:
-                norm = self.grad_norm(held)
+        lists = [state.m, state.v] + ([state.m_scale, state.v_scale] if eight else [])
+        device, dense = self._check_adamw(what, params, grads, outs, lists)
+        lr, lr_at = self._device_value(what, "lr", lr, torch.float32, device)
+        step, step_at = self._device_value(what, "step", step, torch.int64, device)
+        with self._on(used[0]), torch.no_grad():
+            if not dense:
+                grads = [None if g is None else _dense(g) for g in grads]
+                used = [g for g in grads if g is not None]
             norm_at = None
             if max_norm is not None:
-                _, norm_at = self._device_value("adamW", "norm", norm, torch.float32, device)
+                if norm is None:
+                    norm = self.grad_norm(used)
+                norm_at = self._device_value(what, "norm", norm, torch.float32, device)[1]
                 if norm_at is None:
                     raise ValueError("adamW: norm must be a tensor on the GPU")
-            # (pad: the table keeps the number of each tensor among all, which the random bits of its moments go by)
-            table = bytearray()
-            at = 0
-            for (i, p, g, o, moments), d in zip(rows, held):
-                while at < i:
-                    table += _ADAMW_ROW.pack(0, 0, 0, 0, 0, 0, 0, 0, 0.0, 0, 0, 0, state.bits)
-                    at += 1
-                table += _ADAMW_ROW.pack(p.data_ptr(), d.data_ptr(), *(t.data_ptr() for t in moments), *(() if eight else (0, 0)), 0 if o is None else o.data_ptr(), p.numel(),
-                                         decay[i], _FC_TYPES[p.dtype], _FC_TYPES[g.dtype], 0 if o is None else _FC_TYPES[o.dtype], state.bits)
-                at += 1
-            how = _l.AlphaAdamWStep(float(lr), float(beta1), float(beta2), float(eps), 0.0 if max_norm is None else float(max_norm), operator.index(step), norm_at, lr_at, step_at,
-                                    operator.index(seed))
-            _l.check(self.base._lib.alpha_adamW(at, bytes(table), C.byref(how), _stream(self.base._stream)))
+            # a tensor without a gradient has a row of no elements: the others keep their numbers, which the random bits of their moments go by
+            at, code, none = torch.Tensor.data_ptr, _FC_TYPES.__getitem__, itertools.repeat(0)
+            if len(used) == n:
+                g_at, g_code, count = map(at, grads), map(code, map(_dtype_of, grads)), map(torch.Tensor.numel, params)
+            else:
+                g_at, g_code, count = ([0 if g is None else f(x) for g, x in zip(grads, xs)] for f, xs in ((at, grads), (lambda g: code(g.dtype), grads), (torch.Tensor.numel, params)))
+            if outs is None:
+                o_at, o_code = none, none
+            else:
+                o_at, o_code = [0 if o is None else o.data_ptr() for o in outs], [0 if o is None else code(o.dtype) for o in outs]
+            scales = (map(at, lists[2]), map(at, lists[3])) if eight else (none, none)
+            table = _adamw_rows(n).pack(*itertools.chain.from_iterable(zip(map(at, params), g_at, map(at, lists[0]), map(at, lists[1]), *scales, o_at, count, decay,
+                                                                           map(code, map(_dtype_of, params)), g_code, o_code, itertools.repeat(state.bits))))
+            how = _l.AlphaAdamWStep(lr, beta1, beta2, eps, 0.0 if max_norm is None else max_norm, operator.index(step), norm_at, lr_at, step_at, seed)
+            _l.check(self.base._lib.alpha_adamW(n, table, C.byref(how), _stream(self.base._stream)))
         return norm
+
+    @staticmethod
+    def _check_adamw(what, params, grads, outs, lists):
+        """The GPU of a step's tensors and whether all gradients are dense; raises for tensors the library would not take.  (A pass over all tensors for each question.)"""
+        T = torch.Tensor
+        kept = [o for o in outs if o is not None] if outs is not None else []
+        used = grads if all(g is not None for g in grads) else [g for g in grads if g is not None]
+        device = params[0].get_device()
+        written = params + kept
+        good = (device >= 0 and set(map(T.get_device, itertools.chain(written, used, *lists))) == {device} and set(map(_dtype_of, written + used)) <= _FC_TYPES.keys()
+                and all(map(T.is_contiguous, written)) and not any(map(T.is_neg, written)) and list(map(T.numel, lists[0])) == list(map(T.numel, params)))
+        shapes = list(map(_shape_of, params))
+        if good:
+            good = list(map(_shape_of, grads)) == shapes if len(used) == len(grads) else all(g is None or g.shape == s for g, s in zip(grads, shapes))
+        if good and outs is not None:
+            good = all(o is None or o.shape == s for o, s in zip(outs, shapes))
+        if not good:
+            for i, (p, g) in enumerate(zip(params, grads)):
+                o = None if outs is None else outs[i]
+                for name, t in (("parameter", p), ("gradient", g), ("output", o)):
+                    if t is None:
+                        continue
+                    if t.dtype not in _FC_TYPES:
+                        raise ValueError("%s: %s %d must be float32, bfloat16 or float16, not %s" % (what, name, i, t.dtype))
+                    if t.shape != p.shape or t.get_device() != device or device < 0:
+                        raise ValueError("%s: %s %d is %s on %s, parameter %s on %s; all belong on one GPU" % (what, name, i, tuple(t.shape), t.device, tuple(p.shape), params[0].device))
+                    if t is not g and (not t.is_contiguous() or t.is_neg()):
+                        raise ValueError("%s: %s %d must be dense" % (what, name, i))
+                if lists[0][i].numel() != p.numel() or any(t[i].get_device() != device for t in lists):
+                    raise ValueError("%s: moments %d are %s on %s, parameter %s on %s" % (what, i, tuple(lists[0][i].shape), lists[0][i].device, tuple(p.shape), p.device))
+        return device, all(map(T.is_contiguous, used)) and not any(map(T.is_neg, used))
 
     # ---- group normalisation ----
     def groupNorm(self, X, groups, gamma=None, beta=None, eps=1e-5, act="none", k=0.0, save=False):
         """act((X - mean) / sqrt(variance + eps) * gamma + beta) of channels-last tensors X [N, ..., C] (float32, bfloat16, float16), mean and variance over the
         positions and the channels of each of `groups` groups of neighbours.  gamma, beta [C]: of X's type or float32, both or neither.  act as in fullConnect.  save=True
         also returns mean and rstd [N, groups] (float32), which groupNorm_delta reads."""
-        shape, gamma, beta = self._norm_call("groupNorm", X, groups, gamma, beta, eps, act, k, ())
-        if shape is None:
+        plan = self._norm_check("groupNorm", X, operator.index(groups), gamma, beta, act, float(k), float(eps), ())
+        if plan is None:
             return (X.new_empty(X.shape), _new(X, (0, groups)), _new(X, (0, groups))) if save else X.new_empty(X.shape)
-        with self._on(X), torch.no_grad():
-            X = _dense(X)
-            Y = torch.empty(X.shape, dtype=X.dtype, device=X.device)
-            mean, rstd = (_new(X, (X.shape[0], groups)), _new(X, (X.shape[0], groups))) if save else (None, None)
-            self.base.groupNorm(shape, X, gamma, beta, mean, rstd, Y)
+        if self.base._stream is None and X.get_device() == torch._C._cuda_getDevice():
+            return self._norm_run(plan, X, gamma, beta, save)
+        with self._on(X):
+            return self._norm_run(plan, X, gamma, beta, save)
+
+    def _norm_run(self, plan, X, gamma, beta, save):
+        shape, kept = plan
+        Xd, gamma, beta = _dense_now(X), _dense_now(gamma), _dense_now(beta)
+        Y = X.new_empty(X.shape)
+        mean, rstd = (_new(X, kept), _new(X, kept)) if save else (None, None)
+        self.base.groupNorm(shape, Xd, gamma, beta, mean, rstd, Y)
         return (Y, mean, rstd) if save else Y
 
     def groupNorm_delta(self, deltaY, X, mean, rstd, gamma=None, beta=None, act="none", k=0.0):
         """(deltaX, deltaGamma, deltaBeta) of groupNorm from deltaY, its X and the mean and rstd it saved; the latter two None without gamma and beta."""
         if mean.dim() != 2:
             raise ValueError("groupNorm_delta: mean %s, expected [N, groups]" % (tuple(mean.shape),))
-        groups = mean.shape[1]
-        kept = (X.shape[0] if X.dim() else 0, groups)
-        shape, gamma, beta = self._norm_call("groupNorm_delta", X, groups, gamma, beta, 0.0, act, k,
-                                                   (("deltaY", deltaY, tuple(X.shape), X.dtype), ("mean", mean, kept, torch.float32), ("rstd", rstd, kept, torch.float32)))
-        if shape is None:
+        kept = (X.shape[0] if X.dim() else 0, mean.shape[1])
+        plan = self._norm_check("groupNorm_delta", X, mean.shape[1], gamma, beta, act, float(k), 0.0,
+                                (("deltaY", deltaY, X.shape, X.dtype), ("mean", mean, kept, torch.float32), ("rstd", rstd, kept, torch.float32)))
+        if plan is None:
             return X.new_empty(X.shape), *(None if gamma is None else torch.zeros_like(gamma) for _ in range(2))
-        with self._on(X), torch.no_grad():
-            deltaY, X, mean, rstd = _dense(deltaY), _dense(X), _dense(mean), _dense(rstd)
-            dX = torch.empty(X.shape, dtype=X.dtype, device=X.device)
-            dG, dB = (torch.empty_like(gamma), torch.empty_like(gamma)) if gamma is not None else (None, None)
-            self.base.groupNorm_delta(shape, deltaY, X, mean, rstd, gamma, beta, dX, dG, dB)
+        if self.base._stream is None and X.get_device() == torch._C._cuda_getDevice():
+            return self._norm_run_delta(plan[0], deltaY, X, mean, rstd, gamma, beta)
+        with self._on(X):
+            return self._norm_run_delta(plan[0], deltaY, X, mean, rstd, gamma, beta)
+
+    def _norm_run_delta(self, shape, deltaY, X, mean, rstd, gamma, beta):
+        dYd, Xd, meand, rstdd, gamma, beta = map(_dense_now, (deltaY, X, mean, rstd, gamma, beta))
+        dX = X.new_empty(X.shape)
+        dG, dB = (gamma.new_empty(gamma.shape), gamma.new_empty(gamma.shape)) if gamma is not None else (None, None)
+        self.base.groupNorm_delta(shape, dYd, Xd, meand, rstdd, gamma, beta, dX, dG, dB)
         return dX, dG, dB
 
-    def _norm_call(self, what, X, groups, gamma, beta, eps, act, k, others):
-        """The checked call: its shape (None where X holds nothing), gamma and beta as dense memory."""
-        code, groups = _fc_act(what, act), operator.index(groups)
-        if X.dtype not in _FC_TYPES:
-            raise ValueError("%s: float32, bfloat16 or float16 tensors, not %s" % (what, X.dtype))
-        if X.dim() < 2 or groups < 1 or X.shape[-1] < 1 or X.shape[-1] % groups:
-            raise ValueError("%s: X %s in %d groups of channels" % (what, tuple(X.shape), groups))
+    @staticmethod
+    def _norm_check(what, X, groups, gamma, beta, act, k, eps, others):
+        """The checked call's plan (None where X holds nothing)."""
         if (gamma is None) != (beta is None):
             raise ValueError("%s: gamma and beta, or neither" % what)
-        channels, affine = X.shape[-1], X.dtype
-        if gamma is not None:
-            affine = gamma.dtype if gamma.dtype == torch.float32 else X.dtype
-            others += (("gamma", gamma, (channels,), affine), ("beta", beta, (channels,), affine))
-        if X.get_device() < 0:
+        plan = _norm_plan(what, X.shape, groups, X.dtype, None if gamma is None else gamma.dtype, _fc_act(what, act), k, eps)
+        device = X.get_device()
+        if device < 0:
             raise ValueError("%s: tensors must be on a GPU" % what)
+        if gamma is not None:
+            others += (("gamma", gamma, X.shape[-1:], gamma.dtype), ("beta", beta, X.shape[-1:], gamma.dtype))
         for name, t, shape, dtype in others:
-            if tuple(t.shape) != shape:
-                raise ValueError("%s: %s %s, expected %s" % (what, name, tuple(t.shape), shape))
-            if t.dtype != dtype or t.get_device() != X.get_device():
+            if t.shape != shape:
+                raise ValueError("%s: %s %s, expected %s" % (what, name, tuple(t.shape), tuple(shape)))
+            if t.dtype != dtype or t.get_device() != device:
                 raise ValueError("%s: %s is %s on %s, X %s on %s" % (what, name, t.dtype, t.device, X.dtype, X.device))
-        positions = 1
-        for n in X.shape[1:-1]:
-            positions *= n
-        if positions == 0:
-            raise ValueError("%s: X %s has no positions to take a mean of" % (what, tuple(X.shape)))
-        if X.shape[0] == 0:
-            return None, gamma, beta
-        if max(X.shape[0] * channels, positions) >= 2 ** 31:
-            raise ValueError("%s: X %s is too large" % (what, tuple(X.shape)))
-        with self._on(X), torch.no_grad():
-            gamma, beta = (None if t is None else _dense(t) for t in (gamma, beta))
-        return _norm_shape(X.shape[0], positions, channels, groups, _FC_TYPES[X.dtype], _FC_TYPES[affine], code, k, eps), gamma, beta
+        return plan
 
     # Batched products with the engine's memory rule (only the last dimension of a tensor is padded to a multiple
     # of 4) and EngineCore's argument mapping (EngineCore.java:579-623): the row pitch and the logical row length
