@@ -192,9 +192,10 @@ struct PairWork {
     void want(const ProductF32& q, int k) { const size_t bytes = k > 1 ? k * static_cast<size_t>(q.rows) * q.cols * sizeof(float) : 0; if (bytes > parts) parts = bytes; }   // (padding too)
     size_t elements() const { size_t e = 0; for (int i = 0; i < n; ++i) e += static_cast<size_t>(p[i].rows) * p[i].pitch; return e; }
     bool fits() const { return elements() < 4ull << 31; }           // 32-bit indices of words of four
-    int split(cudaStream_t stream)
+    // (the first `now` of them; room for what a second launch sees of the others)
+    int split(cudaStream_t stream, int now = 3)
     {
-        const size_t seen_bytes = (most_split_ctas(sms) * sizeof(uint32_t) + 255) & ~static_cast<size_t>(255);
+        const size_t seen_bytes = (most_split_ctas(sms) * (now < n ? 2 : 1) * sizeof(uint32_t) + 255) & ~static_cast<size_t>(255);
         size_t bytes = parts + seen_bytes;
         for (int i = 0; i < n; ++i) bytes += plane_bytes(p[i]);
         void* ws = nullptr;
@@ -207,7 +208,7 @@ struct PairWork {
         for (int i = 0; i < n; ++i) { p[i].ptr = at; at += plane_bytes(p[i]); }
         part = at;
         const Planes* list[3] = {&p[0], &p[1], &p[2]};
-        return launch_split(list, n, seen, &seen_n, sms, stream);
+        return launch_split(list, now < n ? now : n, seen, &seen_n, sms, stream);
     }
 };
 
@@ -434,6 +435,35 @@ namespace alpha {
 int fc_logits_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Y, cudaStream_t stream)
 {
     return forward(s, X, W, bias, nullptr, nullptr, Y, false, stream);
+}
+int fc_logits_and_gradients_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Z, float* dX, float* dW, int (*between)(void*), void* what, cudaStream_t stream)
+{
+    const int rows = s->rows, IC = s->IC, OC = s->OC, pitch = fc_pitch(OC);
+    const FcEpilogue of_z{bias, nullptr, nullptr, Z, pitch, ALPHA_ACT_NONE, 0.f}, of_x{nullptr, nullptr, nullptr, dX, IC, ALPHA_ACT_NONE, 0.f}, of_w{nullptr, nullptr, nullptr, dW, IC, ALPHA_ACT_NONE, 0.f};
+    const ProductF32 z{X, W, rows, pitch, IC, OC, pitch, 1, IC, IC, of_z}, x{Z, W, rows, IC, pitch, OC, pitch, 1, pitch, IC, of_x}, w{Z, X, pitch, IC, rows, OC, pitch, 1, pitch, IC, of_w};
+    PairWork v;
+    int rc = device_sms(&v.sms);
+    if (!rc) rc = device_status_word(&v.status);
+    if (rc) return rc;
+    const PairPlan pz = pick_pair(rows, 1, OC, false, IC, 1, v.sms), px = pick_pair(rows, 1, IC, false, OC, 1, v.sms), pw = pick_pair(OC, 1, IC, false, rows, 1, v.sms);
+    const int a = v.add(X, rows, IC), b = v.add(W, OC, IC), c = v.add(Z, rows, pitch);
+    v.want(z, pz.parts); v.want(x, px.parts); v.want(w, pw.parts);
+    const double pairs = pz.time + px.time + pw.time + split_time(v.elements()) + 2.0;
+    const double apart = pick_gathered<kFcForward>(z, v.sms).time + pick_gathered<kFcDeltaX>(x, v.sms).time + pick_gathered<kFcDeltaW>(w, v.sms).time;
+    if (!dX || !dW || v.sms < 2 || !v.fits() || !pairs_pay(pairs, apart) || rows <= kSmallRows) return 1;
+    rc = v.split(stream, 2);                       // X and W
+    if (rc) return rc;
+    if (dry_run()) return ALPHA_OK;
+    rc = launch_pair<kFcForward>(z, v.p[a], v.p[b], pz, v.part, v.seen, v.seen_n, v.sms, v.status, stream);
+    if (!rc) rc = between(what);
+    const int seen = v.seen_n;
+    if (!rc) {
+        const Planes* one[1] = {&v.p[c]};
+        rc = launch_split(one, 1, v.seen + seen, &v.seen_n, v.sms, stream);
+    }
+    if (!rc) rc = launch_pair<kFcDeltaX>(x, v.p[c], v.p[b], px, v.part, v.seen, seen + v.seen_n, v.sms, v.status, stream);
+    if (!rc) rc = launch_pair<kFcDeltaW>(w, v.p[c], v.p[a], pw, v.part, v.seen, seen + v.seen_n, v.sms, v.status, stream);
+    return rc;
 }
 int fc_gradients_f32(const AlphaFcShape* s, const float* dZ, const float* X, const float* W, float* dX, float* dW, cudaStream_t stream)
 {

@@ -20,6 +20,9 @@ namespace alpha {
 // fp32 products of a call that has begun (fc_api.cu).
 int fc_logits_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Y, cudaStream_t stream);
 int fc_gradients_f32(const AlphaFcShape* s, const float* dZ, const float* X, const float* W, float* dX, float* dW, cudaStream_t stream);
+// Z = X W^T + bias, then between(what), which makes deltaZ of it in place, then both gradients, the planes of X and W split once; 1 where the products are not all
+// best formed from planes, or their scratch is refused (nothing has been launched then).
+int fc_logits_and_gradients_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Z, float* dX, float* dW, int (*between)(void*), void* what, cudaStream_t stream);
 }
 
 namespace {
@@ -107,12 +110,14 @@ long long piece_classes(long long rows, long long classes, size_t size, long lon
 template <class T> int delta_16(const Loss& c, const float* dL, int dL_step, const float* lse, void* dX, void* dW, void* dB)
 {
     const long long rows = c.s->rows, IC = c.s->IC, OC = c.s->OC, piece = piece_classes(rows, OC, 2, 256), pieces = (OC + piece - 1) / piece;
-    int sms = 0;
+    const int dtype = c.s->dtype, most_pitch = fc_pitch(static_cast<int>(piece));
+    int sms = 0, *status = nullptr;
     int rc = device_sms(&sms);
+    if (!rc) rc = device_status_word(&status);
     void *dz = nullptr, *sums = nullptr, *scale = nullptr;
-    if (!rc) rc = call_scratch(c.stream, static_cast<size_t>(rows) * fc_pitch(static_cast<int>(piece)) * 2, &dz);
+    const bool f16 = dtype == ALPHA_F16;
+    if (!rc) rc = call_scratch(c.stream, static_cast<size_t>(rows) * most_pitch * 2, &dz);
     if (!rc && dX && pieces > 1) rc = call_scratch(c.stream, static_cast<size_t>(rows) * IC * 4, &sums);
-    const bool f16 = c.s->dtype == ALPHA_F16;
     if (!rc && f16 && dL_step) rc = call_scratch(c.stream, 2 * sizeof(float), &scale);
     if (rc) return rc;
     if (scale && !dry_run()) {
@@ -128,26 +133,54 @@ template <class T> int delta_16(const Loss& c, const float* dL, int dL_step, con
     for (long long first = 0; first < OC; first += piece) {
         call_rewind(c.stream, mark);
         const long long cols = std::min(piece, OC - first), pitch = fc_pitch(static_cast<int>(cols));
-        const int dtype = c.s->dtype;
         const T* W = static_cast<const T*>(c.W) + first * IC;
         FcLoss l{};
         l.label = c.label; l.label_bytes = c.label_bytes; l.base = static_cast<int>(first); l.classes = c.s->OC;
         l.lse = lse; l.grad = dL_step ? dL : nullptr; l.scale = static_cast<const float*>(scale); l.held = held;
+        FcLoss of_x{}, of_w{};
+        of_x.out_by = of_w.out_by = out_by; of_x.out_factor = of_w.out_factor = out_factor;
+        of_x.sums = static_cast<float*>(sums); of_x.first = first == 0; of_x.last = first + cols == OC;
+        Product x{dtype, c.s->rows, c.s->IC, c.s->IC, static_cast<int>(cols), 1, 1, false, Operand{dz, false, cols, 1, rows, pitch, pitch}, Operand{W, true, IC, cols, 1, IC, cols * IC},
+                  nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f, of_x};
+        const Product w{dtype, static_cast<int>(cols), c.s->IC, c.s->IC, c.s->rows, 1, 1, false, Operand{dz, true, cols, 1, rows, pitch, pitch}, Operand{c.X, true, IC, rows, 1, IC, rows * IC},
+                        nullptr, nullptr, nullptr, dW ? static_cast<T*>(dW) + first * IC : nullptr, ALPHA_ACT_NONE, 0.f, of_w};
+        // deltaX in parts of the classes where that is the least
+        PartsPlan parts{0, 1, 1e300};
+        void* part = nullptr;
+        if (dX) {
+            double other = 0.0, more = 0.0;
+            pick_plan(x, sms, &other);
+            if (dW) pick_plan(w, sms, &more);
+            parts = pick_parts(x, dW ? &w : nullptr, sms);
+            if (parts.parts > 1 && parts.time < 0.93 * (other + more)) {
+                rc = call_scratch(c.stream, static_cast<size_t>(parts.parts) * rows * IC * 4, &part);
+                if (rc && !scratch_refused(rc)) return rc;
+                if (rc) part = nullptr;                      // (without it in one)
+            }
+        }
         if (!dry_run()) {
             const Product z{dtype, c.s->rows, static_cast<int>(cols), static_cast<int>(pitch), c.s->IC, 1, 1, false, Operand{c.X, false, IC, 1, rows, IC, IC}, Operand{W, false, IC, cols, 1, IC, cols * IC},
                             c.bias ? static_cast<const T*>(c.bias) + first : nullptr, nullptr, nullptr, dz, ALPHA_ACT_NONE, 0.f, l};
             rc = launch_product<kFcSoftmaxDelta>(z, c.stream);
             if (rc) return rc;
-            FcLoss of_x{}, of_w{};
-            of_x.out_by = of_w.out_by = out_by; of_x.out_factor = of_w.out_factor = out_factor;
-            of_x.sums = static_cast<float*>(sums); of_x.first = first == 0; of_x.last = first + cols == OC;
-            const Product x{dtype, c.s->rows, c.s->IC, c.s->IC, static_cast<int>(cols), 1, 1, false, Operand{dz, false, cols, 1, rows, pitch, pitch}, Operand{W, true, IC, cols, 1, IC, cols * IC},
-                            nullptr, nullptr, nullptr, dX, ALPHA_ACT_NONE, 0.f, of_x};
-            const Product w{dtype, static_cast<int>(cols), c.s->IC, c.s->IC, c.s->rows, 1, 1, false, Operand{dz, true, cols, 1, rows, pitch, pitch}, Operand{c.X, true, IC, rows, 1, IC, rows * IC},
-                            nullptr, nullptr, nullptr, dW ? static_cast<T*>(dW) + first * IC : nullptr, ALPHA_ACT_NONE, 0.f, of_w};
-            if (dX && dW) rc = launch_products<kFcSum>(x, w, c.stream);
-            else if (dX) rc = launch_product<kFcSum>(x, c.stream);
-            else if (dW) rc = launch_product<kFcSum>(w, c.stream);
+            if (part) {
+                x.loss.sums = static_cast<float*>(part);
+                x.loss.parts = parts.parts;
+                rc = launch_planned<kFcSum>(x, dW ? &w : nullptr, FcPlan{true, parts.bn, 1}, sms, status, c.stream);
+                if (rc) return rc;
+                note_plan("fc loss pair 256x%d parts=%d", parts.bn, parts.parts);
+                const size_t words = static_cast<size_t>(rows) * IC / 4;
+                launch_after(loss_parts_kernel<T>, static_cast<unsigned>(std::min<size_t>((words + 255) / 256, 8u * sms)), 256, 0, c.stream, static_cast<const float4*>(part), parts.parts, words,
+                             static_cast<float4*>(sums), of_x.first, of_x.last, out_by, out_factor, static_cast<uint2*>(dX));
+                note_launch("fc_loss");
+                rc = launched("loss_parts_kernel");
+            } else if (dX && dW) {
+                rc = launch_products<kFcSum>(x, w, c.stream);
+            } else if (dX) {
+                rc = launch_product<kFcSum>(x, c.stream);
+            } else if (dW) {
+                rc = launch_product<kFcSum>(w, c.stream);
+            }
             if (rc) return rc;
         }
         if (dB) rc = column_sums(static_cast<const T*>(dz), c.s->rows, static_cast<int>(pitch), out_by, out_factor, static_cast<T*>(dB) + first, sms, c.stream);
@@ -194,16 +227,25 @@ int delta_f32(const Loss& c, const float* dL, int dL_step, const float* lse, flo
         s.OC = static_cast<int>(std::min(piece, OC - first));
         const float *X = static_cast<const float*>(c.X), *W = static_cast<const float*>(c.W) + first * IC;
         float* z = static_cast<float*>(dz);
-        rc = fc_logits_f32(&s, X, W, c.bias ? static_cast<const float*>(c.bias) + first : nullptr, z, c.stream);
-        if (!rc && !dry_run()) {
+        const float* bias = c.bias ? static_cast<const float*>(c.bias) + first : nullptr;
+        float* x = dX && first ? static_cast<float*>(more) : dX;
+        float* w = dW ? dW + first * IC : nullptr;
+        auto softmax = [&] {
+            if (dry_run()) return static_cast<int>(ALPHA_OK);
             launch_after(loss_delta_kernel, static_cast<unsigned>(rows), kRowThreads, 0, c.stream, z, fc_pitch(s.OC), s.OC, static_cast<int>(first), c.s->OC, c.label, c.label_bytes, lse, dL, dL_step);
             note_launch("fc_loss");
-            rc = launched("loss_delta_kernel");
+            return launched("loss_delta_kernel");
+        };
+        rc = fc_logits_and_gradients_f32(&s, X, W, bias, z, x, w, [](void* f) { return (*static_cast<decltype(softmax)*>(f))(); }, &softmax, c.stream);
+        if (rc < 0) return rc;
+        if (rc == 1) {
+            call_rewind(c.stream, mark);
+            rc = fc_logits_f32(&s, X, W, bias, z, c.stream);
+            if (!rc) rc = softmax();
+            if (rc) return rc;
+            call_rewind(c.stream, mark);                 // (what the logits' product was given)
+            if (dX || dW) rc = fc_gradients_f32(&s, z, X, W, x, w, c.stream);
         }
-        if (rc) return rc;
-        float* x = dX && first ? static_cast<float*>(more) : dX;
-        call_rewind(c.stream, mark);                 // (what the logits' product was given)
-        if (dX || dW) rc = fc_gradients_f32(&s, z, X, W, x, dW ? dW + first * IC : nullptr, c.stream);
         if (!rc && dX && first && !dry_run()) {
             const size_t words = static_cast<size_t>(rows) * IC / 4;
             launch_after(loss_add_kernel, static_cast<unsigned>(std::min<size_t>((words + 255) / 256, 8u * sms)), 256, 0, c.stream, reinterpret_cast<float4*>(dX), reinterpret_cast<const float4*>(x), words);

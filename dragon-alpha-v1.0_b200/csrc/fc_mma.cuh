@@ -49,6 +49,7 @@ struct FcLoss {
     const float* out_by; float out_factor;   // kFcSum: what outputs are multiplied by (NULL: 1), and once more
     float* sums;                             // [rows][pitch] of kFcSum, or NULL: one product
     int first, last;                         // product of those that add up
+    int parts;                               // kFcSum: parts of the reduction, tiles of their own, which leave [part][rows][pitch] in `sums` (1: none)
 };
 struct FcMma {
     int rows, cols;               // outputs: rows of a half, pitch (glu: of a half of Z too)
@@ -116,12 +117,20 @@ __global__ void __launch_bounds__(kFcThreads, 1)
     const uint32_t tmem_base = *tmem_holder;
 
     // (shared tiles: the launch has a cluster for each)
-    const int tiles = p.m_tiles * p.n_tiles, total = tiles + (TWO ? p2.m_tiles * p2.n_tiles : 0), step = gridDim.x / (CTAS * split), first = blockIdx.x / (CTAS * split);
+    const int tiles = p.m_tiles * p.n_tiles * (EPI == kFcSum ? p.loss.parts : 1), total = tiles + (TWO ? p2.m_tiles * p2.n_tiles : 0), step = gridDim.x / (CTAS * split), first = blockIdx.x / (CTAS * split);
     const FcMma* cur = &p;                        // the product of the tile at hand
     int hm = 0;                                   // the half of its rows
-    auto tile_at = [&](int t, int& m0, int& n0) {
+    int part = 0;                                 // of its reduction
+    auto part_at = [&](int& t) {
         if (TWO) cur = t < tiles ? &p : &p2;
         if (TWO && t >= tiles) t -= tiles;
+        if constexpr (EPI == kFcSum) {
+            part = t / (cur->m_tiles * cur->n_tiles);
+            t -= part * cur->m_tiles * cur->n_tiles;
+        }
+    };
+    auto tile_at = [&](int t, int& m0, int& n0) {
+        part_at(t);
         const int per = kFcGroupM * cur->n_tiles, g = t / per, r = t - g * per, left = cur->m_tiles - g * kFcGroupM, rows = left < kFcGroupM ? left : kFcGroupM;
         const int n = r / rows, m = g * kFcGroupM + r - n * rows;
         hm = m >= cur->m_half ? 1 : 0;
@@ -129,8 +138,8 @@ __global__ void __launch_bounds__(kFcThreads, 1)
         n0 = n * OUT;
     };
     auto steps_of = [&](int& begin, int& end) {
-        const int each = (cur->kb + split - 1) / split;
-        begin = PAIR ? 0 : static_cast<int>(rank) * each;
+        const int ways = EPI == kFcSum && split == 1 ? cur->loss.parts : split, each = (cur->kb + ways - 1) / ways;
+        begin = EPI == kFcSum && split == 1 ? part * each : PAIR ? 0 : static_cast<int>(rank) * each;
         end = begin + each < cur->kb ? begin + each : cur->kb;
     };
     const uint32_t smem_a = smem_u32(smem);
@@ -205,16 +214,17 @@ __global__ void __launch_bounds__(kFcThreads, 1)
             // (a lane has 128 bytes of its row of the fp32 sums)
             const FcLoss& l = cur->loss;
             if (l.sums && row0 + lane < cur->rows) {
-                float* at = l.sums + static_cast<size_t>(row0 + lane) * cur->cols + col0;
+                float* at = l.sums + (static_cast<size_t>(part) * cur->rows + row0 + lane) * cur->cols + col0;
+                const bool alone = l.first || l.parts > 1, keep = !l.last || l.parts > 1;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     if (4 * q >= width || col0 + 4 * q >= cur->cols) continue;
                     float4* word = reinterpret_cast<float4*>(at + 4 * q);
-                    if (!l.first) { const float4 v = *word; z[4 * q] += v.x; z[4 * q + 1] += v.y; z[4 * q + 2] += v.z; z[4 * q + 3] += v.w; }
-                    if (!l.last) *word = make_float4(z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]);
+                    if (!alone) { const float4 v = *word; z[4 * q] += v.x; z[4 * q + 1] += v.y; z[4 * q + 2] += v.z; z[4 * q + 3] += v.w; }
+                    if (keep) *word = make_float4(z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]);
                 }
             }
-            if (l.sums && !l.last) return;
+            if (l.sums && (!l.last || l.parts > 1)) return;
             const float by = (l.out_by ? __ldg(l.out_by) : 1.f) * l.out_factor;
 #pragma unroll
             for (int i = 0; i < 32; ++i) z[i] *= by;
@@ -369,7 +379,8 @@ __global__ void __launch_bounds__(kFcThreads, 1)
             RingPos rp, ap;
             bool next = false;                            // the stage at rp is known to be full
             for (int t = first; t < total && ok; t += step) {
-                if (TWO) cur = t < tiles ? &p : &p2;
+                int at = t;
+                part_at(at);
                 int k_begin, k_end;
                 steps_of(k_begin, k_end);
                 const uint32_t a_k = cur->a_mn ? 128u : 2u, b_k = cur->b_mn ? 128u : 2u, idesc = cur->idesc;      // 16 steps further, in 16-byte units
@@ -506,7 +517,10 @@ __global__ void __launch_bounds__(kFcThreads, 1)
                         if constexpr (GLU) load32(d + OUT + c, u);
                         if (c + 64 >= OUT || n0 + c + 64 >= cur->cols) { give_back(); held = false; }
                         if constexpr (EPI == kFcStats) stats(z, row0 + lane, n0 + c, OUT - c);
-                        else if constexpr (EPI == kFcSoftmaxDelta) { softmax_delta(z, n0 + c); put(z, static_cast<T*>(cur->Y), cur->cols, row0, n0 + c, OUT - c); }
+                        else if constexpr (EPI == kFcSoftmaxDelta) {
+                            softmax_delta(z, n0 + c);
+                            put(z, static_cast<T*>(cur->Y), cur->cols, row0, n0 + c, OUT - c);
+                        }
                         else finish(z, u, r, row0, n0 + c, OUT - c);
                         if (fetching && c + 64 < OUT) fetch(r, row0, n0 + c + 64, OUT - c - 64);
                     }

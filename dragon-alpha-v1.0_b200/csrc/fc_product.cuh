@@ -174,6 +174,7 @@ int prepare(const Product& q, const FcPlan& plan, int a_rows, int* status, Prepa
     p.act = q.act; p.k = q.k; p.keep_z = q.Z != nullptr;
     p.bias = q.bias; p.residual = q.residual; p.Y = q.Y; p.Z = q.Z; p.status = status;
     p.loss = q.loss;
+    if (p.loss.parts < 1) p.loss.parts = 1;
     const int rc = q.A.mn ? make_map(&out->a, q.dtype, q.A, 64, 1, 64) : make_map(&out->a, q.dtype, q.A, 64, 1, a_rows);
     if (rc) return rc;
     return q.B.mn ? make_map(&out->b, q.dtype, q.B, 64, 64, 1) : make_map(&out->b, q.dtype, q.B, 64, plan.pair ? bn / 2 : cols_of, 1);
@@ -183,7 +184,7 @@ template <class T, int PAIR, bool GLU, bool TWO, int EPI>
 void launch_mma(const Prepared& x, const Prepared& y, int sms, cudaStream_t stream)
 {
     const FcMma& p = x.p;
-    const int group = PAIR ? 2 : p.split, total = p.m_tiles * p.n_tiles + (TWO ? y.p.m_tiles * y.p.n_tiles : 0), most = sms / group;
+    const int group = PAIR ? 2 : p.split, total = p.m_tiles * p.n_tiles * p.loss.parts + (TWO ? y.p.m_tiles * y.p.n_tiles : 0), most = sms / group;
     const unsigned grid = static_cast<unsigned>(p.split > 1 || total < most ? total : most) * group;
     const uint32_t smem = p.stages * fc_blocks(PAIR != 0, p.bn) * fc_block_bytes(PAIR != 0, p.a_rows, p.bn) + kFcStaging + 1024 + 512;
     allow_smem<fc_mma_kernel<T, PAIR, GLU, TWO, EPI>>();
@@ -255,6 +256,39 @@ int launch_products(const Product& x, const Product& w, cudaStream_t stream)
     if (best.bn && least < 0.97 * apart) return launch_planned<EPI>(x, &w, best, sms, status, stream);
     rc = launch_planned<EPI>(x, nullptr, px, sms, status, stream);
     return rc ? rc : launch_planned<EPI>(w, nullptr, pw, sms, status, stream);
+}
+// deltaX of a loss, its reduction over the classes in parts of its own tiles, beside deltaW (or alone) in one launch of CTA pairs.
+struct PartsPlan { int bn, parts; double time; };
+PartsPlan pick_parts(const Product& x, const Product* w, int sms)
+{
+    PartsPlan best{0, 1, 1e300};
+    const int pairs = sms / 2, forced = option_fc_tile();
+    if (pairs < 1 || forced == 3 || forced >= 1000) return best;
+    const long long kx = (x.K + 63) / 64, kw = w ? (w->K + 63) / 64 : 0;
+    double bytes = 2.0 * ((double)(x.rows + x.cols) * x.K + (double)x.rows * x.cols);
+    if (w) bytes += 2.0 * ((double)(w->rows + w->cols) * w->K + (double)w->rows * w->cols);
+    for (int bn = 256; bn >= 128; bn /= 2) {
+        if (forced == (bn == 256 ? 11 : 1)) continue;
+        // (a stage holds two blocks of 64 steps where columns are 128)
+        const int unit = fc_blocks(true, bn);
+        const double step = bn == 256 ? 0.32 : fc_block_bytes(true, 128, bn) / 112e3, least = 0.28 + 0.0053 * bn;
+        const long long tx = (long long)((x.rows + 255) / 256) * ((x.cols + bn - 1) / bn), tw = w ? (long long)((w->rows + 255) / 256) * ((w->cols + bn - 1) / bn) : 0, stages = (kx + unit - 1) / unit;
+        // (where the tiles alone fill the pairs parts save nothing)
+        for (int parts = 2; parts <= 16 && parts <= stages && tx < pairs; ++parts) {
+            const long long each = (stages + parts - 1) / parts, items = tx * parts;
+            if ((parts - 1) * each >= stages) continue;
+            const double cx = std::max(each * unit * step, least) + 0.3, cw = std::max(kw * step, least) + 0.3;
+            double busy = 0.0;
+            for (int i = 0; i < pairs; ++i) {
+                const long long nx = items > i ? (items - i + pairs - 1) / pairs : 0, all = items + tw > i ? (items + tw - i + pairs - 1) / pairs : 0;
+                busy = std::max(busy, nx * cx + (all - nx) * cw);
+            }
+            const double joined = 3.5 + (double)x.rows * x.cols * 4e-6 * (parts + 1) / 5.0;
+            const double time = 5.8 + std::max(busy, bytes * 1e-6 / 5.9) + joined;
+            if (time < best.time) best = PartsPlan{bn, parts, time};
+        }
+    }
+    return best;
 }
 
 }  // namespace
