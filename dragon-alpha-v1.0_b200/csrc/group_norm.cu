@@ -43,14 +43,13 @@ Norm norm_of(const AlphaNormShape* s)
 }
 
 // Instructions an element takes: in the passes over shared memory, and in the streamed ones.
-double norm_instructions(const Norm& p, bool back, bool streamed)
+double norm_instructions(const Norm& p, int size, bool back, bool streamed)
 {
-    const bool plain = p.act == ALPHA_ACT_NONE || p.act == ALPHA_ACT_LEAKY_RELU;
-    return streamed ? (back ? (plain ? 26.0 : 42.0) : (plain ? 17.0 : 23.0)) : (back ? (plain ? 14.0 : 22.0) : (plain ? 9.0 : 15.0));
+    const bool plain = p.act == ALPHA_ACT_NONE || p.act == ALPHA_ACT_LEAKY_RELU, once = size == 4;         // (once: dz is kept)
+    return streamed ? (back ? (plain ? 26.0 : 40.0) : (plain ? 16.0 : 21.0)) : (back ? (once ? (plain ? 14.0 : 22.0) : (plain ? 20.0 : 30.0)) : (plain ? 9.0 : 14.0));
 }
 // The slab and the cluster of least estimated time (us); false: no slab fits.  A CTA takes of its SM what its bytes take at 45 KB a us or its instructions at 4000 a us (of a
-// warp), whichever is more - both, and its loads' latency, where it is alone there - and its sums and barriers, 0.9 us (backward 2) and 0.1 for each CTA of the cluster.
-// Measured / estimated over 35 plans of five tensors: 0.98 with a deviation of 12 %.
+// warp), whichever is more - both, and its loads' latency, where it is alone there - and its sums and barriers, 0.9 us (backward 1.2) and 0.1 for each CTA of the cluster.
 bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* least)
 {
     const long long unit = static_cast<long long>(p.D) * 4 / std::gcd(p.D, 4);
@@ -69,9 +68,9 @@ bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* 
             const int fit = static_cast<int>(227 * 1024 / (bytes + 1024)), most = 1024 / kNormThreads, at_once = fit < most ? fit : most;
             const double elements = static_cast<double>(part) * words * 4, places = sms * at_once * (cl < 4 ? 1.0 : 0.9);
             const double row = words * 4.0 * size, narrow = row >= 64 ? 1.0 : row >= 32 ? 1.1 : 2.0;
-            const double memory = elements * size * (back ? 3 : 2) / 45e3 * narrow, math = elements * norm_instructions(p, back, false) / 32 / 4000.0;
+            const double memory = elements * size * (back ? 3 : 2) / 45e3 * narrow, math = elements * norm_instructions(p, size, back, false) / 32 / 4000.0;
             const double alone = at_once == 1 ? 1.0 : at_once == 2 ? 0.4 : 0.0;
-            const double each_cta = std::max(memory, math) + alone * (std::min(memory, math) + 1.5) + (back ? 2.0 : 0.9) + 0.1 * cl;
+            const double each_cta = std::max(memory, math) + alone * (std::min(memory, math) + 1.5) + (back ? 1.2 : 0.9) + 0.1 * cl;
             // (what is there at once runs at once, in whole waves as long as these are few)
             const double waves = ctas / places, rounds = waves <= 1.0 ? 1.0 : waves < 4.0 ? std::ceil(waves) * 0.5 + waves * 0.5 : waves;
             const double on_sm = waves <= 1.0 ? std::max(1.0, std::ceil(static_cast<double>(ctas) / sms)) : at_once;
@@ -112,8 +111,8 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
     const size_t word = 4 * sizeof(T);
     const bool words = p.C % 4 == 0 && aligned(p.X, word) && aligned(p.out, word) && aligned(p.dY, word);
     // streamed: both passes over the tensors, the second through L2 as far as that holds them, and two more launches
-    const double bytes = static_cast<double>(p.N) * p.R * p.C * sizeof(T) * (BACK ? 2 : 1), rate = 45e3 * sms;
-    const double math = static_cast<double>(p.N) * p.R * p.C * norm_instructions(p, BACK, true) / 32 / (3800.0 * sms);
+    const double bytes = static_cast<double>(p.N) * p.R * p.C * sizeof(T) * (BACK ? 2 : 1), rate = 40e3 * sms;
+    const double math = static_cast<double>(p.N) * p.R * p.C * norm_instructions(p, sizeof(T), BACK, true) / 32 / (3800.0 * sms);
     const double streamed = (NORM_FORCE(-1, -1) ? 14.0 : 1e9) + std::max(math, bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate);
     size_t smem = 0;
     double least = 0.0;

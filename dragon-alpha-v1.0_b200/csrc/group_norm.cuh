@@ -10,7 +10,7 @@
 // memory by asynchronous copies, forms the sums there, adds those of its cluster, and writes the outputs from shared memory: each tensor crosses HBM once.  Several CTAs
 // to an SM, so that one copies while another computes or stores.  A thread keeps one word of the row (four channels) and walks the positions, so that the words of
 // neighbouring threads are neighbours in memory and a thread reads only what it copied itself.  Words of four elements, not of 16 bytes: what a thread holds of
-// its channels fits 64 registers, for 32 warps on an SM.  Backward dz is kept in shared memory in fp32, so that a slope is formed once: arithmetic is the second bound.
+// its channels fits 64 registers, for 32 warps on an SM.  Arithmetic is the second bound.
 //
 // Streamed: what does not fit (and widths that are no multiple of four, a thread to an element): partial sums of runs of positions, their sum, and a second pass over
 // the tensors, from their end, so that it begins with what the first left in L2.
@@ -78,6 +78,8 @@ template <class T> struct NormWord<T, 1> {
     static __device__ Raw store(const float2 (&f)[1]) { return static_cast<T>(f[0].x); }
 };
 template <class T> constexpr bool kNormFast = sizeof(T) == 2;
+// Backward: dz takes the place of deltaY in shared memory, so that a slope is formed once - in fp32; of 16-bit tensors it would take twice deltaY's room, and slopes are cheaper.
+template <class T> constexpr bool kKeepDz = sizeof(T) == 4;
 
 // Activations of 16-bit tensors by s = 1 / (1 + exp(-u)), good to 2^-21 of its value down to u = -87 and 0 below that (1e-38); two values at a time.
 __device__ __forceinline__ float2 exp_of(float2 u)                // exp(-u)
@@ -217,10 +219,10 @@ __device__ __forceinline__ void channel_sums(float* red, const Norm& p, int arra
 
 __device__ __forceinline__ void st_cluster_f2(uint32_t at, float x, float y) { asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory"); }
 
-// Shared memory of a resident CTA: its words of X, backward 16 bytes for each of deltaY and dz; four (eight) sums of each thread, the groups' sums of every CTA of the cluster, their total.
+// Shared memory of a resident CTA: its words of X, backward of deltaY; four (eight) sums of each thread, the groups' sums of every CTA of the cluster, their total.
 __host__ __device__ inline size_t norm_smem(bool back, int size, int part, int words, int groups, int cluster)
 {
-    const size_t tensors = (static_cast<size_t>(part) * words * (4 * size + (back ? 16 : 0)) + 15) & ~static_cast<size_t>(15);
+    const size_t tensors = (static_cast<size_t>(part) * words * 4 * size * (back ? 2 : 1) + 15) & ~static_cast<size_t>(15);
     return tensors + kNormThreads * 16 * (back ? 2 : 1) + static_cast<size_t>(groups) * 8 * (cluster + 1);
 }
 
@@ -239,9 +241,9 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_reside
     const int ty = ty_, tx = tx_, c = slab * p.words * 4 + tx * 4;
     const bool busy = ty < p.rows;
     const int first = busy ? ty * p.words + tx : 0, step = p.rows * p.words, last = busy ? mine * p.words : 0;      // its words: first, first + step, ... < last
-    float4* ds = reinterpret_cast<float4*>(smem);                                                                    // deltaY, then dz
-    Raw* xs = reinterpret_cast<Raw*>(smem + (BACK ? static_cast<size_t>(p.part) * p.words * 16 : 0));
-    float* red = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(xs) + ((static_cast<size_t>(p.part) * p.words * sizeof(Raw) + 15) & ~static_cast<size_t>(15)));
+    Raw* xs = reinterpret_cast<Raw*>(smem);
+    Raw* ys = xs + static_cast<size_t>(p.part) * p.words;                                                            // deltaY; of fp32 tensors dz later
+    float* red = reinterpret_cast<float*>(smem + ((static_cast<size_t>(p.part) * p.words * sizeof(Raw) * (BACK ? 2 : 1) + 15) & ~static_cast<size_t>(15)));
     float2* parts = reinterpret_cast<float2*>(red + 4 * kNormThreads * (BACK ? 2 : 1));    // [rank][group], written by every CTA of the cluster
     float2* all = parts + cl * groups;
     const size_t from = (static_cast<size_t>(n) * p.R + r0 + ty) * p.C + c, jump = static_cast<size_t>(p.rows) * p.C, at_group = static_cast<size_t>(n) * p.G + slab * groups;
@@ -249,12 +251,12 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_reside
     grid_dependency_trigger();
     {
         const T *x = static_cast<const T*>(p.X) + from, *y = BACK ? static_cast<const T*>(p.dY) + from : nullptr;
-        const uint32_t to_y = smem_u32(ds), to = smem_u32(xs);
+        const uint32_t to = smem_u32(xs), to_y = smem_u32(ys);
 #pragma unroll 4
         for (int i = first; i < last; i += step) {
             copy_async<sizeof(Raw)>(to + i * sizeof(Raw), x);
             x += jump;
-            if (BACK) { copy_async<sizeof(Raw)>(to_y + i * 16, y); y += jump; }
+            if (BACK) { copy_async<sizeof(Raw)>(to_y + i * sizeof(Raw), y); y += jump; }
         }
     }
     int gi[4];                                                                             // groups of its channels, within the slab
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_reside
             for (int i = first; i < last; i += step) {
                 float2 x[2], y[2];
                 W::load(xs[i], x);
-                W::load(*reinterpret_cast<const Raw*>(ds + i), y);
+                W::load(ys[i], y);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     x[j] = add2(x[j], mean[j]);
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_reside
                     s[j] = add2(s[j], y[j]);
                     q[j] = fma2(y[j], x[j], q[j]);
                 }
-                ds[i] = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+                if constexpr (kKeepDz<T>) ys[i] = W::store(y);
             }
         });
 #pragma unroll
@@ -415,16 +417,23 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_reside
             base[j] = neg2(mul2(rstd[j], make_float2(d.x, e.x)));
             more[j] = neg2(mul2(mul2(rstd[j], rstd[j]), make_float2(d.y, e.y)));
         }
-#pragma unroll 4
-        for (int i = first; i < last; i += step) {
-            float2 x[2];
-            W::load(xs[i], x);
-            const float4 d = ds[i];
-            x[0] = fma2(make_float2(d.x, d.y), scale[0], fma2(add2(x[0], mean[0]), more[0], base[0]));
-            x[1] = fma2(make_float2(d.z, d.w), scale[1], fma2(add2(x[1], mean[1]), more[1], base[1]));
-            *reinterpret_cast<Raw*>(out) = W::store(x);
-            out += jump;
-        }
+        with_act(kKeepDz<T> ? ALPHA_ACT_NONE : p.act, [&](auto a) {
+            constexpr int ACT = decltype(a)::value;
+#pragma unroll 2
+            for (int i = first; i < last; i += step) {
+                float2 x[2], d[2];
+                W::load(xs[i], x);
+                W::load(ys[i], d);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    x[j] = add2(x[j], mean[j]);
+                    if (ACT != ALPHA_ACT_NONE) d[j] = mul2(d[j], norm_slope<ACT, kNormFast<T>>(fma2(x[j], scale[j], beta[j]), p.k));
+                    x[j] = fma2(d[j], scale[j], fma2(x[j], more[j], base[j]));
+                }
+                *reinterpret_cast<Raw*>(out) = W::store(x);
+                out += jump;
+            }
+        });
     }
 }
 
@@ -460,6 +469,28 @@ template <class T, int V, bool TWO> struct NormRows {
                 for (int i = 0; i < have; ++i) copy(i);
             }
             copies_commit();
+        }
+    }
+    // f(word of x, word of y) for each row, a few at a time in the instruction stream (batches unrolled as a whole miss the instruction cache)
+    template <class F> __device__ void rows(F&& f) const
+    {
+        if constexpr (V == 1) {
+            each([&](int, int have, const Raw (&rx)[U], const Raw (&ry)[U]) {
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+                    if (i < have) f(rx[i], ry[i]);
+            });
+        } else {
+            for (int b = 0; b < S - 1; ++b) issue(b);
+            const int batches = (total + U - 1) / U;
+            for (int b = 0; b < batches; ++b) {
+                const int have = min(U, total - b * U);
+                issue(b + S - 1);
+                copies_wait<S - 1>();
+                const Raw* from = at(b, 0, 0);
+#pragma unroll 2
+                for (int i = 0; i < have; ++i, from += (TWO ? 2 : 1) * kNormThreads) f(from[0], from[TWO ? kNormThreads : 0]);
+            }
         }
     }
     // f(first row, rows, words of x, words of y) for each batch; rows < U: the last
@@ -577,21 +608,16 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_sums_k
             }
             with_act(p.act, [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
-                rows.each([&](int, int have, const Raw (&rx)[U], const Raw (&ry)[U]) {
+                rows.rows([&](const Raw& rx, const Raw& ry) {
+                    float2 fx[P], fy[P];
+                    W::load(rx, fx);
+                    W::load(ry, fy);
 #pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        if (i >= have) break;
-                        float2 fx[P], fy[P];
-                        W::load(rx[i], fx);
-                        W::load(ry[i], fy);
-#pragma unroll
-                        for (int j = 0; j < P; ++j) {
-                            fx[j] = add2(fx[j], mean[j]);
-                            const float2 z = fma2(fx[j], gamma[j], beta[j]);
-                            if (ACT != ALPHA_ACT_NONE) fy[j] = mul2(fy[j], norm_slope<ACT, kNormFast<T>>(z, p.k));
-                            s[j] = add2(s[j], fy[j]);
-                            q[j] = fma2(fy[j], fx[j], q[j]);
-                        }
+                    for (int j = 0; j < P; ++j) {
+                        fx[j] = add2(fx[j], mean[j]);
+                        if (ACT != ALPHA_ACT_NONE) fy[j] = mul2(fy[j], norm_slope<ACT, kNormFast<T>>(fma2(fx[j], gamma[j], beta[j]), p.k));
+                        s[j] = add2(s[j], fy[j]);
+                        q[j] = fma2(fy[j], fx[j], q[j]);
                     }
                 });
             });
@@ -733,7 +759,7 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_apply_
     using W = NormWord<T, V>;
     using Rows = NormRows<T, V, BACK>;
     using Raw = typename Rows::Raw;
-    constexpr int U = Rows::U, P = (V + 1) / 2;
+    constexpr int P = (V + 1) / 2;
     extern __shared__ __align__(128) uint8_t smem[];
     grid_dependency_wait();
     grid_dependency_trigger();
@@ -761,27 +787,23 @@ __global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_apply_
     T* out = static_cast<T*>(p.out) + begin;
     with_act(p.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
-        rows.each([&](int, int have, const Raw (&rx)[U], const Raw (&ry)[U]) {
+        rows.rows([&](const Raw& rx, const Raw& ry) {
+            float2 f[P], fy[P];
+            W::load(rx, f);
+            if (BACK) W::load(ry, fy);
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (i >= have) break;
-                float2 f[P], fy[P];
-                W::load(rx[i], f);
-                if (BACK) W::load(ry[i], fy);
-#pragma unroll
-                for (int j = 0; j < P; ++j) {
-                    f[j] = add2(f[j], mean[j]);
-                    const float2 z = fma2(f[j], gamma[j], beta[j]);
-                    if constexpr (BACK) {
-                        if (ACT != ALPHA_ACT_NONE) fy[j] = mul2(fy[j], norm_slope<ACT, kNormFast<T>>(z, p.k));
-                        f[j] = fma2(fy[j], gamma[j], fma2(f[j], more[j], base[j]));
-                    } else {
-                        f[j] = norm_value<ACT, kNormFast<T>>(z, p.k);
-                    }
+            for (int j = 0; j < P; ++j) {
+                f[j] = add2(f[j], mean[j]);
+                const float2 z = fma2(f[j], gamma[j], beta[j]);
+                if constexpr (BACK) {
+                    if (ACT != ALPHA_ACT_NONE) fy[j] = mul2(fy[j], norm_slope<ACT, kNormFast<T>>(z, p.k));
+                    f[j] = fma2(fy[j], gamma[j], fma2(f[j], more[j], base[j]));
+                } else {
+                    f[j] = norm_value<ACT, kNormFast<T>>(z, p.k);
                 }
-                *reinterpret_cast<Raw*>(out) = W::store(f);
-                out += step;
             }
+            *reinterpret_cast<Raw*>(out) = W::store(f);
+            out += step;
         });
     });
 }
