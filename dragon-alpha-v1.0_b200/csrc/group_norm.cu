@@ -8,12 +8,6 @@
 
 using namespace alpha;
 
-#ifdef NORM_DEV
-#include <cstdlib>
-#define NORM_FORCE(w, c) (!getenv("NW") || (w == atoi(getenv("NW")) && c == atoi(getenv("NC"))))
-#else
-#define NORM_FORCE(w, c) true
-#endif
 namespace {
 
 int check_norm(const char* what, const AlphaNormShape* s)
@@ -65,7 +59,7 @@ bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* 
             if (static_cast<long long>(cl - 1) * part >= p.R || part > (1 << 20) || ctas > 2147483647LL) continue;
             const size_t bytes = norm_smem(back, size, part, words, words * 4 / p.D, cl);
             if (bytes > 224 * 1024) continue;
-            const int fit = static_cast<int>(227 * 1024 / (bytes + 1024)), most = 1024 / kNormThreads, at_once = fit < most ? fit : most;
+            const int fit = static_cast<int>(227 * 1024 / (bytes + 1024)), at_once = fit < 4 ? fit : 4;
             const double elements = static_cast<double>(part) * words * 4, places = sms * at_once * (cl < 4 ? 1.0 : 0.9);
             const double row = words * 4.0 * size, narrow = row >= 64 ? 1.0 : row >= 32 ? 1.1 : 2.0;
             const double memory = elements * size * (back ? 3 : 2) / 45e3 * narrow, math = elements * norm_instructions(p, size, back, false) / 32 / 4000.0;
@@ -75,7 +69,7 @@ bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* 
             const double waves = ctas / places, rounds = waves <= 1.0 ? 1.0 : waves < 4.0 ? std::ceil(waves) * 0.5 + waves * 0.5 : waves;
             const double on_sm = waves <= 1.0 ? std::max(1.0, std::ceil(static_cast<double>(ctas) / sms)) : at_once;
             const double time = 4.0 + rounds * on_sm * each_cta;
-            if (NORM_FORCE(words, cl) && time < *least) {
+            if (time < *least) {
                 *least = time;
                 p.words = words; p.slabs = slabs; p.cluster = cl; p.part = part; p.rows = kNormThreads / words;
                 *smem = bytes;
@@ -113,7 +107,7 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
     // streamed: both passes over the tensors, the second through L2 as far as that holds them, and two more launches
     const double bytes = static_cast<double>(p.N) * p.R * p.C * sizeof(T) * (BACK ? 2 : 1), rate = 40e3 * sms;
     const double math = static_cast<double>(p.N) * p.R * p.C * norm_instructions(p, sizeof(T), BACK, true) / 32 / (3800.0 * sms);
-    const double streamed = (NORM_FORCE(-1, -1) ? 14.0 : 1e9) + std::max(math, bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate);
+    const double streamed = 14.0 + std::max(math, bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate);
     size_t smem = 0;
     double least = 0.0;
     const bool resident = words && plan_resident(p, sizeof(T), BACK, sms, &smem, &least) && least < streamed;

@@ -28,10 +28,7 @@
 
 namespace alpha {
 
-#ifndef NORM_T
-#define NORM_T 256
-#endif
-constexpr int kNormThreads = NORM_T;
+constexpr int kNormThreads = 256;
 
 struct Norm {
     const void *X, *dY;
@@ -227,7 +224,7 @@ __host__ __device__ inline size_t norm_smem(bool back, int size, int part, int w
 }
 
 template <class T, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_resident_kernel(const __grid_constant__ Norm p)
+__global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __grid_constant__ Norm p)
 {
     using W = NormWord<T, 4>;
     using Raw = typename W::Raw;
@@ -537,7 +534,7 @@ template <int V> __device__ __forceinline__ NormAt norm_at(const Norm& p, unsign
 }
 // Mean and squared differences of a run, or its sums of dz and dz xh, for every channel.
 template <class T, int V, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_sums_kernel(const __grid_constant__ Norm p)
+__global__ void __launch_bounds__(kNormThreads, 4) norm_sums_kernel(const __grid_constant__ Norm p)
 {
     using W = NormWord<T, V>;
     using Rows = NormRows<T, V, BACK>;
@@ -754,7 +751,7 @@ __global__ void __launch_bounds__(kJoinNormThreads) norm_join_kernel(const __gri
 }
 // The outputs, from the end of the tensors.
 template <class T, int V, bool BACK>
-__global__ void __launch_bounds__(kNormThreads, 1024 / kNormThreads) norm_apply_kernel(const __grid_constant__ Norm p)
+__global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(const __grid_constant__ Norm p)
 {
     using W = NormWord<T, V>;
     using Rows = NormRows<T, V, BACK>;

@@ -573,6 +573,11 @@ def _dense(t):
     return t.resolve_neg().contiguous()
 
 
+def _present(tensors):
+    """Those of a list that are not None: the list itself where all are."""
+    return [t for t in tensors if t is not None] if type(None) in set(map(type, tensors)) else tensors
+
+
 def _dense_now(t):
     """The same without a call where there is nothing to do (None: None)."""
     return t if t is None or (t.is_contiguous() and not t.is_neg()) else _dense(t.detach())
@@ -1078,7 +1083,7 @@ class Engine:
         seed = operator.index(seed)
         if not 0 <= seed < 2 ** 32:
             raise ValueError("adamW: seed must have 32 bits")
-        used = grads if all(g is not None for g in grads) else [g for g in grads if g is not None]
+        used = _present(grads)
         if not used:
             return None if max_norm is None else norm if norm is not None else self.grad_norm([])
         eight = state.bits == 8
@@ -1089,7 +1094,7 @@ class Engine:
         with self._on(used[0]), torch.no_grad():
             if not dense:
                 grads = [None if g is None else _dense(g) for g in grads]
-                used = [g for g in grads if g is not None]
+                used = _present(grads)
             norm_at = None
             if max_norm is not None:
                 if norm is None:
@@ -1105,6 +1110,8 @@ class Engine:
                 g_at, g_code, count = ([0 if g is None else f(x) for g, x in zip(grads, xs)] for f, xs in ((at, grads), (lambda g: code(g.dtype), grads), (torch.Tensor.numel, params)))
             if outs is None:
                 o_at, o_code = none, none
+            elif _present(outs) is outs:
+                o_at, o_code = map(at, outs), map(code, map(_dtype_of, outs))
             else:
                 o_at, o_code = [0 if o is None else o.data_ptr() for o in outs], [0 if o is None else code(o.dtype) for o in outs]
             scales = (map(at, lists[2]), map(at, lists[3])) if eight else (none, none)
@@ -1118,17 +1125,16 @@ class Engine:
     def _check_adamw(what, params, grads, outs, lists):
         """The GPU of a step's tensors and whether all gradients are dense; raises for tensors the library would not take.  (A pass over all tensors for each question.)"""
         T = torch.Tensor
-        kept = [o for o in outs if o is not None] if outs is not None else []
-        used = grads if all(g is not None for g in grads) else [g for g in grads if g is not None]
+        kept, used = [] if outs is None else _present(outs), _present(grads)
         device = params[0].get_device()
         written = params + kept
         good = (device >= 0 and set(map(T.get_device, itertools.chain(written, used, *lists))) == {device} and set(map(_dtype_of, written + used)) <= _FC_TYPES.keys()
                 and all(map(T.is_contiguous, written)) and not any(map(T.is_neg, written)) and list(map(T.numel, lists[0])) == list(map(T.numel, params)))
         shapes = list(map(_shape_of, params))
         if good:
-            good = list(map(_shape_of, grads)) == shapes if len(used) == len(grads) else all(g is None or g.shape == s for g, s in zip(grads, shapes))
+            good = list(map(_shape_of, grads)) == shapes if used is grads else all(g is None or g.shape == s for g, s in zip(grads, shapes))
         if good and outs is not None:
-            good = all(o is None or o.shape == s for o, s in zip(outs, shapes))
+            good = list(map(_shape_of, outs)) == shapes if kept is outs else all(o is None or o.shape == s for o, s in zip(outs, shapes))
         if not good:
             for i, (p, g) in enumerate(zip(params, grads)):
                 o = None if outs is None else outs[i]
