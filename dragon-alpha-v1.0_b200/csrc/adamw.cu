@@ -3,8 +3,10 @@
 //   g' = c g,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 //
-// One pass over every array, one launch for every 128 tensors: bound by HBM.  A CTA takes every gridDim.x-th chunk of 4096 elements of the launch; a thread has 4
-// elements of each of four rows of 1024, so that all its loads are in flight together and every load of a warp is consecutive.
+// One pass over every array, one launch for every 128 tensors: bound by HBM, with moments of 8 bits by the instructions as well.  A CTA takes every gridDim.x-th chunk of 2048
+// elements of the launch; a thread has 4 elements of each of two rows of 1024, so that all its loads are in flight together and every load of a warp is consecutive.
+// 50 million elements, all fp32: 224 us, 6.2 TB/s.  90 million, fp32 weights with bf16 copies and gradients, 8-bit moments: 281 us, 5.2 TB/s (71 instructions an element, of which a third are the
+// hash and the roundings of the codes).  Chunks of 4096 on three CTAs an SM took 231 and 289 us, of 1024 on six 234 and 316.
 //
 // Moments of 8 bits: an e4m3 code for each element and a power of two for each block of 32, the smallest with which none is above 448, so that scaling is exact
 // in both directions.  A code is rounded up or down at random, with the probability that keeps its mean: v moves by one part in 1 / (1 - b2) a step, codes lie 6 to
@@ -29,7 +31,7 @@
 namespace alpha {
 namespace {
 
-constexpr int kAdamTensors = 128, kAdamThreads = 256, kAdamRows = 4;
+constexpr int kAdamTensors = 128, kAdamThreads = 256, kAdamRows = 2, kAdamCtas = 4;       // (CTAs of an SM)
 constexpr int kAdamRow = 4 * kAdamThreads, kAdamChunk = kAdamRow * kAdamRows, kAdamBlock = 32;
 constexpr uint32_t kAdamSeed = 0x243F6A88u;
 enum : unsigned char { kNoType = 255 };
@@ -121,14 +123,14 @@ struct AdamUse { float b1, b1c, b2, b2c, eps, size, root, c; };
 
 __device__ __forceinline__ float sqrt_approx(float x) { float y; asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// Two elements: p, m and v are replaced.
+// Two elements: p is replaced, and m and v, which come times b1 and b2.
 __device__ __forceinline__ void adam_pair(const AdamUse& u, float keep, float2& p, float2 g, float2& m, float2& v)
 {
     g = mul2(g, twice(u.c));
     // (sums one by one: the assembler fuses a packed product with a packed sum, whatever their rounding)
-    const float2 m0 = mul2(m, twice(u.b1)), m1 = mul2(g, twice(u.b1c)), v0 = mul2(v, twice(u.b2)), v1 = mul2(mul2(g, g), twice(u.b2c));
-    m = make_float2(__fadd_rn(m0.x, m1.x), __fadd_rn(m0.y, m1.y));
-    v = make_float2(__fadd_rn(v0.x, v1.x), __fadd_rn(v0.y, v1.y));
+    const float2 m1 = mul2(g, twice(u.b1c)), v1 = mul2(mul2(g, g), twice(u.b2c));
+    m = make_float2(__fadd_rn(m.x, m1.x), __fadd_rn(m.y, m1.y));
+    v = make_float2(__fadd_rn(v.x, v1.x), __fadd_rn(v.y, v1.y));
     const float2 by = fma2(make_float2(sqrt_approx(v.x), sqrt_approx(v.y)), twice(u.root), twice(u.eps));
     p = fma2(mul2(m, make_float2(rcp_approx(by.x), rcp_approx(by.y))), twice(-u.size), mul2(p, twice(keep)));
 }
@@ -150,88 +152,111 @@ __device__ __forceinline__ void put_one(void* p, long long i, int type, float x)
     else static_cast<__half*>(p)[i] = __float2half_rn(x);
 }
 
-// The rows of an array that a thread has of a chunk.
-template <class Raw> __device__ __forceinline__ void get_rows(Raw (&r)[kAdamRows], const void* p, long long first)
+// The rows of an array that a thread has of a chunk; TAIL: of the last one of a tensor, whose words past `count` elements are zeros and whose last word may be a part of one.
+template <class T> __device__ __forceinline__ T zero_word() { T z; memset(&z, 0, sizeof z); return z; }
+template <class Raw, class T, bool TAIL> __device__ __forceinline__ void get_rows(Raw (&r)[kAdamRows], const void* p, long long first, long long count)
 {
     const Raw* at = reinterpret_cast<const Raw*>(p) + first / 4;
 #pragma unroll
-    for (int i = 0; i < kAdamRows; ++i) r[i] = __ldcs(at + i * kAdamThreads);
+    for (int i = 0; i < kAdamRows; ++i) {
+        if constexpr (TAIL) {
+            const long long left = count - first - i * kAdamRow;
+            if (left < 4) {
+                r[i] = zero_word<Raw>();
+                for (int j = 0; j < left; ++j) reinterpret_cast<T*>(&r[i])[j] = static_cast<const T*>(p)[first + i * kAdamRow + j];
+                continue;
+            }
+        }
+        r[i] = __ldcs(at + i * kAdamThreads);
+    }
 }
-template <class T> __device__ __forceinline__ void get_typed(Four (&f)[kAdamRows], const void* p, long long first)
+template <class T, bool TAIL> __device__ __forceinline__ void get_typed(Four (&f)[kAdamRows], const void* p, long long first, long long count)
 {
     typename FourOf<T>::Raw r[kAdamRows];
-    get_rows(r, p, first);
+    get_rows<typename FourOf<T>::Raw, T, TAIL>(r, p, first, count);
 #pragma unroll
     for (int i = 0; i < kAdamRows; ++i) f[i] = FourOf<T>::get(r[i]);
 }
-__device__ __forceinline__ void put_rows(void* p, long long first, int type, const Four (&f)[kAdamRows])
+template <class Raw, class T, bool TAIL> __device__ __forceinline__ void put_row(void* p, long long at, long long count, const Raw& r)
+{
+    if (TAIL && count - at < 4) {
+        for (int j = 0; j < count - at; ++j) static_cast<T*>(p)[at + j] = reinterpret_cast<const T*>(&r)[j];
+        return;
+    }
+    __stcs(reinterpret_cast<Raw*>(p) + at / 4, r);
+}
+template <bool TAIL> __device__ __forceinline__ void put_rows(void* p, long long first, long long count, int type, const Four (&f)[kAdamRows])
 {
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        typename FourOf<T>::Raw* at = reinterpret_cast<typename FourOf<T>::Raw*>(p) + first / 4;
 #pragma unroll
-        for (int i = 0; i < kAdamRows; ++i) __stcs(at + i * kAdamThreads, FourOf<T>::put(f[i]));
+        for (int i = 0; i < kAdamRows; ++i) put_row<typename FourOf<T>::Raw, T, TAIL>(p, first + i * kAdamRow, count, FourOf<T>::put(f[i]));
     });
 }
 
-// (a warp's 32 lanes, or the eight that hold a block)
-template <int LANES> __device__ __forceinline__ float most_of(float x)
+__device__ __forceinline__ float most_of_warp(float x)
 {
 #pragma unroll
-    for (int d = LANES / 2; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
     return x;
 }
 
-template <bool EIGHT>
-__device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamUse& u, float keep, uint32_t key, long long begin)
+template <bool EIGHT, bool TAIL>
+__device__ __forceinline__ void word_chunk(const AdamTensor& t, const AdamUse& u, float keep, uint32_t key, long long begin)
 {
     const long long first = begin + 4 * threadIdx.x;
     Four p[kAdamRows], g[kAdamRows], m[kAdamRows], v[kAdamRows];
     if constexpr (EIGHT) {
         uint32_t mc[kAdamRows], vc[kAdamRows];
         uint8_t ms[kAdamRows], vs[kAdamRows];
-        get_rows(mc, t.m, first);
-        get_rows(vc, t.v, first);
+        get_rows<uint32_t, uint8_t, TAIL>(mc, t.m, first, t.count);
+        get_rows<uint32_t, uint8_t, TAIL>(vc, t.v, first, t.count);
 #pragma unroll
         for (int i = 0; i < kAdamRows; ++i) {
+            if (TAIL && first + i * kAdamRow >= t.count) { ms[i] = vs[i] = 127; continue; }
             ms[i] = t.m_scale[(first + i * kAdamRow) / kAdamBlock];
             vs[i] = t.v_scale[(first + i * kAdamRow) / kAdamBlock];
         }
-        with_type(t.type, [&](auto x) { get_typed<decltype(x)>(p, t.p, first); });
-        with_type(t.grad_type, [&](auto x) { get_typed<decltype(x)>(g, t.g, first); });
+        with_type(t.type, [&](auto x) { get_typed<decltype(x), TAIL>(p, t.p, first, t.count); });
+        with_type(t.grad_type, [&](auto x) { get_typed<decltype(x), TAIL>(g, t.g, first, t.count); });
 #pragma unroll
         for (int i = 0; i < kAdamRows; ++i) {
             m[i] = e4m3_get(mc[i]);
             v[i] = e4m3_get(vc[i]);
-            const float a = scale_of(ms[i]), b = scale_of(vs[i]);
+            const float a = scale_of(ms[i]) * u.b1, b = scale_of(vs[i]) * u.b2;       // (a power of two: code * (scale * b1) is rounded as (code * scale) * b1 is)
 #pragma unroll
             for (int j = 0; j < 2; ++j) { m[i].f[j] = mul2(m[i].f[j], twice(a)); v[i].f[j] = mul2(v[i].f[j], twice(b)); }
         }
     } else {
-        get_typed<float>(m, t.m, first);
-        get_typed<float>(v, t.v, first);
-        with_type(t.type, [&](auto x) { get_typed<decltype(x)>(p, t.p, first); });
-        with_type(t.grad_type, [&](auto x) { get_typed<decltype(x)>(g, t.g, first); });
+        get_typed<float, TAIL>(m, t.m, first, t.count);
+        get_typed<float, TAIL>(v, t.v, first, t.count);
+        with_type(t.type, [&](auto x) { get_typed<decltype(x), TAIL>(p, t.p, first, t.count); });
+        with_type(t.grad_type, [&](auto x) { get_typed<decltype(x), TAIL>(g, t.g, first, t.count); });
     }
 #pragma unroll
     for (int i = 0; i < kAdamRows; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) adam_pair(u, keep, p[i].f[j], g[i].f[j], m[i].f[j], v[i].f[j]);
-    put_rows(t.p, first, t.type, p);
-    if (t.out_type != kNoType) put_rows(t.out, first, t.out_type, p);
+        for (int j = 0; j < 2; ++j) {
+            if (!EIGHT) { m[i].f[j] = mul2(m[i].f[j], twice(u.b1)); v[i].f[j] = mul2(v[i].f[j], twice(u.b2)); }
+            adam_pair(u, keep, p[i].f[j], g[i].f[j], m[i].f[j], v[i].f[j]);
+        }
+    put_rows<TAIL>(t.p, first, t.count, t.type, p);
+    if (t.out_type != kNoType) put_rows<TAIL>(t.out, first, t.count, t.out_type, p);
     if constexpr (!EIGHT) {
-        put_rows(t.m, first, ALPHA_F32, m);
-        put_rows(t.v, first, ALPHA_F32, v);
+        put_rows<TAIL>(t.m, first, t.count, ALPHA_F32, m);
+        put_rows<TAIL>(t.v, first, t.count, ALPHA_F32, v);
         return;
     }
-    uint32_t* mc = reinterpret_cast<uint32_t*>(t.m) + first / 4;
-    uint32_t* vc = reinterpret_cast<uint32_t*>(t.v) + first / 4;
     uint8_t *ms = t.m_scale + first / kAdamBlock, *vs = t.v_scale + first / kAdamBlock;
 #pragma unroll
     for (int i = 0; i < kAdamRows; ++i) {
         const float mm = fmaxf(fmaxf(fabsf(m[i].f[0].x), fabsf(m[i].f[0].y)), fmaxf(fabsf(m[i].f[1].x), fabsf(m[i].f[1].y)));
         const float vm = fmaxf(fmaxf(v[i].f[0].x, v[i].f[0].y), fmaxf(v[i].f[1].x, v[i].f[1].y));
-        const uint32_t a = scale_for(most_of<8>(mm)), b = scale_for(most_of<8>(vm)), at = static_cast<uint32_t>(first) + i * kAdamRow;
+        // (the byte of the largest is the largest byte: both moments' go through the eight lanes of a block together)
+        uint32_t bytes = scale_for(mm) | scale_for(vm) << 16;
+#pragma unroll
+        for (int d = 4; d; d >>= 1) bytes = __vmaxu2(bytes, __shfl_xor_sync(0xffffffffu, bytes, d));
+        const uint32_t a = bytes & 0xffffu, b = bytes >> 16, at = static_cast<uint32_t>(first) + i * kAdamRow;
         const float2 ai = twice(__uint_as_float((254u - a) << 23)), bi = twice(__uint_as_float((254u - b) << 23));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -240,16 +265,16 @@ __device__ __forceinline__ void whole_chunk(const AdamTensor& t, const AdamUse& 
             m[i].f[j] = make_float2(round_e4m3<false>(x.x, (r0 << 4) & 0xffff0u), round_e4m3<false>(x.y, (r1 << 4) & 0xffff0u));
             v[i].f[j] = make_float2(round_e4m3<true>(y.x, (r0 >> 12) & 0xffff0u), round_e4m3<true>(y.y, (r1 >> 12) & 0xffff0u));
         }
-        __stcs(mc + i * kAdamThreads, e4m3_put(m[i]));
-        __stcs(vc + i * kAdamThreads, e4m3_put(v[i]));
-        if ((threadIdx.x & 7) == 0) {
+        put_row<uint32_t, uint8_t, TAIL>(t.m, first + i * kAdamRow, t.count, e4m3_put(m[i]));
+        put_row<uint32_t, uint8_t, TAIL>(t.v, first + i * kAdamRow, t.count, e4m3_put(v[i]));
+        if ((threadIdx.x & 7) == 0 && (!TAIL || first + i * kAdamRow < t.count)) {
             ms[i * (kAdamRow / kAdamBlock)] = static_cast<uint8_t>(a);
             vs[i * (kAdamRow / kAdamBlock)] = static_cast<uint8_t>(b);
         }
     }
 }
 
-// Element by element, a block of 32 to a warp: the end of a tensor, and arrays that do not start on 16-byte boundaries.
+// Element by element, a block of 32 to a warp: arrays that do not start on 16-byte boundaries.
 template <bool EIGHT>
 __device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u, float keep, uint32_t key, long long begin)
 {
@@ -266,6 +291,8 @@ __device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u,
                 m.x = static_cast<const float*>(t.m)[e];
                 v.x = static_cast<const float*>(t.v)[e];
             }
+            m.x *= u.b1;
+            v.x *= u.b2;
             p.x = get_one(t.p, e, t.type);
             adam_pair(u, keep, p, make_float2(get_one(t.g, e, t.grad_type), 0.f), m, v);
             put_one(t.p, e, t.type, p.x);
@@ -278,7 +305,7 @@ __device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u,
             }
             continue;
         }
-        const uint32_t a = scale_for(most_of<32>(fabsf(m.x))), b = scale_for(most_of<32>(v.x));     // (and a barrier of the warp: the old scales have been read)
+        const uint32_t a = scale_for(most_of_warp(fabsf(m.x))), b = scale_for(most_of_warp(v.x));     // (and a barrier of the warp: the old scales have been read)
         const uint32_t random = mix32(static_cast<uint32_t>(e) ^ key);
         m.x = round_e4m3<false>(m.x * __uint_as_float((254u - a) << 23), (random << 4) & 0xffff0u);
         v.x = round_e4m3<true>(v.x * __uint_as_float((254u - b) << 23), (random >> 12) & 0xffff0u);
@@ -295,7 +322,10 @@ __device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u,
 }
 
 template <bool EIGHT>
-__global__ void __launch_bounds__(kAdamThreads, 3) adamw_kernel(const __grid_constant__ AdamTable table, const __grid_constant__ AdamStep s)
+__device__ __noinline__ void tail_chunk(const AdamTensor& t, const AdamUse& u, float keep, uint32_t key, long long begin) { word_chunk<EIGHT, true>(t, u, keep, key, begin); }
+
+template <bool EIGHT>
+__global__ void __launch_bounds__(kAdamThreads, kAdamCtas) adamw_kernel(const __grid_constant__ AdamTable table, const __grid_constant__ AdamStep s)
 {
     __shared__ float shared[2];
     grid_dependency_wait();
@@ -331,7 +361,8 @@ __global__ void __launch_bounds__(kAdamThreads, 3) adamw_kernel(const __grid_con
         const float keep = static_cast<float>(1.0 - lr * t.weight_decay);
         uint32_t key = EIGHT ? mix32(call_key ^ t.number) : 0u;
         if (EIGHT && begin >> 32) key = mix32(key ^ static_cast<uint32_t>(begin >> 32));
-        if (t.words && begin + kAdamChunk <= t.count) whole_chunk<EIGHT>(t, u, keep, key, begin);
+        if (t.words && begin + kAdamChunk <= t.count) word_chunk<EIGHT, false>(t, u, keep, key, begin);
+        else if (t.words) tail_chunk<EIGHT>(t, u, keep, key, begin);
         else ragged_chunk<EIGHT>(t, u, keep, key, begin);
     }
 }
@@ -413,7 +444,7 @@ int run_adamw(int n, const AlphaAdamW* list, const AlphaAdamWStep* s, cudaStream
     t.n = 0;
     long long chunks = 0;
     const bool eight = n && list[0].moment_bits == 8;
-    const long long most = sms * 3LL;
+    const long long most = sms * static_cast<long long>(kAdamCtas);
     for (int i = 0; i <= n; ++i) {
         long long more = 0;
         if (i < n) {
