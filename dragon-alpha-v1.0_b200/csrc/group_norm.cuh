@@ -444,7 +444,7 @@ template <class T, int V, bool TWO> struct NormRows {
     static constexpr int S = 3, U = (sizeof(T) == 2 ? 8 : 4) / (TWO ? 2 : 1);
     static constexpr size_t kBytes = V == 1 ? 0 : static_cast<size_t>(kNormThreads) * sizeof(Raw) * U * S * (TWO ? 2 : 1);
     const T *x, *y;
-    size_t step;                     // elements from a row to the thread's next
+    long long step;                  // elements from a row to the thread's next
     int total;                       // its rows
     Raw* ring;
     __device__ Raw* at(int batch, int i, int second) const { return ring + ((batch % S * U + i) * (TWO ? 2 : 1) + second) * kNormThreads + threadIdx.x; }
@@ -507,7 +507,7 @@ template <class T, int V, bool TWO> struct NormRows {
             } else {
 #pragma unroll
                 for (int i = 0; i < U; ++i) {
-                    const size_t o = (static_cast<size_t>(b) * U + (i < have ? i : 0)) * step;
+                    const long long o = (static_cast<long long>(b) * U + (i < have ? i : 0)) * step;
                     rx[i] = x[o];
                     if (TWO) ry[i] = y[o];
                 }
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_sums_kernel(const __grid
     for (int j = 0; j < P; ++j) s[j] = q[j] = make_float2(0.f, 0.f);
     if (a.busy && a.ty < a.count) {
         const size_t begin = a.from + static_cast<size_t>(a.ty) * p.C;
-        const Rows rows{static_cast<const T*>(p.X) + begin, BACK ? static_cast<const T*>(p.dY) + begin : nullptr, static_cast<size_t>(p.rows) * p.C, (a.count - a.ty + p.rows - 1) / p.rows,
+        const Rows rows{static_cast<const T*>(p.X) + begin, BACK ? static_cast<const T*>(p.dY) + begin : nullptr, static_cast<long long>(p.rows) * p.C, (a.count - a.ty + p.rows - 1) / p.rows,
                         reinterpret_cast<Raw*>(smem)};
         if constexpr (!BACK) {
             float seen = 0.f;                     // s: mean of what has been seen, q: its squared differences
@@ -779,8 +779,11 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(const __gri
             gamma[j] = mul2(gamma[j], make_float2(t.y, u.y));
         }
     }
-    const size_t begin = a.from + static_cast<size_t>(a.ty) * p.C, step = static_cast<size_t>(p.rows) * p.C;
-    const Rows rows{static_cast<const T*>(p.X) + begin, BACK ? static_cast<const T*>(p.dY) + begin : nullptr, step, (a.count - a.ty + p.rows - 1) / p.rows, reinterpret_cast<Raw*>(smem)};
+    // from the last row to the first
+    const int total = (a.count - a.ty + p.rows - 1) / p.rows;
+    const long long step = -static_cast<long long>(p.rows) * p.C;
+    const size_t begin = a.from + (a.ty + static_cast<size_t>(total - 1) * p.rows) * p.C;
+    const Rows rows{static_cast<const T*>(p.X) + begin, BACK ? static_cast<const T*>(p.dY) + begin : nullptr, step, total, reinterpret_cast<Raw*>(smem)};
     T* out = static_cast<T*>(p.out) + begin;
     with_act(p.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
