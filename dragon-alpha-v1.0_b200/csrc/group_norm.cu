@@ -78,17 +78,22 @@ bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* 
     }
     return *least < 1e300;
 }
-// Column blocks of up to 64 words, of whole groups where one fits, and runs of positions that fill the SMs once.
-void plan_streamed(Norm& p, int V, int sms)
+// Column blocks, of whole groups where one fits, that leave the fewest threads idle (8 x 64 x 64 x 640: blocks of 50 words, the last of 10, 61 us; of 40, 55), and runs of positions
+// that fill the SMs once.
+void plan_streamed(Norm& p, int V, int size, int sms)
 {
     const int words = p.C / V;
-    const long long unit = p.D / std::gcd(p.D, V);                   // words of the fewest whole groups
-    p.whole = unit <= 64;
-    p.blocks = (words + 63) / 64;
-    p.words = (words + p.blocks - 1) / p.blocks;
-    if (p.whole) p.words = static_cast<int>(p.words < unit ? unit : p.words / unit * unit);
-    p.blocks = (words + p.words - 1) / p.words;
-    p.rows = kNormThreads / p.words;
+    const long long least_words = p.D / std::gcd(p.D, V);            // words of the fewest whole groups
+    p.whole = least_words <= 128;
+    const int unit = p.whole ? static_cast<int>(least_words) : 1, units = words / unit;
+    double best = 0.0;
+    for (int each = 1; each <= units && each * unit <= kNormThreads; ++each) {
+        const int wide = each * unit, blocks = (units + each - 1) / each, rows = kNormThreads / wide;
+        const double used = static_cast<double>(words) / (static_cast<double>(blocks) * wide) * (rows * wide) / kNormThreads, row = static_cast<double>(wide) * V * size;
+        // (rows of at least 256 bytes of a tensor at a time, where it has them; four rows of threads for the loads of few positions)
+        const double good = used * (row < 256 && blocks > 1 ? 0.7 + row / 853 : 1.0) * (rows < 4 ? 0.97 : 1.0);
+        if (good >= best - 1e-9) { best = std::max(best, good); p.words = wide; p.blocks = blocks; p.rows = rows; }
+    }
     const long long others = static_cast<long long>(p.N) * p.blocks, least = 8LL * p.rows;        // positions of a run
     long long runs = std::max(1LL, 4LL * sms / others);
     runs = std::min(runs, std::max(1LL, p.R / least));
@@ -111,7 +116,7 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
     size_t smem = 0;
     double least = 0.0;
     const bool resident = words && plan_resident(p, sizeof(T), BACK, sms, &smem, &least) && least < streamed;
-    if (!resident) { plan_streamed(p, words ? 4 : 1, sms); p.cluster = 1; }
+    if (!resident) { plan_streamed(p, words ? 4 : 1, sizeof(T), sms); p.cluster = 1; }
     p.by_words = fast_div(p.words); p.by_D = fast_div(p.D);
     if (resident) {
         p.groups = p.words * 4 / p.D;
