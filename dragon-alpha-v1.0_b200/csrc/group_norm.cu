@@ -161,7 +161,7 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
         rc = launched("norm_apply_kernel");
     }
     if (rc || !dgamma) return rc;
-    launch_after(norm_affine_kernel<T>, (p.C + 31) / 32, 256, 0, stream, p.sums, p.N * p.cluster, p.C, dgamma, dbeta, p.affine_f32);
+    launch_after(norm_affine_kernel<T>, (p.C + 31) / 32, kAffineThreads, 0, stream, p.sums, p.N * p.cluster, p.C, dgamma, dbeta, p.affine_f32);
     note_launch("norm");
     return launched("norm_affine_kernel");
 }

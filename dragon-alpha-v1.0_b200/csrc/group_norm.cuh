@@ -808,24 +808,29 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_apply_kernel(const __gri
     });
 }
 
-// deltaGamma and deltaBeta: the samples' sums of a channel, eight rows of 32 threads.
+// deltaGamma and deltaBeta: the sums of a channel over the samples (and the CTAs of their clusters), 32 rows of 32 threads.
+constexpr int kAffineThreads = 1024;
 template <class T>
-__global__ void __launch_bounds__(256) norm_affine_kernel(const float2* __restrict__ sums, int N, int C, void* dgamma, void* dbeta, int f32)
+__global__ void __launch_bounds__(kAffineThreads) norm_affine_kernel(const float2* __restrict__ sums, int rows, int C, void* dgamma, void* dbeta, int f32)
 {
-    __shared__ float2 red[8][33];
+    __shared__ float2 red[32][33];
     grid_dependency_wait();
     grid_dependency_trigger();
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
     float a = 0.f, b = 0.f;
     if (c < C)
-        for (int n = y; n < N; n += 8) { const float2 s = sums[static_cast<size_t>(n) * C + c]; a += s.x; b += s.y; }
+#pragma unroll 4
+        for (int n = y; n < rows; n += 32) { const float2 s = sums[static_cast<size_t>(n) * C + c]; a += s.x; b += s.y; }
     red[y][x] = make_float2(a, b);
     __syncthreads();
-    if (y || c >= C) return;
-#pragma unroll
-    for (int r = 1; r < 8; ++r) { a += red[r][x].x; b += red[r][x].y; }
-    if (f32) { static_cast<float*>(dgamma)[c] = b; static_cast<float*>(dbeta)[c] = a; }
-    else { static_cast<T*>(dgamma)[c] = static_cast<T>(b); static_cast<T*>(dbeta)[c] = static_cast<T>(a); }
+    // a warp to a channel
+    const float2 s = red[x][y];
+    a = warp_sum(s.x);
+    b = warp_sum(s.y);
+    const int mine = blockIdx.x * 32 + y;
+    if (x || mine >= C) return;
+    if (f32) { static_cast<float*>(dgamma)[mine] = b; static_cast<float*>(dbeta)[mine] = a; }
+    else { static_cast<T*>(dgamma)[mine] = static_cast<T>(b); static_cast<T*>(dbeta)[mine] = static_cast<T>(a); }
 }
 
 }  // namespace alpha
