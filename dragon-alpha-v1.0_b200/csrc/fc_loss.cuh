@@ -62,14 +62,15 @@ __global__ void __launch_bounds__(kJoinThreads) loss_join_kernel(const float2* _
     if (loss) loss[row] = label_of(label, label_bytes, row, classes) >= 0 ? l - at_label[row] : 0.f;
 }
 
-// scale[0]: the power of two that brings the largest of |grad| to 2^14 .. 2^15 (1 where it is 0, Inf or NaN), scale[1]: its inverse.
-__global__ void __launch_bounds__(1024) loss_scale_kernel(const float* __restrict__ grad, int n, float* scale)
+// scale[0]: the power of two that brings the largest of |grad|, of the rows that count, to 2^14 .. 2^15 (1 where it is 0, Inf or NaN), scale[1]: its inverse.
+__global__ void __launch_bounds__(1024) loss_scale_kernel(const float* __restrict__ grad, int n, const void* label, int label_bytes, int classes, float* scale)
 {
     __shared__ float shared[32];
     grid_dependency_wait();
     grid_dependency_trigger();
     float m = 0.f;
-    for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, fabsf(grad[i]));
+    for (int i = threadIdx.x; i < n; i += 1024)
+        if (label_of(label, label_bytes, i, classes) >= 0) m = fmaxf(m, fabsf(grad[i]));
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = m;

@@ -153,8 +153,9 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 // (all groups but the last N)
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// (after a __syncwarp: the aligned forms take a whole warp)
+__device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ float warp_sum(float x)
 {
 #pragma unroll
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_resident_kernel(const __
         for (int r = 0; r < cl; ++r) st_cluster_f2(mapa_u32(at, r), x, y);
     };
     auto shared_by_all = [&] {
-        if (cl > 1) cluster_sync_all();
+        if (cl > 1) { cluster_arrive(); cluster_wait(); }
         else __syncthreads();
     };
     // (a cluster's CTAs have all begun before one writes to another)

@@ -512,8 +512,10 @@ int alpha_fullConnect_workspace_bytes(const AlphaFcShape* s, int glu, int op, si
  *   dz = deltaL (exp(z - lse) - [label]),  deltaX = dz W,  deltaW = dz^T X,  deltaB = column sums of dz      (deltaX, deltaW, deltaB: each may be NULL)
  * Sums, exponentials and logarithms are fp32; dz is rounded to the tensors' type once (fp16: times a power of two that brings the largest |deltaL| to 2^14 or
  * above), as the deltaZ of alpha_fullConnect_delta is, and outputs once.  fp32 tensors have fp32 accuracy, and fewer than 2^31 elements (rows x OC among them).
- * No output may overlap anything else.  Results do not depend on scheduling.  Scratch (the function below): parts of the rows' sums, logits or their
- * gradients for a piece of the classes (up to 256 MB), fp32 sums of deltaX where there are several. */
+ * No output may overlap anything else.  Results do not depend on scheduling.  Scratch (the function below): parts of the rows' sums (8 bytes for 64 or
+ * 128 classes of a row, runs of 4096 rows or more that take some 256 MB), logits or their gradients for a piece of the classes (up to 256 MB, or 8 KB a row), and fp32 sums of
+ * deltaX, one for each part of its reduction.  Products of 16-bit tensors read every row of X: a row that does not count adds 0 times its X to deltaW, which is 0 unless it
+ * holds an Inf or a NaN. */
 int alpha_fullConnect_softmax_crossEntropy(const AlphaFcShape* s, const void* X, const void* W, const void* bias, const void* label, int label_bytes, float* loss, float* lse,
                                            alpha_stream_t stream);
 int alpha_fullConnect_softmax_crossEntropy_delta(const AlphaFcShape* s, const float* deltaL, int deltaL_step, const void* X, const void* W, const void* bias, const void* label,

@@ -168,6 +168,20 @@ def test_small_probabilities_in_fp16(eng):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_losses_that_do_not_count(eng, dtype):
+    """Inf, NaN and huge gradients of losses that do not count change nothing: not the scale of fp16 either."""
+    X, W, label, B = make(100, 64, 3000, dtype, True, 0.3, scale=0.3)
+    _, lse = eng.fullConnect_softmax_crossEntropy(X, W, label, B, save=True)
+    dL = torch.full((100,), 1e-4, device="cuda")
+    want = eng.fullConnect_softmax_crossEntropy_delta(dL, X, W, label, lse, B)
+    out = (label < 0).nonzero()[:, 0]
+    assert out.numel() > 4
+    dL[out] = 1e30
+    dL[out[0]], dL[out[1]] = float("inf"), float("nan")
+    assert all(torch.equal(a, b) for a, b in zip(want, eng.fullConnect_softmax_crossEntropy_delta(dL, X, W, label, lse, B)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_masked_classes(eng, dtype):
     """Classes with a bias of -Inf, and of the type's lowest value, have no probability; a row that counts none of its classes has an lse of -Inf."""
     X, W, label, B = make(40, 64, 200, dtype, True, 0.0)
