@@ -890,7 +890,7 @@ class Engine:
 
     # ---- the loss on top of such a layer ----
     def _loss_call(self, what, X, W, label, Bias, others):
-        """The checked call's plan, and label as dense memory."""
+        """The checked call's plan."""
         plan = _fc_plan(what, False, X.shape, W.shape, X.dtype)
         device = _fc_check(what, X, W, (("Bias", Bias, plan[8]),) if Bias is not None else ())
         lead = X.shape[:-1]
@@ -907,14 +907,21 @@ class Engine:
         """The softmax cross entropy of every row of X [..., IC] over the classes of a FullConnect layer, logsumexp(z) - z[label] with z = X W^T + Bias, as float32 [...].
         The logits are not kept.  W [OC, IC]; label [...] int64 or int32; a row whose label is not in [0, OC) does not count: its loss is 0.  save=True also returns
         the logsumexp of every row, which fullConnect_softmax_crossEntropy_delta reads."""
-        IC, OC, ic, oc, rows, *_ = self._loss_call("fullConnect_softmax_crossEntropy", X, W, label, Bias, ())
-        with self._on(X), torch.no_grad():
-            loss = _new(X, X.shape[:-1])
-            lse = _new(X, X.shape[:-1]) if save else None
-            if rows:
-                (Xp, Wp, Bp), _held = _fc_pack(X.dtype, (X, 1, rows, IC, rows, ic), (W, 1, OC, IC, OC, ic), (Bias, 1, 1, OC, 1, oc))
-                label = label.contiguous()
-                self.base.fullConnect_softmax_crossEntropy(loss, lse, Xp, Wp, Bp, label, label.element_size(), rows, ic, OC, _FC_TYPES[X.dtype])
+        plan = self._loss_call("fullConnect_softmax_crossEntropy", X, W, label, Bias, ())
+        if self.base._stream is None and X.get_device() == torch._C._cuda_getDevice():
+            return self._loss_run(plan, X, W, label, Bias, save)
+        with self._on(X):
+            return self._loss_run(plan, X, W, label, Bias, save)
+
+    def _loss_run(self, plan, X, W, label, Bias, save):
+        IC, OC, ic, oc, rows = plan[:5]
+        dtype, lead = X.dtype, X.shape[:-1]
+        loss = _new(X, lead)
+        lse = _new(X, lead) if save else None
+        if rows:
+            (Xp, Wp, Bp), _held = _fc_pack(dtype, (X, 1, rows, IC, rows, ic), (W, 1, OC, IC, OC, ic), (Bias, 1, 1, OC, 1, oc))
+            label = _dense_now(label)
+            self.base.fullConnect_softmax_crossEntropy(loss.data_ptr(), lse, Xp, Wp, Bp, label.data_ptr(), label.element_size(), rows, ic, OC, _FC_TYPES[dtype])
         return (loss, lse) if save else loss
 
     def fullConnect_softmax_crossEntropy_delta(self, deltaL, X, W, label, lse, Bias=None):
@@ -924,19 +931,27 @@ class Engine:
         step = 0
         if isinstance(deltaL, torch.Tensor) and (deltaL.dim() or X.dim() == 1):
             step = 1
-        IC, OC, ic, oc, rows, *_ = self._loss_call(what, X, W, label, Bias, (("lse", lse),) + ((("deltaL", deltaL),) if step else ()))
+        plan = self._loss_call(what, X, W, label, Bias, (("lse", lse),) + ((("deltaL", deltaL),) if step else ()))
         if not step and isinstance(deltaL, torch.Tensor) and (deltaL.dtype != torch.float32 or deltaL.get_device() != X.get_device()):
             raise ValueError("%s: deltaL must be float32 on %s, not %s on %s" % (what, X.device, deltaL.dtype, deltaL.device))
-        with self._on(X), torch.no_grad():
-            if rows == 0:
-                return X.new_empty(X.shape), W.new_zeros(W.shape), None if Bias is None else W.new_zeros((OC,))
-            if not isinstance(deltaL, torch.Tensor):
-                deltaL = torch.full((), float(deltaL), dtype=torch.float32, device=X.device)
-            (Xp, Wp, Bp), _held = _fc_pack(X.dtype, (X, 1, rows, IC, rows, ic), (W, 1, OC, IC, OC, ic), (Bias, 1, 1, OC, 1, oc))
-            label, lse, deltaL = label.contiguous(), _dense(lse), _dense(deltaL)
-            dX, dW = X.new_empty((rows, ic)), W.new_empty((OC, ic))
-            dB = None if Bias is None else W.new_empty((oc,))
-            self.base.fullConnect_softmax_crossEntropy_delta(dX, dW, dB, deltaL, step, Xp, Wp, Bp, label, label.element_size(), lse, rows, ic, OC, _FC_TYPES[X.dtype])
+        if self.base._stream is None and X.get_device() == torch._C._cuda_getDevice():
+            return self._loss_run_delta(plan, deltaL, step, X, W, label, lse, Bias)
+        with self._on(X):
+            return self._loss_run_delta(plan, deltaL, step, X, W, label, lse, Bias)
+
+    def _loss_run_delta(self, plan, deltaL, step, X, W, label, lse, Bias):
+        IC, OC, ic, oc, rows = plan[:5]
+        dtype = X.dtype
+        if rows == 0:
+            return X.new_empty(X.shape), W.new_zeros(W.shape), None if Bias is None else W.new_zeros((OC,))
+        if not isinstance(deltaL, torch.Tensor):
+            deltaL = X.new_full((), float(deltaL), dtype=torch.float32)
+        (Xp, Wp, Bp), _held = _fc_pack(dtype, (X, 1, rows, IC, rows, ic), (W, 1, OC, IC, OC, ic), (Bias, 1, 1, OC, 1, oc))
+        label, lse, deltaL = _dense_now(label), _dense_now(lse), _dense_now(deltaL)
+        dX, dW = X.new_empty((rows, ic)), W.new_empty((OC, ic))
+        dB = None if Bias is None else W.new_empty((oc,))
+        self.base.fullConnect_softmax_crossEntropy_delta(dX.data_ptr(), dW.data_ptr(), dB, deltaL.data_ptr(), step, Xp, Wp, Bp, label.data_ptr(), label.element_size(), lse.data_ptr(),
+                                                         rows, ic, OC, _FC_TYPES[dtype])
         if ic != IC:
             dX, dW = dX.narrow(1, 0, IC), dW.narrow(1, 0, IC)
         return dX if X.dim() == 2 else dX.reshape(X.shape), dW, None if dB is None else dB if oc == OC else dB.narrow(0, 0, OC)
