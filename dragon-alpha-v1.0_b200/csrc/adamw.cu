@@ -68,6 +68,18 @@ __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x)
     return x ^ (x >> 16);
 }
 
+// The random bits of an element's codes, 16 each, times 16 (the place where round_e4m3 wants them): the low half of mix32(element ^ key) for m, the high one for v.  Of four neighbours
+// (element a multiple of 4) `start` is what mix32 forms first, (element ^ key) ^ (element ^ key) >> 16, which differs in the lowest bits only.
+struct Dither { uint32_t m, v; };
+__device__ __forceinline__ uint32_t dither_start(uint32_t element, uint32_t key) { const uint32_t x = element ^ key; return x ^ (x >> 16); }
+__device__ __forceinline__ Dither dither_of(uint32_t start)
+{
+    uint32_t x = start * 0x9E3779B9u;
+    x = (x ^ (x >> 15)) * 0xB7E15163u;
+    const uint32_t high = x >> 12;                 // (x ^ x >> 16 has the high half of x, and the low half xor the high one)
+    return Dither{((x << 4) ^ high) & 0xffff0u, high & 0xffff0u};
+}
+
 // Four elements at a time, as two pairs of floats.
 struct Four { float2 f[2]; };
 template <class T> struct FourOf;
@@ -256,14 +268,14 @@ __device__ __forceinline__ void word_chunk(const AdamTensor& t, const AdamUse& u
         uint32_t bytes = scale_for(mm) | scale_for(vm) << 16;
 #pragma unroll
         for (int d = 4; d; d >>= 1) bytes = __vmaxu2(bytes, __shfl_xor_sync(0xffffffffu, bytes, d));
-        const uint32_t a = bytes & 0xffffu, b = bytes >> 16, at = static_cast<uint32_t>(first) + i * kAdamRow;
+        const uint32_t a = bytes & 0xffffu, b = bytes >> 16, start = dither_start(static_cast<uint32_t>(first) + i * kAdamRow, key);
         const float2 ai = twice(__uint_as_float((254u - a) << 23)), bi = twice(__uint_as_float((254u - b) << 23));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t r0 = mix32((at + 2 * j) ^ key), r1 = mix32((at + 2 * j + 1) ^ key);
+            const Dither r0 = dither_of(start ^ (2 * j)), r1 = dither_of(start ^ (2 * j + 1));
             const float2 x = mul2(m[i].f[j], ai), y = mul2(v[i].f[j], bi);
-            m[i].f[j] = make_float2(round_e4m3<false>(x.x, (r0 << 4) & 0xffff0u), round_e4m3<false>(x.y, (r1 << 4) & 0xffff0u));
-            v[i].f[j] = make_float2(round_e4m3<true>(y.x, (r0 >> 12) & 0xffff0u), round_e4m3<true>(y.y, (r1 >> 12) & 0xffff0u));
+            m[i].f[j] = make_float2(round_e4m3<false>(x.x, r0.m), round_e4m3<false>(x.y, r1.m));
+            v[i].f[j] = make_float2(round_e4m3<true>(y.x, r0.v), round_e4m3<true>(y.y, r1.v));
         }
         put_row<uint32_t, uint8_t, TAIL>(t.m, first + i * kAdamRow, t.count, e4m3_put(m[i]));
         put_row<uint32_t, uint8_t, TAIL>(t.v, first + i * kAdamRow, t.count, e4m3_put(v[i]));
@@ -306,9 +318,9 @@ __device__ __noinline__ void ragged_chunk(const AdamTensor& t, const AdamUse& u,
             continue;
         }
         const uint32_t a = scale_for(most_of_warp(fabsf(m.x))), b = scale_for(most_of_warp(v.x));     // (and a barrier of the warp: the old scales have been read)
-        const uint32_t random = mix32(static_cast<uint32_t>(e) ^ key);
-        m.x = round_e4m3<false>(m.x * __uint_as_float((254u - a) << 23), (random << 4) & 0xffff0u);
-        v.x = round_e4m3<true>(v.x * __uint_as_float((254u - b) << 23), (random >> 12) & 0xffff0u);
+        const Dither random = dither_of(dither_start(static_cast<uint32_t>(e), key));
+        m.x = round_e4m3<false>(m.x * __uint_as_float((254u - a) << 23), random.m);
+        v.x = round_e4m3<true>(v.x * __uint_as_float((254u - b) << 23), random.v);
         if (in) {
             const uint32_t codes = e4m3_put(Four{{make_float2(m.x, v.x), make_float2(0.f, 0.f)}});
             static_cast<uint8_t*>(t.m)[e] = static_cast<uint8_t>(codes);
