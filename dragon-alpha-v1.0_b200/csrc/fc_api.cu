@@ -75,7 +75,8 @@ PairPlan pick_pair(int rows, int m_halves, int out_cols, bool glu, int K, int k_
 double split_time(size_t elements) { return 2.0 + elements * 10e-6 / 8.0; }
 
 template <int FORM>
-int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, const uint32_t* seen, int seen_n, int sms, int* status, cudaStream_t stream)
+int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, const uint32_t* seen, int seen_n, int sms, int* status, cudaStream_t stream,
+                bool join = true)
 {
     constexpr bool GLU = FORM == kFcGlu, A_MN = FORM == kFcDeltaW, B_MN = FORM == kFcDeltaX || FORM == kFcDeltaW;
     const bool forward = FORM == kFcForward || FORM == kFcGlu;
@@ -137,7 +138,7 @@ int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const Pai
     note_launch("fc");
     note_plan("fc planes pair 256x%d parts=%d", bn, parts);
     rc = launched("fc_pair_f32_kernel");
-    return rc || parts == 1 ? rc : launch_parts<GLU>(static_cast<const float*>(ws), size, parts, p.rows * m_halves, q.e, sms, stream);
+    return rc || parts == 1 || !join ? rc : launch_parts<GLU>(static_cast<const float*>(ws), size, parts, p.rows * m_halves, q.e, sms, stream);
 }
 
 // The same from the fp32 tensors as they lie; without `may_split` in no scratch.
@@ -432,11 +433,12 @@ int delta(const char* what, const AlphaFcShape* s, const void* dY, const void* X
 
 namespace alpha {
 
+typedef int (*LogitsReady)(void* what, const float* part, int parts);
 int fc_logits_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Y, cudaStream_t stream)
 {
     return forward(s, X, W, bias, nullptr, nullptr, Y, false, stream);
 }
-int fc_logits_and_gradients_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Z, float* dX, float* dW, int (*between)(void*), void* what, cudaStream_t stream)
+int fc_logits_and_gradients_f32(const AlphaFcShape* s, const float* X, const float* W, const float* bias, float* Z, float* dX, float* dW, LogitsReady between, void* what, cudaStream_t stream)
 {
     const int rows = s->rows, IC = s->IC, OC = s->OC, pitch = fc_pitch(OC);
     const FcEpilogue of_z{bias, nullptr, nullptr, Z, pitch, ALPHA_ACT_NONE, 0.f}, of_x{nullptr, nullptr, nullptr, dX, IC, ALPHA_ACT_NONE, 0.f}, of_w{nullptr, nullptr, nullptr, dW, IC, ALPHA_ACT_NONE, 0.f};
@@ -454,8 +456,8 @@ int fc_logits_and_gradients_f32(const AlphaFcShape* s, const float* X, const flo
     rc = v.split(stream, 2);                       // X and W
     if (rc) return rc;
     if (dry_run()) return ALPHA_OK;
-    rc = launch_pair<kFcForward>(z, v.p[a], v.p[b], pz, v.part, v.seen, v.seen_n, v.sms, v.status, stream);
-    if (!rc) rc = between(what);
+    rc = launch_pair<kFcForward>(z, v.p[a], v.p[b], pz, v.part, v.seen, v.seen_n, v.sms, v.status, stream, false);
+    if (!rc) rc = between(what, pz.parts > 1 ? static_cast<const float*>(v.part) : nullptr, pz.parts);
     const int seen = v.seen_n;
     if (!rc) {
         const Planes* one[1] = {&v.p[c]};

@@ -127,6 +127,26 @@ __global__ void __launch_bounds__(256) loss_bias_kernel(const float* __restrict_
     out[c] = static_cast<T>(s * ((by ? *by : 1.f) * factor));
 }
 
+// The same of few rows at once: a warp's 32 columns, 32 warps.
+template <class T>
+__global__ void __launch_bounds__(1024) loss_few_columns_kernel(const T* __restrict__ a, int rows, int pitch, const float* by, float factor, T* out)
+{
+    __shared__ float red[32][33];
+    grid_dependency_wait();
+    grid_dependency_trigger();
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
+    float s = 0.f;
+    if (c < pitch)
+#pragma unroll 8
+        for (int r = y; r < rows; r += 32) s += static_cast<float>(a[static_cast<size_t>(r) * pitch + c]);
+    red[y][x] = s;
+    __syncthreads();
+    if (y || c >= pitch) return;
+#pragma unroll
+    for (int r = 1; r < 32; ++r) s += red[r][x];
+    out[c] = static_cast<T>(s * ((by ? *by : 1.f) * factor));
+}
+
 // ---- fp32: logits of a piece of the classes lie in memory ---------------------------------------------------------
 
 constexpr int kRowThreads = 256;
@@ -175,8 +195,8 @@ __global__ void __launch_bounds__(kRowThreads) loss_rows_kernel(const float* __r
     const int l = label_of(label, label_bytes, row, classes) - base;
     if (l >= 0 && l < cols) at_label[row] = at[l];
 }
-// Logits become their gradients, in place; the padding of a row 0.
-__global__ void __launch_bounds__(kRowThreads) loss_delta_kernel(float* z, int pitch, int cols, int base, int classes, const void* label, int label_bytes, const float* __restrict__ lse,
+// Logits become their gradients, in place; the padding of a row 0.  Logits that were formed in parts are added first, with the bias.
+__global__ void __launch_bounds__(kRowThreads) loss_delta_kernel(float* z, const float* __restrict__ part, int parts, const float* __restrict__ bias, int rows, int pitch, int cols, int base, int classes, const void* label, int label_bytes, const float* __restrict__ lse,
                                                                  const float* __restrict__ grad, int grad_step)
 {
     grid_dependency_wait();
@@ -185,7 +205,11 @@ __global__ void __launch_bounds__(kRowThreads) loss_delta_kernel(float* z, int p
     const float log_sum = lse[row], g = grad[static_cast<size_t>(row) * grad_step];
     float* at = z + static_cast<size_t>(row) * pitch;
     for (int c = threadIdx.x; c < pitch; c += kRowThreads) {
-        const float p = expf(at[c] - log_sum);
+        float logit = part ? 0.f : at[c];
+        if (part)
+            for (int i = 0; i < parts; ++i) logit += part[(static_cast<size_t>(i) * rows + row) * pitch + c];
+        if (bias) logit += bias[c];
+        const float p = expf(logit - log_sum);
         at[c] = l >= 0 && c < cols ? g * (c == l - base ? p - 1.f : p) : 0.f;
     }
 }
