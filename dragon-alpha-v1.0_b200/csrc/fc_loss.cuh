@@ -22,7 +22,7 @@ __device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s
 
 // lse and loss of rows from the parts of the tiles' columns, [slots][rows].  A CTA has `across` rows (a power of two up to 32, neighbouring lanes) and shares their
 // slots among its other threads.
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 1024;
 __global__ void __launch_bounds__(kJoinThreads) loss_join_kernel(const float2* __restrict__ part, int slots, int rows, int across, const void* label, int label_bytes, int classes,
                                                                   const float* __restrict__ at_label, float* loss, float* lse)
 {
@@ -38,8 +38,15 @@ __global__ void __launch_bounds__(kJoinThreads) loss_join_kernel(const float2* _
             float2 v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = at[static_cast<size_t>(i + j * ways) * rows];
+            // (about one maximum, so that no exponential waits for another)
+            float most = m;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) join_stats(m, s, v[j].x, v[j].y);
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, v[j].x);
+            const float about = most > -__int_as_float(0x7f800000) ? most : 0.f;
+            s *= expf(m - about);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf(v[j].y, expf(v[j].x - about), s);
+            m = most;
         }
         for (; i < slots; i += ways) {
             const float2 v = at[static_cast<size_t>(i) * rows];
@@ -97,6 +104,7 @@ __global__ void __launch_bounds__(256) loss_columns_kernel(const T* __restrict__
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] = 0.f;
     if (word < words)
+#pragma unroll 4
         for (long long r = blockIdx.y * 8 + y; r < rows; r += gridDim.y * 8) {
             float f[N];
             Word16<T>::load(__ldg(reinterpret_cast<const uint4*>(a + r * pitch) + word), f);

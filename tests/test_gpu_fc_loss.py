@@ -365,3 +365,47 @@ def test_a_training_step(eng):
         # the first step is lr g / (|g| + eps): its sign, one rate long
         big = t.abs() > 1e-5
         assert torch.allclose((p0 - p1)[big], 1e-2 * torch.sign(t)[big], rtol=2e-3, atol=1e-6)
+
+
+def test_two_streams_at_once_and_fewer_sms(eng, lib, pkg):
+    """A whole step of these operators on each of two streams, enqueued in turn, and on 100 of the SMs: the same results as one after the other on all."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    X, W, label, B = make(300, 256, 2000, "bf16")
+    N = (torch.randn(4, 40, 40, 64, device="cuda", generator=g)).bfloat16()
+    big = torch.randn(1, 200, 200, 96, device="cuda", generator=g).bfloat16()
+    p = torch.randn(100000, device="cuda", generator=g)
+
+    def step(e):
+        out = []
+        for t, groups in ((N, 8), (big, 6)):
+            y, mean, rstd = e.groupNorm(t, groups, act="silu", save=True)
+            out += [y, mean, rstd, e.groupNorm_delta(y, t, mean, rstd, act="silu")[0]]
+        loss, lse = e.fullConnect_softmax_crossEntropy(X, W, label, B, save=True)
+        out += [loss, lse, *e.fullConnect_softmax_crossEntropy_delta(0.01, X, W, label, lse, B)]
+        q, state = p.clone(), e.adamW_state([p], 8)
+        e.adamW([q], [p], state, 1, 1e-2, max_norm=1.0)
+        return out + [q, state.m[0].view(torch.uint8), state.v[0].view(torch.uint8)]
+
+    want = step(eng)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = step(eng)
+    torch.cuda.synchronize()
+    for each in got:
+        assert all(torch.equal(a, b) for a, b in zip(want, each))
+    old = lib.set_option("SM_BUDGET", 100)
+    try:
+        few = step(eng)
+    finally:
+        lib.set_option("SM_BUDGET", old)
+    # (other plans: other orders of summation; outputs of 16 bits a rounding apart at most where these meet a border)
+    for a, b in zip(want, few):
+        if a.dtype == torch.uint8:
+            assert float((a != b).float().mean()) < 1e-3
+        else:
+            assert float((a.double() - b.double()).norm()) <= 2e-3 * float(a.double().norm())
+    assert lib.device_status() == 0
