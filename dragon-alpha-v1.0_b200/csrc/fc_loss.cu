@@ -203,8 +203,8 @@ int forward_f32(const Loss& c, float* loss, float* lse)
     const long long rows = c.s->rows, IC = c.s->IC, OC = c.s->OC, piece = piece_classes(rows, OC, 4, 8), pieces = (OC + piece - 1) / piece;
     void *z = nullptr, *part = nullptr, *at_label = nullptr;
     int rc = call_scratch(c.stream, static_cast<size_t>(rows) * fc_pitch(static_cast<int>(piece)) * 4, &z);
-    if (!rc) rc = call_scratch(c.stream, static_cast<size_t>(pieces) * rows * sizeof(float2), &part);
-    if (!rc) rc = call_scratch(c.stream, rows * sizeof(float), &at_label);
+    if (!rc && pieces > 1) rc = call_scratch(c.stream, static_cast<size_t>(pieces) * rows * sizeof(float2), &part);
+    if (!rc && pieces > 1) rc = call_scratch(c.stream, rows * sizeof(float), &at_label);
     const ScratchMark mark = call_mark(c.stream);
     for (long long first = 0; first < OC && !rc; first += piece) {
         call_rewind(c.stream, mark);
@@ -213,11 +213,11 @@ int forward_f32(const Loss& c, float* loss, float* lse)
         rc = fc_logits_f32(&s, static_cast<const float*>(c.X), static_cast<const float*>(c.W) + first * IC, c.bias ? static_cast<const float*>(c.bias) + first : nullptr, static_cast<float*>(z), c.stream);
         if (rc || dry_run()) continue;
         launch_after(loss_rows_kernel, static_cast<unsigned>(rows), kRowThreads, 0, c.stream, static_cast<const float*>(z), fc_pitch(s.OC), s.OC, static_cast<int>(first), c.s->OC, c.s->rows, c.label,
-                     c.label_bytes, static_cast<float2*>(part) + first / piece * rows, static_cast<float*>(at_label));
+                     c.label_bytes, part ? static_cast<float2*>(part) + first / piece * rows : nullptr, static_cast<float*>(at_label), loss, lse);
         note_launch("fc_loss");
         rc = launched("loss_rows_kernel");
     }
-    if (rc || dry_run()) return rc;
+    if (rc || dry_run() || pieces == 1) return rc;
     return join(c, static_cast<const float2*>(part), static_cast<int>(pieces), 0, c.s->rows, static_cast<const float*>(at_label), loss, lse);
 }
 

@@ -182,9 +182,10 @@ __device__ __forceinline__ float cta_total(float x, float* shared)
     for (int w = 0; w < kRowThreads / 32; ++w) x += shared[w];
     return x;
 }
-// A CTA to a row: the largest logit of the piece, then the sum about it; slot `piece` of the row's parts, and the label's logit if it lies in the piece.
+// A CTA to a row: the largest logit of the piece, then the sum about it; slot `piece` of the row's parts, and the label's logit if it lies in the piece.  Of a piece that is all the
+// classes (part NULL) lse and loss.
 __global__ void __launch_bounds__(kRowThreads) loss_rows_kernel(const float* __restrict__ z, int pitch, int cols, int base, int classes, int rows, const void* label, int label_bytes,
-                                                                float2* part, float* at_label)
+                                                                float2* part, float* at_label, float* loss, float* lse)
 {
     __shared__ float shared[kRowThreads / 32];
     grid_dependency_wait();
@@ -199,8 +200,14 @@ __global__ void __launch_bounds__(kRowThreads) loss_rows_kernel(const float* __r
     for (int c = threadIdx.x; c < cols; c += kRowThreads) s += expf(at[c] - about);
     s = cta_total(s, shared);
     if (threadIdx.x) return;
-    part[row] = make_float2(m, s);
     const int l = label_of(label, label_bytes, row, classes) - base;
+    if (!part) {
+        const float log_sum = m + logf(s);
+        if (lse) lse[row] = log_sum;
+        if (loss) loss[row] = l >= 0 ? log_sum - at[l] : 0.f;
+        return;
+    }
+    part[row] = make_float2(m, s);
     if (l >= 0 && l < cols) at_label[row] = at[l];
 }
 // Logits become their gradients, in place; the padding of a row 0.  Logits that were formed in parts are added first, with the bias.
