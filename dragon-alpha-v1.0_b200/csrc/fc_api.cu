@@ -74,15 +74,17 @@ PairPlan pick_pair(int rows, int m_halves, int out_cols, bool glu, int K, int k_
 }
 double split_time(size_t elements) { return 2.0 + elements * 10e-6 / 8.0; }
 
+// A product as the kernel of pairs takes it.
+struct PairItems { CUtensorMap a, b, y, z; PairF32 p; size_t size; const float* ws; };
 template <int FORM>
-int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, const uint32_t* seen, int seen_n, int sms, int* status, cudaStream_t stream,
-                bool join = true)
+int prepare_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, const uint32_t* seen, int seen_n, int* status, PairItems* out_items)
 {
     constexpr bool GLU = FORM == kFcGlu, A_MN = FORM == kFcDeltaW, B_MN = FORM == kFcDeltaX || FORM == kFcDeltaW;
     const bool forward = FORM == kFcForward || FORM == kFcGlu;
     const int bn = plan.bn, parts = plan.parts, out = GLU ? bn / 2 : bn, m_halves = A_MN ? q.halves : 1, k_halves = FORM == kFcDeltaX ? q.halves : 1;
     const int cols = forward ? q.OC : q.cols, steps = FORM == kFcDeltaX ? q.OC : q.K;
-    PairF32 p{};
+    PairF32& p = out_items->p;
+    p = PairF32{};
     p.rows = A_MN ? q.OC : q.rows; p.cols = cols; p.pitch = q.e.cols; p.K = steps;
     p.m_half = (p.rows + 255) / 256; p.m_tiles = p.m_half * m_halves; p.n_tiles = (cols + out - 1) / out;
     const int windows = (steps + 63) / 64;
@@ -110,7 +112,7 @@ int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const Pai
         const cuuint32_t box[4] = {32, 1, 32, 1};
         return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    CUtensorMap a, b, y, z;
+    CUtensorMap &a = out_items->a, &b = out_items->b, &y = out_items->y, &z = out_items->z;
     const long long OC = q.OC, pa = A.pitch, pb = B.pitch;
     int rc;
     if constexpr (FORM == kFcDeltaX) {
@@ -125,20 +127,88 @@ int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const Pai
     }
     if (!rc) rc = A_MN ? out_map(&y, ws, q.halves, true, parts) : out_map(&y, ws, GLU && parts > 1 ? 2 : 1, false, parts);
     if (!rc) rc = p.keep_z ? out_map(&z, q.e.Z, GLU ? 2 : 1, false, 1) : (z = y, ALPHA_OK);
+    out_items->size = size;
+    out_items->ws = static_cast<const float*>(ws);
+    return rc;
+}
+template <int FORM>
+int launch_pair(const ProductF32& q, const Planes& A, const Planes& B, const PairPlan& plan, void* part, const uint32_t* seen, int seen_n, int sms, int* status, cudaStream_t stream,
+                bool join = true)
+{
+    constexpr bool GLU = FORM == kFcGlu;
+    PairItems x;
+    int rc = prepare_pair<FORM>(q, A, B, plan, part, seen, seen_n, status, &x);
     if (rc) return rc;
-    const long long items = static_cast<long long>(p.m_tiles) * p.n_tiles * parts;
+    const int bn = plan.bn, parts = plan.parts;
+    const long long items = static_cast<long long>(x.p.m_tiles) * x.p.n_tiles * parts;
     const unsigned pairs = static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
     auto go = [&](auto width) {
         constexpr int BN = decltype(width)::value;
         allow_smem<fc_pair_f32_kernel<GLU, BN>>();
-        launch_after_clusters(fc_pair_f32_kernel<GLU, BN>, dim3(2 * pairs), kPairF32Threads, 2, pair_f32_smem(BN), stream, a, b, y, z, p);
+        launch_after_clusters(fc_pair_f32_kernel<GLU, BN>, dim3(2 * pairs), kPairF32Threads, 2, pair_f32_smem(BN), stream, x.a, x.b, x.y, x.z, x.p);
     };
     if (bn == 256) go(std::integral_constant<int, 256>{});
     else go(std::integral_constant<int, 128>{});
     note_launch("fc");
     note_plan("fc planes pair 256x%d parts=%d", bn, parts);
     rc = launched("fc_pair_f32_kernel");
-    return rc || parts == 1 || !join ? rc : launch_parts<GLU>(static_cast<const float*>(ws), size, parts, p.rows * m_halves, q.e, sms, stream);
+    const int m_halves = FORM == kFcDeltaW ? q.halves : 1;
+    return rc || parts == 1 || !join ? rc : launch_parts<GLU>(x.ws, x.size, parts, x.p.rows * m_halves, q.e, sms, stream);
+}
+
+// deltaX and deltaW by one launch: its columns, the parts of either, and its time (us).  Their items fill the waves together, and one launch's start is saved
+// (softmax cross entropy gradients of 256 x 512 x 1000: 34 us instead of 42 with two; 1024 x 2048 x 1000: 86 instead of 97; 512 x 4096 x 1000: 97 either way).
+struct TwoPairs { int bn, x_parts, w_parts; double time; size_t part_bytes; };
+TwoPairs pick_two_pairs(int rows, int IC, int OC, int sms)
+{
+    TwoPairs best{0, 1, 1, 1e300, 0};
+    const int pairs = sms / 2, x_windows = (OC + 63) / 64, w_windows = (rows + 63) / 64;
+    const double x_size = static_cast<double>(rows) * IC, w_size = static_cast<double>(OC) * IC;
+    for (int bn = 256; bn >= 128; bn /= 2) {
+        if (option_fc_tile() == (bn == 256 ? 11 : 1)) continue;
+        const double window = bn == 256 ? 2.26 : 1.34, tile = bn == 256 ? 2.0 : 1.8;
+        const long long xt = static_cast<long long>((rows + 255) / 256) * ((IC + bn - 1) / bn), wt = static_cast<long long>((OC + 255) / 256) * ((IC + bn - 1) / bn);
+        for (int xp = 1; xp <= 8 && xp <= x_windows; ++xp) {
+            for (int wp = 1; wp <= 8 && wp <= w_windows; ++wp) {
+                const int xe = (x_windows + xp - 1) / xp, we = (w_windows + wp - 1) / wp;
+                if ((xp - 1) * xe >= x_windows || (wp - 1) * we >= w_windows || xe > 8192 || we > 8192) continue;
+                const long long xi = xt * xp, wi = wt * wp;
+                // (a pair's items of either: the counts change at the two remainders only)
+                double busy = 0.0;
+                for (const long long i : {0ll, xi % pairs, (xi + wi) % pairs}) {
+                    const long long nx = xi > i ? (xi - i + pairs - 1) / pairs : 0, all = xi + wi > i ? (xi + wi - i + pairs - 1) / pairs : 0;
+                    busy = std::max(busy, nx * (xe * window + tile) + (all - nx) * (we * window + tile));
+                }
+                const double time = 5.0 + busy + (xp > 1 ? 3.0 + x_size * 4e-6 * (2 * xp + 1) / 6.0 : 0.0) + (wp > 1 ? 3.0 + w_size * 4e-6 * (2 * wp + 1) / 6.0 : 0.0);
+                if (time < best.time) best = TwoPairs{bn, xp, wp, time, static_cast<size_t>(((xp > 1 ? xp * x_size : 0.0) + (wp > 1 ? wp * w_size : 0.0)) * 4) + 512};
+            }
+        }
+    }
+    return best;
+}
+int launch_two_pairs(const ProductF32& x, const ProductF32& w, const Planes& X, const Planes& W, const Planes& Z, const TwoPairs& plan, void* part, const uint32_t* seen, int seen_n, int sms, int* status,
+                     cudaStream_t stream)
+{
+    const size_t x_bytes = plan.x_parts > 1 ? (plan.x_parts * static_cast<size_t>(x.rows) * x.cols * 4 + 255) & ~static_cast<size_t>(255) : 0;
+    PairItems a, b;
+    int rc = prepare_pair<kFcDeltaX>(x, Z, W, PairPlan{plan.bn, plan.x_parts, 0.0}, part, seen, seen_n, status, &a);
+    if (!rc) rc = prepare_pair<kFcDeltaW>(w, Z, X, PairPlan{plan.bn, plan.w_parts, 0.0}, static_cast<char*>(part) + x_bytes, seen, seen_n, status, &b);
+    if (rc) return rc;
+    const long long items = static_cast<long long>(a.p.m_tiles) * a.p.n_tiles * plan.x_parts + static_cast<long long>(b.p.m_tiles) * b.p.n_tiles * plan.w_parts;
+    const unsigned pairs = static_cast<unsigned>(items < sms / 2 ? items : sms / 2);
+    auto go = [&](auto width) {
+        constexpr int BN = decltype(width)::value;
+        allow_smem<fc_pair_f32_two_kernel<BN>>();
+        launch_after_clusters(fc_pair_f32_two_kernel<BN>, dim3(2 * pairs), kPairF32Threads, 2, pair_f32_smem(BN), stream, a.a, a.b, a.y, a.p, b.a, b.b, b.y, b.p);
+    };
+    if (plan.bn == 256) go(std::integral_constant<int, 256>{});
+    else go(std::integral_constant<int, 128>{});
+    note_launch("fc");
+    note_plan("fc planes two pair 256x%d parts=%d,%d", plan.bn, plan.x_parts, plan.w_parts);
+    rc = launched("fc_pair_f32_two_kernel");
+    if (!rc && plan.x_parts > 1) rc = launch_parts<false>(a.ws, a.size, plan.x_parts, a.p.rows, x.e, sms, stream);
+    if (!rc && plan.w_parts > 1) rc = launch_parts<false>(b.ws, b.size, plan.w_parts, b.p.rows, w.e, sms, stream);
+    return rc;
 }
 
 // The same from the fp32 tensors as they lie; without `may_split` in no scratch.
@@ -448,11 +518,16 @@ int fc_logits_and_gradients_f32(const AlphaFcShape* s, const float* X, const flo
     if (!rc) rc = device_status_word(&v.status);
     if (rc) return rc;
     const PairPlan pz = pick_pair(rows, 1, OC, false, IC, 1, v.sms), px = pick_pair(rows, 1, IC, false, OC, 1, v.sms), pw = pick_pair(OC, 1, IC, false, rows, 1, v.sms);
+    if (!dX || !dW || v.sms < 2 || rows <= kSmallRows) return 1;
     const int a = v.add(X, rows, IC), b = v.add(W, OC, IC), c = v.add(Z, rows, pitch);
-    v.want(z, pz.parts); v.want(x, px.parts); v.want(w, pw.parts);
-    const double pairs = pz.time + px.time + pw.time + split_time(v.elements()) + 2.0;
+    const TwoPairs both = pick_two_pairs(rows, IC, OC, v.sms);
+    const bool two = both.bn && both.time < 0.95 * (px.time + pw.time);      // (within 5 %, which the estimates do not tell apart: two launches)
+    v.want(z, pz.parts);
+    if (two) v.parts = std::max(v.parts, both.part_bytes);
+    else { v.want(x, px.parts); v.want(w, pw.parts); }
+    const double pairs = pz.time + (two ? both.time : px.time + pw.time) + split_time(v.elements()) + 2.0;
     const double apart = pick_gathered<kFcForward>(z, v.sms).time + pick_gathered<kFcDeltaX>(x, v.sms).time + pick_gathered<kFcDeltaW>(w, v.sms).time;
-    if (!dX || !dW || v.sms < 2 || !v.fits() || !pairs_pay(pairs, apart) || rows <= kSmallRows) return 1;
+    if (!v.fits() || !pairs_pay(pairs, apart)) return 1;
     rc = v.split(stream, 2);                       // X and W
     if (rc) return rc;
     if (dry_run()) return ALPHA_OK;
@@ -463,6 +538,7 @@ int fc_logits_and_gradients_f32(const AlphaFcShape* s, const float* X, const flo
         const Planes* one[1] = {&v.p[c]};
         rc = launch_split(one, 1, v.seen + seen, &v.seen_n, v.sms, stream);
     }
+    if (!rc && two) return launch_two_pairs(x, w, v.p[a], v.p[b], v.p[c], both, v.part, v.seen, seen + v.seen_n, v.sms, v.status, stream);
     if (!rc) rc = launch_pair<kFcDeltaX>(x, v.p[c], v.p[b], px, v.part, v.seen, seen + v.seen_n, v.sms, v.status, stream);
     if (!rc) rc = launch_pair<kFcDeltaW>(w, v.p[c], v.p[a], pw, v.part, v.seen, seen + v.seen_n, v.sms, v.status, stream);
     return rc;

@@ -266,11 +266,10 @@ static __device__ __noinline__ void stand_or_form(const PairF32& p, const SumsAt
     form_sums_f32(p, s, buf, z);
 }
 
-// tmY: the result, or where parts > 1 the sums, as (column, half, row, part)
-template <bool GLU, int BN>
-__global__ void __launch_bounds__(kPairF32Threads, 1)
-    fc_pair_f32_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
-                       const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ PairF32 p)
+// tmY: the result, or where parts > 1 the sums, as (column, half, row, part).  TWO: the items of a second product (tmA2, tmB2, tmY2, p2) follow those of the first.
+template <bool GLU, int BN, bool TWO>
+__device__ __forceinline__ void pair_f32_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmY, const CUtensorMap& tmZ, const PairF32& p1, const CUtensorMap& tmA2,
+                                              const CUtensorMap& tmB2, const CUtensorMap& tmY2, const PairF32& p2)
 {
     constexpr int S = kPairF32Slots, OUT = GLU ? BN / 2 : BN, HALF = BN / 2, QUARTER = BN / 4;
     constexpr uint32_t kPairF32Slot = pair_f32_slot(BN);
@@ -289,7 +288,8 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         mbar_init(&bars[2 * S + 2], 1); mbar_init(&bars[2 * S + 3], 16);
         fence_barrier_init();
         prefetch_tmap(&tmA); prefetch_tmap(&tmB); prefetch_tmap(&tmY);
-        if (p.keep_z) prefetch_tmap(&tmZ);
+        if (p1.keep_z) prefetch_tmap(&tmZ);
+        if (TWO) { prefetch_tmap(&tmA2); prefetch_tmap(&tmB2); prefetch_tmap(&tmY2); }
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_holder, 512);
@@ -303,9 +303,14 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_holder, smem_a = smem_u32(smem);
 
-    const int tiles = p.m_tiles * p.n_tiles, total = tiles * p.parts, step = gridDim.x / 2, first = blockIdx.x / 2;
+    const int items = p1.m_tiles * p1.n_tiles * p1.parts, total = items + (TWO ? p2.m_tiles * p2.n_tiles * p2.parts : 0), step = gridDim.x / 2, first = blockIdx.x / 2;
+    const PairF32* cur = &p1;                         // the product of the item at hand
     struct Item { int m0, n0, w0, w1, part, hm; };
     auto item_at = [&](int t) {
+        if (TWO) cur = t < items ? &p1 : &p2;
+        if (TWO && t >= items) t -= items;
+        const PairF32& p = *cur;
+        const int tiles = p.m_tiles * p.n_tiles;
         Item i;
         i.part = t / tiles;
         t -= i.part * tiles;
@@ -328,25 +333,27 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         RingPos rp;
         for (int t = first; t < total && ok; t += step) {
             const Item it = item_at(t);
+            const PairF32& p = *cur;
+            const CUtensorMap *mA = TWO && t >= items ? &tmA2 : &tmA, *mB = TWO && t >= items ? &tmB2 : &tmB;
             const int b0 = GLU ? it.n0 : it.n0 + my * HALF;
             for (int s = 3 * it.w0; s < 3 * it.w1; ++s) {
                 ok = __all_sync(0xffffffffu, mbar_wait_a(empty_0 + 8 * rp.idx, rp.phase ^ 1));
-                if (!ok) { report(p.status, kStatusProducerTimeout); settle(); break; }
+                if (!ok) { report(p1.status, kStatusProducerTimeout); settle(); break; }
                 if (elected) {
                     if (my == 0) mbar_arrive_expect_tx_a(full_0 + 8 * rp.idx, 2 * kPairF32Slot);
                     const uint32_t bar = full_L + 8 * rp.idx, a = base + rp.idx * kPairF32Slot, b = a + kPairF32Operand;
                     const int w = s / 3, plane = s % 3, hk = w >= p.w_half ? 1 : 0, k0 = (w - hk * p.w_half) * 64;
                     if (p.a_mn) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) tma_load_4d_pair(a + j * 8192, &tmA, bar, it.m0 + 64 * j, it.hm, k0, plane);
+                        for (int j = 0; j < 2; ++j) tma_load_4d_pair(a + j * 8192, mA, bar, it.m0 + 64 * j, it.hm, k0, plane);
                     } else {
-                        tma_load_4d_pair(a, &tmA, bar, k0, hk, it.m0, plane);
+                        tma_load_4d_pair(a, mA, bar, k0, hk, it.m0, plane);
                     }
                     if (p.b_mn) {
 #pragma unroll
-                        for (int j = 0; j < BN / 128; ++j) tma_load_4d_pair(b + j * 8192, &tmB, bar, b0 + 64 * j, k0, hk, plane);
+                        for (int j = 0; j < BN / 128; ++j) tma_load_4d_pair(b + j * 8192, mB, bar, b0 + 64 * j, k0, hk, plane);
                     } else {
-                        tma_load_4d_pair(b, &tmB, bar, k0, b0, GLU ? my : 0, plane);
+                        tma_load_4d_pair(b, mB, bar, k0, b0, GLU ? my : 0, plane);
                     }
                 }
                 __syncwarp();
@@ -358,11 +365,16 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             const uint32_t base = __shfl_sync(0xffffffffu, smem_a, 0), tmem = __shfl_sync(0xffffffffu, tmem_base, 0), elected = elect_one();
             const uint32_t full_0 = __shfl_sync(0xffffffffu, full_a, 0), empty_0 = full_0 + 8 * S, hh_full = empty_0 + 8 * S, hh_free = hh_full + 8, side_full = hh_free + 8, side_free = side_full + 8;
             constexpr uint32_t dhi = (1024u >> 4) | (1u << 14) | (static_cast<uint32_t>(kSwizzle128B) << 29);
-            const uint32_t a_k = p.a_mn ? 128u : 2u, b_k = p.b_mn ? 128u : 2u;               // 16 steps further, in 16-byte units
-            const uint32_t a_lo0 = smem_desc_lo(base, p.a_mn ? 8192u : 16u), b_lo0 = smem_desc_lo(base + kPairF32Operand, p.b_mn ? 8192u : 16u);
+            uint32_t a_k, b_k, a_lo0, b_lo0, idesc;            // 16 steps further, in 16-byte units; the first descriptors
+            auto take_up = [&](const PairF32& p) {
+                a_k = p.a_mn ? 128u : 2u; b_k = p.b_mn ? 128u : 2u;
+                a_lo0 = smem_desc_lo(base, p.a_mn ? 8192u : 16u); b_lo0 = smem_desc_lo(base + kPairF32Operand, p.b_mn ? 8192u : 16u);
+                idesc = p.idesc;
+            };
+            take_up(p1);
             auto wait = [&](uint32_t bar, uint32_t parity) {
                 if (__all_sync(0xffffffffu, mbar_wait_cluster_a(bar, parity))) return true;
-                report(p.status, kStatusMmaTimeout);
+                report(p1.status, kStatusMmaTimeout);
                 settle();
                 return false;
             };
@@ -370,7 +382,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             auto multiply = [&](uint32_t d, uint32_t x, uint32_t y, bool fresh) {
                 const uint32_t a = a_lo0 + x * (kPairF32Slot >> 4), b = b_lo0 + y * (kPairF32Slot >> 4);
 #pragma unroll
-                for (uint32_t kk = 0; kk < 4; ++kk) mma_16bit<true>(tmem + d, a + kk * a_k, dhi, b + kk * b_k, dhi, p.idesc, fresh && kk == 0 ? 0u : 1u, elected);
+                for (uint32_t kk = 0; kk < 4; ++kk) mma_16bit<true>(tmem + d, a + kk * a_k, dhi, b + kk * b_k, dhi, idesc, fresh && kk == 0 ? 0u : 1u, elected);
             };
             auto commit = [&](uint32_t bar) {
                 if (elected) mma_commit_both(bar);
@@ -380,6 +392,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
             uint32_t window = 0, item = 0;
             for (int t = first; t < total && ok; t += step, ++item) {
                 const Item it = item_at(t);
+                if (TWO) take_up(*cur);
                 for (int w = it.w0; w < it.w1; ++w, ++window) {
                     const uint32_t h = rp.idx, m = h + 1, l = h + 2, phase = rp.phase;       // (slots of a window follow one another: S is a multiple of 3)
                     ok = wait(full_0 + 8 * h, phase) && wait(hh_free, (window & 1) ^ 1);
@@ -426,7 +439,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         };
         auto wait = [&](uint32_t bar, uint32_t parity) {
             ok = __all_sync(0xffffffffu, mbar_wait_a(bar, parity));
-            if (!ok) { report(p.status, kStatusEpilogueTimeout); settle(); }
+            if (!ok) { report(p1.status, kStatusEpilogueTimeout); settle(); }
             return ok;
         };
         auto release = [&](uint32_t bar) {
@@ -446,8 +459,8 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         };
         // what the launch that split has seen, while the first copies are under way: an eighth of it a warp
         uint32_t top = 0, dropped = 0;
-        for (int i = threadIdx.x - 64; i < p.seen_n; i += 256) {
-            const uint32_t w = p.seen[i];
+        for (int i = threadIdx.x - 64; i < p1.seen_n; i += 256) {
+            const uint32_t w = p1.seen[i];
             top = max(top, w & ~1u);
             dropped |= w & 1u;
         }
@@ -460,6 +473,8 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
         uint32_t window = 0, item = 0;
         for (int t = first; t < total && ok; t += step, ++item) {
             const Item it = item_at(t);
+            const PairF32& p = *cur;
+            const CUtensorMap* mY = TWO && t >= items ? &tmY2 : &tmY;
 #pragma unroll
             for (int x = 0; x < QUARTER; ++x) acc[x] = 0ull;
             // R to L2, while the windows run
@@ -535,8 +550,8 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
                     take(col_a + c, col0, 0, z);
                     take(col_b + c, col0, 1, u);
                     if (p.parts > 1) {
-                        put(z, [&] { tma_store_4d_a(&tmY, buf, col0, 0, row0, it.part); });
-                        put(u, [&] { tma_store_4d_a(&tmY, buf, col0, 1, row0, it.part); });
+                        put(z, [&] { tma_store_4d_a(mY, buf, col0, 0, row0, it.part); });
+                        put(u, [&] { tma_store_4d_a(mY, buf, col0, 1, row0, it.part); });
                         continue;
                     }
                     if (p.bias) { add(z, p.bias, col0); add(u, p.bias + p.pitch, col0); }
@@ -548,7 +563,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) z[i] = act_value<decltype(a)::value, false>(z[i], p.k) * u[i];
                     });
-                    put(z, [&] { tma_store_4d_a(&tmY, buf, col0, 0, row0, 0); });
+                    put(z, [&] { tma_store_4d_a(mY, buf, col0, 0, row0, 0); });
                 }
             } else {
 #pragma unroll 1
@@ -566,7 +581,7 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
                         });
                         if (p.residual && row < p.rows) add(z, p.residual + static_cast<size_t>(row) * p.pitch, col0);
                     }
-                    put(z, [&] { tma_store_4d_a(&tmY, buf, col0, it.hm, row0, it.part); });
+                    put(z, [&] { tma_store_4d_a(mY, buf, col0, it.hm, row0, it.part); });
                 }
             }
             release(side_free_L);
@@ -577,6 +592,22 @@ __global__ void __launch_bounds__(kPairF32Threads, 1)
     __syncthreads();
     cluster_sync_all();   // neither CTA leaves while the other may still reach its shared memory
     if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+template <bool GLU, int BN>
+__global__ void __launch_bounds__(kPairF32Threads, 1)
+    fc_pair_f32_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
+                       const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ PairF32 p)
+{
+    pair_f32_body<GLU, BN, false>(tmA, tmB, tmY, tmZ, p, tmA, tmB, tmY, p);
+}
+// Two products without gates, activation, bias or residual, whose operands one launch (or two, with one list of what they saw) has split.
+template <int BN>
+__global__ void __launch_bounds__(kPairF32Threads, 1)
+    fc_pair_f32_two_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY, const __grid_constant__ PairF32 p,
+                           const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmY2, const __grid_constant__ PairF32 p2)
+{
+    pair_f32_body<false, BN, true>(tmA, tmB, tmY, tmY, p, tmA2, tmB2, tmY2, p2);
 }
 
 }  // namespace alpha

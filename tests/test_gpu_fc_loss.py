@@ -101,6 +101,23 @@ def test_values_and_gradients(eng, lib, dtype, shape):
     assert lib.device_status() == 0
 
 
+@pytest.mark.parametrize("tile", (0, 1, 11))
+@pytest.mark.parametrize("shape", ((256, 512, 1000), (300, 700, 501), (513, 512, 1000), (1024, 130, 263), (2048, 512, 1000)))
+def test_both_gradients_by_one_launch_in_f32(eng, lib, shape, tile):
+    """Shapes whose deltaX and deltaW one launch makes, whole and in parts of either, and columns so small and so large that the planes do not hold the products."""
+    old = lib.set_option("FC_TILE", tile)
+    try:
+        X, W, label, B = make(*shape, "f32")
+        check(eng, X, W, label, B)
+        X[:, :8] *= 1e-36
+        X[:, 8:16] *= 1e-30
+        W[:, 8:16] *= 1e30
+        check(eng, X, W, label, B)
+    finally:
+        lib.set_option("FC_TILE", old)
+    assert lib.device_status() == 0
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tile", (1, 11, 1064, 1128, 2064, 4256))
 def test_every_tile(eng, lib, dtype, tile):
