@@ -5,8 +5,8 @@
 //
 // One pass over every array, one launch for every 128 tensors: bound by HBM, with moments of 8 bits by the instructions as well.  A CTA takes every gridDim.x-th chunk of 2048
 // elements of the launch; a thread has 4 elements of each of two rows of 1024, so that all its loads are in flight together and every load of a warp is consecutive.
-// 50 million elements, all fp32: 224 us, 6.2 TB/s.  90 million, fp32 weights with bf16 copies and gradients, 8-bit moments: 281 us, 5.2 TB/s (71 instructions an element, of which a third are the
-// hash and the roundings of the codes).  Chunks of 4096 on three CTAs an SM took 231 and 289 us, of 1024 on six 234 and 316.
+// 50 million elements, all fp32: 224 us, 6.2 TB/s.  90 million, fp32 weights with bf16 copies and gradients, 8-bit moments: 275 us, 5.3 TB/s (some 70 instructions an element, of which a third are
+// the hash and the roundings of the codes).  Chunks of 4096 on three CTAs an SM took 7 and 8 us longer, of 1024 on six 10 and 35.
 //
 // Moments of 8 bits: an e4m3 code for each element and a power of two for each block of 32, the smallest with which none is above 448, so that scaling is exact
 // in both directions.  A code is rounded up or down at random, with the probability that keeps its mean: v moves by one part in 1 / (1 - b2) a step, codes lie 6 to

@@ -42,8 +42,10 @@ double norm_instructions(const Norm& p, int size, bool back, bool streamed)
     const bool plain = p.act == ALPHA_ACT_NONE || p.act == ALPHA_ACT_LEAKY_RELU, once = size == 4;         // (once: dz is kept)
     return streamed ? (back ? (plain ? 26.0 : 40.0) : (plain ? 16.0 : 21.0)) : (back ? (once ? (plain ? 14.0 : 22.0) : (plain ? 20.0 : 30.0)) : (plain ? 9.0 : 14.0));
 }
-// The slab and the cluster of least estimated time (us); false: no slab fits.  A CTA takes of its SM what its bytes take at 45 KB a us or its instructions at 4000 a us (of a
-// warp), whichever is more - both, and its loads' latency, where it is alone there - and its sums and barriers, 0.9 us (backward 1.2) and 0.1 for each CTA of the cluster.
+// The slab and the cluster of least estimated time (us); false: no slab fits.  A CTA takes of its SM what its bytes take at 43 KB a us (rows of fewer than 64 bytes longer) or its
+// instructions at 4100 a us (of a warp), whichever is more, a share of the other and of its loads' latency that is the larger the fewer CTAs an SM holds, and its sums and barriers,
+// 0.9 us (backward 1.4), in a cluster 0.2 and 0.1 for each of its CTAs more.  Fitted to all plans of 189 calls; what it takes is 2.4 % above a call's fastest on (geometric)
+// average (gradients of 128 x 56 x 56 x 64 fp32: two CTAs of 106 KB to an SM 81 us, one of 204 KB 88).
 bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* least)
 {
     const long long unit = static_cast<long long>(p.D) * 4 / std::gcd(p.D, 4);
@@ -60,15 +62,15 @@ bool plan_resident(Norm& p, int size, bool back, int sms, size_t* smem, double* 
             const size_t bytes = norm_smem(back, size, part, words, words * 4 / p.D, cl);
             if (bytes > 224 * 1024) continue;
             const int fit = static_cast<int>(227 * 1024 / (bytes + 1024)), at_once = fit < 4 ? fit : 4;
-            const double elements = static_cast<double>(part) * words * 4, places = sms * at_once * (cl < 4 ? 1.0 : 0.9);
-            const double row = words * 4.0 * size, narrow = row >= 64 ? 1.0 : row >= 32 ? 1.1 : 2.0;
-            const double memory = elements * size * (back ? 3 : 2) / 45e3 * narrow, math = elements * norm_instructions(p, size, back, false) / 32 / 4000.0;
-            const double alone = at_once == 1 ? 1.0 : at_once == 2 ? 0.4 : 0.0;
-            const double each_cta = std::max(memory, math) + alone * (std::min(memory, math) + 1.5) + (back ? 1.2 : 0.9) + 0.1 * cl;
+            const double elements = static_cast<double>(part) * words * 4;
             // (what is there at once runs at once, in whole waves as long as these are few)
-            const double waves = ctas / places, rounds = waves <= 1.0 ? 1.0 : waves < 4.0 ? std::ceil(waves) * 0.5 + waves * 0.5 : waves;
-            const double on_sm = waves <= 1.0 ? std::max(1.0, std::ceil(static_cast<double>(ctas) / sms)) : at_once;
-            const double time = 4.0 + rounds * on_sm * each_cta;
+            const double waves = static_cast<double>(ctas) / (static_cast<double>(sms) * at_once), rounds = waves <= 1.0 ? 1.0 : waves < 4.0 ? std::ceil(waves) : waves;
+            const int on_sm = waves <= 1.0 ? static_cast<int>((ctas + sms - 1) / sms) : at_once;
+            const double row = words * 4.0 * size, narrow = row >= 64 ? 1.0 : row >= 32 ? 1.16 : 2.3;
+            const double memory = elements * size * (back ? 3 : 2) / 43e3 * narrow, math = elements * norm_instructions(p, size, back, false) / 32 / 4100.0;
+            const double alone = on_sm == 1 ? 1.1 : on_sm == 2 ? 0.38 : on_sm == 3 ? 0.09 : 0.0;
+            const double each_cta = std::max(memory, math) + alone * (std::min(memory, math) + 1.1) + (back ? 1.4 : 0.9) + 0.1 * cl + (cl > 1 ? 0.2 : 0.0);
+            const double time = 2.2 + rounds * on_sm * each_cta;
             if (time < *least) {
                 *least = time;
                 p.words = words; p.slabs = slabs; p.cluster = cl; p.part = part; p.rows = kNormThreads / words;
@@ -110,9 +112,9 @@ template <class T, bool BACK> int run_norm(Norm& p, const char* what, void* dgam
     const size_t word = 4 * sizeof(T);
     const bool words = p.C % 4 == 0 && aligned(p.X, word) && aligned(p.out, word) && aligned(p.dY, word);
     // streamed: both passes over the tensors, the second through L2 as far as that holds them, and two more launches
-    const double bytes = static_cast<double>(p.N) * p.R * p.C * sizeof(T) * (BACK ? 2 : 1), rate = 40e3 * sms;
-    const double math = static_cast<double>(p.N) * p.R * p.C * norm_instructions(p, sizeof(T), BACK, true) / 32 / (3800.0 * sms);
-    const double streamed = 14.0 + std::max(math, bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate);
+    const double bytes = static_cast<double>(p.N) * p.R * p.C * sizeof(T) * (BACK ? 2 : 1), rate = 43.5e3 * sms;
+    const double math = static_cast<double>(p.N) * p.R * p.C * norm_instructions(p, sizeof(T), BACK, true) / 32 / ((BACK ? 3900.0 : 3200.0) * sms);
+    const double streamed = (BACK ? 16.0 : 12.0) + std::max(math, bytes / rate + (bytes * (bytes > 80e6 ? 1.0 : 0.5) + bytes / (BACK ? 2 : 1)) / rate);
     size_t smem = 0;
     double least = 0.0;
     const bool resident = words && plan_resident(p, sizeof(T), BACK, sms, &smem, &least) && least < streamed;
