@@ -199,13 +199,18 @@ template <class T> int delta_16(const Loss& c, const float* dL, int dL_step, con
     return ALPHA_OK;
 }
 
+// CTAs to a row in the passes over fp32 logits: some 512 in all, a thousand logits each at least (13 x 122368: gradients of the logits 78 us by one to a row, 10 by 39).
+int row_ctas(long long rows, long long cols) { return static_cast<int>(std::max(1LL, std::min(512 / rows, cols / 1024))); }
+
 int forward_f32(const Loss& c, float* loss, float* lse)
 {
     const long long rows = c.s->rows, IC = c.s->IC, OC = c.s->OC, piece = piece_classes(rows, OC, 4, 8), pieces = (OC + piece - 1) / piece;
+    const int across = row_ctas(rows, piece);
+    const long long slots = pieces * across;
     void *z = nullptr, *part = nullptr, *at_label = nullptr;
     int rc = call_scratch(c.stream, static_cast<size_t>(rows) * fc_pitch(static_cast<int>(piece)) * 4, &z);
-    if (!rc && pieces > 1) rc = call_scratch(c.stream, static_cast<size_t>(pieces) * rows * sizeof(float2), &part);
-    if (!rc && pieces > 1) rc = call_scratch(c.stream, rows * sizeof(float), &at_label);
+    if (!rc && slots > 1) rc = call_scratch(c.stream, static_cast<size_t>(slots) * rows * sizeof(float2), &part);
+    if (!rc && slots > 1) rc = call_scratch(c.stream, rows * sizeof(float), &at_label);
     const ScratchMark mark = call_mark(c.stream);
     for (long long first = 0; first < OC && !rc; first += piece) {
         call_rewind(c.stream, mark);
@@ -213,13 +218,13 @@ int forward_f32(const Loss& c, float* loss, float* lse)
         s.OC = static_cast<int>(std::min(piece, OC - first));
         rc = fc_logits_f32(&s, static_cast<const float*>(c.X), static_cast<const float*>(c.W) + first * IC, c.bias ? static_cast<const float*>(c.bias) + first : nullptr, static_cast<float*>(z), c.stream);
         if (rc || dry_run()) continue;
-        launch_after(loss_rows_kernel, static_cast<unsigned>(rows), kRowThreads, 0, c.stream, static_cast<const float*>(z), fc_pitch(s.OC), s.OC, static_cast<int>(first), c.s->OC, c.s->rows, c.label,
-                     c.label_bytes, part ? static_cast<float2*>(part) + first / piece * rows : nullptr, static_cast<float*>(at_label), loss, lse);
+        launch_after(loss_rows_kernel, dim3(static_cast<unsigned>(rows), across), kRowThreads, 0, c.stream, static_cast<const float*>(z), fc_pitch(s.OC), s.OC, static_cast<int>(first), c.s->OC, c.s->rows, c.label,
+                     c.label_bytes, part ? static_cast<float2*>(part) + first / piece * across * rows : nullptr, static_cast<float*>(at_label), loss, lse);
         note_launch("fc_loss");
         rc = launched("loss_rows_kernel");
     }
-    if (rc || dry_run() || pieces == 1) return rc;
-    return join(c, static_cast<const float2*>(part), static_cast<int>(pieces), 0, c.s->rows, static_cast<const float*>(at_label), loss, lse);
+    if (rc || dry_run() || slots == 1) return rc;
+    return join(c, static_cast<const float2*>(part), static_cast<int>(slots), 0, c.s->rows, static_cast<const float*>(at_label), loss, lse);
 }
 
 int delta_f32(const Loss& c, const float* dL, int dL_step, const float* lse, float* dX, float* dW, float* dB)
@@ -242,7 +247,7 @@ int delta_f32(const Loss& c, const float* dL, int dL_step, const float* lse, flo
         float* w = dW ? dW + first * IC : nullptr;
         auto softmax = [&](const float* part, int parts) {
             if (dry_run()) return static_cast<int>(ALPHA_OK);
-            launch_after(loss_delta_kernel, static_cast<unsigned>(rows), kRowThreads, 0, c.stream, z, part, parts, part ? bias : nullptr, static_cast<int>(rows), fc_pitch(s.OC), s.OC, static_cast<int>(first),
+            launch_after(loss_delta_kernel, dim3(static_cast<unsigned>(rows), row_ctas(rows, s.OC)), kRowThreads, 0, c.stream, z, part, parts, part ? bias : nullptr, static_cast<int>(rows), fc_pitch(s.OC), s.OC, static_cast<int>(first),
                          c.s->OC, c.label, c.label_bytes, lse, dL, dL_step);
             note_launch("fc_loss");
             return launched("loss_delta_kernel");

@@ -182,22 +182,22 @@ __device__ __forceinline__ float cta_total(float x, float* shared)
     for (int w = 0; w < kRowThreads / 32; ++w) x += shared[w];
     return x;
 }
-// A CTA to a row: the largest logit of the piece, then the sum about it; slot `piece` of the row's parts, and the label's logit if it lies in the piece.  Of a piece that is all the
-// classes (part NULL) lse and loss.
+// gridDim.y CTAs to a row: the largest logit of a CTA's share of the piece, then the sum about it, a slot of the row's parts, and from the first the label's logit if it lies in the piece.
+// Of a share that is all the classes (part NULL) lse and loss.
 __global__ void __launch_bounds__(kRowThreads) loss_rows_kernel(const float* __restrict__ z, int pitch, int cols, int base, int classes, int rows, const void* label, int label_bytes,
                                                                 float2* part, float* at_label, float* loss, float* lse)
 {
     __shared__ float shared[kRowThreads / 32];
     grid_dependency_wait();
     grid_dependency_trigger();
-    const int row = blockIdx.x;
+    const int row = blockIdx.x, first = blockIdx.y * kRowThreads + threadIdx.x, step = gridDim.y * kRowThreads;
     const float* at = z + static_cast<size_t>(row) * pitch;
     float m = -__int_as_float(0x7f800000);
-    for (int c = threadIdx.x; c < cols; c += kRowThreads) m = fmaxf(m, at[c]);
+    for (int c = first; c < cols; c += step) m = fmaxf(m, at[c]);
     m = cta_most(m, shared);
     const float about = m > -__int_as_float(0x7f800000) ? m : 0.f;
     float s = 0.f;
-    for (int c = threadIdx.x; c < cols; c += kRowThreads) s += expf(at[c] - about);
+    for (int c = first; c < cols; c += step) s += expf(at[c] - about);
     s = cta_total(s, shared);
     if (threadIdx.x) return;
     const int l = label_of(label, label_bytes, row, classes) - base;
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kRowThreads) loss_rows_kernel(const float* __r
         if (loss) loss[row] = l >= 0 ? log_sum - at[l] : 0.f;
         return;
     }
-    part[row] = make_float2(m, s);
-    if (l >= 0 && l < cols) at_label[row] = at[l];
+    part[static_cast<size_t>(blockIdx.y) * rows + row] = make_float2(m, s);
+    if (l >= 0 && l < cols && blockIdx.y == 0) at_label[row] = at[l];
 }
 // Logits become their gradients, in place; the padding of a row 0.  Logits that were formed in parts are added first, with the bias.
 __global__ void __launch_bounds__(kRowThreads) loss_delta_kernel(float* z, const float* __restrict__ part, int parts, const float* __restrict__ bias, int rows, int pitch, int cols, int base, int classes, const void* label, int label_bytes, const float* __restrict__ lse,
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kRowThreads) loss_delta_kernel(float* z, const
     const int row = blockIdx.x, l = label_of(label, label_bytes, row, classes);
     const float log_sum = lse[row], g = grad[static_cast<size_t>(row) * grad_step];
     float* at = z + static_cast<size_t>(row) * pitch;
-    for (int c = threadIdx.x; c < pitch; c += kRowThreads) {
+    for (int c = blockIdx.y * kRowThreads + threadIdx.x; c < pitch; c += gridDim.y * kRowThreads) {
         float logit = part ? 0.f : at[c];
         if (part)
             for (int i = 0; i < parts; ++i) logit += part[(static_cast<size_t>(i) * rows + row) * pitch + c];

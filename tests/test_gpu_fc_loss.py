@@ -101,6 +101,17 @@ def test_values_and_gradients(eng, lib, dtype, shape):
     assert lib.device_status() == 0
 
 
+@pytest.mark.parametrize("shape", ((1, 40, 3001), (2, 72, 9000), (13, 64, 40001), (100, 24, 6000), (256, 8, 300000)))
+def test_few_rows_of_many_classes_in_f32(eng, lib, shape):
+    """Several CTAs to a row, of one piece of the classes or of two (the last shape), and shares of a row that hold masked classes only."""
+    X, W, label, B = make(*shape, "f32")
+    check(eng, X, W, label, B)
+    B[5:] = -float("inf")
+    label.clamp_(-1, 4)
+    check(eng, X, W, label, B)
+    assert lib.device_status() == 0
+
+
 @pytest.mark.parametrize("tile", (0, 1, 11))
 @pytest.mark.parametrize("shape", ((256, 512, 1000), (300, 700, 501), (513, 512, 1000), (1024, 130, 263), (2048, 512, 1000)))
 def test_both_gradients_by_one_launch_in_f32(eng, lib, shape, tile):
